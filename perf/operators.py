@@ -77,7 +77,7 @@ def draw(rng):
     cap = float(rng.choice([20, 30, 50])) if mod == "cap" else 0.0
     if rng.random() < 0.5:
         prefix = rng.choice([0.0, 0.0, 0.3, 0.6])
-        T = _log(rng, 64, 6000 if prefix else 8192)
+        T = _log(rng, 64, 5900 if prefix else 8192)
         tokens = 8192 * (1 if T > 4096 or prefix else 2)
         if model == "7b":
             tokens //= 2
@@ -88,7 +88,7 @@ def draw(rng):
                      bias=mod == "bias", train=rng.random() < 0.7)
     n = _log(rng, 1, 64)
     hi = _log(rng, 64, 60000)
-    B = max(1, min(16, 65536 // hi, _log(rng, 1, 16)))
+    B = max(1, min(16, 60000 // hi, _log(rng, 1, 16)))
     lo = rng.choice([hi, hi, 0, hi // 2]) if B > 1 else hi
     return _tree(model, B, n, lo, hi, hi + n + rng.randrange(0, 200), cap=cap, bias=mod == "bias")
 
