@@ -81,7 +81,7 @@ def draw(rng):
         tokens = 8192 * (1 if T > 4096 or prefix else 2)
         if model == "7b":
             tokens //= 2
-            T = min(T, 5000)
+            T = min(T, 4900)
         B = max(1, min(8, tokens // T, _log(rng, 1, 8)))
         doc = rng.choice([0, _log(rng, 40, 1500)])
         return _span(model, B, T, doc, prefix=prefix, pad=rng.choice([0, 0, T // 9]), cap=cap,
