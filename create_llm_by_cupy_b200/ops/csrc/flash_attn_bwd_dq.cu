@@ -39,6 +39,7 @@ struct DqGemmParams {
   const float* unrot_sin;   // inverse rotation applied
   int unrot_ld;
   int* status;
+  const int4* qtab;      // spans (see span_mask.cu): the key tiles of each query tile, [B, n_tiles]
 };
 
 struct DqGemmSmem {
@@ -48,7 +49,8 @@ struct DqGemmSmem {
 };
 
 // kD: head dimension (128, or 64: one 64-column box of K per key tile, N = 64, 64 output columns).
-template <int kD>
+// kSpans: the keys are those of the tables, in place of all up to the diagonal and the valid length.
+template <int kD, bool kSpans>
 __global__ void __launch_bounds__(DQG_THREADS, 2)
 flash_bwd_dq_gemm_kernel(const __grid_constant__ CUtensorMap tmDS, const __grid_constant__ CUtensorMap tmK,
                          const DqGemmParams p) {
@@ -94,9 +96,16 @@ flash_bwd_dq_gemm_kernel(const __grid_constant__ CUtensorMap tmDS, const __grid_
   // No pdl_trigger() here and in the dK/dV kernels: with CTAs of the next kernel placed between their rounds the backward of
   // 4 x 2048 tokens, 16 / 4 heads of 128, took 267 us where it takes 232 without (241 without any early start).
   pdl_wait();                            // by every role: their bounded waits start counting behind it
-  const int vlen = p.valid_len ? checked_index(p.valid_len[b], T, p.status, 303) : T;
   // 64-key steps: everything up to the end of the diagonal tile, cut at the valid length
-  const int n_tiles = min(2 * (mtile + 1), (max(vlen, 1) + DQG_KEYS - 1) / DQG_KEYS);
+  int key0 = 0, n_tiles;
+  if constexpr (kSpans) {
+    const int4 r = p.qtab[size_t(b) * p.n_tiles + mtile];
+    key0 = r.x * 128;
+    n_tiles = 2 * (r.y - r.x);           // 0: no row of the tile sees a key, and dQ is zero
+  } else {
+    const int vlen = p.valid_len ? checked_index(p.valid_len[b], T, p.status, 303) : T;
+    n_tiles = min(2 * (mtile + 1), (max(vlen, 1) + DQG_KEYS - 1) / DQG_KEYS);
+  }
 
   if (warp == 0) {
     if (lane == 0) {
@@ -107,10 +116,11 @@ flash_bwd_dq_gemm_kernel(const __grid_constant__ CUtensorMap tmDS, const __grid_
         uint8_t* sK = sA + DQG_TILE;
         mbar_expect_tx(&full[s], DQG_TILE + DQG_KEYS * kD * 2);
         // dS^T: key rows j * 64 .., query columns m0 .. (two boxes of 64 queries); K: the same key rows
-        tma_load_4d(sA, &tmDS, &full[s], m0, h, j * DQG_KEYS, b);
-        tma_load_4d(sA + DQG_BOX, &tmDS, &full[s], m0 + 64, h, j * DQG_KEYS, b);
-        tma_load_4d(sK, &tmK, &full[s], 0, kvh, j * DQG_KEYS, b);
-        if (kD == 128) tma_load_4d(sK + DQG_BOX, &tmK, &full[s], 64, kvh, j * DQG_KEYS, b);
+        const int key = key0 + j * DQG_KEYS;
+        tma_load_4d(sA, &tmDS, &full[s], m0, h, key, b);
+        tma_load_4d(sA + DQG_BOX, &tmDS, &full[s], m0 + 64, h, key, b);
+        tma_load_4d(sK, &tmK, &full[s], 0, kvh, key, b);
+        if (kD == 128) tma_load_4d(sK + DQG_BOX, &tmK, &full[s], 64, kvh, key, b);
       }
     }
   } else if (warp == 1) {
@@ -141,7 +151,12 @@ flash_bwd_dq_gemm_kernel(const __grid_constant__ CUtensorMap tmDS, const __grid_
       load_row_tables(tab[0], cs, sn, p.unrot_ld, 0);
       load_row_tables(tab[1], cs, sn, p.unrot_ld, 16);
     }
-    if (mbar_wait_warp(done, 0, abort_flag)) {
+    if (kSpans && n_tiles == 0) {
+      if (lane < live) {
+        bf16* row = p.dq + b * p.dq_bs + (long long)(row0 + lane) * p.dq_ts + h * p.dq_hs;
+        for (int c = 0; c < kD; c += 8) *reinterpret_cast<uint4*>(row + c) = make_uint4(0, 0, 0, 0);
+      }
+    } else if (mbar_wait_warp(done, 0, abort_flag)) {
       tc_fence_after();
       bf16* rows = p.dq + b * p.dq_bs + (long long)min(row0, T - 1) * p.dq_ts + h * p.dq_hs;
       uint8_t* buf = smem + q * 4096;                 // every product has read its operands: the first stage is free
@@ -177,7 +192,7 @@ flash_bwd_dq_gemm_kernel(const __grid_constant__ CUtensorMap tmDS, const __grid_
 // 128) times K. Strides in elements: k (batch, token, head), dq (batch, token, head).
 int flash_bwd_dq_from_ds(const void* ds, const void* k, void* dq, const void* valid_len, const long long* ks,
                          const long long* dqs, int B, int T, int QH, int KVH, int D, int bchunk,
-                         const float* unrot_cos, const float* unrot_sin, int unrot_ld, cudaStream_t st) {
+                         const float* unrot_cos, const float* unrot_sin, int unrot_ld, cudaStream_t st, const int4* qtab) {
   if (D != 128 && D != 64) return static_cast<int>(cudaErrorInvalidValue);
   const int nt = (T + 127) / 128;
   const unsigned long long Tp = (unsigned long long)nt * 128;
@@ -185,23 +200,24 @@ int flash_bwd_dq_from_ds(const void* ds, const void* k, void* dq, const void* va
       get_tensor_map_bthd(ds, B, Tp, QH, Tp, (unsigned long long)QH * Tp * Tp, Tp, Tp * Tp, DQG_KEYS, 64);
   TensorMap tk = get_tensor_map_bthd(k, B, T, KVH, D, ks[0], ks[1], ks[2], DQG_KEYS, 64);
   if (!tds || !tk) return static_cast<int>(cudaErrorInvalidValue);
-  DqGemmParams p;
+  DqGemmParams p = {};
   p.dq = static_cast<bf16*>(dq);
   p.valid_len = static_cast<const int*>(valid_len);
   p.dq_bs = dqs[0]; p.dq_ts = dqs[1]; p.dq_hs = dqs[2];
   p.B = B; p.T = T; p.QH = QH; p.KVH = KVH; p.n_tiles = nt; p.bchunk = bchunk < 1 ? 1 : bchunk;
   p.unrot_cos = unrot_cos; p.unrot_sin = unrot_sin; p.unrot_ld = unrot_ld;
   p.status = status_ptr();
+  p.qtab = qtab;
   static bool configured = false;
   if (!configured) {
-    B200_CHECK(cudaFuncSetAttribute(flash_bwd_dq_gemm_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    DqGemmSmem::kTotal));
-    B200_CHECK(cudaFuncSetAttribute(flash_bwd_dq_gemm_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                    DqGemmSmem::kTotal));
+    for (auto* kern : {flash_bwd_dq_gemm_kernel<128, false>, flash_bwd_dq_gemm_kernel<64, false>, flash_bwd_dq_gemm_kernel<128, true>,
+                       flash_bwd_dq_gemm_kernel<64, true>})
+      B200_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, DqGemmSmem::kTotal));
     configured = true;
   }
-  return static_cast<int>(launch_pdl(D == 128 ? flash_bwd_dq_gemm_kernel<128> : flash_bwd_dq_gemm_kernel<64>,
-                                     dim3(nt * QH * B), dim3(DQG_THREADS), DqGemmSmem::kTotal, st, 0, *tds, *tk, p));
+  auto* kern = qtab != nullptr ? (D == 128 ? flash_bwd_dq_gemm_kernel<128, true> : flash_bwd_dq_gemm_kernel<64, true>)
+                               : (D == 128 ? flash_bwd_dq_gemm_kernel<128, false> : flash_bwd_dq_gemm_kernel<64, false>);
+  return static_cast<int>(launch_pdl(kern, dim3(nt * QH * B), dim3(DQG_THREADS), DqGemmSmem::kTotal, st, 0, *tds, *tk, p));
 }
 
 }  // namespace b200

@@ -57,7 +57,16 @@ struct FlashBwdTcParams {
   int unrot_ld;
   float scale;
   int* status;
+  // spans (flash_bwd_dkv_wide_kernel with kMod >= 0; see span_mask.cu)
+  const int2* spans;     // [B, T]
+  const int2* ktab;      // [B, n_tiles]
+  float cap;             // kCap
+  const float* slopes;   // kBias: [QH]
 };
+
+// What was done to the scores, as in flash_attn_tc3.cu: the causal mask and the valid length alone; the spans' mask; that and a cap;
+// that and a distance bias.
+constexpr int kCausal = -1, kSpan = 0, kCap = 1, kBias = 2;
 
 __device__ __forceinline__ void named_bar_sync(int id, int nthreads) {
   asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(nthreads) : "memory");
@@ -736,14 +745,17 @@ flash_bwd_dkv_tc_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_co
 // no division in the loops: 58.1 | 161.2. A second S^T tile for head_dim 64 gains nothing and needs barriers of its own
 // for each warpgroup: the one that ran ahead completed a phase for the other.
 constexpr int FKW_BQ = 128;                      // query rows per iteration
-template <int kD>
+template <int kD, int kMod = kCausal>
 struct FdkwSmem {
   static constexpr int kTile = 128 * kD * 2;                               // a K, V, Q_i or dO_i tile
   static constexpr int kStages = kD == 128 ? 2 : 3;                        // ring of Q_i, dO_i and their statistics
   static constexpr int kK = 0, kV = kTile, kQ = 2 * kTile;                 // stage s: Q_i, dO_i
   static constexpr int kStage = kQ + kStages * 2 * kTile;                  // [2] dS^T staging tiles (one per warpgroup)
   static constexpr int kStats = kStage + 2 * FKV_STG;                      // stage s: lse2[128], delta * scale [128]
-  static constexpr int kBar = kStats + kStages * 2 * FKW_BQ * 4;
+  // ... spans: also the part of the key tile that each query sees (first key | number of keys << 8), and whether that is not
+  // always all of it
+  static constexpr int kStatBytes = 2 * FKW_BQ * 4 + (kMod == kCausal ? 0 : FKW_BQ * 2 + 16);
+  static constexpr int kBar = kStats + kStages * kStatBytes;
   // kv_full, q_full[3], q_empty[3], st_full[3], s_full, dp_full, p_ready, ds_ready, acc_done, acc_free,
   // stg_full[2], stg_free[2] (head_dim 128: two of the threes)
   static constexpr int kBars = 11 + 3 * kStages;
@@ -753,13 +765,22 @@ struct FdkwSmem {
   static constexpr int kTotal = kD == 128 ? 232448 : kUsed + 1024;
 };
 static_assert(FdkwSmem<128>::kUsed <= FdkwSmem<128>::kTotal, "dK/dV kernel: shared memory");
+static_assert(FdkwSmem<128, kSpan>::kUsed <= FdkwSmem<128, kSpan>::kTotal, "dK/dV kernel with spans: shared memory");
 
 struct DkwPass {
   int n0, i_first, n_qt, iters;
 };
-__device__ __forceinline__ DkwPass dkw_pass(int ntile, int T, int R, int vlen) {
+template <int kMod>
+__device__ __forceinline__ DkwPass dkw_pass(int ntile, int T, int R, int vlen, const FlashBwdTcParams& p, int b) {
   DkwPass d;
   d.n0 = ntile * 128;
+  if constexpr (kMod != kCausal) {
+    const int2 r = p.ktab[size_t(b) * p.n_tiles + ntile];     // the query tiles that meet it
+    d.i_first = r.x;
+    d.n_qt = r.y - r.x;
+    d.iters = R * d.n_qt;
+    return d;
+  }
   d.i_first = ntile;                                          // first 128-query tile at / below the diagonal
   d.n_qt = (T + FKW_BQ - 1) / FKW_BQ - d.i_first;
   d.iters = (d.n0 < vlen) ? R * d.n_qt : 0;
@@ -789,6 +810,54 @@ __device__ __forceinline__ void fb_p_chunk(uint32_t (&rs)[16], uint32_t (&pk)[8]
       const bf162 t0 = __floats2bfloat162_rn(pv[u], pv[u + 1]);
       pk[(e + u) >> 1] = *reinterpret_cast<const uint32_t*>(&t0);
     }
+  }
+}
+
+// The same under spans: `see` holds the keys of the tile that each of the 16 queries sees, krow is this thread's key in it.
+// A cap leaves P (1 - tanh^2) in place of P in rs, which is what dS is made from: x = c tanh(s / c) = c - 2 c r with
+// r = 1 / (1 + exp(2 s / c)), and 1 - tanh^2 = 4 r (1 - r). A bias: dist = first query's position minus the key's.
+template <bool kMask, int kMod>
+__device__ __forceinline__ void fb_p_chunk_span(uint32_t (&rs)[16], uint32_t (&pk)[8], float kc, float c2, const float* lse2,
+                                                const uint32_t* see, uint32_t krow, float slope2, float dist) {
+#pragma unroll
+  for (int e = 0; e < 16; e += 4) {
+    const float4 l4 = *reinterpret_cast<const float4*>(lse2 + e);
+    const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+    uint2 w = make_uint2(0u, 0u);
+    if (kMask) w = *reinterpret_cast<const uint2*>(see + e / 2);
+    const uint32_t sv[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
+    float pv[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float x = __uint_as_float(rs[e + u]);
+      float pe, r = 0.f;
+      if constexpr (kMod == kCap) {
+        r = __fdividef(1.f, 1.f + exp2f(x * kc));
+        pe = exp2f(fmaf(-2.f * c2, r, c2 - lv[u]));
+      } else if constexpr (kMod == kBias) {
+        pe = exp2f(fmaf(x, kc, fmaf(-slope2, fabsf(dist + float(e + u)), -lv[u])));
+      } else {
+        pe = exp2f(fmaf(x, kc, -lv[u]));
+      }
+      if (kMask) {
+        if (krow - (sv[u] & 0xffu) >= (sv[u] >> 8)) pe = 0.f;
+      }
+      pv[u] = pe;
+      rs[e + u] = __float_as_uint(kMod == kCap ? pe * (4.f * fmaf(-r, r, r)) : pe);
+    }
+#pragma unroll
+    for (int u = 0; u < 4; u += 2) {
+      const bf162 t0 = __floats2bfloat162_rn(pv[u], pv[u + 1]);
+      pk[(e + u) >> 1] = *reinterpret_cast<const uint32_t*>(&t0);
+    }
+  }
+}
+
+__device__ __forceinline__ void fb_pack16(const uint32_t* f, uint32_t (&pk)[8]) {
+#pragma unroll
+  for (int e = 0; e < 16; e += 2) {
+    const bf162 t = __floats2bfloat162_rn(__uint_as_float(f[e]), __uint_as_float(f[e + 1]));
+    pk[e >> 1] = *reinterpret_cast<const uint32_t*>(&t);
   }
 }
 
@@ -827,12 +896,12 @@ __device__ __forceinline__ void fb_ds_from_p_chunk(const uint32_t (&rp)[16], con
   }
 }
 
-template <int kD>
+template <int kD, int kMod>
 __global__ void __launch_bounds__(FBT_THREADS, 1)
 flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
                           const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                           const __grid_constant__ CUtensorMap tmDS, const FlashBwdTcParams p) {
-  using Smem = FdkwSmem<kD>;
+  using Smem = FdkwSmem<kD, kMod>;
   constexpr int kSt = Smem::kStages, kTile = Smem::kTile;
   extern __shared__ uint8_t fb_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(fb_smem_raw) + 1023) & ~uintptr_t(1023));
@@ -905,7 +974,7 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
       bool ok = true;
 #pragma unroll 1
       for (int ps = 0; ps < n_pass && ok; ++ps) {
-        const DkwPass d = dkw_pass(tile_of_pass[ps], T, R, vlen);
+        const DkwPass d = dkw_pass<kMod>(tile_of_pass[ps], T, R, vlen, p, b);
         if (d.iters == 0) continue;
         if (ps > 0) {             // K / V of the previous pass are read by its MMAs until they have all completed
           if (!mbar_wait(acc_done, (ps - 1) & 1, abort_flag)) break;
@@ -936,12 +1005,12 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
     bool ok = true;
 #pragma unroll 1
     for (int ps = 0; ps < n_pass && ok; ++ps) {
-      const DkwPass d = dkw_pass(tile_of_pass[ps], T, R, vlen);
+      const DkwPass d = dkw_pass<kMod>(tile_of_pass[ps], T, R, vlen, p, b);
       for (int it = 0, h = kvh * R, i = d.i_first; it < d.iters; ++it, ++g) {
         const int s = g % kSt;
         const int m0 = i * FKW_BQ;
         if (!mbar_wait(&q_empty[s], ((g / kSt) & 1) ^ 1, abort_flag)) { ok = false; break; }
-        float* st = reinterpret_cast<float*>(smem + Smem::kStats + s * 2 * FKW_BQ * 4);
+        float* st = reinterpret_cast<float*>(smem + Smem::kStats + s * Smem::kStatBytes);
         // all eight loads in flight before the first store: one after the other (a store to shared memory may not
         // pass a later global load the compiler cannot tell apart from it) they cost four round trips to L2 per
         // iteration, which made this warp the slowest part of the kernel
@@ -952,6 +1021,23 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
           const size_t idx = (size_t(b) * p.QH + h) * T + min(row, T - 1);
           lv[j] = p.lse[idx];
           dv[j] = p.delta[idx];
+        }
+        if constexpr (kMod != kCausal) {
+          // spans: the keys of this tile that each query sees, and rows that see nothing at all (lse -inf) as rows past T
+          int2 sp[FKW_BQ / 32];
+#pragma unroll
+          for (int j = 0; j < FKW_BQ / 32; ++j) sp[j] = p.spans[size_t(b) * T + min(m0 + lane + 32 * j, T - 1)];
+          uint16_t* see = reinterpret_cast<uint16_t*>(st + 2 * FKW_BQ);
+          bool part = false;
+#pragma unroll
+          for (int j = 0; j < FKW_BQ / 32; ++j) {
+            const int lo = min(max(sp[j].x - d.n0, 0), 128), hi = min(max(sp[j].y - d.n0, 0), 128);
+            see[lane + 32 * j] = uint16_t(lo | (max(hi - lo, 0) << 8));
+            part = part || lo > 0 || hi < 128;
+            if (lv[j] == -INFINITY) lv[j] = INFINITY;
+          }
+          part = __any_sync(0xffffffffu, part);
+          if (lane == 0) *reinterpret_cast<uint32_t*>(see + FKW_BQ) = part;
         }
 #pragma unroll
         for (int j = 0; j < FKW_BQ / 32; ++j) {
@@ -971,7 +1057,7 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
       bool ok = true;
 #pragma unroll 1
       for (int ps = 0; ps < n_pass && ok; ++ps) {
-        const DkwPass d = dkw_pass(tile_of_pass[ps], T, R, vlen);
+        const DkwPass d = dkw_pass<kMod>(tile_of_pass[ps], T, R, vlen, p, b);
         for (int it = 0, h = kvh * R, i = d.i_first; it < d.iters && ok; ++it, ++uses) {
           const int m0 = i * FKW_BQ;
           for (int w = 0; w < 2; ++w) {
@@ -1016,7 +1102,7 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
       int g0 = 0, kv_loads = 0;
 #pragma unroll 1
       for (int ps = 0; ps < n_pass && ok; ++ps) {
-        const DkwPass d = dkw_pass(tile_of_pass[ps], T, R, vlen);
+        const DkwPass d = dkw_pass<kMod>(tile_of_pass[ps], T, R, vlen, p, b);
         if (d.iters > 0) {
           if (!mbar_wait_warp(kv_full, kv_loads & 1, abort_flag)) { ok = false; break; }
           ++kv_loads;
@@ -1069,6 +1155,7 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
     const int half = wg;                      // dK / dV columns this warpgroup stores at the end of a pass
     const uint32_t lane_sel = uint32_t(q * 32) << 16;
     const float sl2 = p.scale * kFbLog2e;
+    const float kc = kMod == kCap ? 2.f * kFbLog2e * p.scale / p.cap : sl2, c2 = kMod == kCap ? p.cap * kFbLog2e : 0.f;
     uint8_t* stg_row = smem + Smem::kStage + wg * FKV_STG + (q * 32 + lane) * 128;
     const uint32_t swz = uint32_t(lane & 7);
     const bool ds_on = p.ds != nullptr;
@@ -1078,20 +1165,28 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
     int g0 = 0;
 #pragma unroll 1
     for (int ps = 0; ps < n_pass && ok; ++ps) {
-      const DkwPass d = dkw_pass(tile_of_pass[ps], T, R, vlen);
+      const DkwPass d = dkw_pass<kMod>(tile_of_pass[ps], T, R, vlen, p, b);
       const int n0 = d.n0;
       const int key = n0 + q * 32 + lane;
       const bool key_dead = key >= vlen;
+      int h = kvh * R;                        // kBias: whose slope
+      float slope2 = kMod == kBias ? p.slopes[h] * kFbLog2e : 0.f;
       for (int it = 0, i = d.i_first; it < d.iters && ok; ++it) {
         const int g = g0 + it, s2 = g % kSt;
         const int m0 = i * FKW_BQ;
-        if (++i == d.i_first + d.n_qt) i = d.i_first;
+        const float slope_now = slope2;
+        if (++i == d.i_first + d.n_qt) {
+          i = d.i_first;
+          if (kMod == kBias && it + 1 < d.iters) slope2 = p.slopes[++h] * kFbLog2e;
+        }
         const int qb = m0 + wg * 64;                                     // first query column of this warpgroup
-        const float* st = reinterpret_cast<const float*>(smem + Smem::kStats + s2 * 2 * FKW_BQ * 4) + wg * 64;
-        const bool need_mask = (m0 < n0 + 128) || (n0 + 128 > vlen);     // the diagonal tile or the padded tail
+        const float* st = reinterpret_cast<const float*>(smem + Smem::kStats + s2 * Smem::kStatBytes) + wg * 64;
+        bool need_mask = (m0 < n0 + 128) || (n0 + 128 > vlen);     // the diagonal tile or the padded tail
         // This thread's P^T between the two phases: packed (head_dim 128), or as it is (64, which has the registers)
         uint32_t pk[4][8], sc[64];
         if (!mbar_wait(&st_full[s2], (g / kSt) & 1, abort_flag)) { ok = false; break; }
+        const uint32_t* see = reinterpret_cast<const uint32_t*>(st - wg * 64 + 2 * FKW_BQ);
+        if (kMod != kCausal) need_mask = see[FKW_BQ / 2] != 0u;
         if (!mbar_wait(s_full, g & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
         // all 64 columns in one go: a tensor-memory load queues behind the products that are running, so four loads one
@@ -1102,9 +1197,17 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t(&rs)[16] = *reinterpret_cast<uint32_t(*)[16]>(&sc[16 * c]);
-          if (need_mask) fb_p_chunk<true>(rs, pk[c], sl2, st + c * 16, qb + c * 16, key, key_dead);
-          else fb_p_chunk<false>(rs, pk[c], sl2, st + c * 16, 0, 0, false);
+          if constexpr (kMod == kCausal) {
+            if (need_mask) fb_p_chunk<true>(rs, pk[c], sl2, st + c * 16, qb + c * 16, key, key_dead);
+            else fb_p_chunk<false>(rs, pk[c], sl2, st + c * 16, 0, 0, false);
+          } else {
+            const float dist = float(qb + c * 16 - key);
+            if (need_mask)
+              fb_p_chunk_span<true, kMod>(rs, pk[c], kc, c2, st + c * 16, see + (wg * 64 + c * 16) / 2, uint32_t(key - n0), slope_now, dist);
+            else fb_p_chunk_span<false, kMod>(rs, pk[c], kc, c2, st + c * 16, see, 0u, slope_now, dist);
+          }
           tmem_st_32x32b_x8(tS + c * 8, pk[c]);
+          if (kMod == kCap && kD == 128) fb_pack16(&sc[16 * c], pk[c]);      // kept for dS: P (1 - tanh^2)
         }
         tmem_st_wait();
         tc_fence_before();
@@ -1214,7 +1317,8 @@ static SideStream* side_stream() {
 
 int flash_bwd_dq_from_ds(const void* ds, const void* k, void* dq, const void* valid_len, const long long* ks,
                          const long long* dqs, int B, int T, int QH, int KVH, int D, int bchunk,
-                         const float* unrot_cos, const float* unrot_sin, int unrot_ld, cudaStream_t st);
+                         const float* unrot_cos, const float* unrot_sin, int unrot_ld, cudaStream_t st,
+                         const int4* qtab = nullptr);
 
 static int g_dkv_wide = 1;
 
@@ -1226,13 +1330,13 @@ __global__ void smem_base_probe_kernel(int* out) {
   extern __shared__ uint8_t probe_raw[];
   if (threadIdx.x == 0) *out = int(reinterpret_cast<uintptr_t>(probe_raw) & 1023);
 }
-static bool dkv_wide_fits() {
+static bool dkv_wide_fits(int used = FdkwSmem<128>::kUsed) {
   static std::mutex mu;
-  static int fits[64];            // 0 unknown, 1 yes, -1 no
+  static int pads[64];            // 0 unknown, else 1 + the bytes lost to the round-up of the base
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return false;
   std::lock_guard<std::mutex> lock(mu);
-  if (fits[dev] == 0) {
+  if (pads[dev] == 0) {
     int* d = nullptr;
     int off = -1;
     if (cudaMalloc(&d, sizeof(int)) == cudaSuccess) {
@@ -1240,10 +1344,9 @@ static bool dkv_wide_fits() {
       if (cudaMemcpy(&off, d, sizeof(int), cudaMemcpyDeviceToHost) != cudaSuccess) off = -1;
       cudaFree(d);
     }
-    const int pad = off < 0 ? 1024 : (1024 - off) & 1023;        // bytes lost to the round-up of the base
-    fits[dev] = (FdkwSmem<128>::kUsed + pad <= FdkwSmem<128>::kTotal) ? 1 : -1;
+    pads[dev] = 1 + (off < 0 ? 1024 : (1024 - off) & 1023);
   }
-  return fits[dev] > 0;
+  return used + pads[dev] - 1 <= FdkwSmem<128>::kTotal;
 }
 static int g_dkv_pairing = -1;      // -1: by the number of key tiles per SM; 0 / 1: forced (A/B runs)
 
@@ -1278,7 +1381,7 @@ B200_API int b200_flash_bwd_tc(const void* q, const void* k, const void* v, cons
   TensorMap tk = get_tensor_map_bthd(k, B, T, KVH, D, s[3], s[4], s[5], 128, 64);
   TensorMap tv = get_tensor_map_bthd(v, B, T, KVH, D, s[6], s[7], s[8], 128, 64);
   if (!tq128 || !tdo128 || !tq64 || !tdo64 || !tk || !tv) return static_cast<int>(cudaErrorInvalidValue);
-  FlashBwdTcParams p;
+  FlashBwdTcParams p = {};
   p.dq = static_cast<bf16*>(dq); p.dk = static_cast<bf16*>(dk); p.dv = static_cast<bf16*>(dv);
   p.lse = static_cast<const float*>(lse); p.delta = static_cast<const float*>(delta);
   p.valid_len = static_cast<const int*>(valid_len);
@@ -1294,9 +1397,9 @@ B200_API int b200_flash_bwd_tc(const void* q, const void* k, const void* v, cons
                                     FdkvSmem::kTotal));
     B200_CHECK(cudaFuncSetAttribute(flash_bwd_dkv_tc_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     FdkvSmem::kTotal));
-    B200_CHECK(cudaFuncSetAttribute(flash_bwd_dkv_wide_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    B200_CHECK(cudaFuncSetAttribute(flash_bwd_dkv_wide_kernel<64, kCausal>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     FdkwSmem<64>::kTotal));
-    B200_CHECK(cudaFuncSetAttribute(flash_bwd_dkv_wide_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+    B200_CHECK(cudaFuncSetAttribute(flash_bwd_dkv_wide_kernel<128, kCausal>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                     FdkwSmem<128>::kTotal));
     configured = true;
   }
@@ -1333,10 +1436,10 @@ B200_API int b200_flash_bwd_tc(const void* q, const void* k, const void* v, cons
   // head_dim 64: 128-query iterations from 65 tokens on (100: 11.4 us, 12.1 with 64-query ones; 64: 11.3 / 8.5, half of every
   // tile would be past the end)
   if (D == 64 && T > 64)
-    B200_CHECK(launch_pdl(flash_bwd_dkv_wide_kernel<64>, dim3(dkv_ctas), dim3(FBT_THREADS), FdkwSmem<64>::kTotal, st, 0, *tq128,
+    B200_CHECK(launch_pdl(flash_bwd_dkv_wide_kernel<64, kCausal>, dim3(dkv_ctas), dim3(FBT_THREADS), FdkwSmem<64>::kTotal, st, 0, *tq128,
                           *tdo128, *tk, *tv, *tds, p));
   else if (D == 128 && g_dkv_wide && dkv_wide_fits())
-    B200_CHECK(launch_pdl(flash_bwd_dkv_wide_kernel<128>, dim3(dkv_ctas), dim3(FBT_THREADS), FdkwSmem<128>::kTotal, st, 0, *tq128,
+    B200_CHECK(launch_pdl(flash_bwd_dkv_wide_kernel<128, kCausal>, dim3(dkv_ctas), dim3(FBT_THREADS), FdkwSmem<128>::kTotal, st, 0, *tq128,
                           *tdo128, *tk, *tv, *tds, p));
   else
     B200_CHECK(launch_pdl(D == 128 ? flash_bwd_dkv_tc_kernel<128> : flash_bwd_dkv_tc_kernel<64>, dim3(dkv_ctas),
@@ -1356,6 +1459,75 @@ B200_API int b200_flash_bwd_tc(const void* q, const void* k, const void* v, cons
   B200_CHECK(cudaEventRecord(side->join, side->stream));
   B200_CHECK(cudaStreamWaitEvent(st, side->join, 0));
   return 0;
+}
+
+template <int kD, int kMod>
+static int launch_dkv_span(const FlashBwdTcParams& p, const TensorMap (&m)[5], int ctas, cudaStream_t st) {
+  using Smem = FdkwSmem<kD, kMod>;
+  static bool configured = false;
+  if (!configured) {
+    B200_CHECK(cudaFuncSetAttribute(flash_bwd_dkv_wide_kernel<kD, kMod>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem::kTotal));
+    configured = true;
+  }
+  return static_cast<int>(launch_pdl(flash_bwd_dkv_wide_kernel<kD, kMod>, dim3(ctas), dim3(FBT_THREADS), Smem::kTotal, st, 0, *m[0],
+                                     *m[1], *m[2], *m[3], *m[4], p));
+}
+
+// Gradients under a span mask (b200_span_mask), with the cap or the distance bias of b200_flash_fwd_span. Tensors, strides,
+// workspace (not optional) and rotary tables as in b200_flash_bwd_tc.
+B200_API int b200_flash_bwd_span(const void* q, const void* k, const void* v, const void* dout, const void* lse,
+                                 const void* delta, void* dq, void* dk, void* dv, const void* spans, const void* qtab,
+                                 const void* ktab, const long long* s, int B, int T, int QH, int KVH, int D, float scale, float cap,
+                                 const void* slopes, void* ds_ws, const void* unrot_cos, const void* unrot_sin, int unrot_ld,
+                                 cudaStream_t st) {
+  if (B <= 0 || T <= 0) return 0;
+  if ((D != 128 && D != 64) || KVH <= 0 || QH % KVH != 0 || ds_ws == nullptr) return static_cast<int>(cudaErrorInvalidValue);
+  if (cap < 0.f || (cap > 0.f && slopes != nullptr)) return static_cast<int>(cudaErrorInvalidValue);
+  for (int i = 0; i < 21; ++i)
+    if (s[i] % 8 != 0) return static_cast<int>(cudaErrorInvalidValue);
+  if (((reinterpret_cast<uintptr_t>(dq) | reinterpret_cast<uintptr_t>(dk) | reinterpret_cast<uintptr_t>(dv)) & 15) != 0)
+    return static_cast<int>(cudaErrorInvalidValue);
+  if (unrot_cos != nullptr && (unrot_sin == nullptr || unrot_ld < T)) return static_cast<int>(cudaErrorInvalidValue);
+  if (D == 128 && !dkv_wide_fits(FdkwSmem<128, kSpan>::kUsed)) return static_cast<int>(cudaErrorInvalidConfiguration);
+  const int nt = (T + 127) / 128;
+  const unsigned long long Tp = (unsigned long long)nt * 128;
+  const TensorMap maps[5] = {get_tensor_map_bthd(q, B, T, QH, D, s[0], s[1], s[2], 128, 64),
+                             get_tensor_map_bthd(dout, B, T, QH, D, s[9], s[10], s[11], 128, 64),
+                             get_tensor_map_bthd(k, B, T, KVH, D, s[3], s[4], s[5], 128, 64),
+                             get_tensor_map_bthd(v, B, T, KVH, D, s[6], s[7], s[8], 128, 64),
+                             get_tensor_map_bthd(ds_ws, B, Tp, QH, Tp, (unsigned long long)QH * Tp * Tp, Tp, Tp * Tp, 128, 64)};
+  for (const TensorMap& m : maps)
+    if (!m) return static_cast<int>(cudaErrorInvalidValue);
+  FlashBwdTcParams p = {};
+  p.dq = static_cast<bf16*>(dq); p.dk = static_cast<bf16*>(dk); p.dv = static_cast<bf16*>(dv);
+  p.lse = static_cast<const float*>(lse); p.delta = static_cast<const float*>(delta);
+  p.dq_bs = s[12]; p.dq_ts = s[13]; p.dq_hs = s[14];
+  p.dk_bs = s[15]; p.dk_ts = s[16]; p.dk_hs = s[17];
+  p.dv_bs = s[18]; p.dv_ts = s[19]; p.dv_hs = s[20];
+  p.B = B; p.T = T; p.QH = QH; p.KVH = KVH; p.scale = scale; p.status = status_ptr();
+  p.n_tiles = nt;
+  p.ds = static_cast<bf16*>(ds_ws);
+  p.ds_tp = (long long)Tp;
+  p.unrot_cos = static_cast<const float*>(unrot_cos);
+  p.unrot_sin = static_cast<const float*>(unrot_sin);
+  p.unrot_ld = unrot_ld;
+  p.spans = static_cast<const int2*>(spans);
+  p.ktab = static_cast<const int2*>(ktab);
+  p.cap = cap;
+  p.slopes = static_cast<const float*>(slopes);
+  {
+    const int bc = int(80.0e6 / (2.0 * T * D * (2.0 * QH + 2.0 * KVH)));       // as in b200_flash_bwd_tc
+    p.bchunk = bc < 1 ? 1 : (bc > B ? B : bc);
+  }
+  const int ctas = nt * KVH * B;                  // one key tile each: what a tile costs depends on the documents
+  int rc;
+  if (D == 64) rc = cap > 0.f ? launch_dkv_span<64, kCap>(p, maps, ctas, st)
+                    : slopes ? launch_dkv_span<64, kBias>(p, maps, ctas, st) : launch_dkv_span<64, kSpan>(p, maps, ctas, st);
+  else rc = cap > 0.f ? launch_dkv_span<128, kCap>(p, maps, ctas, st)
+            : slopes ? launch_dkv_span<128, kBias>(p, maps, ctas, st) : launch_dkv_span<128, kSpan>(p, maps, ctas, st);
+  if (rc != 0) return rc;
+  return flash_bwd_dq_from_ds(ds_ws, k, dq, nullptr, s + 3, s + 12, B, T, QH, KVH, D, p.bchunk, p.unrot_cos, p.unrot_sin, p.unrot_ld,
+                              st, static_cast<const int4*>(qtab));
 }
 
 // 1 (default): head_dim 128 runs the dK/dV kernel with 128-query iterations (flash_bwd_dkv_wide_kernel); 0: the

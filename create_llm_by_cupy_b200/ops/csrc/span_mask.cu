@@ -1,0 +1,206 @@
+// Which keys each query of a batch sees, and which tiles of 128 queries and 128 keys meet.
+//
+// Query t of row b sees the keys [lo, hi): lo is the first position of its document, hi the position behind it, or the end
+// of the document's leading prefix run if it is part of that; padding (a negative document) sees nothing. The attention
+// kernels read, per query tile, the key tiles it meets and whether a key tile is seen whole by all its rows, and per key
+// tile the query tiles that meet it.
+//
+// One CTA per row: lo is a running maximum over the starts of documents, the end of a prefix run a running minimum from
+// behind. A warp holds 128 consecutive tokens, four to a lane, which are one tile of the tables. A step of a training
+// run makes one mask for all its layers.
+#include <climits>
+
+#include "common.cuh"
+
+namespace b200 {
+
+constexpr int SM_THREADS = 1024;
+constexpr int SM_PER = 4;                             // tokens of a thread
+constexpr int SM_CHUNK = SM_THREADS * SM_PER;         // tokens of a pass
+constexpr int SM_MAX_TILES = 5632;                    // ranges kept in shared memory: 44 KiB, 720896 tokens
+
+struct SpanMaskParams {
+  const int* docs;              // [B, T] or null: one document
+  const unsigned char* prefix;  // [B, T] or null
+  const int* valid_len;         // [B] or null
+  const int* lo_in;             // [B, T]: spans as they are given, in place of all of the above
+  const int* hi_in;
+  int2* spans;                  // [B, T]
+  int4* qtab;                   // [B, nt]: first key tile, end; largest lo, smallest hi of its rows
+  int2* ktab;                   // [B, nt]: first query tile, end
+  int B, T, nt;
+  int* status;
+};
+
+struct MaxOp {
+  static constexpr int kNone = -1;
+  __device__ static int of(int a, int b) { return max(a, b); }
+};
+struct MinOp {
+  static constexpr int kNone = INT_MAX;
+  __device__ static int of(int a, int b) { return min(a, b); }
+};
+
+// v over the threads before this one (kUp) or behind it, the carry first; `carry` leaves with the whole block in it.
+template <class Op, bool kUp>
+__device__ __forceinline__ int block_scan_excl(int v, int& carry, int* warp_v) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  int x = v;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = kUp ? __shfl_up_sync(0xffffffffu, x, o) : __shfl_down_sync(0xffffffffu, x, o);
+    if (kUp ? lane >= o : lane + o < 32) x = Op::of(x, y);
+  }
+  __syncthreads();                                    // the last scan's values have been read
+  if (lane == (kUp ? 31 : 0)) warp_v[warp] = x;
+  int e = kUp ? __shfl_up_sync(0xffffffffu, x, 1) : __shfl_down_sync(0xffffffffu, x, 1);
+  if (lane == (kUp ? 0 : 31)) e = Op::kNone;
+  __syncthreads();
+  int before = carry, all = carry;
+  for (int w = 0; w < SM_THREADS / 32; ++w) {
+    const int y = warp_v[w];
+    if (kUp ? w < warp : w > warp) before = Op::of(before, y);
+    all = Op::of(all, y);
+  }
+  carry = all;
+  return Op::of(before, e);
+}
+
+__device__ __forceinline__ int warp_min(int v) { return __reduce_min_sync(0xffffffffu, v); }
+__device__ __forceinline__ int warp_max(int v) { return __reduce_max_sync(0xffffffffu, v); }
+
+__global__ void __launch_bounds__(SM_THREADS)
+span_mask_kernel(const SpanMaskParams p) {
+  extern __shared__ int2 s_range[];                   // [nt]: key tiles of each query tile
+  __shared__ int warp_v[SM_THREADS / 32];
+  const int b = blockIdx.x, T = p.T;
+  const size_t row0 = size_t(b) * T;
+  pdl_wait();
+  pdl_trigger();
+  const int vlen = p.valid_len ? checked_index(p.valid_len[b], T, p.status, 340) : T;
+  int2* spans = p.spans + row0;
+  const int* docs = p.docs ? p.docs + row0 : nullptr;
+  const unsigned char* pre = p.prefix ? p.prefix + row0 : nullptr;
+
+  // From behind: where the prefix run that a token may be part of ends (the first start or unflagged token behind it). Kept
+  // in the spans' hi until the other pass has lo.
+  if (pre != nullptr && p.lo_in == nullptr) {
+    int carry = T;
+    for (int c0 = (T - 1) / SM_CHUNK * SM_CHUNK; c0 >= 0; c0 -= SM_CHUNK) {
+      const int t0 = c0 + int(threadIdx.x) * SM_PER;
+      int stop[SM_PER], v = MinOp::kNone;
+#pragma unroll
+      for (int i = SM_PER - 1; i >= 0; --i) {
+        const int t = t0 + i;
+        const bool here = t < T && (pre[t] == 0 || t == 0 || (docs != nullptr && docs[t] != docs[t - 1]));
+        stop[i] = v;                                  // the first stop of this thread behind t
+        if (here) v = t;
+      }
+      const int behind = block_scan_excl<MinOp, false>(v, carry, warp_v);
+#pragma unroll
+      for (int i = 0; i < SM_PER; ++i)
+        if (t0 + i < T) spans[t0 + i].y = min(stop[i], behind);
+    }
+    __syncthreads();
+  }
+
+  int carry_start = 0, carry_plain = -1;
+  for (int c0 = 0; c0 < T; c0 += SM_CHUNK) {
+    const int t0 = c0 + int(threadIdx.x) * SM_PER;
+    int lo[SM_PER], hi[SM_PER];
+    if (p.lo_in != nullptr) {
+#pragma unroll
+      for (int i = 0; i < SM_PER; ++i) {
+        lo[i] = t0 + i < T ? p.lo_in[row0 + t0 + i] : 0;
+        hi[i] = t0 + i < T ? p.hi_in[row0 + t0 + i] : 0;
+      }
+    } else {
+      int start[SM_PER], plain[SM_PER], id[SM_PER], s = -1, u = -1;
+#pragma unroll
+      for (int i = 0; i < SM_PER; ++i) {
+        const int t = t0 + i;
+        id[i] = t < T && docs != nullptr ? docs[t] : 0;
+        if (t < T && docs != nullptr && t > 0 && id[i] != (i > 0 ? id[i - 1] : docs[t - 1])) s = t;
+        if (t < T && pre != nullptr && pre[t] == 0) u = t;
+        start[i] = s;
+        plain[i] = u;
+      }
+      const int s_before = block_scan_excl<MaxOp, true>(s, carry_start, warp_v);
+      const int u_before = pre != nullptr ? block_scan_excl<MaxOp, true>(u, carry_plain, warp_v) : -1;
+#pragma unroll
+      for (int i = 0; i < SM_PER; ++i) {
+        const int t = t0 + i;
+        lo[i] = max(start[i], s_before);
+        hi[i] = t + 1;
+        if (pre != nullptr && t < T && max(plain[i], u_before) < lo[i]) hi[i] = spans[t].y;
+        if (id[i] < 0 || t >= vlen) hi[i] = 0;
+        hi[i] = min(hi[i], vlen);
+      }
+    }
+    int lo_min = INT_MAX, lo_max = 0, hi_min = INT_MAX, hi_max = 0;
+#pragma unroll
+    for (int i = 0; i < SM_PER; ++i) {
+      const int t = t0 + i;
+      if (t >= T) continue;
+      lo[i] = max(lo[i], 0);
+      hi[i] = min(hi[i], T);
+      const bool none = hi[i] <= lo[i];
+      spans[t] = none ? make_int2(0, 0) : make_int2(lo[i], hi[i]);
+      if (none) {
+        lo_max = INT_MAX;                             // some row of the tile sees nothing: no key tile is seen by all
+      } else {
+        lo_min = min(lo_min, lo[i]);
+        lo_max = max(lo_max, lo[i]);
+        hi_min = min(hi_min, hi[i]);
+        hi_max = max(hi_max, hi[i]);
+      }
+    }
+    lo_min = warp_min(lo_min);
+    lo_max = warp_max(lo_max);
+    hi_min = warp_min(hi_min);
+    hi_max = warp_max(hi_max);
+    const int tile = t0 / 128;                        // the same for the warp
+    if ((threadIdx.x & 31) == 0 && tile < p.nt) {
+      const int2 r = hi_max > 0 ? make_int2(lo_min / 128, (hi_max + 127) / 128) : make_int2(0, 0);
+      p.qtab[size_t(b) * p.nt + tile] = make_int4(r.x, r.y, lo_max, hi_min);
+      s_range[tile] = r;
+    }
+  }
+  __syncthreads();
+  for (int n = threadIdx.x; n < p.nt; n += SM_THREADS) {
+    int first = INT_MAX, end = 0;
+    for (int m = 0; m < p.nt; ++m) {
+      const int2 r = s_range[m];
+      if (n >= r.x && n < r.y) {
+        first = min(first, m);
+        end = m + 1;
+      }
+    }
+    p.ktab[size_t(b) * p.nt + n] = end > 0 ? make_int2(first, end) : make_int2(0, 0);
+  }
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+// Fills `spans` [B, T] (lo, hi), `qtab` [B, nt] (4 ints) and `ktab` [B, nt] (2 ints), nt = tiles of 128 tokens, from documents,
+// prefix flags and valid lengths (each may be null), or from the spans lo / hi [B, T].
+B200_API int b200_span_mask(const void* docs, const void* prefix, const void* valid_len, const void* lo, const void* hi,
+                            void* spans, void* qtab, void* ktab, int B, int T, cudaStream_t st) {
+  if (B <= 0 || T <= 0) return 0;
+  const int nt = (T + 127) / 128;
+  if (nt > SM_MAX_TILES || (lo == nullptr) != (hi == nullptr)) return static_cast<int>(cudaErrorInvalidValue);
+  SpanMaskParams p;
+  p.docs = static_cast<const int*>(docs);
+  p.prefix = static_cast<const unsigned char*>(prefix);
+  p.valid_len = static_cast<const int*>(valid_len);
+  p.lo_in = static_cast<const int*>(lo);
+  p.hi_in = static_cast<const int*>(hi);
+  p.spans = static_cast<int2*>(spans);
+  p.qtab = static_cast<int4*>(qtab);
+  p.ktab = static_cast<int2*>(ktab);
+  p.B = B; p.T = T; p.nt = nt;
+  p.status = status_ptr();
+  return static_cast<int>(launch_pdl(span_mask_kernel, dim3(B), dim3(SM_THREADS), size_t(nt) * sizeof(int2), st, 0, p));
+}

@@ -1,0 +1,335 @@
+"""Attention beyond one causal sequence per row: packed documents, prefixes and padding (span masks), scores that are capped by
+a tanh or get a bias that grows with the distance, and trees of drafted tokens over a KV cache.
+
+As in ``functional``, every function has two bodies: CUDA tensors go to the hand-written sm_100a kernels (bf16 storage, fp32
+scores, softmax statistics and sums), CPU tensors take a plain torch restatement (fp32, or fp64 for fp64 inputs).
+
+Training and scoring:
+
+    mask = span_mask(B, T, device, docs=ids)                   # once per batch, for all layers
+    o, lse = span_attn_fwd(q, k, v, mask, softcap=50.0)
+    dq, dk, dv = span_attn_bwd(dout, q, k, v, o, lse, mask, softcap=50.0)
+
+Serving, ``n`` drafted tokens of each sequence (n = 1: the decoded token):
+
+    o = tree_attn_append(kqv, kcache, vcache, lens, tree_mask(parents, device), QH, KVH, cos, sin, softcap=50.0)
+
+A cap c makes c tanh(s / c) of every scaled score s; a bias takes slope[head] * |query position - key position| from it.
+"""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import torch
+
+from . import functional as F
+from . import native
+
+_f = ctypes.c_float
+_i = ctypes.c_int
+
+
+# --------------------------------------------------------------------------- span masks
+class SpanMask:
+    """Which keys each query of a [B, T] batch sees: positions [lo, hi) per query, and (CUDA) the tables of tiles of 128 tokens
+    that the kernels walk by. Made by ``span_mask`` or ``SpanMask.from_spans``; one serves any number of layers and heads."""
+
+    def __init__(self, spans, qtab, ktab):
+        self.spans, self.qtab, self.ktab = spans, qtab, ktab        # int32 [B, T, 2]; CUDA: [B, nt, 4], [B, nt, 2]
+        self.B, self.T = spans.shape[0], spans.shape[1]
+
+    @property
+    def device(self):
+        return self.spans.device
+
+    @classmethod
+    def from_spans(cls, lo: torch.Tensor, hi: torch.Tensor) -> "SpanMask":
+        """Query t of row b sees keys lo[b, t] <= s < hi[b, t] (int32 [B, T]; cut to [0, T), nothing where hi <= lo)."""
+        if lo.dim() != 2 or lo.shape != hi.shape or lo.dtype != torch.int32 or hi.dtype != torch.int32 or lo.device != hi.device:
+            raise ValueError("SpanMask.from_spans: lo and hi are int32 [B, T] on one device")
+        return _make_mask(*lo.shape, lo.device, lo=lo.contiguous(), hi=hi.contiguous())
+
+    def rows(self, b0: int, b1: int) -> "SpanMask":
+        """The mask of batch elements [b0, b1), on the same memory."""
+        if self.qtab is None:
+            return SpanMask(self.spans[b0:b1], None, None)
+        return SpanMask(self.spans[b0:b1], self.qtab[b0:b1], self.ktab[b0:b1])
+
+    def dense(self) -> torch.Tensor:
+        """bool [B, T, T]: query t (second) sees key s (third). For verification and small sizes."""
+        s = torch.arange(self.T, device=self.device)
+        return (s >= self.spans[..., :1]) & (s < self.spans[..., 1:])
+
+
+def _make_mask(B, T, device, docs=None, prefix=None, valid_len=None, lo=None, hi=None) -> SpanMask:
+    if torch.device(device).type != "cuda":
+        if lo is None:
+            lo, hi = _spans_reference(B, T, docs, prefix, valid_len)
+        lo, hi = lo.clamp_min(0), hi.clamp_max(T)
+        none = hi <= lo
+        return SpanMask(torch.stack([lo.masked_fill(none, 0), hi.masked_fill(none, 0)], -1).to(torch.int32), None, None)
+    nt = (T + 127) // 128
+    # the tables, whose entries are the wider ones, first
+    buf = torch.empty(B * (6 * nt + 2 * T), dtype=torch.int32, device=device)
+    qtab = buf[:4 * B * nt].view(B, nt, 4)
+    ktab = buf[4 * B * nt:6 * B * nt].view(B, nt, 2)
+    spans = buf[6 * B * nt:].view(B, T, 2)
+    native.check(F._lib().b200_span_mask(native.ptr(docs), native.ptr(prefix), native.ptr(valid_len), native.ptr(lo), native.ptr(hi),
+                                         native.ptr(spans), native.ptr(qtab), native.ptr(ktab), B, T, native.stream_ptr()),
+                 "span_mask")
+    native.bump()
+    return SpanMask(spans, qtab, ktab)
+
+
+def _spans_reference(B, T, docs, prefix, valid_len):
+    t = torch.arange(T)[None].expand(B, T)
+    docs = torch.zeros(B, T, dtype=torch.int32) if docs is None else docs
+    start = torch.ones(B, T, dtype=torch.bool)
+    start[:, 1:] = docs[:, 1:] != docs[:, :-1]
+    lo = torch.cummax(torch.where(start, t, 0), 1).values
+    hi = t + 1
+    if prefix is not None:
+        plain = torch.cummax(torch.where(prefix, -1, t), 1).values           # the last token that is not flagged
+        stop = torch.where(start | ~prefix, t, T)
+        nxt = torch.full((B, T), T)
+        nxt[:, :-1] = torch.flip(torch.cummin(torch.flip(stop[:, 1:], [1]), 1).values, [1])
+        hi = torch.where(prefix & (plain < lo), nxt, hi)
+    vlen = torch.full((B, 1), T) if valid_len is None else valid_len[:, None].long().clamp(0, T)
+    hi = torch.minimum(hi, vlen)
+    return lo, torch.where((docs < 0) | (t >= vlen), torch.zeros_like(hi), hi)
+
+
+def span_mask(B: int, T: int, device, docs=None, prefix=None, valid_len=None) -> SpanMask:
+    """Mask of ``B`` rows of ``T`` tokens. ``docs`` int32 [B, T]: which document a token belongs to; a change of the number
+    starts the next one, a negative one is padding, which sees nothing and is not seen. ``prefix`` bool [B, T]: a document's leading
+    flagged tokens see one another whichever comes first; every other token sees its document up to itself. ``valid_len``
+    int32 [B]: tokens from there on are padding too. Without any of them: plain causal rows."""
+    if B < 0 or T < 0:
+        raise ValueError("span_mask: negative size")
+    for name, x, dt, shape in (("docs", docs, torch.int32, (B, T)), ("prefix", prefix, torch.bool, (B, T)),
+                               ("valid_len", valid_len, torch.int32, (B,))):
+        if x is not None and (x.dtype != dt or tuple(x.shape) != shape):
+            raise ValueError(f"span_mask: {name} is {dt} {list(shape)}")
+        if x is not None and x.device.type != torch.device(device).type:
+            raise ValueError(f"span_mask: {name} is not on {device}")
+    if T > 720896:
+        raise ValueError("span_mask: more than 720896 tokens in a row")
+    docs, prefix, valid_len = (x if x is None else x.contiguous() for x in (docs, prefix, valid_len))
+    return _make_mask(B, T, device, docs, prefix, valid_len)
+
+
+# --------------------------------------------------------------------------- span attention
+def _heads(name: str, q, k, v):
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+        raise ValueError(f"{name}: q is [B, T, query heads, D], k and v are [B, T, KV heads, D]")
+    if k.shape[2] == 0 or q.shape[2] % k.shape[2] != 0:
+        raise ValueError(f"{name}: the query heads are a multiple of the KV heads")
+
+
+def _modifier(name: str, q_heads: int, softcap: float, slopes, device) -> None:
+    if not (softcap >= 0.0 and math.isfinite(softcap)):
+        raise ValueError(f"{name}: softcap is 0 (none) or a positive number")
+    if slopes is None:
+        return
+    if softcap > 0.0:
+        raise ValueError(f"{name}: scores are capped or biased, not both")
+    if slopes.dtype != torch.float32 or tuple(slopes.shape) != (q_heads,) or slopes.device != device:
+        raise ValueError(f"{name}: slopes is float32 [query heads] on the device of q")
+
+
+def _check_mask(name: str, mask: SpanMask, q) -> None:
+    if not isinstance(mask, SpanMask):
+        raise TypeError(f"{name}: mask is a SpanMask")
+    if (mask.B, mask.T) != tuple(q.shape[:2]) or mask.device != q.device:
+        raise ValueError(f"{name}: the mask is of {mask.B} x {mask.T} tokens on {mask.device}, q of {q.shape[0]} x {q.shape[1]} on {q.device}")
+
+
+def _scale(scale, D: int) -> float:
+    scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
+    if not (scale > 0.0 and math.isfinite(scale)):
+        raise ValueError("attention: scale is a positive number")
+    return scale
+
+
+def _tile_view(t: torch.Tensor) -> torch.Tensor:
+    """``t`` [B, T, heads, D] if tiles can be copied from it as it lies (16-byte rows), else a copy."""
+    s, n = t.stride(), t.shape
+    ok = s[3] == 1 and t.data_ptr() % 16 == 0 and all(n[i] == 1 or (s[i] % 8 == 0 and s[i] > 0) for i in range(3))
+    return t if ok else t.clone(memory_format=torch.contiguous_format)
+
+
+def _strides3(t: torch.Tensor) -> list[int]:
+    """(batch, token, head) strides; of a dimension of one, which is never stepped along, one that a tile copy can have."""
+    return [t.stride(i) if t.shape[i] > 1 else 8 for i in range(3)]
+
+
+def _work_dtype(x):
+    return torch.float64 if x.dtype == torch.float64 else torch.float32
+
+
+def _scores_reference(q, k, mask_bool, scale, softcap, slopes, dist):
+    """(modified scores [B, QH, n, S] with -inf where ``mask_bool`` [B, n, S] is False, 1 - tanh^2 or None)."""
+    dt = _work_dtype(q)
+    kx = k.to(dt).repeat_interleave(q.shape[2] // k.shape[2], dim=2)
+    x = torch.einsum("bthd,bshd->bhts", q.to(dt), kx) * scale
+    slope = None
+    if softcap > 0.0:
+        th = torch.tanh(x / softcap)
+        x, slope = softcap * th, 1 - th * th
+    if slopes is not None:
+        x = x - slopes.to(dt)[None, :, None, None] * dist.to(dt)
+    return x.masked_fill(~mask_bool[:, None], float("-inf")), slope
+
+
+def _softmax_reference(x):
+    m = x.amax(-1, keepdim=True) if x.shape[-1] else x.new_full((*x.shape[:-1], 1), float("-inf"))
+    m = torch.where(m == float("-inf"), torch.zeros_like(m), m)
+    e = torch.exp(x - m)
+    total = e.sum(-1, keepdim=True)
+    return e / torch.where(total == 0, torch.ones_like(total), total), (m + torch.log(total))[..., 0]
+
+
+def _span_reference(q, k, v, mask, scale, softcap, slopes):
+    T = q.shape[1]
+    t = torch.arange(T, device=q.device)
+    x, slope = _scores_reference(q, k, mask.dense(), scale, softcap, slopes, (t[:, None] - t[None, :]).abs())
+    p, lse = _softmax_reference(x)
+    vx = v.to(p.dtype).repeat_interleave(q.shape[2] // k.shape[2], dim=2)
+    return torch.einsum("bhts,bshd->bthd", p, vx), lse, p, slope
+
+
+def span_attn_fwd(q, k, v, mask: SpanMask, *, scale: float | None = None, softcap: float = 0.0, slopes=None):
+    """Attention of q [B, T, QH, D] over k, v [B, T, KVH, D] (already rotated; any strides) under ``mask``. CUDA: bf16, D 64 or
+    128. Returns (o [B, T, QH, D] contiguous, lse [B, QH, T] fp32); a query that sees nothing gets zeros and -inf.
+
+    Keys and values that no query of a 128-token tile sees are not read; of those that are, all have to be finite: one that is
+    masked for a single query still goes through the tensor core with weight 0."""
+    _heads("span_attn_fwd", q, k, v)
+    _check_mask("span_attn_fwd", mask, q)
+    B, T, QH, D = q.shape
+    KVH = k.shape[2]
+    _modifier("span_attn_fwd", QH, softcap, slopes, q.device)
+    scale = _scale(scale, D)
+    if not q.is_cuda:
+        o, lse, _, _ = _span_reference(q, k, v, mask, scale, softcap, slopes)
+        return o.to(q.dtype).contiguous(), lse
+    F._bf16(q, k, v)
+    if D not in (64, 128):
+        raise ValueError("span_attn_fwd: CUDA kernels exist for a head dimension of 64 or 128")
+    q, k, v = _tile_view(q), _tile_view(k), _tile_view(v)
+    o = torch.empty((B, T, QH, D), dtype=q.dtype, device=q.device)
+    lse = torch.empty((B, QH, T), dtype=torch.float32, device=q.device)
+    arr = (ctypes.c_longlong * 12)(*_strides3(q), *_strides3(k), *_strides3(v), *_strides3(o))
+    slopes = slopes if slopes is None else slopes.contiguous()
+    native.check(F._lib().b200_flash_fwd_span(native.ptr(q), native.ptr(k), native.ptr(v), native.ptr(o), native.ptr(lse),
+                                              native.ptr(mask.spans), native.ptr(mask.qtab), arr, B, T, QH, KVH, D, _f(scale),
+                                              _f(softcap), native.ptr(slopes), native.stream_ptr()), "flash_fwd_span")
+    native.bump()
+    return o, lse
+
+
+def span_attn_bwd(dout, q, k, v, o, lse, mask: SpanMask, *, scale: float | None = None, softcap: float = 0.0, slopes=None, out=None,
+                  unrotate=None):
+    """Gradients (dq, dk, dv) of ``span_attn_fwd`` with its results ``o``, ``lse``. ``out``: three [B, T, heads, D] views to
+    write into; ``unrotate`` = (cos, sin) tables [>= T, D / 2]: dq and dk leave as gradients of the un-rotated q and k. The
+    kernels keep dS^T of as many batch elements or KV heads at a time as ``functional.FLASH_DQ_GEMM_MAX_BYTES`` holds, of one KV
+    head at least. Deterministic: no atomics."""
+    _heads("span_attn_bwd", q, k, v)
+    _check_mask("span_attn_bwd", mask, q)
+    B, T, QH, D = q.shape
+    KVH = k.shape[2]
+    if dout.shape != q.shape or o.shape != q.shape or tuple(lse.shape) != (B, QH, T):
+        raise ValueError("span_attn_bwd: dout and o are like q, lse is [B, query heads, T]")
+    _modifier("span_attn_bwd", QH, softcap, slopes, q.device)
+    if unrotate is not None and any(x.shape[0] < T or x.shape[1] != D // 2 for x in unrotate):
+        raise ValueError("span_attn_bwd: rotary tables are [>= T, D / 2]")
+    scale = _scale(scale, D)
+    if not q.is_cuda:
+        return _span_bwd_reference(dout, q, k, v, o, mask, scale, softcap, slopes, out, unrotate)
+    F._bf16(dout, q, k, v, o)
+    if D not in (64, 128):
+        raise ValueError("span_attn_bwd: CUDA kernels exist for a head dimension of 64 or 128")
+    if lse.dtype != torch.float32:
+        raise TypeError("span_attn_bwd: lse is float32")
+    q, k, v, dout, o = (_tile_view(t) for t in (q, k, v, dout, o))
+    lse = lse.contiguous()
+    if out is None:
+        dq = torch.empty((B, T, QH, D), dtype=q.dtype, device=q.device)
+        dk, dv = torch.empty((B, T, KVH, D), dtype=q.dtype, device=q.device), torch.empty((B, T, KVH, D), dtype=q.dtype, device=q.device)
+    else:
+        dq, dk, dv = out
+        if dq.shape != q.shape or dk.shape != k.shape or dv.shape != v.shape:
+            raise ValueError("span_attn_bwd: out has the shapes of q, k and v")
+        F._bf16(dq, dk, dv)
+        if any(_tile_view(t) is not t for t in out):
+            raise ValueError("span_attn_bwd: out needs rows on 16-byte boundaries")
+    if B == 0 or T == 0:
+        return dq, dk, dv
+    delta = torch.empty((B, QH, T), dtype=torch.float32, device=q.device)
+    F.flash_delta(o, dout, delta)
+    ucos = usin = None
+    if unrotate is not None:
+        from .gemm import rope_tables_transposed
+        ucos, usin = rope_tables_transposed(unrotate[0].contiguous(), unrotate[1].contiguous())[:2]
+    uld = ucos.shape[1] if ucos is not None else 0
+    slopes = slopes if slopes is None else slopes.contiguous()
+    R = QH // KVH
+    arr = (ctypes.c_longlong * 21)(*_strides3(q), *_strides3(k), *_strides3(v), *_strides3(dout), *_strides3(dq), *_strides3(dk),
+                                   *_strides3(dv))
+    tp = (T + 127) // 128 * 128
+    bc = F._ds_batch_chunk(B, QH, T)
+    if bc >= 1:
+        ws = torch.empty(bc * QH * tp * tp, dtype=torch.bfloat16, device=q.device)
+        chunks = [(b0, min(b0 + bc, B), 0, KVH) for b0 in range(0, B, bc)]
+    else:                                                  # KV heads of one batch element, with their query heads
+        kc = max(1, min(KVH, F._ds_batch_chunk(KVH, R, T)))
+        ws = torch.empty(kc * R * tp * tp, dtype=torch.bfloat16, device=q.device)
+        chunks = [(b0, b0 + 1, g0, min(g0 + kc, KVH)) for b0 in range(B) for g0 in range(0, KVH, kc)]
+    for b0, b1, g0, g1 in chunks:                          # slices along batch and heads keep every stride
+        def qs(t):
+            return native.ptr(t[b0:b1, :, g0 * R:g1 * R])
+
+        def ks(t):
+            return native.ptr(t[b0:b1, :, g0:g1])
+
+        def rows(t):
+            return native.ptr(t[b0:b1, g0 * R:g1 * R])     # contiguous: head slices only come with one batch element
+        m = mask.rows(b0, b1)
+        native.check(F._lib().b200_flash_bwd_span(
+            qs(q), ks(k), ks(v), qs(dout), rows(lse), rows(delta), qs(dq), ks(dk), ks(dv), native.ptr(m.spans), native.ptr(m.qtab),
+            native.ptr(m.ktab), arr, b1 - b0, T, (g1 - g0) * R, g1 - g0, D, _f(scale), _f(softcap),
+            native.ptr(slopes if slopes is None else slopes[g0 * R:g1 * R]), native.ptr(ws), native.ptr(ucos), native.ptr(usin), uld,
+            native.stream_ptr()), "flash_bwd_span")
+    native.bump(2 * len(chunks))
+    return dq, dk, dv
+
+
+def _span_bwd_reference(dout, q, k, v, o, mask, scale, softcap, slopes, out, unrotate):
+    R = q.shape[2] // k.shape[2]
+    B, T, KVH, D = k.shape
+    _, _, p, slope = _span_reference(q, k, v, mask, scale, softcap, slopes)
+    dt = p.dtype
+    do = dout.to(dt)
+    vx, kx = (x.to(dt).repeat_interleave(R, dim=2) for x in (v, k))
+    dp = torch.einsum("bthd,bshd->bhts", do, vx)
+    delta = (do * o.to(dt)).sum(-1).permute(0, 2, 1)
+    ds = p * (dp - delta[..., None]) * scale
+    if slope is not None:
+        ds = ds * slope
+    dq = torch.einsum("bhts,bshd->bthd", ds, kx)
+    dk = torch.einsum("bhts,bthd->bshd", ds, q.to(dt)).reshape(B, T, KVH, R, D).sum(3)
+    dv = torch.einsum("bhts,bthd->bshd", p, do).reshape(B, T, KVH, R, D).sum(3)
+    if unrotate is not None:
+        c, s = (x[:T].to(dt)[None, :, None] for x in unrotate)
+
+        def back(x):
+            y1, y2 = x[..., :D // 2], x[..., D // 2:]
+            return torch.cat([y1 * c + y2 * s, y2 * c - y1 * s], -1)
+        dq, dk = back(dq), back(dk)
+    res = (dq.to(q.dtype), dk.to(q.dtype), dv.to(q.dtype))
+    if out is not None:
+        for dst, src in zip(out, res):
+            dst.copy_(src)
+        return tuple(out)
+    return res
