@@ -63,7 +63,7 @@ TensorMap get_tensor_map_2d(const void* base, uint64_t rows, uint64_t cols, uint
                             uint32_t box_cols, int elem_bytes, int swizzle);
 
 TensorMap get_tensor_map_bthd(const void* base, uint64_t B, uint64_t T, uint64_t heads, uint64_t D, uint64_t bs,
-                              uint64_t ts, uint64_t hs, uint32_t box_t, uint32_t box_d);
+                              uint64_t ts, uint64_t hs, uint32_t box_t, uint32_t box_d, uint32_t box_h = 1);
 
 int num_sms();
 

@@ -1,0 +1,653 @@
+// Attention of drafted tokens over a KV cache (head_dim 128 or 64): n <= 64 drafts per sequence, a tree of them, one of them in
+// the plain decoded step.
+//
+// Draft i of sequence b stands at position len + depth(i). It sees the len cached keys, its ancestors and itself. K, Q, V come
+// packed from the projection, un-rotated: a first kernel rotates Q and K and appends K and V to the caches at len + i.
+//
+//   x = q k scale, capped (c tanh(x / c)) or biased (x - slope |distance|);  o = softmax(x) V
+//
+// The rows of a tile are the drafts times the query heads that share a KV head: every key is read once for all of them, which is
+// all that bounds the kernel while there are few (64 rows of head_dim 128 do 64 multiply-adds per byte read). The work is one
+// list of 128-key tiles, over sequences, KV heads and groups of 128 rows, the drafts a tile of their own behind each
+// sequence's cached ones; the list is cut into as many equal pieces as there are CTAs, so sequences of any mix of lengths keep all
+// SMs busy. A piece that is not all of its rows' keys leaves its maximum, sum and values in a workspace, and a second kernel
+// joins them in the order of the keys.
+//
+// Roles: warp 0 streams Q and the tiles of K and V by TMA, warp 1 issues the products (scores Q K^T into tensor memory, O += P V
+// from it), warps 2..5 do the softmax, a row per thread. Cached rows
+// past the length, which may hold anything, are masked as scores and cleared as values. Every wait is bounded (see ptx.cuh).
+#include <algorithm>
+
+#include "common.cuh"
+#include "ptx.cuh"
+
+namespace b200 {
+
+constexpr float kTaLog2e = 1.4426950408889634f;
+constexpr float kTaRescaleStep = 8.f;
+constexpr int TA_THREADS = 192;
+constexpr int TA_MAX_DRAFTS = 64;                        // the bits of a draft's mask
+constexpr int kTreePlain = 0, kTreeCap = 1, kTreeBias = 2;
+
+struct TreeParams {
+  const bf16* kqv;          // [B * n][ld]: K | Q | V
+  bf16* kc;                 // [B, KVH, Tmax, D]
+  bf16* vc;
+  bf16* q;                  // [B, n, QH, D]: rotated
+  bf16* out;                // [B, n, QH, D]
+  const int* lens;          // [B]
+  const unsigned long long* tree;   // [B, n]: bit j: draft i sees draft j
+  const float* cosr;        // [rows, D / 2]
+  const float* sinr;
+  const float* slopes;      // kTreeBias: [QH]
+  float* part_o;            // [2 * CTAs][128][D]
+  float2* part_ml;          // [2 * CTAs][128]: maximum (log2 units), sum
+  int B, n, QH, KVH, Tmax, table_rows;
+  long long ld;
+  int R, tok, row_tiles;    // query heads of a KV head; drafts of a row tile (R tok <= 128); row tiles of a sequence and KV head
+  int ctas;                 // pieces of the list
+  float scale, cap;
+  int* status;
+};
+
+template <int kD>
+struct TA {
+  static constexpr int kTile = 128 * kD * 2;
+  static constexpr int kStages = 3;
+  static constexpr int kCtas = kD == 128 ? 1 : 2;
+  static constexpr int kQ = 0, kK = kTile, kV = kK + kStages * kTile;
+  static constexpr int kBar = kV + kStages * kTile;
+  // k_full, k_empty, v_full, v_empty [3]; q_full, q_empty, s_full, s_read, p_full, pv_done, o_free
+  static constexpr int kBars = 4 * kStages + 7;
+  static constexpr int kSmem = kBar + kBars * 8 + 64 + 1024;
+  static constexpr int kCols = kD == 128 ? 512 : 256;
+  static constexpr uint32_t kColS = 0, kColO = 128, kColP = 128 + kD;
+};
+
+// A stretch of one (sequence, KV head, row tile): tiles [t0, t1) of its nt, the last of which are the drafts.
+struct TreeSeg {
+  int b, kvh, rt, t0, t1, nt, len;
+};
+
+__device__ __forceinline__ int tree_len(const TreeParams& p, int b) { return checked_index(p.lens[b], p.Tmax, p.status, 350); }
+__device__ __forceinline__ int tree_tiles(int len) { return (len + 127) / 128 + 1; }
+
+// The list position `at` as (sequence, first list position of it), and the list's length; by a whole warp.
+__device__ __forceinline__ void tree_find(const TreeParams& p, long long num, long long den, int lane, long long& total, long long& at,
+                                          int& b_at, long long& b_first) {
+  const int per = p.KVH * p.row_tiles;
+  long long sum = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int b = b0 + lane;
+    int v = b < p.B ? tree_tiles(tree_len(p, b)) : 0;
+    sum += __reduce_add_sync(0xffffffffu, v);
+  }
+  total = sum * per;
+  at = num * total / den;
+  b_at = 0;
+  b_first = 0;
+  for (int b = 0; b < p.B; ++b) {
+    const long long next = b_first + (long long)tree_tiles(tree_len(p, b)) * per;
+    if (at < next) {
+      b_at = b;
+      return;
+    }
+    b_first = next;
+  }
+  b_at = p.B;
+}
+
+// Walks the pieces of one CTA.
+struct TreeWalk {
+  long long left;           // tiles that are left to it
+  int b, idx, tile;         // where it stands: sequence, KV head * row tiles + row tile, tile
+  __device__ __forceinline__ bool next(const TreeParams& p, TreeSeg& s) {
+    if (left <= 0) return false;
+    s.b = b;
+    s.len = tree_len(p, b);
+    s.nt = tree_tiles(s.len);
+    s.kvh = idx / p.row_tiles;
+    s.rt = idx % p.row_tiles;
+    s.t0 = tile;
+    s.t1 = int(min((long long)s.nt, tile + left));
+    left -= s.t1 - s.t0;
+    tile = s.t1;
+    if (tile == s.nt) {
+      tile = 0;
+      if (++idx == p.KVH * p.row_tiles) {
+        idx = 0;
+        ++b;
+      }
+    }
+    return true;
+  }
+};
+
+__device__ __forceinline__ void ta_unpack(const uint4& u, float (&f)[8]) {
+  const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    f[2 * i] = __uint_as_float(w[i] << 16);
+    f[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+  }
+}
+
+// 8 elements from chunk `c` of the head at `x`, rotated by the table row of `pos` (half-split pairs) and rounded to bf16: the type
+// of the cache, and of the tensor core's operands.
+template <int kD>
+__device__ __forceinline__ uint4 ta_rotated(const TreeParams& p, const bf16* x, int c, int pos) {
+  constexpr int kHalf = kD / 16;
+  float a[8], b[8];
+  ta_unpack(reinterpret_cast<const uint4*>(x)[c], a);
+  ta_unpack(reinterpret_cast<const uint4*>(x)[c ^ kHalf], b);
+  const int j = (c % kHalf) * 8;
+  const size_t row = size_t(min(max(pos, 0), p.table_rows - 1)) * (kD / 2) + j;
+  uint4 u;
+  uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const float4 cs = *reinterpret_cast<const float4*>(p.cosr + row + 4 * h), sn = *reinterpret_cast<const float4*>(p.sinr + row + 4 * h);
+    const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
+    float y[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) y[e] = c < kHalf ? a[4 * h + e] * cv[e] - b[4 * h + e] * sv[e] : a[4 * h + e] * cv[e] + b[4 * h + e] * sv[e];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const bf162 t = __floats2bfloat162_rn(y[2 * e], y[2 * e + 1]);
+      w[2 * h + e] = *reinterpret_cast<const uint32_t*>(&t);
+    }
+  }
+  return u;
+}
+
+__device__ __forceinline__ int tree_depth(unsigned long long bits) { return max(__popcll(bits) - 1, 0); }
+
+// A thread per 16 bytes of the packed projection: K (rotated) and V to the caches, Q (rotated) to its workspace.
+template <int kD>
+__global__ void __launch_bounds__(256)
+tree_append_kernel(const TreeParams p) {
+  constexpr int kChunks = kD / 8;
+  pdl_wait();
+  pdl_trigger();
+  const int heads = p.QH + 2 * p.KVH;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= (long long)p.B * p.n * heads * kChunks) return;
+  const int c = int(i % kChunks), head = int(i / kChunks % heads);
+  const long long row = i / kChunks / heads;
+  const int b = int(row / p.n), d = int(row % p.n);
+  const int len = tree_len(p, b), pos = len + tree_depth(p.tree[row]);
+  const bf16* x = p.kqv + row * p.ld + head * kD;
+  if (head >= p.KVH && head < p.KVH + p.QH) {
+    reinterpret_cast<uint4*>(p.q + (row * p.QH + head - p.KVH) * kD)[c] = ta_rotated<kD>(p, x, c, pos);
+    return;
+  }
+  const bool value = head >= p.KVH;
+  if (len + d >= p.Tmax) return;
+  const uint4 u = value ? reinterpret_cast<const uint4*>(x)[c] : ta_rotated<kD>(p, x, c, pos);
+  const int kvh = value ? head - p.KVH - p.QH : head;
+  reinterpret_cast<uint4*>((value ? p.vc : p.kc) + ((size_t(b) * p.KVH + kvh) * p.Tmax + len + d) * kD)[c] = u;
+}
+
+// 16-byte chunk `c` of row `r` in a tile of 128-byte rows (64 columns a box, 16 KiB apart), as TMA writes it.
+__device__ __forceinline__ uint4* ta_chunk(uint8_t* tile, int r, int c) {
+  return reinterpret_cast<uint4*>(tile + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+__device__ __forceinline__ void ta_bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
+
+template <int kD, int kMod>
+__global__ void __launch_bounds__(TA_THREADS, TA<kD>::kCtas)
+tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
+                 const TreeParams p) {
+  using L = TA<kD>;
+  constexpr int kSt = L::kStages;
+  constexpr uint32_t kTile = L::kTile;
+  extern __shared__ uint8_t ta_smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ta_smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::kBar);
+  uint64_t* k_empty = k_full + kSt;
+  uint64_t* v_full = k_empty + kSt;
+  uint64_t* v_empty = v_full + kSt;
+  uint64_t* q_full = v_empty + kSt;      // Q of a piece has arrived
+  uint64_t* q_empty = q_full + 1;        // every score product of a piece has read it
+  uint64_t* s_full = q_empty + 1;        // scores of a tile are in tensor memory
+  uint64_t* s_read = s_full + 1;         // the softmax has them in registers (128)
+  uint64_t* p_full = s_read + 1;         // P of a tile is in tensor memory (128)
+  uint64_t* pv_done = p_full + 1;        // O includes the tile
+  uint64_t* o_free = pv_done + 1;        // O of a piece has been stored (128)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_free + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  long long* walk_at = reinterpret_cast<long long*>(tmem_slot + 2);          // [0] tiles of this CTA, [1] sequence, [2] place in it
+  __shared__ unsigned char s_depth[TA_MAX_DRAFTS];                           // kTreeBias: of the piece's drafts
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kSt; ++s) {
+      mbar_init(&k_full[s], 1);
+      mbar_init(&k_empty[s], 1);
+      mbar_init(&v_full[s], 1);
+      mbar_init(&v_empty[s], 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(q_empty, 1);
+    mbar_init(s_full, 1);
+    mbar_init(s_read, 128);
+    mbar_init(p_full, 128);
+    mbar_init(pv_done, 1);
+    mbar_init(o_free, 128);
+    *abort_flag = 0;
+    mbar_fence_init();
+    tma_prefetch_desc(&tmQ);
+    tma_prefetch_desc(&tmK);
+    tma_prefetch_desc(&tmV);
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, L::kCols);
+  pdl_wait();
+  pdl_trigger();
+  if (warp == 0) {
+    long long total, at, b_first, end;
+    int b_at;
+    tree_find(p, blockIdx.x, p.ctas, lane, total, at, b_at, b_first);
+    end = (long long)(blockIdx.x + 1) * total / p.ctas;
+    if (lane == 0) {
+      walk_at[0] = end - at;
+      walk_at[1] = b_at;
+      walk_at[2] = at - b_first;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem_base = *tmem_slot;
+  TreeWalk walk;
+  walk.left = walk_at[0];
+  walk.b = int(walk_at[1]);
+  {
+    const int nt = walk.left > 0 ? tree_tiles(tree_len(p, walk.b)) : 1;
+    walk.idx = int(walk_at[2] / nt);
+    walk.tile = int(walk_at[2] % nt);
+  }
+  TreeSeg s;
+
+  if (warp == 0) {
+    // ---------------------------------------------------------------- TMA
+    if (lane == 0) {
+      int g = 0, seg = 0;
+      bool ok = true;
+      while (ok && walk.next(p, s)) {
+        if (seg > 0 && !mbar_wait(q_empty, (seg - 1) & 1, abort_flag)) break;
+        ++seg;
+        const int d0 = s.rt * p.tok;
+        mbar_expect_tx(q_full, uint32_t(p.R * p.tok) * kD * 2);          // (rows past the box: whatever, their results go nowhere)
+        tma_load_4d(smem + L::kQ, &tmQ, q_full, 0, s.kvh * p.R, d0, s.b);
+        if (kD == 128) tma_load_4d(smem + L::kQ + 16384, &tmQ, q_full, 64, s.kvh * p.R, d0, s.b);
+        for (int t = s.t0; t < s.t1; ++t, ++g) {
+          const int row = t == s.nt - 1 ? s.len : t * 128;               // the drafts stand behind the cached keys
+          const int st = g % kSt;
+          const uint32_t par = ((g / kSt) & 1) ^ 1;
+          if (!mbar_wait(&k_empty[st], par, abort_flag)) { ok = false; break; }
+          uint8_t* sK = smem + L::kK + st * kTile;
+          mbar_expect_tx(&k_full[st], kTile);
+          tma_load_4d(sK, &tmK, &k_full[st], 0, s.kvh, row, s.b);
+          if (kD == 128) tma_load_4d(sK + 16384, &tmK, &k_full[st], 64, s.kvh, row, s.b);
+          if (!mbar_wait(&v_empty[st], par, abort_flag)) { ok = false; break; }
+          uint8_t* sV = smem + L::kV + st * kTile;
+          mbar_expect_tx(&v_full[st], kTile);
+          tma_load_4d(sV, &tmV, &v_full[st], 0, s.kvh, row, s.b);
+          if (kD == 128) tma_load_4d(sV + 16384, &tmV, &v_full[st], 64, s.kvh, row, s.b);
+        }
+      }
+    }
+  } else if (warp == 1) {
+    // ---------------------------------------------------------------- products
+    constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128, 0, 0), idesc_s64 = umma_idesc_bf16(128, 64, 0, 0);
+    constexpr uint32_t idesc_pv = umma_idesc_bf16(128, kD, 0, 1);
+    int g = 0, seg = 0;
+    bool ok = true;
+    auto issue_s = [&](int g, bool drafts) {             // 64 keys are enough for the drafts
+      const uint64_t dQ = umma_smem_desc(smem_u32(smem + L::kQ), 16, 1024);
+      const uint64_t dK = umma_smem_desc(smem_u32(smem + L::kK + (g % kSt) * kTile), 16, 1024);
+#pragma unroll
+      for (int kk = 0; kk < kD / 16; ++kk) {
+        const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+        umma_bf16_ss_warp(tmem_base + L::kColS, dQ + off, dK + off, drafts ? idesc_s64 : idesc_s, kk != 0);
+      }
+      umma_commit_warp(s_full);
+      umma_commit_warp(&k_empty[g % kSt]);
+    };
+    auto issue_pv = [&](int g, bool drafts, bool first) {
+      const uint64_t dV = umma_smem_desc(smem_u32(smem + L::kV + (g % kSt) * kTile), 16384, 1024);
+#pragma unroll
+      for (int kk = 0; kk < 8; ++kk)
+        if (kk < 4 || !drafts)
+          umma_bf16_ts_warp(tmem_base + L::kColO, tmem_base + L::kColP + kk * 8, dV + kk * 128, idesc_pv, !first || kk != 0);
+      umma_commit_warp(pv_done);
+      umma_commit_warp(&v_empty[g % kSt]);
+    };
+    while (ok && walk.next(p, s)) {
+      ok = mbar_wait_warp(q_full, seg & 1, abort_flag);
+      for (int t = s.t0; t < s.t1 && ok; ++t, ++g) {
+        // scores of the first tile here, of every other one ahead of the P V of the tile before it
+        auto scores = [&](int u, int gu) {
+          if (gu > 0 && !mbar_wait_warp(s_read, (gu - 1) & 1, abort_flag)) return false;
+          if (!mbar_wait_warp(&k_full[gu % kSt], (gu / kSt) & 1, abort_flag)) return false;
+          tc_fence_after();
+          issue_s(gu, u == s.nt - 1);
+          if (u + 1 == s.t1) umma_commit_warp(q_empty);
+          return true;
+        };
+        if (t == s.t0 && !scores(t, g)) { ok = false; break; }
+        if (t + 1 < s.t1 && !scores(t + 1, g + 1)) { ok = false; break; }
+        if (t == s.t0 && seg > 0 && !mbar_wait_warp(o_free, (seg - 1) & 1, abort_flag)) { ok = false; break; }
+        if (!mbar_wait_warp(p_full, g & 1, abort_flag) || !mbar_wait_warp(&v_full[g % kSt], (g / kSt) & 1, abort_flag)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        issue_pv(g, t == s.nt - 1, t == s.t0);
+      }
+      ++seg;
+    }
+  } else {
+    // ---------------------------------------------------------------- softmax: a row per thread
+    const int q = warp & 3, r = q * 32 + lane;           // the quarter of tensor memory that a warp reaches is its number modulo 4
+    const uint32_t lane_sel = uint32_t(q * 32) << 16;
+    const uint32_t tS = tmem_base + lane_sel + L::kColS, tO = tmem_base + lane_sel + L::kColO, tP = tmem_base + lane_sel + L::kColP;
+    const float sl2 = kMod == kTreePlain ? p.scale * kTaLog2e : 1.f;
+    const float kc = kMod == kTreeCap ? 2.f * kTaLog2e * p.scale / p.cap : p.scale * kTaLog2e, c2 = kMod == kTreeCap ? p.cap * kTaLog2e : 0.f;
+    const long long first = (long long)blockIdx.x;
+    int g = 0, seg = 0;
+    bool ok = true;
+    while (ok && walk.next(p, s)) {
+      const int live = min(p.n - s.rt * p.tok, p.tok) * p.R;
+      const bool work = q * 32 < live;                   // this warp has rows at all
+      const int d = min(s.rt * p.tok + r / p.R, p.n - 1), h = s.kvh * p.R + r % p.R;
+      const unsigned long long bits = p.tree[size_t(s.b) * p.n + d];
+      float slope2 = 0.f, pos = 0.f;
+      if constexpr (kMod == kTreeBias) {
+        slope2 = p.slopes[h] * kTaLog2e;
+        pos = float(s.len + tree_depth(bits));
+        ta_bar_sync(2, 128);                             // the last piece's depths have been read
+        for (int i = r; i < TA_MAX_DRAFTS; i += 128)
+          s_depth[i] = i < p.n ? tree_depth(p.tree[size_t(s.b) * p.n + i]) : 0;
+        ta_bar_sync(2, 128);
+      }
+      float m_ref = -INFINITY, l_run = 0.f;
+      for (int t = s.t0; t < s.t1 && ok; ++t, ++g) {
+        if (!mbar_wait(s_full, g & 1, abort_flag)) { ok = false; break; }
+        tc_fence_after();
+        const bool drafts = t == s.nt - 1;
+        const int rem = drafts ? p.n : min(s.len - t * 128, 128);        // keys of the tile
+        uint32_t sc[128];
+        if (work) {
+          tmem_ld_32x32b_x32(tS, *reinterpret_cast<uint32_t(*)[32]>(&sc[0]));
+          tmem_ld_32x32b_x32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&sc[32]));
+          tmem_ld_32x32b_x32(tS + 64, *reinterpret_cast<uint32_t(*)[32]>(&sc[64]));
+          tmem_ld_32x32b_x32(tS + 96, *reinterpret_cast<uint32_t(*)[32]>(&sc[96]));
+          tmem_ld_wait();
+        }
+        tc_fence_before();
+        mbar_arrive(s_read);
+        float rs0 = 0.f, rs1 = 0.f;
+        if (work) {
+          if constexpr (kMod == kTreeCap) {
+#pragma unroll
+            for (int e = 0; e < 128; ++e)
+              sc[e] = __float_as_uint(fmaf(-2.f * c2, __fdividef(1.f, 1.f + exp2f(__uint_as_float(sc[e]) * kc)), c2));
+          } else if constexpr (kMod == kTreeBias) {
+            const float dist = pos - float(t * 128);
+#pragma unroll
+            for (int e = 0; e < 128; ++e) {
+              const float far = drafts ? fabsf(pos - float(s.len + s_depth[e & 63])) : fabsf(dist - float(e));
+              sc[e] = __float_as_uint(fmaf(__uint_as_float(sc[e]), kc, -slope2 * far));
+            }
+          }
+          if (drafts) {
+#pragma unroll
+            for (int e = 0; e < 128; ++e)
+              if (e >= 64 || !((bits >> (e & 63)) & 1) || e >= rem) sc[e] = 0xff800000u;
+          } else if (rem < 128) {
+#pragma unroll
+            for (int e = 0; e < 128; ++e)
+              if (e >= rem) sc[e] = 0xff800000u;
+          }
+          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+          for (int e = 0; e < 128; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(sc[e]));
+          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
+          // the reference maximum moves when a tile exceeds it by more than 2^8, as in the attention forward
+          const bool need = mx > m_ref + kTaRescaleStep;
+          if (t == s.t0) {
+            m_ref = mx;
+          } else if (__any_sync(0xffffffffu, need)) {
+            if (!__all_sync(0xffffffffu, mbar_wait(pv_done, (g - 1) & 1, abort_flag))) { ok = false; break; }
+            tc_fence_after();
+            const float corr = need ? exp2f(m_ref - mx) : 1.f;
+            l_run *= corr;
+#pragma unroll 1
+            for (int c = 0; c < kD / 16; ++c) {
+              uint32_t o[16];
+              tmem_ld_32x32b_x16(tO + c * 16, o);
+              tmem_ld_wait();
+#pragma unroll
+              for (int e = 0; e < 16; ++e) o[e] = corr == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * corr);
+              tmem_st_32x32b_x16(tO + c * 16, o);
+            }
+            tmem_st_wait();
+            if (need) m_ref = mx;
+          }
+          const float m_sub = m_ref == -INFINITY ? 0.f : m_ref;
+#pragma unroll
+          for (int e = 0; e < 128; e += 2) {
+            const float p0 = exp2f(fmaf(__uint_as_float(sc[e]), sl2, -m_sub)), p1 = exp2f(fmaf(__uint_as_float(sc[e + 1]), sl2, -m_sub));
+            rs0 += p0;
+            rs1 += p1;
+            const bf162 x = __floats2bfloat162_rn(p0, p1);
+            sc[e >> 1] = *reinterpret_cast<const uint32_t*>(&x);
+          }
+        }
+        // P of the tile before has been read
+        if (t > s.t0 && !__all_sync(0xffffffffu, mbar_wait(pv_done, (g - 1) & 1, abort_flag))) { ok = false; break; }
+        tc_fence_after();
+        if (work) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) tmem_st_32x32b_x16(tP + c * 16, *reinterpret_cast<const uint32_t(*)[16]>(&sc[16 * c]));
+          tmem_st_wait();
+          l_run += rs0 + rs1;
+        }
+        if (rem < (drafts ? 64 : 128)) {                 // values past the length may be anything, and 0 times that
+          const int st = g % kSt;
+          if (!__all_sync(0xffffffffu, mbar_wait(&v_full[st], (g / kSt) & 1, abort_flag))) { ok = false; break; }
+          for (int i = r; i < ((drafts ? 64 : 128) - rem) * (kD / 8); i += 128)
+            *ta_chunk(smem + L::kV + st * kTile, rem + i / (kD / 8), i % (kD / 8)) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async_smem();
+        }
+        tc_fence_before();
+        mbar_arrive(p_full);
+      }
+      if (!ok) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(pv_done, (g - 1) & 1, abort_flag))) { ok = false; break; }
+      tc_fence_after();
+      const bool whole = s.t0 == 0 && s.t1 == s.nt, alive = r < live;
+      if (work) {
+        const size_t slot = size_t(2 * first + (seg == 0 ? 0 : 1)) * 128 + r;
+        const float inv = whole ? (l_run == 0.f ? 0.f : 1.f / l_run) : 1.f;
+        bf16* orow = p.out + ((size_t(s.b) * p.n + d) * p.QH + h) * kD;
+        if (alive && !whole) p.part_ml[slot] = make_float2(m_ref, l_run);
+#pragma unroll 1
+        for (int c = 0; c < kD / 32; ++c) {
+          uint32_t o[32];
+          tmem_ld_32x32b_x32(tO + c * 32, o);
+          tmem_ld_wait();
+          if (!alive) continue;
+          if (l_run == 0.f) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = 0u;
+          }
+          if (whole) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+              uint4 u;
+              bf162* u2 = reinterpret_cast<bf162*>(&u);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                u2[e] = __floats2bfloat162_rn(__uint_as_float(o[8 * k + 2 * e]) * inv, __uint_as_float(o[8 * k + 2 * e + 1]) * inv);
+              reinterpret_cast<uint4*>(orow + c * 32)[k] = u;
+            }
+          } else {
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+              reinterpret_cast<uint4*>(p.part_o + slot * kD + c * 32)[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+          }
+        }
+      }
+      tc_fence_before();
+      mbar_arrive(o_free);
+      ++seg;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem_base, L::kCols);
+  }
+  if (threadIdx.x == 0 && *abort_flag != 0 && p.status != nullptr) {
+    if (atomicCAS(p.status, 0, int(*abort_flag)) == 0) p.status[1] = 351;
+  }
+}
+
+// Joins the pieces of every (sequence, KV head, row tile) that was cut: grid (those, 4), 32 rows a CTA, a warp a row at a time.
+template <int kD>
+__global__ void __launch_bounds__(256)
+tree_join_kernel(const TreeParams p) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  pdl_wait();
+  pdl_trigger();
+  const int per = p.KVH * p.row_tiles, b = blockIdx.x / per, idx = blockIdx.x % per, kvh = idx / p.row_tiles, rt = idx % p.row_tiles;
+  const int live = min(p.n - rt * p.tok, p.tok) * p.R, row0 = blockIdx.y * 32;
+  if (row0 >= live) return;
+  long long sum = 0, before = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int v = b0 + lane < p.B ? tree_tiles(tree_len(p, b0 + lane)) : 0;
+    sum += __reduce_add_sync(0xffffffffu, v);
+    before += __reduce_add_sync(0xffffffffu, b0 + lane < b ? v : 0);
+  }
+  const int nt = tree_tiles(tree_len(p, b));
+  const long long total = sum * per, t0 = before * per + (long long)idx * nt, G = p.ctas;
+  // tile t is in the piece of CTA ((t + 1) G - 1) / total
+  const long long c0 = ((t0 + 1) * G - 1) / total, c1 = ((t0 + nt) * G - 1) / total;
+  if (c0 == c1) return;
+  for (int r = row0 + warp; r < min(row0 + 32, live); r += 8) {
+    constexpr int kV = kD / 32;
+    float mx = -INFINITY;
+    for (long long c = c0 + lane; c <= c1; c += 32) {
+      if (c * total / G == (c + 1) * total / G) continue;
+      const long long slot = 2 * c + (c == c0 && c * total / G < t0 ? 1 : 0);
+      mx = fmaxf(mx, p.part_ml[slot * 128 + r].x);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    const float ref = mx == -INFINITY ? 0.f : mx;
+    float l = 0.f, acc[kV];
+#pragma unroll
+    for (int e = 0; e < kV; ++e) acc[e] = 0.f;
+    for (long long c = c0; c <= c1; ++c) {
+      if (c * total / G == (c + 1) * total / G) continue;
+      const long long slot = (2 * c + (c == c0 && c * total / G < t0 ? 1 : 0)) * 128 + r;
+      const float2 ml = p.part_ml[slot];
+      const float f = exp2f(ml.x - ref);
+      l += ml.y * f;
+      const float* o = p.part_o + slot * kD + lane * kV;
+#pragma unroll
+      for (int e = 0; e < kV; ++e) acc[e] += o[e] * f;
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const int d = rt * p.tok + r / p.R, h = kvh * p.R + r % p.R;
+    bf16* out = p.out + ((size_t(b) * p.n + d) * p.QH + h) * kD + lane * kV;
+#pragma unroll
+    for (int e = 0; e < kV; e += 2) *reinterpret_cast<bf162*>(out + e) = __floats2bfloat162_rn(acc[e] * inv, acc[e + 1] * inv);
+  }
+}
+
+template <int kD, int kMod>
+static int launch_tree(const TreeParams& p, const TensorMap& tq, const TensorMap& tk, const TensorMap& tv, cudaStream_t st) {
+  static bool configured = false;
+  if (!configured) {
+    B200_CHECK(cudaFuncSetAttribute(tree_attn_kernel<kD, kMod>, cudaFuncAttributeMaxDynamicSharedMemorySize, TA<kD>::kSmem));
+    configured = true;
+  }
+  const long long chunks = (long long)p.B * p.n * (p.QH + 2 * p.KVH) * (kD / 8);
+  B200_CHECK(launch_pdl(tree_append_kernel<kD>, dim3(unsigned((chunks + 255) / 256)), dim3(256), 0, st, 0, p));
+  B200_CHECK(launch_pdl(tree_attn_kernel<kD, kMod>, dim3(p.ctas), dim3(TA_THREADS), TA<kD>::kSmem, st, 0, *tq, *tk, *tv, p));
+  return static_cast<int>(launch_pdl(tree_join_kernel<kD>, dim3(p.B * p.KVH * p.row_tiles, 4), dim3(256), 0, st, 0, p));
+}
+
+static int tree_row_tiles(int n, int R) { return (n + 128 / R - 1) / (128 / R); }
+
+// Pieces that the list of tiles is cut into: what runs at once, or every tile if there are fewer of full caches.
+static int tree_ctas(int B, int n, int QH, int KVH, int Tmax, int D) {
+  const long long tiles = (long long)B * KVH * tree_row_tiles(n, QH / KVH) * ((Tmax + 127) / 128 + 1);
+  const int slots = num_sms() * (D == 128 ? TA<128>::kCtas : TA<64>::kCtas);
+  return int(tiles < slots ? tiles : slots);
+}
+
+static bool tree_shape_ok(int B, int n, int QH, int KVH, int Tmax, int D) {
+  return B >= 0 && n >= 1 && n <= TA_MAX_DRAFTS && (D == 64 || D == 128) && KVH > 0 && QH > 0 && QH % KVH == 0 && QH / KVH <= 128 &&
+         Tmax > 0 && (long long)B * KVH * tree_row_tiles(n, QH / KVH) <= 0x7fffffffLL;
+}
+
+}  // namespace b200
+
+using namespace b200;
+
+// Bytes of the workspace that b200_tree_attn_append wants (16-byte aligned); 0: sizes that it does not take.
+B200_API long long b200_tree_attn_workspace(int B, int n, int QH, int KVH, int Tmax, int D) {
+  if (!tree_shape_ok(B, n, QH, KVH, Tmax, D)) return 0;
+  return 2LL * tree_ctas(B, n, QH, KVH, Tmax, D) * 128 * (D * 4 + 8) + 2LL * B * n * QH * D;
+}
+
+// kqv [B * n][ld] (K | Q | V, un-rotated), caches [B, KVH, Tmax, D], out [B, n, QH, D], lens [B], tree [B, n] (64 bits each), rotary
+// tables [table_rows, D / 2]. cap > 0: scores c tanh(s / c); slopes [QH]: scores minus slope times distance (not both).
+B200_API int b200_tree_attn_append(const void* kqv, void* kc, void* vc, void* out, const void* lens, const void* tree, const void* cosr,
+                                   const void* sinr, const void* slopes, void* workspace, int B, int n, int QH, int KVH, int Tmax, int D,
+                                   int table_rows, long long ld, float scale, float cap, cudaStream_t st) {
+  if (!tree_shape_ok(B, n, QH, KVH, Tmax, D)) return static_cast<int>(cudaErrorInvalidValue);
+  if (B == 0) return 0;
+  if (cap < 0.f || (cap > 0.f && slopes != nullptr) || table_rows < 1 || ld % 8 != 0) return static_cast<int>(cudaErrorInvalidValue);
+  for (const void* x : {kqv, (const void*)kc, (const void*)vc, (const void*)out, cosr, sinr, (const void*)workspace})
+    if (x == nullptr || (reinterpret_cast<uintptr_t>(x) & 15) != 0) return static_cast<int>(cudaErrorInvalidValue);
+  const unsigned long long hs = (unsigned long long)Tmax * D;
+  const TensorMap tk = get_tensor_map_bthd(kc, B, Tmax, KVH, D, KVH * hs, D, hs, 128, 64);
+  const TensorMap tv = get_tensor_map_bthd(vc, B, Tmax, KVH, D, KVH * hs, D, hs, 128, 64);
+  TreeParams p;
+  p.kqv = static_cast<const bf16*>(kqv);
+  p.kc = static_cast<bf16*>(kc);
+  p.vc = static_cast<bf16*>(vc);
+  p.out = static_cast<bf16*>(out);
+  p.lens = static_cast<const int*>(lens);
+  p.tree = static_cast<const unsigned long long*>(tree);
+  p.cosr = static_cast<const float*>(cosr);
+  p.sinr = static_cast<const float*>(sinr);
+  p.slopes = static_cast<const float*>(slopes);
+  p.B = B; p.n = n; p.QH = QH; p.KVH = KVH; p.Tmax = Tmax; p.table_rows = table_rows; p.ld = ld;
+  p.R = QH / KVH;
+  p.tok = std::min(n, 128 / p.R);
+  p.row_tiles = tree_row_tiles(n, p.R);
+  p.ctas = tree_ctas(B, n, QH, KVH, Tmax, D);
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + 2LL * p.ctas * 128 * D);
+  p.q = reinterpret_cast<bf16*>(p.part_ml + 2LL * p.ctas * 128);
+  p.scale = scale;
+  p.cap = cap;
+  p.status = status_ptr();
+  const TensorMap tq = get_tensor_map_bthd(p.q, B, n, QH, D, (unsigned long long)n * QH * D, (unsigned long long)QH * D, D, p.tok, 64, p.R);
+  if (!tq || !tk || !tv) return static_cast<int>(cudaErrorInvalidValue);
+  if (D == 128) {
+    if (cap > 0.f) return launch_tree<128, kTreeCap>(p, tq, tk, tv, st);
+    return slopes != nullptr ? launch_tree<128, kTreeBias>(p, tq, tk, tv, st) : launch_tree<128, kTreePlain>(p, tq, tk, tv, st);
+  }
+  if (cap > 0.f) return launch_tree<64, kTreeCap>(p, tq, tk, tv, st);
+  return slopes != nullptr ? launch_tree<64, kTreeBias>(p, tq, tk, tv, st) : launch_tree<64, kTreePlain>(p, tq, tk, tv, st);
+}

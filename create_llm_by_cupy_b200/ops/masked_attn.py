@@ -333,3 +333,111 @@ def _span_bwd_reference(dout, q, k, v, o, mask, scale, softcap, slopes, out, unr
             dst.copy_(src)
         return tuple(out)
     return res
+
+
+# --------------------------------------------------------------------------- drafted tokens over a KV cache
+def tree_mask(parents, device) -> torch.Tensor:
+    """int64 [B, n] masks for ``tree_attn_append`` from ``parents`` [B, n] (lists, or an integer tensor; read on the host):
+    the draft that each draft continues, which stands before it in its row, or -1 for the cached text. Bit j of an entry is set
+    when the draft sees draft j: its ancestors and itself. n is at most 64."""
+    rows = parents.tolist() if isinstance(parents, torch.Tensor) else parents
+    out = []
+    for row in rows:
+        if len(row) > 64:
+            raise ValueError("tree_mask: more than 64 drafts")
+        bits = []
+        for i, par in enumerate(row):
+            if not -1 <= par < i:
+                raise ValueError("tree_mask: a draft's parent stands before it")
+            bits.append((1 << i) | (bits[par] if par >= 0 else 0))
+        out.append([x - (1 << 64) if x >> 63 else x for x in bits])
+    return torch.tensor(out, dtype=torch.int64, device=device)
+
+
+def tree_attn_append(kqv, kcache, vcache, lens, tree, QH: int, KVH: int, cos, sin, *, scale: float | None = None,
+                     softcap: float = 0.0, slopes=None):
+    """Attention of ``n`` drafted tokens of each of ``B`` sequences over their KV caches. ``kqv`` [B * n, (2 KVH + QH) * D]: the packed
+    projection K | Q | V, un-rotated; ``kcache``, ``vcache`` [B, KVH, Tmax, D] (K rotated); ``lens`` int32 [B]: cached tokens;
+    ``tree`` int64 [B, n] (``tree_mask``); ``cos``, ``sin`` fp32 [>= Tmax, D / 2].
+
+    Draft i stands at position lens + its depth, sees the cached tokens and the drafts of its mask, and its K (rotated) and V
+    are appended to the caches at lens + i (one behind the end of the cache is not kept). n = 1 with mask 1 is a decoded token.
+    Returns [B, n, QH, D]. A mask of 0 leaves the cached tokens alone; with none of them the result is 0. Cache rows from
+    lens + n on may hold anything."""
+    if kcache.dim() != 4 or kcache.shape != vcache.shape or tree.dim() != 2 or kqv.dim() != 2:
+        raise ValueError("tree_attn_append: caches are [B, KV heads, Tmax, D], tree is [B, n], kqv [B * n, columns]")
+    B, n = tree.shape
+    Tmax, D = kcache.shape[2:]
+    if KVH <= 0 or QH <= 0 or QH % KVH != 0 or kcache.shape[:2] != (B, KVH) or tuple(kqv.shape) != (B * n, (2 * KVH + QH) * D):
+        raise ValueError("tree_attn_append: sizes of kqv, caches and tree do not go together")
+    if not 1 <= n <= 64 or QH // KVH > 128 or Tmax == 0:
+        raise ValueError("tree_attn_append: 1 to 64 drafts, up to 128 query heads to a KV head, caches of at least one position")
+    if tuple(lens.shape) != (B,) or lens.dtype != torch.int32 or tree.dtype != torch.int64:
+        raise ValueError("tree_attn_append: lens is int32 [B], tree int64 [B, n]")
+    if cos.shape != sin.shape or cos.dim() != 2 or cos.shape[0] < Tmax or cos.shape[1] != D // 2:
+        raise ValueError("tree_attn_append: rotary tables are [>= Tmax, D / 2]")
+    if any(t.device != kqv.device for t in (kcache, vcache, lens, tree, cos, sin)):
+        raise ValueError("tree_attn_append: all tensors are on one device")
+    _modifier("tree_attn_append", QH, softcap, slopes, kqv.device)
+    scale = _scale(scale, D)
+    if not kqv.is_cuda:
+        return _tree_reference(kqv, kcache, vcache, lens, tree, QH, KVH, cos, sin, scale, softcap, slopes)
+    F._bf16(kqv, kcache, vcache)
+    if D not in (64, 128):
+        raise ValueError("tree_attn_append: CUDA kernels exist for a head dimension of 64 or 128")
+    if cos.dtype != torch.float32 or sin.dtype != torch.float32:
+        raise TypeError("tree_attn_append: rotary tables are float32")
+    if not (kcache.is_contiguous() and vcache.is_contiguous()) or (kcache.data_ptr() | vcache.data_ptr()) % 16:
+        raise ValueError("tree_attn_append: caches are contiguous and start on a 16-byte boundary")
+    if kqv.stride(1) != 1 or (B * n > 1 and kqv.stride(0) % 8) or kqv.data_ptr() % 16:
+        kqv = kqv.clone(memory_format=torch.contiguous_format)
+    cos, sin, lens, tree = cos.contiguous(), sin.contiguous(), lens.contiguous(), tree.contiguous()
+    cos, sin = (t if t.data_ptr() % 16 == 0 else t.clone() for t in (cos, sin))
+    slopes = slopes if slopes is None else slopes.contiguous()
+    out = torch.empty((B, n, QH, D), dtype=torch.bfloat16, device=kqv.device)
+    if B == 0:
+        return out
+    lib = F._lib()
+    lib.b200_tree_attn_workspace.restype = ctypes.c_longlong
+    ws = torch.empty(lib.b200_tree_attn_workspace(B, n, QH, KVH, Tmax, D), dtype=torch.uint8, device=kqv.device)
+    native.check(lib.b200_tree_attn_append(
+        native.ptr(kqv), native.ptr(kcache), native.ptr(vcache), native.ptr(out), native.ptr(lens), native.ptr(tree), native.ptr(cos),
+        native.ptr(sin), native.ptr(slopes), native.ptr(ws), B, n, QH, KVH, Tmax, D, cos.shape[0],
+        ctypes.c_longlong(kqv.stride(0) if B * n > 1 else kqv.shape[1]), _f(scale), _f(softcap), native.stream_ptr()), "tree_attn_append")
+    native.bump(3)
+    return out
+
+
+def _tree_reference(kqv, kcache, vcache, lens, tree, QH, KVH, cos, sin, scale, softcap, slopes):
+    B, n = tree.shape
+    Tmax, D = kcache.shape[2:]
+    j = torch.arange(n, device=kqv.device)
+    sees = ((tree[:, :, None] >> j) & 1).bool()
+    depth = (sees.sum(-1) - 1).clamp_min(0)
+    lens = lens.long().clamp(0, Tmax)
+    pos = lens[:, None] + depth
+    dt = _work_dtype(kqv)
+    k, q, v = kqv.to(dt).view(B, n, -1).split([KVH * D, QH * D, KVH * D], dim=2)
+    c, s = (x.to(dt)[pos.clamp_max(x.shape[0] - 1)][:, :, None] for x in (cos, sin))
+
+    def rot(x):
+        a, b = x[..., :D // 2], x[..., D // 2:]
+        return torch.cat([a * c - b * s, b * c + a * s], -1)
+    q, k = rot(q.reshape(B, n, QH, D)), rot(k.reshape(B, n, KVH, D)).to(kcache.dtype)
+    v = v.reshape(B, n, KVH, D)
+    t = torch.arange(Tmax, device=kqv.device)
+    for b in range(B):
+        keep = min(n, Tmax - int(lens[b]))
+        at = int(lens[b])
+        kcache[b, :, at:at + keep] = k[b, :keep].transpose(0, 1)
+        vcache[b, :, at:at + keep] = v[b, :keep].transpose(0, 1).to(vcache.dtype)
+    off = t - lens[:, None]                                   # which draft a position is
+    draft = off.clamp(0, n - 1)
+    seen = (off < 0)[:, None] | (((off >= 0) & (off < n))[:, None] & torch.gather(sees, 2, draft[:, None].expand(B, n, Tmax)))
+    kpos = torch.where(off < 0, t, lens[:, None] + torch.gather(depth, 1, draft))
+    dist = (pos[:, :, None] - kpos[:, None, :]).abs()[:, None]
+    used = (off < n)[:, None, :, None]                         # rows behind the drafts may hold anything
+    kc, vc = (torch.where(used, x.to(dt), torch.zeros((), dtype=dt, device=x.device)).transpose(1, 2) for x in (kcache, vcache))
+    x, _ = _scores_reference(q, kc, seen, scale, softcap, slopes, dist)
+    p, _ = _softmax_reference(x)
+    return torch.einsum("bhts,bshd->bthd", p, vc.repeat_interleave(QH // KVH, dim=2)).to(kqv.dtype)
