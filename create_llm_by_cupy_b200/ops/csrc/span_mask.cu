@@ -14,9 +14,8 @@
 
 namespace b200 {
 
-constexpr int SM_THREADS = 1024;
+constexpr int SM_THREADS = 1024;                      // at most: as many as there are tokens for
 constexpr int SM_PER = 4;                             // tokens of a thread
-constexpr int SM_CHUNK = SM_THREADS * SM_PER;         // tokens of a pass
 constexpr int SM_MAX_TILES = 5632;                    // ranges kept in shared memory: 44 KiB, 720896 tokens
 
 struct SpanMaskParams {
@@ -35,35 +34,54 @@ struct SpanMaskParams {
 struct MaxOp {
   static constexpr int kNone = -1;
   __device__ static int of(int a, int b) { return max(a, b); }
+  __device__ static int warp(int v) { return __reduce_max_sync(0xffffffffu, v); }
 };
 struct MinOp {
   static constexpr int kNone = INT_MAX;
   __device__ static int of(int a, int b) { return min(a, b); }
+  __device__ static int warp(int v) { return __reduce_min_sync(0xffffffffu, v); }
 };
 
 // v over the threads before this one (kUp) or behind it, the carry first; `carry` leaves with the whole block in it.
 template <class Op, bool kUp>
 __device__ __forceinline__ int block_scan_excl(int v, int& carry, int* warp_v) {
-  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
   int x = v;
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = kUp ? __shfl_up_sync(0xffffffffu, x, o) : __shfl_down_sync(0xffffffffu, x, o);
     if (kUp ? lane >= o : lane + o < 32) x = Op::of(x, y);
   }
-  __syncthreads();                                    // the last scan's values have been read
-  if (lane == (kUp ? 31 : 0)) warp_v[warp] = x;
   int e = kUp ? __shfl_up_sync(0xffffffffu, x, 1) : __shfl_down_sync(0xffffffffu, x, 1);
   if (lane == (kUp ? 0 : 31)) e = Op::kNone;
+  __syncthreads();                                    // the last scan's values have been read
+  if (lane == (kUp ? 31 : 0)) warp_v[warp] = x;
   __syncthreads();
-  int before = carry, all = carry;
-  for (int w = 0; w < SM_THREADS / 32; ++w) {
-    const int y = warp_v[w];
-    if (kUp ? w < warp : w > warp) before = Op::of(before, y);
-    all = Op::of(all, y);
+  const int y = lane < warps ? warp_v[lane] : Op::kNone;
+  const int before = Op::warp((kUp ? lane < warp : lane > warp) ? y : Op::kNone);
+  const int all = Op::warp(y), out = Op::of(Op::of(carry, before), e);
+  carry = Op::of(carry, all);
+  return out;
+}
+
+// Four tokens' values from `at` on: one load where the row allows it.
+__device__ __forceinline__ void load4(const int* p, int at, int T, bool wide, int none, int (&v)[SM_PER]) {
+  if (wide && at + 3 < T) {
+    const int4 x = *reinterpret_cast<const int4*>(p + at);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    return;
   }
-  carry = all;
-  return Op::of(before, e);
+#pragma unroll
+  for (int i = 0; i < SM_PER; ++i) v[i] = at + i < T ? p[at + i] : none;
+}
+__device__ __forceinline__ void load4(const unsigned char* p, int at, int T, bool wide, int none, int (&v)[SM_PER]) {
+  if (wide && at + 3 < T) {
+    const uchar4 x = *reinterpret_cast<const uchar4*>(p + at);
+    v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < SM_PER; ++i) v[i] = at + i < T ? p[at + i] : none;
 }
 
 __device__ __forceinline__ int warp_min(int v) { return __reduce_min_sync(0xffffffffu, v); }
@@ -82,30 +100,48 @@ span_mask_kernel(const SpanMaskParams p) {
   const int* docs = p.docs ? p.docs + row0 : nullptr;
   const unsigned char* pre = p.prefix ? p.prefix + row0 : nullptr;
 
+  const int chunk = int(blockDim.x) * SM_PER;
+  const bool wide_docs = (reinterpret_cast<uintptr_t>(docs) & 15) == 0, wide_pre = (reinterpret_cast<uintptr_t>(pre) & 3) == 0;
+  // document, whether one starts here, and prefix flag of this thread's four tokens
+  auto tokens = [&](int t0, int (&id)[SM_PER], bool (&start)[SM_PER], int (&flag)[SM_PER]) {
+    int last = 0;
+    if (docs != nullptr) {
+      load4(docs, t0, T, wide_docs, 0, id);
+      if (t0 > 0 && t0 < T) last = docs[t0 - 1];
+    }
+    if (pre != nullptr) load4(pre, t0, T, wide_pre, 0, flag);
+#pragma unroll
+    for (int i = 0; i < SM_PER; ++i) {
+      if (docs == nullptr) id[i] = 0;
+      if (pre == nullptr) flag[i] = 0;
+      start[i] = t0 + i < T && (t0 + i == 0 || (docs != nullptr && id[i] != (i > 0 ? id[i - 1] : last)));
+    }
+  };
+
   // From behind: where the prefix run that a token may be part of ends (the first start or unflagged token behind it). Kept
   // in the spans' hi until the other pass has lo.
   if (pre != nullptr && p.lo_in == nullptr) {
     int carry = T;
-    for (int c0 = (T - 1) / SM_CHUNK * SM_CHUNK; c0 >= 0; c0 -= SM_CHUNK) {
+    for (int c0 = (T - 1) / chunk * chunk; c0 >= 0; c0 -= chunk) {
       const int t0 = c0 + int(threadIdx.x) * SM_PER;
-      int stop[SM_PER], v = MinOp::kNone;
+      int id[SM_PER], flag[SM_PER], stop[SM_PER], v = MinOp::kNone;
+      bool start[SM_PER];
+      tokens(t0, id, start, flag);
 #pragma unroll
       for (int i = SM_PER - 1; i >= 0; --i) {
-        const int t = t0 + i;
-        const bool here = t < T && (pre[t] == 0 || t == 0 || (docs != nullptr && docs[t] != docs[t - 1]));
-        stop[i] = v;                                  // the first stop of this thread behind t
-        if (here) v = t;
+        stop[i] = v;                                  // the first stop of this thread behind it
+        if (t0 + i < T && (flag[i] == 0 || start[i])) v = t0 + i;
       }
       const int behind = block_scan_excl<MinOp, false>(v, carry, warp_v);
 #pragma unroll
       for (int i = 0; i < SM_PER; ++i)
         if (t0 + i < T) spans[t0 + i].y = min(stop[i], behind);
     }
-    __syncthreads();
+    // (a thread reads back its own tokens' alone)
   }
 
   int carry_start = 0, carry_plain = -1;
-  for (int c0 = 0; c0 < T; c0 += SM_CHUNK) {
+  for (int c0 = 0; c0 < T; c0 += chunk) {
     const int t0 = c0 + int(threadIdx.x) * SM_PER;
     int lo[SM_PER], hi[SM_PER];
     if (p.lo_in != nullptr) {
@@ -115,14 +151,15 @@ span_mask_kernel(const SpanMaskParams p) {
         hi[i] = t0 + i < T ? p.hi_in[row0 + t0 + i] : 0;
       }
     } else {
-      int start[SM_PER], plain[SM_PER], id[SM_PER], s = -1, u = -1;
+      int start_at[SM_PER], plain[SM_PER], id[SM_PER], flag[SM_PER], s = -1, u = -1;
+      bool start[SM_PER];
+      tokens(t0, id, start, flag);
 #pragma unroll
       for (int i = 0; i < SM_PER; ++i) {
         const int t = t0 + i;
-        id[i] = t < T && docs != nullptr ? docs[t] : 0;
-        if (t < T && docs != nullptr && t > 0 && id[i] != (i > 0 ? id[i - 1] : docs[t - 1])) s = t;
-        if (t < T && pre != nullptr && pre[t] == 0) u = t;
-        start[i] = s;
+        if (start[i]) s = t;
+        if (t < T && flag[i] == 0) u = t;
+        start_at[i] = s;
         plain[i] = u;
       }
       const int s_before = block_scan_excl<MaxOp, true>(s, carry_start, warp_v);
@@ -130,7 +167,7 @@ span_mask_kernel(const SpanMaskParams p) {
 #pragma unroll
       for (int i = 0; i < SM_PER; ++i) {
         const int t = t0 + i;
-        lo[i] = max(start[i], s_before);
+        lo[i] = max(start_at[i], s_before);
         hi[i] = t + 1;
         if (pre != nullptr && t < T && max(plain[i], u_before) < lo[i]) hi[i] = spans[t].y;
         if (id[i] < 0 || t >= vlen) hi[i] = 0;
@@ -167,7 +204,7 @@ span_mask_kernel(const SpanMaskParams p) {
     }
   }
   __syncthreads();
-  for (int n = threadIdx.x; n < p.nt; n += SM_THREADS) {
+  for (int n = threadIdx.x; n < p.nt; n += blockDim.x) {
     int first = INT_MAX, end = 0;
     for (int m = 0; m < p.nt; ++m) {
       const int2 r = s_range[m];
@@ -202,5 +239,6 @@ B200_API int b200_span_mask(const void* docs, const void* prefix, const void* va
   p.ktab = static_cast<int2*>(ktab);
   p.B = B; p.T = T; p.nt = nt;
   p.status = status_ptr();
-  return static_cast<int>(launch_pdl(span_mask_kernel, dim3(B), dim3(SM_THREADS), size_t(nt) * sizeof(int2), st, 0, p));
+  const int threads = nt * 32 < SM_THREADS ? nt * 32 : SM_THREADS;             // a warp to a tile
+  return static_cast<int>(launch_pdl(span_mask_kernel, dim3(B), dim3(threads), size_t(nt) * sizeof(int2), st, 0, p));
 }

@@ -518,57 +518,71 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   }
 }
 
-// Joins the pieces of every (sequence, KV head, row tile) that was cut: grid (those, 4), 32 rows a CTA, a warp a row at a time.
+// Joins the pieces of every (sequence, KV head, row tile) that was cut: grid (those, 16), a warp a row, its pieces' sums in the
+// order of the keys. A lane looks a piece up, so that no load waits for a division.
 template <int kD>
 __global__ void __launch_bounds__(256)
 tree_join_kernel(const TreeParams p) {
+  constexpr int kV = kD / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
   const int per = p.KVH * p.row_tiles, b = blockIdx.x / per, idx = blockIdx.x % per, kvh = idx / p.row_tiles, rt = idx % p.row_tiles;
-  const int live = min(p.n - rt * p.tok, p.tok) * p.R, row0 = blockIdx.y * 32;
-  if (row0 >= live) return;
-  long long sum = 0, before = 0;
+  const int live = min(p.n - rt * p.tok, p.tok) * p.R, r = blockIdx.y * 8 + warp;
+  if (r >= live) return;
+  unsigned long long sum = 0, before = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int v = b0 + lane < p.B ? tree_tiles(tree_len(p, b0 + lane)) : 0;
     sum += __reduce_add_sync(0xffffffffu, v);
     before += __reduce_add_sync(0xffffffffu, b0 + lane < b ? v : 0);
   }
-  const int nt = tree_tiles(tree_len(p, b));
-  const long long total = sum * per, t0 = before * per + (long long)idx * nt, G = p.ctas;
+  const unsigned nt = tree_tiles(tree_len(p, b));
+  const unsigned long long total = sum * per, t0 = before * per + (unsigned long long)idx * nt, G = p.ctas;
   // tile t is in the piece of CTA ((t + 1) G - 1) / total
-  const long long c0 = ((t0 + 1) * G - 1) / total, c1 = ((t0 + nt) * G - 1) / total;
+  const int c0 = int(((t0 + 1) * G - 1) / total), c1 = int(((t0 + nt) * G - 1) / total);
   if (c0 == c1) return;
-  for (int r = row0 + warp; r < min(row0 + 32, live); r += 8) {
-    constexpr int kV = kD / 32;
-    float mx = -INFINITY;
-    for (long long c = c0 + lane; c <= c1; c += 32) {
-      if (c * total / G == (c + 1) * total / G) continue;
-      const long long slot = 2 * c + (c == c0 && c * total / G < t0 ? 1 : 0);
-      mx = fmaxf(mx, p.part_ml[slot * 128 + r].x);
-    }
+  // the piece of CTA c: its slot, or -1 where the CTA has no tile at all
+  auto slot_of = [&](int c) {
+    if (c > c1) return -1;
+    const unsigned long long from = c * total / G;
+    return from == (c + 1) * total / G ? -1 : (2 * c + (from < t0 ? 1 : 0)) * 128 + r;
+  };
+  float m = -INFINITY, l = 0.f, acc[kV];                 // the maximum so far; this lane's pieces of the sum
+#pragma unroll
+  for (int e = 0; e < kV; ++e) acc[e] = 0.f;
+  for (int c = c0; c <= c1; c += 32) {
+    const int slot = slot_of(c + lane);
+    const float2 ml = slot >= 0 ? p.part_ml[slot] : make_float2(-INFINITY, 0.f);
+    float mx = ml.x;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    const float ref = mx == -INFINITY ? 0.f : mx;
-    float l = 0.f, acc[kV];
+    mx = fmaxf(mx, m);
+    const float ref = mx == -INFINITY ? 0.f : mx, corr = exp2f(m - ref), f = exp2f(ml.x - ref);
+    m = mx;
+    l = l * corr + ml.y * f;
 #pragma unroll
-    for (int e = 0; e < kV; ++e) acc[e] = 0.f;
-    for (long long c = c0; c <= c1; ++c) {
-      if (c * total / G == (c + 1) * total / G) continue;
-      const long long slot = (2 * c + (c == c0 && c * total / G < t0 ? 1 : 0)) * 128 + r;
-      const float2 ml = p.part_ml[slot];
-      const float f = exp2f(ml.x - ref);
-      l += ml.y * f;
-      const float* o = p.part_o + slot * kD + lane * kV;
+    for (int e = 0; e < kV; ++e) acc[e] *= corr;
+    const int count = min(32, c1 - c + 1);
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) {
+      const int si = __shfl_sync(0xffffffffu, slot, i);
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      if (si < 0) continue;
+      const float* o = p.part_o + size_t(si) * kD + lane * kV;
+      float v[kV];
+      if constexpr (kV == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(o);
+      else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(o);
 #pragma unroll
-      for (int e = 0; e < kV; ++e) acc[e] += o[e] * f;
+      for (int e = 0; e < kV; ++e) acc[e] += v[e] * fi;
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
-    const int d = rt * p.tok + r / p.R, h = kvh * p.R + r % p.R;
-    bf16* out = p.out + ((size_t(b) * p.n + d) * p.QH + h) * kD + lane * kV;
-#pragma unroll
-    for (int e = 0; e < kV; e += 2) *reinterpret_cast<bf162*>(out + e) = __floats2bfloat162_rn(acc[e] * inv, acc[e + 1] * inv);
   }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int d = rt * p.tok + r / p.R, h = kvh * p.R + r % p.R;
+  bf16* out = p.out + ((size_t(b) * p.n + d) * p.QH + h) * kD + lane * kV;
+#pragma unroll
+  for (int e = 0; e < kV; e += 2) *reinterpret_cast<bf162*>(out + e) = __floats2bfloat162_rn(acc[e] * inv, acc[e + 1] * inv);
 }
 
 template <int kD, int kMod>
@@ -581,7 +595,7 @@ static int launch_tree(const TreeParams& p, const TensorMap& tq, const TensorMap
   const long long chunks = (long long)p.B * p.n * (p.QH + 2 * p.KVH) * (kD / 8);
   B200_CHECK(launch_pdl(tree_append_kernel<kD>, dim3(unsigned((chunks + 255) / 256)), dim3(256), 0, st, 0, p));
   B200_CHECK(launch_pdl(tree_attn_kernel<kD, kMod>, dim3(p.ctas), dim3(TA_THREADS), TA<kD>::kSmem, st, 0, *tq, *tk, *tv, p));
-  return static_cast<int>(launch_pdl(tree_join_kernel<kD>, dim3(p.B * p.KVH * p.row_tiles, 4), dim3(256), 0, st, 0, p));
+  return static_cast<int>(launch_pdl(tree_join_kernel<kD>, dim3(p.B * p.KVH * p.row_tiles, (p.tok * p.R + 7) / 8), dim3(256), 0, st, 0, p));
 }
 
 static int tree_row_tiles(int n, int R) { return (n + 128 / R - 1) / (128 / R); }
