@@ -30,6 +30,7 @@
 #include "common.cuh"
 #include "ptx.cuh"
 #include "flash_rope_epilogue.cuh"
+#include "score_cap.cuh"
 
 namespace b200 {
 
@@ -60,7 +61,7 @@ struct FlashBwdTcParams {
   // spans (flash_bwd_dkv_wide_kernel with kMod >= 0; see span_mask.cu)
   const int2* spans;     // [B, T]
   const int2* ktab;      // [B, n_tiles]
-  float cap;             // kCap
+  ScoreCap cap;          // kCap
   const float* slopes;   // kBias: [QH]
 };
 
@@ -814,10 +815,10 @@ __device__ __forceinline__ void fb_p_chunk(uint32_t (&rs)[16], uint32_t (&pk)[8]
 }
 
 // The same under spans: `see` holds the keys of the tile that each of the 16 queries sees, krow is this thread's key in it.
-// A cap leaves P (1 - tanh^2) in place of P in rs, which is what dS is made from: x = c tanh(s / c) = c - 2 c r with
-// r = 1 / (1 + exp(2 s / c)), and 1 - tanh^2 = 4 r (1 - r). A bias: dist = first query's position minus the key's.
+// Capped scores come in rs as they leave the cap; P (1 - tanh^2) replaces P there, which is what dS is made from. A bias: dist =
+// first query's position minus the key's.
 template <bool kMask, int kMod>
-__device__ __forceinline__ void fb_p_chunk_span(uint32_t (&rs)[16], uint32_t (&pk)[8], float kc, float c2, const float* lse2,
+__device__ __forceinline__ void fb_p_chunk_span(uint32_t (&rs)[16], uint32_t (&pk)[8], float sl2, float inv_c2, const float* lse2,
                                                 const uint32_t* see, uint32_t krow, float slope2, float dist) {
 #pragma unroll
   for (int e = 0; e < 16; e += 4) {
@@ -830,20 +831,16 @@ __device__ __forceinline__ void fb_p_chunk_span(uint32_t (&rs)[16], uint32_t (&p
 #pragma unroll
     for (int u = 0; u < 4; ++u) {
       const float x = __uint_as_float(rs[e + u]);
-      float pe, r = 0.f;
-      if constexpr (kMod == kCap) {
-        r = __fdividef(1.f, 1.f + exp2f(x * kc));
-        pe = exp2f(fmaf(-2.f * c2, r, c2 - lv[u]));
-      } else if constexpr (kMod == kBias) {
-        pe = exp2f(fmaf(x, kc, fmaf(-slope2, fabsf(dist + float(e + u)), -lv[u])));
-      } else {
-        pe = exp2f(fmaf(x, kc, -lv[u]));
-      }
+      float pe;
+      if constexpr (kMod == kCap) pe = exp2f(x - lv[u]);
+      else if constexpr (kMod == kBias) pe = exp2f(fmaf(x, sl2, fmaf(-slope2, fabsf(dist + float(e + u)), -lv[u])));
+      else pe = exp2f(fmaf(x, sl2, -lv[u]));
       if (kMask) {
         if (krow - (sv[u] & 0xffu) >= (sv[u] >> 8)) pe = 0.f;
       }
       pv[u] = pe;
-      rs[e + u] = __float_as_uint(kMod == kCap ? pe * (4.f * fmaf(-r, r, r)) : pe);
+      const float th = x * inv_c2;
+      rs[e + u] = __float_as_uint(kMod == kCap ? fmaf(-th * th, pe, pe) : pe);
     }
 #pragma unroll
     for (int u = 0; u < 4; u += 2) {
@@ -1155,7 +1152,6 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
     const int half = wg;                      // dK / dV columns this warpgroup stores at the end of a pass
     const uint32_t lane_sel = uint32_t(q * 32) << 16;
     const float sl2 = p.scale * kFbLog2e;
-    const float kc = kMod == kCap ? 2.f * kFbLog2e * p.scale / p.cap : sl2, c2 = kMod == kCap ? p.cap * kFbLog2e : 0.f;
     uint8_t* stg_row = smem + Smem::kStage + wg * FKV_STG + (q * 32 + lane) * 128;
     const uint32_t swz = uint32_t(lane & 7);
     const bool ds_on = p.ds != nullptr;
@@ -1194,6 +1190,7 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
         tmem_ld_32x32b_x32(tS, *reinterpret_cast<uint32_t(*)[32]>(&sc[0]));
         tmem_ld_32x32b_x32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&sc[32]));
         tmem_ld_wait();
+        if constexpr (kMod == kCap) cap_scores(sc, p.cap);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t(&rs)[16] = *reinterpret_cast<uint32_t(*)[16]>(&sc[16 * c]);
@@ -1203,8 +1200,8 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
           } else {
             const float dist = float(qb + c * 16 - key);
             if (need_mask)
-              fb_p_chunk_span<true, kMod>(rs, pk[c], kc, c2, st + c * 16, see + (wg * 64 + c * 16) / 2, uint32_t(key - n0), slope_now, dist);
-            else fb_p_chunk_span<false, kMod>(rs, pk[c], kc, c2, st + c * 16, see, 0u, slope_now, dist);
+              fb_p_chunk_span<true, kMod>(rs, pk[c], sl2, p.cap.inv_c2, st + c * 16, see + (wg * 64 + c * 16) / 2, uint32_t(key - n0), slope_now, dist);
+            else fb_p_chunk_span<false, kMod>(rs, pk[c], sl2, p.cap.inv_c2, st + c * 16, see, 0u, slope_now, dist);
           }
           tmem_st_32x32b_x8(tS + c * 8, pk[c]);
           if (kMod == kCap && kD == 128) fb_pack16(&sc[16 * c], pk[c]);      // kept for dS: P (1 - tanh^2)
@@ -1513,7 +1510,7 @@ B200_API int b200_flash_bwd_span(const void* q, const void* k, const void* v, co
   p.unrot_ld = unrot_ld;
   p.spans = static_cast<const int2*>(spans);
   p.ktab = static_cast<const int2*>(ktab);
-  p.cap = cap;
+  p.cap = make_score_cap(scale, cap);
   p.slopes = static_cast<const float*>(slopes);
   {
     const int bc = int(80.0e6 / (2.0 * T * D * (2.0 * QH + 2.0 * KVH)));       // as in b200_flash_bwd_tc

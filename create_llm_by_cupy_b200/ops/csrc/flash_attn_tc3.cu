@@ -34,6 +34,7 @@
 // Q / K / V / O tile instead of two, four k-steps in S = Q K^T and N = 64 in O += P V.
 #include "common.cuh"
 #include "ptx.cuh"
+#include "score_cap.cuh"
 
 namespace b200 {
 
@@ -51,7 +52,7 @@ struct Flash3Params {
   const int2* spans;     // [B, T]
   const int4* qtab;      // [B, n_tiles]
   int n_tiles;
-  float cap;             // kCap
+  ScoreCap cap;          // kCap
   const float* slopes;   // kBias: [QH]
 };
 
@@ -136,12 +137,6 @@ __device__ __forceinline__ float f3_row_max_span(uint32_t (&sc)[128], int key0, 
     mx[(e >> 1) & 3] = f3_max3(mx[(e >> 1) & 3], __uint_as_float(sc[e]), __uint_as_float(sc[e + 1]));
   }
   return fmaxf(f3_max3(mx[0], mx[1], mx[2]), mx[3]);
-}
-
-// c tanh(s / c) in log2 units: c tanh(y) = c - 2 c / (1 + exp(2 y)); kc = 2 log2(e) scale / c, c2 = c log2(e). Far out the
-// exponential is 0 or infinite and the result -c or c.
-__device__ __forceinline__ float f3_capped(float s, float kc, float c2) {
-  return fmaf(-2.f * c2, __fdividef(1.f, 1.f + exp2f(s * kc)), c2);
 }
 
 // P = exp2(s * sl2 - m_ref) for scores [kLo, kHi) of one row, packed to bf16 pairs IN PLACE (pair e / 2 lands in
@@ -396,7 +391,6 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const uint32_t tP = tmem_base + lane_sel + kColP + w * 128;
     // log2 units per score; a cap or a bias leaves them in log2 units
     const float sl2 = kMod == kCap || kMod == kBias ? 1.f : p.scale * kF3Log2e;
-    const float kc = kMod == kCap ? 2.f * kF3Log2e * p.scale / p.cap : p.scale * kF3Log2e, c2 = kMod == kCap ? p.cap * kF3Log2e : 0.f;
     float m_ref = 0.f, l_run = 0.f;          // reference maximum (log2 units) and the row sum relative to it
     bool ok = true;
     for (int j = 0; j < my_tiles && ok; ++j) {
@@ -421,12 +415,11 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         mx = (need_mask ? f3_row_max<true>(sc, key0, row, vlen) : f3_row_max<false>(sc, key0, row, vlen)) * sl2;
       } else {
         if constexpr (kMod == kCap) {
-#pragma unroll
-          for (int e = 0; e < 128; ++e) sc[e] = __float_as_uint(f3_capped(__uint_as_float(sc[e]), kc, c2));
+          cap_scores(sc, p.cap);
         } else if constexpr (kMod == kBias) {
           const float dist = float(key0 - row);
 #pragma unroll
-          for (int e = 0; e < 128; ++e) sc[e] = __float_as_uint(fmaf(__uint_as_float(sc[e]), kc, -slope2 * fabsf(dist + float(e))));
+          for (int e = 0; e < 128; ++e) sc[e] = __float_as_uint(fmaf(__uint_as_float(sc[e]), p.scale * kF3Log2e, -slope2 * fabsf(dist + float(e))));
         }
         mx = (need_mask ? f3_row_max_span<true>(sc, key0, span.x, span.y) : f3_row_max_span<false>(sc, key0, 0, 0)) * sl2;
       }
@@ -612,7 +605,7 @@ B200_API int b200_flash_fwd_span(const void* q, const void* k, const void* v, vo
   p.spans = static_cast<const int2*>(spans);
   p.qtab = static_cast<const int4*>(qtab);
   p.n_tiles = (T + 127) / 128;
-  p.cap = cap;
+  p.cap = make_score_cap(scale, cap);
   p.slopes = static_cast<const float*>(slopes);
   if (cap > 0.f) return launch_flash_fwd<kCap>(q, k, v, o, strides, KVH, D, p, st);
   if (slopes != nullptr) return launch_flash_fwd<kBias>(q, k, v, o, strides, KVH, D, p, st);

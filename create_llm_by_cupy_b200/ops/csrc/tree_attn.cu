@@ -20,6 +20,7 @@
 
 #include "common.cuh"
 #include "ptx.cuh"
+#include "score_cap.cuh"
 
 namespace b200 {
 
@@ -46,7 +47,8 @@ struct TreeParams {
   long long ld;
   int R, tok, row_tiles;    // query heads of a KV head; drafts of a row tile (R tok <= 128); row tiles of a sequence and KV head
   int ctas;                 // pieces of the list
-  float scale, cap;
+  float scale;
+  ScoreCap cap;             // kTreeCap
   int* status;
 };
 
@@ -354,7 +356,6 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     const uint32_t lane_sel = uint32_t(q * 32) << 16;
     const uint32_t tS = tmem_base + lane_sel + L::kColS, tO = tmem_base + lane_sel + L::kColO, tP = tmem_base + lane_sel + L::kColP;
     const float sl2 = kMod == kTreePlain ? p.scale * kTaLog2e : 1.f;
-    const float kc = kMod == kTreeCap ? 2.f * kTaLog2e * p.scale / p.cap : p.scale * kTaLog2e, c2 = kMod == kTreeCap ? p.cap * kTaLog2e : 0.f;
     const long long first = (long long)blockIdx.x;
     int g = 0, seg = 0;
     bool ok = true;
@@ -391,15 +392,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         float rs0 = 0.f, rs1 = 0.f;
         if (work) {
           if constexpr (kMod == kTreeCap) {
-#pragma unroll
-            for (int e = 0; e < 128; ++e)
-              sc[e] = __float_as_uint(fmaf(-2.f * c2, __fdividef(1.f, 1.f + exp2f(__uint_as_float(sc[e]) * kc)), c2));
+            cap_scores(sc, p.cap);
           } else if constexpr (kMod == kTreeBias) {
             const float dist = pos - float(t * 128);
 #pragma unroll
             for (int e = 0; e < 128; ++e) {
               const float far = drafts ? fabsf(pos - float(s.len + s_depth[e & 63])) : fabsf(dist - float(e));
-              sc[e] = __float_as_uint(fmaf(__uint_as_float(sc[e]), kc, -slope2 * far));
+              sc[e] = __float_as_uint(fmaf(__uint_as_float(sc[e]), p.scale * kTaLog2e, -slope2 * far));
             }
           }
           if (drafts) {
@@ -654,7 +653,7 @@ B200_API int b200_tree_attn_append(const void* kqv, void* kc, void* vc, void* ou
   p.part_ml = reinterpret_cast<float2*>(p.part_o + 2LL * p.ctas * 128 * D);
   p.q = reinterpret_cast<bf16*>(p.part_ml + 2LL * p.ctas * 128);
   p.scale = scale;
-  p.cap = cap;
+  p.cap = make_score_cap(scale, cap);
   p.status = status_ptr();
   const TensorMap tq = get_tensor_map_bthd(p.q, B, n, QH, D, (unsigned long long)n * QH * D, (unsigned long long)QH * D, D, p.tok, 64, p.R);
   if (!tq || !tk || !tv) return static_cast<int>(cudaErrorInvalidValue);
