@@ -21,6 +21,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdint>
 #include <limits>
 #include <optional>
@@ -51,6 +52,15 @@ struct Api {
   int (*decode_attn_block)(cptr, cptr, cptr, cptr, void*, void*, void*, void*, void*, cptr, cptr, cptr, int, int, int, int,
                            int, int, int, int, int, float, stream_t);
   int (*mlp_few_rows)(cptr, cptr, cptr, cptr, void*, void*, int, int, int, int, int, stream_t);
+  int (*span_mask)(cptr, cptr, cptr, cptr, cptr, void*, void*, void*, int, int, stream_t);
+  int (*flash_fwd_span)(cptr, cptr, cptr, void*, void*, cptr, cptr, const long long*, int, int, int, int, int, float, float, cptr,
+                        stream_t);
+  int (*flash_delta)(cptr, cptr, void*, const long long*, int, int, int, int, stream_t);
+  int (*flash_bwd_span)(cptr, cptr, cptr, cptr, cptr, cptr, void*, void*, void*, cptr, cptr, cptr, const long long*, int, int, int, int,
+                        int, float, float, cptr, void*, cptr, cptr, int, stream_t);
+  long long (*tree_attn_workspace)(int, int, int, int, int, int);
+  int (*tree_attn_append)(cptr, void*, void*, void*, cptr, cptr, cptr, cptr, cptr, void*, int, int, int, int, int, int, int, long long,
+                          float, float, stream_t);
 };
 Api api;
 
@@ -442,6 +452,183 @@ PyObject* mlp_few_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END
 }
 
+// The tables of a span mask in its buffer (see ``masked_attn._make_mask``): of query tiles, of key tiles, the spans themselves.
+struct SpanTables {
+  int* qtab;
+  int* ktab;
+  int* spans;
+};
+SpanTables span_tables(const Tensor& buf, int64_t B, int64_t T) {
+  int* p = static_cast<int*>(const_cast<void*>(buf.const_data_ptr()));
+  const int64_t nt = (T + 127) / 128;
+  return {p, p + 4 * B * nt, p + 6 * B * nt};
+}
+int64_t span_ints(int64_t B, int64_t T) { return B * (6 * ((T + 127) / 128) + 2 * T); }
+
+// span_mask(B, T, docs or None, prefix or None, valid_len or None) -> the mask's buffer
+PyObject* span_mask(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  ARGS(5)
+  const int64_t B = as_int(a[0]), T = as_int(a[1]);
+  const Tensor *docs, *prefix, *vl;
+  CHECK_NUMBERS
+  if (!optional(a[2], &docs) || !optional(a[3], &prefix) || !optional(a[4], &vl) || B <= 0 || T <= 0 || T > 720896) Py_RETURN_NONE;
+  const Tensor* like = docs ? docs : prefix ? prefix : vl;
+  if (!like) Py_RETURN_NONE;
+  auto rows = [&](const Tensor* t, at::ScalarType dt) {
+    return !t || (on(*t, dev) && t->scalar_type() == dt && t->dim() == 2 && t->size(0) == B && t->size(1) == T && t->is_contiguous());
+  };
+  if (!rows(docs, at::kInt) || !rows(prefix, at::kBool)) Py_RETURN_NONE;
+  if (vl && (!on(*vl, dev) || vl->scalar_type() != at::kInt || vl->dim() != 1 || vl->size(0) != B || !vl->is_contiguous())) Py_RETURN_NONE;
+  Tensor buf = empty({span_ints(B, T)}, *like, at::kInt);
+  const SpanTables t = span_tables(buf, B, T);
+  if (launched([&] {
+        return api.span_mask(docs ? docs->const_data_ptr() : nullptr, prefix ? prefix->const_data_ptr() : nullptr,
+                             vl ? vl->const_data_ptr() : nullptr, nullptr, nullptr, t.spans, t.qtab, t.ktab, int(B), int(T), stream(dev));
+      }))
+    return wrap(buf);
+  END
+}
+
+// q like k, v [B, T, heads, D], in rows that tiles can be copied from, with the mask of B x T tokens
+bool span_heads(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& buf, int64_t mB, int64_t mT, const Tensor* slopes,
+                int dev) {
+  for (const Tensor* t : {&q, &k, &v})
+    if (!bf16_on(*t, dev) || t->dim() != 4 || t->stride(3) != 1 || !aligned16(t->const_data_ptr())) return false;
+  const int64_t B = q.size(0), T = q.size(1), QH = q.size(2), D = q.size(3), KVH = k.size(2);
+  if (k.sizes() != v.sizes() || k.size(0) != B || k.size(1) != T || k.size(3) != D || !fits(B) || !fits(T) || !fits(QH) || !fits(KVH) ||
+      QH % KVH != 0 || (D != 64 && D != 128) || mB != B || mT != T)
+    return false;
+  for (const Tensor* t : {&q, &k, &v})
+    for (int d = 0; d < 3; ++d)
+      if (t->size(d) > 1 && (t->stride(d) % 8 != 0 || t->stride(d) <= 0)) return false;
+  if (slopes && (!on(*slopes, dev) || slopes->scalar_type() != at::kFloat || slopes->dim() != 1 || slopes->size(0) != QH ||
+                 !slopes->is_contiguous()))
+    return false;
+  return on(buf, dev) && buf.scalar_type() == at::kInt && buf.is_contiguous() && buf.numel() == span_ints(B, T);
+}
+// (batch, token, head) strides; of a dimension of one, which is never stepped along, one that a tile copy can have
+void put_strides(long long* st, std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    for (int d = 0; d < 3; ++d) *st++ = t->size(d) > 1 ? t->stride(d) : 8;
+}
+// Scale (0: of the head dimension) and cap as the front ends take them; the others are theirs to refuse.
+bool score_numbers(float* scale, float cap, const Tensor* slopes, int64_t D) {
+  if (*scale == 0.f) *scale = float(1.0 / std::sqrt(double(D)));
+  return *scale > 0.f && *scale < INFINITY && cap >= 0.f && cap < INFINITY && !(cap > 0.f && slopes);
+}
+
+// span_fwd(q, k, v, mask buffer, B, T, scale, softcap, slopes or None) -> (o, lse)
+PyObject* span_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  ARGS(9)
+  const Tensor *q = plain(a[0]), *k = plain(a[1]), *v = plain(a[2]), *buf = plain(a[3]), *sl;
+  const int64_t mB = as_int(a[4]), mT = as_int(a[5]);
+  float scale = as_float(a[6]);
+  const float cap = as_float(a[7]);
+  CHECK_NUMBERS
+  if (!q || !k || !v || !buf || !optional(a[8], &sl) || !span_heads(*q, *k, *v, *buf, mB, mT, sl, dev)) Py_RETURN_NONE;
+  const int64_t B = q->size(0), T = q->size(1), QH = q->size(2), D = q->size(3), KVH = k->size(2);
+  if (!score_numbers(&scale, cap, sl, D)) Py_RETURN_NONE;
+  Tensor o = empty({B, T, QH, D}, *q, at::kBFloat16), lse = empty({B, QH, T}, *q, at::kFloat);
+  long long st[12];
+  put_strides(st, {q, k, v, &o});
+  const SpanTables t = span_tables(*buf, B, T);
+  if (launched([&] {
+        return api.flash_fwd_span(q->const_data_ptr(), k->const_data_ptr(), v->const_data_ptr(), o.mutable_data_ptr(),
+                                  lse.mutable_data_ptr(), t.spans, t.qtab, st, int(B), int(T), int(QH), int(KVH), int(D), scale, cap,
+                                  sl ? sl->const_data_ptr() : nullptr, stream(dev));
+      }))
+    return wrap2(o, lse);
+  END
+}
+
+// span_bwd(dout, q, k, v, o, lse, mask buffer, B, T, scale, softcap, slopes or None, most bytes of dS^T) -> (dq, dk, dv); where dS^T
+// of the whole batch is no more than that
+PyObject* span_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  ARGS(13)
+  const Tensor *dout = plain(a[0]), *q = plain(a[1]), *k = plain(a[2]), *v = plain(a[3]), *o = plain(a[4]), *lse = plain(a[5]),
+               *buf = plain(a[6]), *sl;
+  const int64_t mB = as_int(a[7]), mT = as_int(a[8]);
+  float scale = as_float(a[9]);
+  const float cap = as_float(a[10]);
+  const long long most = PyLong_Check(a[12]) ? PyLong_AsLongLong(a[12]) : 0;
+  CHECK_NUMBERS
+  if (!dout || !q || !k || !v || !o || !lse || !buf || !optional(a[11], &sl) || !span_heads(*q, *k, *v, *buf, mB, mT, sl, dev))
+    Py_RETURN_NONE;
+  const int64_t B = q->size(0), T = q->size(1), QH = q->size(2), D = q->size(3), KVH = k->size(2), Tp = (T + 127) / 128 * 128;
+  const double ds = 2.0 * double(B) * double(QH) * double(Tp) * double(Tp);
+  if (!score_numbers(&scale, cap, sl, D) || ds > double(most)) Py_RETURN_NONE;
+  for (const Tensor* t : {dout, o}) {
+    if (!bf16_on(*t, dev) || t->sizes() != q->sizes() || t->stride(3) != 1 || !aligned16(t->const_data_ptr())) Py_RETURN_NONE;
+    for (int d = 0; d < 3; ++d)
+      if (t->size(d) > 1 && (t->stride(d) % 8 != 0 || t->stride(d) <= 0)) Py_RETURN_NONE;
+  }
+  if (!on(*lse, dev) || lse->scalar_type() != at::kFloat || !lse->is_contiguous() || lse->sizes() != at::IntArrayRef({B, QH, T}))
+    Py_RETURN_NONE;
+  Tensor dq = empty({B, T, QH, D}, *q, at::kBFloat16), dk = empty({B, T, KVH, D}, *q, at::kBFloat16),
+         dv = empty({B, T, KVH, D}, *q, at::kBFloat16), delta = empty({B, QH, T}, *q, at::kFloat),
+         ws = empty({B * QH * Tp * Tp}, *q, at::kBFloat16);
+  long long st6[6], st[21];
+  put_strides(st6, {o, dout});
+  put_strides(st, {q, k, v, dout, &dq, &dk, &dv});
+  const SpanTables t = span_tables(*buf, B, T);
+  if (!launched([&] {
+        const int rc = api.flash_delta(o->const_data_ptr(), dout->const_data_ptr(), delta.mutable_data_ptr(), st6, int(B), int(T), int(QH),
+                                       int(D), stream(dev));
+        if (rc != 0) return rc;
+        return api.flash_bwd_span(q->const_data_ptr(), k->const_data_ptr(), v->const_data_ptr(), dout->const_data_ptr(),
+                                  lse->const_data_ptr(), delta.const_data_ptr(), dq.mutable_data_ptr(), dk.mutable_data_ptr(),
+                                  dv.mutable_data_ptr(), t.spans, t.qtab, t.ktab, st, int(B), int(T), int(QH), int(KVH), int(D), scale, cap,
+                                  sl ? sl->const_data_ptr() : nullptr, ws.mutable_data_ptr(), nullptr, nullptr, 0, stream(dev));
+      }))
+    Py_RETURN_NONE;
+  PyObject* r = PyTuple_New(3);
+  if (r == nullptr) return nullptr;
+  PyTuple_SET_ITEM(r, 0, wrap(dq));
+  PyTuple_SET_ITEM(r, 1, wrap(dk));
+  PyTuple_SET_ITEM(r, 2, wrap(dv));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
+// tree_attn(kqv, kcache, vcache, lens, tree, QH, KVH, cos, sin, scale, softcap, slopes or None) -> out
+PyObject* tree_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  ARGS(12)
+  const Tensor *x = plain(a[0]), *kc = plain(a[1]), *vc = plain(a[2]), *lens = plain(a[3]), *tree = plain(a[4]), *c = plain(a[7]),
+               *s = plain(a[8]), *sl;
+  const int QH = as_int(a[5]), KVH = as_int(a[6]);
+  float scale = as_float(a[9]);
+  const float cap = as_float(a[10]);
+  CHECK_NUMBERS
+  if (!x || !kc || !vc || !lens || !tree || !c || !s || !optional(a[11], &sl) || !tma_rows(*x, dev)) Py_RETURN_NONE;
+  if (!bf16_on(*kc, dev) || !bf16_on(*vc, dev) || kc->dim() != 4 || kc->sizes() != vc->sizes() || !kc->is_contiguous() ||
+      !vc->is_contiguous() || !aligned16(kc->const_data_ptr()) || !aligned16(vc->const_data_ptr()))
+    Py_RETURN_NONE;
+  if (!on(*tree, dev) || tree->scalar_type() != at::kLong || tree->dim() != 2 || !tree->is_contiguous()) Py_RETURN_NONE;
+  const int64_t B = tree->size(0), nd = tree->size(1), Tmax = kc->size(2), D = kc->size(3);
+  if (!on(*lens, dev) || lens->scalar_type() != at::kInt || lens->dim() != 1 || lens->size(0) != B || !lens->is_contiguous()) Py_RETURN_NONE;
+  if (QH <= 0 || KVH <= 0 || QH % KVH != 0 || (D != 64 && D != 128) || kc->size(0) != B || kc->size(1) != KVH || !fits(B) || !fits(Tmax) ||
+      nd < 1 || nd > 64 || x->size(0) != B * nd || x->size(1) != (2 * int64_t(KVH) + QH) * D)
+    Py_RETURN_NONE;
+  for (const Tensor* t : {c, s})
+    if (!on(*t, dev) || t->scalar_type() != at::kFloat || t->dim() != 2 || !t->is_contiguous() || t->sizes() != c->sizes() ||
+        t->size(0) < Tmax || t->size(1) != D / 2 || !aligned16(t->const_data_ptr()))
+      Py_RETURN_NONE;
+  if (sl && (!on(*sl, dev) || sl->scalar_type() != at::kFloat || sl->dim() != 1 || sl->size(0) != QH || !sl->is_contiguous()))
+    Py_RETURN_NONE;
+  if (!score_numbers(&scale, cap, sl, D)) Py_RETURN_NONE;
+  const long long bytes = api.tree_attn_workspace(int(B), int(nd), QH, KVH, int(Tmax), int(D));
+  if (bytes <= 0) Py_RETURN_NONE;
+  Tensor out = empty({B, nd, QH, D}, *x, at::kBFloat16), ws = empty({bytes}, *x, at::kByte);
+  if (launched([&] {
+        return api.tree_attn_append(x->const_data_ptr(), kc->mutable_data_ptr(), vc->mutable_data_ptr(), out.mutable_data_ptr(),
+                                    lens->const_data_ptr(), tree->const_data_ptr(), c->const_data_ptr(), s->const_data_ptr(),
+                                    sl ? sl->const_data_ptr() : nullptr, ws.mutable_data_ptr(), int(B), int(nd), QH, KVH, int(Tmax), int(D),
+                                    int(c->size(0)), x->stride(0), scale, cap, stream(dev));
+      }))
+    return wrap(out);
+  END
+}
+
 // memory_room(device index, bytes of the device) -> see ``native.memory_room``
 PyObject* memory_room(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -479,6 +666,12 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   get(api.flash_fwd_tc3, "b200_flash_fwd_tc3");
   get(api.decode_attn_block, "b200_decode_attn_block");
   get(api.mlp_few_rows, "b200_mlp_few_rows");
+  get(api.span_mask, "b200_span_mask");
+  get(api.flash_fwd_span, "b200_flash_fwd_span");
+  get(api.flash_delta, "b200_flash_delta");
+  get(api.flash_bwd_span, "b200_flash_bwd_span");
+  get(api.tree_attn_workspace, "b200_tree_attn_workspace");
+  get(api.tree_attn_append, "b200_tree_attn_append");
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -494,7 +687,8 @@ PyObject* device_ready(PyObject*, PyObject* const* a, Py_ssize_t n) {
 #define METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void*>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {METHOD(bind), METHOD(device_ready), METHOD(memory_room), METHOD(rmsnorm_fwd), METHOD(rmsnorm_bwd),
                          METHOD(embedding_fwd), METHOD(gemm), METHOD(tma_ok), METHOD(gemm_rope), METHOD(gemm_swiglu),
-                         METHOD(flash_fwd), METHOD(split_heads), METHOD(decode_attn_block), METHOD(mlp_few_rows), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(flash_fwd), METHOD(split_heads), METHOD(decode_attn_block), METHOD(mlp_few_rows),
+                         METHOD(span_mask), METHOD(span_fwd), METHOD(span_bwd), METHOD(tree_attn), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_b200host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

@@ -392,8 +392,10 @@ __global__ void __launch_bounds__(256) flash_delta_vec_kernel(const FlashParams 
   constexpr int RPW = 32 / LPR;                      // rows per warp and step
   const int lane = threadIdx.x & 31;
   const int sub = lane / LPR, li = lane % LPR;
+  pdl_wait();
+  pdl_trigger();
   // Rows of one batch element (blockIdx.y), heads fastest: 32-bit division. With 64-bit row numbers over the whole batch the divisions
-  // were the kernel: 4 x 2048 tokens, 16 heads of 128, 45 us; like this @DELTA@.
+  // were the kernel: 4 x 2048 tokens, 16 heads of 128, 45 us; like this 22.
   const int total = p.QH * p.T, b = blockIdx.y;
   const int warp0 = int((blockIdx.x * blockDim.x + threadIdx.x) >> 5), nwarps = int((gridDim.x * blockDim.x) >> 5);
   for (int r0 = warp0 * RPW * U; r0 < total; r0 += nwarps * RPW * U) {
@@ -428,7 +430,8 @@ __global__ void __launch_bounds__(256) flash_delta_vec_kernel(const FlashParams 
   }
 }
 
-static bool launch_delta_vec(const FlashParams& p, int D, cudaStream_t st) {
+// False where it does not apply; an error of the launch in *rc.
+static bool launch_delta_vec(const FlashParams& p, int D, cudaStream_t st, int* rc) {
   const long long strides[6] = {p.o_bs, p.o_ts, p.o_hs, p.do_bs, p.do_ts, p.do_hs};
   for (long long v : strides)
     if (v % 8 != 0) return false;
@@ -442,9 +445,9 @@ static bool launch_delta_vec(const FlashParams& p, int D, cudaStream_t st) {
     const long long cap = ((long long)num_sms() * 8 + p.B - 1) / p.B;
     return dim3(unsigned(blocks < cap ? (blocks < 1 ? 1 : blocks) : cap), unsigned(p.B));
   };
-  if (D == 128) flash_delta_vec_kernel<16, U><<<grid_for_rows(2), 256, 0, st>>>(p);
-  else if (D == 64) flash_delta_vec_kernel<8, U><<<grid_for_rows(4), 256, 0, st>>>(p);
-  else if (D == 32) flash_delta_vec_kernel<4, U><<<grid_for_rows(8), 256, 0, st>>>(p);
+  if (D == 128) *rc = launch_pdl(flash_delta_vec_kernel<16, U>, grid_for_rows(2), dim3(256), 0, st, 0, p);
+  else if (D == 64) *rc = launch_pdl(flash_delta_vec_kernel<8, U>, grid_for_rows(4), dim3(256), 0, st, 0, p);
+  else if (D == 32) *rc = launch_pdl(flash_delta_vec_kernel<4, U>, grid_for_rows(8), dim3(256), 0, st, 0, p);
   else return false;
   return true;
 }
@@ -753,10 +756,12 @@ static int launch_fwd(const FlashParams& p, bool rope, cudaStream_t st) {
 
 template <int D>
 static int launch_bwd(const FlashParams& p, bool rope, cudaStream_t st) {
-  if (!launch_delta_vec(p, D, st)) {
+  int rc = 0;
+  if (!launch_delta_vec(p, D, st, &rc)) {
     const int total_warps = p.B * p.QH * p.T;
     flash_delta_kernel<<<(total_warps + 7) / 8, 256, 0, st>>>(p, D);
   }
+  if (rc != 0) return rc;
   const int smem_kv = (2 * FB_BN + 2 * FB_BM) * D * 2 + 2 * FB_BM * 4;
   const int smem_q = (2 * FA_BM + 2 * FA_BN) * D * 2;
   dim3 grid_kv((p.T + FB_BN - 1) / FB_BN, p.KVH, p.B);
@@ -865,9 +870,9 @@ B200_API int b200_flash_delta(const void* o, const void* dout, void* delta, cons
   p.o_bs = strides[0]; p.o_ts = strides[1]; p.o_hs = strides[2];
   p.do_bs = strides[3]; p.do_ts = strides[4]; p.do_hs = strides[5];
   p.B = B; p.T = T; p.QH = QH;
-  if (!launch_delta_vec(p, D, st)) {
-    const int total_warps = B * QH * T;
-    flash_delta_kernel<<<(total_warps + 7) / 8, 256, 0, st>>>(p, D);
-  }
+  int rc = 0;
+  if (launch_delta_vec(p, D, st, &rc)) return rc;
+  const int total_warps = B * QH * T;
+  flash_delta_kernel<<<(total_warps + 7) / 8, 256, 0, st>>>(p, D);
   return static_cast<int>(cudaGetLastError());
 }

@@ -26,6 +26,7 @@
 //
 // Reference counterpart: cupy_flash_gqa_backward (model/flash_attention.py:109-176).
 #include <mutex>
+#include <type_traits>
 
 #include "common.cuh"
 #include "ptx.cuh"
@@ -815,37 +816,49 @@ __device__ __forceinline__ void fb_p_chunk(uint32_t (&rs)[16], uint32_t (&pk)[8]
 }
 
 // The same under spans: `see` holds the keys of the tile that each of the 16 queries sees, krow is this thread's key in it.
-// Capped scores come in rs as they leave the cap; P (1 - tanh^2) replaces P there, which is what dS is made from. A bias: dist =
-// first query's position minus the key's.
-template <bool kMask, int kMod>
-__device__ __forceinline__ void fb_p_chunk_span(uint32_t (&rs)[16], uint32_t (&pk)[8], float sl2, float inv_c2, const float* lse2,
+// minus_lse2 points at the 16 per-query values. A cap leaves P (1 - tanh^2) in place of P in rs, which is what dS is made from
+// (kTier: see score_cap.cuh). A bias: dist = first query's position minus the key's.
+template <bool kMask, int kMod, int kTier = 0>
+__device__ __forceinline__ void fb_p_chunk_span(uint32_t (&rs)[16], uint32_t (&pk)[8], float sl2, const ScoreCap& cap, const float* minus_lse2,
                                                 const uint32_t* see, uint32_t krow, float slope2, float dist) {
 #pragma unroll
   for (int e = 0; e < 16; e += 4) {
-    const float4 l4 = *reinterpret_cast<const float4*>(lse2 + e);
-    const float lv[4] = {l4.x, l4.y, l4.z, l4.w};
+    const float4 l4 = *reinterpret_cast<const float4*>(minus_lse2 + e);
+    const float ml[4] = {l4.x, l4.y, l4.z, l4.w};
     uint2 w = make_uint2(0u, 0u);
     if (kMask) w = *reinterpret_cast<const uint2*>(see + e / 2);
     const uint32_t sv[4] = {w.x & 0xffffu, w.x >> 16, w.y & 0xffffu, w.y >> 16};
-    float pv[4];
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-      const float x = __uint_as_float(rs[e + u]);
-      float pe;
-      if constexpr (kMod == kCap) pe = exp2f(x - lv[u]);
-      else if constexpr (kMod == kBias) pe = exp2f(fmaf(x, sl2, fmaf(-slope2, fabsf(dist + float(e + u)), -lv[u])));
-      else pe = exp2f(fmaf(x, sl2, -lv[u]));
-      if (kMask) {
-        if (krow - (sv[u] & 0xffu) >= (sv[u] >> 8)) pe = 0.f;
-      }
-      pv[u] = pe;
-      const float th = x * inv_c2;
-      rs[e + u] = __float_as_uint(kMod == kCap ? fmaf(-th * th, pe, pe) : pe);
-    }
 #pragma unroll
     for (int u = 0; u < 4; u += 2) {
-      const bf162 t0 = __floats2bfloat162_rn(pv[u], pv[u + 1]);
+      const float x0 = __uint_as_float(rs[e + u]), x1 = __uint_as_float(rs[e + u + 1]);
+      float2 a, capped;
+      if constexpr (kMod == kCap) {
+        if constexpr (kTier == kCapAny) {
+          capped = make_float2(cap_any(x0, cap), cap_any(x1, cap));
+        } else {
+          const uint64_t x = pair_of(x0, x1);
+          capped = unpair(mul2(x, cap_factor<kTier>(x, cap)));
+        }
+        a = unpair(add2(pair_of(capped), pair_of(ml[u], ml[u + 1])));
+      } else if constexpr (kMod == kBias) {
+        a = make_float2(fmaf(x0, sl2, fmaf(-slope2, fabsf(dist + float(e + u)), ml[u])),
+                        fmaf(x1, sl2, fmaf(-slope2, fabsf(dist + float(e + u + 1)), ml[u + 1])));
+      } else {
+        a = make_float2(fmaf(x0, sl2, ml[u]), fmaf(x1, sl2, ml[u + 1]));
+      }
+      float2 pe = make_float2(exp2f(a.x), exp2f(a.y));
+      if (kMask) {
+        if (krow - (sv[u] & 0xffu) >= (sv[u] >> 8)) pe.x = 0.f;
+        if (krow - (sv[u + 1] & 0xffu) >= (sv[u + 1] >> 8)) pe.y = 0.f;
+      }
+      const bf162 t0 = __floats2bfloat162_rn(pe.x, pe.y);
       pk[(e + u) >> 1] = *reinterpret_cast<const uint32_t*>(&t0);
+      if constexpr (kMod == kCap) {
+        const uint64_t c = pair_of(capped);
+        pe = unpair(mul2(pair_of(pe), fma2(mul2(c, c), pair_of(cap.minus_inv2), pair_of(1.f, 1.f))));
+      }
+      rs[e + u] = __float_as_uint(pe.x);
+      rs[e + u + 1] = __float_as_uint(pe.y);
     }
   }
 }
@@ -1039,7 +1052,8 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
 #pragma unroll
         for (int j = 0; j < FKW_BQ / 32; ++j) {
           const int r = lane + 32 * j;
-          st[r] = (m0 + r < T) ? lv[j] * kFbLog2e : INFINITY;       // +inf => P = 0 for rows past T
+          const float l2 = (m0 + r < T) ? lv[j] * kFbLog2e : INFINITY;       // +inf => P = 0 for rows past T
+          st[r] = kMod == kCausal ? l2 : -l2;
           st[FKW_BQ + r] = (m0 + r < T) ? dv[j] * p.scale : 0.f;
         }
         mbar_arrive(&st_full[s]);
@@ -1190,7 +1204,8 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
         tmem_ld_32x32b_x32(tS, *reinterpret_cast<uint32_t(*)[32]>(&sc[0]));
         tmem_ld_32x32b_x32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&sc[32]));
         tmem_ld_wait();
-        if constexpr (kMod == kCap) cap_scores(sc, p.cap);
+        int tier = 0;
+        if constexpr (kMod == kCap) tier = cap_tier(sc, p.cap);
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           uint32_t(&rs)[16] = *reinterpret_cast<uint32_t(*)[16]>(&sc[16 * c]);
@@ -1199,9 +1214,20 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
             else fb_p_chunk<false>(rs, pk[c], sl2, st + c * 16, 0, 0, false);
           } else {
             const float dist = float(qb + c * 16 - key);
-            if (need_mask)
-              fb_p_chunk_span<true, kMod>(rs, pk[c], sl2, p.cap.inv_c2, st + c * 16, see + (wg * 64 + c * 16) / 2, uint32_t(key - n0), slope_now, dist);
-            else fb_p_chunk_span<false, kMod>(rs, pk[c], sl2, p.cap.inv_c2, st + c * 16, see, 0u, slope_now, dist);
+            const uint32_t* see_c = see + (wg * 64 + c * 16) / 2;
+            auto chunk = [&](auto mask, auto t) {
+              fb_p_chunk_span<decltype(mask)::value, kMod, decltype(t)::value>(rs, pk[c], sl2, p.cap, st + c * 16, see_c, uint32_t(key - n0),
+                                                                               slope_now, dist);
+            };
+            using True = std::true_type;
+            if (kMod == kCap && tier != kCapNear) {
+              if (tier == kCapMid) chunk(True{}, std::integral_constant<int, kCapMid>{});
+              else chunk(True{}, std::integral_constant<int, kCapAny>{});
+            } else if (need_mask) {
+              chunk(True{}, std::integral_constant<int, kCapNear>{});
+            } else {
+              chunk(std::false_type{}, std::integral_constant<int, kCapNear>{});
+            }
           }
           tmem_st_32x32b_x8(tS + c * 8, pk[c]);
           if (kMod == kCap && kD == 128) fb_pack16(&sc[16 * c], pk[c]);      // kept for dS: P (1 - tanh^2)

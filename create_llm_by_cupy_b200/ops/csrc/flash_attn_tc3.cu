@@ -389,7 +389,7 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const uint32_t tS = tmem_base + lane_sel + kColS + w * 128;
     const uint32_t tO = tmem_base + lane_sel + kColO + w * 128;
     const uint32_t tP = tmem_base + lane_sel + kColP + w * 128;
-    // log2 units per score; a cap or a bias leaves them in log2 units
+    // log2 units per score; a bias leaves them in log2 units, a cap is taken on the way into the exponentials
     const float sl2 = kMod == kCap || kMod == kBias ? 1.f : p.scale * kF3Log2e;
     float m_ref = 0.f, l_run = 0.f;          // reference maximum (log2 units) and the row sum relative to it
     bool ok = true;
@@ -411,17 +411,22 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         mbar_arrive(&early[w]);
       }
       float mx;
+      bool cap_now = false;              // kCap: the exponentials take the cap
       if constexpr (kMod == kCausal) {
         mx = (need_mask ? f3_row_max<true>(sc, key0, row, vlen) : f3_row_max<false>(sc, key0, row, vlen)) * sl2;
       } else {
         if constexpr (kMod == kCap) {
-          cap_scores(sc, p.cap);
-        } else if constexpr (kMod == kBias) {
+          const int tier = cap_tier(sc, p.cap);
+          cap_now = tier == kCapNear && !need_mask;
+          if (!cap_now) cap_scores(sc, p.cap, tier);
+        }
+        if constexpr (kMod == kBias) {
           const float dist = float(key0 - row);
 #pragma unroll
           for (int e = 0; e < 128; ++e) sc[e] = __float_as_uint(fmaf(__uint_as_float(sc[e]), p.scale * kF3Log2e, -slope2 * fabsf(dist + float(e))));
         }
         mx = (need_mask ? f3_row_max_span<true>(sc, key0, span.x, span.y) : f3_row_max_span<false>(sc, key0, 0, 0)) * sl2;
+        if (kMod == kCap && cap_now) mx = cap_any(mx, p.cap);          // the cap keeps the order of the scores
       }
       // The reference maximum is set by the first tile and afterwards moves only when a tile exceeds it by
       // more than 2^8; then O_w and the row sum are rescaled by the row's own thread.
@@ -456,18 +461,21 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       float rs0 = 0.f, rs1 = 0.f;
       const float m_sub = kMod != kCausal && m_ref == -INFINITY ? 0.f : m_ref;      // nothing seen yet: exp2(-inf) is 0
       if (kOwnP) {
-        f3_row_p<0, 128>(sc, sl2, m_sub, rs0, rs1);
+        if (kMod == kCap && cap_now) cap_row_p<0, 128>(sc, p.cap, m_sub, rs0, rs1);
+        else f3_row_p<0, 128>(sc, sl2, m_sub, rs0, rs1);
         if (j > 0 && !mbar_wait(&pv_done[w], (j - 1) & 1, abort_flag)) { ok = false; break; }   // P_w has been read
         tc_fence_after();
       } else {
         // head_dim 128: the next scores wait for this P V, so its first half is handed over early
-        f3_row_p<0, 64>(sc, sl2, m_sub, rs0, rs1);
+        if (kMod == kCap && cap_now) cap_row_p<0, 64>(sc, p.cap, m_sub, rs0, rs1);
+        else f3_row_p<0, 64>(sc, sl2, m_sub, rs0, rs1);
         tmem_st_32x32b_x16(tP, *reinterpret_cast<const uint32_t(*)[16]>(&sc[0]));
         tmem_st_32x32b_x16(tP + 16, *reinterpret_cast<const uint32_t(*)[16]>(&sc[16]));
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&early[w]);
-        f3_row_p<64, 128>(sc, sl2, m_sub, rs0, rs1);
+        if (kMod == kCap && cap_now) cap_row_p<64, 128>(sc, p.cap, m_sub, rs0, rs1);
+        else f3_row_p<64, 128>(sc, sl2, m_sub, rs0, rs1);
       }
 #pragma unroll
       for (int c = kOwnP ? 0 : 2; c < 4; ++c)

@@ -391,9 +391,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         mbar_arrive(s_read);
         float rs0 = 0.f, rs1 = 0.f;
         if (work) {
+          bool cap_now = false;                          // the exponentials take the cap
           if constexpr (kMod == kTreeCap) {
-            cap_scores(sc, p.cap);
-          } else if constexpr (kMod == kTreeBias) {
+            const int tier = cap_tier(sc, p.cap);
+            cap_now = tier == kCapNear && rem >= 128;
+            if (!cap_now) cap_scores(sc, p.cap, tier);
+          }
+          if constexpr (kMod == kTreeBias) {
             const float dist = pos - float(t * 128);
 #pragma unroll
             for (int e = 0; e < 128; ++e) {
@@ -413,7 +417,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
           for (int e = 0; e < 128; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(sc[e]));
-          const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
+          float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
+          if (kMod == kTreeCap && cap_now) mx = cap_any(mx, p.cap);      // the cap keeps the order of the scores
           // the reference maximum moves when a tile exceeds it by more than 2^8, as in the attention forward
           const bool need = mx > m_ref + kTaRescaleStep;
           if (t == s.t0) {
@@ -436,13 +441,17 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
             if (need) m_ref = mx;
           }
           const float m_sub = m_ref == -INFINITY ? 0.f : m_ref;
+          if (kMod == kTreeCap && cap_now) {
+            cap_row_p<0, 128>(sc, p.cap, m_sub, rs0, rs1);
+          } else {
 #pragma unroll
-          for (int e = 0; e < 128; e += 2) {
-            const float p0 = exp2f(fmaf(__uint_as_float(sc[e]), sl2, -m_sub)), p1 = exp2f(fmaf(__uint_as_float(sc[e + 1]), sl2, -m_sub));
-            rs0 += p0;
-            rs1 += p1;
-            const bf162 x = __floats2bfloat162_rn(p0, p1);
-            sc[e >> 1] = *reinterpret_cast<const uint32_t*>(&x);
+            for (int e = 0; e < 128; e += 2) {
+              const float p0 = exp2f(fmaf(__uint_as_float(sc[e]), sl2, -m_sub)), p1 = exp2f(fmaf(__uint_as_float(sc[e + 1]), sl2, -m_sub));
+              rs0 += p0;
+              rs1 += p1;
+              const bf162 x = __floats2bfloat162_rn(p0, p1);
+              sc[e >> 1] = *reinterpret_cast<const uint32_t*>(&x);
+            }
           }
         }
         // P of the tile before has been read

@@ -35,13 +35,26 @@ class SpanMask:
     """Which keys each query of a [B, T] batch sees: positions [lo, hi) per query, and (CUDA) the tables of tiles of 128 tokens
     that the kernels walk by. Made by ``span_mask`` or ``SpanMask.from_spans``; one serves any number of layers and heads."""
 
-    def __init__(self, spans, qtab, ktab):
-        self.spans, self.qtab, self.ktab = spans, qtab, ktab        # int32 [B, T, 2]; CUDA: [B, nt, 4], [B, nt, 2]
-        self.B, self.T = spans.shape[0], spans.shape[1]
+    def __init__(self, buf: torch.Tensor, B: int, T: int):
+        # CUDA: [B, nt, 4] key tiles of every query tile, [B, nt, 2] query tiles of every key tile, then the spans [B, T, 2] (lo, hi);
+        # the tables, whose entries are the wider ones, first. CPU: the spans alone.
+        self.buf, self.B, self.T = buf, B, T
 
     @property
     def device(self):
-        return self.spans.device
+        return self.buf.device
+
+    @property
+    def spans(self) -> torch.Tensor:
+        """int32 [B, T, 2]: lo, hi."""
+        n = self.B * self.T * 2
+        return self.buf[self.buf.numel() - n:].view(self.B, self.T, 2)
+
+    def _ptrs(self, b0: int = 0):
+        """Addresses of spans, query-tile and key-tile table from batch element ``b0`` on (CUDA)."""
+        nt, p = (self.T + 127) // 128, self.buf.data_ptr()
+        return (native.c_void_p(p + 4 * (6 * self.B * nt + 2 * b0 * self.T)), native.c_void_p(p + 16 * b0 * nt),
+                native.c_void_p(p + 4 * (4 * self.B * nt + 2 * b0 * nt)))
 
     @classmethod
     def from_spans(cls, lo: torch.Tensor, hi: torch.Tensor) -> "SpanMask":
@@ -50,16 +63,10 @@ class SpanMask:
             raise ValueError("SpanMask.from_spans: lo and hi are int32 [B, T] on one device")
         return _make_mask(*lo.shape, lo.device, lo=lo.contiguous(), hi=hi.contiguous())
 
-    def rows(self, b0: int, b1: int) -> "SpanMask":
-        """The mask of batch elements [b0, b1), on the same memory."""
-        if self.qtab is None:
-            return SpanMask(self.spans[b0:b1], None, None)
-        return SpanMask(self.spans[b0:b1], self.qtab[b0:b1], self.ktab[b0:b1])
-
     def dense(self) -> torch.Tensor:
         """bool [B, T, T]: query t (second) sees key s (third). For verification and small sizes."""
-        s = torch.arange(self.T, device=self.device)
-        return (s >= self.spans[..., :1]) & (s < self.spans[..., 1:])
+        s, spans = torch.arange(self.T, device=self.device), self.spans
+        return (s >= spans[..., :1]) & (s < spans[..., 1:])
 
 
 def _make_mask(B, T, device, docs=None, prefix=None, valid_len=None, lo=None, hi=None) -> SpanMask:
@@ -68,18 +75,13 @@ def _make_mask(B, T, device, docs=None, prefix=None, valid_len=None, lo=None, hi
             lo, hi = _spans_reference(B, T, docs, prefix, valid_len)
         lo, hi = lo.clamp_min(0), hi.clamp_max(T)
         none = hi <= lo
-        return SpanMask(torch.stack([lo.masked_fill(none, 0), hi.masked_fill(none, 0)], -1).to(torch.int32), None, None)
+        return SpanMask(torch.stack([lo.masked_fill(none, 0), hi.masked_fill(none, 0)], -1).to(torch.int32).reshape(-1), B, T)
     nt = (T + 127) // 128
-    # the tables, whose entries are the wider ones, first
-    buf = torch.empty(B * (6 * nt + 2 * T), dtype=torch.int32, device=device)
-    qtab = buf[:4 * B * nt].view(B, nt, 4)
-    ktab = buf[4 * B * nt:6 * B * nt].view(B, nt, 2)
-    spans = buf[6 * B * nt:].view(B, T, 2)
+    mask = SpanMask(torch.empty(B * (6 * nt + 2 * T), dtype=torch.int32, device=device), B, T)
     native.check(F._lib().b200_span_mask(native.ptr(docs), native.ptr(prefix), native.ptr(valid_len), native.ptr(lo), native.ptr(hi),
-                                         native.ptr(spans), native.ptr(qtab), native.ptr(ktab), B, T, native.stream_ptr()),
-                 "span_mask")
+                                         *mask._ptrs(), B, T, native.stream_ptr()), "span_mask")
     native.bump()
-    return SpanMask(spans, qtab, ktab)
+    return mask
 
 
 def _spans_reference(B, T, docs, prefix, valid_len):
@@ -105,6 +107,11 @@ def span_mask(B: int, T: int, device, docs=None, prefix=None, valid_len=None) ->
     starts the next one, a negative one is padding, which sees nothing and is not seen. ``prefix`` bool [B, T]: a document's leading
     flagged tokens see one another whichever comes first; every other token sees its document up to itself. ``valid_len``
     int32 [B]: tokens from there on are padding too. Without any of them: plain causal rows."""
+    if native.host is not None:
+        buf = native.host.span_mask(B, T, docs, prefix, valid_len)
+        if buf is not None and (buf.device == device or torch.device(device).type == "cuda"):
+            native.bump()
+            return SpanMask(buf, B, T)
     if B < 0 or T < 0:
         raise ValueError("span_mask: negative size")
     for name, x, dt, shape in (("docs", docs, torch.int32, (B, T)), ("prefix", prefix, torch.bool, (B, T)),
@@ -205,6 +212,11 @@ def span_attn_fwd(q, k, v, mask: SpanMask, *, scale: float | None = None, softca
 
     Keys and values that no query of a 128-token tile sees are not read; of those that are, all have to be finite: one that is
     masked for a single query still goes through the tensor core with weight 0."""
+    if native.host is not None and type(mask) is SpanMask:
+        r = native.host.span_fwd(q, k, v, mask.buf, mask.B, mask.T, 0.0 if scale is None else scale or -1.0, softcap, slopes)
+        if r is not None:
+            native.bump()
+            return r
     _heads("span_attn_fwd", q, k, v)
     _check_mask("span_attn_fwd", mask, q)
     B, T, QH, D = q.shape
@@ -223,7 +235,7 @@ def span_attn_fwd(q, k, v, mask: SpanMask, *, scale: float | None = None, softca
     arr = (ctypes.c_longlong * 12)(*_strides3(q), *_strides3(k), *_strides3(v), *_strides3(o))
     slopes = slopes if slopes is None else slopes.contiguous()
     native.check(F._lib().b200_flash_fwd_span(native.ptr(q), native.ptr(k), native.ptr(v), native.ptr(o), native.ptr(lse),
-                                              native.ptr(mask.spans), native.ptr(mask.qtab), arr, B, T, QH, KVH, D, _f(scale),
+                                              *mask._ptrs()[:2], arr, B, T, QH, KVH, D, _f(scale),
                                               _f(softcap), native.ptr(slopes), native.stream_ptr()), "flash_fwd_span")
     native.bump()
     return o, lse
@@ -235,6 +247,12 @@ def span_attn_bwd(dout, q, k, v, o, lse, mask: SpanMask, *, scale: float | None 
     write into; ``unrotate`` = (cos, sin) tables [>= T, D / 2]: dq and dk leave as gradients of the un-rotated q and k. The
     kernels keep dS^T of as many batch elements or KV heads at a time as ``functional.FLASH_DQ_GEMM_MAX_BYTES`` holds, of one KV
     head at least. Deterministic: no atomics."""
+    if native.host is not None and type(mask) is SpanMask and out is None and unrotate is None:
+        r = native.host.span_bwd(dout, q, k, v, o, lse, mask.buf, mask.B, mask.T, 0.0 if scale is None else scale or -1.0, softcap, slopes,
+                                 F.FLASH_DQ_GEMM_MAX_BYTES)
+        if r is not None:
+            native.bump(3)
+            return r
     _heads("span_attn_bwd", q, k, v)
     _check_mask("span_attn_bwd", mask, q)
     B, T, QH, D = q.shape
@@ -295,10 +313,8 @@ def span_attn_bwd(dout, q, k, v, o, lse, mask: SpanMask, *, scale: float | None 
 
         def rows(t):
             return native.ptr(t[b0:b1, g0 * R:g1 * R])     # contiguous: head slices only come with one batch element
-        m = mask.rows(b0, b1)
         native.check(F._lib().b200_flash_bwd_span(
-            qs(q), ks(k), ks(v), qs(dout), rows(lse), rows(delta), qs(dq), ks(dk), ks(dv), native.ptr(m.spans), native.ptr(m.qtab),
-            native.ptr(m.ktab), arr, b1 - b0, T, (g1 - g0) * R, g1 - g0, D, _f(scale), _f(softcap),
+            qs(q), ks(k), ks(v), qs(dout), rows(lse), rows(delta), qs(dq), ks(dk), ks(dv), *mask._ptrs(b0), arr, b1 - b0, T, (g1 - g0) * R, g1 - g0, D, _f(scale), _f(softcap),
             native.ptr(slopes if slopes is None else slopes[g0 * R:g1 * R]), native.ptr(ws), native.ptr(ucos), native.ptr(usin), uld,
             native.stream_ptr()), "flash_bwd_span")
     native.bump(2 * len(chunks))
@@ -364,6 +380,12 @@ def tree_attn_append(kqv, kcache, vcache, lens, tree, QH: int, KVH: int, cos, si
     are appended to the caches at lens + i (one behind the end of the cache is not kept). n = 1 with mask 1 is a decoded token.
     Returns [B, n, QH, D]. A mask of 0 leaves the cached tokens alone; with none of them the result is 0. Cache rows from
     lens + n on may hold anything."""
+    if native.host is not None:
+        out = native.host.tree_attn(kqv, kcache, vcache, lens, tree, QH, KVH, cos, sin, 0.0 if scale is None else scale or -1.0, softcap,
+                                    slopes)
+        if out is not None:
+            native.bump(3)
+            return out
     if kcache.dim() != 4 or kcache.shape != vcache.shape or tree.dim() != 2 or kqv.dim() != 2:
         raise ValueError("tree_attn_append: caches are [B, KV heads, Tmax, D], tree is [B, n], kqv [B * n, columns]")
     B, n = tree.shape
