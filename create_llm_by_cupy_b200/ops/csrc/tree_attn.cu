@@ -8,14 +8,19 @@
 //
 // The rows of a tile are the drafts times the query heads that share a KV head: every key is read once for all of them, which is
 // all that bounds the kernel while there are few (64 rows of head_dim 128 do 64 multiply-adds per byte read). The work is one
-// list of 128-key tiles, over sequences, KV heads and groups of 128 rows, the drafts a tile of their own behind each
-// sequence's cached ones; the list is cut into as many equal pieces as there are CTAs, so sequences of any mix of lengths keep all
-// SMs busy. A piece that is not all of its rows' keys leaves its maximum, sum and values in a workspace, and a second kernel
+// list of 128-key tiles, over sequences, KV heads and groups of up to 256 rows, the drafts a tile of their own behind each
+// sequence's cached ones; the list is cut into as many equal pieces as there are SMs, so sequences of any mix of lengths keep all
+// of them busy. A piece that is not all of its rows' keys leaves its maximum, sum and values in a workspace, and a last kernel
 // joins them in the order of the keys.
 //
 // Roles: warp 0 streams Q and the tiles of K and V by TMA, warp 1 issues the products (scores Q K^T into tensor memory, O += P V
-// from it), warps 2..5 do the softmax, a row per thread. Cached rows
-// past the length, which may hold anything, are masked as scores and cleared as values. Every wait is bounded (see ptx.cuh).
+// from it), and two warpgroups do the softmax, a row per thread, each with scores and an output of its own in tensor memory
+// (columns S_0, S_1, O_0, O_1; P lies over S). A group of more than 128 rows gives each warpgroup a tile of rows; one of up to 128
+// gives them the odd and the even key tiles, and the first one adds up what the two have. Either way the tensor core works for one
+// while the other is in its exponentials: with one warpgroup a tile took 2.1 us at 128 rows of head_dim 128 where its 64 KiB
+// arrive in 1.5.
+// Cached rows past the length, which may hold anything, are masked as scores and cleared as values. Every wait is bounded (see
+// ptx.cuh).
 #include <algorithm>
 
 #include "common.cuh"
@@ -26,7 +31,7 @@ namespace b200 {
 
 constexpr float kTaLog2e = 1.4426950408889634f;
 constexpr float kTaRescaleStep = 8.f;
-constexpr int TA_THREADS = 192;
+constexpr int TA_THREADS = 320;
 constexpr int TA_MAX_DRAFTS = 64;                        // the bits of a draft's mask
 constexpr int kTreePlain = 0, kTreeCap = 1, kTreeBias = 2;
 
@@ -41,11 +46,11 @@ struct TreeParams {
   const float* cosr;        // [rows, D / 2]
   const float* sinr;
   const float* slopes;      // kTreeBias: [QH]
-  float* part_o;            // [2 * CTAs][128][D]
-  float2* part_ml;          // [2 * CTAs][128]: maximum (log2 units), sum
+  float* part_o;            // [2 * CTAs][2][128][D]: a CTA's first and last piece, row tile in the group
+  float2* part_ml;          // [2 * CTAs][2][128]: maximum (log2 units), sum
   int B, n, QH, KVH, Tmax, table_rows;
   long long ld;
-  int R, tok, row_tiles;    // query heads of a KV head; drafts of a row tile (R tok <= 128); row tiles of a sequence and KV head
+  int R, tok, groups;       // query heads of a KV head; drafts of a row tile (R tok <= 128); groups of two row tiles (or one)
   int ctas;                 // pieces of the list
   float scale;
   ScoreCap cap;             // kTreeCap
@@ -55,20 +60,20 @@ struct TreeParams {
 template <int kD>
 struct TA {
   static constexpr int kTile = 128 * kD * 2;
-  static constexpr int kStages = 3;
-  static constexpr int kCtas = kD == 128 ? 1 : 2;
-  static constexpr int kQ = 0, kK = kTile, kV = kK + kStages * kTile;
-  static constexpr int kBar = kV + kStages * kTile;
-  // k_full, k_empty, v_full, v_empty [3]; q_full, q_empty, s_full, s_read, p_full, pv_done, o_free
-  static constexpr int kBars = 4 * kStages + 7;
-  static constexpr int kSmem = kBar + kBars * 8 + 64 + 1024;
-  static constexpr int kCols = kD == 128 ? 512 : 256;
-  static constexpr uint32_t kColS = 0, kColO = 128, kColP = 128 + kD;
+  static constexpr int kStK = kD == 128 ? 2 : 4, kStV = kD == 128 ? 3 : 4;      // rings of K and V
+  static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + kStK * kTile;
+  static constexpr int kBar = kV + kStV * kTile;
+  // k_full, k_empty [kStK]; v_full, v_empty [kStV]; q_full, q_empty; s_full, p_half, p_full, pv_done, o_free [2]; ml_full, ml_empty
+  static constexpr int kBars = 2 * kStK + 2 * kStV + 2 + 10 + 2;
+  static constexpr int kMl = kBar + kBars * 8 + 48;
+  static constexpr int kSmem = kMl + 128 * 8 + 1024;
+  static constexpr uint32_t kColS = 0, kColO = 256;                             // [2] each, 128 columns apart
 };
 
-// A stretch of one (sequence, KV head, row tile): tiles [t0, t1) of its nt, the last of which are the drafts.
+// A stretch of one (sequence, KV head, row group): tiles [t0, t1) of its nt, the last of which are the drafts.
 struct TreeSeg {
-  int b, kvh, rt, t0, t1, nt, len;
+  int b, kvh, rg, t0, t1, nt, len;
+  bool pair;                // two row tiles
 };
 
 __device__ __forceinline__ int tree_len(const TreeParams& p, int b) { return checked_index(p.lens[b], p.Tmax, p.status, 350); }
@@ -77,7 +82,7 @@ __device__ __forceinline__ int tree_tiles(int len) { return (len + 127) / 128 + 
 // The list position `at` as (sequence, first list position of it), and the list's length; by a whole warp.
 __device__ __forceinline__ void tree_find(const TreeParams& p, long long num, long long den, int lane, long long& total, long long& at,
                                           int& b_at, long long& b_first) {
-  const int per = p.KVH * p.row_tiles;
+  const int per = p.KVH * p.groups;
   long long sum = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int b = b0 + lane;
@@ -102,21 +107,22 @@ __device__ __forceinline__ void tree_find(const TreeParams& p, long long num, lo
 // Walks the pieces of one CTA.
 struct TreeWalk {
   long long left;           // tiles that are left to it
-  int b, idx, tile;         // where it stands: sequence, KV head * row tiles + row tile, tile
+  int b, idx, tile;         // where it stands: sequence, KV head * groups + group, tile
   __device__ __forceinline__ bool next(const TreeParams& p, TreeSeg& s) {
     if (left <= 0) return false;
     s.b = b;
     s.len = tree_len(p, b);
     s.nt = tree_tiles(s.len);
-    s.kvh = idx / p.row_tiles;
-    s.rt = idx % p.row_tiles;
+    s.kvh = idx / p.groups;
+    s.rg = idx % p.groups;
+    s.pair = p.n > (2 * s.rg + 1) * p.tok;
     s.t0 = tile;
     s.t1 = int(min((long long)s.nt, tile + left));
     left -= s.t1 - s.t0;
     tile = s.t1;
     if (tile == s.nt) {
       tile = 0;
-      if (++idx == p.KVH * p.row_tiles) {
+      if (++idx == p.KVH * p.groups) {
         idx = 0;
         ++b;
       }
@@ -195,55 +201,61 @@ __device__ __forceinline__ uint4* ta_chunk(uint8_t* tile, int r, int c) {
   return reinterpret_cast<uint4*>(tile + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-__device__ __forceinline__ void ta_bar_sync(int id, int threads) { asm volatile("bar.sync %0, %1;" ::"r"(id), "r"(threads) : "memory"); }
-
 template <int kD, int kMod>
-__global__ void __launch_bounds__(TA_THREADS, TA<kD>::kCtas)
+__global__ void __launch_bounds__(TA_THREADS, 1)
 tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                  const TreeParams p) {
   using L = TA<kD>;
-  constexpr int kSt = L::kStages;
+  constexpr int kStK = L::kStK, kStV = L::kStV;
   constexpr uint32_t kTile = L::kTile;
   extern __shared__ uint8_t ta_smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(ta_smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* k_full = reinterpret_cast<uint64_t*>(smem + L::kBar);
-  uint64_t* k_empty = k_full + kSt;
-  uint64_t* v_full = k_empty + kSt;
-  uint64_t* v_empty = v_full + kSt;
-  uint64_t* q_full = v_empty + kSt;      // Q of a piece has arrived
-  uint64_t* q_empty = q_full + 1;        // every score product of a piece has read it
-  uint64_t* s_full = q_empty + 1;        // scores of a tile are in tensor memory
-  uint64_t* s_read = s_full + 1;         // the softmax has them in registers (128)
-  uint64_t* p_full = s_read + 1;         // P of a tile is in tensor memory (128)
-  uint64_t* pv_done = p_full + 1;        // O includes the tile
-  uint64_t* o_free = pv_done + 1;        // O of a piece has been stored (128)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(o_free + 1);
+  uint64_t* k_empty = k_full + kStK;
+  uint64_t* v_full = k_empty + kStK;
+  uint64_t* v_empty = v_full + kStV;
+  uint64_t* q_full = v_empty + kStV;     // Q of a stretch has arrived
+  uint64_t* q_empty = q_full + 1;        // every score product of a stretch has read it
+  uint64_t* s_full = q_empty + 1;        // [w]: scores of warpgroup w's next tile are in tensor memory
+  uint64_t* p_half = s_full + 2;         // [w]: it has written P of the first 64 keys (128 arrivals)
+  uint64_t* p_full = p_half + 2;         // [w]: of all (128)
+  uint64_t* pv_done = p_full + 2;        // [w]: O_w includes the tile
+  uint64_t* o_free = pv_done + 2;        // [w]: O_w of a stretch has been read (128)
+  uint64_t* ml_full = o_free + 2;        // the second warpgroup's maxima and sums of a stretch are in shared memory (128)
+  uint64_t* ml_empty = ml_full + 1;      // the first has read them (128)
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ml_empty + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
   long long* walk_at = reinterpret_cast<long long*>(tmem_slot + 2);          // [0] tiles of this CTA, [1] sequence, [2] place in it
-  __shared__ unsigned char s_depth[TA_MAX_DRAFTS];                           // kTreeBias: of the piece's drafts
+  float2* s_ml = reinterpret_cast<float2*>(smem + L::kMl);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kSt; ++s) {
+    for (int s = 0; s < kStK; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
+    }
+    for (int s = 0; s < kStV; ++s) {
       mbar_init(&v_full[s], 1);
       mbar_init(&v_empty[s], 1);
     }
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
-    mbar_init(s_full, 1);
-    mbar_init(s_read, 128);
-    mbar_init(p_full, 128);
-    mbar_init(pv_done, 1);
-    mbar_init(o_free, 128);
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(&s_full[w], 1);
+      mbar_init(&p_half[w], 128);
+      mbar_init(&p_full[w], 128);
+      mbar_init(&pv_done[w], 1);
+      mbar_init(&o_free[w], 128);
+    }
+    mbar_init(ml_full, 128);
+    mbar_init(ml_empty, 128);
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmQ);
     tma_prefetch_desc(&tmK);
     tma_prefetch_desc(&tmV);
   }
-  if (warp == 1) tmem_alloc(tmem_slot, L::kCols);
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
   pdl_wait();
   pdl_trigger();
   if (warp == 0) {
@@ -279,173 +291,190 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       while (ok && walk.next(p, s)) {
         if (seg > 0 && !mbar_wait(q_empty, (seg - 1) & 1, abort_flag)) break;
         ++seg;
-        const int d0 = s.rt * p.tok;
-        mbar_expect_tx(q_full, uint32_t(p.R * p.tok) * kD * 2);          // (rows past the box: whatever, their results go nowhere)
-        tma_load_4d(smem + L::kQ, &tmQ, q_full, 0, s.kvh * p.R, d0, s.b);
-        if (kD == 128) tma_load_4d(smem + L::kQ + 16384, &tmQ, q_full, 64, s.kvh * p.R, d0, s.b);
+        mbar_expect_tx(q_full, uint32_t((s.pair ? 2 : 1) * p.R * p.tok) * kD * 2);   // (rows past the box: whatever, their results go nowhere)
+        for (int w = 0; w < (s.pair ? 2 : 1); ++w) {
+          const int d0 = (2 * s.rg + w) * p.tok;
+          uint8_t* sQ = smem + L::kQ + w * kTile;
+          tma_load_4d(sQ, &tmQ, q_full, 0, s.kvh * p.R, d0, s.b);
+          if (kD == 128) tma_load_4d(sQ + 16384, &tmQ, q_full, 64, s.kvh * p.R, d0, s.b);
+        }
         for (int t = s.t0; t < s.t1; ++t, ++g) {
           const int row = t == s.nt - 1 ? s.len : t * 128;               // the drafts stand behind the cached keys
-          const int st = g % kSt;
-          const uint32_t par = ((g / kSt) & 1) ^ 1;
-          if (!mbar_wait(&k_empty[st], par, abort_flag)) { ok = false; break; }
-          uint8_t* sK = smem + L::kK + st * kTile;
-          mbar_expect_tx(&k_full[st], kTile);
-          tma_load_4d(sK, &tmK, &k_full[st], 0, s.kvh, row, s.b);
-          if (kD == 128) tma_load_4d(sK + 16384, &tmK, &k_full[st], 64, s.kvh, row, s.b);
-          if (!mbar_wait(&v_empty[st], par, abort_flag)) { ok = false; break; }
-          uint8_t* sV = smem + L::kV + st * kTile;
-          mbar_expect_tx(&v_full[st], kTile);
-          tma_load_4d(sV, &tmV, &v_full[st], 0, s.kvh, row, s.b);
-          if (kD == 128) tma_load_4d(sV + 16384, &tmV, &v_full[st], 64, s.kvh, row, s.b);
+          if (!mbar_wait(&k_empty[g % kStK], ((g / kStK) & 1) ^ 1, abort_flag)) { ok = false; break; }
+          uint8_t* sK = smem + L::kK + (g % kStK) * kTile;
+          mbar_expect_tx(&k_full[g % kStK], kTile);
+          tma_load_4d(sK, &tmK, &k_full[g % kStK], 0, s.kvh, row, s.b);
+          if (kD == 128) tma_load_4d(sK + 16384, &tmK, &k_full[g % kStK], 64, s.kvh, row, s.b);
+          if (!mbar_wait(&v_empty[g % kStV], ((g / kStV) & 1) ^ 1, abort_flag)) { ok = false; break; }
+          uint8_t* sV = smem + L::kV + (g % kStV) * kTile;
+          mbar_expect_tx(&v_full[g % kStV], kTile);
+          tma_load_4d(sV, &tmV, &v_full[g % kStV], 0, s.kvh, row, s.b);
+          if (kD == 128) tma_load_4d(sV + 16384, &tmV, &v_full[g % kStV], 64, s.kvh, row, s.b);
         }
       }
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- products
+    // Item u of a stretch is warpgroup u & 1's: with two row tiles both items of a key tile, else every key tile one item. The scores
+    // of item u + 2 go out behind P V of item u, whose P they overwrite.
     constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128, 0, 0), idesc_s64 = umma_idesc_bf16(128, 64, 0, 0);
     constexpr uint32_t idesc_pv = umma_idesc_bf16(128, kD, 0, 1);
-    int g = 0, seg = 0;
+    int g0 = 0, seg = 0, done0 = 0, done1 = 0;           // tiles before the stretch; items that each warpgroup has had
     bool ok = true;
-    auto issue_s = [&](int g, bool drafts) {             // 64 keys are enough for the drafts
-      const uint64_t dQ = umma_smem_desc(smem_u32(smem + L::kQ), 16, 1024);
-      const uint64_t dK = umma_smem_desc(smem_u32(smem + L::kK + (g % kSt) * kTile), 16, 1024);
-#pragma unroll
-      for (int kk = 0; kk < kD / 16; ++kk) {
-        const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
-        umma_bf16_ss_warp(tmem_base + L::kColS, dQ + off, dK + off, drafts ? idesc_s64 : idesc_s, kk != 0);
-      }
-      umma_commit_warp(s_full);
-      umma_commit_warp(&k_empty[g % kSt]);
-    };
-    auto issue_pv = [&](int g, bool drafts, bool first) {
-      const uint64_t dV = umma_smem_desc(smem_u32(smem + L::kV + (g % kSt) * kTile), 16384, 1024);
-#pragma unroll
-      for (int kk = 0; kk < 8; ++kk)
-        if (kk < 4 || !drafts)
-          umma_bf16_ts_warp(tmem_base + L::kColO, tmem_base + L::kColP + kk * 8, dV + kk * 128, idesc_pv, !first || kk != 0);
-      umma_commit_warp(pv_done);
-      umma_commit_warp(&v_empty[g % kSt]);
-    };
     while (ok && walk.next(p, s)) {
-      ok = mbar_wait_warp(q_full, seg & 1, abort_flag);
-      for (int t = s.t0; t < s.t1 && ok; ++t, ++g) {
-        // scores of the first tile here, of every other one ahead of the P V of the tile before it
-        auto scores = [&](int u, int gu) {
-          if (gu > 0 && !mbar_wait_warp(s_read, (gu - 1) & 1, abort_flag)) return false;
-          if (!mbar_wait_warp(&k_full[gu % kSt], (gu / kSt) & 1, abort_flag)) return false;
-          tc_fence_after();
-          issue_s(gu, u == s.nt - 1);
-          if (u + 1 == s.t1) umma_commit_warp(q_empty);
-          return true;
-        };
-        if (t == s.t0 && !scores(t, g)) { ok = false; break; }
-        if (t + 1 < s.t1 && !scores(t + 1, g + 1)) { ok = false; break; }
-        if (t == s.t0 && seg > 0 && !mbar_wait_warp(o_free, (seg - 1) & 1, abort_flag)) { ok = false; break; }
-        if (!mbar_wait_warp(p_full, g & 1, abort_flag) || !mbar_wait_warp(&v_full[g % kSt], (g / kSt) & 1, abort_flag)) {
-          ok = false;
-          break;
-        }
+      const int sh = s.pair ? 1 : 0, items = (s.t1 - s.t0) << sh;
+      auto scores = [&](int u) {
+        const int t = u >> sh, g = g0 + t, w = u & 1;
+        if ((!s.pair || w == 0) && !mbar_wait_warp(&k_full[g % kStK], (g / kStK) & 1, abort_flag)) return false;
         tc_fence_after();
-        issue_pv(g, t == s.nt - 1, t == s.t0);
+        const uint64_t dQ = umma_smem_desc(smem_u32(smem + L::kQ + (s.pair ? w : 0) * kTile), 16, 1024);
+        const uint64_t dK = umma_smem_desc(smem_u32(smem + L::kK + (g % kStK) * kTile), 16, 1024);
+        const bool drafts = s.t0 + t == s.nt - 1;        // 64 keys are enough for them
+#pragma unroll
+        for (int kk = 0; kk < kD / 16; ++kk) {
+          const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
+          umma_bf16_ss_warp(tmem_base + L::kColS + w * 128, dQ + off, dK + off, drafts ? idesc_s64 : idesc_s, kk != 0);
+        }
+        umma_commit_warp(&s_full[w]);
+        if (!s.pair || w == 1) umma_commit_warp(&k_empty[g % kStK]);
+        if (u + 1 == items) umma_commit_warp(q_empty);
+        return true;
+      };
+      ok = mbar_wait_warp(q_full, seg & 1, abort_flag) && scores(0) && (items < 2 || scores(1));
+      for (int u = 0; u < items && ok; ++u) {
+        const int t = u >> sh, g = g0 + t, w = u & 1;
+        const bool drafts = s.t0 + t == s.nt - 1;
+        const uint32_t ph = (w == 0 ? done0 : done1) & 1;
+        const uint64_t dV = umma_smem_desc(smem_u32(smem + L::kV + (g % kStV) * kTile), 16384, 1024);
+        const uint32_t tO = tmem_base + L::kColO + w * 128, tP = tmem_base + L::kColS + w * 128;
+        if (u < 2 && seg > 0) ok = mbar_wait_warp(&o_free[w], (seg - 1) & 1, abort_flag);
+        ok = ok && mbar_wait_warp(&p_half[w], ph, abort_flag);
+        if (ok && (!s.pair || w == 0)) ok = mbar_wait_warp(&v_full[g % kStV], (g / kStV) & 1, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+#pragma unroll
+        for (int kk = 0; kk < 4; ++kk) umma_bf16_ts_warp(tO, tP + kk * 8, dV + kk * 128, idesc_pv, u >= 2 || kk != 0);
+        ok = mbar_wait_warp(&p_full[w], ph, abort_flag);
+        if (!ok) break;
+        tc_fence_after();
+        if (!drafts) {
+#pragma unroll
+          for (int kk = 4; kk < 8; ++kk) umma_bf16_ts_warp(tO, tP + kk * 8, dV + kk * 128, idesc_pv, 1);
+        }
+        umma_commit_warp(&pv_done[w]);
+        if (!s.pair || w == 1) umma_commit_warp(&v_empty[g % kStV]);
+        if (w == 0) ++done0;
+        else ++done1;
+        if (u + 2 < items) ok = scores(u + 2);
       }
+      g0 += s.t1 - s.t0;
       ++seg;
     }
   } else {
     // ---------------------------------------------------------------- softmax: a row per thread
-    const int q = warp & 3, r = q * 32 + lane;           // the quarter of tensor memory that a warp reaches is its number modulo 4
+    const int w = (warp - 2) >> 2, q = warp & 3, r = q * 32 + lane;      // the quarter of tensor memory that a warp reaches is its number mod 4
     const uint32_t lane_sel = uint32_t(q * 32) << 16;
-    const uint32_t tS = tmem_base + lane_sel + L::kColS, tO = tmem_base + lane_sel + L::kColO, tP = tmem_base + lane_sel + L::kColP;
+    const uint32_t tS = tmem_base + lane_sel + L::kColS + w * 128, tO = tmem_base + lane_sel + L::kColO + w * 128;
     const float sl2 = kMod == kTreePlain ? p.scale * kTaLog2e : 1.f;
-    const long long first = (long long)blockIdx.x;
-    int g = 0, seg = 0;
+    int g0 = 0, seg = 0, done = 0, swaps = 0;            // tiles before the stretch; items so far; sums handed from the second warpgroup
     bool ok = true;
     while (ok && walk.next(p, s)) {
-      const int live = min(p.n - s.rt * p.tok, p.tok) * p.R;
+      const int rt = 2 * s.rg + (s.pair ? w : 0);
+      const int live = min(p.n - rt * p.tok, p.tok) * p.R;
       const bool work = q * 32 < live;                   // this warp has rows at all
-      const int d = min(s.rt * p.tok + r / p.R, p.n - 1), h = s.kvh * p.R + r % p.R;
+      const int d = min(rt * p.tok + r / p.R, p.n - 1), h = s.kvh * p.R + r % p.R;
       const unsigned long long bits = p.tree[size_t(s.b) * p.n + d];
-      float slope2 = 0.f, pos = 0.f;
-      if constexpr (kMod == kTreeBias) {
-        slope2 = p.slopes[h] * kTaLog2e;
-        pos = float(s.len + tree_depth(bits));
-        ta_bar_sync(2, 128);                             // the last piece's depths have been read
-        for (int i = r; i < TA_MAX_DRAFTS; i += 128)
-          s_depth[i] = i < p.n ? tree_depth(p.tree[size_t(s.b) * p.n + i]) : 0;
-        ta_bar_sync(2, 128);
-      }
+      const float slope2 = kMod == kTreeBias ? p.slopes[h] * kTaLog2e : 0.f, depth = float(tree_depth(bits));
       float m_ref = -INFINITY, l_run = 0.f;
-      for (int t = s.t0; t < s.t1 && ok; ++t, ++g) {
-        if (!mbar_wait(s_full, g & 1, abort_flag)) { ok = false; break; }
+      const int step = s.pair ? 1 : 2, first = s.t0 + (s.pair ? 0 : w);
+      for (int t = first; t < s.t1 && ok; t += step, ++done) {
+        if (!mbar_wait(&s_full[w], done & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
         const bool drafts = t == s.nt - 1;
         const int rem = drafts ? p.n : min(s.len - t * 128, 128);        // keys of the tile
-        uint32_t sc[128];
-        if (work) {
-          tmem_ld_32x32b_x32(tS, *reinterpret_cast<uint32_t(*)[32]>(&sc[0]));
-          tmem_ld_32x32b_x32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&sc[32]));
-          tmem_ld_32x32b_x32(tS + 64, *reinterpret_cast<uint32_t(*)[32]>(&sc[64]));
-          tmem_ld_32x32b_x32(tS + 96, *reinterpret_cast<uint32_t(*)[32]>(&sc[96]));
-          tmem_ld_wait();
+        if (rem < (drafts ? 64 : 128) && (w == 0 || !s.pair)) {
+          // values past the length may be anything, and 0 times that (two row tiles: P V of the first one comes first)
+          const int g = g0 + t - s.t0, st = g % kStV;
+          if (!__all_sync(0xffffffffu, mbar_wait(&v_full[st], (g / kStV) & 1, abort_flag))) { ok = false; break; }
+          for (int i = r; i < ((drafts ? 64 : 128) - rem) * (kD / 8); i += 128)
+            *ta_chunk(smem + L::kV + st * kTile, rem + i / (kD / 8), i % (kD / 8)) = make_uint4(0u, 0u, 0u, 0u);
+          fence_proxy_async_smem();
         }
-        tc_fence_before();
-        mbar_arrive(s_read);
-        float rs0 = 0.f, rs1 = 0.f;
-        if (work) {
-          bool cap_now = false;                          // the exponentials take the cap
-          if constexpr (kMod == kTreeCap) {
-            const int tier = cap_tier(sc, p.cap);
-            cap_now = tier == kCapNear && rem >= 128;
-            if (!cap_now) cap_scores(sc, p.cap, tier);
-          }
-          if constexpr (kMod == kTreeBias) {
-            const float dist = pos - float(t * 128);
+        if (!work) {                                     // rows that nobody asked for: their P may be anything
+          mbar_arrive(&p_half[w]);
+          mbar_arrive(&p_full[w]);
+          continue;
+        }
+        uint32_t sc[128];
+        tmem_ld_32x32b_x32(tS, *reinterpret_cast<uint32_t(*)[32]>(&sc[0]));
+        tmem_ld_32x32b_x32(tS + 32, *reinterpret_cast<uint32_t(*)[32]>(&sc[32]));
+        tmem_ld_32x32b_x32(tS + 64, *reinterpret_cast<uint32_t(*)[32]>(&sc[64]));
+        tmem_ld_32x32b_x32(tS + 96, *reinterpret_cast<uint32_t(*)[32]>(&sc[96]));
+        tmem_ld_wait();
+        bool cap_now = false;                            // the exponentials take the cap
+        if constexpr (kMod == kTreeCap) {
+          const int tier = cap_tier(sc, p.cap);
+          cap_now = tier == kCapNear && rem >= 128;
+          if (!cap_now) cap_scores(sc, p.cap, tier);
+        }
+        if (drafts) {
 #pragma unroll
-            for (int e = 0; e < 128; ++e) {
-              const float far = drafts ? fabsf(pos - float(s.len + s_depth[e & 63])) : fabsf(dist - float(e));
-              sc[e] = __float_as_uint(fmaf(__uint_as_float(sc[e]), p.scale * kTaLog2e, -slope2 * far));
+          for (int e = 0; e < 64; ++e) {
+            if constexpr (kMod == kTreeBias) {
+              const float dj = e < p.n ? float(tree_depth(p.tree[size_t(s.b) * p.n + e])) : 0.f;
+              sc[e] = __float_as_uint(fmaf(__uint_as_float(sc[e]), p.scale * kTaLog2e, -slope2 * fabsf(depth - dj)));
             }
+            if (!((bits >> e) & 1) || e >= rem) sc[e] = 0xff800000u;
           }
-          if (drafts) {
 #pragma unroll
-            for (int e = 0; e < 128; ++e)
-              if (e >= 64 || !((bits >> (e & 63)) & 1) || e >= rem) sc[e] = 0xff800000u;
-          } else if (rem < 128) {
+          for (int e = 64; e < 128; ++e) sc[e] = 0xff800000u;
+        } else {
+          if constexpr (kMod == kTreeBias) {
+            const float dist = float(s.len - t * 128) + depth;
+#pragma unroll
+            for (int e = 0; e < 128; ++e) sc[e] = __float_as_uint(fmaf(__uint_as_float(sc[e]), p.scale * kTaLog2e, -slope2 * (dist - float(e))));
+          }
+          if (rem < 128) {
 #pragma unroll
             for (int e = 0; e < 128; ++e)
               if (e >= rem) sc[e] = 0xff800000u;
           }
-          float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+        }
+        float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int e = 0; e < 128; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(sc[e]));
-          float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
-          if (kMod == kTreeCap && cap_now) mx = cap_any(mx, p.cap);      // the cap keeps the order of the scores
-          // the reference maximum moves when a tile exceeds it by more than 2^8, as in the attention forward
-          const bool need = mx > m_ref + kTaRescaleStep;
-          if (t == s.t0) {
-            m_ref = mx;
-          } else if (__any_sync(0xffffffffu, need)) {
-            if (!__all_sync(0xffffffffu, mbar_wait(pv_done, (g - 1) & 1, abort_flag))) { ok = false; break; }
-            tc_fence_after();
-            const float corr = need ? exp2f(m_ref - mx) : 1.f;
-            l_run *= corr;
+        for (int e = 0; e < 128; ++e) mx4[e & 3] = fmaxf(mx4[e & 3], __uint_as_float(sc[e]));
+        float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
+        if (kMod == kTreeCap && cap_now) mx = cap_any(mx, p.cap);      // the cap keeps the order of the scores
+        // the reference maximum moves when a tile exceeds it by more than 2^8, as in the attention forward
+        const bool need = mx > m_ref + kTaRescaleStep;
+        if (t == first) {
+          m_ref = mx;
+        } else if (__any_sync(0xffffffffu, need)) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[w], (done - 1) & 1, abort_flag))) { ok = false; break; }
+          tc_fence_after();
+          const float corr = need ? exp2f(m_ref - mx) : 1.f;
+          l_run *= corr;
 #pragma unroll 1
-            for (int c = 0; c < kD / 16; ++c) {
-              uint32_t o[16];
-              tmem_ld_32x32b_x16(tO + c * 16, o);
-              tmem_ld_wait();
+          for (int c = 0; c < kD / 16; ++c) {
+            uint32_t o[16];
+            tmem_ld_32x32b_x16(tO + c * 16, o);
+            tmem_ld_wait();
 #pragma unroll
-              for (int e = 0; e < 16; ++e) o[e] = corr == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * corr);
-              tmem_st_32x32b_x16(tO + c * 16, o);
-            }
-            tmem_st_wait();
-            if (need) m_ref = mx;
+            for (int e = 0; e < 16; ++e) o[e] = corr == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * corr);
+            tmem_st_32x32b_x16(tO + c * 16, o);
           }
-          const float m_sub = m_ref == -INFINITY ? 0.f : m_ref;
+          tmem_st_wait();
+          if (need) m_ref = mx;
+        }
+        const float m_sub = m_ref == -INFINITY ? 0.f : m_ref;
+        float rs0 = 0.f, rs1 = 0.f;
+        auto half = [&](auto lo_tag) {                   // P of 64 keys, handed over as soon as it is there
+          constexpr int kLo = decltype(lo_tag)::value;
           if (kMod == kTreeCap && cap_now) {
-            cap_row_p<0, 128>(sc, p.cap, m_sub, rs0, rs1);
+            cap_row_p<kLo, kLo + 64>(sc, p.cap, m_sub, rs0, rs1);
           } else {
 #pragma unroll
-            for (int e = 0; e < 128; e += 2) {
+            for (int e = kLo; e < kLo + 64; e += 2) {
               const float p0 = exp2f(fmaf(__uint_as_float(sc[e]), sl2, -m_sub)), p1 = exp2f(fmaf(__uint_as_float(sc[e + 1]), sl2, -m_sub));
               rs0 += p0;
               rs1 += p1;
@@ -453,53 +482,81 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
               sc[e >> 1] = *reinterpret_cast<const uint32_t*>(&x);
             }
           }
-        }
-        // P of the tile before has been read
-        if (t > s.t0 && !__all_sync(0xffffffffu, mbar_wait(pv_done, (g - 1) & 1, abort_flag))) { ok = false; break; }
-        tc_fence_after();
-        if (work) {
-#pragma unroll
-          for (int c = 0; c < 4; ++c) tmem_st_32x32b_x16(tP + c * 16, *reinterpret_cast<const uint32_t(*)[16]>(&sc[16 * c]));
+          tmem_st_32x32b_x16(tS + kLo / 2, *reinterpret_cast<const uint32_t(*)[16]>(&sc[kLo / 2]));
+          tmem_st_32x32b_x16(tS + kLo / 2 + 16, *reinterpret_cast<const uint32_t(*)[16]>(&sc[kLo / 2 + 16]));
           tmem_st_wait();
-          l_run += rs0 + rs1;
-        }
-        if (rem < (drafts ? 64 : 128)) {                 // values past the length may be anything, and 0 times that
-          const int st = g % kSt;
-          if (!__all_sync(0xffffffffu, mbar_wait(&v_full[st], (g / kSt) & 1, abort_flag))) { ok = false; break; }
-          for (int i = r; i < ((drafts ? 64 : 128) - rem) * (kD / 8); i += 128)
-            *ta_chunk(smem + L::kV + st * kTile, rem + i / (kD / 8), i % (kD / 8)) = make_uint4(0u, 0u, 0u, 0u);
-          fence_proxy_async_smem();
-        }
-        tc_fence_before();
-        mbar_arrive(p_full);
+          tc_fence_before();
+          mbar_arrive(kLo == 0 ? &p_half[w] : &p_full[w]);
+        };
+        half(std::integral_constant<int, 0>{});
+        if (drafts) mbar_arrive(&p_full[w]);             // nothing behind the first 64
+        else half(std::integral_constant<int, 64>{});
+        l_run += rs0 + rs1;
       }
       if (!ok) break;
-      if (!__all_sync(0xffffffffu, mbar_wait(pv_done, (g - 1) & 1, abort_flag))) { ok = false; break; }
+      // The stretch's end: with one row tile the second warpgroup hands its maximum and sum to the first, which reads both outputs.
+      const bool any = first < s.t1, other = !s.pair && s.t1 - s.t0 > 1;
+      if (any && !__all_sync(0xffffffffu, mbar_wait(&pv_done[w], (done - 1) & 1, abort_flag))) { ok = false; break; }
       tc_fence_after();
-      const bool whole = s.t0 == 0 && s.t1 == s.nt, alive = r < live;
+      g0 += s.t1 - s.t0;
+      const int seg_now = seg++;
+      if (!s.pair && w == 1) {
+        if (other) {
+          if (swaps > 0 && !__all_sync(0xffffffffu, mbar_wait(ml_empty, (swaps - 1) & 1, abort_flag))) { ok = false; break; }
+          s_ml[r] = make_float2(m_ref, l_run);
+          tc_fence_before();
+          mbar_arrive(ml_full);
+          ++swaps;
+        }
+        continue;
+      }
+      float f0 = 1.f, f1 = 0.f;                          // what the two outputs are multiplied with
+      if (other) {
+        if (!__all_sync(0xffffffffu, mbar_wait(ml_full, swaps & 1, abort_flag))) { ok = false; break; }
+        tc_fence_after();
+        const float2 ml = s_ml[r];
+        mbar_arrive(ml_empty);
+        ++swaps;
+        const float m = fmaxf(m_ref, ml.x), m_sub = m == -INFINITY ? 0.f : m;
+        f0 = exp2f(m_ref - m_sub);
+        f1 = exp2f(ml.x - m_sub);
+        l_run = l_run * f0 + ml.y * f1;
+        m_ref = m;
+      }
       if (work) {
-        const size_t slot = size_t(2 * first + (seg == 0 ? 0 : 1)) * 128 + r;
+        const bool whole = s.t0 == 0 && s.t1 == s.nt, alive = r < live;
+        const size_t slot = size_t((2 * int(blockIdx.x) + (seg_now == 0 ? 0 : 1)) * 2 + (s.pair ? w : 0)) * 128 + r;
         const float inv = whole ? (l_run == 0.f ? 0.f : 1.f / l_run) : 1.f;
+        f0 = f0 == 0.f ? 0.f : f0 * inv;
+        f1 *= inv;
         bf16* orow = p.out + ((size_t(s.b) * p.n + d) * p.QH + h) * kD;
         if (alive && !whole) p.part_ml[slot] = make_float2(m_ref, l_run);
 #pragma unroll 1
         for (int c = 0; c < kD / 32; ++c) {
           uint32_t o[32];
           tmem_ld_32x32b_x32(tO + c * 32, o);
-          tmem_ld_wait();
-          if (!alive) continue;
-          if (l_run == 0.f) {
+          if (other) {
+            uint32_t o1[32];
+            tmem_ld_32x32b_x32(tO + 128 + c * 32, o1);
+            tmem_ld_wait();
 #pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = 0u;
+            for (int e = 0; e < 32; ++e) {               // (what weighs nothing may be anything)
+              const float x0 = f0 == 0.f ? 0.f : __uint_as_float(o[e]) * f0;
+              o[e] = __float_as_uint(f1 == 0.f ? x0 : fmaf(__uint_as_float(o1[e]), f1, x0));
+            }
+          } else {
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = l_run == 0.f ? 0u : __float_as_uint(__uint_as_float(o[e]) * f0);
           }
+          if (!alive) continue;
           if (whole) {
 #pragma unroll
             for (int k = 0; k < 4; ++k) {
               uint4 u;
               bf162* u2 = reinterpret_cast<bf162*>(&u);
 #pragma unroll
-              for (int e = 0; e < 4; ++e)
-                u2[e] = __floats2bfloat162_rn(__uint_as_float(o[8 * k + 2 * e]) * inv, __uint_as_float(o[8 * k + 2 * e + 1]) * inv);
+              for (int e = 0; e < 4; ++e) u2[e] = __floats2bfloat162_rn(__uint_as_float(o[8 * k + 2 * e]), __uint_as_float(o[8 * k + 2 * e + 1]));
               reinterpret_cast<uint4*>(orow + c * 32)[k] = u;
             }
           } else {
@@ -510,8 +567,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         }
       }
       tc_fence_before();
-      mbar_arrive(o_free);
-      ++seg;
+      mbar_arrive(&o_free[w]);
+      if (!s.pair) mbar_arrive(&o_free[1]);
     }
   }
 
@@ -519,14 +576,14 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem_base, L::kCols);
+    tmem_dealloc(tmem_base, 512);
   }
   if (threadIdx.x == 0 && *abort_flag != 0 && p.status != nullptr) {
     if (atomicCAS(p.status, 0, int(*abort_flag)) == 0) p.status[1] = 351;
   }
 }
 
-// Joins the pieces of every (sequence, KV head, row tile) that was cut: grid (those, 16), a warp a row, its pieces' sums in the
+// Joins the pieces of every (sequence, KV head, row group) that was cut: grid (those, 32 or 16), a warp a row, its pieces' sums in the
 // order of the keys. A lane looks a piece up, so that no load waits for a division.
 template <int kD>
 __global__ void __launch_bounds__(256)
@@ -535,9 +592,9 @@ tree_join_kernel(const TreeParams p) {
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
-  const int per = p.KVH * p.row_tiles, b = blockIdx.x / per, idx = blockIdx.x % per, kvh = idx / p.row_tiles, rt = idx % p.row_tiles;
-  const int live = min(p.n - rt * p.tok, p.tok) * p.R, r = blockIdx.y * 8 + warp;
-  if (r >= live) return;
+  const int per = p.KVH * p.groups, b = blockIdx.x / per, idx = blockIdx.x % per, kvh = idx / p.groups, rg = idx % p.groups;
+  const int row = blockIdx.y * 8 + warp, rows = p.tok * p.R, r = row % rows, rt = 2 * rg + row / rows;
+  if (row >= 2 * rows || r >= min(p.n - rt * p.tok, p.tok) * p.R) return;
   unsigned long long sum = 0, before = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int v = b0 + lane < p.B ? tree_tiles(tree_len(p, b0 + lane)) : 0;
@@ -553,7 +610,7 @@ tree_join_kernel(const TreeParams p) {
   auto slot_of = [&](int c) {
     if (c > c1) return -1;
     const unsigned long long from = c * total / G;
-    return from == (c + 1) * total / G ? -1 : (2 * c + (from < t0 ? 1 : 0)) * 128 + r;
+    return from == (c + 1) * total / G ? -1 : ((2 * c + (from < t0 ? 1 : 0)) * 2 + row / rows) * 128 + r;
   };
   float m = -INFINITY, l = 0.f, acc[kV];                 // the maximum so far; this lane's pieces of the sum
 #pragma unroll
@@ -603,21 +660,21 @@ static int launch_tree(const TreeParams& p, const TensorMap& tq, const TensorMap
   const long long chunks = (long long)p.B * p.n * (p.QH + 2 * p.KVH) * (kD / 8);
   B200_CHECK(launch_pdl(tree_append_kernel<kD>, dim3(unsigned((chunks + 255) / 256)), dim3(256), 0, st, 0, p));
   B200_CHECK(launch_pdl(tree_attn_kernel<kD, kMod>, dim3(p.ctas), dim3(TA_THREADS), TA<kD>::kSmem, st, 0, *tq, *tk, *tv, p));
-  return static_cast<int>(launch_pdl(tree_join_kernel<kD>, dim3(p.B * p.KVH * p.row_tiles, (p.tok * p.R + 7) / 8), dim3(256), 0, st, 0, p));
+  return static_cast<int>(launch_pdl(tree_join_kernel<kD>, dim3(p.B * p.KVH * p.groups, ((p.n > p.tok ? 2 : 1) * p.tok * p.R + 7) / 8), dim3(256), 0, st, 0, p));
 }
 
-static int tree_row_tiles(int n, int R) { return (n + 128 / R - 1) / (128 / R); }
+// Groups of two tiles of 128 / R drafts.
+static int tree_groups(int n, int R) { return (n + 2 * (128 / R) - 1) / (2 * (128 / R)); }
 
-// Pieces that the list of tiles is cut into: what runs at once, or every tile if there are fewer of full caches.
-static int tree_ctas(int B, int n, int QH, int KVH, int Tmax, int D) {
-  const long long tiles = (long long)B * KVH * tree_row_tiles(n, QH / KVH) * ((Tmax + 127) / 128 + 1);
-  const int slots = num_sms() * (D == 128 ? TA<128>::kCtas : TA<64>::kCtas);
-  return int(tiles < slots ? tiles : slots);
+// Pieces that the list of tiles is cut into: one for every SM, or every tile if there are fewer of full caches.
+static int tree_ctas(int B, int n, int QH, int KVH, int Tmax) {
+  const long long tiles = (long long)B * KVH * tree_groups(n, QH / KVH) * ((Tmax + 127) / 128 + 1);
+  return int(tiles < num_sms() ? tiles : num_sms());
 }
 
 static bool tree_shape_ok(int B, int n, int QH, int KVH, int Tmax, int D) {
   return B >= 0 && n >= 1 && n <= TA_MAX_DRAFTS && (D == 64 || D == 128) && KVH > 0 && QH > 0 && QH % KVH == 0 && QH / KVH <= 128 &&
-         Tmax > 0 && (long long)B * KVH * tree_row_tiles(n, QH / KVH) <= 0x7fffffffLL;
+         Tmax > 0 && (long long)B * KVH * tree_groups(n, QH / KVH) <= 0x7fffffffLL;
 }
 
 }  // namespace b200
@@ -627,7 +684,7 @@ using namespace b200;
 // Bytes of the workspace that b200_tree_attn_append wants (16-byte aligned); 0: sizes that it does not take.
 B200_API long long b200_tree_attn_workspace(int B, int n, int QH, int KVH, int Tmax, int D) {
   if (!tree_shape_ok(B, n, QH, KVH, Tmax, D)) return 0;
-  return 2LL * tree_ctas(B, n, QH, KVH, Tmax, D) * 128 * (D * 4 + 8) + 2LL * B * n * QH * D;
+  return 4LL * tree_ctas(B, n, QH, KVH, Tmax) * 128 * (D * 4 + 8) + 2LL * B * n * QH * D;
 }
 
 // kqv [B * n][ld] (K | Q | V, un-rotated), caches [B, KVH, Tmax, D], out [B, n, QH, D], lens [B], tree [B, n] (64 bits each), rotary
@@ -656,11 +713,11 @@ B200_API int b200_tree_attn_append(const void* kqv, void* kc, void* vc, void* ou
   p.B = B; p.n = n; p.QH = QH; p.KVH = KVH; p.Tmax = Tmax; p.table_rows = table_rows; p.ld = ld;
   p.R = QH / KVH;
   p.tok = std::min(n, 128 / p.R);
-  p.row_tiles = tree_row_tiles(n, p.R);
-  p.ctas = tree_ctas(B, n, QH, KVH, Tmax, D);
+  p.groups = tree_groups(n, p.R);
+  p.ctas = tree_ctas(B, n, QH, KVH, Tmax);
   p.part_o = static_cast<float*>(workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + 2LL * p.ctas * 128 * D);
-  p.q = reinterpret_cast<bf16*>(p.part_ml + 2LL * p.ctas * 128);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + 4LL * p.ctas * 128 * D);
+  p.q = reinterpret_cast<bf16*>(p.part_ml + 4LL * p.ctas * 128);
   p.scale = scale;
   p.cap = make_score_cap(scale, cap);
   p.status = status_ptr();
