@@ -98,13 +98,14 @@ __device__ __forceinline__ float max_abs3(float m, float a, float b) {
   return r;
 }
 
-// Which form the raw scores of a warp's rows need: one answer for the warp. (A NaN stays one in any of them.)
+// Which form the raw scores of a warp's rows need: one answer for the warp (rows that are not `live` do not count). A NaN stays one in
+// any of them.
 template <int N>
-__device__ __forceinline__ int cap_tier(const uint32_t (&s)[N], const ScoreCap& c) {
+__device__ __forceinline__ int cap_tier(const uint32_t (&s)[N], const ScoreCap& c, bool live = true) {
   float far[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int e = 0; e < N; e += 2) far[(e >> 1) & 3] = max_abs3(far[(e >> 1) & 3], __uint_as_float(s[e]), __uint_as_float(s[e + 1]));
-  const float m = max_abs3(fmaxf(far[0], far[1]), far[2], far[3]);
+  const float m = live ? max_abs3(fmaxf(far[0], far[1]), far[2], far[3]) : 0.f;
   if (__all_sync(0xffffffffu, m <= c.reach_near)) return kCapNear;
   return __all_sync(0xffffffffu, m <= c.reach_mid) ? kCapMid : kCapAny;
 }

@@ -14,7 +14,7 @@
 // joins them in the order of the keys.
 //
 // Roles: warp 0 streams Q and the tiles of K and V by TMA, warp 1 issues the products (scores Q K^T into tensor memory, O += P V
-// from it), and two warpgroups do the softmax, a row per thread, each with scores and an output of its own in tensor memory
+// from it), and two warpgroups (warps 4..11) do the softmax, a row per thread, each with scores and an output of its own in tensor memory
 // (columns S_0, S_1, O_0, O_1; P lies over S). A group of more than 128 rows gives each warpgroup a tile of rows; one of up to 128
 // gives them the odd and the even key tiles, and the first one adds up what the two have. Either way the tensor core works for one
 // while the other is in its exponentials: with one warpgroup a tile took 2.1 us at 128 rows of head_dim 128 where its 64 KiB
@@ -31,7 +31,10 @@ namespace b200 {
 
 constexpr float kTaLog2e = 1.4426950408889634f;
 constexpr float kTaRescaleStep = 8.f;
-constexpr int TA_THREADS = 320;
+constexpr int TA_THREADS = 384;
+// 384 x 168 registers at launch, shared out again: 88 for each thread of the first warpgroup, 208 for each of the other two (88 + 2 * 208 =
+// 3 * 168): a row's 128 scores and the arithmetic on them stay in registers.
+constexpr int TA_REGS_FEW = 88, TA_REGS_MANY = 208;
 constexpr int TA_MAX_DRAFTS = 64;                        // the bits of a draft's mask
 constexpr int kTreePlain = 0, kTreeCap = 1, kTreeBias = 2;
 
@@ -52,6 +55,7 @@ struct TreeParams {
   long long ld;
   int R, tok, groups;       // query heads of a KV head; drafts of a row tile (R tok <= 128); groups of two row tiles (or one)
   int ctas;                 // pieces of the list
+  int* arrived;             // [B * KVH * groups]: pieces that are done, where the last of them joins them all; else null
   float scale;
   ScoreCap cap;             // kTreeCap
   int* status;
@@ -63,8 +67,9 @@ struct TA {
   static constexpr int kStK = kD == 128 ? 2 : 4, kStV = kD == 128 ? 3 : 4;      // rings of K and V
   static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + kStK * kTile;
   static constexpr int kBar = kV + kStV * kTile;
-  // k_full, k_empty [kStK]; v_full, v_empty [kStV]; q_full, q_empty; s_full, p_half, p_full, pv_done, o_free [2]; ml_full, ml_empty
-  static constexpr int kBars = 2 * kStK + 2 * kStV + 2 + 10 + 2;
+  // k_full, k_empty [kStK]; v_full, v_empty [kStV]; q_full, q_empty; s_full, p_half, p_full, pv_done, o_free [2]; ml_full, ml_empty;
+  // part_out, last_known
+  static constexpr int kBars = 2 * kStK + 2 * kStV + 2 + 10 + 2 + 2;
   static constexpr int kMl = kBar + kBars * 8 + 48;
   static constexpr int kSmem = kMl + 128 * 8 + 1024;
   static constexpr uint32_t kColS = 0, kColO = 256;                             // [2] each, 128 columns apart
@@ -179,6 +184,8 @@ tree_append_kernel(const TreeParams p) {
   pdl_trigger();
   const int heads = p.QH + 2 * p.KVH;
   const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (p.arrived != nullptr)
+    for (long long c = i; c < (long long)p.B * p.KVH * p.groups; c += (long long)gridDim.x * 256) p.arrived[c] = 0;
   if (i >= (long long)p.B * p.n * heads * kChunks) return;
   const int c = int(i % kChunks), head = int(i / kChunks % heads);
   const long long row = i / kChunks / heads;
@@ -199,6 +206,92 @@ tree_append_kernel(const TreeParams p) {
 // 16-byte chunk `c` of row `r` in a tile of 128-byte rows (64 columns a box, 16 KiB apart), as TMA writes it.
 __device__ __forceinline__ uint4* ta_chunk(uint8_t* tile, int r, int c) {
   return reinterpret_cast<uint4*>(tile + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
+}
+
+// The pieces that a (sequence, KV head, row group) is cut into: those of CTAs [c0, c1] that have tiles at all. CTA c has the tiles from
+// c total / G on, so tile t is in the piece of CTA ((t + 1) G - 1) / total. Nearly all lists are short enough for 32-bit division.
+struct TreePieces {
+  unsigned long long total, t0;
+  unsigned G;
+  int c0, c1, count;
+  bool narrow;
+  __device__ __forceinline__ unsigned long long from(int c) const {
+    return narrow ? unsigned(c) * unsigned(total) / G : (unsigned long long)c * total / G;
+  }
+  __device__ __forceinline__ bool has(int c) const { return from(c) != from(c + 1); }
+  // slot of row r of row tile `w` in the group
+  __device__ __forceinline__ int slot(int c, int w, int r) const { return ((2 * c + (from(c) < t0 ? 1 : 0)) * 2 + w) * 128 + r; }
+};
+
+__device__ __forceinline__ TreePieces tree_pieces(const TreeParams& p, unsigned long long total, unsigned long long t0, int nt) {
+  TreePieces x;
+  x.total = total;
+  x.t0 = t0;
+  x.G = p.ctas;
+  x.narrow = (total + 1) * (x.G + 1) < 0x100000000ull;
+  if (x.narrow) {
+    x.c0 = int((unsigned(t0 + 1) * x.G - 1) / unsigned(total));
+    x.c1 = int((unsigned(t0 + nt) * x.G - 1) / unsigned(total));
+  } else {
+    x.c0 = int(((t0 + 1) * x.G - 1) / total);
+    x.c1 = int(((t0 + nt) * x.G - 1) / total);
+  }
+  // with no more CTAs than tiles every CTA has one
+  x.count = x.c1 - x.c0 + 1;
+  if (total < x.G) {
+    x.count = 0;
+    for (int c = x.c0; c <= x.c1; ++c) x.count += x.has(c);
+  }
+  return x;
+}
+
+// First list position of a stretch's (sequence, KV head, row group).
+__device__ __forceinline__ unsigned long long combo_first(const TreeParams& p, const TreeSeg& s) {
+  unsigned long long before = 0;
+  for (int b = 0; b < s.b; ++b) before += tree_tiles(tree_len(p, b));
+  return before * (p.KVH * p.groups) + (unsigned long long)(s.kvh * p.groups + s.rg) * s.nt;
+}
+
+// One row's result from its pieces, by a warp: a lane looks a piece up, so that no load waits for a division; sums in the order of the keys.
+template <int kD>
+__device__ __forceinline__ void tree_join_row(const TreeParams& p, int b, int kvh, int rt, int r, int w, const TreePieces& pc, int lane) {
+  constexpr int kV = kD / 32;
+  float m = -INFINITY, l = 0.f, acc[kV];                 // the maximum so far; this lane's pieces of the sum
+#pragma unroll
+  for (int e = 0; e < kV; ++e) acc[e] = 0.f;
+  for (int c = pc.c0; c <= pc.c1; c += 32) {
+    const int slot = c + lane <= pc.c1 && pc.has(c + lane) ? pc.slot(c + lane, w, r) : -1;
+    const float2 ml = slot >= 0 ? p.part_ml[slot] : make_float2(-INFINITY, 0.f);
+    float mx = ml.x;
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    mx = fmaxf(mx, m);
+    const float ref = mx == -INFINITY ? 0.f : mx, corr = exp2f(m - ref), f = exp2f(ml.x - ref);
+    m = mx;
+    l = l * corr + ml.y * f;
+#pragma unroll
+    for (int e = 0; e < kV; ++e) acc[e] *= corr;
+    const int count = min(32, pc.c1 - c + 1);
+#pragma unroll 4
+    for (int i = 0; i < count; ++i) {
+      const int si = __shfl_sync(0xffffffffu, slot, i);
+      const float fi = __shfl_sync(0xffffffffu, f, i);
+      if (si < 0) continue;
+      const float* o = p.part_o + size_t(si) * kD + lane * kV;
+      float v[kV];
+      if constexpr (kV == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(o);
+      else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(o);
+#pragma unroll
+      for (int e = 0; e < kV; ++e) acc[e] += v[e] * fi;
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  const int d = rt * p.tok + r / p.R, h = kvh * p.R + r % p.R;
+  bf16* out = p.out + ((size_t(b) * p.n + d) * p.QH + h) * kD + lane * kV;
+#pragma unroll
+  for (int e = 0; e < kV; e += 2) *reinterpret_cast<bf162*>(out + e) = __floats2bfloat162_rn(acc[e] * inv, acc[e + 1] * inv);
 }
 
 template <int kD, int kMod>
@@ -223,9 +316,12 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   uint64_t* o_free = pv_done + 2;        // [w]: O_w of a stretch has been read (128)
   uint64_t* ml_full = o_free + 2;        // the second warpgroup's maxima and sums of a stretch are in shared memory (128)
   uint64_t* ml_empty = ml_full + 1;      // the first has read them (128)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(ml_empty + 1);
+  uint64_t* part_out = ml_empty + 1;     // a piece's sums are in the workspace (128)
+  uint64_t* last_known = part_out + 1;   // whether it was the last of its rows' pieces
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last_known + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  long long* walk_at = reinterpret_cast<long long*>(tmem_slot + 2);          // [0] tiles of this CTA, [1] sequence, [2] place in it
+  long long* walk_at = reinterpret_cast<long long*>(tmem_slot + 2);          // [0] tiles of this CTA, [1] sequence, [2] place in it, [3] the list's
+  volatile int* is_last = reinterpret_cast<volatile int*>(walk_at + 4);
   float2* s_ml = reinterpret_cast<float2*>(smem + L::kMl);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -249,6 +345,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     }
     mbar_init(ml_full, 128);
     mbar_init(ml_empty, 128);
+    mbar_init(part_out, 128);
+    mbar_init(last_known, 1);
     *abort_flag = 0;
     mbar_fence_init();
     tma_prefetch_desc(&tmQ);
@@ -267,6 +365,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       walk_at[0] = end - at;
       walk_at[1] = b_at;
       walk_at[2] = at - b_first;
+      walk_at[3] = total;
     }
   }
   tc_fence_before();
@@ -285,6 +384,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA
+    setmaxnreg_dec<TA_REGS_FEW>();
     if (lane == 0) {
       int g = 0, seg = 0;
       bool ok = true;
@@ -315,6 +415,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
     }
   } else if (warp == 1) {
     // ---------------------------------------------------------------- products
+    setmaxnreg_dec<TA_REGS_FEW>();
     // Item u of a stretch is warpgroup u & 1's: with two row tiles both items of a key tile, else every key tile one item. The scores
     // of item u + 2 go out behind P V of item u, whose P they overwrite.
     constexpr uint32_t idesc_s = umma_idesc_bf16(128, 128, 0, 0), idesc_s64 = umma_idesc_bf16(128, 64, 0, 0);
@@ -370,13 +471,16 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       g0 += s.t1 - s.t0;
       ++seg;
     }
+  } else if (warp < 4) {
+    setmaxnreg_dec<TA_REGS_FEW>();
   } else {
     // ---------------------------------------------------------------- softmax: a row per thread
-    const int w = (warp - 2) >> 2, q = warp & 3, r = q * 32 + lane;      // the quarter of tensor memory that a warp reaches is its number mod 4
+    setmaxnreg_inc<TA_REGS_MANY>();
+    const int w = (warp - 4) >> 2, q = warp & 3, r = q * 32 + lane;      // the quarter of tensor memory that a warp reaches is its number mod 4
     const uint32_t lane_sel = uint32_t(q * 32) << 16;
     const uint32_t tS = tmem_base + lane_sel + L::kColS + w * 128, tO = tmem_base + lane_sel + L::kColO + w * 128;
     const float sl2 = kMod == kTreePlain ? p.scale * kTaLog2e : 1.f;
-    int g0 = 0, seg = 0, done = 0, swaps = 0;            // tiles before the stretch; items so far; sums handed from the second warpgroup
+    int g0 = 0, seg = 0, done = 0, swaps = 0, parts = 0; // tiles before the stretch; items so far; sums handed from the second warpgroup; pieces
     bool ok = true;
     while (ok && walk.next(p, s)) {
       const int rt = 2 * s.rg + (s.pair ? w : 0);
@@ -413,7 +517,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         tmem_ld_wait();
         bool cap_now = false;                            // the exponentials take the cap
         if constexpr (kMod == kTreeCap) {
-          const int tier = cap_tier(sc, p.cap);
+          const int tier = cap_tier(sc, p.cap, r < live);
           cap_now = tier == kCapNear && rem >= 128;
           if (!cap_now) cap_scores(sc, p.cap, tier);
         }
@@ -446,7 +550,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * sl2;
         if (kMod == kTreeCap && cap_now) mx = cap_any(mx, p.cap);      // the cap keeps the order of the scores
         // the reference maximum moves when a tile exceeds it by more than 2^8, as in the attention forward
-        const bool need = mx > m_ref + kTaRescaleStep;
+        const bool need = r < live && mx > m_ref + kTaRescaleStep;
         if (t == first) {
           m_ref = mx;
         } else if (__any_sync(0xffffffffu, need)) {
@@ -523,8 +627,9 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         l_run = l_run * f0 + ml.y * f1;
         m_ref = m;
       }
+      const bool whole = s.t0 == 0 && s.t1 == s.nt;
       if (work) {
-        const bool whole = s.t0 == 0 && s.t1 == s.nt, alive = r < live;
+        const bool alive = r < live;
         const size_t slot = size_t((2 * int(blockIdx.x) + (seg_now == 0 ? 0 : 1)) * 2 + (s.pair ? w : 0)) * 128 + r;
         const float inv = whole ? (l_run == 0.f ? 0.f : 1.f / l_run) : 1.f;
         f0 = f0 == 0.f ? 0.f : f0 * inv;
@@ -569,6 +674,22 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       tc_fence_before();
       mbar_arrive(&o_free[w]);
       if (!s.pair) mbar_arrive(&o_free[1]);
+      if (p.arrived != nullptr && !whole) {              // few rows: whoever comes last joins them
+        const int combo = (s.b * p.KVH + s.kvh) * p.groups + s.rg;
+        const TreePieces pc = tree_pieces(p, walk_at[3], combo_first(p, s), s.nt);
+        __threadfence();
+        mbar_arrive(part_out);
+        if (r == 0 && mbar_wait(part_out, parts & 1, abort_flag)) {
+          *is_last = atomicAdd(&p.arrived[combo], 1) == pc.count - 1;
+          mbar_arrive(last_known);
+        }
+        if (!__all_sync(0xffffffffu, mbar_wait(last_known, parts & 1, abort_flag))) { ok = false; break; }
+        ++parts;
+        if (*is_last != 0) {
+          __threadfence();
+          for (int row = q; row < live; row += 4) tree_join_row<kD>(p, s.b, s.kvh, 2 * s.rg, row, 0, pc, lane);
+        }
+      }
     }
   }
 
@@ -583,71 +704,26 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   }
 }
 
-// Joins the pieces of every (sequence, KV head, row group) that was cut: grid (those, 32 or 16), a warp a row, its pieces' sums in the
-// order of the keys. A lane looks a piece up, so that no load waits for a division.
+// Joins the pieces of every (sequence, KV head, row group) that was cut: grid (those, rows / 8), a warp a row.
 template <int kD>
 __global__ void __launch_bounds__(256)
 tree_join_kernel(const TreeParams p) {
-  constexpr int kV = kD / 32;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
   const int per = p.KVH * p.groups, b = blockIdx.x / per, idx = blockIdx.x % per, kvh = idx / p.groups, rg = idx % p.groups;
-  const int row = blockIdx.y * 8 + warp, rows = p.tok * p.R, r = row % rows, rt = 2 * rg + row / rows;
+  const int row = blockIdx.y * 8 + warp, rows = p.tok * p.R, w = row >= rows ? 1 : 0, r = row - w * rows, rt = 2 * rg + w;
   if (row >= 2 * rows || r >= min(p.n - rt * p.tok, p.tok) * p.R) return;
   unsigned long long sum = 0, before = 0;
+  int nt = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
     const int v = b0 + lane < p.B ? tree_tiles(tree_len(p, b0 + lane)) : 0;
     sum += __reduce_add_sync(0xffffffffu, v);
     before += __reduce_add_sync(0xffffffffu, b0 + lane < b ? v : 0);
+    if (b >= b0 && b < b0 + 32) nt = __shfl_sync(0xffffffffu, v, b - b0);
   }
-  const unsigned nt = tree_tiles(tree_len(p, b));
-  const unsigned long long total = sum * per, t0 = before * per + (unsigned long long)idx * nt, G = p.ctas;
-  // tile t is in the piece of CTA ((t + 1) G - 1) / total
-  const int c0 = int(((t0 + 1) * G - 1) / total), c1 = int(((t0 + nt) * G - 1) / total);
-  if (c0 == c1) return;
-  // the piece of CTA c: its slot, or -1 where the CTA has no tile at all
-  auto slot_of = [&](int c) {
-    if (c > c1) return -1;
-    const unsigned long long from = c * total / G;
-    return from == (c + 1) * total / G ? -1 : ((2 * c + (from < t0 ? 1 : 0)) * 2 + row / rows) * 128 + r;
-  };
-  float m = -INFINITY, l = 0.f, acc[kV];                 // the maximum so far; this lane's pieces of the sum
-#pragma unroll
-  for (int e = 0; e < kV; ++e) acc[e] = 0.f;
-  for (int c = c0; c <= c1; c += 32) {
-    const int slot = slot_of(c + lane);
-    const float2 ml = slot >= 0 ? p.part_ml[slot] : make_float2(-INFINITY, 0.f);
-    float mx = ml.x;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    mx = fmaxf(mx, m);
-    const float ref = mx == -INFINITY ? 0.f : mx, corr = exp2f(m - ref), f = exp2f(ml.x - ref);
-    m = mx;
-    l = l * corr + ml.y * f;
-#pragma unroll
-    for (int e = 0; e < kV; ++e) acc[e] *= corr;
-    const int count = min(32, c1 - c + 1);
-#pragma unroll 4
-    for (int i = 0; i < count; ++i) {
-      const int si = __shfl_sync(0xffffffffu, slot, i);
-      const float fi = __shfl_sync(0xffffffffu, f, i);
-      if (si < 0) continue;
-      const float* o = p.part_o + size_t(si) * kD + lane * kV;
-      float v[kV];
-      if constexpr (kV == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(o);
-      else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(o);
-#pragma unroll
-      for (int e = 0; e < kV; ++e) acc[e] += v[e] * fi;
-    }
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-  const float inv = l == 0.f ? 0.f : 1.f / l;
-  const int d = rt * p.tok + r / p.R, h = kvh * p.R + r % p.R;
-  bf16* out = p.out + ((size_t(b) * p.n + d) * p.QH + h) * kD + lane * kV;
-#pragma unroll
-  for (int e = 0; e < kV; e += 2) *reinterpret_cast<bf162*>(out + e) = __floats2bfloat162_rn(acc[e] * inv, acc[e + 1] * inv);
+  const TreePieces pc = tree_pieces(p, sum * per, before * per + (unsigned long long)idx * nt, nt);
+  if (pc.c0 != pc.c1) tree_join_row<kD>(p, b, kvh, rt, r, w, pc, lane);
 }
 
 template <int kD, int kMod>
@@ -660,6 +736,7 @@ static int launch_tree(const TreeParams& p, const TensorMap& tq, const TensorMap
   const long long chunks = (long long)p.B * p.n * (p.QH + 2 * p.KVH) * (kD / 8);
   B200_CHECK(launch_pdl(tree_append_kernel<kD>, dim3(unsigned((chunks + 255) / 256)), dim3(256), 0, st, 0, p));
   B200_CHECK(launch_pdl(tree_attn_kernel<kD, kMod>, dim3(p.ctas), dim3(TA_THREADS), TA<kD>::kSmem, st, 0, *tq, *tk, *tv, p));
+  if (p.arrived != nullptr) return 0;
   return static_cast<int>(launch_pdl(tree_join_kernel<kD>, dim3(p.B * p.KVH * p.groups, ((p.n > p.tok ? 2 : 1) * p.tok * p.R + 7) / 8), dim3(256), 0, st, 0, p));
 }
 
@@ -684,7 +761,7 @@ using namespace b200;
 // Bytes of the workspace that b200_tree_attn_append wants (16-byte aligned); 0: sizes that it does not take.
 B200_API long long b200_tree_attn_workspace(int B, int n, int QH, int KVH, int Tmax, int D) {
   if (!tree_shape_ok(B, n, QH, KVH, Tmax, D)) return 0;
-  return 4LL * tree_ctas(B, n, QH, KVH, Tmax) * 128 * (D * 4 + 8) + 2LL * B * n * QH * D;
+  return 4LL * tree_ctas(B, n, QH, KVH, Tmax) * 128 * (D * 4 + 8) + 2LL * B * n * QH * D + 4LL * B * KVH * tree_groups(n, QH / KVH);
 }
 
 // kqv [B * n][ld] (K | Q | V, un-rotated), caches [B, KVH, Tmax, D], out [B, n, QH, D], lens [B], tree [B, n] (64 bits each), rotary
@@ -718,6 +795,11 @@ B200_API int b200_tree_attn_append(const void* kqv, void* kc, void* vc, void* ou
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + 4LL * p.ctas * 128 * D);
   p.q = reinterpret_cast<bf16*>(p.part_ml + 4LL * p.ctas * 128);
+  // Few rows times few pieces: the CTA that finishes a (sequence, KV head) last joins its pieces, where a kernel of its own takes 3 to 5 us
+  // more than that; more of them would keep that one SM busy for longer.
+  const long long combos = (long long)B * KVH * p.groups;
+  p.arrived = n * p.R <= 64 && (p.ctas / combos + 2) * n * p.R <= 512
+                  ? reinterpret_cast<int*>(p.q + (size_t)B * n * QH * D) : nullptr;
   p.scale = scale;
   p.cap = make_score_cap(scale, cap);
   p.status = status_ptr();
