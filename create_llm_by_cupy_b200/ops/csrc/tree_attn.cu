@@ -49,7 +49,7 @@ struct TreeParams {
   const float* cosr;        // [rows, D / 2]
   const float* sinr;
   const float* slopes;      // kTreeBias: [QH]
-  float* part_o;            // [2 * CTAs][2][128][D]: a CTA's first and last piece, row tile in the group
+  float4* part_o;           // [2 * CTAs][2][D / 4][128]: a CTA's first and last piece, row tile in the group; rows side by side
   float2* part_ml;          // [2 * CTAs][2][128]: maximum (log2 units), sum
   int B, n, QH, KVH, Tmax, table_rows;
   long long ld;
@@ -84,30 +84,36 @@ struct TreeSeg {
 __device__ __forceinline__ int tree_len(const TreeParams& p, int b) { return checked_index(p.lens[b], p.Tmax, p.status, 350); }
 __device__ __forceinline__ int tree_tiles(int len) { return (len + 127) / 128 + 1; }
 
-// The list position `at` as (sequence, first list position of it), and the list's length; by a whole warp.
-__device__ __forceinline__ void tree_find(const TreeParams& p, long long num, long long den, int lane, long long& total, long long& at,
-                                          int& b_at, long long& b_first) {
-  const int per = p.KVH * p.groups;
+// The list's length, and the sequence that its tile `at` belongs to with that sequence's first tile; by a whole warp.
+__device__ __forceinline__ long long tree_total(const TreeParams& p, int lane) {
   long long sum = 0;
-  for (int b0 = 0; b0 < p.B; b0 += 32) {
-    const int b = b0 + lane;
-    int v = b < p.B ? tree_tiles(tree_len(p, b)) : 0;
-    sum += __reduce_add_sync(0xffffffffu, v);
-  }
-  total = sum * per;
-  at = num * total / den;
-  b_at = 0;
-  b_first = 0;
-  for (int b = 0; b < p.B; ++b) {
-    const long long next = b_first + (long long)tree_tiles(tree_len(p, b)) * per;
-    if (at < next) {
-      b_at = b;
-      return;
-    }
-    b_first = next;
-  }
-  b_at = p.B;
+  for (int b0 = 0; b0 < p.B; b0 += 32) sum += __reduce_add_sync(0xffffffffu, b0 + lane < p.B ? tree_tiles(tree_len(p, b0 + lane)) : 0);
+  return sum * (p.KVH * p.groups);
 }
+__device__ __forceinline__ int tree_find(const TreeParams& p, long long at, int lane, long long& first) {
+  const int per = p.KVH * p.groups;
+  first = 0;
+  for (int b0 = 0; b0 < p.B; b0 += 32) {
+    const int v = b0 + lane < p.B ? tree_tiles(tree_len(p, b0 + lane)) : 0;
+    int before = v;                                      // of the lanes up to this one
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, before, o);
+      if (lane >= o) before += y;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, at < first + (long long)before * per);
+    if (hit != 0) {
+      const int l = __ffs(hit) - 1;
+      first += (long long)__shfl_sync(0xffffffffu, before - v, l) * per;
+      return b0 + l;
+    }
+    first += (long long)__shfl_sync(0xffffffffu, before, 31) * per;
+  }
+  return p.B;
+}
+
+// The list is cut into as many pieces as there are CTAs, or tiles if those are fewer: piece c has the tiles from c total / G on.
+__device__ __forceinline__ long long tree_pieces_of(const TreeParams& p, long long total) { return total < p.ctas ? total : p.ctas; }
 
 // Walks the pieces of one CTA.
 struct TreeWalk {
@@ -208,39 +214,24 @@ __device__ __forceinline__ uint4* ta_chunk(uint8_t* tile, int r, int c) {
   return reinterpret_cast<uint4*>(tile + (c >> 3) * 16384 + r * 128 + (((c & 7) ^ (r & 7)) << 4));
 }
 
-// The pieces that a (sequence, KV head, row group) is cut into: those of CTAs [c0, c1] that have tiles at all. CTA c has the tiles from
-// c total / G on, so tile t is in the piece of CTA ((t + 1) G - 1) / total. Nearly all lists are short enough for 32-bit division.
+// Pieces [c0, c1] that a (sequence, KV head, row group) is cut into, whose tiles are [t0, t0 + nt) of the list: tile t is in piece
+// ((t + 1) G - 1) / total. Nearly all lists are short enough for 32-bit division.
 struct TreePieces {
-  unsigned long long total, t0;
-  unsigned G;
-  int c0, c1, count;
-  bool narrow;
-  __device__ __forceinline__ unsigned long long from(int c) const {
-    return narrow ? unsigned(c) * unsigned(total) / G : (unsigned long long)c * total / G;
-  }
-  __device__ __forceinline__ bool has(int c) const { return from(c) != from(c + 1); }
-  // slot of row r of row tile `w` in the group
-  __device__ __forceinline__ int slot(int c, int w, int r) const { return ((2 * c + (from(c) < t0 ? 1 : 0)) * 2 + w) * 128 + r; }
+  int c0, c1, late;         // late: the first one began with other rows
+  __device__ __forceinline__ int slot(int c, int w) const { return 4 * c + (c == c0 ? 2 * late : 0) + w; }      // of row tile w in the group
 };
 
 __device__ __forceinline__ TreePieces tree_pieces(const TreeParams& p, unsigned long long total, unsigned long long t0, int nt) {
+  const unsigned G = unsigned(tree_pieces_of(p, total));
   TreePieces x;
-  x.total = total;
-  x.t0 = t0;
-  x.G = p.ctas;
-  x.narrow = (total + 1) * (x.G + 1) < 0x100000000ull;
-  if (x.narrow) {
-    x.c0 = int((unsigned(t0 + 1) * x.G - 1) / unsigned(total));
-    x.c1 = int((unsigned(t0 + nt) * x.G - 1) / unsigned(total));
+  if ((total + 1) * (G + 1) < 0x100000000ull) {
+    x.c0 = int((unsigned(t0 + 1) * G - 1) / unsigned(total));
+    x.c1 = int((unsigned(t0 + nt) * G - 1) / unsigned(total));
+    x.late = unsigned(x.c0) * unsigned(total) / G < unsigned(t0) ? 1 : 0;
   } else {
-    x.c0 = int(((t0 + 1) * x.G - 1) / total);
-    x.c1 = int(((t0 + nt) * x.G - 1) / total);
-  }
-  // with no more CTAs than tiles every CTA has one
-  x.count = x.c1 - x.c0 + 1;
-  if (total < x.G) {
-    x.count = 0;
-    for (int c = x.c0; c <= x.c1; ++c) x.count += x.has(c);
+    x.c0 = int(((t0 + 1) * G - 1) / total);
+    x.c1 = int(((t0 + nt) * G - 1) / total);
+    x.late = (unsigned long long)x.c0 * total / G < t0 ? 1 : 0;
   }
   return x;
 }
@@ -252,46 +243,46 @@ __device__ __forceinline__ unsigned long long combo_first(const TreeParams& p, c
   return before * (p.KVH * p.groups) + (unsigned long long)(s.kvh * p.groups + s.rg) * s.nt;
 }
 
-// One row's result from its pieces, by a warp: a lane looks a piece up, so that no load waits for a division; sums in the order of the keys.
+// Four columns of one row's result from its pieces, in the order of the keys; eight pieces' loads at a time.
 template <int kD>
-__device__ __forceinline__ void tree_join_row(const TreeParams& p, int b, int kvh, int rt, int r, int w, const TreePieces& pc, int lane) {
-  constexpr int kV = kD / 32;
-  float m = -INFINITY, l = 0.f, acc[kV];                 // the maximum so far; this lane's pieces of the sum
+__device__ __forceinline__ void tree_join_task(const TreeParams& p, int b, int kvh, int rt, int w, int r, int chunk, const TreePieces& pc) {
+  constexpr int kBatch = 8;
+  float m = -INFINITY, l = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+  for (int c = pc.c0; c <= pc.c1; c += kBatch) {
+    float2 ml[kBatch];
+    float4 o[kBatch];
 #pragma unroll
-  for (int e = 0; e < kV; ++e) acc[e] = 0.f;
-  for (int c = pc.c0; c <= pc.c1; c += 32) {
-    const int slot = c + lane <= pc.c1 && pc.has(c + lane) ? pc.slot(c + lane, w, r) : -1;
-    const float2 ml = slot >= 0 ? p.part_ml[slot] : make_float2(-INFINITY, 0.f);
-    float mx = ml.x;
+    for (int u = 0; u < kBatch; ++u) {
+      const size_t slot = pc.slot(min(c + u, pc.c1), w);
+      ml[u] = p.part_ml[slot * 128 + r];
+      o[u] = p.part_o[(slot * (kD / 4) + chunk) * 128 + r];
+    }
+    float mx = m;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-    mx = fmaxf(mx, m);
-    const float ref = mx == -INFINITY ? 0.f : mx, corr = exp2f(m - ref), f = exp2f(ml.x - ref);
+    for (int u = 0; u < kBatch; ++u) mx = fmaxf(mx, ml[u].x);
+    const float ref = mx == -INFINITY ? 0.f : mx, corr = exp2f(m - ref);
     m = mx;
-    l = l * corr + ml.y * f;
+    l *= corr;
 #pragma unroll
-    for (int e = 0; e < kV; ++e) acc[e] *= corr;
-    const int count = min(32, pc.c1 - c + 1);
-#pragma unroll 4
-    for (int i = 0; i < count; ++i) {
-      const int si = __shfl_sync(0xffffffffu, slot, i);
-      const float fi = __shfl_sync(0xffffffffu, f, i);
-      if (si < 0) continue;
-      const float* o = p.part_o + size_t(si) * kD + lane * kV;
-      float v[kV];
-      if constexpr (kV == 4) *reinterpret_cast<float4*>(v) = *reinterpret_cast<const float4*>(o);
-      else *reinterpret_cast<float2*>(v) = *reinterpret_cast<const float2*>(o);
+    for (int e = 0; e < 4; ++e) a[e] *= corr;
 #pragma unroll
-      for (int e = 0; e < kV; ++e) acc[e] += v[e] * fi;
+    for (int u = 0; u < kBatch; ++u) {
+      const float f = c + u <= pc.c1 ? exp2f(ml[u].x - ref) : 0.f;
+      l += ml[u].y * f;
+      a[0] += o[u].x * f;
+      a[1] += o[u].y * f;
+      a[2] += o[u].z * f;
+      a[3] += o[u].w * f;
     }
   }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int d = rt * p.tok + r / p.R, h = kvh * p.R + r % p.R;
-  bf16* out = p.out + ((size_t(b) * p.n + d) * p.QH + h) * kD + lane * kV;
-#pragma unroll
-  for (int e = 0; e < kV; e += 2) *reinterpret_cast<bf162*>(out + e) = __floats2bfloat162_rn(acc[e] * inv, acc[e + 1] * inv);
+  const bf162 x = __floats2bfloat162_rn(a[0] * inv, a[1] * inv), y = __floats2bfloat162_rn(a[2] * inv, a[3] * inv);
+  uint2 u;
+  u.x = *reinterpret_cast<const uint32_t*>(&x);
+  u.y = *reinterpret_cast<const uint32_t*>(&y);
+  *reinterpret_cast<uint2*>(p.out + ((size_t(b) * p.n + d) * p.QH + h) * kD + chunk * 4) = u;
 }
 
 template <int kD, int kMod>
@@ -357,10 +348,17 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   pdl_wait();
   pdl_trigger();
   if (warp == 0) {
-    long long total, at, b_first, end;
-    int b_at;
-    tree_find(p, blockIdx.x, p.ctas, lane, total, at, b_at, b_first);
-    end = (long long)(blockIdx.x + 1) * total / p.ctas;
+    const long long total = tree_total(p, lane), G = tree_pieces_of(p, total);
+    long long at, end, b_first;
+    if ((total + 1) * (G + 1) < 0x100000000ll) {
+      at = unsigned(blockIdx.x) * unsigned(total) / unsigned(G);
+      end = (unsigned(blockIdx.x) + 1) * unsigned(total) / unsigned(G);
+    } else {
+      at = blockIdx.x * total / G;
+      end = (blockIdx.x + 1) * total / G;
+    }
+    if (blockIdx.x >= G) at = end = 0;
+    const int b_at = tree_find(p, at, lane, b_first);
     if (lane == 0) {
       walk_at[0] = end - at;
       walk_at[1] = b_at;
@@ -630,12 +628,12 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const bool whole = s.t0 == 0 && s.t1 == s.nt;
       if (work) {
         const bool alive = r < live;
-        const size_t slot = size_t((2 * int(blockIdx.x) + (seg_now == 0 ? 0 : 1)) * 2 + (s.pair ? w : 0)) * 128 + r;
+        const size_t slot = size_t((2 * int(blockIdx.x) + (seg_now == 0 ? 0 : 1)) * 2 + (s.pair ? w : 0));
         const float inv = whole ? (l_run == 0.f ? 0.f : 1.f / l_run) : 1.f;
         f0 = f0 == 0.f ? 0.f : f0 * inv;
         f1 *= inv;
         bf16* orow = p.out + ((size_t(s.b) * p.n + d) * p.QH + h) * kD;
-        if (alive && !whole) p.part_ml[slot] = make_float2(m_ref, l_run);
+        if (alive && !whole) p.part_ml[slot * 128 + r] = make_float2(m_ref, l_run);
 #pragma unroll 1
         for (int c = 0; c < kD / 32; ++c) {
           uint32_t o[32];
@@ -667,7 +665,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-              reinterpret_cast<uint4*>(p.part_o + slot * kD + c * 32)[k] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+              reinterpret_cast<uint4*>(p.part_o)[(slot * (kD / 4) + c * 8 + k) * 128 + r] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           }
         }
       }
@@ -680,14 +678,14 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         __threadfence();
         mbar_arrive(part_out);
         if (r == 0 && mbar_wait(part_out, parts & 1, abort_flag)) {
-          *is_last = atomicAdd(&p.arrived[combo], 1) == pc.count - 1;
+          *is_last = atomicAdd(&p.arrived[combo], 1) == pc.c1 - pc.c0;
           mbar_arrive(last_known);
         }
         if (!__all_sync(0xffffffffu, mbar_wait(last_known, parts & 1, abort_flag))) { ok = false; break; }
         ++parts;
         if (*is_last != 0) {
           __threadfence();
-          for (int row = q; row < live; row += 4) tree_join_row<kD>(p, s.b, s.kvh, 2 * s.rg, row, 0, pc, lane);
+          for (int i = r; i < live * (kD / 4); i += 128) tree_join_task<kD>(p, s.b, s.kvh, 2 * s.rg, 0, i % live, i / live, pc);
         }
       }
     }
@@ -704,16 +702,14 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   }
 }
 
-// Joins the pieces of every (sequence, KV head, row group) that was cut: grid (those, rows / 8), a warp a row.
+// Joins the pieces of every (sequence, KV head, row group) that was cut: grid (those, rows * D / 4 / 256), a thread four columns of a row.
 template <int kD>
 __global__ void __launch_bounds__(256)
 tree_join_kernel(const TreeParams p) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31;
   pdl_wait();
   pdl_trigger();
   const int per = p.KVH * p.groups, b = blockIdx.x / per, idx = blockIdx.x % per, kvh = idx / p.groups, rg = idx % p.groups;
-  const int row = blockIdx.y * 8 + warp, rows = p.tok * p.R, w = row >= rows ? 1 : 0, r = row - w * rows, rt = 2 * rg + w;
-  if (row >= 2 * rows || r >= min(p.n - rt * p.tok, p.tok) * p.R) return;
   unsigned long long sum = 0, before = 0;
   int nt = 0;
   for (int b0 = 0; b0 < p.B; b0 += 32) {
@@ -723,7 +719,10 @@ tree_join_kernel(const TreeParams p) {
     if (b >= b0 && b < b0 + 32) nt = __shfl_sync(0xffffffffu, v, b - b0);
   }
   const TreePieces pc = tree_pieces(p, sum * per, before * per + (unsigned long long)idx * nt, nt);
-  if (pc.c0 != pc.c1) tree_join_row<kD>(p, b, kvh, rt, r, w, pc, lane);
+  if (pc.c0 == pc.c1) return;
+  const int rows = p.tok * p.R, task = blockIdx.y * 256 + threadIdx.x, all = p.n > p.tok ? 2 * rows : rows, row = task % all, chunk = task / all;
+  const int w = row >= rows ? 1 : 0, r = row - w * rows, rt = 2 * rg + w;
+  if (chunk < kD / 4 && r < min(p.n - rt * p.tok, p.tok) * p.R) tree_join_task<kD>(p, b, kvh, rt, w, r, chunk, pc);
 }
 
 template <int kD, int kMod>
@@ -737,7 +736,7 @@ static int launch_tree(const TreeParams& p, const TensorMap& tq, const TensorMap
   B200_CHECK(launch_pdl(tree_append_kernel<kD>, dim3(unsigned((chunks + 255) / 256)), dim3(256), 0, st, 0, p));
   B200_CHECK(launch_pdl(tree_attn_kernel<kD, kMod>, dim3(p.ctas), dim3(TA_THREADS), TA<kD>::kSmem, st, 0, *tq, *tk, *tv, p));
   if (p.arrived != nullptr) return 0;
-  return static_cast<int>(launch_pdl(tree_join_kernel<kD>, dim3(p.B * p.KVH * p.groups, ((p.n > p.tok ? 2 : 1) * p.tok * p.R + 7) / 8), dim3(256), 0, st, 0, p));
+  return static_cast<int>(launch_pdl(tree_join_kernel<kD>, dim3(p.B * p.KVH * p.groups, ((p.n > p.tok ? 2 : 1) * p.tok * p.R * (kD / 4) + 255) / 256), dim3(256), 0, st, 0, p));
 }
 
 // Groups of two tiles of 128 / R drafts.
@@ -792,13 +791,13 @@ B200_API int b200_tree_attn_append(const void* kqv, void* kc, void* vc, void* ou
   p.tok = std::min(n, 128 / p.R);
   p.groups = tree_groups(n, p.R);
   p.ctas = tree_ctas(B, n, QH, KVH, Tmax);
-  p.part_o = static_cast<float*>(workspace);
-  p.part_ml = reinterpret_cast<float2*>(p.part_o + 4LL * p.ctas * 128 * D);
+  p.part_o = static_cast<float4*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + 4LL * p.ctas * 128 * (D / 4));
   p.q = reinterpret_cast<bf16*>(p.part_ml + 4LL * p.ctas * 128);
   // Few rows times few pieces: the CTA that finishes a (sequence, KV head) last joins its pieces, where a kernel of its own takes 3 to 5 us
   // more than that; more of them would keep that one SM busy for longer.
   const long long combos = (long long)B * KVH * p.groups;
-  p.arrived = n * p.R <= 64 && (p.ctas / combos + 2) * n * p.R <= 512
+  p.arrived = n * p.R <= 8 && (p.ctas / combos + 2) * n * p.R <= 512
                   ? reinterpret_cast<int*>(p.q + (size_t)B * n * QH * D) : nullptr;
   p.scale = scale;
   p.cap = make_score_cap(scale, cap);
