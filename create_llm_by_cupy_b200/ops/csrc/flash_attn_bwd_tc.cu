@@ -25,6 +25,9 @@
 // that GEMM are templates on the head dimension (128 or 64).
 //
 // Reference counterpart: cupy_flash_gqa_backward (model/flash_attention.py:109-176).
+#include <cooperative_groups.h>
+
+#include <algorithm>
 #include <mutex>
 #include <type_traits>
 
@@ -34,6 +37,7 @@
 #include "score_cap.cuh"
 
 namespace b200 {
+namespace cg = cooperative_groups;
 
 constexpr int FB_D = 128;
 constexpr int FBT_THREADS = 384;          // warps 0-3: producer / MMA / TMEM; warps 4-11: two math warpgroups
@@ -64,6 +68,7 @@ struct FlashBwdTcParams {
   const int2* ktab;      // [B, n_tiles]
   ScoreCap cap;          // kCap
   const float* slopes;   // kBias: [QH]
+  int split;             // CTAs of a cluster that share a key tile's query heads
 };
 
 // What was done to the scores, as in flash_attn_tc3.cu: the causal mask and the valid length alone; the spans' mask; that and a cap;
@@ -906,6 +911,110 @@ __device__ __forceinline__ void fb_ds_from_p_chunk(const uint32_t (&rp)[16], con
   }
 }
 
+// The accumulators of a cluster's CTAs, which hold the sums over their query heads, added up and stored: by every warp of every CTA.
+// dK and dV are two halves each (pairs of columns j and j + kD / 2, so that a rotation stays in one): with two CTAs each finishes a
+// matrix, with four a half, with three dK, a half of dV, the other. A CTA writes what it does not finish to the finisher's shared memory, where
+// Q and dO tiles were (between two barriers of the cluster), rows side by side; sums in the order of the CTAs behind the
+// finisher's own: no atomics, the same bits every time.
+template <int kD>
+__device__ __forceinline__ void dkv_cluster_sum(const FlashBwdTcParams& p, uint8_t* ring, uint32_t tmem_base, uint32_t col_dk, uint32_t col_dv,
+                                                int ntile, int kvh, int b, int rank, volatile int* abort_flag) {
+  constexpr int kN = kD / 8;                                  // columns of a run: a warpgroup has two runs of every half
+  constexpr int kRun = 128 * kN * 4, kHalf = 4 * kRun;        // bytes of a run of 128 rows, of a half
+  cg::cluster_group cluster = cg::this_cluster();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, q = warp & 3, wg = (warp - 4) >> 2, row = q * 32 + lane;
+  const int C = p.split;
+  const int2 met = p.ktab[size_t(b) * p.n_tiles + ntile];
+  const bool any = met.y > met.x;                             // the same for the whole cluster
+  auto owner = [&](int half) { return C == 2 ? half >> 1 : C == 4 ? half : max(half - 1, 0); };
+  auto place = [&](int half) { return C == 2 ? half & 1 : C == 3 && half == 1 ? 1 : 0; };      // among its finisher's halves
+  auto halves = [&](int r) { return C == 2 || (C == 3 && r == 0) ? 2 : 1; };
+  auto taddr = [&](int half, int run) {
+    return tmem_base + (uint32_t(q * 32) << 16) + (half < 2 ? col_dk : col_dv) + (half & 1) * (kD / 4) + wg * kN + run * (kD / 2);
+  };
+  auto load = [&](int half, int run, uint32_t (&v)[kN]) {
+    if constexpr (kN == 16) tmem_ld_32x32b_x16(taddr(half, run), v);
+    else tmem_ld_32x32b_x8(taddr(half, run), v);
+  };
+  tc_fence_before();
+  cluster.sync();                                             // every CTA's products are done, its ring is free
+  tc_fence_after();
+  if (warp >= 4 && any && *abort_flag == 0) {
+#pragma unroll 1
+    for (int half = 0; half < 4; ++half) {
+      const int to = owner(half);
+      if (to == rank) continue;
+      const int from = rank < to ? rank : rank - 1;           // this CTA among the finisher's others
+      uint8_t* dst = static_cast<uint8_t*>(cluster.map_shared_rank(ring, to)) + (from * halves(to) + place(half)) * kHalf + wg * 2 * kRun;
+#pragma unroll 1
+      for (int run = 0; run < 2; ++run) {
+        uint32_t v[kN];
+        load(half, run, v);
+        tmem_ld_wait();
+#pragma unroll
+        for (int c = 0; c < kN / 4; ++c)
+          reinterpret_cast<uint4*>(dst + run * kRun)[c * 128 + row] = make_uint4(v[4 * c], v[4 * c + 1], v[4 * c + 2], v[4 * c + 3]);
+      }
+    }
+  }
+  cluster.sync();                                             // what this CTA finishes is here
+  if (warp < 4 || *abort_flag != 0) return;
+  const int key = ntile * 128 + row;
+  const bool live = key < p.T;
+  const int pos = min(key, p.T - 1);
+#pragma unroll 1
+  for (int half = 0; half < 4; ++half) {
+    if (owner(half) != rank) continue;
+    float x[2][kN];
+#pragma unroll
+    for (int run = 0; run < 2; ++run) {
+      if (!any) {
+#pragma unroll
+        for (int e = 0; e < kN; ++e) x[run][e] = 0.f;
+        continue;
+      }
+      uint32_t v[kN];
+      load(half, run, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int e = 0; e < kN; ++e) x[run][e] = __uint_as_float(v[e]);
+      for (int o = 0; o < C - 1; ++o) {
+        const uint8_t* src = ring + (o * halves(rank) + place(half)) * kHalf + (wg * 2 + run) * kRun;
+#pragma unroll
+        for (int c = 0; c < kN / 4; ++c) {
+          const float4 y = reinterpret_cast<const float4*>(src)[c * 128 + row];
+          x[run][4 * c] += y.x;
+          x[run][4 * c + 1] += y.y;
+          x[run][4 * c + 2] += y.z;
+          x[run][4 * c + 3] += y.w;
+        }
+      }
+    }
+    const int j0 = (half & 1) * (kD / 4) + wg * kN;           // columns [j0, j0 + kN) and the same behind kD / 2
+    if (half < 2 && p.unrot_cos != nullptr) {
+#pragma unroll
+      for (int e = 0; e < kN; ++e) {
+        const float c = p.unrot_cos[size_t(j0 + e) * p.unrot_ld + pos], sn = p.unrot_sin[size_t(j0 + e) * p.unrot_ld + pos];
+        const float y1 = fmaf(x[0][e], c, x[1][e] * sn), y2 = fmaf(x[1][e], c, -x[0][e] * sn);
+        x[0][e] = y1;
+        x[1][e] = y2;
+      }
+    }
+    if (!live) continue;
+    bf16* out = half < 2 ? p.dk + b * p.dk_bs + (long long)key * p.dk_ts + kvh * p.dk_hs : p.dv + b * p.dv_bs + (long long)key * p.dv_ts + kvh * p.dv_hs;
+#pragma unroll
+    for (int run = 0; run < 2; ++run)
+#pragma unroll
+      for (int c = 0; c < kN / 8; ++c) {
+        uint4 u;
+        bf162* u2 = reinterpret_cast<bf162*>(&u);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) u2[e] = __floats2bfloat162_rn(x[run][8 * c + 2 * e], x[run][8 * c + 2 * e + 1]);
+        *reinterpret_cast<uint4*>(out + run * (kD / 2) + j0 + 8 * c) = u;
+      }
+  }
+}
+
 template <int kD, int kMod>
 __global__ void __launch_bounds__(FBT_THREADS, 1)
 flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmDO,
@@ -940,14 +1049,19 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
   {
     const int n_pairs = p.pairing ? (p.n_tiles + 1) / 2 : p.n_tiles;
     const int per_chunk = n_pairs * p.KVH * p.bchunk;
-    const int chunk = int(blockIdx.x) / per_chunk, r = int(blockIdx.x) - chunk * per_chunk;
+    const int unit = kMod == kCausal ? int(blockIdx.x) : int(blockIdx.x) / p.split;
+    const int chunk = unit / per_chunk, r = unit - chunk * per_chunk;
     const int hb = p.KVH * min(p.bchunk, p.B - chunk * p.bchunk);
     pair = r / hb;
     kvh = (r % hb) % p.KVH;
     b = chunk * p.bchunk + (r % hb) / p.KVH;
   }
   const int T = p.T;
-  const int R = p.QH / p.KVH;
+  // Spans: the CTAs of a cluster take a part of the query heads each
+  const int group = p.QH / p.KVH, rank = kMod == kCausal ? 0 : int(blockIdx.x) % p.split;
+  const int first = kMod == kCausal ? 0 : rank * group / p.split;
+  const int R = kMod == kCausal ? group : (rank + 1) * group / p.split - first;
+  const int h_first = kvh * group + first;
   const int tile_of_pass[2] = {pair, p.pairing ? p.n_tiles - 1 - pair : pair};
   int n_pass = tile_of_pass[0] == tile_of_pass[1] ? 1 : 2;
   // Known to be 1 or 2, this made a copy of every loop for each pass, and the second pass waited for its instructions to come
@@ -994,7 +1108,7 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
         if (kD == 128) tma_load_4d(smem + Smem::kK + 16384, &tmK, kv_full, 64, kvh, d.n0, b);
         tma_load_4d(smem + Smem::kV, &tmV, kv_full, 0, kvh, d.n0, b);
         if (kD == 128) tma_load_4d(smem + Smem::kV + 16384, &tmV, kv_full, 64, kvh, d.n0, b);
-        for (int it = 0, h = kvh * R, i = d.i_first; it < d.iters; ++it, ++g) {
+        for (int it = 0, h = h_first, i = d.i_first; it < d.iters; ++it, ++g) {
           const int s = g % kSt;
           const int m0 = i * FKW_BQ;
           if (!mbar_wait(&q_empty[s], ((g / kSt) & 1) ^ 1, abort_flag)) { ok = false; break; }
@@ -1016,7 +1130,7 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
 #pragma unroll 1
     for (int ps = 0; ps < n_pass && ok; ++ps) {
       const DkwPass d = dkw_pass<kMod>(tile_of_pass[ps], T, R, vlen, p, b);
-      for (int it = 0, h = kvh * R, i = d.i_first; it < d.iters; ++it, ++g) {
+      for (int it = 0, h = h_first, i = d.i_first; it < d.iters; ++it, ++g) {
         const int s = g % kSt;
         const int m0 = i * FKW_BQ;
         if (!mbar_wait(&q_empty[s], ((g / kSt) & 1) ^ 1, abort_flag)) { ok = false; break; }
@@ -1069,7 +1183,7 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
 #pragma unroll 1
       for (int ps = 0; ps < n_pass && ok; ++ps) {
         const DkwPass d = dkw_pass<kMod>(tile_of_pass[ps], T, R, vlen, p, b);
-        for (int it = 0, h = kvh * R, i = d.i_first; it < d.iters && ok; ++it, ++uses) {
+        for (int it = 0, h = h_first, i = d.i_first; it < d.iters && ok; ++it, ++uses) {
           const int m0 = i * FKW_BQ;
           for (int w = 0; w < 2; ++w) {
             if (!mbar_wait(&stg_full[w], uses & 1, abort_flag)) { ok = false; break; }
@@ -1179,7 +1293,7 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
       const int n0 = d.n0;
       const int key = n0 + q * 32 + lane;
       const bool key_dead = key >= vlen;
-      int h = kvh * R;                        // kBias: whose slope
+      int h = h_first;                        // kBias: whose slope
       float slope2 = kMod == kBias ? p.slopes[h] * kFbLog2e : 0.f;
       for (int it = 0, i = d.i_first; it < d.iters && ok; ++it) {
         const int g = g0 + it, s2 = g % kSt;
@@ -1274,6 +1388,10 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
       }
       if (!ok) break;
       g0 += d.iters;
+      if (kMod != kCausal && p.split > 1) {   // the cluster adds up its accumulators: below, by every warp of it
+        mbar_wait_warp(acc_done, ps & 1, abort_flag);
+        break;
+      }
       // End of the pass: the accumulators of this key tile are complete once every MMA has run. Each warp stores 32 rows:
       // head_dim 64: dK by warpgroup 0, dV by 1; 128: half of the columns of both by each.
       const int live = max(0, min(32, T - (n0 + q * 32))), pos = min(key, T - 1);
@@ -1307,6 +1425,9 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
     }
   }
 
+  if constexpr (kMod != kCausal) {
+    if (p.split > 1) dkv_cluster_sum<kD>(p, smem + Smem::kQ, tmem_base, kColDK, kColDV, tile_of_pass[0], kvh, b, rank, abort_flag);
+  }
   tc_fence_before();
   __syncthreads();
   if (warp == 2) {
@@ -1484,16 +1605,30 @@ B200_API int b200_flash_bwd_tc(const void* q, const void* k, const void* v, cons
   return 0;
 }
 
+static int g_span_split = 0;        // 0: by the number of key tiles; else forced where the heads allow it (A/B runs and tests)
+
+// CTAs of a cluster that share a key tile's query heads. What a key tile costs is a matter of the documents, which only the device
+// knows: a few long ones decide when the kernel ends, and where there are fewer tiles than SMs most stand idle. But every CTA has about
+// 10 us of its own (its first loads and scores, the cluster's sum). Forward and backward in us with 1 / 2 / 3 or 4 CTAs to a tile:
+// 24 tiles of 3 heads of 64 46 / 39 / 33, 84 of them 80 / 53 / 53, 256 of them 104 / 124 (uneven) / 136; 256 tiles of 4 heads of 128,
+// documents of about 600 tokens 340 / 288 / 325, one of 8192 1370 / 1331 / 1435.
+static int span_split(int group, long long tiles) {
+  const int most = group >= 4 ? 4 : group;
+  if (g_span_split > 0) return std::min(g_span_split, most);
+  if (tiles <= num_sms()) return most;
+  return tiles < 3LL * num_sms() && group % 2 == 0 ? 2 : 1;
+}
+
 template <int kD, int kMod>
-static int launch_dkv_span(const FlashBwdTcParams& p, const TensorMap (&m)[5], int ctas, cudaStream_t st) {
+static int launch_dkv_span(const FlashBwdTcParams& p, const TensorMap (&m)[5], int tiles, cudaStream_t st) {
   using Smem = FdkwSmem<kD, kMod>;
   static bool configured = false;
   if (!configured) {
     B200_CHECK(cudaFuncSetAttribute(flash_bwd_dkv_wide_kernel<kD, kMod>, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem::kTotal));
     configured = true;
   }
-  return static_cast<int>(launch_pdl(flash_bwd_dkv_wide_kernel<kD, kMod>, dim3(ctas), dim3(FBT_THREADS), Smem::kTotal, st, 0, *m[0],
-                                     *m[1], *m[2], *m[3], *m[4], p));
+  return static_cast<int>(launch_pdl(flash_bwd_dkv_wide_kernel<kD, kMod>, dim3(tiles * p.split), dim3(FBT_THREADS), Smem::kTotal, st,
+                                     p.split > 1 ? p.split : 0, *m[0], *m[1], *m[2], *m[3], *m[4], p));
 }
 
 // Gradients under a span mask (b200_span_mask), with the cap or the distance bias of b200_flash_fwd_span. Tensors, strides,
@@ -1542,15 +1677,25 @@ B200_API int b200_flash_bwd_span(const void* q, const void* k, const void* v, co
     const int bc = int(80.0e6 / (2.0 * T * D * (2.0 * QH + 2.0 * KVH)));       // as in b200_flash_bwd_tc
     p.bchunk = bc < 1 ? 1 : (bc > B ? B : bc);
   }
-  const int ctas = nt * KVH * B;                  // one key tile each: what a tile costs depends on the documents
+  const long long tiles = (long long)nt * KVH * B;
+  if (tiles > 0x1fffffffLL) return static_cast<int>(cudaErrorInvalidValue);
+  p.split = span_split(QH / KVH, tiles);
   int rc;
-  if (D == 64) rc = cap > 0.f ? launch_dkv_span<64, kCap>(p, maps, ctas, st)
-                    : slopes ? launch_dkv_span<64, kBias>(p, maps, ctas, st) : launch_dkv_span<64, kSpan>(p, maps, ctas, st);
-  else rc = cap > 0.f ? launch_dkv_span<128, kCap>(p, maps, ctas, st)
-            : slopes ? launch_dkv_span<128, kBias>(p, maps, ctas, st) : launch_dkv_span<128, kSpan>(p, maps, ctas, st);
+  if (D == 64) rc = cap > 0.f ? launch_dkv_span<64, kCap>(p, maps, int(tiles), st)
+                    : slopes ? launch_dkv_span<64, kBias>(p, maps, int(tiles), st) : launch_dkv_span<64, kSpan>(p, maps, int(tiles), st);
+  else rc = cap > 0.f ? launch_dkv_span<128, kCap>(p, maps, int(tiles), st)
+            : slopes ? launch_dkv_span<128, kBias>(p, maps, int(tiles), st) : launch_dkv_span<128, kSpan>(p, maps, int(tiles), st);
   if (rc != 0) return rc;
   return flash_bwd_dq_from_ds(ds_ws, k, dq, nullptr, s + 3, s + 12, B, T, QH, KVH, D, p.bchunk, p.unrot_cos, p.unrot_sin, p.unrot_ld,
                               st, static_cast<const int4*>(qtab));
+}
+
+// CTAs that share a key tile's query heads in the dK/dV kernel under a span mask: 0 (default) by the number of key tiles, else up to that
+// many (1 to 4). Returns the previous value; a negative argument only reads it.
+B200_API int b200_flash_span_split(int n) {
+  const int old = g_span_split;
+  if (n >= 0) g_span_split = n > 4 ? 4 : n;
+  return old;
 }
 
 // 1 (default): head_dim 128 runs the dK/dV kernel with 128-query iterations (flash_bwd_dkv_wide_kernel); 0: the
