@@ -18,6 +18,7 @@ import math
 import torch
 
 from ..ops import functional as F
+from ..ops import masked_attn as A
 
 
 def init_weight(shape, std: float, dtype, device, generator=None) -> torch.Tensor:
@@ -82,11 +83,16 @@ class GroupedQueryAttention:
 
     params: ``W_KQV [H, KVH*D + H + KVH*D]`` (column order K, Q, V) and ``W_O [H, H]``, both
     ``[in, out]`` as in the reference (model/fast_layers.py:101-105).
+
+    ``valid_len`` of the passes is one length per row, or a ``masked_attn.SpanMask`` of packed documents. ``softcap`` > 0 caps the
+    scores (c tanh(s / c)), in training, prefill and decoding. Both run on the span kernels, which know no dropout on the
+    probabilities.
     """
 
     def __init__(self, hidden_size, time_size, q_head, kv_head, layer_num, dropout_rate=0.0,
-                 dtype=torch.bfloat16, device="cpu", generator=None, init_std=None, rope_base=10000.0):
+                 dtype=torch.bfloat16, device="cpu", generator=None, init_std=None, rope_base=10000.0, softcap=0.0):
         assert hidden_size % q_head == 0 and q_head % kv_head == 0
+        self.softcap = float(softcap)
         self.H, self.T = hidden_size, time_size
         self.QH, self.KVH = q_head, kv_head
         self.D = hidden_size // q_head
@@ -112,6 +118,7 @@ class GroupedQueryAttention:
         self.drop_attn = TimeDropout(dropout_rate, dtype, generator) if dropout_rate else None
         self.drop = TimeDropout(dropout_rate, dtype, generator) if dropout_rate else None
         self._dense = False              # the pass in flight runs the dense attention path
+        self._mask = None                # SpanMask of the pass in flight
 
     # -- helpers ---------------------------------------------------------------------------
     def _split(self, kqv: torch.Tensor, B: int, T: int):
@@ -125,7 +132,13 @@ class GroupedQueryAttention:
         take Q and K already rotated: the rotary embedding is then applied in place to the [K|Q] columns of
         the packed projection (one pass over 5/6 of it) and undone on d[K|Q] in the epilogues of the
         backward kernels (head_dim 128) or by a pass after them."""
-        return x.is_cuda and not self._dense and F.flash_tc_forward_dim(self.D)
+        return self._mask is not None or (x.is_cuda and not self._dense and F.flash_tc_forward_dim(self.D))
+
+    def _span_mask(self, valid_len, B, T, device):
+        """The span mask that the pass runs under; None: the plain causal kernels do."""
+        if isinstance(valid_len, A.SpanMask):
+            return valid_len
+        return A.span_mask(B, T, device, valid_len=valid_len) if self.softcap > 0.0 else None
 
     def _project(self, x, T, tabs, first: bool):
         """K | Q | V projection; on the pre-rotating path K and Q leave it rotated - inside the GEMM's epilogue
@@ -141,6 +154,11 @@ class GroupedQueryAttention:
         return kqv
 
     def _attend(self, q, k, v, valid_len, tabs, train_flg: bool = False):
+        if self._mask is not None:
+            if not self._dense:
+                return A.span_attn_fwd(q, k, v, self._mask, scale=self.scale, softcap=self.softcap)
+            o, lse, _, _ = A._span_reference(q, k, v, self._mask, self.scale, self.softcap, None)
+            return o.to(q.dtype).contiguous(), lse
         if self._dense:
             o, lse, p, _, _ = F._attn_reference(q, k, v, valid_len, self.scale, tabs[0], tabs[1])
             if self.drop_attn is not None and train_flg:
@@ -157,6 +175,12 @@ class GroupedQueryAttention:
         """x: normed input [M, H]. Returns W_O(attn) (+ residual) as [M, H]."""
         tabs = self._rope(T, x.device)
         self._dense = self.flash_backend == "none" or (self.drop_attn is not None and train_flg)
+        self._mask = self._span_mask(valid_len, B, T, x.device)
+        if self._mask is not None:
+            if self.drop_attn is not None and train_flg:
+                raise ValueError("GroupedQueryAttention: dropout on the attention probabilities goes with neither span masks nor "
+                                 "capped scores")
+            valid_len = self._mask
         kqv = self._project(x, T, tabs, True)
         q, k, v = self._split(kqv, B, T)
         o, lse = self._attend(q, k, v, valid_len, tabs, train_flg)
@@ -174,6 +198,7 @@ class GroupedQueryAttention:
 
     def backward(self, dout: torch.Tensor, grad_out=None) -> torch.Tensor:
         x, B, T, valid_len, kqv, o, lse = self.cache
+        self._mask = valid_len if isinstance(valid_len, A.SpanMask) else None
         if self.drop is not None:
             dout = self.drop.backward(dout)
         tabs = self._rope(T, x.device)
@@ -197,7 +222,14 @@ class GroupedQueryAttention:
             do = F.gemm(dout, self.params[1], trans_b=True)
         dkqv = torch.empty_like(kqv)
         dq, dk, dv = self._split(dkqv, B, T)
-        if self._dense:
+        if self._mask is not None:
+            do = do.view(B, T, self.QH, self.D)
+            if self._dense:
+                A._span_bwd_reference(do, q, k, v, o, self._mask, self.scale, self.softcap, None, (dq, dk, dv), tabs)
+            else:
+                A.span_attn_bwd(do, q, k, v, o, lse, self._mask, scale=self.scale, softcap=self.softcap, out=(dq, dk, dv), unrotate=tabs,
+                                delta=delta)
+        elif self._dense:
             # dense path (verification, or training with attention dropout): the fp32 restatement, on the
             # device the tensors live on
             F._attn_bwd_reference(do.view(B, T, self.QH, self.D), q, k, v, o, valid_len, self.scale, tabs[0], tabs[1],
@@ -228,7 +260,9 @@ class GroupedQueryAttention:
         q, k, v = self._split(kqv, B, T)
         kcache[:, :, :T].copy_(k.permute(0, 2, 1, 3))
         vcache[:, :, :T].copy_(v.permute(0, 2, 1, 3))
-        if self.flash_backend == "none":
+        if self.softcap > 0.0:
+            o, _ = A.span_attn_fwd(q, k, v, A.span_mask(B, T, x.device), scale=self.scale, softcap=self.softcap)
+        elif self.flash_backend == "none":
             o, _, _, _, _ = F._attn_reference(q, k, v, None, self.scale, None, None)
             o = o.to(x.dtype).contiguous()
         else:
@@ -239,6 +273,9 @@ class GroupedQueryAttention:
         """x: [B, H] normed hidden state of the token at position ``pos`` (same for the batch)."""
         B = x.shape[0]
         tabs = self._rope(kcache.shape[2], x.device)
+        if self.softcap > 0.0:
+            one = torch.ones((B, 1), dtype=torch.int64, device=x.device)
+            return self.decode_drafts(x, one, kcache, vcache, lens - 1, residual)
         out = F.decode_attn_block(x, self.params[0], self.params[1], kcache, vcache, lens, pos, self.QH, self.KVH,
                                   tabs[0], tabs[1], self.scale, residual)
         if out is not None:
@@ -256,6 +293,14 @@ class GroupedQueryAttention:
         vcache[:, :, pos].copy_(v)
         o = F.decode_attn(q.contiguous(), kcache, vcache, lens, self.scale)
         return F.gemm(o.view(B, self.H), self.params[1], add=residual)
+
+    def decode_drafts(self, x, tree, kcache, vcache, lens, residual=None):
+        """x: [B * n, H] normed hidden states of ``n`` drafted tokens per sequence, ``tree`` [B, n] whom each of them sees
+        (``masked_attn.tree_mask``), ``lens`` [B] cached tokens. Their K and V are appended to the caches."""
+        tabs = self._rope(kcache.shape[2], x.device)
+        o = A.tree_attn_append(F.gemm(x, self.params[0]), kcache, vcache, lens, tree, self.QH, self.KVH, tabs[0], tabs[1], scale=self.scale,
+                               softcap=self.softcap)
+        return F.gemm(o.view(x.shape[0], self.H), self.params[1], add=residual)
 
     @staticmethod
     def convert_legacy_weights(W_K, W_Q, W_V, W_O):

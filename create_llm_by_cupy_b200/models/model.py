@@ -22,6 +22,7 @@ import numpy as np
 import torch
 
 from ..ops import functional as F
+from ..ops.masked_attn import SpanMask, span_mask, tree_mask
 from .layers import (ChunkedCrossEntropy_Share, GroupedQueryAttention, RMSNorm, SwiGLU, TimeDropout,
                      TimeEmbedding_shard, init_weight)
 from .sampling import apply_repetition_penalty, top_p_sampling
@@ -119,6 +120,7 @@ class Cupa_ver4:
         self.ffn_size = d.get("ffn_size")
         self.tie_embeddings = bool(d.get("tie_embeddings", True))
         self.rope_base = float(d.get("rope_base", 10000.0))
+        self.attn_softcap = float(d.get("attn_softcap", 0.0))
         self.init_std = d.get("init_std")
         self.seed = int(d.get("seed", 0))
         if device is None:
@@ -165,7 +167,7 @@ class Cupa_ver4:
             self.dropout_ = TimeDropout(self.dropout_rate, self.dtype)
         for _ in range(self.layernum):
             gqa = GroupedQueryAttention(self.hidden_size, self.time_size, self.q_head, self.kv_head, self.layernum,
-                                        self.dropout_rate, rope_base=self.rope_base, **kw)
+                                        self.dropout_rate, rope_base=self.rope_base, softcap=self.attn_softcap, **kw)
             feed = SwiGLU(self.hidden_size, self.layernum, dropout_rate=self.dropout_rate, ffn_size=self.ffn_size, **kw)
             norm1 = RMSNorm(self.hidden_size, self.dtype, self.device)
             norm2 = RMSNorm(self.hidden_size, self.dtype, self.device)
@@ -299,14 +301,17 @@ class Cupa_ver4:
 
     def forward(self, x, t, x_pa=None, manager=None, train_flg: bool = True):
         """x, t: int token ids [B, T]; x_pa: int32 [B] valid key length per sequence (keys at
-        positions >= x_pa are masked) or None. Returns the mean CE loss as a device scalar."""
+        positions >= x_pa are masked), a ``masked_attn.SpanMask`` of the documents that are packed into the rows, or None.
+        Returns the mean CE loss as a device scalar."""
         manager = manager if manager is not None else self._local_manager()
         self._manager = manager
         manager.phase = "fwd"
         self.grads = []
         B, T = x.shape
         self._BT = (B, T)
-        valid_len = None if x_pa is None else x_pa.to(torch.int32)
+        valid_len = x_pa if x_pa is None or isinstance(x_pa, SpanMask) else x_pa.to(torch.int32)
+        if self.attn_softcap > 0.0 and not isinstance(valid_len, SpanMask):
+            valid_len = span_mask(B, T, x.device, valid_len=valid_len)           # one for all layers
 
         W = manager.gather_embedding()
         h = self.embed.forward(W, x, train_flg)
@@ -437,12 +442,13 @@ class Cupa_ver4:
         """Full-sequence fp32 logits [B, T, V] (no cache); for tests and scoring."""
         manager = manager if manager is not None else self._local_manager()
         B, T = x.shape
+        mask = span_mask(B, T, x.device) if self.attn_softcap > 0.0 else None
         W = manager.gather_embedding()
         h = self.embed.forward(W, x, False)
         for b in range(self.layernum):
             gqa, feed, norm1, norm2 = self.block_modules(b)
             manager.gather_modules([gqa, feed, norm1, norm2])
-            h = gqa.forward(norm1.forward(h, False), B, T, None, residual=h, train_flg=False)
+            h = gqa.forward(norm1.forward(h, False), B, T, mask, residual=h, train_flg=False)
             h = feed.forward(norm2.forward(h, False), residual=h, train_flg=False)
             manager.release_modules([gqa, feed, norm1, norm2])
         manager.gather_module(self.norm_)
@@ -511,6 +517,70 @@ class Cupa_ver4:
                 h = gqa.decode_step(norm1.forward(h, False), pos, kc[b], vc[b], lens, residual=h)
                 h = feed.forward(norm2.forward(h, False), residual=h, train_flg=False)
             h_last = self.norm_.forward(h, False)
+        return out
+
+    @torch.no_grad()
+    def generate_drafted(self, prompt, draft, start_id=None, end_id=None, padding_id=None, max_new_tokens: int | None = None):
+        """Greedy decoding that checks a tree of drafted tokens per pass: the same choices as ``generate(..., greedy=True)``, in as many
+        passes as the drafts are wrong. ``draft(tokens)`` gets all tokens so far and returns proposals for those that follow as
+        (token, parent) pairs, at most 63: ``parent`` is the index of an earlier proposal of the same list, or -1 for the last token. A
+        drafted token whose predecessors were all chosen, and which the model chooses, is kept with its cached K and V."""
+        pad = self.padding_id if padding_id is None else padding_id
+        toks = ([int(start_id)] if start_id is not None else []) + [int(p) for p in prompt]
+        if not toks:
+            raise ValueError("generate_drafted needs at least one token of context")
+        Tmax = self.time_size
+        toks = toks[:Tmax - 1]
+        budget = Tmax - len(toks) if max_new_tokens is None else min(max_new_tokens, Tmax - len(toks))
+        dev, dt = self.device, self.dtype
+        kc = [torch.zeros((1, self.kv_head, Tmax, self.head_dim), dtype=dt, device=dev) for _ in range(self.layernum)]
+        vc = [torch.zeros_like(kc[0]) for _ in range(self.layernum)]
+        W = self.Af_Em_para[0]
+        Wh = self.head_para[0] if self.head_para is not None else W
+
+        def choose(h):
+            logits = F.gemm(self.norm_.forward(h, False), Wh, trans_b=True, out_dtype=torch.float32)
+            if 0 <= pad < self.vocab_size:
+                logits[:, pad] = float("-inf")
+            return torch.argmax(logits, -1).tolist()
+
+        h = F.embedding_fwd(W, torch.tensor(toks, dtype=torch.int32, device=dev), -1)
+        for b in range(self.layernum):
+            gqa, feed, norm1, norm2 = self.block_modules(b)
+            h = gqa.prefill(norm1.forward(h, False), 1, len(toks), kc[b], vc[b], residual=h)
+            h = feed.forward(norm2.forward(h, False), residual=h, train_flg=False)
+        out, cached = [], len(toks)
+        if budget > 0:
+            out.append(choose(h[-1:])[0])
+        while 0 < len(out) < budget and (end_id is None or out[-1] != end_id) and cached < Tmax - 1:
+            room = min(64, Tmax - cached)
+            proposals = [(int(t), int(p)) for t, p in list(draft(toks + out))[:room - 1]]
+            if any(not -1 <= p < i for i, (_, p) in enumerate(proposals)):
+                raise ValueError("generate_drafted: a proposal's parent stands before it, or is -1")
+            ids = [out[-1]] + [t for t, _ in proposals]                          # the last token, which is not cached yet, is the root
+            parents = [-1] + [p + 1 for _, p in proposals]
+            h = F.embedding_fwd(W, torch.tensor(ids, dtype=torch.int32, device=dev), -1)
+            tree, lens = tree_mask([parents], dev), torch.tensor([cached], dtype=torch.int32, device=dev)
+            for b in range(self.layernum):
+                gqa, feed, norm1, norm2 = self.block_modules(b)
+                h = gqa.decode_drafts(norm1.forward(h, False), tree, kc[b], vc[b], lens, residual=h)
+                h = feed.forward(norm2.forward(h, False), residual=h, train_flg=False)
+            best, path = choose(h), [0]
+            while True:                                                          # down the tree as far as the drafts are right
+                out.append(best[path[-1]])
+                if len(out) >= budget or (end_id is not None and out[-1] == end_id):
+                    break
+                child = next((i for i in range(1, len(ids)) if parents[i] == path[-1] and ids[i] == out[-1]), None)
+                if child is None:
+                    break
+                path.append(child)
+            moved = [i for j, i in enumerate(path) if i != j]
+            if moved:                                                            # their rows to where the tokens stand now
+                src = torch.tensor([cached + i for i in moved], device=dev)
+                at = cached + len(path) - len(moved)
+                for c in kc + vc:
+                    c[:, :, at:at + len(moved)] = c[:, :, src]
+            cached += len(path)
         return out
 
     def chat_generate(self, prompt, user_id, bot_id, end_id, padding_id=None, **kw):

@@ -242,12 +242,13 @@ def span_attn_fwd(q, k, v, mask: SpanMask, *, scale: float | None = None, softca
 
 
 def span_attn_bwd(dout, q, k, v, o, lse, mask: SpanMask, *, scale: float | None = None, softcap: float = 0.0, slopes=None, out=None,
-                  unrotate=None):
+                  unrotate=None, delta=None):
     """Gradients (dq, dk, dv) of ``span_attn_fwd`` with its results ``o``, ``lse``. ``out``: three [B, T, heads, D] views to
-    write into; ``unrotate`` = (cos, sin) tables [>= T, D / 2]: dq and dk leave as gradients of the un-rotated q and k. The
+    write into; ``unrotate`` = (cos, sin) tables [>= T, D / 2]: dq and dk leave as gradients of the un-rotated q and k; ``delta``
+    [B, QH, T] fp32, sum over D of dout * o, where the caller has it (``gemm.gemm_delta``). The
     kernels keep dS^T of as many batch elements or KV heads at a time as ``functional.FLASH_DQ_GEMM_MAX_BYTES`` holds, of one KV
     head at least. Deterministic: no atomics."""
-    if native.host is not None and type(mask) is SpanMask and out is None and unrotate is None:
+    if native.host is not None and type(mask) is SpanMask and out is None and unrotate is None and delta is None:
         r = native.host.span_bwd(dout, q, k, v, o, lse, mask.buf, mask.B, mask.T, 0.0 if scale is None else scale or -1.0, softcap, slopes,
                                  F.FLASH_DQ_GEMM_MAX_BYTES)
         if r is not None:
@@ -284,8 +285,10 @@ def span_attn_bwd(dout, q, k, v, o, lse, mask: SpanMask, *, scale: float | None 
             raise ValueError("span_attn_bwd: out needs rows on 16-byte boundaries")
     if B == 0 or T == 0:
         return dq, dk, dv
-    delta = torch.empty((B, QH, T), dtype=torch.float32, device=q.device)
-    F.flash_delta(o, dout, delta)
+    if delta is None:
+        delta = F.flash_delta(o, dout, torch.empty((B, QH, T), dtype=torch.float32, device=q.device))
+    elif tuple(delta.shape) != (B, QH, T) or delta.dtype != torch.float32 or not delta.is_contiguous():
+        raise ValueError("span_attn_bwd: delta is float32 [B, query heads, T], contiguous")
     ucos = usin = None
     if unrotate is not None:
         from .gemm import rope_tables_transposed
@@ -462,4 +465,4 @@ def _tree_reference(kqv, kcache, vcache, lens, tree, QH, KVH, cos, sin, scale, s
     kc, vc = (torch.where(used, x.to(dt), torch.zeros((), dtype=dt, device=x.device)).transpose(1, 2) for x in (kcache, vcache))
     x, _ = _scores_reference(q, kc, seen, scale, softcap, slopes, dist)
     p, _ = _softmax_reference(x)
-    return torch.einsum("bhts,bshd->bthd", p, vc.repeat_interleave(QH // KVH, dim=2)).to(kqv.dtype)
+    return torch.einsum("bhts,bshd->bthd", p, vc.repeat_interleave(QH // KVH, dim=2)).to(kqv.dtype).contiguous()

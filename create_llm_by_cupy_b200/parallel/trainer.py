@@ -168,7 +168,10 @@ class Trainer:
         """Returns (loss, stats, step_scale) device tensors of a replayed step, or None when this step
         has to run eagerly (warm-up steps, a batch of another shape)."""
         from ..ops import native
+        from ..ops.masked_attn import SpanMask
         x, t, x_pa = batches[0]
+        if isinstance(x_pa, SpanMask):        # its documents are another step's shapes of work: run eagerly
+            return None
         if self._graph is None:
             if self._graph_warm < 2:          # lazy one-time set-up (tensor maps, attributes, streams) happens eagerly
                 self._graph_warm += 1
