@@ -52,12 +52,12 @@ struct Api {
   int (*decode_attn_block)(cptr, cptr, cptr, cptr, void*, void*, void*, void*, void*, cptr, cptr, cptr, int, int, int, int,
                            int, int, int, int, int, float, stream_t);
   int (*mlp_few_rows)(cptr, cptr, cptr, cptr, void*, void*, int, int, int, int, int, stream_t);
-  int (*span_mask)(cptr, cptr, cptr, cptr, cptr, void*, void*, void*, int, int, stream_t);
-  int (*flash_fwd_span)(cptr, cptr, cptr, void*, void*, cptr, cptr, const long long*, int, int, int, int, int, float, float, cptr,
+  int (*span_mask)(cptr, cptr, cptr, cptr, cptr, void*, void*, void*, void*, int, int, stream_t);
+  int (*flash_fwd_span)(cptr, cptr, cptr, void*, void*, cptr, cptr, cptr, const long long*, int, int, int, int, int, float, float, cptr,
                         stream_t);
   int (*flash_delta)(cptr, cptr, void*, const long long*, int, int, int, int, stream_t);
-  int (*flash_bwd_span)(cptr, cptr, cptr, cptr, cptr, cptr, void*, void*, void*, cptr, cptr, cptr, const long long*, int, int, int, int,
-                        int, float, float, cptr, void*, cptr, cptr, int, stream_t);
+  int (*flash_bwd_span)(cptr, cptr, cptr, cptr, cptr, cptr, void*, void*, void*, cptr, cptr, cptr, cptr, cptr, const long long*, int, int,
+                        int, int, int, float, float, cptr, void*, cptr, cptr, int, stream_t);
   long long (*tree_attn_workspace)(int, int, int, int, int, int);
   int (*tree_attn_append)(cptr, void*, void*, void*, cptr, cptr, cptr, cptr, cptr, void*, int, int, int, int, int, int, int, long long,
                           float, float, stream_t);
@@ -452,18 +452,25 @@ PyObject* mlp_few_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END
 }
 
-// The tables of a span mask in its buffer (see ``masked_attn._make_mask``): of query tiles, of key tiles, the spans themselves.
+// The tables of a span mask in its buffer (see ``masked_attn.SpanMask``): of query tiles, of key tiles, the spans themselves, the orders of
+// query tiles, of pairs of them, of key tiles.
 struct SpanTables {
   int* qtab;
   int* ktab;
   int* spans;
+  int* order_q;
+  int* order_k;
 };
 SpanTables span_tables(const Tensor& buf, int64_t B, int64_t T) {
   int* p = static_cast<int*>(const_cast<void*>(buf.const_data_ptr()));
   const int64_t nt = (T + 127) / 128;
-  return {p, p + 4 * B * nt, p + 6 * B * nt};
+  int* order = p + B * (6 * nt + 2 * T);
+  return {p, p + 4 * B * nt, p + 6 * B * nt, order, order + B * (nt + (nt + 1) / 2)};
 }
-int64_t span_ints(int64_t B, int64_t T) { return B * (6 * ((T + 127) / 128) + 2 * T); }
+int64_t span_ints(int64_t B, int64_t T) {
+  const int64_t nt = (T + 127) / 128;
+  return B * (8 * nt + (nt + 1) / 2 + 2 * T);
+}
 
 // span_mask(B, T, docs or None, prefix or None, valid_len or None) -> the mask's buffer
 PyObject* span_mask(PyObject*, PyObject* const* a, Py_ssize_t n) {
@@ -471,7 +478,7 @@ PyObject* span_mask(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const int64_t B = as_int(a[0]), T = as_int(a[1]);
   const Tensor *docs, *prefix, *vl;
   CHECK_NUMBERS
-  if (!optional(a[2], &docs) || !optional(a[3], &prefix) || !optional(a[4], &vl) || B <= 0 || T <= 0 || T > 720896) Py_RETURN_NONE;
+  if (!optional(a[2], &docs) || !optional(a[3], &prefix) || !optional(a[4], &vl) || B <= 0 || T <= 0 || T > 512000) Py_RETURN_NONE;
   const Tensor* like = docs ? docs : prefix ? prefix : vl;
   if (!like) Py_RETURN_NONE;
   auto rows = [&](const Tensor* t, at::ScalarType dt) {
@@ -483,7 +490,7 @@ PyObject* span_mask(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const SpanTables t = span_tables(buf, B, T);
   if (launched([&] {
         return api.span_mask(docs ? docs->const_data_ptr() : nullptr, prefix ? prefix->const_data_ptr() : nullptr,
-                             vl ? vl->const_data_ptr() : nullptr, nullptr, nullptr, t.spans, t.qtab, t.ktab, int(B), int(T), stream(dev));
+                             vl ? vl->const_data_ptr() : nullptr, nullptr, nullptr, t.spans, t.qtab, t.ktab, t.order_q, int(B), int(T), stream(dev));
       }))
     return wrap(buf);
   END
@@ -509,7 +516,7 @@ bool span_heads(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor&
 // (batch, token, head) strides; of a dimension of one, which is never stepped along, one that a tile copy can have
 void put_strides(long long* st, std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
-    for (int d = 0; d < 3; ++d) *st++ = t->size(d) > 1 ? t->stride(d) : 8;
+    for (int d = 0; d < 3; ++d) *st++ = t->size(d) > 1 ? t->stride(d) : 16;
 }
 // Scale (0: of the head dimension) and cap as the front ends take them; the others are theirs to refuse.
 bool score_numbers(float* scale, float cap, const Tensor* slopes, int64_t D) {
@@ -534,7 +541,7 @@ PyObject* span_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const SpanTables t = span_tables(*buf, B, T);
   if (launched([&] {
         return api.flash_fwd_span(q->const_data_ptr(), k->const_data_ptr(), v->const_data_ptr(), o.mutable_data_ptr(),
-                                  lse.mutable_data_ptr(), t.spans, t.qtab, st, int(B), int(T), int(QH), int(KVH), int(D), scale, cap,
+                                  lse.mutable_data_ptr(), t.spans, t.qtab, t.order_q, st, int(B), int(T), int(QH), int(KVH), int(D), scale, cap,
                                   sl ? sl->const_data_ptr() : nullptr, stream(dev));
       }))
     return wrap2(o, lse);
@@ -577,7 +584,7 @@ PyObject* span_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (rc != 0) return rc;
         return api.flash_bwd_span(q->const_data_ptr(), k->const_data_ptr(), v->const_data_ptr(), dout->const_data_ptr(),
                                   lse->const_data_ptr(), delta.const_data_ptr(), dq.mutable_data_ptr(), dk.mutable_data_ptr(),
-                                  dv.mutable_data_ptr(), t.spans, t.qtab, t.ktab, st, int(B), int(T), int(QH), int(KVH), int(D), scale, cap,
+                                  dv.mutable_data_ptr(), t.spans, t.qtab, t.ktab, t.order_k, t.order_q, st, int(B), int(T), int(QH), int(KVH), int(D), scale, cap,
                                   sl ? sl->const_data_ptr() : nullptr, ws.mutable_data_ptr(), nullptr, nullptr, 0, stream(dev));
       }))
     Py_RETURN_NONE;

@@ -40,6 +40,7 @@ struct DqGemmParams {
   int unrot_ld;
   int* status;
   const int4* qtab;      // spans (see span_mask.cu): the key tiles of each query tile, [B, n_tiles]
+  const int* order_q;    // spans: query tiles, those with most keys first, [B, n_tiles]
 };
 
 struct DqGemmSmem {
@@ -74,7 +75,6 @@ flash_bwd_dq_gemm_kernel(const __grid_constant__ CUtensorMap tmDS, const __grid_
     b = chunk * p.bchunk + (r % hb) / p.QH;
   }
   const int kvh = h / (p.QH / p.KVH);
-  const int m0 = mtile * 128;
   const int T = p.T;
 
   if (threadIdx.x == 0) {
@@ -99,6 +99,7 @@ flash_bwd_dq_gemm_kernel(const __grid_constant__ CUtensorMap tmDS, const __grid_
   // 64-key steps: everything up to the end of the diagonal tile, cut at the valid length
   int key0 = 0, n_tiles;
   if constexpr (kSpans) {
+    mtile = p.order_q[size_t(b) * p.n_tiles + p.n_tiles - 1 - mtile];
     const int4 r = p.qtab[size_t(b) * p.n_tiles + mtile];
     key0 = r.x * 128;
     n_tiles = 2 * (r.y - r.x);           // 0: no row of the tile sees a key, and dQ is zero
@@ -106,6 +107,8 @@ flash_bwd_dq_gemm_kernel(const __grid_constant__ CUtensorMap tmDS, const __grid_
     const int vlen = p.valid_len ? checked_index(p.valid_len[b], T, p.status, 303) : T;
     n_tiles = min(2 * (mtile + 1), (max(vlen, 1) + DQG_KEYS - 1) / DQG_KEYS);
   }
+
+  const int m0 = mtile * 128;
 
   if (warp == 0) {
     if (lane == 0) {
@@ -192,7 +195,8 @@ flash_bwd_dq_gemm_kernel(const __grid_constant__ CUtensorMap tmDS, const __grid_
 // 128) times K. Strides in elements: k (batch, token, head), dq (batch, token, head).
 int flash_bwd_dq_from_ds(const void* ds, const void* k, void* dq, const void* valid_len, const long long* ks,
                          const long long* dqs, int B, int T, int QH, int KVH, int D, int bchunk,
-                         const float* unrot_cos, const float* unrot_sin, int unrot_ld, cudaStream_t st, const int4* qtab) {
+                         const float* unrot_cos, const float* unrot_sin, int unrot_ld, cudaStream_t st, const int4* qtab,
+                         const int* order_q) {
   if (D != 128 && D != 64) return static_cast<int>(cudaErrorInvalidValue);
   const int nt = (T + 127) / 128;
   const unsigned long long Tp = (unsigned long long)nt * 128;
@@ -208,6 +212,7 @@ int flash_bwd_dq_from_ds(const void* ds, const void* k, void* dq, const void* va
   p.unrot_cos = unrot_cos; p.unrot_sin = unrot_sin; p.unrot_ld = unrot_ld;
   p.status = status_ptr();
   p.qtab = qtab;
+  p.order_q = order_q;
   static bool configured = false;
   if (!configured) {
     for (auto* kern : {flash_bwd_dq_gemm_kernel<128, false>, flash_bwd_dq_gemm_kernel<64, false>, flash_bwd_dq_gemm_kernel<128, true>,

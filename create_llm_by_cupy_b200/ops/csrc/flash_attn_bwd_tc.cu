@@ -66,6 +66,7 @@ struct FlashBwdTcParams {
   // spans (flash_bwd_dkv_wide_kernel with kMod >= 0; see span_mask.cu)
   const int2* spans;     // [B, T]
   const int2* ktab;      // [B, n_tiles]
+  const int* order_k;    // [B, n_tiles]: key tiles, those with most to do first
   ScoreCap cap;          // kCap
   const float* slopes;   // kBias: [QH]
   int split;             // CTAs of a cluster that share a key tile's query heads
@@ -1062,7 +1063,7 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
   const int first = kMod == kCausal ? 0 : rank * group / p.split;
   const int R = kMod == kCausal ? group : (rank + 1) * group / p.split - first;
   const int h_first = kvh * group + first;
-  const int tile_of_pass[2] = {pair, p.pairing ? p.n_tiles - 1 - pair : pair};
+  int tile_of_pass[2] = {pair, p.pairing ? p.n_tiles - 1 - pair : pair};
   int n_pass = tile_of_pass[0] == tile_of_pass[1] ? 1 : 2;
   // Known to be 1 or 2, this made a copy of every loop for each pass, and the second pass waited for its instructions to come
   // from memory: 11000 to 19000 clocks for its first iteration where the others take 3000.
@@ -1090,6 +1091,7 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
   const uint32_t tmem_base = *tmem_slot;
   pdl_wait();                            // by every role: their bounded waits start counting behind it
   const int vlen = p.valid_len ? checked_index(p.valid_len[b], T, p.status, 302) : T;
+  if constexpr (kMod != kCausal) tile_of_pass[0] = tile_of_pass[1] = p.order_k[size_t(b) * p.n_tiles + pair];
   constexpr uint32_t kColST = 0, kColDPT = 128, kColDV = 256, kColDK = 256 + kD;
 
   if (warp == 0) {
@@ -1462,7 +1464,7 @@ static SideStream* side_stream() {
 int flash_bwd_dq_from_ds(const void* ds, const void* k, void* dq, const void* valid_len, const long long* ks,
                          const long long* dqs, int B, int T, int QH, int KVH, int D, int bchunk,
                          const float* unrot_cos, const float* unrot_sin, int unrot_ld, cudaStream_t st,
-                         const int4* qtab = nullptr);
+                         const int4* qtab = nullptr, const int* order_q = nullptr);
 
 static int g_dkv_wide = 1;
 
@@ -1635,8 +1637,8 @@ static int launch_dkv_span(const FlashBwdTcParams& p, const TensorMap (&m)[5], i
 // workspace (not optional) and rotary tables as in b200_flash_bwd_tc.
 B200_API int b200_flash_bwd_span(const void* q, const void* k, const void* v, const void* dout, const void* lse,
                                  const void* delta, void* dq, void* dk, void* dv, const void* spans, const void* qtab,
-                                 const void* ktab, const long long* s, int B, int T, int QH, int KVH, int D, float scale, float cap,
-                                 const void* slopes, void* ds_ws, const void* unrot_cos, const void* unrot_sin, int unrot_ld,
+                                 const void* ktab, const void* order_k, const void* order_q, const long long* s, int B, int T, int QH, int KVH, int D,
+                                 float scale, float cap, const void* slopes, void* ds_ws, const void* unrot_cos, const void* unrot_sin, int unrot_ld,
                                  cudaStream_t st) {
   if (B <= 0 || T <= 0) return 0;
   if ((D != 128 && D != 64) || KVH <= 0 || QH % KVH != 0 || ds_ws == nullptr) return static_cast<int>(cudaErrorInvalidValue);
@@ -1671,6 +1673,7 @@ B200_API int b200_flash_bwd_span(const void* q, const void* k, const void* v, co
   p.unrot_ld = unrot_ld;
   p.spans = static_cast<const int2*>(spans);
   p.ktab = static_cast<const int2*>(ktab);
+  p.order_k = static_cast<const int*>(order_k);
   p.cap = make_score_cap(scale, cap);
   p.slopes = static_cast<const float*>(slopes);
   {
@@ -1687,7 +1690,7 @@ B200_API int b200_flash_bwd_span(const void* q, const void* k, const void* v, co
             : slopes ? launch_dkv_span<128, kBias>(p, maps, int(tiles), st) : launch_dkv_span<128, kSpan>(p, maps, int(tiles), st);
   if (rc != 0) return rc;
   return flash_bwd_dq_from_ds(ds_ws, k, dq, nullptr, s + 3, s + 12, B, T, QH, KVH, D, p.bchunk, p.unrot_cos, p.unrot_sin, p.unrot_ld,
-                              st, static_cast<const int4*>(qtab));
+                              st, static_cast<const int4*>(qtab), static_cast<const int*>(order_q));
 }
 
 // CTAs that share a key tile's query heads in the dK/dV kernel under a span mask: 0 (default) by the number of key tiles, else up to that

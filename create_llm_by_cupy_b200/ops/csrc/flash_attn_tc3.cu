@@ -34,7 +34,6 @@
 // Q / K / V / O tile instead of two, four k-steps in S = Q K^T and N = 64 in O += P V.
 #include "common.cuh"
 #include "ptx.cuh"
-#include "score_cap.cuh"
 
 namespace b200 {
 
@@ -48,17 +47,7 @@ struct Flash3Params {
   int bchunk;            // batch elements whose K and V stay in L2 together
   float scale;
   int* status;
-  // spans (kMod >= 0; see span_mask.cu)
-  const int2* spans;     // [B, T]
-  const int4* qtab;      // [B, n_tiles]
-  int n_tiles;
-  ScoreCap cap;          // kCap
-  const float* slopes;   // kBias: [QH]
 };
-
-// What the kernel does to the scores: nothing beside the causal mask and the valid length; the spans' mask; that and a cap; that
-// and a distance bias.
-constexpr int kCausal = -1, kSpan = 0, kCap = 1, kBias = 2;
 
 template <int kD>
 struct F3 {
@@ -123,22 +112,6 @@ __device__ __forceinline__ float f3_row_max(uint32_t (&sc)[128], int key0, int r
   return fmaxf(f3_max3(mx[0], mx[1], mx[2]), mx[3]);
 }
 
-// The same for a row that sees keys [lo, hi).
-template <bool kMask>
-__device__ __forceinline__ float f3_row_max_span(uint32_t (&sc)[128], int key0, int lo, int hi) {
-  float mx[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-  const uint32_t off = uint32_t(key0 - lo), n = uint32_t(hi - lo);
-#pragma unroll
-  for (int e = 0; e < 128; e += 2) {
-    if (kMask) {
-      if (off + e >= n) sc[e] = 0xff800000u;
-      if (off + (e + 1) >= n) sc[e + 1] = 0xff800000u;
-    }
-    mx[(e >> 1) & 3] = f3_max3(mx[(e >> 1) & 3], __uint_as_float(sc[e]), __uint_as_float(sc[e + 1]));
-  }
-  return fmaxf(f3_max3(mx[0], mx[1], mx[2]), mx[3]);
-}
-
 // P = exp2(s * sl2 - m_ref) for scores [kLo, kHi) of one row, packed to bf16 pairs IN PLACE (pair e / 2 lands in
 // register e / 2, which has been consumed by then); adds to the two partial row sums.
 template <int kLo, int kHi>
@@ -154,7 +127,7 @@ __device__ __forceinline__ void f3_row_p(uint32_t (&sc)[128], float sl2, float m
   }
 }
 
-template <int kD, int kMod>
+template <int kD>
 __global__ void __launch_bounds__(F3<kD>::kThreads, F3<kD>::kCtas)
 flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                      const __grid_constant__ CUtensorMap tmV, const __grid_constant__ CUtensorMap tmO,
@@ -224,44 +197,20 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
   constexpr uint32_t kColS = L::kColS, kColO = L::kColO, kColP = L::kColP;
   pdl_wait();                            // by every role: their bounded waits start counting behind it
   pdl_trigger();
-  // The CTA walks key tiles j0, j0 + 1, ...; query tile w takes part from step st[w] up to step nt[w].
-  int vlen = T, j0 = 0, st[2] = {0, 0}, nt[2] = {0, 0};
-  if constexpr (kMod == kCausal) {
-    if (p.valid_len) vlen = checked_index(p.valid_len[b], T, p.status, 301);
-    const int kv_tiles = (max(vlen, 1) + 127) / 128;
+  const int vlen = p.valid_len ? checked_index(p.valid_len[b], T, p.status, 301) : T;
+  const int kv_tiles = (max(vlen, 1) + 127) / 128;
+  int nt[2] = {0, 0};
 #pragma unroll
-    for (int w = 0; w < kW; ++w) {
-      const int mt = kW * pt + w;
-      nt[w] = (mt * 128 < T) ? min(mt + 1, kv_tiles) : 0;
-    }
-  } else {
-#pragma unroll
-    for (int w = 0; w < kW; ++w) {
-      const int mt = kW * pt + w;
-      if (mt * 128 >= T) continue;
-      const int4 r = p.qtab[size_t(b) * p.n_tiles + mt];
-      st[w] = r.x;
-      nt[w] = r.y;                       // 0: no row of the tile sees a key
-    }
-    if (kW == 2 && nt[0] > 0 && nt[1] > 0) {
-      // no step without a query tile: the rings of K and V go on only by products (the masked tiles weigh nothing)
-      if (st[1] > nt[0]) nt[0] = st[1];
-      else if (st[0] > nt[1]) nt[1] = st[0];
-    }
-    j0 = nt[0] > 0 ? (nt[1] > 0 ? min(st[0], st[1]) : st[0]) : st[1];
-#pragma unroll
-    for (int w = 0; w < kW; ++w) {
-      if (nt[w] == 0) continue;
-      st[w] -= j0;
-      nt[w] -= j0;
-    }
+  for (int w = 0; w < kW; ++w) {
+    const int mt = kW * pt + w;
+    nt[w] = (mt * 128 < T) ? min(mt + 1, kv_tiles) : 0;
   }
   const int nmax = max(nt[0], nt[1]);
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
     if (lane == 0) {
-      mbar_expect_tx(q_full, ((nt[0] > 0) + (nt[1] > 0)) * kTile);
+      mbar_expect_tx(q_full, (nt[1] > 0 ? 2 : 1) * kTile);
       for (int w = 0; w < kW; ++w) {
         if (nt[w] == 0) continue;
         uint8_t* sQ = smem + L::kQ + w * kTile;
@@ -274,13 +223,13 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         if (!mbar_wait(&k_empty[s], par, abort_flag)) break;
         uint8_t* sK = smem + L::kK + s * kTile;
         mbar_expect_tx(&k_full[s], kTile);
-        tma_load_4d(sK, &tmK, &k_full[s], 0, kvh, (j0 + j) * 128, b);
-        if (kD == 128) tma_load_4d(sK + 16384, &tmK, &k_full[s], 64, kvh, (j0 + j) * 128, b);
+        tma_load_4d(sK, &tmK, &k_full[s], 0, kvh, j * 128, b);
+        if (kD == 128) tma_load_4d(sK + 16384, &tmK, &k_full[s], 64, kvh, j * 128, b);
         if (!mbar_wait(&v_empty[s], par, abort_flag)) break;
         uint8_t* sV = smem + L::kV + s * kTile;
         mbar_expect_tx(&v_full[s], kTile);
-        tma_load_4d(sV, &tmV, &v_full[s], 0, kvh, (j0 + j) * 128, b);
-        if (kD == 128) tma_load_4d(sV + 16384, &tmV, &v_full[s], 64, kvh, (j0 + j) * 128, b);
+        tma_load_4d(sV, &tmV, &v_full[s], 0, kvh, j * 128, b);
+        if (kD == 128) tma_load_4d(sV + 16384, &tmV, &v_full[s], 64, kvh, j * 128, b);
       }
     }
   } else if (warp == 1) {
@@ -304,7 +253,7 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         if (ok) {
           tc_fence_after();
           for (int w = 0; w < kW; ++w)
-            if (nt[w] > 0 && st[w] == 0) issue_s(w, 0);
+            if (nt[w] > 0) issue_s(w, 0);
           umma_commit_warp(&k_empty[0]);
         }
       }
@@ -315,7 +264,7 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 #pragma unroll
         for (int kk = 0; kk < 8; ++kk)
           if (kk >= lo && kk < hi)
-            umma_bf16_ts_warp(tmem_base + kColO + w * 128, tP + kk * 8, dV + kk * 128, idesc_pv, j != st[w] || kk != 0);
+            umma_bf16_ts_warp(tmem_base + kColO + w * 128, tP + kk * 8, dV + kk * 128, idesc_pv, (j | kk) != 0);
       };
       for (int j = 0; j < nmax && ok; ++j) {
         bool v_ready = false, k_ready = false;
@@ -331,19 +280,14 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         if (kOwnP) {
           for (int w = 0; w < kW && ok; ++w) {
             if (j + 1 >= nt[w]) continue;
-            ok = mbar_wait_warp(&early[w], j & 1, abort_flag) && next_s(w);      // one query tile: it starts at step 0
+            ok = mbar_wait_warp(&early[w], j & 1, abort_flag) && next_s(w);
           }
           if (!ok) break;
           if (j + 1 < nmax) umma_commit_warp(&k_empty[(j + 1) & 1]);
         }
         for (int w = 0; w < kW && ok; ++w) {
           if (j >= nt[w]) continue;
-          if (!kOwnP && j < st[w]) {                       // its first scores come with this step's products
-            if (j + 1 == st[w] && !next_s(w)) { ok = false; break; }
-            continue;
-          }
-          const uint32_t ph = (j - st[w]) & 1;
-          if (!mbar_wait_warp(kOwnP ? &p_full[w] : &early[w], ph, abort_flag)) { ok = false; break; }
+          if (!mbar_wait_warp(kOwnP ? &p_full[w] : &early[w], j & 1, abort_flag)) { ok = false; break; }
           if (!v_ready) {
             if (!mbar_wait_warp(&v_full[j & 1], (j >> 1) & 1, abort_flag)) { ok = false; break; }
             v_ready = true;
@@ -353,7 +297,7 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             issue_pv(w, j, 0, 8);
           } else {
             issue_pv(w, j, 0, 4);
-            if (!mbar_wait_warp(&p_full[w], ph, abort_flag)) { ok = false; break; }
+            if (!mbar_wait_warp(&p_full[w], j & 1, abort_flag)) { ok = false; break; }
             tc_fence_after();
             issue_pv(w, j, 4, 8);
           }
@@ -372,32 +316,19 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
     const int rloc = q * 32 + lane;
     const int mt = kW * pt + w;
     const int row = mt * 128 + rloc;
-    const int my_tiles = nt[w] - st[w];
-    int2 span = make_int2(0, 0);             // the keys that the row sees
-    int lo_max = 0, hi_min = 0;              // a key tile in [lo_max, hi_min) is seen whole by every row of the query tile
-    float slope2 = 0.f;
-    if constexpr (kMod != kCausal) {
-      if (row < T) span = p.spans[size_t(b) * T + row];
-      if (my_tiles > 0) {
-        const int4 r = p.qtab[size_t(b) * p.n_tiles + mt];
-        lo_max = r.z;
-        hi_min = r.w;
-      }
-      if constexpr (kMod == kBias) slope2 = p.slopes[h] * kF3Log2e;
-    }
+    const int my_tiles = nt[w];
     const uint32_t lane_sel = uint32_t(q * 32) << 16;
     const uint32_t tS = tmem_base + lane_sel + kColS + w * 128;
     const uint32_t tO = tmem_base + lane_sel + kColO + w * 128;
     const uint32_t tP = tmem_base + lane_sel + kColP + w * 128;
-    // log2 units per score; a bias leaves them in log2 units, a cap is taken on the way into the exponentials
-    const float sl2 = kMod == kCap || kMod == kBias ? 1.f : p.scale * kF3Log2e;
+    const float sl2 = p.scale * kF3Log2e;
     float m_ref = 0.f, l_run = 0.f;          // reference maximum (log2 units) and the row sum relative to it
     bool ok = true;
     for (int j = 0; j < my_tiles && ok; ++j) {
       if (!mbar_wait(&s_full[w], j & 1, abort_flag)) { ok = false; break; }
       tc_fence_after();
-      const int key0 = (kMod == kCausal ? j : j0 + st[w] + j) * 128;
-      const bool need_mask = kMod == kCausal ? (j == mt) || (j * 128 + 128 > vlen) : key0 < lo_max || key0 + 128 > hi_min;
+      const bool need_mask = (j == mt) || (j * 128 + 128 > vlen);
+      const int key0 = j * 128;
       // The whole row (128 raw scores) is read in one go: four loads, one wait. A tensor-memory load queues
       // behind the MMAs the other warpgroup has in flight, so every separate round trip costs that wait again.
       uint32_t sc[128];
@@ -410,28 +341,11 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         tc_fence_before();
         mbar_arrive(&early[w]);
       }
-      float mx;
-      bool cap_now = false;              // kCap: the exponentials take the cap
-      if constexpr (kMod == kCausal) {
-        mx = (need_mask ? f3_row_max<true>(sc, key0, row, vlen) : f3_row_max<false>(sc, key0, row, vlen)) * sl2;
-      } else {
-        if constexpr (kMod == kCap) {
-          const int tier = cap_tier(sc, p.cap);
-          cap_now = tier == kCapNear && !need_mask;
-          if (!cap_now) cap_scores(sc, p.cap, tier);
-        }
-        if constexpr (kMod == kBias) {
-          const float dist = float(key0 - row);
-#pragma unroll
-          for (int e = 0; e < 128; ++e) sc[e] = __float_as_uint(fmaf(__uint_as_float(sc[e]), p.scale * kF3Log2e, -slope2 * fabsf(dist + float(e))));
-        }
-        mx = (need_mask ? f3_row_max_span<true>(sc, key0, span.x, span.y) : f3_row_max_span<false>(sc, key0, 0, 0)) * sl2;
-        if (kMod == kCap && cap_now) mx = cap_any(mx, p.cap);          // the cap keeps the order of the scores
-      }
+      float mx = (need_mask ? f3_row_max<true>(sc, key0, row, vlen) : f3_row_max<false>(sc, key0, row, vlen)) * sl2;
       // The reference maximum is set by the first tile and afterwards moves only when a tile exceeds it by
       // more than 2^8; then O_w and the row sum are rescaled by the row's own thread.
       if (j == 0) {
-        m_ref = (mx == -INFINITY && kMod == kCausal) ? 0.f : mx;       // spans: a row may see nothing of its tile's first keys
+        m_ref = (mx == -INFINITY) ? 0.f : mx;
       } else {
         const bool need = mx > m_ref + kF3RescaleStep;
         if (__any_sync(0xffffffffu, need)) {
@@ -447,10 +361,6 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
             tmem_ld_wait();
 #pragma unroll
             for (int e = 0; e < 16; ++e) t[e] = __float_as_uint(__uint_as_float(t[e]) * corr);
-            if (kMod != kCausal && corr == 0.f) {       // nothing of the tiles so far is this row's, infinite values neither
-#pragma unroll
-              for (int e = 0; e < 16; ++e) t[e] = 0u;
-            }
             tmem_st_32x32b_x16(tO + c * 16, t);
           }
           tmem_st_wait();
@@ -459,23 +369,19 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       }
       // P = exp2(s * scale - m_ref) as bf16 pairs, packed in place over the first 64 registers, and its row sum
       float rs0 = 0.f, rs1 = 0.f;
-      const float m_sub = kMod != kCausal && m_ref == -INFINITY ? 0.f : m_ref;      // nothing seen yet: exp2(-inf) is 0
       if (kOwnP) {
-        if (kMod == kCap && cap_now) cap_row_p<0, 128>(sc, p.cap, m_sub, rs0, rs1);
-        else f3_row_p<0, 128>(sc, sl2, m_sub, rs0, rs1);
+        f3_row_p<0, 128>(sc, sl2, m_ref, rs0, rs1);
         if (j > 0 && !mbar_wait(&pv_done[w], (j - 1) & 1, abort_flag)) { ok = false; break; }   // P_w has been read
         tc_fence_after();
       } else {
         // head_dim 128: the next scores wait for this P V, so its first half is handed over early
-        if (kMod == kCap && cap_now) cap_row_p<0, 64>(sc, p.cap, m_sub, rs0, rs1);
-        else f3_row_p<0, 64>(sc, sl2, m_sub, rs0, rs1);
+        f3_row_p<0, 64>(sc, sl2, m_ref, rs0, rs1);
         tmem_st_32x32b_x16(tP, *reinterpret_cast<const uint32_t(*)[16]>(&sc[0]));
         tmem_st_32x32b_x16(tP + 16, *reinterpret_cast<const uint32_t(*)[16]>(&sc[16]));
         tmem_st_wait();
         tc_fence_before();
         mbar_arrive(&early[w]);
-        if (kMod == kCap && cap_now) cap_row_p<64, 128>(sc, p.cap, m_sub, rs0, rs1);
-        else f3_row_p<64, 128>(sc, sl2, m_sub, rs0, rs1);
+        f3_row_p<64, 128>(sc, sl2, m_ref, rs0, rs1);
       }
 #pragma unroll
       for (int c = kOwnP ? 0 : 2; c < 4; ++c)
@@ -485,27 +391,19 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
       mbar_arrive(&p_full[w]);
       l_run += rs0 + rs1;
     }
-    // spans: a query tile that sees nothing still has zeros to store
-    const bool empty = kMod != kCausal && my_tiles == 0 && mt * 128 < T;
-    if (ok && (my_tiles > 0 || empty)) {
-      if (empty || mbar_wait(&pv_done[w], (my_tiles - 1) & 1, abort_flag)) {
+    if (ok && my_tiles > 0) {
+      if (mbar_wait(&pv_done[w], (my_tiles - 1) & 1, abort_flag)) {
         tc_fence_after();
         // all MMAs of this query tile have completed: its Q tile in shared memory is free and becomes
         // the staging area of the output (two 128 x 64 boxes, 128-byte swizzle)
-        const float inv = kMod != kCausal ? (l_run == 0.f ? 0.f : 1.f / l_run) : (l_run > 0.f ? 1.f / l_run : 0.f);
+        const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
         uint8_t* stg = smem + L::kQ + w * kTile;
         const uint32_t swz = uint32_t(rloc & 7);
 #pragma unroll 1
         for (int c = 0; c < kD / 32; ++c) {
           uint32_t r[32];
-          if (!empty) {
-            tmem_ld_32x32b_x32(tO + c * 32, r);
-            tmem_ld_wait();
-          }
-          if (kMod != kCausal && (empty || l_run == 0.f)) {      // (an infinite value times 0 is none)
-#pragma unroll
-            for (int e = 0; e < 32; ++e) r[e] = 0u;
-          }
+          tmem_ld_32x32b_x32(tO + c * 32, r);
+          tmem_ld_wait();
           uint8_t* rowp = stg + (c >> 1) * 16384 + rloc * 128;
 #pragma unroll
           for (int k = 0; k < 4; ++k) {
@@ -520,7 +418,7 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
         }
         if (row < T)
           p.lse[(size_t(b) * p.QH + h) * T + row] =
-              kMod != kCausal && l_run != l_run ? l_run : l_run > 0.f ? m_ref * 0.6931471805599453f + logf(l_run) : -INFINITY;
+              l_run > 0.f ? m_ref * 0.6931471805599453f + logf(l_run) : -INFINITY;
         fence_proxy_async_smem();
         mbar_arrive(&stage_bar[w]);
         if (q == 0 && lane == 0) {
@@ -550,13 +448,13 @@ flash_fwd_tc3_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_const
 
 using namespace b200;
 
-// q, k, v (already rotated), o: [B, T, heads, D] by element strides. What the two entry points below share.
-template <int kMod>
-static int launch_flash_fwd(const void* q, const void* k, const void* v, void* o, const long long* strides, int KVH, int D,
-                            Flash3Params p, cudaStream_t st) {
-  const int B = p.B, T = p.T, QH = p.QH;
+// Same contract as b200_flash_fwd_tc (inputs already rotated) for head_dim 128 or 64; the output must be
+// TMA-addressable (16-byte aligned base, strides that are multiples of 8 elements).
+B200_API int b200_flash_fwd_tc3(const void* q, const void* k, const void* v, void* o, void* lse, const void* valid_len,
+                                const long long* strides, int B, int T, int QH, int KVH, int D, float scale,
+                                cudaStream_t st) {
   if (B <= 0 || T <= 0) return 0;
-  if ((D != 128 && D != 64) || KVH <= 0 || QH % KVH != 0) return static_cast<int>(cudaErrorInvalidValue);
+  if ((D != 128 && D != 64) || QH % KVH != 0) return static_cast<int>(cudaErrorInvalidValue);
   for (int i = 0; i < 12; ++i)
     if (strides[i] % 8 != 0) return static_cast<int>(cudaErrorInvalidValue);
   if ((reinterpret_cast<uintptr_t>(o) & 15) != 0) return static_cast<int>(cudaErrorInvalidValue);
@@ -565,12 +463,15 @@ static int launch_flash_fwd(const void* q, const void* k, const void* v, void* o
   TensorMap tv = get_tensor_map_bthd(v, B, T, KVH, D, strides[6], strides[7], strides[8], 128, 64);
   TensorMap to = get_tensor_map_bthd(o, B, T, QH, D, strides[9], strides[10], strides[11], 128, 64);
   if (!tq || !tk || !tv || !to) return static_cast<int>(cudaErrorInvalidValue);
-  p.KVH = KVH;
+  Flash3Params p;
+  p.lse = static_cast<float*>(lse);
+  p.valid_len = static_cast<const int*>(valid_len);
+  p.B = B; p.T = T; p.QH = QH; p.KVH = KVH; p.scale = scale;
   p.status = status_ptr();
   static bool configured = false;
   if (!configured) {
-    B200_CHECK(cudaFuncSetAttribute(flash_fwd_tc3_kernel<128, kMod>, cudaFuncAttributeMaxDynamicSharedMemorySize, F3<128>::kSmem));
-    B200_CHECK(cudaFuncSetAttribute(flash_fwd_tc3_kernel<64, kMod>, cudaFuncAttributeMaxDynamicSharedMemorySize, F3<64>::kSmem));
+    B200_CHECK(cudaFuncSetAttribute(flash_fwd_tc3_kernel<128>, cudaFuncAttributeMaxDynamicSharedMemorySize, F3<128>::kSmem));
+    B200_CHECK(cudaFuncSetAttribute(flash_fwd_tc3_kernel<64>, cudaFuncAttributeMaxDynamicSharedMemorySize, F3<64>::kSmem));
     configured = true;
   }
   {
@@ -583,39 +484,8 @@ static int launch_flash_fwd(const void* q, const void* k, const void* v, void* o
   if (ctas > 0x7fffffffLL) return static_cast<int>(cudaErrorInvalidValue);
   const dim3 grid(static_cast<unsigned>(ctas));
   if (D == 128)
-    return static_cast<int>(launch_pdl(flash_fwd_tc3_kernel<128, kMod>, grid, dim3(F3<128>::kThreads), F3<128>::kSmem, st, 0, *tq,
-                                       *tk, *tv, *to, p));
-  return static_cast<int>(launch_pdl(flash_fwd_tc3_kernel<64, kMod>, grid, dim3(F3<64>::kThreads), F3<64>::kSmem, st, 0, *tq, *tk,
+    return static_cast<int>(launch_pdl(flash_fwd_tc3_kernel<128>, grid, dim3(F3<128>::kThreads), F3<128>::kSmem, st, 0, *tq, *tk,
+                                       *tv, *to, p));
+  return static_cast<int>(launch_pdl(flash_fwd_tc3_kernel<64>, grid, dim3(F3<64>::kThreads), F3<64>::kSmem, st, 0, *tq, *tk,
                                      *tv, *to, p));
-}
-
-// Same contract as b200_flash_fwd_tc (inputs already rotated) for head_dim 128 or 64; the output must be
-// TMA-addressable (16-byte aligned base, strides that are multiples of 8 elements).
-B200_API int b200_flash_fwd_tc3(const void* q, const void* k, const void* v, void* o, void* lse, const void* valid_len,
-                                const long long* strides, int B, int T, int QH, int KVH, int D, float scale,
-                                cudaStream_t st) {
-  Flash3Params p = {};
-  p.lse = static_cast<float*>(lse);
-  p.valid_len = static_cast<const int*>(valid_len);
-  p.B = B; p.T = T; p.QH = QH; p.scale = scale;
-  return launch_flash_fwd<kCausal>(q, k, v, o, strides, KVH, D, p, st);
-}
-
-// The same under a span mask (b200_span_mask). cap > 0: scores c tanh(s / c); slopes [QH]: scores minus slope times distance
-// (not both).
-B200_API int b200_flash_fwd_span(const void* q, const void* k, const void* v, void* o, void* lse, const void* spans,
-                                 const void* qtab, const long long* strides, int B, int T, int QH, int KVH, int D, float scale,
-                                 float cap, const void* slopes, cudaStream_t st) {
-  if (cap < 0.f || (cap > 0.f && slopes != nullptr)) return static_cast<int>(cudaErrorInvalidValue);
-  Flash3Params p = {};
-  p.lse = static_cast<float*>(lse);
-  p.B = B; p.T = T; p.QH = QH; p.scale = scale;
-  p.spans = static_cast<const int2*>(spans);
-  p.qtab = static_cast<const int4*>(qtab);
-  p.n_tiles = (T + 127) / 128;
-  p.cap = make_score_cap(scale, cap);
-  p.slopes = static_cast<const float*>(slopes);
-  if (cap > 0.f) return launch_flash_fwd<kCap>(q, k, v, o, strides, KVH, D, p, st);
-  if (slopes != nullptr) return launch_flash_fwd<kBias>(q, k, v, o, strides, KVH, D, p, st);
-  return launch_flash_fwd<kSpan>(q, k, v, o, strides, KVH, D, p, st);
 }

@@ -16,7 +16,7 @@ namespace b200 {
 
 constexpr int SM_THREADS = 1024;                      // at most: as many as there are tokens for
 constexpr int SM_PER = 4;                             // tokens of a thread
-constexpr int SM_MAX_TILES = 5632;                    // ranges kept in shared memory: 44 KiB, 720896 tokens
+constexpr int SM_MAX_TILES = 4000;                    // ranges and counts kept in shared memory: 47 KiB, 512000 tokens
 
 struct SpanMaskParams {
   const int* docs;              // [B, T] or null: one document
@@ -27,6 +27,7 @@ struct SpanMaskParams {
   int2* spans;                  // [B, T]
   int4* qtab;                   // [B, nt]: first key tile, end; largest lo, smallest hi of its rows
   int2* ktab;                   // [B, nt]: first query tile, end
+  int* order;                   // [B, nt] query tiles, [B, (nt + 1) / 2] pairs of them, [B, nt] key tiles: those with most to do first
   int B, T, nt;
   int* status;
 };
@@ -90,6 +91,7 @@ __device__ __forceinline__ int warp_max(int v) { return __reduce_max_sync(0xffff
 __global__ void __launch_bounds__(SM_THREADS)
 span_mask_kernel(const SpanMaskParams p) {
   extern __shared__ int2 s_range[];                   // [nt]: key tiles of each query tile
+  int* s_count = reinterpret_cast<int*>(s_range + p.nt);      // [nt]: query tiles of each key tile
   __shared__ int warp_v[SM_THREADS / 32];
   const int b = blockIdx.x, T = p.T;
   const size_t row0 = size_t(b) * T;
@@ -214,6 +216,34 @@ span_mask_kernel(const SpanMaskParams p) {
       }
     }
     p.ktab[size_t(b) * p.nt + n] = end > 0 ? make_int2(first, end) : make_int2(0, 0);
+    s_count[n] = end > 0 ? end - first : 0;
+  }
+  __syncthreads();
+  // Places in the orders: how many have more to do (or as much, and a lower number).
+  const int pairs = (p.nt + 1) / 2;
+  int *order_q = p.order + size_t(b) * p.nt, *order_p = p.order + size_t(p.B) * p.nt + size_t(b) * pairs,
+      *order_k = p.order + size_t(p.B) * (p.nt + pairs) + size_t(b) * p.nt;
+  auto steps = [&](int u) {                           // of a pair: the walk that the two share
+    const int2 x = s_range[2 * u], y = 2 * u + 1 < p.nt ? s_range[2 * u + 1] : make_int2(0, 0);
+    return x.y == 0 ? y.y - y.x : y.y == 0 ? x.y - x.x : max(x.y, y.y) - min(x.x, y.x);
+  };
+  for (int n = threadIdx.x; n < p.nt; n += blockDim.x) {
+    const int mine = s_range[n].y - s_range[n].x, count = s_count[n], both = n < pairs ? steps(n) : 0;
+    int at_q = 0, at_k = 0, at_p = 0;
+    for (int m = 0; m < p.nt; ++m) {
+      const int other = s_range[m].y - s_range[m].x, c = s_count[m];
+      at_q += other > mine || (other == mine && m < n);
+      at_k += c > count || (c == count && m < n);
+    }
+    order_q[at_q] = n;
+    order_k[at_k] = n;
+    if (n < pairs) {
+      for (int m = 0; m < pairs; ++m) {
+        const int other = steps(m);
+        at_p += other > both || (other == both && m < n);
+      }
+      order_p[at_p] = n;
+    }
   }
 }
 
@@ -221,10 +251,11 @@ span_mask_kernel(const SpanMaskParams p) {
 
 using namespace b200;
 
-// Fills `spans` [B, T] (lo, hi), `qtab` [B, nt] (4 ints) and `ktab` [B, nt] (2 ints), nt = tiles of 128 tokens, from documents,
+// Fills `spans` [B, T] (lo, hi), `qtab` [B, nt] (4 ints), `ktab` [B, nt] (2 ints) and `order` [B, nt], [B, (nt + 1) / 2], [B, nt] (query tiles,
+// pairs of them, key tiles; most to do first), nt = tiles of 128 tokens, from documents,
 // prefix flags and valid lengths (each may be null), or from the spans lo / hi [B, T].
 B200_API int b200_span_mask(const void* docs, const void* prefix, const void* valid_len, const void* lo, const void* hi,
-                            void* spans, void* qtab, void* ktab, int B, int T, cudaStream_t st) {
+                            void* spans, void* qtab, void* ktab, void* order, int B, int T, cudaStream_t st) {
   if (B <= 0 || T <= 0) return 0;
   const int nt = (T + 127) / 128;
   if (nt > SM_MAX_TILES || (lo == nullptr) != (hi == nullptr)) return static_cast<int>(cudaErrorInvalidValue);
@@ -237,8 +268,9 @@ B200_API int b200_span_mask(const void* docs, const void* prefix, const void* va
   p.spans = static_cast<int2*>(spans);
   p.qtab = static_cast<int4*>(qtab);
   p.ktab = static_cast<int2*>(ktab);
+  p.order = static_cast<int*>(order);
   p.B = B; p.T = T; p.nt = nt;
   p.status = status_ptr();
   const int threads = nt * 32 < SM_THREADS ? nt * 32 : SM_THREADS;             // a warp to a tile
-  return static_cast<int>(launch_pdl(span_mask_kernel, dim3(B), dim3(threads), size_t(nt) * sizeof(int2), st, 0, p));
+  return static_cast<int>(launch_pdl(span_mask_kernel, dim3(B), dim3(threads), size_t(nt) * (sizeof(int2) + sizeof(int)), st, 0, p));
 }

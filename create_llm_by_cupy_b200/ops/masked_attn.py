@@ -36,8 +36,9 @@ class SpanMask:
     that the kernels walk by. Made by ``span_mask`` or ``SpanMask.from_spans``; one serves any number of layers and heads."""
 
     def __init__(self, buf: torch.Tensor, B: int, T: int):
-        # CUDA: [B, nt, 4] key tiles of every query tile, [B, nt, 2] query tiles of every key tile, then the spans [B, T, 2] (lo, hi);
-        # the tables, whose entries are the wider ones, first. CPU: the spans alone.
+        # CUDA: [B, nt, 4] key tiles of every query tile, [B, nt, 2] query tiles of every key tile, the spans [B, T, 2] (lo, hi), and
+        # the orders, those with most to do first: [B, nt] query tiles, [B, (nt + 1) / 2] pairs of them, [B, nt] key tiles. What has the
+        # wider entries comes first. CPU: the spans alone.
         self.buf, self.B, self.T = buf, B, T
 
     @property
@@ -48,13 +49,20 @@ class SpanMask:
     def spans(self) -> torch.Tensor:
         """int32 [B, T, 2]: lo, hi."""
         n = self.B * self.T * 2
-        return self.buf[self.buf.numel() - n:].view(self.B, self.T, 2)
+        at = 6 * self.B * ((self.T + 127) // 128) if self.buf.is_cuda else 0
+        return self.buf[at:at + n].view(self.B, self.T, 2)
 
     def _ptrs(self, b0: int = 0):
         """Addresses of spans, query-tile and key-tile table from batch element ``b0`` on (CUDA)."""
         nt, p = (self.T + 127) // 128, self.buf.data_ptr()
         return (native.c_void_p(p + 4 * (6 * self.B * nt + 2 * b0 * self.T)), native.c_void_p(p + 16 * b0 * nt),
                 native.c_void_p(p + 4 * (4 * self.B * nt + 2 * b0 * nt)))
+
+    def _orders(self, b0: int = 0):
+        """Addresses of the orders of query tiles and of key tiles (CUDA); those of pairs stand between them."""
+        nt = (self.T + 127) // 128
+        pairs, p = (nt + 1) // 2, self.buf.data_ptr() + 4 * self.B * (6 * nt + 2 * self.T)
+        return native.c_void_p(p + 4 * b0 * nt), native.c_void_p(p + 4 * (self.B * (nt + pairs) + b0 * nt))
 
     @classmethod
     def from_spans(cls, lo: torch.Tensor, hi: torch.Tensor) -> "SpanMask":
@@ -77,9 +85,9 @@ def _make_mask(B, T, device, docs=None, prefix=None, valid_len=None, lo=None, hi
         none = hi <= lo
         return SpanMask(torch.stack([lo.masked_fill(none, 0), hi.masked_fill(none, 0)], -1).to(torch.int32).reshape(-1), B, T)
     nt = (T + 127) // 128
-    mask = SpanMask(torch.empty(B * (6 * nt + 2 * T), dtype=torch.int32, device=device), B, T)
+    mask = SpanMask(torch.empty(B * (8 * nt + (nt + 1) // 2 + 2 * T), dtype=torch.int32, device=device), B, T)
     native.check(F._lib().b200_span_mask(native.ptr(docs), native.ptr(prefix), native.ptr(valid_len), native.ptr(lo), native.ptr(hi),
-                                         *mask._ptrs(), B, T, native.stream_ptr()), "span_mask")
+                                         *mask._ptrs(), mask._orders()[0], B, T, native.stream_ptr()), "span_mask")
     native.bump()
     return mask
 
@@ -120,8 +128,8 @@ def span_mask(B: int, T: int, device, docs=None, prefix=None, valid_len=None) ->
             raise ValueError(f"span_mask: {name} is {dt} {list(shape)}")
         if x is not None and x.device.type != torch.device(device).type:
             raise ValueError(f"span_mask: {name} is not on {device}")
-    if T > 720896:
-        raise ValueError("span_mask: more than 720896 tokens in a row")
+    if T > 512000:
+        raise ValueError("span_mask: more than 512000 tokens in a row")
     docs, prefix, valid_len = (x if x is None else x.contiguous() for x in (docs, prefix, valid_len))
     return _make_mask(B, T, device, docs, prefix, valid_len)
 
@@ -168,7 +176,7 @@ def _tile_view(t: torch.Tensor) -> torch.Tensor:
 
 def _strides3(t: torch.Tensor) -> list[int]:
     """(batch, token, head) strides; of a dimension of one, which is never stepped along, one that a tile copy can have."""
-    return [t.stride(i) if t.shape[i] > 1 else 8 for i in range(3)]
+    return [t.stride(i) if t.shape[i] > 1 else 16 for i in range(3)]
 
 
 def _work_dtype(x):
@@ -235,7 +243,7 @@ def span_attn_fwd(q, k, v, mask: SpanMask, *, scale: float | None = None, softca
     arr = (ctypes.c_longlong * 12)(*_strides3(q), *_strides3(k), *_strides3(v), *_strides3(o))
     slopes = slopes if slopes is None else slopes.contiguous()
     native.check(F._lib().b200_flash_fwd_span(native.ptr(q), native.ptr(k), native.ptr(v), native.ptr(o), native.ptr(lse),
-                                              *mask._ptrs()[:2], arr, B, T, QH, KVH, D, _f(scale),
+                                              *mask._ptrs()[:2], mask._orders()[0], arr, B, T, QH, KVH, D, _f(scale),
                                               _f(softcap), native.ptr(slopes), native.stream_ptr()), "flash_fwd_span")
     native.bump()
     return o, lse
@@ -317,7 +325,8 @@ def span_attn_bwd(dout, q, k, v, o, lse, mask: SpanMask, *, scale: float | None 
         def rows(t):
             return native.ptr(t[b0:b1, g0 * R:g1 * R])     # contiguous: head slices only come with one batch element
         native.check(F._lib().b200_flash_bwd_span(
-            qs(q), ks(k), ks(v), qs(dout), rows(lse), rows(delta), qs(dq), ks(dk), ks(dv), *mask._ptrs(b0), arr, b1 - b0, T, (g1 - g0) * R, g1 - g0, D, _f(scale), _f(softcap),
+            qs(q), ks(k), ks(v), qs(dout), rows(lse), rows(delta), qs(dq), ks(dk), ks(dv), *mask._ptrs(b0), mask._orders(b0)[1],
+            mask._orders(b0)[0], arr, b1 - b0, T, (g1 - g0) * R, g1 - g0, D, _f(scale), _f(softcap),
             native.ptr(slopes if slopes is None else slopes[g0 * R:g1 * R]), native.ptr(ws), native.ptr(ucos), native.ptr(usin), uld,
             native.stream_ptr()), "flash_bwd_span")
     native.bump(2 * len(chunks))

@@ -185,7 +185,7 @@ def test_span_refusals():
     with pytest.raises(ValueError):
         A.span_mask(-1, 4, "cpu")
     with pytest.raises(ValueError):
-        A.span_mask(1, 720897, "cpu")
+        A.span_mask(1, 512001, "cpu")
     with pytest.raises(ValueError):
         A.SpanMask.from_spans(torch.zeros(2, 4), torch.zeros(2, 4))
     with pytest.raises(TypeError):
