@@ -8,9 +8,9 @@
 // 1024 / 128 at documents of 200 tokens), and a CTA's life was mostly its own start and end: 11.5 us of 26.7 at 4096 tokens, 32 / 8 heads of
 // 128, documents of 700 - barriers and tensor memory, tables, Q, the output's way out. So the CTAs stay:
 //
-//   * one per SM (head_dim 128, two query tiles side by side) or two (64, one each), and each takes query tiles from the list of all
-//     of them, longest first, there and back: round k of CTA c is tile k G + c, or k G + G - 1 - c in odd rounds, so that what
-//     the CTAs get adds up to about the same;
+//   * one per SM (head_dim 128, two query tiles side by side) or two (64, one each); the grid has a CTA for every unit of work, those
+//     with most to do first, and a CTA that is about to finish one takes the next that the grid has not started (with a fixed share of
+//     the list for each the slowest took 20 to 30 % longer than the mean: what a tile costs is not its keys alone);
 //   * loads of the next tile's Q, K and V start when the last scores of the present one are done, its first scores when the last P V
 //     is, and the output leaves through a staging buffer of its own while they run.
 //
@@ -41,17 +41,19 @@ struct FlashSpanParams {
   int B, T, QH, KVH;
   int n_tiles, n_units;
   int bchunk;            // batch elements whose K and V stay in L2 together
-  unsigned items;        // n_units * QH * B
   float scale;
   ScoreCap cap;          // kSpanCap
   const float* slopes;   // kSpanBias: [QH]
   int* status;
 };
 
-template <int kD, int kW>
+template <int kD>
 struct FS {
+  // Query tiles of a unit. (head_dim 128 with one, two CTAs to an SM and one tile of K and V each: documents of 600 tokens 57 -> 54 us, one of
+  // 8192 251 -> 268, capped scores no different.)
+  static constexpr int kW = kD == 128 ? 2 : 1;
   static constexpr int kCtas = 3 - kW;                                 // CTAs of an SM
-  static constexpr int kRing = kD == 128 && kW == 1 ? 1 : 2;           // tiles of K, and of V, in shared memory
+  static constexpr int kRing = 2;                                      // tiles of K, and of V, in shared memory
   static constexpr int kFirst = 4;                                     // first softmax warp
   // A warpgroup for the two issuing warps, so that registers can be shared out: of 3 x 168 (2 x 128) at launch
   static constexpr int kRegsFew = kW == 2 ? 88 : 64, kRegsMany = kW == 2 ? 208 : 192;
@@ -61,8 +63,8 @@ struct FS {
   static constexpr int kK = kW * kTile;                                // K ring
   static constexpr int kV = kK + kRing * kTile;                        // V ring
   static constexpr int kBar = kV + kRing * kTile;
-  // q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], early[2], p_full[2], pv_done[2], o_free[2]
-  static constexpr int kSmem = kBar + 20 * 8 + 16 + 1024;
+  // q_full, q_empty, k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], early[2], p_full[2], pv_done[2], o_free[2], u_full, u_empty
+  static constexpr int kSmem = kBar + 22 * 8 + 16 + 16 + 1024;
   static constexpr bool kOwnP = kD == 64;                              // P beside S, not over it
   static constexpr int kCols = kW == 2 ? 512 : 256;
   static constexpr int kColS = 0, kColO = kW * 128, kColP = kOwnP ? kColO + kD : 0;
@@ -75,12 +77,7 @@ struct SpanItem {
 };
 
 template <int kW>
-__device__ __forceinline__ bool span_item(const FlashSpanParams& p, unsigned round, SpanItem& it) {
-  const unsigned G = gridDim.x;
-  if (round * G >= p.items) return false;
-  const unsigned i = round * G + ((round & 1) ? G - 1 - blockIdx.x : blockIdx.x);
-  it.unit = -1;
-  if (i >= p.items) return true;                     // the last round does not reach this CTA
+__device__ __forceinline__ void span_item(const FlashSpanParams& p, unsigned i, SpanItem& it) {
   const unsigned per_chunk = p.n_units * p.QH * p.bchunk;
   const unsigned chunk = i / per_chunk, r = i - chunk * per_chunk;
   const unsigned hb = p.QH * min(p.bchunk, int(p.B - chunk * p.bchunk));
@@ -111,8 +108,35 @@ __device__ __forceinline__ bool span_item(const FlashSpanParams& p, unsigned rou
     it.nt[w] -= it.j0;
   }
   it.steps = max(it.nt[0], it.nt[1]);
-  return true;
 }
+
+// The units of a CTA: its own, then those that it takes over. One answer at a time stands in shared memory, until every role has read it.
+struct SpanQueue {
+  uint64_t* full;            // the answer is there
+  uint64_t* empty;           // it has been read: by the MMA warp and every softmax warp
+  uint4* answer;
+  uint32_t asked;            // answers so far
+  // The next unit, -1: there is none (or a wait ran out). The TMA thread asks when it has sent for all of the present one, which is then two
+  // tiles from its end (asked at its start, a CTA sat on a second long unit while others ran out of work).
+  __device__ __forceinline__ int ask(volatile int* abort_flag) {
+    if (asked > 0 && !mbar_wait(empty, (asked - 1) & 1, abort_flag)) return -1;
+    mbar_expect_tx(full, 16);
+    take_cta(answer, full);
+    if (!mbar_wait(full, asked & 1, abort_flag)) return -1;
+    ++asked;
+    return taken_cta(answer);
+  }
+  // By a whole warp of another role.
+  __device__ __forceinline__ int next(volatile int* abort_flag) {
+    if (!mbar_wait_warp(full, asked & 1, abort_flag)) return -1;
+    ++asked;
+    const int unit = taken_cta(answer);
+    fence_proxy_async_smem();                        // read before the next answer is written over it
+    __syncwarp();
+    if (lane_id() == 0) mbar_arrive(empty);
+    return unit;
+  }
+};
 
 // 32 bytes, one sector, in one store.
 __device__ __forceinline__ void fs_store32(void* at, const uint32_t* v) {
@@ -175,12 +199,12 @@ __device__ __forceinline__ void fs_row_p(uint32_t (&sc)[128], int blocks, float 
   }
 }
 
-template <int kD, int kW, int kMod>
-__global__ void __launch_bounds__(FS<kD, kW>::kThreads, FS<kD, kW>::kCtas)
+template <int kD, int kMod>
+__global__ void __launch_bounds__(FS<kD>::kThreads, FS<kD>::kCtas)
 flash_fwd_span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK,
                       const __grid_constant__ CUtensorMap tmV, const FlashSpanParams p) {
-  using L = FS<kD, kW>;
-  constexpr int kRing = L::kRing;
+  using L = FS<kD>;
+  constexpr int kW = L::kW, kRing = L::kRing;
   constexpr bool kOwnP = L::kOwnP;
   constexpr uint32_t kTile = L::kTile;
   extern __shared__ uint8_t fs_smem_raw[];
@@ -197,13 +221,18 @@ flash_fwd_span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   uint64_t* p_full = bars + 14;      // [w]: P_w has been written (128)
   uint64_t* pv_done = bars + 16;     // [w]: O_w includes the key tile whose P V was committed last
   uint64_t* o_free = bars + 18;      // [w]: O_w of an item has been read (128)
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 20);
+  uint64_t* u_full = bars + 20;      // the next unit's number has arrived
+  uint64_t* u_empty = bars + 21;     // every role has read it
+  uint4* answer = reinterpret_cast<uint4*>(bars + 22);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 24);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   if (threadIdx.x == 0) {
     mbar_init(q_full, 1);
     mbar_init(q_empty, 1);
+    mbar_init(u_full, 1);
+    mbar_init(u_empty, 1 + 4 * kW);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&k_full[s], 1);
       mbar_init(&k_empty[s], 1);
@@ -230,6 +259,7 @@ flash_fwd_span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   pdl_wait();                            // by every role: their bounded waits start counting behind it
   pdl_trigger();
   SpanItem it;
+  SpanQueue queue = {u_full, u_empty, answer, 0};
 
   if (warp == 0) {
     // ---------------------------------------------------------------- TMA producer
@@ -237,8 +267,9 @@ flash_fwd_span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     if (lane == 0) {
       int g = 0, active = 0;             // key tiles and items so far
       bool ok = true;
-      for (unsigned round = 0; ok && span_item<kW>(p, round, it); ++round) {
-        if (it.unit < 0 || it.steps == 0) continue;
+      for (int unit = blockIdx.x; ok && unit >= 0; unit = queue.ask(abort_flag)) {
+        span_item<kW>(p, unit, it);
+        if (it.steps == 0) continue;
         const int kvh = it.h / (p.QH / p.KVH);
         if (active > 0 && !mbar_wait(q_empty, (active - 1) & 1, abort_flag)) break;
         ++active;
@@ -273,8 +304,9 @@ flash_fwd_span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     int g0 = 0, active = 0;
     int tiles0 = 0, tiles1 = 0, outs0 = 0, outs1 = 0;      // key tiles and outputs that each warpgroup has had
     bool ok = true;
-    for (unsigned round = 0; ok && span_item<kW>(p, round, it); ++round) {
-      if (it.unit < 0 || it.steps == 0) continue;
+    for (int unit = blockIdx.x; ok && unit >= 0; unit = queue.next(abort_flag)) {
+      span_item<kW>(p, unit, it);
+      if (it.steps == 0) continue;
       auto issue_s = [&](int w, int j) {
         const uint64_t dQ = umma_smem_desc(smem_u32(smem + L::kQ + w * kTile), 16, 1024);
         const uint64_t dK = umma_smem_desc(smem_u32(smem + L::kK + ((g0 + j) % kRing) * kTile), 16, 1024);
@@ -379,14 +411,14 @@ flash_fwd_span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     int done = 0;                          // key tiles so far
     bool ok = true;
     // the next unit's tables and this row's keys in it are asked for before the present one's output is waited for
-    unsigned round = 0;
-    int b = 0, h = 0, mt = -1, first = 0, my_tiles = 0;      // mt < 0: nothing for this warpgroup in the round
+    int unit = blockIdx.x, b = 0, h = 0, mt = -1, first = 0, my_tiles = 0;      // mt < 0: nothing in the unit for this warpgroup
     int2 span = make_int2(0, 0);
     auto next_unit = [&]() {
+      if (unit < 0) return false;
       SpanItem u;
-      if (!span_item<kW>(p, round++, u)) return false;
+      span_item<kW>(p, unit, u);
       mt = kW * u.unit + w;
-      if (u.unit < 0 || mt >= p.n_tiles) mt = -1;
+      if (mt >= p.n_tiles) mt = -1;
       b = u.b;
       h = u.h;
       first = u.j0 + u.st[w];
@@ -397,6 +429,7 @@ flash_fwd_span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
     bool more = next_unit();
     while (ok && more) {
       if (mt < 0) {
+        unit = queue.next(abort_flag);
         more = next_unit();
         continue;
       }
@@ -516,6 +549,7 @@ flash_fwd_span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       bf16* out = p.o + b * p.o_bs + (long long)min(row, T - 1) * p.o_ts + h * p.o_hs;
       float* lse = p.lse + (size_t(b) * p.QH + h) * T + min(row, T - 1);
       const bool any = my_tiles > 0, live = row < T;
+      unit = queue.next(abort_flag);
       more = next_unit();
       if (any) {
         if (!__all_sync(0xffffffffu, mbar_wait(&pv_done[w], (done - 1) & 1, abort_flag))) { ok = false; break; }
@@ -559,33 +593,20 @@ flash_fwd_span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
   }
 }
 
-template <int kD, int kW, int kMod>
-static int launch_fwd_span_as(FlashSpanParams p, const TensorMap (&m)[3], cudaStream_t st) {
-  using L = FS<kD, kW>;
+template <int kD, int kMod>
+static int launch_fwd_span(FlashSpanParams p, const TensorMap (&m)[3], cudaStream_t st) {
+  using L = FS<kD>;
   static bool configured = false;
   if (!configured) {
-    B200_CHECK(cudaFuncSetAttribute(flash_fwd_span_kernel<kD, kW, kMod>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem));
+    B200_CHECK(cudaFuncSetAttribute(flash_fwd_span_kernel<kD, kMod>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem));
     configured = true;
   }
-  p.n_units = (p.n_tiles + kW - 1) / kW;
+  p.n_units = (p.n_tiles + L::kW - 1) / L::kW;
   const long long items = (long long)p.n_units * p.QH * p.B;
-  const unsigned most = unsigned(num_sms()) * L::kCtas;
   if (items > 0x7fffffffLL) return static_cast<int>(cudaErrorInvalidValue);
-  p.items = unsigned(items);
-  p.order += kW == 2 ? (size_t)p.B * p.n_tiles : 0;      // the orders of pairs stand behind those of single tiles
-  const unsigned grid = p.items < most ? p.items : most;
-  return static_cast<int>(launch_pdl(flash_fwd_span_kernel<kD, kW, kMod>, dim3(grid), dim3(L::kThreads), L::kSmem, st, 0, *m[0], *m[1], *m[2], p));
-}
-
-static int g_span_pairs = -1;       // head_dim 128: -1: by the rule below; 0 / 1: forced (A/B runs and tests)
-
-template <int kD, int kMod>
-static int launch_fwd_span(const FlashSpanParams& p, const TensorMap (&m)[3], cudaStream_t st) {
-  if constexpr (kD == 128) {
-    const bool pairs = g_span_pairs >= 0 ? g_span_pairs != 0 : true;
-    if (pairs) return launch_fwd_span_as<128, 2, kMod>(p, m, st);
-  }
-  return launch_fwd_span_as<kD, 1, kMod>(p, m, st);
+  if (L::kW == 2) p.order += (size_t)p.B * p.n_tiles;      // the orders of pairs stand behind those of single tiles
+  return static_cast<int>(launch_pdl(flash_fwd_span_kernel<kD, kMod>, dim3(unsigned(items)), dim3(L::kThreads), L::kSmem, st, 0, *m[0], *m[1],
+                                     *m[2], p));
 }
 
 }  // namespace b200
@@ -632,11 +653,4 @@ B200_API int b200_flash_fwd_span(const void* q, const void* k, const void* v, vo
   }
   if (cap > 0.f) return launch_fwd_span<64, kSpanCap>(p, m, st);
   return slopes != nullptr ? launch_fwd_span<64, kSpanBias>(p, m, st) : launch_fwd_span<64, kSpanOnly>(p, m, st);
-}
-
-// Query tiles of head_dim 128 that walk their keys together: -1 (default) by the sizes, 0 one, 1 two. Returns the previous value.
-B200_API int b200_flash_span_pairs(int mode) {
-  const int old = g_span_pairs;
-  if (mode >= -1 && mode <= 1) g_span_pairs = mode;
-  return old;
 }

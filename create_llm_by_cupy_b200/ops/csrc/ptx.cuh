@@ -60,6 +60,27 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
+// A CTA takes the work of one that the grid has not started yet: asks for it (16 bytes to `resp`, counted on `bar`); one thread. The answer's
+// first coordinate, or -1 when nothing was left: then it is not asked again.
+__device__ __forceinline__ void take_cta(void* resp, uint64_t* bar) {
+  asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
+               ::"r"(smem_u32(resp)), "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ int taken_cta(const void* resp) {
+  int x;
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .b128 a;\n\t.reg .pred p;\n\t"
+      "ld.shared.b128 a, [%2];\n\t"
+      "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+      "selp.u32 %1, 1, 0, p;\n\t"
+      "mov.b32 %0, 0;\n\t"
+      "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%0, _, _, _}, a;\n\t}"
+      : "=r"(x), "=r"(ok)
+      : "r"(smem_u32(resp))
+      : "memory");
+  return ok != 0 ? x : -1;
+}
 // Bounded wait. `abort_flag` lives in shared memory and is shared by all roles of the CTA.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag) {
   if (mbar_try_wait(bar, parity)) return true;
