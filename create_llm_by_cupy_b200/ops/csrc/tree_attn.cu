@@ -243,20 +243,24 @@ __device__ __forceinline__ unsigned long long combo_first(const TreeParams& p, c
   return before * (p.KVH * p.groups) + (unsigned long long)(s.kvh * p.groups + s.rg) * s.nt;
 }
 
-// Four columns of one row's result from its pieces, in the order of the keys; eight pieces' loads at a time.
-template <int kD>
-__device__ __forceinline__ void tree_join_task(const TreeParams& p, int b, int kvh, int rt, int w, int r, int chunk, const TreePieces& pc) {
-  constexpr int kBatch = 8;
-  float m = -INFINITY, l = 0.f, a[4] = {0.f, 0.f, 0.f, 0.f};
+// 4 kQuads columns of one row's result from its pieces, in the order of the keys; some pieces' loads at a time.
+template <int kD, int kQuads>
+__device__ __forceinline__ void tree_join_task(const TreeParams& p, int b, int kvh, int rt, int w, int r, int part, const TreePieces& pc) {
+  constexpr int kBatch = 8 / kQuads;
+  float m = -INFINITY, l = 0.f, a[4 * kQuads];
+#pragma unroll
+  for (int e = 0; e < 4 * kQuads; ++e) a[e] = 0.f;
 #pragma unroll 1
   for (int c = pc.c0; c <= pc.c1; c += kBatch) {
     float2 ml[kBatch];
-    float4 o[kBatch];
+    float4 o[kBatch][kQuads];
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
-      const size_t slot = pc.slot(min(c + u, pc.c1), w);
+      const unsigned slot = pc.slot(min(c + u, pc.c1), w);
       ml[u] = p.part_ml[slot * 128 + r];
-      o[u] = p.part_o[(slot * (kD / 4) + chunk) * 128 + r];
+      const float4* at = p.part_o + ((size_t)slot * (kD / 4) + kQuads * part) * 128 + r;
+#pragma unroll
+      for (int k = 0; k < kQuads; ++k) o[u][k] = at[128 * k];
     }
     float mx = m;
 #pragma unroll
@@ -265,24 +269,31 @@ __device__ __forceinline__ void tree_join_task(const TreeParams& p, int b, int k
     m = mx;
     l *= corr;
 #pragma unroll
-    for (int e = 0; e < 4; ++e) a[e] *= corr;
+    for (int e = 0; e < 4 * kQuads; ++e) a[e] *= corr;
 #pragma unroll
     for (int u = 0; u < kBatch; ++u) {
       const float f = c + u <= pc.c1 ? exp2f(ml[u].x - ref) : 0.f;
       l += ml[u].y * f;
-      a[0] += o[u].x * f;
-      a[1] += o[u].y * f;
-      a[2] += o[u].z * f;
-      a[3] += o[u].w * f;
+#pragma unroll
+      for (int k = 0; k < kQuads; ++k) {
+        a[4 * k] += o[u][k].x * f;
+        a[4 * k + 1] += o[u][k].y * f;
+        a[4 * k + 2] += o[u][k].z * f;
+        a[4 * k + 3] += o[u][k].w * f;
+      }
     }
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   const int d = rt * p.tok + r / p.R, h = kvh * p.R + r % p.R;
-  const bf162 x = __floats2bfloat162_rn(a[0] * inv, a[1] * inv), y = __floats2bfloat162_rn(a[2] * inv, a[3] * inv);
-  uint2 u;
-  u.x = *reinterpret_cast<const uint32_t*>(&x);
-  u.y = *reinterpret_cast<const uint32_t*>(&y);
-  *reinterpret_cast<uint2*>(p.out + ((size_t(b) * p.n + d) * p.QH + h) * kD + chunk * 4) = u;
+  uint32_t u[2 * kQuads];
+#pragma unroll
+  for (int e = 0; e < 2 * kQuads; ++e) {
+    const bf162 x = __floats2bfloat162_rn(a[2 * e] * inv, a[2 * e + 1] * inv);
+    u[e] = *reinterpret_cast<const uint32_t*>(&x);
+  }
+  bf16* out = p.out + ((size_t(b) * p.n + d) * p.QH + h) * kD + part * 4 * kQuads;
+  if constexpr (kQuads == 2) *reinterpret_cast<uint4*>(out) = make_uint4(u[0], u[1], u[2], u[3]);
+  else *reinterpret_cast<uint2*>(out) = make_uint2(u[0], u[1]);
 }
 
 template <int kD, int kMod>
@@ -685,7 +696,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         ++parts;
         if (*is_last != 0) {
           __threadfence();
-          for (int i = r; i < live * (kD / 4); i += 128) tree_join_task<kD>(p, s.b, s.kvh, 2 * s.rg, 0, i % live, i / live, pc);
+          for (int i = r; i < live * (kD / 4); i += 128) tree_join_task<kD, 1>(p, s.b, s.kvh, 2 * s.rg, 0, i % live, i / live, pc);
         }
       }
     }
@@ -702,8 +713,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   }
 }
 
-// Joins the pieces of every (sequence, KV head, row group) that was cut: grid (those, rows * D / 4 / 256), a thread four columns of a row.
-template <int kD>
+// Joins the pieces of every (sequence, KV head, row group) that was cut: grid (those, rows * D / (4 kQuads) / 256).
+template <int kD, int kQuads>
 __global__ void __launch_bounds__(256)
 tree_join_kernel(const TreeParams p) {
   const int lane = threadIdx.x & 31;
@@ -720,9 +731,9 @@ tree_join_kernel(const TreeParams p) {
   }
   const TreePieces pc = tree_pieces(p, sum * per, before * per + (unsigned long long)idx * nt, nt);
   if (pc.c0 == pc.c1) return;
-  const int rows = p.tok * p.R, task = blockIdx.y * 256 + threadIdx.x, all = p.n > p.tok ? 2 * rows : rows, row = task % all, chunk = task / all;
+  const int rows = p.tok * p.R, task = blockIdx.y * 256 + threadIdx.x, all = p.n > p.tok ? 2 * rows : rows, row = task % all, part = task / all;
   const int w = row >= rows ? 1 : 0, r = row - w * rows, rt = 2 * rg + w;
-  if (chunk < kD / 4 && r < min(p.n - rt * p.tok, p.tok) * p.R) tree_join_task<kD>(p, b, kvh, rt, w, r, chunk, pc);
+  if (part < kD / (4 * kQuads) && r < min(p.n - rt * p.tok, p.tok) * p.R) tree_join_task<kD, kQuads>(p, b, kvh, rt, w, r, part, pc);
 }
 
 template <int kD, int kMod>
@@ -736,7 +747,12 @@ static int launch_tree(const TreeParams& p, const TensorMap& tq, const TensorMap
   B200_CHECK(launch_pdl(tree_append_kernel<kD>, dim3(unsigned((chunks + 255) / 256)), dim3(256), 0, st, 0, p));
   B200_CHECK(launch_pdl(tree_attn_kernel<kD, kMod>, dim3(p.ctas), dim3(TA_THREADS), TA<kD>::kSmem, st, 0, *tq, *tk, *tv, p));
   if (p.arrived != nullptr) return 0;
-  return static_cast<int>(launch_pdl(tree_join_kernel<kD>, dim3(p.B * p.KVH * p.groups, ((p.n > p.tok ? 2 : 1) * p.tok * p.R * (kD / 4) + 255) / 256), dim3(256), 0, st, 0, p));
+  // Eight columns to a thread where there are threads enough (8 x 3000 keys, 24 drafts, 32 / 8 heads of 128 43 us with four, 40 like this),
+  // four and more pieces at a time else (1 x 60001 keys, 32 drafts 63.5, 65 with eight).
+  const int combos = p.B * p.KVH * p.groups, rows = (p.n > p.tok ? 2 : 1) * p.tok * p.R;
+  if ((long long)combos * rows * (kD / 8) >= 256LL * num_sms())
+    return static_cast<int>(launch_pdl(tree_join_kernel<kD, 2>, dim3(combos, (rows * (kD / 8) + 255) / 256), dim3(256), 0, st, 0, p));
+  return static_cast<int>(launch_pdl(tree_join_kernel<kD, 1>, dim3(combos, (rows * (kD / 4) + 255) / 256), dim3(256), 0, st, 0, p));
 }
 
 // Groups of two tiles of 128 / R drafts.
