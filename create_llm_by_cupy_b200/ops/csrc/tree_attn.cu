@@ -7,7 +7,7 @@
 //   x = q k scale, capped (c tanh(x / c)) or biased (x - slope |distance|);  o = softmax(x) V
 //
 // The rows of a tile are the drafts times the query heads that share a KV head: every key is read once for all of them, which is
-// all that bounds the kernel while there are few (64 rows of head_dim 128 do 64 multiply-adds per byte read). The work is one
+// all that bounds the kernel while there are few (64 rows of head_dim 128 do 96 multiply-adds per byte read). The work is one
 // list of 128-key tiles, over sequences, KV heads and groups of up to 256 rows, the drafts a tile of their own behind each
 // sequence's cached ones; the list is cut into as many equal pieces as there are SMs, so sequences of any mix of lengths keep all
 // of them busy. A piece that is not all of its rows' keys leaves its maximum, sum and values in a workspace, and a last kernel
@@ -18,7 +18,11 @@
 // (columns S_0, S_1, O_0, O_1; P lies over S). A group of more than 128 rows gives each warpgroup a tile of rows; one of up to 128
 // gives them the odd and the even key tiles, and the first one adds up what the two have. Either way the tensor core works for one
 // while the other is in its exponentials: with one warpgroup a tile took 2.1 us at 128 rows of head_dim 128 where its 64 KiB
-// arrive in 1.5.
+// arrive in 1.5. The whole call at 32 drafts, 32 / 8 heads of 128: 17 us at 1000 keys, 69 at 60000, 114 at 120000 (0.74 us per 1000 keys, 5.5 TB/s,
+// and 25 us of three launches, the ramp and the join).
+//
+// Roundings to bf16: rotated K and V, as the caches hold them; Q in two parts, which is 16 bits; P, for the tensor core (sums of P and
+// the accumulators are fp32); the result.
 // Cached rows past the length, which may hold anything, are masked as scores and cleared as values. Every wait is bounded (see
 // ptx.cuh).
 #include <algorithm>
@@ -42,7 +46,7 @@ struct TreeParams {
   const bf16* kqv;          // [B * n][ld]: K | Q | V
   bf16* kc;                 // [B, KVH, Tmax, D]
   bf16* vc;
-  bf16* q;                  // [B, n, QH, D]: rotated
+  bf16* q;                  // [2, B, n, QH, D]: rotated, as bf16 and what that leaves, as bf16 again
   bf16* out;                // [B, n, QH, D]
   const int* lens;          // [B]
   const unsigned long long* tree;   // [B, n]: bit j: draft i sees draft j
@@ -61,11 +65,13 @@ struct TreeParams {
   int* status;
 };
 
-template <int kD>
+// kPair: there are groups of two row tiles.
+template <int kD, bool kPair>
 struct TA {
   static constexpr int kTile = 128 * kD * 2;
-  static constexpr int kStK = kD == 128 ? 2 : 4, kStV = kD == 128 ? 3 : 4;      // rings of K and V
-  static constexpr int kQ = 0, kK = 2 * kTile, kV = kK + kStK * kTile;
+  // Rings of K and V. Two row tiles take more of the memory, and twice the time for a key tile.
+  static constexpr int kStK = kD == 64 ? 4 : kPair ? 1 : 2, kStV = kD == 64 ? 4 : kPair ? 2 : 3;
+  static constexpr int kQ = 0, kK = (kPair ? 4 : 2) * kTile, kV = kK + kStK * kTile;       // Q: the two parts of each row tile
   static constexpr int kBar = kV + kStV * kTile;
   // k_full, k_empty [kStK]; v_full, v_empty [kStV]; q_full, q_empty; s_full, p_half, p_full, pv_done, o_free [2]; ml_full, ml_empty;
   // part_out, last_known
@@ -126,7 +132,7 @@ struct TreeWalk {
     s.nt = tree_tiles(s.len);
     s.kvh = idx / p.groups;
     s.rg = idx % p.groups;
-    s.pair = p.n > (2 * s.rg + 1) * p.tok;
+    s.pair = p.n > (2 * s.rg + 1) * p.tok;        // (never where no group has two)
     s.t0 = tile;
     s.t1 = int(min((long long)s.nt, tile + left));
     left -= s.t1 - s.t0;
@@ -151,10 +157,10 @@ __device__ __forceinline__ void ta_unpack(const uint4& u, float (&f)[8]) {
   }
 }
 
-// 8 elements from chunk `c` of the head at `x`, rotated by the table row of `pos` (half-split pairs) and rounded to bf16: the type
-// of the cache, and of the tensor core's operands.
+// 8 elements from chunk `c` of the head at `x`, rotated by the table row of `pos` (half-split pairs) and rounded to bf16, the type of the
+// cache and of the tensor core's operands; in `rest` what that leaves, as bf16.
 template <int kD>
-__device__ __forceinline__ uint4 ta_rotated(const TreeParams& p, const bf16* x, int c, int pos) {
+__device__ __forceinline__ uint4 ta_rotated(const TreeParams& p, const bf16* x, int c, int pos, uint4& rest) {
   constexpr int kHalf = kD / 16;
   float a[8], b[8];
   ta_unpack(reinterpret_cast<const uint4*>(x)[c], a);
@@ -162,7 +168,7 @@ __device__ __forceinline__ uint4 ta_rotated(const TreeParams& p, const bf16* x, 
   const int j = (c % kHalf) * 8;
   const size_t row = size_t(min(max(pos, 0), p.table_rows - 1)) * (kD / 2) + j;
   uint4 u;
-  uint32_t* w = reinterpret_cast<uint32_t*>(&u);
+  uint32_t *w = reinterpret_cast<uint32_t*>(&u), *v = reinterpret_cast<uint32_t*>(&rest);
 #pragma unroll
   for (int h = 0; h < 2; ++h) {
     const float4 cs = *reinterpret_cast<const float4*>(p.cosr + row + 4 * h), sn = *reinterpret_cast<const float4*>(p.sinr + row + 4 * h);
@@ -173,7 +179,10 @@ __device__ __forceinline__ uint4 ta_rotated(const TreeParams& p, const bf16* x, 
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const bf162 t = __floats2bfloat162_rn(y[2 * e], y[2 * e + 1]);
+      const float2 f = __bfloat1622float2(t);
+      const bf162 l = __floats2bfloat162_rn(y[2 * e] - f.x, y[2 * e + 1] - f.y);
       w[2 * h + e] = *reinterpret_cast<const uint32_t*>(&t);
+      v[2 * h + e] = *reinterpret_cast<const uint32_t*>(&l);
     }
   }
   return u;
@@ -181,7 +190,7 @@ __device__ __forceinline__ uint4 ta_rotated(const TreeParams& p, const bf16* x, 
 
 __device__ __forceinline__ int tree_depth(unsigned long long bits) { return max(__popcll(bits) - 1, 0); }
 
-// A thread per 16 bytes of the packed projection: K (rotated) and V to the caches, Q (rotated) to its workspace.
+// A thread per 16 bytes of the packed projection: K (rotated) and V to the caches, Q (rotated, in two parts) to its workspace.
 template <int kD>
 __global__ void __launch_bounds__(256)
 tree_append_kernel(const TreeParams p) {
@@ -199,12 +208,17 @@ tree_append_kernel(const TreeParams p) {
   const int len = tree_len(p, b), pos = len + tree_depth(p.tree[row]);
   const bf16* x = p.kqv + row * p.ld + head * kD;
   if (head >= p.KVH && head < p.KVH + p.QH) {
-    reinterpret_cast<uint4*>(p.q + (row * p.QH + head - p.KVH) * kD)[c] = ta_rotated<kD>(p, x, c, pos);
+    uint4 rest;
+    const uint4 u = ta_rotated<kD>(p, x, c, pos, rest);
+    bf16* q = p.q + (row * p.QH + head - p.KVH) * kD;
+    reinterpret_cast<uint4*>(q)[c] = u;
+    reinterpret_cast<uint4*>(q + (size_t)p.B * p.n * p.QH * kD)[c] = rest;
     return;
   }
   const bool value = head >= p.KVH;
   if (len + d >= p.Tmax) return;
-  const uint4 u = value ? reinterpret_cast<const uint4*>(x)[c] : ta_rotated<kD>(p, x, c, pos);
+  uint4 rest;                                            // (the cache holds bf16)
+  const uint4 u = value ? reinterpret_cast<const uint4*>(x)[c] : ta_rotated<kD>(p, x, c, pos, rest);
   const int kvh = value ? head - p.KVH - p.QH : head;
   reinterpret_cast<uint4*>((value ? p.vc : p.kc) + ((size_t(b) * p.KVH + kvh) * p.Tmax + len + d) * kD)[c] = u;
 }
@@ -296,11 +310,11 @@ __device__ __forceinline__ void tree_join_task(const TreeParams& p, int b, int k
   else *reinterpret_cast<uint2*>(out) = make_uint2(u[0], u[1]);
 }
 
-template <int kD, int kMod>
+template <int kD, int kMod, bool kPair>
 __global__ void __launch_bounds__(TA_THREADS, 1)
 tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant__ CUtensorMap tmK, const __grid_constant__ CUtensorMap tmV,
                  const TreeParams p) {
-  using L = TA<kD>;
+  using L = TA<kD, kPair>;
   constexpr int kStK = L::kStK, kStV = L::kStV;
   constexpr uint32_t kTile = L::kTile;
   extern __shared__ uint8_t ta_smem_raw[];
@@ -400,12 +414,12 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       while (ok && walk.next(p, s)) {
         if (seg > 0 && !mbar_wait(q_empty, (seg - 1) & 1, abort_flag)) break;
         ++seg;
-        mbar_expect_tx(q_full, uint32_t((s.pair ? 2 : 1) * p.R * p.tok) * kD * 2);   // (rows past the box: whatever, their results go nowhere)
-        for (int w = 0; w < (s.pair ? 2 : 1); ++w) {
-          const int d0 = (2 * s.rg + w) * p.tok;
-          uint8_t* sQ = smem + L::kQ + w * kTile;
-          tma_load_4d(sQ, &tmQ, q_full, 0, s.kvh * p.R, d0, s.b);
-          if (kD == 128) tma_load_4d(sQ + 16384, &tmQ, q_full, 64, s.kvh * p.R, d0, s.b);
+        mbar_expect_tx(q_full, uint32_t((s.pair ? 4 : 2) * p.R * p.tok) * kD * 2);   // (rows past the box: whatever, their results go nowhere)
+        for (int i = 0; i < (s.pair ? 4 : 2); ++i) {                     // row tile i / 2, part i % 2
+          const int d0 = (2 * s.rg + (i >> 1)) * p.tok, b = s.b + (i & 1) * p.B;
+          uint8_t* sQ = smem + L::kQ + i * kTile;
+          tma_load_4d(sQ, &tmQ, q_full, 0, s.kvh * p.R, d0, b);
+          if (kD == 128) tma_load_4d(sQ + 16384, &tmQ, q_full, 64, s.kvh * p.R, d0, b);
         }
         for (int t = s.t0; t < s.t1; ++t, ++g) {
           const int row = t == s.nt - 1 ? s.len : t * 128;               // the drafts stand behind the cached keys
@@ -437,13 +451,18 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const int t = u >> sh, g = g0 + t, w = u & 1;
         if ((!s.pair || w == 0) && !mbar_wait_warp(&k_full[g % kStK], (g / kStK) & 1, abort_flag)) return false;
         tc_fence_after();
-        const uint64_t dQ = umma_smem_desc(smem_u32(smem + L::kQ + (s.pair ? w : 0) * kTile), 16, 1024);
+        const uint64_t dQ = umma_smem_desc(smem_u32(smem + L::kQ + (s.pair ? 2 * w : 0) * kTile), 16, 1024);
         const uint64_t dK = umma_smem_desc(smem_u32(smem + L::kK + (g % kStK) * kTile), 16, 1024);
         const bool drafts = s.t0 + t == s.nt - 1;        // 64 keys are enough for them
+        // Q's two parts, so that the scores are those of an unrounded rotation. Rounded to bf16 it was the largest error of the result: 4.4e-3
+        // of it at 60001 keys, 2.2e-3 like this, of which the result's own rounding is 1.7e-3. It costs 0 to 8 % of the whole call's time at up
+        // to 3200 keys, 15 % at 60001 (67 -> 77 us).
 #pragma unroll
-        for (int kk = 0; kk < kD / 16; ++kk) {
-          const uint32_t off = ((kk >> 2) * 16384 + (kk & 3) * 32) >> 4;
-          umma_bf16_ss_warp(tmem_base + L::kColS + w * 128, dQ + off, dK + off, drafts ? idesc_s64 : idesc_s, kk != 0);
+        for (int kk = 0; kk < kD / 8; ++kk) {
+          const int k = kk % (kD / 16);
+          const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
+          umma_bf16_ss_warp(tmem_base + L::kColS + w * 128, dQ + (kk / (kD / 16)) * (kTile >> 4) + off, dK + off, drafts ? idesc_s64 : idesc_s,
+                            kk != 0);
         }
         umma_commit_warp(&s_full[w]);
         if (!s.pair || w == 1) umma_commit_warp(&k_empty[g % kStK]);
@@ -736,16 +755,23 @@ tree_join_kernel(const TreeParams p) {
   if (part < kD / (4 * kQuads) && r < min(p.n - rt * p.tok, p.tok) * p.R) tree_join_task<kD, kQuads>(p, b, kvh, rt, w, r, part, pc);
 }
 
-template <int kD, int kMod>
-static int launch_tree(const TreeParams& p, const TensorMap& tq, const TensorMap& tk, const TensorMap& tv, cudaStream_t st) {
+template <int kD, int kMod, bool kPair>
+static int launch_tree_attn(const TreeParams& p, const TensorMap& tq, const TensorMap& tk, const TensorMap& tv, cudaStream_t st) {
+  using L = TA<kD, kPair>;
   static bool configured = false;
   if (!configured) {
-    B200_CHECK(cudaFuncSetAttribute(tree_attn_kernel<kD, kMod>, cudaFuncAttributeMaxDynamicSharedMemorySize, TA<kD>::kSmem));
+    B200_CHECK(cudaFuncSetAttribute(tree_attn_kernel<kD, kMod, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, L::kSmem));
     configured = true;
   }
+  return static_cast<int>(launch_pdl(tree_attn_kernel<kD, kMod, kPair>, dim3(p.ctas), dim3(TA_THREADS), L::kSmem, st, 0, *tq, *tk, *tv, p));
+}
+
+template <int kD, int kMod>
+static int launch_tree(const TreeParams& p, const TensorMap& tq, const TensorMap& tk, const TensorMap& tv, cudaStream_t st) {
   const long long chunks = (long long)p.B * p.n * (p.QH + 2 * p.KVH) * (kD / 8);
   B200_CHECK(launch_pdl(tree_append_kernel<kD>, dim3(unsigned((chunks + 255) / 256)), dim3(256), 0, st, 0, p));
-  B200_CHECK(launch_pdl(tree_attn_kernel<kD, kMod>, dim3(p.ctas), dim3(TA_THREADS), TA<kD>::kSmem, st, 0, *tq, *tk, *tv, p));
+  const int rc = p.n > p.tok ? launch_tree_attn<kD, kMod, true>(p, tq, tk, tv, st) : launch_tree_attn<kD, kMod, false>(p, tq, tk, tv, st);
+  if (rc != 0) return rc;
   if (p.arrived != nullptr) return 0;
   // Eight columns to a thread where there are threads enough (8 x 3000 keys, 24 drafts, 32 / 8 heads of 128 43 us with four, 40 like this),
   // four and more pieces at a time else (1 x 60001 keys, 32 drafts 63.5, 65 with eight).
@@ -776,7 +802,7 @@ using namespace b200;
 // Bytes of the workspace that b200_tree_attn_append wants (16-byte aligned); 0: sizes that it does not take.
 B200_API long long b200_tree_attn_workspace(int B, int n, int QH, int KVH, int Tmax, int D) {
   if (!tree_shape_ok(B, n, QH, KVH, Tmax, D)) return 0;
-  return 4LL * tree_ctas(B, n, QH, KVH, Tmax) * 128 * (D * 4 + 8) + 2LL * B * n * QH * D + 4LL * B * KVH * tree_groups(n, QH / KVH);
+  return 4LL * tree_ctas(B, n, QH, KVH, Tmax) * 128 * (D * 4 + 8) + 4LL * B * n * QH * D + 4LL * B * KVH * tree_groups(n, QH / KVH);
 }
 
 // kqv [B * n][ld] (K | Q | V, un-rotated), caches [B, KVH, Tmax, D], out [B, n, QH, D], lens [B], tree [B, n] (64 bits each), rotary
@@ -814,11 +840,11 @@ B200_API int b200_tree_attn_append(const void* kqv, void* kc, void* vc, void* ou
   // more than that; more of them would keep that one SM busy for longer.
   const long long combos = (long long)B * KVH * p.groups;
   p.arrived = n * p.R <= 8 && (p.ctas / combos + 2) * n * p.R <= 512
-                  ? reinterpret_cast<int*>(p.q + (size_t)B * n * QH * D) : nullptr;
+                  ? reinterpret_cast<int*>(p.q + 2 * (size_t)B * n * QH * D) : nullptr;
   p.scale = scale;
   p.cap = make_score_cap(scale, cap);
   p.status = status_ptr();
-  const TensorMap tq = get_tensor_map_bthd(p.q, B, n, QH, D, (unsigned long long)n * QH * D, (unsigned long long)QH * D, D, p.tok, 64, p.R);
+  const TensorMap tq = get_tensor_map_bthd(p.q, 2 * B, n, QH, D, (unsigned long long)n * QH * D, (unsigned long long)QH * D, D, p.tok, 64, p.R);
   if (!tq || !tk || !tv) return static_cast<int>(cudaErrorInvalidValue);
   if (D == 128) {
     if (cap > 0.f) return launch_tree<128, kTreeCap>(p, tq, tk, tv, st);
