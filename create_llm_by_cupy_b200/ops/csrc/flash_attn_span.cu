@@ -12,10 +12,13 @@
 //     with most to do first, and a CTA that is about to finish one takes the next that the grid has not started (with a fixed share of
 //     the list for each the slowest took 20 to 30 % longer than the mean: what a tile costs is not its keys alone);
 //   * loads of the next tile's Q, K and V start when the last scores of the present one are done, its first scores when the last P V
-//     is, and the output leaves through a staging buffer of its own while they run.
+//     is, and the output leaves straight from tensor memory while they run.
 //
-// What bounds it then: as in the causal forward a tile's chain scores -> maximum -> exp2 -> P V, 2.1 us a step at head_dim 128, and
-// masked parts of tiles (18 to 68 % of the pairs that are computed at the documents above).
+// What bounds it then: a tile's exponentials (2048 of a warpgroup's 2242 clocks a tile), the chain scores -> maximum -> exp2 -> P V
+// around them, and masked parts of tiles (18 to 68 % of the pairs that are computed at the documents above). Measured, 32 / 8 heads
+// of 128: 4096 tokens in documents of 700 97 us with the mask's tables; 16 / 4 heads, a cap, 8192 tokens in documents of 600 85 us.
+//
+// Roundings to bf16: P, for the tensor core (its sums are fp32), and the output.
 //
 //   tensor memory, head_dim 128: S_0, S_1 (P over them), O_0, O_1, 128 columns each;  64: S, O, P
 #include <climits>
@@ -151,18 +154,11 @@ __device__ __forceinline__ float fs_max3(float a, float b, float c) {
   return r;
 }
 
-// What the 32 rows of a warp see of 32 consecutive keys: nothing, all of it, or some rows some of it. A mask costs a tile three
-// operations per score on a pipe that takes two clocks for each (a masked tile took 3 us where others take 1.3); by blocks, what nobody
-// sees costs nothing, not even its exponentials, and of the diagonal only one block in four is masked score by score.
-constexpr int kBlockNone = 0, kBlockAll = 1, kBlockSome = 2;
-
+// The keys that a thread's row sees, and those that every row of its warp sees: a tile inside the latter needs no mask, which costs a tile
+// three operations per score (a masked tile keeps a warpgroup for 3100 to 3500 clocks, another for 2242). Skipping the 32-key
+// blocks of a masked tile that no row of the warp sees was slower: its branches part the loads from the arithmetic.
 struct RowSpans {
-  int lo, hi;                              // of this thread's row
-  int lo_min, lo_max, hi_min, hi_max;      // over the warp's rows
-  __device__ __forceinline__ int block(int key) const {
-    if (key >= hi_max || key + 32 <= lo_min) return kBlockNone;
-    return key >= lo_max && key + 32 <= hi_min ? kBlockAll : kBlockSome;
-  }
+  int lo, hi, all_lo, all_hi;
 };
 
 // Maximum of 32 scores of one row from key `key` on; masked ones become -inf in place.
@@ -181,21 +177,17 @@ __device__ __forceinline__ float fs_block_max(uint32_t (&sc)[32], int key, const
   return fmaxf(mx[0], mx[1]);
 }
 
-// P = exp2(s * sl2 - m) for scores [kLo, kHi) of one row, packed to bf16 pairs in place; adds to the two partial row sums. `blocks`: two
-// bits for every 32 keys.
+// P = exp2(s * sl2 - m) for scores [kLo, kHi) of one row, packed to bf16 pairs in place; adds to the two partial row sums.
 template <int kLo, int kHi>
-__device__ __forceinline__ void fs_row_p(uint32_t (&sc)[128], int blocks, float sl2, float m, float& rs0, float& rs1) {
+__device__ __forceinline__ void fs_row_p(uint32_t (&sc)[128], float sl2, float m, float& rs0, float& rs1) {
 #pragma unroll
-  for (int b = kLo / 32; b < kHi / 32; ++b) {
-#pragma unroll
-    for (int e = 32 * b; e < 32 * b + 32; e += 2) {
-      const float p0 = exp2f(fmaf(__uint_as_float(sc[e]), sl2, -m));
-      const float p1 = exp2f(fmaf(__uint_as_float(sc[e + 1]), sl2, -m));
-      rs0 += p0;
-      rs1 += p1;
-      const bf162 t = __floats2bfloat162_rn(p0, p1);
-      sc[e >> 1] = *reinterpret_cast<const uint32_t*>(&t);
-    }
+  for (int e = kLo; e < kHi; e += 2) {
+    const float p0 = exp2f(fmaf(__uint_as_float(sc[e]), sl2, -m));
+    const float p1 = exp2f(fmaf(__uint_as_float(sc[e + 1]), sl2, -m));
+    rs0 += p0;
+    rs1 += p1;
+    const bf162 t = __floats2bfloat162_rn(p0, p1);
+    sc[e >> 1] = *reinterpret_cast<const uint32_t*>(&t);
   }
 }
 
@@ -436,13 +428,10 @@ flash_fwd_span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       const int row = mt * 128 + rloc;
       RowSpans spans;
       {
-        const bool none = span.y <= span.x;                // a row that sees nothing: of no use for all, in nobody's way for nothing
         spans.lo = span.x;
         spans.hi = span.y;
-        spans.lo_min = __reduce_min_sync(0xffffffffu, none ? INT_MAX : span.x);
-        spans.lo_max = __reduce_max_sync(0xffffffffu, none ? INT_MAX : span.x);
-        spans.hi_min = __reduce_min_sync(0xffffffffu, span.y);
-        spans.hi_max = __reduce_max_sync(0xffffffffu, span.y);
+        spans.all_lo = __reduce_max_sync(0xffffffffu, span.y <= span.x ? INT_MAX : span.x);
+        spans.all_hi = __reduce_min_sync(0xffffffffu, span.y);
       }
       const float slope2 = kMod == kSpanBias ? p.slopes[h] * kFsLog2e : 0.f;
       float m_ref = -INFINITY, l_run = 0.f;          // reference maximum (log2 units) and the row sum relative to it
@@ -450,11 +439,7 @@ flash_fwd_span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         if (!mbar_wait(&s_full[w], done & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
         const int key0 = (first + j) * 128;
-        int blocks = 0;                    // two bits for each 32 keys
-#pragma unroll
-        for (int b = 0; b < 4; ++b) blocks |= spans.block(key0 + 32 * b) << (2 * b);
-        const bool full = blocks == 0x55;
-        blocks = full ? 0x55 : 0xaa;
+        const bool full = key0 >= spans.all_lo && key0 + 128 <= spans.all_hi;
         // The whole row in one go: four loads, one wait.
         uint32_t sc[128];
         tmem_ld_32x32b_x32(tS, *reinterpret_cast<uint32_t(*)[32]>(&sc[0]));
@@ -519,21 +504,21 @@ flash_fwd_span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
         const float m_sub = m_ref == -INFINITY ? 0.f : m_ref;      // nothing seen yet: exp2(-inf) is 0
         if (kOwnP) {
           if (kMod == kSpanCap && cap_now) cap_row_p<0, 128>(sc, p.cap, m_sub, rs0, rs1);
-          else fs_row_p<0, 128>(sc, blocks, sl2, m_sub, rs0, rs1);
+          else fs_row_p<0, 128>(sc, sl2, m_sub, rs0, rs1);
           // P_w has been read (across items too: the output's way out waited for the last one)
           if (j > 0 && !__all_sync(0xffffffffu, mbar_wait(&pv_done[w], (done - 1) & 1, abort_flag))) { ok = false; break; }
           tc_fence_after();
         } else {
           // head_dim 128: the next scores wait for this P V, so its first half is handed over early
           if (kMod == kSpanCap && cap_now) cap_row_p<0, 64>(sc, p.cap, m_sub, rs0, rs1);
-          else fs_row_p<0, 64>(sc, blocks, sl2, m_sub, rs0, rs1);
+          else fs_row_p<0, 64>(sc, sl2, m_sub, rs0, rs1);
           tmem_st_32x32b_x16(tP, *reinterpret_cast<const uint32_t(*)[16]>(&sc[0]));
           tmem_st_32x32b_x16(tP + 16, *reinterpret_cast<const uint32_t(*)[16]>(&sc[16]));
           tmem_st_wait();
           tc_fence_before();
           mbar_arrive(&early[w]);
           if (kMod == kSpanCap && cap_now) cap_row_p<64, 128>(sc, p.cap, m_sub, rs0, rs1);
-          else fs_row_p<64, 128>(sc, blocks, sl2, m_sub, rs0, rs1);
+          else fs_row_p<64, 128>(sc, sl2, m_sub, rs0, rs1);
         }
 #pragma unroll
         for (int c = kOwnP ? 0 : 2; c < 4; ++c)
@@ -545,7 +530,7 @@ flash_fwd_span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       }
       if (!ok) break;
       // The output: a row's 32 columns at a time from tensor memory to bf16 to its place, a whole sector to a store (a tile through shared
-      // memory and the copy engine kept the warpgroup for 4400 clocks, this for @EPI@).
+      // memory and the copy engine kept the warpgroup for 4400 clocks, twice the time of a key tile).
       bf16* out = p.o + b * p.o_bs + (long long)min(row, T - 1) * p.o_ts + h * p.o_hs;
       float* lse = p.lse + (size_t(b) * p.QH + h) * T + min(row, T - 1);
       const bool any = my_tiles > 0, live = row < T;
