@@ -824,9 +824,12 @@ __device__ __forceinline__ void fb_p_chunk(uint32_t (&rs)[16], uint32_t (&pk)[8]
 // The same under spans: `see` holds the keys of the tile that each of the 16 queries sees, krow is this thread's key in it.
 // minus_lse2 points at the 16 per-query values. A cap leaves P (1 - tanh^2) in place of P in rs, which is what dS is made from
 // (kTier: see score_cap.cuh). A bias: dist = first query's position minus the key's.
+// Roundings to bf16, here and behind it: P for dV, dS for dK and dQ (the tensor core's operands), and at head_dim 128 what dS is made from,
+// which is kept between the two phases in the registers that there are. With delta, whose output is bf16, they leave dq and dk 2.9 to
+// 3.6e-3 (root mean square) from the 64-bit result, of which their own rounding is 1.7e-3.
 template <bool kMask, int kMod, int kTier = 0>
-__device__ __forceinline__ void fb_p_chunk_span(uint32_t (&rs)[16], uint32_t (&pk)[8], float sl2, const ScoreCap& cap, const float* minus_lse2,
-                                                const uint32_t* see, uint32_t krow, float slope2, float dist) {
+__device__ __forceinline__ void fb_p_chunk_span(uint32_t (&rs)[16], uint32_t (&pk)[8], float sl2, const ScoreCap& cap,
+                                                const float* minus_lse2, const uint32_t* see, uint32_t krow, float slope2, float dist) {
 #pragma unroll
   for (int e = 0; e < 16; e += 4) {
     const float4 l4 = *reinterpret_cast<const float4*>(minus_lse2 + e);
@@ -914,12 +917,12 @@ __device__ __forceinline__ void fb_ds_from_p_chunk(const uint32_t (&rp)[16], con
 
 // The accumulators of a cluster's CTAs, which hold the sums over their query heads, added up and stored: by every warp of every CTA.
 // dK and dV are two halves each (pairs of columns j and j + kD / 2, so that a rotation stays in one): with two CTAs each finishes a
-// matrix, with four a half, with three dK, a half of dV, the other. A CTA writes what it does not finish to the finisher's shared memory, where
-// Q and dO tiles were (between two barriers of the cluster), rows side by side; sums in the order of the CTAs behind the
+// matrix, with four a half, with three dK, a half of dV, the other. A CTA writes what it does not finish to the finisher's shared memory,
+// where Q and dO tiles were (between two barriers of the cluster), rows side by side; sums in the order of the CTAs behind the
 // finisher's own: no atomics, the same bits every time.
 template <int kD>
-__device__ __forceinline__ void dkv_cluster_sum(const FlashBwdTcParams& p, uint8_t* ring, uint32_t tmem_base, uint32_t col_dk, uint32_t col_dv,
-                                                int ntile, int kvh, int b, int rank, volatile int* abort_flag) {
+__device__ __forceinline__ void dkv_cluster_sum(const FlashBwdTcParams& p, uint8_t* ring, uint32_t tmem_base, uint32_t col_dk,
+                                                uint32_t col_dv, int ntile, int kvh, int b, int rank, volatile int* abort_flag) {
   constexpr int kN = kD / 8;                                  // columns of a run: a warpgroup has two runs of every half
   constexpr int kRun = 128 * kN * 4, kHalf = 4 * kRun;        // bytes of a run of 128 rows, of a half
   cg::cluster_group cluster = cg::this_cluster();
@@ -1002,7 +1005,8 @@ __device__ __forceinline__ void dkv_cluster_sum(const FlashBwdTcParams& p, uint8
       }
     }
     if (!live) continue;
-    bf16* out = half < 2 ? p.dk + b * p.dk_bs + (long long)key * p.dk_ts + kvh * p.dk_hs : p.dv + b * p.dv_bs + (long long)key * p.dv_ts + kvh * p.dv_hs;
+    bf16* out = half < 2 ? p.dk + b * p.dk_bs + (long long)key * p.dk_ts + kvh * p.dk_hs
+                         : p.dv + b * p.dv_bs + (long long)key * p.dv_ts + kvh * p.dv_hs;
 #pragma unroll
     for (int run = 0; run < 2; ++run)
 #pragma unroll
@@ -1332,8 +1336,8 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
             const float dist = float(qb + c * 16 - key);
             const uint32_t* see_c = see + (wg * 64 + c * 16) / 2;
             auto chunk = [&](auto mask, auto t) {
-              fb_p_chunk_span<decltype(mask)::value, kMod, decltype(t)::value>(rs, pk[c], sl2, p.cap, st + c * 16, see_c, uint32_t(key - n0),
-                                                                               slope_now, dist);
+              fb_p_chunk_span<decltype(mask)::value, kMod, decltype(t)::value>(rs, pk[c], sl2, p.cap, st + c * 16, see_c,
+                                                                               uint32_t(key - n0), slope_now, dist);
             };
             using True = std::true_type;
             if (kMod == kCap && tier != kCapNear) {
@@ -1637,8 +1641,9 @@ static int launch_dkv_span(const FlashBwdTcParams& p, const TensorMap (&m)[5], i
 // workspace (not optional) and rotary tables as in b200_flash_bwd_tc.
 B200_API int b200_flash_bwd_span(const void* q, const void* k, const void* v, const void* dout, const void* lse,
                                  const void* delta, void* dq, void* dk, void* dv, const void* spans, const void* qtab,
-                                 const void* ktab, const void* order_k, const void* order_q, const long long* s, int B, int T, int QH, int KVH, int D,
-                                 float scale, float cap, const void* slopes, void* ds_ws, const void* unrot_cos, const void* unrot_sin, int unrot_ld,
+                                 const void* ktab, const void* order_k, const void* order_q, const long long* s, int B, int T, int QH,
+                                 int KVH, int D, float scale, float cap, const void* slopes, void* ds_ws, const void* unrot_cos,
+                                 const void* unrot_sin, int unrot_ld,
                                  cudaStream_t st) {
   if (B <= 0 || T <= 0) return 0;
   if ((D != 128 && D != 64) || KVH <= 0 || QH % KVH != 0 || ds_ws == nullptr) return static_cast<int>(cudaErrorInvalidValue);

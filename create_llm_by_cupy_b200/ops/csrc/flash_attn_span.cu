@@ -5,8 +5,8 @@
 // The arithmetic of a tile is that of the causal forward (flash_attn_tc3.cu): a query row per thread, scores and outputs in tensor
 // memory, an online softmax whose reference maximum m moves only when a tile exceeds it by 2^8; P is rounded to bf16 for
 // the tensor core, sums and statistics are fp32. What differs is the walk. Packed documents leave a query tile few key tiles (2.5 of
-// 1024 / 128 at documents of 200 tokens), and a CTA's life was mostly its own start and end: 11.5 us of 26.7 at 4096 tokens, 32 / 8 heads of
-// 128, documents of 700 - barriers and tensor memory, tables, Q, the output's way out. So the CTAs stay:
+// 1024 / 128 at documents of 200 tokens), and a CTA's life was mostly its own start and end: 11.5 us of 26.7 at 4096 tokens, 32 / 8 heads
+// of 128, documents of 700 - barriers and tensor memory, tables, Q, the output's way out. So the CTAs stay:
 //
 //   * one per SM (head_dim 128, two query tiles side by side) or two (64, one each); the grid has a CTA for every unit of work, those
 //     with most to do first, and a CTA that is about to finish one takes the next that the grid has not started (with a fixed share of
@@ -52,8 +52,8 @@ struct FlashSpanParams {
 
 template <int kD>
 struct FS {
-  // Query tiles of a unit. (head_dim 128 with one, two CTAs to an SM and one tile of K and V each: documents of 600 tokens 57 -> 54 us, one of
-  // 8192 251 -> 268, capped scores no different.)
+  // Query tiles of a unit. (head_dim 128 with one, two CTAs to an SM and one tile of K and V each: documents of 600 tokens 57 -> 54 us, one
+  // of 8192 251 -> 268, capped scores no different.)
   static constexpr int kW = kD == 128 ? 2 : 1;
   static constexpr int kCtas = 3 - kW;                                 // CTAs of an SM
   static constexpr int kRing = 2;                                      // tiles of K, and of V, in shared memory
@@ -119,8 +119,8 @@ struct SpanQueue {
   uint64_t* empty;           // it has been read: by the MMA warp and every softmax warp
   uint4* answer;
   uint32_t asked;            // answers so far
-  // The next unit, -1: there is none (or a wait ran out). The TMA thread asks when it has sent for all of the present one, which is then two
-  // tiles from its end (asked at its start, a CTA sat on a second long unit while others ran out of work).
+  // The next unit, -1: there is none (or a wait ran out). The TMA thread asks when it has sent for all of the present one, which is then
+  // two tiles from its end (asked at its start, a CTA sat on a second long unit while others ran out of work).
   __device__ __forceinline__ int ask(volatile int* abort_flag) {
     if (asked > 0 && !mbar_wait(empty, (asked - 1) & 1, abort_flag)) return -1;
     mbar_expect_tx(full, 16);
@@ -415,7 +415,8 @@ flash_fwd_span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
       h = u.h;
       first = u.j0 + u.st[w];
       my_tiles = u.nt[w] - u.st[w];
-      if (mt >= 0) span = p.spans[size_t(b) * T + min(mt * 128 + rloc, T - 1)];      // (rows past the end as the last one: nobody stores them)
+      // (rows past the end as the last one: nobody stores them)
+      if (mt >= 0) span = p.spans[size_t(b) * T + min(mt * 128 + rloc, T - 1)];
       return true;
     };
     bool more = next_unit();
@@ -471,7 +472,8 @@ flash_fwd_span_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_cons
           for (int b = 0; b < 4; ++b) mx = fmaxf(mx, fs_block_max<false>(*reinterpret_cast<uint32_t(*)[32]>(&sc[32 * b]), 0, spans));
         } else {
 #pragma unroll
-          for (int b = 0; b < 4; ++b) mx = fmaxf(mx, fs_block_max<true>(*reinterpret_cast<uint32_t(*)[32]>(&sc[32 * b]), key0 + 32 * b, spans));
+          for (int b = 0; b < 4; ++b)
+            mx = fmaxf(mx, fs_block_max<true>(*reinterpret_cast<uint32_t(*)[32]>(&sc[32 * b]), key0 + 32 * b, spans));
         }
         mx *= sl2;
         if (kMod == kSpanCap && cap_now) mx = cap_any(mx, p.cap);          // the cap keeps the order of the scores
@@ -590,16 +592,17 @@ static int launch_fwd_span(FlashSpanParams p, const TensorMap (&m)[3], cudaStrea
   const long long items = (long long)p.n_units * p.QH * p.B;
   if (items > 0x7fffffffLL) return static_cast<int>(cudaErrorInvalidValue);
   if (L::kW == 2) p.order += (size_t)p.B * p.n_tiles;      // the orders of pairs stand behind those of single tiles
-  return static_cast<int>(launch_pdl(flash_fwd_span_kernel<kD, kMod>, dim3(unsigned(items)), dim3(L::kThreads), L::kSmem, st, 0, *m[0], *m[1],
-                                     *m[2], p));
+  return static_cast<int>(launch_pdl(flash_fwd_span_kernel<kD, kMod>, dim3(unsigned(items)), dim3(L::kThreads), L::kSmem, st, 0, *m[0],
+                                     *m[1], *m[2], p));
 }
 
 }  // namespace b200
 
 using namespace b200;
 
-// q, k, v (already rotated) and o [B, T, heads, D] by element strides (batch, token, head each; of o multiples of 16), lse [B, QH, T]; spans,
-// qtab and order as b200_span_mask makes them. cap > 0: scores c tanh(s / c); slopes [QH]: scores minus slope times distance (not both).
+// q, k, v (already rotated) and o [B, T, heads, D] by element strides (batch, token, head each; of o multiples of 16), lse [B, QH, T];
+// spans, qtab and order as b200_span_mask makes them. cap > 0: scores c tanh(s / c); slopes [QH]: scores minus slope times distance (not
+// both).
 B200_API int b200_flash_fwd_span(const void* q, const void* k, const void* v, void* o, void* lse, const void* spans, const void* qtab,
                                  const void* order, const long long* strides, int B, int T, int QH, int KVH, int D, float scale,
                                  float cap, const void* slopes, cudaStream_t st) {

@@ -60,8 +60,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
       : "memory");
   return done != 0;
 }
-// A CTA takes the work of one that the grid has not started yet: asks for it (16 bytes to `resp`, counted on `bar`); one thread. The answer's
-// first coordinate, or -1 when nothing was left: then it is not asked again.
+// A CTA takes the work of one that the grid has not started yet: asks for it (16 bytes to `resp`, counted on `bar`); one thread. The
+// answer's first coordinate, or -1 when nothing was left: then it is not asked again.
 __device__ __forceinline__ void take_cta(void* resp, uint64_t* bar) {
   asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];"
                ::"r"(smem_u32(resp)), "r"(smem_u32(bar)) : "memory");

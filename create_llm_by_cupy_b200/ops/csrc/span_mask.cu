@@ -251,8 +251,8 @@ span_mask_kernel(const SpanMaskParams p) {
 
 using namespace b200;
 
-// Fills `spans` [B, T] (lo, hi), `qtab` [B, nt] (4 ints), `ktab` [B, nt] (2 ints) and `order` [B, nt], [B, (nt + 1) / 2], [B, nt] (query tiles,
-// pairs of them, key tiles; most to do first), nt = tiles of 128 tokens, from documents,
+// Fills `spans` [B, T] (lo, hi), `qtab` [B, nt] (4 ints), `ktab` [B, nt] (2 ints) and `order` [B, nt], [B, (nt + 1) / 2], [B, nt] (query
+// tiles, pairs of them, key tiles; most to do first), nt = tiles of 128 tokens, from documents,
 // prefix flags and valid lengths (each may be null), or from the spans lo / hi [B, T].
 B200_API int b200_span_mask(const void* docs, const void* prefix, const void* valid_len, const void* lo, const void* hi,
                             void* spans, void* qtab, void* ktab, void* order, int B, int T, cudaStream_t st) {

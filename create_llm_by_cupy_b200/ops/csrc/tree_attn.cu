@@ -18,8 +18,8 @@
 // (columns S_0, S_1, O_0, O_1; P lies over S). A group of more than 128 rows gives each warpgroup a tile of rows; one of up to 128
 // gives them the odd and the even key tiles, and the first one adds up what the two have. Either way the tensor core works for one
 // while the other is in its exponentials: with one warpgroup a tile took 2.1 us at 128 rows of head_dim 128 where its 64 KiB
-// arrive in 1.5. The whole call at 32 drafts, 32 / 8 heads of 128: 17 us at 1000 keys, 69 at 60000, 114 at 120000 (0.74 us per 1000 keys, 5.5 TB/s,
-// and 25 us of three launches, the ramp and the join).
+// arrive in 1.5. The whole call at 32 drafts, 32 / 8 heads of 128: 17 us at 1000 keys, 69 at 60000, 114 at 120000 (0.74 us per 1000 keys,
+// 5.5 TB/s, and 25 us of three launches, the ramp and the join).
 //
 // Roundings to bf16: rotated K and V, as the caches hold them; Q in two parts, which is 16 bits; P, for the tensor core (sums of P and
 // the accumulators are fp32); the result.
@@ -175,7 +175,10 @@ __device__ __forceinline__ uint4 ta_rotated(const TreeParams& p, const bf16* x, 
     const float cv[4] = {cs.x, cs.y, cs.z, cs.w}, sv[4] = {sn.x, sn.y, sn.z, sn.w};
     float y[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) y[e] = c < kHalf ? a[4 * h + e] * cv[e] - b[4 * h + e] * sv[e] : a[4 * h + e] * cv[e] + b[4 * h + e] * sv[e];
+    for (int e = 0; e < 4; ++e) {
+      const float x = a[4 * h + e] * cv[e], z = b[4 * h + e] * sv[e];
+      y[e] = c < kHalf ? x - z : x + z;
+    }
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
       const bf162 t = __floats2bfloat162_rn(y[2 * e], y[2 * e + 1]);
@@ -232,7 +235,8 @@ __device__ __forceinline__ uint4* ta_chunk(uint8_t* tile, int r, int c) {
 // ((t + 1) G - 1) / total. Nearly all lists are short enough for 32-bit division.
 struct TreePieces {
   int c0, c1, late;         // late: the first one began with other rows
-  __device__ __forceinline__ int slot(int c, int w) const { return 4 * c + (c == c0 ? 2 * late : 0) + w; }      // of row tile w in the group
+  // of row tile w in the group
+  __device__ __forceinline__ int slot(int c, int w) const { return 4 * c + (c == c0 ? 2 * late : 0) + w; }
 };
 
 __device__ __forceinline__ TreePieces tree_pieces(const TreeParams& p, unsigned long long total, unsigned long long t0, int nt) {
@@ -336,7 +340,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   uint64_t* last_known = part_out + 1;   // whether it was the last of its rows' pieces
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(last_known + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-  long long* walk_at = reinterpret_cast<long long*>(tmem_slot + 2);          // [0] tiles of this CTA, [1] sequence, [2] place in it, [3] the list's
+  // [0] tiles of this CTA, [1] sequence, [2] place in it, [3] the list's
+  long long* walk_at = reinterpret_cast<long long*>(tmem_slot + 2);
   volatile int* is_last = reinterpret_cast<volatile int*>(walk_at + 4);
   float2* s_ml = reinterpret_cast<float2*>(smem + L::kMl);
 
@@ -414,7 +419,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       while (ok && walk.next(p, s)) {
         if (seg > 0 && !mbar_wait(q_empty, (seg - 1) & 1, abort_flag)) break;
         ++seg;
-        mbar_expect_tx(q_full, uint32_t((s.pair ? 4 : 2) * p.R * p.tok) * kD * 2);   // (rows past the box: whatever, their results go nowhere)
+        // (rows past the box: whatever, their results go nowhere)
+        mbar_expect_tx(q_full, uint32_t((s.pair ? 4 : 2) * p.R * p.tok) * kD * 2);
         for (int i = 0; i < (s.pair ? 4 : 2); ++i) {                     // row tile i / 2, part i % 2
           const int d0 = (2 * s.rg + (i >> 1)) * p.tok, b = s.b + (i & 1) * p.B;
           uint8_t* sQ = smem + L::kQ + i * kTile;
@@ -454,15 +460,15 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const uint64_t dQ = umma_smem_desc(smem_u32(smem + L::kQ + (s.pair ? 2 * w : 0) * kTile), 16, 1024);
         const uint64_t dK = umma_smem_desc(smem_u32(smem + L::kK + (g % kStK) * kTile), 16, 1024);
         const bool drafts = s.t0 + t == s.nt - 1;        // 64 keys are enough for them
-        // Q's two parts, so that the scores are those of an unrounded rotation. Rounded to bf16 it was the largest error of the result: 4.4e-3
-        // of it at 60001 keys, 2.2e-3 like this, of which the result's own rounding is 1.7e-3. It costs 0 to 8 % of the whole call's time at up
-        // to 3200 keys, 15 % at 60001 (67 -> 77 us).
+        // Q's two parts, so that the scores are those of an unrounded rotation. Rounded to bf16 it was the largest error of the result:
+        // 4.4e-3 of it at 60001 keys, 2.2e-3 like this, of which the result's own rounding is 1.7e-3. It costs 0 to 8 % of the whole call's
+        // time at up to 3200 keys, 15 % at 60001 (67 -> 77 us).
 #pragma unroll
         for (int kk = 0; kk < kD / 8; ++kk) {
           const int k = kk % (kD / 16);
           const uint32_t off = ((k >> 2) * 16384 + (k & 3) * 32) >> 4;
-          umma_bf16_ss_warp(tmem_base + L::kColS + w * 128, dQ + (kk / (kD / 16)) * (kTile >> 4) + off, dK + off, drafts ? idesc_s64 : idesc_s,
-                            kk != 0);
+          umma_bf16_ss_warp(tmem_base + L::kColS + w * 128, dQ + (kk / (kD / 16)) * (kTile >> 4) + off, dK + off,
+                            drafts ? idesc_s64 : idesc_s, kk != 0);
         }
         umma_commit_warp(&s_full[w]);
         if (!s.pair || w == 1) umma_commit_warp(&k_empty[g % kStK]);
@@ -504,11 +510,13 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   } else {
     // ---------------------------------------------------------------- softmax: a row per thread
     setmaxnreg_inc<TA_REGS_MANY>();
-    const int w = (warp - 4) >> 2, q = warp & 3, r = q * 32 + lane;      // the quarter of tensor memory that a warp reaches is its number mod 4
+    // the quarter of tensor memory that a warp reaches is its number mod 4
+    const int w = (warp - 4) >> 2, q = warp & 3, r = q * 32 + lane;
     const uint32_t lane_sel = uint32_t(q * 32) << 16;
     const uint32_t tS = tmem_base + lane_sel + L::kColS + w * 128, tO = tmem_base + lane_sel + L::kColO + w * 128;
     const float sl2 = kMod == kTreePlain ? p.scale * kTaLog2e : 1.f;
-    int g0 = 0, seg = 0, done = 0, swaps = 0, parts = 0; // tiles before the stretch; items so far; sums handed from the second warpgroup; pieces
+    // tiles before the stretch; items so far; sums handed from the second warpgroup; pieces
+    int g0 = 0, seg = 0, done = 0, swaps = 0, parts = 0;
     bool ok = true;
     while (ok && walk.next(p, s)) {
       const int rt = 2 * s.rg + (s.pair ? w : 0);
@@ -564,7 +572,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
           if constexpr (kMod == kTreeBias) {
             const float dist = float(s.len - t * 128) + depth;
 #pragma unroll
-            for (int e = 0; e < 128; ++e) sc[e] = __float_as_uint(fmaf(__uint_as_float(sc[e]), p.scale * kTaLog2e, -slope2 * (dist - float(e))));
+            for (int e = 0; e < 128; ++e)
+              sc[e] = __float_as_uint(fmaf(__uint_as_float(sc[e]), p.scale * kTaLog2e, -slope2 * (dist - float(e))));
           }
           if (rem < 128) {
 #pragma unroll
@@ -689,13 +698,15 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
               uint4 u;
               bf162* u2 = reinterpret_cast<bf162*>(&u);
 #pragma unroll
-              for (int e = 0; e < 4; ++e) u2[e] = __floats2bfloat162_rn(__uint_as_float(o[8 * k + 2 * e]), __uint_as_float(o[8 * k + 2 * e + 1]));
+              for (int e = 0; e < 4; ++e)
+                u2[e] = __floats2bfloat162_rn(__uint_as_float(o[8 * k + 2 * e]), __uint_as_float(o[8 * k + 2 * e + 1]));
               reinterpret_cast<uint4*>(orow + c * 32)[k] = u;
             }
           } else {
 #pragma unroll
             for (int k = 0; k < 8; ++k)
-              reinterpret_cast<uint4*>(p.part_o)[(slot * (kD / 4) + c * 8 + k) * 128 + r] = make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
+              reinterpret_cast<uint4*>(p.part_o)[(slot * (kD / 4) + c * 8 + k) * 128 + r] =
+                  make_uint4(o[4 * k], o[4 * k + 1], o[4 * k + 2], o[4 * k + 3]);
           }
         }
       }
@@ -750,7 +761,8 @@ tree_join_kernel(const TreeParams p) {
   }
   const TreePieces pc = tree_pieces(p, sum * per, before * per + (unsigned long long)idx * nt, nt);
   if (pc.c0 == pc.c1) return;
-  const int rows = p.tok * p.R, task = blockIdx.y * 256 + threadIdx.x, all = p.n > p.tok ? 2 * rows : rows, row = task % all, part = task / all;
+  const int rows = p.tok * p.R, all = p.n > p.tok ? 2 * rows : rows;
+  const int task = blockIdx.y * 256 + threadIdx.x, row = task % all, part = task / all;
   const int w = row >= rows ? 1 : 0, r = row - w * rows, rt = 2 * rg + w;
   if (part < kD / (4 * kQuads) && r < min(p.n - rt * p.tok, p.tok) * p.R) tree_join_task<kD, kQuads>(p, b, kvh, rt, w, r, part, pc);
 }
@@ -844,7 +856,8 @@ B200_API int b200_tree_attn_append(const void* kqv, void* kc, void* vc, void* ou
   p.scale = scale;
   p.cap = make_score_cap(scale, cap);
   p.status = status_ptr();
-  const TensorMap tq = get_tensor_map_bthd(p.q, 2 * B, n, QH, D, (unsigned long long)n * QH * D, (unsigned long long)QH * D, D, p.tok, 64, p.R);
+  const unsigned long long qs = (unsigned long long)QH * D;
+  const TensorMap tq = get_tensor_map_bthd(p.q, 2 * B, n, QH, D, n * qs, qs, D, p.tok, 64, p.R);
   if (!tq || !tk || !tv) return static_cast<int>(cudaErrorInvalidValue);
   if (D == 128) {
     if (cap > 0.f) return launch_tree<128, kTreeCap>(p, tq, tk, tv, st);

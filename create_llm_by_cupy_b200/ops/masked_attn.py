@@ -157,7 +157,8 @@ def _check_mask(name: str, mask: SpanMask, q) -> None:
     if not isinstance(mask, SpanMask):
         raise TypeError(f"{name}: mask is a SpanMask")
     if (mask.B, mask.T) != tuple(q.shape[:2]) or mask.device != q.device:
-        raise ValueError(f"{name}: the mask is of {mask.B} x {mask.T} tokens on {mask.device}, q of {q.shape[0]} x {q.shape[1]} on {q.device}")
+        raise ValueError(f"{name}: the mask is of {mask.B} x {mask.T} tokens on {mask.device}, "
+                         f"q of {q.shape[0]} x {q.shape[1]} on {q.device}")
 
 
 def _scale(scale, D: int) -> float:
