@@ -2,7 +2,8 @@
 // the plain decoded step.
 //
 // Draft i of sequence b stands at position len + depth(i). It sees the len cached keys, its ancestors and itself. K, Q, V come
-// packed from the projection, un-rotated: a first kernel rotates Q and K and appends K and V to the caches at len + i.
+// packed from the projection, un-rotated: a first kernel rotates Q and K and appends K and V to the caches at len + i; a draft that
+// has no room there is not seen by any, itself included.
 //
 //   x = q k scale, capped (c tanh(x / c)) or biased (x - slope |distance|);  o = softmax(x) V
 //
@@ -531,7 +532,8 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         if (!mbar_wait(&s_full[w], done & 1, abort_flag)) { ok = false; break; }
         tc_fence_after();
         const bool drafts = t == s.nt - 1;
-        const int rem = drafts ? p.n : min(s.len - t * 128, 128);        // keys of the tile
+        // keys of the tile: of the drafts those that the cache has room for (rows behind its end arrive as zeros, and would count)
+        const int rem = drafts ? min(p.n, p.Tmax - s.len) : min(s.len - t * 128, 128);
         if (rem < (drafts ? 64 : 128) && (w == 0 || !s.pair)) {
           // values past the length may be anything, and 0 times that (two row tiles: P V of the first one comes first)
           const int g = g0 + t - s.t0, st = g % kStV;

@@ -390,7 +390,8 @@ def tree_attn_append(kqv, kcache, vcache, lens, tree, QH: int, KVH: int, cos, si
     ``tree`` int64 [B, n] (``tree_mask``); ``cos``, ``sin`` fp32 [>= Tmax, D / 2].
 
     Draft i stands at position lens + its depth, sees the cached tokens and the drafts of its mask, and its K (rotated) and V
-    are appended to the caches at lens + i (one behind the end of the cache is not kept). n = 1 with mask 1 is a decoded token.
+    are appended to the caches at lens + i. One that would stand behind the end of the cache is not kept, and no draft sees it, itself
+    included: its own result is that of the cached tokens and of its ancestors that were kept. n = 1 with mask 1 is a decoded token.
     Returns [B, n, QH, D]. A mask of 0 leaves the cached tokens alone; with none of them the result is 0. Cache rows from
     lens + n on may hold anything."""
     if native.host is not None:
