@@ -377,7 +377,6 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   }
   if (warp == 1) tmem_alloc(tmem_slot, 512);
   pdl_wait();
-  pdl_trigger();
   if (warp == 0) {
     const long long total = tree_total(p, lane), G = tree_pieces_of(p, total);
     long long at, end, b_first;
@@ -400,6 +399,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  pdl_trigger();                         // behind the allocation: a CTA of the next kernel must not take columns that this one waits for
   const uint32_t tmem_base = *tmem_slot;
   TreeWalk walk;
   walk.left = walk_at[0];
