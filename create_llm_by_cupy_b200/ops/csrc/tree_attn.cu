@@ -192,6 +192,10 @@ __device__ __forceinline__ uint4 ta_rotated(const TreeParams& p, const bf16* x, 
   return u;
 }
 
+// Whom draft i of sequence b sees; bits of drafts that are not there count for nothing, neither here nor in its depth.
+__device__ __forceinline__ unsigned long long tree_bits(const TreeParams& p, int b, int i) {
+  return p.tree[size_t(b) * p.n + i] & (~0ull >> (64 - p.n));
+}
 __device__ __forceinline__ int tree_depth(unsigned long long bits) { return max(__popcll(bits) - 1, 0); }
 
 // A thread per 16 bytes of the packed projection: K (rotated) and V to the caches, Q (rotated, in two parts) to its workspace.
@@ -209,7 +213,7 @@ tree_append_kernel(const TreeParams p) {
   const int c = int(i % kChunks), head = int(i / kChunks % heads);
   const long long row = i / kChunks / heads;
   const int b = int(row / p.n), d = int(row % p.n);
-  const int len = tree_len(p, b), pos = len + tree_depth(p.tree[row]);
+  const int len = tree_len(p, b), pos = len + tree_depth(tree_bits(p, b, d));
   const bf16* x = p.kqv + row * p.ld + head * kD;
   if (head >= p.KVH && head < p.KVH + p.QH) {
     uint4 rest;
@@ -524,7 +528,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
       const int live = min(p.n - rt * p.tok, p.tok) * p.R;
       const bool work = q * 32 < live;                   // this warp has rows at all
       const int d = min(rt * p.tok + r / p.R, p.n - 1), h = s.kvh * p.R + r % p.R;
-      const unsigned long long bits = p.tree[size_t(s.b) * p.n + d];
+      const unsigned long long bits = tree_bits(p, s.b, d);
       const float slope2 = kMod == kTreeBias ? p.slopes[h] * kTaLog2e : 0.f, depth = float(tree_depth(bits));
       float m_ref = -INFINITY, l_run = 0.f;
       const int step = s.pair ? 1 : 2, first = s.t0 + (s.pair ? 0 : w);
@@ -563,7 +567,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
 #pragma unroll
           for (int e = 0; e < 64; ++e) {
             if constexpr (kMod == kTreeBias) {
-              const float dj = e < p.n ? float(tree_depth(p.tree[size_t(s.b) * p.n + e])) : 0.f;
+              const float dj = e < p.n ? float(tree_depth(tree_bits(p, s.b, e))) : 0.f;
               sc[e] = __float_as_uint(fmaf(__uint_as_float(sc[e]), p.scale * kTaLog2e, -slope2 * fabsf(depth - dj)));
             }
             if (!((bits >> e) & 1) || e >= rem) sc[e] = 0xff800000u;
