@@ -140,6 +140,12 @@ def _heads(name: str, q, k, v):
         raise ValueError(f"{name}: q is [B, T, query heads, D], k and v are [B, T, KV heads, D]")
     if k.shape[2] == 0 or q.shape[2] % k.shape[2] != 0:
         raise ValueError(f"{name}: the query heads are a multiple of the KV heads")
+    _same_device(name, q, k, v)
+
+
+def _same_device(name: str, first, *others) -> None:
+    if any(t.device != first.device for t in others):
+        raise ValueError(f"{name}: all tensors are on one device")
 
 
 def _modifier(name: str, q_heads: int, softcap: float, slopes, device) -> None:
@@ -270,16 +276,21 @@ def span_attn_bwd(dout, q, k, v, o, lse, mask: SpanMask, *, scale: float | None 
     if dout.shape != q.shape or o.shape != q.shape or tuple(lse.shape) != (B, QH, T):
         raise ValueError("span_attn_bwd: dout and o are like q, lse is [B, query heads, T]")
     _modifier("span_attn_bwd", QH, softcap, slopes, q.device)
-    if unrotate is not None and any(x.shape[0] < T or x.shape[1] != D // 2 for x in unrotate):
+    if unrotate is not None and any(x.dim() != 2 or x.shape[0] < T or x.shape[1] != D // 2 for x in unrotate):
         raise ValueError("span_attn_bwd: rotary tables are [>= T, D / 2]")
+    if out is not None and [x.shape for x in out] != [q.shape, k.shape, v.shape]:
+        raise ValueError("span_attn_bwd: out has the shapes of q, k and v")
+    if delta is not None and tuple(delta.shape) != (B, QH, T):
+        raise ValueError("span_attn_bwd: delta is [B, query heads, T]")
+    _same_device("span_attn_bwd", q, dout, o, lse, *(unrotate or ()), *(out or ()), *(() if delta is None else (delta,)))
     scale = _scale(scale, D)
     if not q.is_cuda:
         return _span_bwd_reference(dout, q, k, v, o, mask, scale, softcap, slopes, out, unrotate)
     F._bf16(dout, q, k, v, o)
     if D not in (64, 128):
         raise ValueError("span_attn_bwd: CUDA kernels exist for a head dimension of 64 or 128")
-    if lse.dtype != torch.float32:
-        raise TypeError("span_attn_bwd: lse is float32")
+    if any(x.dtype != torch.float32 for x in (lse, *(unrotate or ()))):
+        raise TypeError("span_attn_bwd: lse and the rotary tables are float32")
     q, k, v, dout, o = (_tile_view(t) for t in (q, k, v, dout, o))
     lse = lse.contiguous()
     if out is None:
@@ -287,8 +298,6 @@ def span_attn_bwd(dout, q, k, v, o, lse, mask: SpanMask, *, scale: float | None 
         dk, dv = torch.empty((B, T, KVH, D), dtype=q.dtype, device=q.device), torch.empty((B, T, KVH, D), dtype=q.dtype, device=q.device)
     else:
         dq, dk, dv = out
-        if dq.shape != q.shape or dk.shape != k.shape or dv.shape != v.shape:
-            raise ValueError("span_attn_bwd: out has the shapes of q, k and v")
         F._bf16(dq, dk, dv)
         if any(_tile_view(t) is not t for t in out):
             raise ValueError("span_attn_bwd: out needs rows on 16-byte boundaries")
@@ -296,7 +305,7 @@ def span_attn_bwd(dout, q, k, v, o, lse, mask: SpanMask, *, scale: float | None 
         return dq, dk, dv
     if delta is None:
         delta = F.flash_delta(o, dout, torch.empty((B, QH, T), dtype=torch.float32, device=q.device))
-    elif tuple(delta.shape) != (B, QH, T) or delta.dtype != torch.float32 or not delta.is_contiguous():
+    elif delta.dtype != torch.float32 or not delta.is_contiguous():
         raise ValueError("span_attn_bwd: delta is float32 [B, query heads, T], contiguous")
     ucos = usin = None
     if unrotate is not None:
