@@ -110,14 +110,20 @@ def _spans_reference(B, T, docs, prefix, valid_len):
     return lo, torch.where((docs < 0) | (t >= vlen), torch.zeros_like(hi), hi)
 
 
+def _is_device(x: torch.Tensor, device) -> bool:
+    """Whether ``x`` is on ``device``: a GPU without a number is the current one."""
+    d = torch.device(device)
+    return x.device.type == d.type and (d.type != "cuda" or x.device.index == (torch.cuda.current_device() if d.index is None else d.index))
+
+
 def span_mask(B: int, T: int, device, docs=None, prefix=None, valid_len=None) -> SpanMask:
     """Mask of ``B`` rows of ``T`` tokens. ``docs`` int32 [B, T]: which document a token belongs to; a change of the number
     starts the next one, a negative one is padding, which sees nothing and is not seen. ``prefix`` bool [B, T]: a document's leading
     flagged tokens see one another whichever comes first; every other token sees its document up to itself. ``valid_len``
     int32 [B]: tokens from there on are padding too. Without any of them: plain causal rows."""
     if native.host is not None:
-        buf = native.host.span_mask(B, T, docs, prefix, valid_len)
-        if buf is not None and (buf.device == device or torch.device(device).type == "cuda"):
+        buf = native.host.span_mask(B, T, docs, prefix, valid_len)      # (on the current device, as docs, prefix and valid_len are)
+        if buf is not None and (device == "cuda" or _is_device(buf, device)):
             native.bump()
             return SpanMask(buf, B, T)
     if B < 0 or T < 0:
@@ -126,7 +132,7 @@ def span_mask(B: int, T: int, device, docs=None, prefix=None, valid_len=None) ->
                                ("valid_len", valid_len, torch.int32, (B,))):
         if x is not None and (x.dtype != dt or tuple(x.shape) != shape):
             raise ValueError(f"span_mask: {name} is {dt} {list(shape)}")
-        if x is not None and x.device.type != torch.device(device).type:
+        if x is not None and not _is_device(x, device):
             raise ValueError(f"span_mask: {name} is not on {device}")
     if T > 512000:
         raise ValueError("span_mask: more than 512000 tokens in a row")

@@ -36,3 +36,14 @@ def test_span_attention(path):
         with pytest.raises(TypeError):
             A.span_attn_bwd(**{**good, **kw})
     assert native.read_status() == (0, 0)
+
+
+def test_the_mask_is_made_where_it_was_asked_for(path):
+    docs = torch.zeros(1, 64, dtype=torch.int32, device=DEV)
+    for device in (DEV, torch.device(DEV), torch.device(DEV, torch.cuda.current_device())):
+        assert A.span_mask(1, 64, device, docs=docs).device == docs.device
+    for device in ("cpu", torch.device(DEV, torch.cuda.current_device() + 1)):
+        with pytest.raises(ValueError):
+            A.span_mask(1, 64, device, docs=docs)
+    with pytest.raises(ValueError):
+        A.span_mask(1, 64, DEV, docs=docs, valid_len=torch.tensor([3], dtype=torch.int32))
