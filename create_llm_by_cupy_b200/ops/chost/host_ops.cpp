@@ -519,9 +519,10 @@ void put_strides(long long* st, std::initializer_list<const Tensor*> ts) {
     for (int d = 0; d < 3; ++d) *st++ = t->size(d) > 1 ? t->stride(d) : 16;
 }
 // Scale (0: of the head dimension) and cap as the front ends take them; the others are theirs to refuse.
-bool score_numbers(float* scale, float cap, const Tensor* slopes, int64_t D) {
-  if (*scale == 0.f) *scale = float(1.0 / std::sqrt(double(D)));
-  return *scale > 0.f && *scale < INFINITY && cap >= 0.f && cap < INFINITY && !(cap > 0.f && slopes);
+bool score_numbers(double* scale, double cap, const Tensor* slopes, int64_t D) {
+  auto takes = [](double x) { return x >= 1e-18 && x <= 1e18; };
+  if (*scale == 0.0) *scale = 1.0 / std::sqrt(double(D));
+  return takes(*scale) && (cap == 0.0 || takes(cap)) && !(cap > 0.0 && slopes);
 }
 
 // span_fwd(q, k, v, mask buffer, B, T, scale, softcap, slopes or None) -> (o, lse)
@@ -529,8 +530,8 @@ PyObject* span_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   ARGS(9)
   const Tensor *q = plain(a[0]), *k = plain(a[1]), *v = plain(a[2]), *buf = plain(a[3]), *sl;
   const int64_t mB = as_int(a[4]), mT = as_int(a[5]);
-  float scale = as_float(a[6]);
-  const float cap = as_float(a[7]);
+  double scale = PyFloat_AsDouble(a[6]);
+  const double cap = PyFloat_AsDouble(a[7]);
   CHECK_NUMBERS
   if (!q || !k || !v || !buf || !optional(a[8], &sl) || !span_heads(*q, *k, *v, *buf, mB, mT, sl, dev)) Py_RETURN_NONE;
   const int64_t B = q->size(0), T = q->size(1), QH = q->size(2), D = q->size(3), KVH = k->size(2);
@@ -541,8 +542,8 @@ PyObject* span_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const SpanTables t = span_tables(*buf, B, T);
   if (launched([&] {
         return api.flash_fwd_span(q->const_data_ptr(), k->const_data_ptr(), v->const_data_ptr(), o.mutable_data_ptr(),
-                                  lse.mutable_data_ptr(), t.spans, t.qtab, t.order_q, st, int(B), int(T), int(QH), int(KVH), int(D), scale, cap,
-                                  sl ? sl->const_data_ptr() : nullptr, stream(dev));
+                                  lse.mutable_data_ptr(), t.spans, t.qtab, t.order_q, st, int(B), int(T), int(QH), int(KVH), int(D), float(scale),
+                                  float(cap), sl ? sl->const_data_ptr() : nullptr, stream(dev));
       }))
     return wrap2(o, lse);
   END
@@ -555,8 +556,8 @@ PyObject* span_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor *dout = plain(a[0]), *q = plain(a[1]), *k = plain(a[2]), *v = plain(a[3]), *o = plain(a[4]), *lse = plain(a[5]),
                *buf = plain(a[6]), *sl;
   const int64_t mB = as_int(a[7]), mT = as_int(a[8]);
-  float scale = as_float(a[9]);
-  const float cap = as_float(a[10]);
+  double scale = PyFloat_AsDouble(a[9]);
+  const double cap = PyFloat_AsDouble(a[10]);
   const long long most = PyLong_Check(a[12]) ? PyLong_AsLongLong(a[12]) : 0;
   CHECK_NUMBERS
   if (!dout || !q || !k || !v || !o || !lse || !buf || !optional(a[11], &sl) || !span_heads(*q, *k, *v, *buf, mB, mT, sl, dev))
@@ -584,8 +585,8 @@ PyObject* span_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
         if (rc != 0) return rc;
         return api.flash_bwd_span(q->const_data_ptr(), k->const_data_ptr(), v->const_data_ptr(), dout->const_data_ptr(),
                                   lse->const_data_ptr(), delta.const_data_ptr(), dq.mutable_data_ptr(), dk.mutable_data_ptr(),
-                                  dv.mutable_data_ptr(), t.spans, t.qtab, t.ktab, t.order_k, t.order_q, st, int(B), int(T), int(QH), int(KVH), int(D), scale, cap,
-                                  sl ? sl->const_data_ptr() : nullptr, ws.mutable_data_ptr(), nullptr, nullptr, 0, stream(dev));
+                                  dv.mutable_data_ptr(), t.spans, t.qtab, t.ktab, t.order_k, t.order_q, st, int(B), int(T), int(QH),
+                                  int(KVH), int(D), float(scale), float(cap), sl ? sl->const_data_ptr() : nullptr, ws.mutable_data_ptr(), nullptr, nullptr, 0, stream(dev));
       }))
     Py_RETURN_NONE;
   PyObject* r = PyTuple_New(3);
@@ -603,8 +604,8 @@ PyObject* tree_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const Tensor *x = plain(a[0]), *kc = plain(a[1]), *vc = plain(a[2]), *lens = plain(a[3]), *tree = plain(a[4]), *c = plain(a[7]),
                *s = plain(a[8]), *sl;
   const int QH = as_int(a[5]), KVH = as_int(a[6]);
-  float scale = as_float(a[9]);
-  const float cap = as_float(a[10]);
+  double scale = PyFloat_AsDouble(a[9]);
+  const double cap = PyFloat_AsDouble(a[10]);
   CHECK_NUMBERS
   if (!x || !kc || !vc || !lens || !tree || !c || !s || !optional(a[11], &sl) || !tma_rows(*x, dev)) Py_RETURN_NONE;
   if (!bf16_on(*kc, dev) || !bf16_on(*vc, dev) || kc->dim() != 4 || kc->sizes() != vc->sizes() || !kc->is_contiguous() ||
@@ -630,7 +631,7 @@ PyObject* tree_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
         return api.tree_attn_append(x->const_data_ptr(), kc->mutable_data_ptr(), vc->mutable_data_ptr(), out.mutable_data_ptr(),
                                     lens->const_data_ptr(), tree->const_data_ptr(), c->const_data_ptr(), s->const_data_ptr(),
                                     sl ? sl->const_data_ptr() : nullptr, ws.mutable_data_ptr(), int(B), int(nd), QH, KVH, int(Tmax), int(D),
-                                    int(c->size(0)), x->stride(0), scale, cap, stream(dev));
+                                    int(c->size(0)), x->stride(0), float(scale), float(cap), stream(dev));
       }))
     return wrap(out);
   END

@@ -10,6 +10,7 @@
 #pragma once
 #include <stdint.h>
 
+#include <cmath>
 #include <type_traits>
 
 namespace b200 {
@@ -35,8 +36,9 @@ inline ScoreCap make_score_cap(float scale, float cap) {
     if (i < 4) c.near[i] = make_float2(float(kNear[i] * f), float(kNear[i] * f));
     c.mid[i] = make_float2(float(kMid[i] * f), float(kMid[i] * f));
   }
-  c.reach_near = float(0.4 * double(cap) / scale);
-  c.reach_mid = float(double(cap) / scale);
+  // a cap so small that a coefficient is no fp32 number: the exponential form alone
+  c.reach_near = std::isfinite(c.near[3].x) ? float(0.4 * double(cap) / scale) : -1.f;
+  c.reach_mid = std::isfinite(c.mid[6].x) ? float(double(cap) / scale) : -1.f;
   c.kc = float(2.0 * kLog2e * scale / cap);
   c.c2 = float(kLog2e * cap);
   const float inv2 = float(-1.0 / (kLog2e * cap) / (kLog2e * cap));

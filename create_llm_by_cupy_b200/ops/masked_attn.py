@@ -28,6 +28,8 @@ from . import native
 
 _f = ctypes.c_float
 _i = ctypes.c_int
+# Caps and scales that the kernels' arithmetic has room for: a cap's square, and the quotient of the two, are fp32 numbers.
+LEAST, MOST = 1e-18, 1e18
 
 
 # --------------------------------------------------------------------------- span masks
@@ -155,8 +157,8 @@ def _same_device(name: str, first, *others) -> None:
 
 
 def _modifier(name: str, q_heads: int, softcap: float, slopes, device) -> None:
-    if not (softcap >= 0.0 and math.isfinite(softcap)):
-        raise ValueError(f"{name}: softcap is 0 (none) or a positive number")
+    if softcap != 0.0 and not LEAST <= softcap <= MOST:
+        raise ValueError(f"{name}: softcap is 0 (none) or a number from {LEAST} to {MOST}")
     if slopes is None:
         return
     if softcap > 0.0:
@@ -175,8 +177,8 @@ def _check_mask(name: str, mask: SpanMask, q) -> None:
 
 def _scale(scale, D: int) -> float:
     scale = 1.0 / math.sqrt(D) if scale is None else float(scale)
-    if not (scale > 0.0 and math.isfinite(scale)):
-        raise ValueError("attention: scale is a positive number")
+    if not LEAST <= scale <= MOST:
+        raise ValueError(f"attention: scale is a number from {LEAST} to {MOST}")
     return scale
 
 
