@@ -85,20 +85,26 @@ class GroupedQueryAttention:
     ``[in, out]`` as in the reference (model/fast_layers.py:101-105).
 
     ``valid_len`` of the passes is one length per row, or a ``masked_attn.SpanMask`` of packed documents. ``softcap`` > 0 caps the
-    scores (c tanh(s / c)), in training, prefill and decoding. Both run on the span kernels, which know no dropout on the
-    probabilities.
+    scores (c tanh(s / c)), in training, prefill and decoding. ``distance_bias``: scores lose slope[head] * distance, slopes
+    2^(-8 (head + 1) / heads), and Q and K are not rotated: the bias says where a token stands. All of these run on the span kernels, which
+    know no dropout on the probabilities.
     """
 
     def __init__(self, hidden_size, time_size, q_head, kv_head, layer_num, dropout_rate=0.0,
-                 dtype=torch.bfloat16, device="cpu", generator=None, init_std=None, rope_base=10000.0, softcap=0.0):
+                 dtype=torch.bfloat16, device="cpu", generator=None, init_std=None, rope_base=10000.0, softcap=0.0,
+                 distance_bias=False):
         assert hidden_size % q_head == 0 and q_head % kv_head == 0
         self.softcap = float(softcap)
+        if distance_bias and self.softcap > 0.0:
+            raise ValueError("GroupedQueryAttention: scores are capped or biased, not both")
+        self.slopes = (torch.tensor([2.0 ** (-8.0 * (h + 1) / q_head) for h in range(q_head)], dtype=torch.float32, device=device)
+                       if distance_bias else None)
         self.H, self.T = hidden_size, time_size
         self.QH, self.KVH = q_head, kv_head
         self.D = hidden_size // q_head
         self.KV = kv_head * self.D
         self.scale = 1.0 / math.sqrt(self.D)
-        self.rope_base = rope_base
+        self.rope_base = None if distance_bias else rope_base
         self.dropout_rate = dropout_rate
         std_in = init_std if init_std is not None else 1.0 / math.sqrt(hidden_size)
         std_out = init_std if init_std is not None else 1.0 / math.sqrt(2.0 * hidden_size * layer_num)
@@ -138,7 +144,12 @@ class GroupedQueryAttention:
         """The span mask that the pass runs under; None: the plain causal kernels do."""
         if isinstance(valid_len, A.SpanMask):
             return valid_len
-        return A.span_mask(B, T, device, valid_len=valid_len) if self.softcap > 0.0 else None
+        return A.span_mask(B, T, device, valid_len=valid_len) if self.modified else None
+
+    @property
+    def modified(self) -> bool:
+        """Scores are capped or biased, so that every pass runs on the span and tree kernels."""
+        return self.softcap > 0.0 or self.slopes is not None
 
     def _project(self, x, T, tabs, first: bool):
         """K | Q | V projection; on the pre-rotating path K and Q leave it rotated - inside the GEMM's epilogue
@@ -156,8 +167,8 @@ class GroupedQueryAttention:
     def _attend(self, q, k, v, valid_len, tabs, train_flg: bool = False):
         if self._mask is not None:
             if not self._dense:
-                return A.span_attn_fwd(q, k, v, self._mask, scale=self.scale, softcap=self.softcap)
-            o, lse, _, _ = A._span_reference(q, k, v, self._mask, self.scale, self.softcap, None)
+                return A.span_attn_fwd(q, k, v, self._mask, scale=self.scale, softcap=self.softcap, slopes=self.slopes)
+            o, lse, _, _ = A._span_reference(q, k, v, self._mask, self.scale, self.softcap, self.slopes)
             return o.to(q.dtype).contiguous(), lse
         if self._dense:
             o, lse, p, _, _ = F._attn_reference(q, k, v, valid_len, self.scale, tabs[0], tabs[1])
@@ -179,7 +190,7 @@ class GroupedQueryAttention:
         if self._mask is not None:
             if self.drop_attn is not None and train_flg:
                 raise ValueError("GroupedQueryAttention: dropout on the attention probabilities goes with neither span masks nor "
-                                 "capped scores")
+                                 "capped or biased scores")
             valid_len = self._mask
         kqv = self._project(x, T, tabs, True)
         q, k, v = self._split(kqv, B, T)
@@ -225,10 +236,10 @@ class GroupedQueryAttention:
         if self._mask is not None:
             do = do.view(B, T, self.QH, self.D)
             if self._dense:
-                A._span_bwd_reference(do, q, k, v, o, self._mask, self.scale, self.softcap, None, (dq, dk, dv), tabs)
+                A._span_bwd_reference(do, q, k, v, o, self._mask, self.scale, self.softcap, self.slopes, (dq, dk, dv), tabs)
             else:
-                A.span_attn_bwd(do, q, k, v, o, lse, self._mask, scale=self.scale, softcap=self.softcap, out=(dq, dk, dv), unrotate=tabs,
-                                delta=delta)
+                A.span_attn_bwd(do, q, k, v, o, lse, self._mask, scale=self.scale, softcap=self.softcap, slopes=self.slopes,
+                                out=(dq, dk, dv), unrotate=tabs, delta=delta)
         elif self._dense:
             # dense path (verification, or training with attention dropout): the fp32 restatement, on the
             # device the tensors live on
@@ -260,8 +271,8 @@ class GroupedQueryAttention:
         q, k, v = self._split(kqv, B, T)
         kcache[:, :, :T].copy_(k.permute(0, 2, 1, 3))
         vcache[:, :, :T].copy_(v.permute(0, 2, 1, 3))
-        if self.softcap > 0.0:
-            o, _ = A.span_attn_fwd(q, k, v, A.span_mask(B, T, x.device), scale=self.scale, softcap=self.softcap)
+        if self.modified:
+            o, _ = A.span_attn_fwd(q, k, v, A.span_mask(B, T, x.device), scale=self.scale, softcap=self.softcap, slopes=self.slopes)
         elif self.flash_backend == "none":
             o, _, _, _, _ = F._attn_reference(q, k, v, None, self.scale, None, None)
             o = o.to(x.dtype).contiguous()
@@ -273,7 +284,7 @@ class GroupedQueryAttention:
         """x: [B, H] normed hidden state of the token at position ``pos`` (same for the batch)."""
         B = x.shape[0]
         tabs = self._rope(kcache.shape[2], x.device)
-        if self.softcap > 0.0:
+        if self.modified:
             one = torch.ones((B, 1), dtype=torch.int64, device=x.device)
             return self.decode_drafts(x, one, kcache, vcache, lens - 1, residual)
         out = F.decode_attn_block(x, self.params[0], self.params[1], kcache, vcache, lens, pos, self.QH, self.KVH,
@@ -299,7 +310,7 @@ class GroupedQueryAttention:
         (``masked_attn.tree_mask``), ``lens`` [B] cached tokens. Their K and V are appended to the caches."""
         tabs = self._rope(kcache.shape[2], x.device)
         o = A.tree_attn_append(F.gemm(x, self.params[0]), kcache, vcache, lens, tree, self.QH, self.KVH, tabs[0], tabs[1], scale=self.scale,
-                               softcap=self.softcap)
+                               softcap=self.softcap, slopes=self.slopes)
         return F.gemm(o.view(x.shape[0], self.H), self.params[1], add=residual)
 
     @staticmethod

@@ -121,6 +121,7 @@ class Cupa_ver4:
         self.tie_embeddings = bool(d.get("tie_embeddings", True))
         self.rope_base = float(d.get("rope_base", 10000.0))
         self.attn_softcap = float(d.get("attn_softcap", 0.0))
+        self.attn_distance_bias = bool(d.get("attn_distance_bias", False))
         self.init_std = d.get("init_std")
         self.seed = int(d.get("seed", 0))
         if device is None:
@@ -167,7 +168,8 @@ class Cupa_ver4:
             self.dropout_ = TimeDropout(self.dropout_rate, self.dtype)
         for _ in range(self.layernum):
             gqa = GroupedQueryAttention(self.hidden_size, self.time_size, self.q_head, self.kv_head, self.layernum,
-                                        self.dropout_rate, rope_base=self.rope_base, softcap=self.attn_softcap, **kw)
+                                        self.dropout_rate, rope_base=self.rope_base, softcap=self.attn_softcap,
+                                        distance_bias=self.attn_distance_bias, **kw)
             feed = SwiGLU(self.hidden_size, self.layernum, dropout_rate=self.dropout_rate, ffn_size=self.ffn_size, **kw)
             norm1 = RMSNorm(self.hidden_size, self.dtype, self.device)
             norm2 = RMSNorm(self.hidden_size, self.dtype, self.device)
@@ -310,7 +312,7 @@ class Cupa_ver4:
         B, T = x.shape
         self._BT = (B, T)
         valid_len = x_pa if x_pa is None or isinstance(x_pa, SpanMask) else x_pa.to(torch.int32)
-        if self.attn_softcap > 0.0 and not isinstance(valid_len, SpanMask):
+        if (self.attn_softcap > 0.0 or self.attn_distance_bias) and not isinstance(valid_len, SpanMask):
             valid_len = span_mask(B, T, x.device, valid_len=valid_len)           # one for all layers
 
         W = manager.gather_embedding()
@@ -442,7 +444,7 @@ class Cupa_ver4:
         """Full-sequence fp32 logits [B, T, V] (no cache); for tests and scoring."""
         manager = manager if manager is not None else self._local_manager()
         B, T = x.shape
-        mask = span_mask(B, T, x.device) if self.attn_softcap > 0.0 else None
+        mask = span_mask(B, T, x.device) if self.attn_softcap > 0.0 or self.attn_distance_bias else None
         W = manager.gather_embedding()
         h = self.embed.forward(W, x, False)
         for b in range(self.layernum):

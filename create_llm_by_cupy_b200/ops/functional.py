@@ -230,15 +230,17 @@ def swiglu_bwd(dact: torch.Tensor, gate_val: torch.Tensor) -> torch.Tensor:
 _rope_cache: dict = {}
 
 
-def rope_table(T: int, D: int, base: float, device) -> tuple[torch.Tensor, torch.Tensor]:
-    """cos/sin [T, D/2] fp32 with freq_j = base^(-2j/D)."""
+def rope_table(T: int, D: int, base: float | None, device) -> tuple[torch.Tensor, torch.Tensor]:
+    """cos/sin [T, D/2] fp32 with freq_j = base^(-2j/D); without a base those of no rotation (1 and 0)."""
     if not isinstance(device, torch.device):
         device = torch.device(device)
-    key = (T, D, float(base), device)
+    key = (T, D, base if base is None else float(base), device)
     hit = _rope_cache.get(key)
     if hit is not None:
         return hit
-    if device.type != "cuda":
+    if base is None:
+        res = (torch.ones((T, D // 2), dtype=torch.float32, device=device), torch.zeros((T, D // 2), dtype=torch.float32, device=device))
+    elif device.type != "cuda":
         j = torch.arange(D // 2, dtype=torch.float32)
         freq = torch.pow(torch.tensor(float(base)), -2.0 * j / D)
         ang = torch.arange(T, dtype=torch.float32)[:, None] * freq[None, :]
