@@ -262,8 +262,9 @@ class GroupedQueryAttention:
         return dx
 
     # -- incremental decoding --------------------------------------------------------------
-    def prefill(self, x, B, T, kcache, vcache, residual=None):
-        """Full-sequence forward that also fills the KV cache [B, KVH, Tmax, D] (K stored rotated)."""
+    def prefill(self, x, B, T, kcache, vcache, residual=None, mask=None):
+        """Full-sequence forward that also fills the KV cache [B, KVH, Tmax, D] (K stored rotated). ``mask``: a ``SpanMask`` in place of
+        plain causal rows."""
         kqv = F.gemm(x, self.params[0])
         tabs = self._rope(kcache.shape[2], x.device)
         F.rope_inplace(kqv, tabs[0], tabs[1], T, self.KVH, self.D, col0=0)
@@ -271,8 +272,9 @@ class GroupedQueryAttention:
         q, k, v = self._split(kqv, B, T)
         kcache[:, :, :T].copy_(k.permute(0, 2, 1, 3))
         vcache[:, :, :T].copy_(v.permute(0, 2, 1, 3))
-        if self.modified:
-            o, _ = A.span_attn_fwd(q, k, v, A.span_mask(B, T, x.device), scale=self.scale, softcap=self.softcap, slopes=self.slopes)
+        if mask is not None or self.modified:
+            mask = A.span_mask(B, T, x.device) if mask is None else mask
+            o, _ = A.span_attn_fwd(q, k, v, mask, scale=self.scale, softcap=self.softcap, slopes=self.slopes)
         elif self.flash_backend == "none":
             o, _, _, _, _ = F._attn_reference(q, k, v, None, self.scale, None, None)
             o = o.to(x.dtype).contiguous()

@@ -312,8 +312,8 @@ class Cupa_ver4:
         B, T = x.shape
         self._BT = (B, T)
         valid_len = x_pa if x_pa is None or isinstance(x_pa, SpanMask) else x_pa.to(torch.int32)
-        if (self.attn_softcap > 0.0 or self.attn_distance_bias) and not isinstance(valid_len, SpanMask):
-            valid_len = span_mask(B, T, x.device, valid_len=valid_len)           # one for all layers
+        mask = self._rows_mask(B, T, valid_len)
+        valid_len = valid_len if mask is None else mask
 
         W = manager.gather_embedding()
         h = self.embed.forward(W, x, train_flg)
@@ -440,17 +440,30 @@ class Cupa_ver4:
         """Loss of a batch without keeping anything for backward (validation)."""
         return self.forward(x, t, x_pa, manager, train_flg=False)
 
-    def logits(self, x, manager=None) -> torch.Tensor:
-        """Full-sequence fp32 logits [B, T, V] (no cache); for tests and scoring."""
+    def _rows_mask(self, B: int, T: int, x_pa, prefix: int = 0):
+        """The span mask of a pass over ``B`` rows of ``T`` tokens, one for all layers; None where the plain causal kernels do.
+        ``prefix``: tokens at a row's start that see one another whichever comes first."""
+        if isinstance(x_pa, SpanMask):
+            return x_pa
+        if prefix <= 0 and self.attn_softcap == 0.0 and not self.attn_distance_bias:
+            return None
+        flags = (torch.arange(T, device=self.device) < prefix).expand(B, T).contiguous() if prefix > 0 else None
+        return span_mask(B, T, self.device, prefix=flags, valid_len=x_pa)
+
+    def logits(self, x, manager=None, x_pa=None) -> torch.Tensor:
+        """Full-sequence fp32 logits [B, T, V] (no cache); for tests and scoring. ``x_pa`` as in ``forward``: lengths, or a ``SpanMask``
+        (documents, prefixes that see themselves whole)."""
         manager = manager if manager is not None else self._local_manager()
         B, T = x.shape
-        mask = span_mask(B, T, x.device) if self.attn_softcap > 0.0 or self.attn_distance_bias else None
+        x_pa = x_pa if x_pa is None or isinstance(x_pa, SpanMask) else x_pa.to(torch.int32)
+        mask = self._rows_mask(B, T, x_pa)
+        valid_len = x_pa if mask is None else mask
         W = manager.gather_embedding()
         h = self.embed.forward(W, x, False)
         for b in range(self.layernum):
             gqa, feed, norm1, norm2 = self.block_modules(b)
             manager.gather_modules([gqa, feed, norm1, norm2])
-            h = gqa.forward(norm1.forward(h, False), B, T, mask, residual=h, train_flg=False)
+            h = gqa.forward(norm1.forward(h, False), B, T, valid_len, residual=h, train_flg=False)
             h = feed.forward(norm2.forward(h, False), residual=h, train_flg=False)
             manager.release_modules([gqa, feed, norm1, norm2])
         manager.gather_module(self.norm_)
@@ -461,7 +474,8 @@ class Cupa_ver4:
 
     @torch.no_grad()
     def generate(self, prompt, start_id=None, end_id=None, padding_id=None, temp: float = 0.7, top: float = 0.9,
-                 penalty: float = 1.2, max_new_tokens: int | None = None, greedy: bool = False, seed: int | None = None):
+                 penalty: float = 1.2, max_new_tokens: int | None = None, greedy: bool = False, seed: int | None = None,
+                 prefix: int = 0):
         """Autoregressive decoding with a KV cache (reference intent: model/model.py:439-480).
 
         ``prompt``: list of token ids. The sequence is ``[start_id] + prompt`` when ``start_id`` is
@@ -469,7 +483,8 @@ class Cupa_ver4:
         pass through the decode-attention kernel. Sampling: pad id excluded, repetition penalty,
         temperature, nucleus (top-p) with a probability-weighted draw; ``greedy`` takes the argmax.
         Stops at ``end_id`` or when the context (``time_size``) is full. Parameters must be
-        resident (single process), as in the reference.
+        resident (single process), as in the reference. ``prefix``: the first tokens of the sequence that see one another
+        whichever comes first, for a model trained on such documents (``masked_attn.span_mask``).
         """
         pad = self.padding_id if padding_id is None else padding_id
         toks = ([int(start_id)] if start_id is not None else []) + [int(p) for p in prompt]
@@ -489,11 +504,12 @@ class Cupa_ver4:
         Wh = self.head_para[0] if self.head_para is not None else W
 
         T0 = len(toks)
+        mask = self._rows_mask(1, T0, None, prefix)
         ids = torch.tensor(toks, dtype=torch.int32, device=dev)
         h = F.embedding_fwd(W, ids, -1)
         for b in range(self.layernum):
             gqa, feed, norm1, norm2 = self.block_modules(b)
-            h = gqa.prefill(norm1.forward(h, False), 1, T0, kc[b], vc[b], residual=h)
+            h = gqa.prefill(norm1.forward(h, False), 1, T0, kc[b], vc[b], residual=h, mask=mask)
             h = feed.forward(norm2.forward(h, False), residual=h, train_flg=False)
         h_last = self.norm_.forward(h[T0 - 1:T0], False)
         out = []
@@ -522,11 +538,13 @@ class Cupa_ver4:
         return out
 
     @torch.no_grad()
-    def generate_drafted(self, prompt, draft, start_id=None, end_id=None, padding_id=None, max_new_tokens: int | None = None):
+    def generate_drafted(self, prompt, draft, start_id=None, end_id=None, padding_id=None, max_new_tokens: int | None = None,
+                         prefix: int = 0):
         """Greedy decoding that checks a tree of drafted tokens per pass: the same choices as ``generate(..., greedy=True)``, in as many
         passes as the drafts are wrong. ``draft(tokens)`` gets all tokens so far and returns proposals for those that follow as
         (token, parent) pairs, at most 63: ``parent`` is the index of an earlier proposal of the same list, or -1 for the last token. A
-        drafted token whose predecessors were all chosen, and which the model chooses, is kept with its cached K and V."""
+        drafted token whose predecessors were all chosen, and which the model chooses, is kept with its cached K and V. ``prefix`` as in
+        ``generate``."""
         pad = self.padding_id if padding_id is None else padding_id
         toks = ([int(start_id)] if start_id is not None else []) + [int(p) for p in prompt]
         if not toks:
@@ -546,10 +564,11 @@ class Cupa_ver4:
                 logits[:, pad] = float("-inf")
             return torch.argmax(logits, -1).tolist()
 
+        mask = self._rows_mask(1, len(toks), None, prefix)
         h = F.embedding_fwd(W, torch.tensor(toks, dtype=torch.int32, device=dev), -1)
         for b in range(self.layernum):
             gqa, feed, norm1, norm2 = self.block_modules(b)
-            h = gqa.prefill(norm1.forward(h, False), 1, len(toks), kc[b], vc[b], residual=h)
+            h = gqa.prefill(norm1.forward(h, False), 1, len(toks), kc[b], vc[b], residual=h, mask=mask)
             h = feed.forward(norm2.forward(h, False), residual=h, train_flg=False)
         out, cached = [], len(toks)
         if budget > 0:
