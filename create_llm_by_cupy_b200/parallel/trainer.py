@@ -166,12 +166,13 @@ class Trainer:
 
     def _graph_step(self, batches, scale: float):
         """Returns (loss, stats, step_scale) device tensors of a replayed step, or None when this step
-        has to run eagerly (warm-up steps, a batch of another shape)."""
+        has to run eagerly (warm-up steps, a batch of another shape, lengths in place of documents)."""
         from ..ops import native
         from ..ops.masked_attn import SpanMask
         x, t, x_pa = batches[0]
-        if isinstance(x_pa, SpanMask):        # its documents are another step's shapes of work: run eagerly
-            return None
+        # lengths, or the tables of the packed documents, whose size is a matter of the batch's alone
+        spans = isinstance(x_pa, SpanMask)
+        keys = x_pa.buf if spans else x_pa
         if self._graph is None:
             if self._graph_warm < 2:          # lazy one-time set-up (tensor maps, attributes, streams) happens eagerly
                 self._graph_warm += 1
@@ -179,7 +180,8 @@ class Trainer:
             self.join_optimizer()
             self.manager.unit_ready = {}
             torch.cuda.synchronize(self.device)
-            self._gx, self._gt, self._gpa = x.clone(), t.clone(), x_pa.clone()
+            self._gx, self._gt, self._gkeys = x.clone(), t.clone(), keys.clone()
+            self._gpa = SpanMask(self._gkeys, x_pa.B, x_pa.T) if spans else self._gkeys
             self._hyper = torch.zeros(4, dtype=torch.float32, device=self.device)
             self._hyper_host = torch.zeros(4, dtype=torch.float32).pin_memory()
             self._graph_scale = scale
@@ -189,11 +191,12 @@ class Trainer:
                 self._g_loss, self._g_stats = self._graph_body(scale)
             self._graph_launches = native.launch_count() - n0
             self._graph = graph
-        if x.shape != self._gx.shape or t.shape != self._gt.shape or scale != self._graph_scale:
+        if (x.shape != self._gx.shape or t.shape != self._gt.shape or scale != self._graph_scale
+                or spans != isinstance(self._gpa, SpanMask) or keys.shape != self._gkeys.shape):
             return None
         self._gx.copy_(x, non_blocking=True)
         self._gt.copy_(t, non_blocking=True)
-        self._gpa.copy_(x_pa, non_blocking=True)
+        self._gkeys.copy_(keys, non_blocking=True)
         self.optimizer.advance()
         step_scale = 1.0 / (self.world_size * scale)
         self._hyper_host.copy_(torch.tensor(self.optimizer.hyper_values(step_scale), dtype=torch.float32))
