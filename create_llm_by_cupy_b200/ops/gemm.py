@@ -338,13 +338,15 @@ _rope_t_cache: dict = {}
 
 def rope_tables_transposed(cos: torch.Tensor, sin: torch.Tensor):
     """([D/2, T] cos, [D/2, T] sin) copies of the [T, D/2] rotary tables, cached per table. The kernels'
-    epilogues own one row (position) per thread, so a warp reads consecutive words from this layout."""
+    epilogues own one row (position) per thread, so a warp reads consecutive words from this layout. Tables that were changed in
+    place since are laid out again (in inference mode tensors do not count their changes: there they have to stay as they are)."""
     key = (cos.data_ptr(), sin.data_ptr(), tuple(cos.shape))
+    version = None if cos.is_inference() or sin.is_inference() else (cos._version, sin._version)
     tt = _rope_t_cache.get(key)
-    if tt is None:
+    if tt is None or tt[4] != version:
         if len(_rope_t_cache) > 16:
             _rope_t_cache.clear()
-        tt = _rope_t_cache[key] = (cos.t().contiguous(), sin.t().contiguous(), cos, sin)   # keeps the sources alive
+        tt = _rope_t_cache[key] = (cos.t().contiguous(), sin.t().contiguous(), cos, sin, version)   # keeps the sources alive
     return tt
 
 
