@@ -146,7 +146,7 @@ def span_mask(B: int, T: int, device, docs=None, prefix=None, valid_len=None) ->
 def _heads(name: str, q, k, v):
     if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
         raise ValueError(f"{name}: q is [B, T, query heads, D], k and v are [B, T, KV heads, D]")
-    if k.shape[2] == 0 or q.shape[2] % k.shape[2] != 0:
+    if k.shape[2] == 0 or q.shape[2] == 0 or q.shape[2] % k.shape[2] != 0:
         raise ValueError(f"{name}: the query heads are a multiple of the KV heads")
     _same_device(name, q, k, v)
 
@@ -470,7 +470,7 @@ def _tree_reference(kqv, kcache, vcache, lens, tree, QH, KVH, cos, sin, scale, s
     lens = lens.long().clamp(0, Tmax)
     pos = lens[:, None] + depth
     dt = _work_dtype(kqv)
-    k, q, v = kqv.to(dt).view(B, n, -1).split([KVH * D, QH * D, KVH * D], dim=2)
+    k, q, v = kqv.to(dt).view(B, n, kqv.shape[1]).split([KVH * D, QH * D, KVH * D], dim=2)
     c, s = (x.to(dt)[pos.clamp_max(x.shape[0] - 1)][:, :, None] for x in (cos, sin))
 
     def rot(x):
