@@ -824,9 +824,8 @@ __device__ __forceinline__ void fb_p_chunk(uint32_t (&rs)[16], uint32_t (&pk)[8]
 // The same under spans: `see` holds the keys of the tile that each of the 16 queries sees, krow is this thread's key in it.
 // minus_lse2 points at the 16 per-query values. A cap leaves P (1 - tanh^2) in place of P in rs, which is what dS is made from
 // (kTier: see score_cap.cuh). A bias: dist = first query's position minus the key's.
-// Roundings to bf16, here and behind it: P for dV, dS for dK and dQ (the tensor core's operands), and at head_dim 128 what dS is made from,
-// which is kept between the two phases in the registers that there are. With delta, whose output is bf16, they leave dq and dk 2.9 to
-// 3.6e-3 (root mean square) from the 64-bit result, of which their own rounding is 1.7e-3.
+// Roundings to bf16, here and behind it: P for dV, dS for dK and dQ (the tensor core's operands). With delta, whose output is bf16, they
+// leave dq and dk 2.6 to 3.1e-3 (root mean square) from the 64-bit result, of which their own rounding is 1.7e-3.
 template <bool kMask, int kMod, int kTier = 0>
 __device__ __forceinline__ void fb_p_chunk_span(uint32_t (&rs)[16], uint32_t (&pk)[8], float sl2, const ScoreCap& cap,
                                                 const float* minus_lse2, const uint32_t* see, uint32_t krow, float slope2, float dist) {
@@ -869,14 +868,6 @@ __device__ __forceinline__ void fb_p_chunk_span(uint32_t (&rs)[16], uint32_t (&p
       rs[e + u] = __float_as_uint(pe.x);
       rs[e + u + 1] = __float_as_uint(pe.y);
     }
-  }
-}
-
-__device__ __forceinline__ void fb_pack16(const uint32_t* f, uint32_t (&pk)[8]) {
-#pragma unroll
-  for (int e = 0; e < 16; e += 2) {
-    const bf162 t = __floats2bfloat162_rn(__uint_as_float(f[e]), __uint_as_float(f[e + 1]));
-    pk[e >> 1] = *reinterpret_cast<const uint32_t*>(&t);
   }
 }
 
@@ -1312,7 +1303,10 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
         const int qb = m0 + wg * 64;                                     // first query column of this warpgroup
         const float* st = reinterpret_cast<const float*>(smem + Smem::kStats + s2 * Smem::kStatBytes) + wg * 64;
         bool need_mask = (m0 < n0 + 128) || (n0 + 128 > vlen);     // the diagonal tile or the padded tail
-        // This thread's P^T between the two phases: packed (head_dim 128), or as it is (64, which has the registers)
+        // This thread's P^T (under a cap P^T (1 - tanh^2)) between the two phases: as it is, in fp32. Kept as bf16 pairs, as the
+        // causal form of head_dim 128 does, it left dq and dk at 3.1 to 3.6e-3, not 2.6 to 3.1e-3, and the capped form packed it a second time:
+        // 8192 tokens, 16 / 4 heads, forward and backward 1476 us, 1402 like this; four rows of 2048 292 / 283.
+        constexpr bool kKeep32 = kD == 64 || kMod != kCausal;
         uint32_t pk[4][8], sc[64];
         if (!mbar_wait(&st_full[s2], (g / kSt) & 1, abort_flag)) { ok = false; break; }
         const uint32_t* see = reinterpret_cast<const uint32_t*>(st - wg * 64 + 2 * FKW_BQ);
@@ -1350,7 +1344,6 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
             }
           }
           tmem_st_32x32b_x8(tS + c * 8, pk[c]);
-          if (kMod == kCap && kD == 128) fb_pack16(&sc[16 * c], pk[c]);      // kept for dS: P (1 - tanh^2)
         }
         tmem_st_wait();
         tc_fence_before();
@@ -1363,7 +1356,7 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
         }
         auto ds_chunk = [&](const uint32_t* rp, int c) {
           uint32_t dk_[8];
-          if (kD == 64) fb_ds_chunk16(&sc[16 * c], rp, dk_, p.scale, st + FKW_BQ + c * 16);
+          if (kKeep32) fb_ds_chunk16(&sc[16 * c], rp, dk_, p.scale, st + FKW_BQ + c * 16);
           else fb_ds_from_p_chunk(*reinterpret_cast<const uint32_t(*)[16]>(rp), pk[c], dk_, p.scale, st + FKW_BQ + c * 16);
           tmem_st_32x32b_x8(tP + c * 8, dk_);
           if (ds_on) {            // 16 queries = two 16-byte chunks of this key's 128-byte staging row
@@ -1373,11 +1366,11 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
         };
         uint32_t ra[32], rb[32];
         tmem_ld_32x32b_x32(tP, ra);
-        if (kD == 128) tmem_ld_32x32b_x32(tP + 32, rb);
+        if (!kKeep32) tmem_ld_32x32b_x32(tP + 32, rb);
         tmem_ld_wait();
         ds_chunk(&ra[0], 0);
         ds_chunk(&ra[16], 1);
-        if (kD == 64) {
+        if (kKeep32) {
           tmem_ld_32x32b_x32(tP + 32, rb);
           tmem_ld_wait();
         }
@@ -1616,8 +1609,8 @@ static int g_span_split = 0;        // 0: by the number of key tiles; else force
 // CTAs of a cluster that share a key tile's query heads. What a key tile costs is a matter of the documents, which only the device
 // knows: a few long ones decide when the kernel ends, and where there are fewer tiles than SMs most stand idle. But every CTA has about
 // 10 us of its own (its first loads and scores, the cluster's sum). Forward and backward in us with 1 / 2 / 3 or 4 CTAs to a tile:
-// 24 tiles of 3 heads of 64 46 / 39 / 33, 84 of them 80 / 53 / 53, 256 of them 104 / 124 (uneven) / 136; 256 tiles of 4 heads of 128,
-// documents of about 600 tokens 340 / 288 / 325, one of 8192 1370 / 1331 / 1435.
+// 24 tiles of 3 heads of 64 43 / 39 / 34, 84 of them 62 / 56 / 55, 256 of them 102 / 126 (uneven) / 138; 256 tiles of 4 heads of 128,
+// documents of about 600 tokens 304 / 279 / 328, one of 8192 1323 / 1308 to 1331 / 1377.
 static int span_split(int group, long long tiles) {
   const int most = group >= 4 ? 4 : group;
   if (g_span_split > 0) return std::min(g_span_split, most);

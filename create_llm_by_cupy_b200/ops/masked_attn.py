@@ -233,8 +233,10 @@ def span_attn_fwd(q, k, v, mask: SpanMask, *, scale: float | None = None, softca
     """Attention of q [B, T, QH, D] over k, v [B, T, KVH, D] (already rotated; any strides) under ``mask``. CUDA: bf16, D 64 or
     128. Returns (o [B, T, QH, D] contiguous, lse [B, QH, T] fp32); a query that sees nothing gets zeros and -inf.
 
-    Keys and values that no query of a 128-token tile sees are not read; of those that are, all have to be finite: one that is
-    masked for a single query still goes through the tensor core with weight 0."""
+    For every two neighbouring tiles of 128 queries the tiles of 128 keys from the first to the last that one of them sees are read, gaps
+    between spans included. All that is read has to be finite, padding too: a value that is masked goes through the tensor core with
+    weight 0. Weights are rounded to bf16 for the tensor core (sums and statistics are fp32): with the result's own rounding 1.8 to
+    2.2e-3 of the result, root mean square."""
     if native.host is not None and type(mask) is SpanMask:
         r = native.host.span_fwd(q, k, v, mask.buf, mask.B, mask.T, 0.0 if scale is None else scale or -1.0, softcap, slopes)
         if r is not None:
@@ -270,7 +272,12 @@ def span_attn_bwd(dout, q, k, v, o, lse, mask: SpanMask, *, scale: float | None 
     write into; ``unrotate`` = (cos, sin) tables [>= T, D / 2]: dq and dk leave as gradients of the un-rotated q and k; ``delta``
     [B, QH, T] fp32, sum over D of dout * o, where the caller has it (``gemm.gemm_delta``). The
     kernels keep dS^T of as many batch elements or KV heads at a time as ``functional.FLASH_DQ_GEMM_MAX_BYTES`` holds, of one KV
-    head at least. Deterministic: no atomics."""
+    head at least, whatever its spans: 2 T^2 bytes for each of its query heads. That is where one GPU ends: 34 GB at 65536 tokens and four
+    of them, 137 GB at 131072. Deterministic: no atomics.
+
+    All inputs have to be finite, also where nothing is seen. dq and dk are 2.6 to 3.1e-3 (root mean square) from exact ones, dv
+    2.3e-3, where the rounding of a bf16 result alone is 1.7e-3: P and dS are bf16 for the tensor core, and ``delta`` comes from an ``o``
+    that is bf16."""
     if native.host is not None and type(mask) is SpanMask and out is None and unrotate is None and delta is None:
         r = native.host.span_bwd(dout, q, k, v, o, lse, mask.buf, mask.B, mask.T, 0.0 if scale is None else scale or -1.0, softcap, slopes,
                                  F.FLASH_DQ_GEMM_MAX_BYTES)
@@ -409,6 +416,7 @@ def tree_attn_append(kqv, kcache, vcache, lens, tree, QH: int, KVH: int, cos, si
     Draft i stands at position lens + its depth, sees the cached tokens and the drafts of its mask, and its K (rotated) and V
     are appended to the caches at lens + i. One that would stand behind the end of the cache is not kept, and no draft sees it, itself
     included: its own result is that of the cached tokens and of its ancestors that were kept. n = 1 with mask 1 is a decoded token.
+    Weights are rounded to bf16 for the tensor core; the rotated Q goes in as two bf16 parts.
     Returns [B, n, QH, D]. A mask of 0 leaves the cached tokens alone; with none of them the result is 0. Cache rows from
     lens + n on may hold anything."""
     if native.host is not None:
