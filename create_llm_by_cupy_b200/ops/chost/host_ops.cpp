@@ -490,7 +490,8 @@ PyObject* span_mask(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const SpanTables t = span_tables(buf, B, T);
   if (launched([&] {
         return api.span_mask(docs ? docs->const_data_ptr() : nullptr, prefix ? prefix->const_data_ptr() : nullptr,
-                             vl ? vl->const_data_ptr() : nullptr, nullptr, nullptr, t.spans, t.qtab, t.ktab, t.order_q, int(B), int(T), stream(dev));
+                             vl ? vl->const_data_ptr() : nullptr, nullptr, nullptr, t.spans, t.qtab, t.ktab, t.order_q, int(B), int(T),
+                             stream(dev));
       }))
     return wrap(buf);
   END
@@ -542,8 +543,8 @@ PyObject* span_fwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
   const SpanTables t = span_tables(*buf, B, T);
   if (launched([&] {
         return api.flash_fwd_span(q->const_data_ptr(), k->const_data_ptr(), v->const_data_ptr(), o.mutable_data_ptr(),
-                                  lse.mutable_data_ptr(), t.spans, t.qtab, t.order_q, st, int(B), int(T), int(QH), int(KVH), int(D), float(scale),
-                                  float(cap), sl ? sl->const_data_ptr() : nullptr, stream(dev));
+                                  lse.mutable_data_ptr(), t.spans, t.qtab, t.order_q, st, int(B), int(T), int(QH), int(KVH), int(D),
+                                  float(scale), float(cap), sl ? sl->const_data_ptr() : nullptr, stream(dev));
       }))
     return wrap2(o, lse);
   END
@@ -586,7 +587,8 @@ PyObject* span_bwd(PyObject*, PyObject* const* a, Py_ssize_t n) {
         return api.flash_bwd_span(q->const_data_ptr(), k->const_data_ptr(), v->const_data_ptr(), dout->const_data_ptr(),
                                   lse->const_data_ptr(), delta.const_data_ptr(), dq.mutable_data_ptr(), dk.mutable_data_ptr(),
                                   dv.mutable_data_ptr(), t.spans, t.qtab, t.ktab, t.order_k, t.order_q, st, int(B), int(T), int(QH),
-                                  int(KVH), int(D), float(scale), float(cap), sl ? sl->const_data_ptr() : nullptr, ws.mutable_data_ptr(), nullptr, nullptr, 0, stream(dev));
+                                  int(KVH), int(D), float(scale), float(cap), sl ? sl->const_data_ptr() : nullptr,
+                                  ws.mutable_data_ptr(), nullptr, nullptr, 0, stream(dev));
       }))
     Py_RETURN_NONE;
   PyObject* r = PyTuple_New(3);
@@ -613,7 +615,8 @@ PyObject* tree_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   if (!on(*tree, dev) || tree->scalar_type() != at::kLong || tree->dim() != 2 || !tree->is_contiguous()) Py_RETURN_NONE;
   const int64_t B = tree->size(0), nd = tree->size(1), Tmax = kc->size(2), D = kc->size(3);
-  if (!on(*lens, dev) || lens->scalar_type() != at::kInt || lens->dim() != 1 || lens->size(0) != B || !lens->is_contiguous()) Py_RETURN_NONE;
+  if (!on(*lens, dev) || lens->scalar_type() != at::kInt || lens->dim() != 1 || lens->size(0) != B || !lens->is_contiguous())
+    Py_RETURN_NONE;
   if (QH <= 0 || KVH <= 0 || QH % KVH != 0 || (D != 64 && D != 128) || kc->size(0) != B || kc->size(1) != KVH || !fits(B) || !fits(Tmax) ||
       nd < 1 || nd > 64 || x->size(0) != B * nd || x->size(1) != (2 * int64_t(KVH) + QH) * D)
     Py_RETURN_NONE;

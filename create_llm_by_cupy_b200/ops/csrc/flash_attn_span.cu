@@ -14,8 +14,10 @@
 //   * loads of the next tile's Q, K and V start when the last scores of the present one are done, its first scores when the last P V
 //     is, and the output leaves straight from tensor memory while they run.
 //
-// What bounds it then: a tile's exponentials (2048 of a warpgroup's 2242 clocks a tile), the chain scores -> maximum -> exp2 -> P V
-// around them, and masked parts of tiles (18 to 68 % of the pairs that are computed at the documents above). Measured, 32 / 8 heads
+// What bounds it then: the chain scores -> maximum -> exp2 -> P V of two warpgroups (2242 clocks a tile with both of them at it, 2048 of
+// exponentials that they share a unit for; a masked tile 3100 to 3500), of which a CTA is in the middle only part of its life: over
+// the whole kernel the exponential unit is at 37 %, the tensor core at 36, issue at 35. And masked parts of tiles (18 to 68 % of the pairs
+// that are computed at the documents above). Measured, 32 / 8 heads
 // of 128: 4096 tokens in documents of 700 97 us with the mask's tables; 16 / 4 heads, a cap, 8192 tokens in documents of 600 85 us.
 //
 // Roundings to bf16: P, for the tensor core (its sums are fp32), and the output.

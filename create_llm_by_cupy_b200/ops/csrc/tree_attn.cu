@@ -8,19 +8,20 @@
 //   x = q k scale, capped (c tanh(x / c)) or biased (x - slope |distance|);  o = softmax(x) V
 //
 // The rows of a tile are the drafts times the query heads that share a KV head: every key is read once for all of them, which is
-// all that bounds the kernel while there are few (64 rows of head_dim 128 do 96 multiply-adds per byte read). The work is one
-// list of 128-key tiles, over sequences, KV heads and groups of up to 256 rows, the drafts a tile of their own behind each
-// sequence's cached ones; the list is cut into as many equal pieces as there are SMs, so sequences of any mix of lengths keep all
-// of them busy. A piece that is not all of its rows' keys leaves its maximum, sum and values in a workspace, and a last kernel
-// joins them in the order of the keys.
+// all that bounds the kernel while there are few (64 rows of head_dim 128 do 48 multiply-adds per byte read, two products for the scores
+// and one for the values; the tensor core makes 96 of them, its tiles have 128 rows). The work is one list of 128-key tiles, over
+// sequences, KV heads and groups of up to 256 rows, the drafts a tile of their own behind each sequence's cached ones; the list is cut into
+// as many equal pieces as there are SMs, so sequences of any mix of lengths keep all of them busy. A piece that is not all of its rows'
+// keys leaves its maximum, sum and values in a workspace, and a last kernel joins them in the order of the keys.
 //
 // Roles: warp 0 streams Q and the tiles of K and V by TMA, warp 1 issues the products (scores Q K^T into tensor memory, O += P V
 // from it), and two warpgroups (warps 4..11) do the softmax, a row per thread, each with scores and an output of its own in tensor memory
 // (columns S_0, S_1, O_0, O_1; P lies over S). A group of more than 128 rows gives each warpgroup a tile of rows; one of up to 128
 // gives them the odd and the even key tiles, and the first one adds up what the two have. Either way the tensor core works for one
-// while the other is in its exponentials: with one warpgroup a tile took 2.1 us at 128 rows of head_dim 128 where its 64 KiB
-// arrive in 1.5. The whole call at 32 drafts, 32 / 8 heads of 128: 17 us at 1000 keys, 69 at 60000, 114 at 120000 (0.74 us per 1000 keys,
-// 5.5 TB/s, and 25 us of three launches, the ramp and the join).
+// while the other is in its exponentials: with one warpgroup, and Q as one part, a tile took 2.1 us at 128 rows of head_dim 128 where its
+// 64 KiB arrive in 1.5. The whole call at 32 drafts, 32 / 8 heads of 128, one after the other on caches that are not in L2: 17.5 us at
+// 1000 keys, 68 to 71 at 60000, 111 to 114 at 120000: 0.71 us per 1000 keys from there on, 5.8 TB/s, and 26 to 28 us of three launches,
+// the ramp and the join (a tree of 32 over 60001 keys of a cache of 65536: 73 to 77).
 //
 // Roundings to bf16: rotated K and V, as the caches hold them; Q in two parts, which is 16 bits; P, for the tensor core (sums of P and
 // the accumulators are fp32); the result.
@@ -467,7 +468,7 @@ tree_attn_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_constant_
         const bool drafts = s.t0 + t == s.nt - 1;        // 64 keys are enough for them
         // Q's two parts, so that the scores are those of an unrounded rotation. Rounded to bf16 it was the largest error of the result:
         // 4.4e-3 of it at 60001 keys, 2.2e-3 like this, of which the result's own rounding is 1.7e-3. It costs 0 to 8 % of the whole call's
-        // time at up to 3200 keys, 15 % at 60001 (67 -> 77 us).
+        // time at up to 3200 keys, 15 % at 60001 (67 -> 77 us, the header's last figure).
 #pragma unroll
         for (int kk = 0; kk < kD / 8; ++kk) {
           const int k = kk % (kD / 16);
@@ -791,8 +792,8 @@ static int launch_tree(const TreeParams& p, const TensorMap& tq, const TensorMap
   const int rc = p.n > p.tok ? launch_tree_attn<kD, kMod, true>(p, tq, tk, tv, st) : launch_tree_attn<kD, kMod, false>(p, tq, tk, tv, st);
   if (rc != 0) return rc;
   if (p.arrived != nullptr) return 0;
-  // Eight columns to a thread where there are threads enough (8 x 3000 keys, 24 drafts, 32 / 8 heads of 128 43 us with four, 40 like this),
-  // four and more pieces at a time else (1 x 60001 keys, 32 drafts 63.5, 65 with eight).
+  // Eight columns to a thread where there are threads enough (the call at 8 x 3000 keys, 24 drafts, 32 / 8 heads of 128: 47.0 us with four,
+  // 44.0 like this), four and more pieces at a time else (1 x 60001 keys, 32 drafts: 77.1, 77.5 with eight).
   const int combos = p.B * p.KVH * p.groups, rows = (p.n > p.tok ? 2 : 1) * p.tok * p.R;
   if ((long long)combos * rows * (kD / 8) >= 256LL * num_sms())
     return static_cast<int>(launch_pdl(tree_join_kernel<kD, 2>, dim3(combos, (rows * (kD / 8) + 255) / 256), dim3(256), 0, st, 0, p));
@@ -854,8 +855,8 @@ B200_API int b200_tree_attn_append(const void* kqv, void* kc, void* vc, void* ou
   p.part_o = static_cast<float4*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + 4LL * p.ctas * 128 * (D / 4));
   p.q = reinterpret_cast<bf16*>(p.part_ml + 4LL * p.ctas * 128);
-  // Few rows times few pieces: the CTA that finishes a (sequence, KV head) last joins its pieces, where a kernel of its own takes 3 to 5 us
-  // more than that; more of them would keep that one SM busy for longer.
+  // Few rows times few pieces: the CTA that finishes a (sequence, KV head) last joins its pieces (one token over 1801 keys, 16 / 4 heads of
+  // 128: 15.6 us, 18.0 with a kernel of its own); more of them would keep that one SM busy for longer.
   const long long combos = (long long)B * KVH * p.groups;
   p.arrived = n * p.R <= 8 && (p.ctas / combos + 2) * n * p.R <= 512
                   ? reinterpret_cast<int*>(p.q + 2 * (size_t)B * n * QH * D) : nullptr;
