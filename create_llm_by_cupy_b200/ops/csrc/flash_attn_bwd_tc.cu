@@ -825,7 +825,7 @@ __device__ __forceinline__ void fb_p_chunk(uint32_t (&rs)[16], uint32_t (&pk)[8]
 // minus_lse2 points at the 16 per-query values. A cap leaves P (1 - tanh^2) in place of P in rs, which is what dS is made from
 // (kTier: see score_cap.cuh). A bias: dist = first query's position minus the key's.
 // Roundings to bf16, here and behind it: P for dV, dS for dK and dQ (the tensor core's operands). With delta, whose output is bf16, they
-// leave dq and dk 2.6 to 3.1e-3 (root mean square) from the 64-bit result, of which their own rounding is 1.7e-3.
+// leave dq and dk 2.6 to 3.3e-3 (root mean square) from the 64-bit result, of which their own rounding is 1.7e-3.
 template <bool kMask, int kMod, int kTier = 0>
 __device__ __forceinline__ void fb_p_chunk_span(uint32_t (&rs)[16], uint32_t (&pk)[8], float sl2, const ScoreCap& cap,
                                                 const float* minus_lse2, const uint32_t* see, uint32_t krow, float slope2, float dist) {
@@ -1304,8 +1304,8 @@ flash_bwd_dkv_wide_kernel(const __grid_constant__ CUtensorMap tmQ, const __grid_
         const float* st = reinterpret_cast<const float*>(smem + Smem::kStats + s2 * Smem::kStatBytes) + wg * 64;
         bool need_mask = (m0 < n0 + 128) || (n0 + 128 > vlen);     // the diagonal tile or the padded tail
         // This thread's P^T (under a cap P^T (1 - tanh^2)) between the two phases: as it is, in fp32. Kept as bf16 pairs, as the
-        // causal form of head_dim 128 does, it left dq and dk at 3.1 to 3.6e-3, not 2.6 to 3.1e-3, and the capped form packed it a second time:
-        // 8192 tokens, 16 / 4 heads, forward and backward 1476 us, 1402 like this; four rows of 2048 292 / 283.
+        // causal form of head_dim 128 does, it left dq and dk at 3.1 to 3.6e-3, not 2.6 to 3.1e-3, and the capped form packed it a
+        // second time: 8192 tokens, 16 / 4 heads, forward and backward 1476 us, 1402 like this; four rows of 2048 292 / 283.
         constexpr bool kKeep32 = kD == 64 || kMod != kCausal;
         uint32_t pk[4][8], sc[64];
         if (!mbar_wait(&st_full[s2], (g / kSt) & 1, abort_flag)) { ok = false; break; }
