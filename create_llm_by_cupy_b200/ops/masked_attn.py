@@ -418,7 +418,7 @@ def tree_attn_append(kqv, kcache, vcache, lens, tree, QH: int, KVH: int, cos, si
     included: its own result is that of the cached tokens and of its ancestors that were kept. n = 1 with mask 1 is a decoded token.
     Weights are rounded to bf16 for the tensor core; the rotated Q goes in as two bf16 parts.
     Returns [B, n, QH, D]. A mask of 0 leaves the cached tokens alone; with none of them the result is 0. Cache rows from
-    lens + n on may hold anything."""
+    lens + n on may hold anything; the cached ones and all drafts have to be finite (a value that a draft does not see has weight 0)."""
     if native.host is not None:
         out = native.host.tree_attn(kqv, kcache, vcache, lens, tree, QH, KVH, cos, sin, 0.0 if scale is None else scale or -1.0, softcap,
                                     slopes)
