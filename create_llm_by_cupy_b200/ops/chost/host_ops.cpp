@@ -61,6 +61,12 @@ struct Api {
   long long (*tree_attn_workspace)(int, int, int, int, int, int);
   int (*tree_attn_append)(cptr, void*, void*, void*, cptr, cptr, cptr, cptr, cptr, void*, int, int, int, int, int, int, int, long long,
                           float, float, stream_t);
+  int (*paged_append)(cptr, cptr, void*, void*, void*, void*, cptr, cptr, cptr, cptr, cptr, int, long long, long long, long long, int, int,
+                      int, int, int, int, int, stream_t);
+  int (*paged_read)(void*, void*, void*, void*, cptr, cptr, cptr, void*, void*, int, int, int, int, int, int, int, int, stream_t);
+  int (*paged_attn_append)(cptr, void*, void*, void*, void*, cptr, cptr, cptr, cptr, cptr, void*, int, long long, int, int, int, int, int,
+                           int, int, int, float, float, stream_t);
+  int (*verify_drafts)(cptr, cptr, cptr, cptr, cptr, cptr, void*, void*, void*, void*, int, int, int, int, double, double, stream_t);
 };
 Api api;
 
@@ -640,6 +646,161 @@ PyObject* tree_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   END
 }
 
+// A pool of pages and the table of its sequences (see ``paged.PagedCache``).
+struct Pool {
+  void *k, *v, *ks, *vs;
+  cptr table;
+  int64_t pages, KVH, page, D, B, width;
+  int log_page, held;
+};
+bool int32_vector(const Tensor& t, int64_t n, int dev) {
+  return on(t, dev) && t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous();
+}
+// a[0..4]: k, v, k_scale or None, v_scale or None, table
+bool pool(PyObject* const* a, int dev, Pool* p) {
+  const Tensor *k = plain(a[0]), *v = plain(a[1]), *ks, *vs, *table = plain(a[4]);
+  if (!k || !v || !table || !optional(a[2], &ks) || !optional(a[3], &vs)) return false;
+  const auto dt = k->scalar_type();
+  p->held = dt == at::kBFloat16 ? 0 : dt == at::kChar ? 1 : dt == at::kFloat8_e4m3fn ? 2 : -1;
+  if (p->held < 0 || !on(*k, dev) || !on(*v, dev) || v->scalar_type() != dt || k->dim() != 4 || k->sizes() != v->sizes() ||
+      !k->is_contiguous() || !v->is_contiguous() || !aligned16(k->const_data_ptr()) || !aligned16(v->const_data_ptr()))
+    return false;
+  p->pages = k->size(0), p->KVH = k->size(1), p->page = k->size(2), p->D = k->size(3);
+  if (!fits(p->pages) || !fits(p->KVH) || (p->D != 64 && p->D != 128)) return false;
+  for (p->log_page = 5; p->log_page <= 10 && p->page != int64_t(1) << p->log_page;) ++p->log_page;
+  if (p->log_page > 10) return false;
+  if ((p->held != 0) != (ks != nullptr) || (ks != nullptr) != (vs != nullptr)) return false;
+  for (const Tensor* s : {ks, vs})
+    if (s && (!on(*s, dev) || s->scalar_type() != at::kFloat || s->dim() != 3 || !s->is_contiguous() || s->sizes() != k->sizes().slice(0, 3)))
+      return false;
+  if (!on(*table, dev) || table->scalar_type() != at::kInt || table->dim() != 2 || !table->is_contiguous()) return false;
+  p->B = table->size(0), p->width = table->size(1);
+  if (!fits(p->B) || !fits(p->width) || p->width * p->page >= int64_t(1) << 31) return false;
+  p->k = k->mutable_data_ptr(), p->v = v->mutable_data_ptr();
+  p->ks = ks ? ks->mutable_data_ptr() : nullptr, p->vs = vs ? vs->mutable_data_ptr() : nullptr;
+  p->table = table->const_data_ptr();
+  return true;
+}
+bool rotary(const Tensor& c, const Tensor& s, int64_t D, int dev) {
+  for (const Tensor* t : {&c, &s})
+    if (!on(*t, dev) || t->scalar_type() != at::kFloat || t->dim() != 2 || !t->is_contiguous() || t->sizes() != c.sizes() ||
+        !fits(t->size(0)) || t->size(1) != D / 2 || !aligned16(t->const_data_ptr()))
+      return false;
+  return true;
+}
+
+// paged_append(k, v, pool k, v, k_scale, v_scale, table, seq, pos, cos or None, sin or None) -> True
+PyObject* paged_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  ARGS(11)
+  const Tensor *k = plain(a[0]), *v = plain(a[1]), *seq = plain(a[7]), *pos = plain(a[8]), *c, *s;
+  Pool p;
+  if (!k || !v || !seq || !pos || !optional(a[9], &c) || !optional(a[10], &s) || (c == nullptr) != (s == nullptr) || !pool(a + 2, dev, &p))
+    Py_RETURN_NONE;
+  const int64_t M = k->dim() == 3 ? k->size(0) : 0;
+  if (M <= 0 || (c && !rotary(*c, *s, p.D, dev)) || !int32_vector(*seq, M, dev) || !int32_vector(*pos, M, dev)) Py_RETURN_NONE;
+  int64_t ld[2];
+  for (int i = 0; i < 2; ++i) {
+    const Tensor& t = i == 0 ? *k : *v;
+    if (!bf16_on(t, dev) || t.sizes() != at::IntArrayRef({M, p.KVH, p.D}) || t.stride(2) != 1 || t.stride(1) != p.D ||
+        !aligned16(t.const_data_ptr()))
+      Py_RETURN_NONE;
+    ld[i] = M > 1 ? t.stride(0) : p.KVH * p.D;
+    if (ld[i] % 8 != 0 || ld[i] <= 0) Py_RETURN_NONE;
+  }
+  if (launched([&] {
+        return api.paged_append(k->const_data_ptr(), v->const_data_ptr(), p.k, p.v, p.ks, p.vs, p.table, seq->const_data_ptr(),
+                                pos->const_data_ptr(), c ? c->const_data_ptr() : nullptr, s ? s->const_data_ptr() : nullptr,
+                                c ? int(c->size(0)) : 0, M, ld[0], ld[1], int(p.B), int(p.width), int(p.pages), int(p.KVH), p.log_page,
+                                int(p.D), p.held, stream(dev));
+      }))
+    Py_RETURN_TRUE;
+  END
+}
+
+// paged_read(pool k, v, k_scale, v_scale, table, lens, kcache, vcache, start or None) -> True
+PyObject* paged_read(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  ARGS(9)
+  const Tensor *lens = plain(a[5]), *kc = plain(a[6]), *vc = plain(a[7]), *start;
+  Pool p;
+  if (!lens || !kc || !vc || !optional(a[8], &start) || !pool(a, dev, &p) || p.B > 32767 || p.KVH > 65535) Py_RETURN_NONE;
+  for (const Tensor* t : {kc, vc})
+    if (!bf16_on(*t, dev) || t->dim() != 4 || !t->is_contiguous() || t->size(0) != p.B || t->size(1) != p.KVH || !fits(t->size(2)) ||
+        t->size(3) != p.D || t->size(2) != kc->size(2) || !aligned16(t->const_data_ptr()))
+      Py_RETURN_NONE;
+  if (!int32_vector(*lens, p.B, dev) || (start && !int32_vector(*start, p.B, dev))) Py_RETURN_NONE;
+  if (launched([&] {
+        return api.paged_read(p.k, p.v, p.ks, p.vs, p.table, start ? start->const_data_ptr() : nullptr, lens->const_data_ptr(),
+                              kc->mutable_data_ptr(), vc->mutable_data_ptr(), int(kc->size(2)), int(p.B), int(p.width), int(p.pages),
+                              int(p.KVH), p.log_page, int(p.D), p.held, stream(dev));
+      }))
+    Py_RETURN_TRUE;
+  END
+}
+
+// paged_attn(kqv, pool k, v, k_scale, v_scale, table, lens, QH, KVH, cos, sin, scale, softcap, slopes or None) -> out
+PyObject* paged_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  ARGS(14)
+  const Tensor *x = plain(a[0]), *lens = plain(a[6]), *c = plain(a[9]), *s = plain(a[10]), *sl;
+  const int QH = as_int(a[7]), KVH = as_int(a[8]);
+  double scale = PyFloat_AsDouble(a[11]);
+  const double cap = PyFloat_AsDouble(a[12]);
+  CHECK_NUMBERS
+  Pool p;
+  if (!x || !lens || !c || !s || !optional(a[13], &sl) || !tma_rows(*x, dev) || !pool(a + 1, dev, &p)) Py_RETURN_NONE;
+  if (QH <= 0 || KVH != p.KVH || QH % KVH != 0 || p.B > 65535 || int64_t(KVH) * ((QH / KVH + 7) / 8) > 65535 || x->size(0) != p.B ||
+      x->size(1) != (2 * int64_t(KVH) + QH) * p.D || (p.B > 1 && x->stride(0) <= 0))
+    Py_RETURN_NONE;
+  if (!int32_vector(*lens, p.B, dev) || !rotary(*c, *s, p.D, dev)) Py_RETURN_NONE;
+  if (sl && (!on(*sl, dev) || sl->scalar_type() != at::kFloat || sl->dim() != 1 || sl->size(0) != QH || !sl->is_contiguous()))
+    Py_RETURN_NONE;
+  if (!score_numbers(&scale, cap, sl, p.D)) Py_RETURN_NONE;
+  Tensor out = empty({p.B, QH, p.D}, *x, at::kBFloat16);
+  if (launched([&] {
+        return api.paged_attn_append(x->const_data_ptr(), p.k, p.v, p.ks, p.vs, p.table, lens->const_data_ptr(), c->const_data_ptr(),
+                                     s->const_data_ptr(), sl ? sl->const_data_ptr() : nullptr, out.mutable_data_ptr(), int(c->size(0)),
+                                     x->stride(0), int(p.B), int(p.width), int(p.pages), QH, KVH, p.log_page, int(p.D), p.held,
+                                     float(scale), float(cap), stream(dev));
+      }))
+    return wrap(out);
+  END
+}
+
+// verify_drafts(logits, tokens, parents, u, temp, top, draft_probs or None, accept or None) -> (tokens, path, count)
+PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  ARGS(8)
+  const Tensor *x = plain(a[0]), *tok = plain(a[1]), *par = plain(a[2]), *u = plain(a[3]), *q, *acc;
+  const double temp = PyFloat_AsDouble(a[4]), top = PyFloat_AsDouble(a[5]);
+  CHECK_NUMBERS
+  if (!x || !tok || !par || !u || !optional(a[6], &q) || !optional(a[7], &acc) || (q == nullptr) != (acc == nullptr)) Py_RETURN_NONE;
+  if (!on(*x, dev) || (x->scalar_type() != at::kFloat && x->scalar_type() != at::kBFloat16) || x->dim() != 3 || !x->is_contiguous())
+    Py_RETURN_NONE;
+  const int64_t B = x->size(0), nodes = x->size(1), V = x->size(2);
+  if (!fits(B) || nodes < 1 || nodes > 64 || !fits(V) || V > 8 * 416 * 128 || !(temp == 0. || temp >= 1e-6) || !std::isfinite(temp) ||
+      !(top > 0.))
+    Py_RETURN_NONE;
+  for (const Tensor* t : {tok, par, u, acc})
+    if (t && (!on(*t, dev) || t->scalar_type() != (t == u || t == acc ? at::kFloat : at::kInt) || t->sizes() != at::IntArrayRef({B, nodes}) ||
+              !t->is_contiguous()))
+      Py_RETURN_NONE;
+  if (q && (!on(*q, dev) || q->scalar_type() != at::kFloat || q->sizes() != x->sizes() || !q->is_contiguous())) Py_RETURN_NONE;
+  Tensor out = empty({B, nodes}, *x, at::kInt), path = empty({B, nodes}, *x, at::kInt), count = empty({B}, *x, at::kInt),
+         ws = empty({2 * B * nodes}, *x, at::kInt);
+  if (!launched([&] {
+        return api.verify_drafts(x->const_data_ptr(), q ? q->const_data_ptr() : nullptr, tok->const_data_ptr(), par->const_data_ptr(),
+                                 u->const_data_ptr(), acc ? acc->const_data_ptr() : nullptr, out.mutable_data_ptr(),
+                                 path.mutable_data_ptr(), count.mutable_data_ptr(), ws.mutable_data_ptr(), x->scalar_type() == at::kBFloat16,
+                                 int(B), int(nodes), int(V), temp, top, stream(dev));
+      }))
+    Py_RETURN_NONE;
+  PyObject* r = PyTuple_New(3);
+  if (r == nullptr) return nullptr;
+  PyTuple_SET_ITEM(r, 0, wrap(out));
+  PyTuple_SET_ITEM(r, 1, wrap(path));
+  PyTuple_SET_ITEM(r, 2, wrap(count));
+  return r;
+  END_HANDLE_TH_ERRORS
+}
+
 // memory_room(device index, bytes of the device) -> see ``native.memory_room``
 PyObject* memory_room(PyObject*, PyObject* const* a, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -683,6 +844,10 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   get(api.flash_bwd_span, "b200_flash_bwd_span");
   get(api.tree_attn_workspace, "b200_tree_attn_workspace");
   get(api.tree_attn_append, "b200_tree_attn_append");
+  get(api.paged_append, "b200_paged_append");
+  get(api.paged_read, "b200_paged_read");
+  get(api.paged_attn_append, "b200_paged_attn_append");
+  get(api.verify_drafts, "b200_verify_drafts");
   Py_RETURN_NONE;
   END_HANDLE_TH_ERRORS
 }
@@ -699,7 +864,8 @@ PyObject* device_ready(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {METHOD(bind), METHOD(device_ready), METHOD(memory_room), METHOD(rmsnorm_fwd), METHOD(rmsnorm_bwd),
                          METHOD(embedding_fwd), METHOD(gemm), METHOD(tma_ok), METHOD(gemm_rope), METHOD(gemm_swiglu),
                          METHOD(flash_fwd), METHOD(split_heads), METHOD(decode_attn_block), METHOD(mlp_few_rows),
-                         METHOD(span_mask), METHOD(span_fwd), METHOD(span_bwd), METHOD(tree_attn), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(span_mask), METHOD(span_fwd), METHOD(span_bwd), METHOD(tree_attn),
+                         METHOD(paged_append), METHOD(paged_read), METHOD(paged_attn), METHOD(verify_drafts), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_b200host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace
