@@ -15,6 +15,7 @@
 
 #include <atomic>
 #include <cmath>
+#include <cstring>
 
 #include "common.cuh"
 
@@ -23,7 +24,8 @@ namespace cg = cooperative_groups;
 
 typedef unsigned long long u64;
 
-constexpr int VD_THREADS = 512, VD_WARPS = VD_THREADS / 32, VD_SEG = 128, VD_MAX_SEGS = 416, VD_MAX_NODES = 64, VD_MAX_CLUSTER = 8;
+constexpr int VD_THREADS = 512, VD_WARPS = VD_THREADS / 32, VD_SEG = 128, VD_MAX_SEGS = 195, VD_MAX_NODES = 64, VD_MAX_CLUSTER = 8;
+constexpr int VD_BINS = 2048, VD_LIST = 512;      // bins of masses; tokens that are put in order one by one
 
 struct VerifyParams {
   const void* logits;        // [B, n, V], fp32 or bf16
@@ -39,21 +41,51 @@ struct VerifyParams {
   double inv_temp;           // 0: the largest logit
   u64 top;                   // the nucleus' mass is top 2^-top_shift; 0: everything
   int top_shift;
+  u64 tail;                  // weights (as bits) below it cannot be where the nucleus ends
+  int wide;                  // logits [node] start where four can be loaded at once
 };
 
 struct VerifyShared {
   u64 warp[VD_WARPS];
-  u64 part[2][2];            // what this CTA adds to a sum over the row
-  u64 seg[VD_MAX_SEGS];
-  int first[VD_WARPS];
+  u64 part[2];               // what this CTA adds to a sum over the row, two in turn
+  u64 seg[VD_MAX_SEGS + 1];
+  u64 above;                 // of the nucleus' search: mass above the bin, and the bin
+  int bin, listed;
+  u64 list_w[VD_LIST];
+  int list_i[VD_LIST];
+  u64 all_w[VD_LIST];
+  int all_i[VD_LIST];
+  u64 cut_w;
+  int cut_i;
+  u64 bins[VD_BINS];
 };
+constexpr int kVerifyShared = int((sizeof(VerifyShared) + 15) / 16 * 16);
 
-// Order of fp32 numbers as an order of unsigned ones; NaN has become -infinity, and +infinity the largest number, before.
-__device__ __forceinline__ uint32_t order_key(float x) {
+// What a logit counts as: NaN as -infinity, +infinity as the largest number.
+__device__ __forceinline__ float tidy(float x) { return fminf(fmaxf(x, -CUDART_INF_F), 3.402823466e38f); }
+// fp32 -> fp64 by moving bits: the conversion runs at an eighth of the rate. Exact but for 0 and numbers below 2^-126, which come out
+// as some number below 2^-126, and infinity, which is 2^128.
+__device__ __forceinline__ double wide_of(float x) {
   const uint32_t u = __float_as_uint(x);
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  return __hiloint2double(int((u & 0x80000000u) | (((u & 0x7fffffffu) >> 3) + 0x38000000u)), int(u << 29));
 }
-__device__ __forceinline__ float tidy(float x) { return x != x ? -CUDART_INF_F : fminf(x, 3.402823466e38f); }
+// e^x for x <= 0 by Tang's table-driven method (ACM TOMS 15, 1989): x = (32 k + i) ln2 / 32 + r, |r| <= ln2 / 64, e^x = 2^k 2^(i / 32)
+// e^r, e^r by its Taylor sum to r^5. `scaled` is x 32 / ln2. Off by at most 3e-13 (the sum's rest 2e-15, the argument's rounding the
+// rest), 0 below e^-700. The table lies in the lanes of a warp, which all take part.
+__device__ __forceinline__ double exp_of(double x, double scaled, double power) {
+  const double big = 6755399441055744.;                      // 1.5 2^52: the sum's last place is 1
+  const double t = scaled + big;
+  const int n = __double2loint(t);
+  const double r = fma(big - t, 0.021660849392498290, x);
+  double p = fma(r, 1. / 120, 1. / 24);
+  p = fma(p, r, 1. / 6);
+  p = fma(p, r, .5);
+  p = fma(p, r, 1.) * r;
+  const int i = n & 31;
+  const double T = __hiloint2double(__shfl_sync(0xffffffffu, __double2hiint(power), i), __shfl_sync(0xffffffffu, __double2loint(power), i));
+  const double y = fma(T, p, T);
+  return x < -700. ? 0. : __hiloint2double(__double2hiint(y) + (n >> 5) * (1 << 20), __double2loint(y));
+}
 
 // x * total for x = m 2^-k in [0, 1], rounded down or up: exact, so that masses that are equal are so here.
 __device__ __forceinline__ u64 part_of(u64 m, int k, u64 total, bool up) {
@@ -77,20 +109,58 @@ __device__ __forceinline__ u64 warp_sum(u64 v) {
   for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
   return v;
 }
+// Sums of the lanes up to and with this one.
+__device__ __forceinline__ u64 warp_scan(u64 v, int lane) {
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += x;
+  }
+  return v;
+}
 
 template <bool kBf16>
-__global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const VerifyParams p) {
+__device__ __forceinline__ float logit_at(const VerifyParams& p, long long node, int j) {
+  const long long at = node * p.V + j;
+  return tidy(kBf16 ? __bfloat162float(static_cast<const bf16*>(p.logits)[at]) : static_cast<const float*>(p.logits)[at]);
+}
+
+// Four logits from an aligned place, as they are.
+template <bool kBf16>
+__device__ __forceinline__ float4 logits_at(const VerifyParams& p, long long node, int j) {
+  const long long at = node * p.V + j;
+  if (!kBf16) return *reinterpret_cast<const float4*>(static_cast<const float*>(p.logits) + at);
+  const uint2 u = *reinterpret_cast<const uint2*>(static_cast<const bf16*>(p.logits) + at);
+  return make_float4(__uint_as_float(u.x << 16), __uint_as_float(u.x & 0xffff0000u), __uint_as_float(u.y << 16),
+                     __uint_as_float(u.y & 0xffff0000u));
+}
+
+// Grid (cluster, nodes), cluster (size, 1, 1).
+//
+// A CTA's slice of the row goes through shared memory once, in segments of 128 that belong to one warp throughout (four neighbouring
+// tokens to a lane; token e of lane l stands at 32 e + l, so that eight-byte accesses meet no bank twice): the logits, in their place the
+// weights, and from then on passes over the weights only. The nucleus' end is looked for in a histogram of masses over the weights' bits
+// (an order of positive numbers), in finer ones while too many tokens share the bin, and then token by token.
+template <bool kBf16>
+__global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const VerifyParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   VerifyShared& sh = *reinterpret_cast<VerifyShared*>(smem);
-  float* xs = reinterpret_cast<float*>(smem + (sizeof(VerifyShared) + 15) / 16 * 16);
+  double* ws = reinterpret_cast<double*>(smem + kVerifyShared);
   cg::cluster_group cluster = cg::this_cluster();
   const int cs = gridDim.x, rank = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int lo = min(rank * p.slice, p.V), size = min(p.slice, p.V - lo);
   const int segs = (size + VD_SEG - 1) / VD_SEG;
-  const double unit = exp2(double(62 - (32 - __clz(p.V))));
+  const int bits = min(62 - (32 - __clz(p.V)), 51);
+  const double unit = __hiloint2double((1023 + bits) << 20, 0);      // 2^bits
+  const double kRest = 2251799813685248.;                    // 2^51, the same for what refusals leave
+  const double power = exp2(double(lane) / 32.);
   pdl_wait();
   pdl_trigger();
   int phase = 0;
+  auto meet = [&] {
+    if (cs > 1) cluster.sync();
+    else __syncthreads();
+  };
   // Sum over the row, with what stands in front of this CTA; all threads.
   auto row_sum = [&](u64 v, u64* before) {
     v = warp_sum(v);
@@ -98,12 +168,12 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const VerifyPar
     __syncthreads();
     if (warp == 0) {
       v = warp_sum(lane < VD_WARPS ? sh.warp[lane] : 0);
-      if (lane == 0) sh.part[phase][0] = v;
+      if (lane == 0) sh.part[phase] = v;
     }
-    cluster.sync();
+    meet();
     u64 all = 0, ahead = 0;
     for (int c = 0; c < cs; ++c) {
-      const u64 x = *cluster.map_shared_rank(&sh.part[phase][0], c);
+      const u64 x = *cluster.map_shared_rank(&sh.part[phase], c);
       if (c < rank) ahead += x;
       all += x;
     }
@@ -111,42 +181,59 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const VerifyPar
     if (before != nullptr) *before = ahead;
     return all;
   };
-  auto row_max = [&](u64 v) {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
+  auto row_max = [&](uint32_t v) {
+    v = __reduce_max_sync(0xffffffffu, v);
     if (lane == 0) sh.warp[warp] = v;
     __syncthreads();
     if (warp == 0) {
-      v = lane < VD_WARPS ? sh.warp[lane] : 0;
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) v = max(v, __shfl_xor_sync(0xffffffffu, v, o));
-      if (lane == 0) sh.part[phase][0] = v;
+      v = __reduce_max_sync(0xffffffffu, lane < VD_WARPS ? uint32_t(sh.warp[lane]) : 0u);
+      if (lane == 0) sh.part[phase] = v;
     }
-    cluster.sync();
-    u64 all = 0;
-    for (int c = 0; c < cs; ++c) all = max(all, *cluster.map_shared_rank(&sh.part[phase][0], c));
+    meet();
+    uint32_t all = 0;
+    for (int c = 0; c < cs; ++c) all = max(all, uint32_t(*cluster.map_shared_rank(&sh.part[phase], c)));
     phase ^= 1;
     return all;
   };
+  // An integer number of units, rounded to nearest: the last bits of a sum with 2^52.
+  auto fixed = [](double w, double u) { return u64(__double_as_longlong(fma(w, u, 4503599627370496.))) - 0x4330000000000000ull; };
 
   for (long long node = blockIdx.y; node < p.rows; node += gridDim.y) {
     const int i = int(node % p.n);
     const long long first = node - i;                        // the sequence's node 0
     const int up = i == 0 ? -1 : p.parents[node];
     if (i > 0 && (up < 0 || up >= i)) continue;              // not there (the same for the whole cluster)
-    auto at = [&](int j) {
-      return tidy(kBf16 ? __bfloat162float(static_cast<const bf16*>(p.logits)[node * p.V + j]) : static_cast<const float*>(p.logits)[node * p.V + j]);
-    };
-    u64 best = 0;                                            // largest logit, lowest index
     __syncthreads();
-    for (int j = tid; j < size; j += VD_THREADS) {
-      const float x = at(lo + j);
-      xs[j] = x;
-      best = max(best, u64(order_key(x)) << 32 | uint32_t(~(lo + j)));
+    float top = -CUDART_INF_F;
+    for (int s0 = warp; s0 < segs; s0 += 4 * VD_WARPS) {     // four segments on their way at a time
+      float4 x[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int j = (s0 + c * VD_WARPS) * VD_SEG + 4 * lane;
+        if (p.wide && j + 3 < size) {
+          x[c] = logits_at<kBf16>(p, node, lo + j);
+        } else {
+          x[c].x = j < size ? logit_at<kBf16>(p, node, lo + j) : -CUDART_INF_F;
+          x[c].y = j + 1 < size ? logit_at<kBf16>(p, node, lo + j + 1) : -CUDART_INF_F;
+          x[c].z = j + 2 < size ? logit_at<kBf16>(p, node, lo + j + 2) : -CUDART_INF_F;
+          x[c].w = j + 3 < size ? logit_at<kBf16>(p, node, lo + j + 3) : -CUDART_INF_F;
+        }
+      }
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        if (s0 + c * VD_WARPS >= segs) break;
+        float* to = reinterpret_cast<float*>(ws + (s0 + c * VD_WARPS) * VD_SEG + lane);
+        const float y[4] = {tidy(x[c].x), tidy(x[c].y), tidy(x[c].z), tidy(x[c].w)};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          to[64 * e] = y[e];
+          top = fmaxf(top, y[e]);
+        }
+      }
     }
-    best = row_max(best);
-    const int arg = int(~uint32_t(best));
-    const float largest = tidy(at(arg));
+    // fp32 numbers in the order of unsigned ones
+    const uint32_t ub = __float_as_uint(top), most = row_max(ub & 0x80000000u ? ~ub : ub | 0x80000000u);
+    const float largest = __uint_as_float(most & 0x80000000u ? most & 0x7fffffffu : ~most);
     if (largest == -CUDART_INF_F) {                          // nothing to choose
       if (rank == 0 && tid == 0) {
         p.choice[node] = -1;
@@ -154,156 +241,293 @@ __global__ void __launch_bounds__(VD_THREADS) verify_rows_kernel(const VerifyPar
       }
       continue;
     }
-    auto raw = [&](float x, int j) {                         // weight of token j, 1 for the largest
-      return p.inv_temp == 0. ? (j == arg ? 1. : 0.) : exp((double(x) - double(largest)) * p.inv_temp);
+    int arg = -1;                                            // temperature 0: the first of the largest
+    if (p.inv_temp == 0.) {
+      uint32_t lowest = 0;
+      for (int s = warp; s < segs; s += VD_WARPS)
+#pragma unroll
+        for (int e = 3; e >= 0; --e)
+          if (*reinterpret_cast<const float*>(ws + s * VD_SEG + 32 * e + lane) == largest) lowest = max(lowest, ~uint32_t(lo + s * VD_SEG + 4 * lane + e));
+      arg = int(~row_max(lowest));
+    }
+    const double zero = wide_of(largest), per32 = p.inv_temp * 46.166241308446828;       // 32 / ln2
+    auto raw = [&](float x, int j) {                         // weight of token j, 1 for the largest; whole warps
+      if (p.inv_temp == 0.) return j == arg ? 1. : 0.;
+      const double d = wide_of(x) - zero;
+      return exp_of(d * p.inv_temp, d * per32, power);
     };
-    auto fixed = [&](double w) { return u64(__double2ull_rn(w * unit)); };
+    const bool nucleus = p.top != 0 && p.inv_temp != 0.;
+    u64 cut_w = 0;                                           // weights below it are cut off, and those equal to it behind token cut_i
+    int cut_i = 0x7fffffff;
+    u64 khi = 0x3ff0000000000001ull, above = 0;              // the end lies in [klo, khi) (bits of weights), and this much above it
+    u64 klo = p.tail;
+    int shift = 0;
+    if (nucleus) {
+      while ((khi - klo - 1) >> shift >= VD_BINS) ++shift;
+      for (int t = tid; t < VD_BINS; t += VD_THREADS) sh.bins[t] = 0;
+      __syncthreads();
+    }
+    // Weights in the logits' place; sums of the segments, or the first histogram.
     u64 mine = 0;
-    for (int j = tid; j < size; j += VD_THREADS) mine += fixed(raw(xs[j], lo + j));
-    u64 total = row_sum(mine, nullptr);
-    uint32_t cut = 0;                                        // keys below it are cut off, and those equal to it behind `last`
-    int last = 0x7fffffff;
-    if (p.top != 0 && p.inv_temp != 0.) {
-      // The largest key with which the tokens from it on reach the mass.
+    for (int s = warp; s < segs; s += VD_WARPS) {
+      u64 v = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        double* at = ws + s * VD_SEG + 32 * e + lane;
+        const double w = raw(*reinterpret_cast<const float*>(at), lo + s * VD_SEG + 4 * lane + e);
+        *at = w;
+        const u64 f = fixed(w, unit), k = u64(__double_as_longlong(w));
+        v += f;
+        if (nucleus && k >= klo) atomicAdd(&sh.bins[(khi - 1 - k) >> shift], f);
+      }
+      mine += v;
+      if (!nucleus) {
+        v = warp_sum(v);
+        if (lane == 0) sh.seg[s] = v;
+      }
+    }
+    u64 before, total = row_sum(mine, &before);
+    if (nucleus) {
       const u64 want = part_of(p.top, p.top_shift, total, true);
-      for (int bit = 31; bit >= 0; --bit) {
-        const uint32_t trial = cut | 1u << bit;
-        mine = 0;
-        for (int j = tid; j < size; j += VD_THREADS)
-          if (order_key(xs[j]) >= trial) mine += fixed(raw(xs[j], lo + j));
-        if (row_sum(mine, nullptr) >= want) cut = trial;
-      }
-      mine = 0;
-      u64 same = 0;
-      for (int j = tid; j < size; j += VD_THREADS) {
-        const uint32_t k = order_key(xs[j]);
-        if (k > cut) mine += fixed(raw(xs[j], lo + j));
-        if (k == cut) ++same;
-      }
-      const u64 above = row_sum(mine, nullptr), ties = row_sum(same, nullptr);
-      if (ties > 1) {
-        const uint32_t ku = cut & 0x80000000u ? cut & 0x7fffffffu : ~cut;
-        const u64 each = fixed(raw(__uint_as_float(ku), -1));
-        // how many of the equal ones: the fewest that reach the mass
-        const u64 need = each == 0 || want <= above + each ? 1 : (want - above + each - 1) / each;
-        if (need < ties) {                                   // the index of the last one that is kept
-          int low = 0, high = p.V - 1;
-          while (low < high) {
-            const int mid = low + (high - low) / 2;
-            same = 0;
-            for (int j = tid; j < size; j += VD_THREADS) same += order_key(xs[j]) == cut && lo + j <= mid;
-            if (row_sum(same, nullptr) >= need) high = mid;
-            else low = mid + 1;
+      while (true) {
+        // The bin in which the masses of all CTAs reach `want`: four bins to a thread.
+        u64 v[VD_BINS / VD_THREADS], sum = 0;
+#pragma unroll
+        for (int e = 0; e < VD_BINS / VD_THREADS; ++e) v[e] = 0;
+        for (int c = 0; c < cs; ++c) {
+          const ulonglong2* from = reinterpret_cast<const ulonglong2*>(cluster.map_shared_rank(&sh.bins[tid * (VD_BINS / VD_THREADS)], c));
+#pragma unroll
+          for (int e = 0; e < VD_BINS / VD_THREADS; e += 2) {
+            const ulonglong2 x = from[e / 2];
+            v[e] += x.x;
+            v[e + 1] += x.y;
           }
-          last = low;
+        }
+#pragma unroll
+        for (int e = 0; e < VD_BINS / VD_THREADS; ++e) sum += v[e];
+        const u64 scan = warp_scan(sum, lane);
+        if (lane == 31) sh.warp[warp] = scan;
+        if (tid == 0) {
+          sh.bin = -1;
+          sh.listed = 0;
+        }
+        __syncthreads();
+        u64 at = above + scan - sum;
+        for (int w = 0; w < warp; ++w) at += sh.warp[w];
+        if (at < want && at + sum >= want) {
+          int e = 0;
+          while (e < VD_BINS / VD_THREADS - 1 && at + v[e] < want) at += v[e++];
+          sh.bin = tid * (VD_BINS / VD_THREADS) + e;
+          sh.above = at;
+        }
+        __syncthreads();
+        if (sh.bin < 0) break;                               // (cannot be: everything is kept)
+        above = sh.above;
+        khi -= u64(sh.bin) << shift;
+        klo = khi - klo > 1ull << shift ? khi - (1ull << shift) : klo;
+        // Its tokens, if they are few.
+        for (int s = warp; s < segs; s += VD_WARPS)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const u64 k = u64(__double_as_longlong(ws[s * VD_SEG + 32 * e + lane]));
+            if (k >= klo && k < khi && s * VD_SEG + 4 * lane + e < size) {
+              const int n = atomicAdd(&sh.listed, 1);
+              if (n < VD_LIST) {
+                sh.list_w[n] = k;
+                sh.list_i[n] = lo + s * VD_SEG + 4 * lane + e;
+              }
+            }
+          }
+        meet();
+        int all = 0;
+        for (int c = 0; c < cs; ++c) all = min(all + *cluster.map_shared_rank(&sh.listed, c), 1 << 24);
+        if (all <= VD_LIST) {
+          int n = 0;
+          for (int c = 0; c < cs; ++c) {
+            const int m = *cluster.map_shared_rank(&sh.listed, c);
+            if (tid < m) {
+              sh.all_w[n + tid] = *cluster.map_shared_rank(&sh.list_w[tid], c);
+              sh.all_i[n + tid] = *cluster.map_shared_rank(&sh.list_i[tid], c);
+            }
+            n += m;
+          }
+          __syncthreads();
+          if (tid < all) {
+            const u64 k = sh.all_w[tid];
+            const int j = sh.all_i[tid];
+            u64 front = above;
+            for (int o = 0; o < all; ++o) {
+              const u64 ko = sh.all_w[o];
+              if (ko > k || (ko == k && sh.all_i[o] < j)) front += fixed(__longlong_as_double((long long)ko), unit);
+            }
+            const u64 f = fixed(__longlong_as_double((long long)k), unit);
+            if (front < want && front + f >= want) {
+              sh.cut_w = k;
+              sh.cut_i = j;
+            }
+          }
+          __syncthreads();
+          cut_w = sh.cut_w;
+          cut_i = sh.cut_i;
+          break;
+        }
+        if (shift == 0) {                                    // one weight, which many tokens have: the first of them that reach the mass
+          const u64 each = fixed(__longlong_as_double((long long)klo), unit);
+          u64 need = each == 0 || want <= above + each ? 1 : (want - above + each - 1) / each;
+          mine = 0;
+          for (int s = warp; s < segs; s += VD_WARPS) {
+            u64 n = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) n += u64(__double_as_longlong(ws[s * VD_SEG + 32 * e + lane])) == klo && s * VD_SEG + 4 * lane + e < size;
+            n = warp_sum(n);
+            if (lane == 0) sh.seg[s] = n;
+            mine += lane == 0 ? n : 0;
+          }
+          const u64 ties = row_sum(mine, &before);
+          need = min(need, ties);
+          cut_w = klo;
+          if (tid == 0) sh.cut_i = -1;
+          __syncthreads();
+          if (warp == 0) {                                   // the owner of the last one: its segment, then its place
+            u64 sum = before;
+            for (int s = 0; s < segs; ++s) {
+              if (sum < need && sum + sh.seg[s] >= need) {
+                u64 n = 0;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) n += u64(__double_as_longlong(ws[s * VD_SEG + 32 * e + lane])) == klo && s * VD_SEG + 4 * lane + e < size;
+                u64 at = sum + warp_scan(n, lane) - n;
+                if (at < need && at + n >= need)
+                  for (int e = 0; e < 4; ++e)
+                    if (u64(__double_as_longlong(ws[s * VD_SEG + 32 * e + lane])) == klo && s * VD_SEG + 4 * lane + e < size && ++at == need)
+                      sh.cut_i = lo + s * VD_SEG + 4 * lane + e;
+              }
+              sum += sh.seg[s];
+            }
+          }
+          __syncthreads();
+          cut_i = int(row_max(tid == 0 ? uint32_t(sh.cut_i + 1) : 0u)) - 1;
+          break;
+        }
+        // Too many: their masses in finer bins.
+        shift = shift > 11 ? shift - 11 : 0;
+        for (int t = tid; t < VD_BINS; t += VD_THREADS) sh.bins[t] = 0;
+        __syncthreads();
+        for (int s = warp; s < segs; s += VD_WARPS)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const double w = ws[s * VD_SEG + 32 * e + lane];
+            const u64 k = u64(__double_as_longlong(w));
+            if (k >= klo && k < khi) atomicAdd(&sh.bins[(khi - 1 - k) >> shift], fixed(w, unit));
+          }
+        meet();
+      }
+    }
+    const float* q = p.q != nullptr ? p.q + node * p.V : nullptr;
+    double used = 0., mass = 1., norm = 0.;
+    auto kept = [&](double w, int j) {                       // of the nucleus
+      const u64 k = u64(__double_as_longlong(w));
+      return k > cut_w || (k == cut_w && j <= cut_i);
+    };
+    // Sums of the segments of w, or of max(p - used q, 0) in units of kRest.
+    auto share = [&](int s, int e, bool rest) {
+      const int j = s * VD_SEG + 4 * lane + e;
+      if (j >= size) return u64(0);
+      double w = ws[s * VD_SEG + 32 * e + lane];
+      if (!kept(w, lo + j)) w = 0.;
+      return rest ? (w > 0. ? fixed(fmax(w * norm - used * double(q[lo + j]), 0.), kRest) : 0) : fixed(w, unit);
+    };
+    auto sum_up = [&](bool rest) {
+      u64 sum = 0;
+      for (int s = warp; s < segs; s += VD_WARPS) {
+        u64 v = 0;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v += share(s, e, rest);
+        v = warp_sum(v);
+        if (lane == 0) {
+          sh.seg[s] = v;
+          sum += v;
         }
       }
-    }
-    auto weight = [&](float x, int j) {
-      const uint32_t k = order_key(x);
-      return k > cut || (k == cut && j <= last) ? raw(x, j) : 0.;
+      return row_sum(sum, &before);
     };
-    if (cut != 0) {
-      mine = 0;
-      for (int j = tid; j < size; j += VD_THREADS) mine += fixed(weight(xs[j], lo + j));
-      total = row_sum(mine, nullptr);
-    }
-    // Children, as bits.
-    u64 kids = 0;
-    for (int j = i + 1; j < p.n; ++j) kids |= u64(p.parents[first + j] == i) << j;
+    if (nucleus) total = sum_up(false);
+    norm = unit / double(total);                             // weight -> probability
+    u64 kids = 0;                                            // children, as bits
+    for (int j = lane; j < p.n; j += 32) kids |= u64(j > i && p.parents[first + j] == i) << j;
+    kids = u64(__reduce_or_sync(0xffffffffu, uint32_t(kids >> 32))) << 32 | __reduce_or_sync(0xffffffffu, uint32_t(kids));
     int go = -1;
-    double used = 0., mass = 1.;
-    const double norm = unit / double(total);                // weight -> probability
-    const double kUnit = 1152921504606846976.;               // 2^60
-    const float* q = p.q != nullptr ? p.q + node * p.V : nullptr;
+    u64 all = total;
+    bool rest = false;
     if (q != nullptr) {
       for (u64 left = kids; left != 0 && go < 0; left &= left - 1) {
         const int j = __ffsll((long long)left) - 1, t = p.tokens[first + j];
         if (t < 0 || t >= p.V) continue;
-        const double px = weight(at(t), t) * norm, qx = double(q[t]);
+        const double w = raw(logit_at<kBf16>(p, node, t), t);
+        const double px = kept(w, t) ? w * norm : 0., qx = double(q[t]);
         if (double(p.accept[first + j]) * qx * mass < fmax(px - used * qx, 0.)) {
           go = j;
         } else {
           used += mass;
-          mine = 0;
-          for (int v = tid; v < size; v += VD_THREADS)
-            mine += __double2ull_rn(fmax(weight(xs[v], lo + v) * norm - used * double(q[lo + v]), 0.) * kUnit);
-          mass = double(row_sum(mine, nullptr)) / kUnit;
+          rest = true;
+          all = sum_up(true);
+          mass = double(all) / kRest;
         }
+      }
+      if (go < 0 && rest && all == 0) {                      // nothing left: p itself
+        rest = false;
+        all = sum_up(false);
       }
     }
-    int token = -1;
-    if (go < 0) {
-      // Where the number falls, in the order of the tokens: the segment of 128, then the token.
-      const bool rest = q != nullptr && used > 0. && mass > 0.;
-      auto share = [&](int j) {                              // j: place in the slice
-        if (j >= size) return u64(0);
-        const double w = weight(xs[j], lo + j);
-        return rest ? u64(__double2ull_rn(fmax(w * norm - used * double(q[lo + j]), 0.) * kUnit)) : fixed(w);
-      };
-      mine = 0;
-      for (int s = warp; s < segs; s += VD_WARPS) {
-        u64 v = 0;
-#pragma unroll
-        for (int e = 0; e < VD_SEG / 32; ++e) v += share(s * VD_SEG + lane * (VD_SEG / 32) + e);
-        v = warp_sum(v);
-        if (lane == 0) sh.seg[s] = v;
-        mine += lane == 0 ? v : 0;
+    if (go >= 0) {
+      if (rank == 0 && tid == 0) {
+        p.choice[node] = go;
+        p.drawn[node] = -1;
       }
-      u64 before;
-      const u64 all = row_sum(mine, &before);
-      const u64 target = min(part_of(p.u[node], all), all - 1);
-      const u64 own = sh.part[phase ^ 1][0];
-      if (target >= before && target < before + own && warp == 0) {
-        u64 sum = before;
-        int s = 0;
-        for (int s0 = 0; s0 < segs; s0 += 32) {              // 32 segments at a time
-          u64 v = s0 + lane < segs ? sh.seg[s0 + lane] : 0;
-#pragma unroll
-          for (int o = 1; o < 32; o <<= 1) {
-            const u64 x = __shfl_up_sync(0xffffffffu, v, o);
-            if (lane >= o) v += x;
-          }
-          const uint32_t over = __ballot_sync(0xffffffffu, sum + v > target);
-          if (over != 0) {
-            const int l = __ffs(over) - 1;
-            s = s0 + l;
-            const u64 x = __shfl_sync(0xffffffffu, v, max(l - 1, 0));
-            sum += l > 0 ? x : 0;
-            break;
-          }
-          sum += __shfl_sync(0xffffffffu, v, 31);
+      continue;
+    }
+    // Where the number falls, in the order of the tokens: the CTA, the segment, the token.
+    const u64 target = min(part_of(p.u[node], all), all - 1), own = sh.part[phase ^ 1];
+    if (target >= before && target < before + own && warp == 0) {
+      u64 sum = before;
+      int s = 0;
+      for (int s0 = 0; s0 < segs; s0 += 32) {
+        const u64 v = warp_scan(s0 + lane < segs ? sh.seg[s0 + lane] : 0, lane);
+        const uint32_t over = __ballot_sync(0xffffffffu, sum + v > target);
+        if (over != 0) {
+          const int l = __ffs(over) - 1;
+          s = s0 + l;
+          const u64 x = __shfl_sync(0xffffffffu, v, max(l - 1, 0));
+          sum += l > 0 ? x : 0;
+          break;
         }
-        u64 v[VD_SEG / 32], here = 0;
-#pragma unroll
-        for (int e = 0; e < VD_SEG / 32; ++e) here += v[e] = share(s * VD_SEG + lane * (VD_SEG / 32) + e);
-        u64 upto = here;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-          const u64 x = __shfl_up_sync(0xffffffffu, upto, o);
-          if (lane >= o) upto += x;
-        }
-        const uint32_t over = __ballot_sync(0xffffffffu, sum + upto > target);
-        if (lane == __ffs(over) - 1) {
-          u64 c = sum + upto - here;
-          int e = 0;
-          while (e < VD_SEG / 32 - 1 && c + v[e] <= target) c += v[e++];
-          token = lo + s * VD_SEG + lane * (VD_SEG / 32) + e;
-          if (q == nullptr)
-            for (u64 left = kids; left != 0 && go < 0; left &= left - 1) {
-              const int j = __ffsll((long long)left) - 1;
-              if (p.tokens[first + j] == token) go = j;
-            }
-          p.choice[node] = go;
-          p.drawn[node] = token;
-        }
+        sum += __shfl_sync(0xffffffffu, v, 31);
       }
-    } else if (rank == 0 && tid == 0) {
-      p.choice[node] = go;
-      p.drawn[node] = -1;
+      u64 v[4], here = 0;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) here += v[e] = share(s, e, rest);
+      const u64 upto = warp_scan(here, lane);
+      const uint32_t over = __ballot_sync(0xffffffffu, sum + upto > target);
+      if (lane == __ffs(over) - 1) {
+        u64 c = sum + upto - here;
+        int e = 0;
+#pragma unroll
+        for (int x = 0; x < 3; ++x)
+          if (e == x && c + v[x] <= target) {
+            c += v[x];
+            ++e;
+          }
+        const int token = lo + s * VD_SEG + 4 * lane + e;
+        if (q == nullptr)
+          for (u64 left = kids; left != 0 && go < 0; left &= left - 1) {
+            const int j = __ffsll((long long)left) - 1;
+            if (p.tokens[first + j] == token) go = j;
+          }
+        p.choice[node] = go;
+        p.drawn[node] = token;
+      }
     }
   }
-  cluster.sync();                                            // peers read this CTA's sums until here
+  if (cs > 1) cluster.sync();                                // peers read this CTA's numbers until here
 }
 
 struct WalkParams {
@@ -389,19 +613,22 @@ B200_API int b200_verify_drafts(const void* logits, const void* q, const void* t
     p.top = static_cast<u64>(std::ldexp(std::frexp(top, &e), 53));
     p.top_shift = 53 - e;
   }
+  const double missing = 1. - top, tail = missing > 1e-6 ? 0.9 * missing / V : 0.;
+  p.tail = 0;
+  memcpy(&p.tail, &tail, 8);
+  p.wide = V % 4 == 0 && (reinterpret_cast<uintptr_t>(logits) & (is_bf16 ? 7 : 15)) == 0;
   constexpr int kMostSlice = VD_MAX_SEGS * VD_SEG;
   int cs = 1;
-  while (cs < VD_MAX_CLUSTER && (long long)cs * kMostSlice < V) cs *= 2;
+  while (cs < VD_MAX_CLUSTER && (cs * 8192LL < V || cs * p.rows * 2 <= num_sms())) cs *= 2;
   if ((long long)cs * kMostSlice < V) return static_cast<int>(cudaErrorInvalidValue);
   p.slice = ((V + cs - 1) / cs + VD_SEG - 1) / VD_SEG * VD_SEG;
-  const int smem = int((sizeof(VerifyShared) + 15) / 16 * 16) + p.slice * 4;
+  const int smem = kVerifyShared + p.slice * 8;
   static std::atomic<bool> allowed[2][64];
   const auto kern = is_bf16 ? verify_rows_kernel<true> : verify_rows_kernel<false>;
   int dev = 0;
   B200_CHECK(cudaGetDevice(&dev));
   if (dev < 0 || dev >= 64 || !allowed[is_bf16 != 0][dev].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                               int((sizeof(VerifyShared) + 15) / 16 * 16) + kMostSlice * 4);
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kVerifyShared + kMostSlice * 8);
     if (e != cudaSuccess) {
       cudaGetLastError();
       return static_cast<int>(e);
