@@ -13,6 +13,7 @@
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
+#include <algorithm>
 #include <atomic>
 #include <cmath>
 #include <cstring>
@@ -24,8 +25,8 @@ namespace cg = cooperative_groups;
 
 typedef unsigned long long u64;
 
-constexpr int VD_THREADS = 512, VD_WARPS = VD_THREADS / 32, VD_SEG = 128, VD_MAX_SEGS = 195, VD_MAX_NODES = 64, VD_MAX_CLUSTER = 8;
-constexpr int VD_BINS = 2048, VD_LIST = 512;      // bins of masses; tokens that are put in order one by one
+constexpr int VD_THREADS = 512, VD_WARPS = VD_THREADS / 32, VD_SEG = 128, VD_MAX_SEGS = 376, VD_MAX_NODES = 64, VD_MAX_CLUSTER = 8;
+constexpr int VD_BINS = 2048, VD_COARSE = VD_BINS / 32, VD_LIST = 512;      // bins of masses; tokens that are put in order one by one
 
 struct VerifyParams {
   const void* logits;        // [B, n, V], fp32 or bf16
@@ -39,44 +40,43 @@ struct VerifyParams {
   long long rows;
   int n, V, slice;
   double inv_temp;           // 0: the largest logit
+  float reach;               // 699 temperatures
   u64 top;                   // the nucleus' mass is top 2^-top_shift; 0: everything
   int top_shift;
   u64 tail;                  // weights (as bits) below it cannot be where the nucleus ends
+  int shift;                 // bits of a weight that the first histogram does not look at
+  int lazy;                  // more nodes than clusters: nodes that are out of question are passed over
   int wide;                  // logits [node] start where four can be loaded at once
 };
 
 struct VerifyShared {
-  u64 warp[VD_WARPS];
+  u64 warp[32];
   u64 part[2];               // what this CTA adds to a sum over the row, two in turn
   u64 seg[VD_MAX_SEGS + 1];
   u64 above;                 // of the nucleus' search: mass above the bin, and the bin
   int bin, listed;
+  int off[2];                // whether the node is passed over, in turn: peers may still read the one before
   u64 list_w[VD_LIST];
   int list_i[VD_LIST];
   u64 all_w[VD_LIST];
   int all_i[VD_LIST];
   u64 cut_w;
   int cut_i;
+  u64 coarse[VD_COARSE];     // sums of 32 bins
   u64 bins[VD_BINS];
 };
+constexpr u64 kMostWeight = 0x3ff0000000000100ull;      // bits of 1 + 2^-44
+enum : int { kUnknown = -2 };          // a node that is not decided yet
 constexpr int kVerifyShared = int((sizeof(VerifyShared) + 15) / 16 * 16);
 
 // What a logit counts as: NaN as -infinity, +infinity as the largest number.
 __device__ __forceinline__ float tidy(float x) { return fminf(fmaxf(x, -CUDART_INF_F), 3.402823466e38f); }
-// fp32 -> fp64 by moving bits: the conversion runs at an eighth of the rate. Exact but for 0 and numbers below 2^-126, which come out
-// as some number below 2^-126, and infinity, which is 2^128.
-__device__ __forceinline__ double wide_of(float x) {
-  const uint32_t u = __float_as_uint(x);
-  return __hiloint2double(int((u & 0x80000000u) | (((u & 0x7fffffffu) >> 3) + 0x38000000u)), int(u << 29));
-}
 // e^x for x <= 0 by Tang's table-driven method (ACM TOMS 15, 1989): x = (32 k + i) ln2 / 32 + r, |r| <= ln2 / 64, e^x = 2^k 2^(i / 32)
-// e^r, e^r by its Taylor sum to r^5. `scaled` is x 32 / ln2. Off by at most 3e-13 (the sum's rest 2e-15, the argument's rounding the
-// rest), 0 below e^-700. The table lies in the lanes of a warp, which all take part.
-__device__ __forceinline__ double exp_of(double x, double scaled, double power) {
-  const double big = 6755399441055744.;                      // 1.5 2^52: the sum's last place is 1
-  const double t = scaled + big;
+// e^r, e^r by its Taylor sum to r^5. `t` is x 32 / ln2 + 1.5 2^52, whose last place is 1. Off by at most 3e-13 (the sum's rest 2e-15, the
+// argument's rounding the rest); below e^-693 what comes out is at most that. The table lies in the lanes of a warp, which all take part.
+__device__ __forceinline__ double exp_of(double x, double t, double power) {
   const int n = __double2loint(t);
-  const double r = fma(big - t, 0.021660849392498290, x);
+  const double r = fma(6755399441055744. - t, 0.021660849392498290, x);
   double p = fma(r, 1. / 120, 1. / 24);
   p = fma(p, r, 1. / 6);
   p = fma(p, r, .5);
@@ -84,7 +84,7 @@ __device__ __forceinline__ double exp_of(double x, double scaled, double power) 
   const int i = n & 31;
   const double T = __hiloint2double(__shfl_sync(0xffffffffu, __double2hiint(power), i), __shfl_sync(0xffffffffu, __double2loint(power), i));
   const double y = fma(T, p, T);
-  return x < -700. ? 0. : __hiloint2double(__double2hiint(y) + (n >> 5) * (1 << 20), __double2loint(y));
+  return __hiloint2double(__double2hiint(y) + (max(n, -32000) >> 5) * (1 << 20), __double2loint(y));
 }
 
 // x * total for x = m 2^-k in [0, 1], rounded down or up: exact, so that masses that are equal are so here.
@@ -119,6 +119,16 @@ __device__ __forceinline__ u64 warp_scan(u64 v, int lane) {
   return v;
 }
 
+// The same over the first eight lanes.
+__device__ __forceinline__ u64 warp_scan8(u64 v, int lane) {
+#pragma unroll
+  for (int o = 1; o < VD_MAX_CLUSTER; o <<= 1) {
+    const u64 x = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += x;
+  }
+  return v;
+}
+
 template <bool kBf16>
 __device__ __forceinline__ float logit_at(const VerifyParams& p, long long node, int j) {
   const long long at = node * p.V + j;
@@ -137,15 +147,15 @@ __device__ __forceinline__ float4 logits_at(const VerifyParams& p, long long nod
 
 // Grid (cluster, nodes), cluster (size, 1, 1).
 //
-// A CTA's slice of the row goes through shared memory once, in segments of 128 that belong to one warp throughout (four neighbouring
-// tokens to a lane; token e of lane l stands at 32 e + l, so that eight-byte accesses meet no bank twice): the logits, in their place the
-// weights, and from then on passes over the weights only. The nucleus' end is looked for in a histogram of masses over the weights' bits
-// (an order of positive numbers), in finer ones while too many tokens share the bin, and then token by token.
+// A CTA's slice of the row goes into shared memory once, in segments of 128 that belong to one warp throughout, four neighbouring tokens
+// to a lane. One pass makes all weights and their sum; where the row's weights are needed again they are made again, of the segments alone
+// that hold a logit in question. The nucleus' end is looked for in a histogram of masses over the weights' bits (an order of positive
+// numbers), in finer ones while too many tokens share the bin, and then token by token.
 template <bool kBf16>
 __global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const VerifyParams p) {
   extern __shared__ __align__(16) uint8_t smem[];
   VerifyShared& sh = *reinterpret_cast<VerifyShared*>(smem);
-  double* ws = reinterpret_cast<double*>(smem + kVerifyShared);
+  float* xs = reinterpret_cast<float*>(smem + kVerifyShared);
   cg::cluster_group cluster = cg::this_cluster();
   const int cs = gridDim.x, rank = blockIdx.x, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int lo = min(rank * p.slice, p.V), size = min(p.slice, p.V - lo);
@@ -156,7 +166,7 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const Verify
   const double power = exp2(double(lane) / 32.);
   pdl_wait();
   pdl_trigger();
-  int phase = 0;
+  int phase = 0, parity = 0;
   auto meet = [&] {
     if (cs > 1) cluster.sync();
     else __syncthreads();
@@ -171,15 +181,12 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const Verify
       if (lane == 0) sh.part[phase] = v;
     }
     meet();
-    u64 all = 0, ahead = 0;
-    for (int c = 0; c < cs; ++c) {
-      const u64 x = *cluster.map_shared_rank(&sh.part[phase], c);
-      if (c < rank) ahead += x;
-      all += x;
-    }
+    // a lane for each CTA: one after the other the reads would be eight times as long on their way
+    const u64 x = lane < cs ? *cluster.map_shared_rank(&sh.part[phase], lane) : 0;
     phase ^= 1;
-    if (before != nullptr) *before = ahead;
-    return all;
+    const u64 upto = warp_scan8(x, lane);
+    if (before != nullptr) *before = __shfl_sync(0xffffffffu, upto - x, rank);
+    return __shfl_sync(0xffffffffu, upto, VD_MAX_CLUSTER - 1);
   };
   auto row_max = [&](uint32_t v) {
     v = __reduce_max_sync(0xffffffffu, v);
@@ -190,20 +197,70 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const Verify
       if (lane == 0) sh.part[phase] = v;
     }
     meet();
-    uint32_t all = 0;
-    for (int c = 0; c < cs; ++c) all = max(all, uint32_t(*cluster.map_shared_rank(&sh.part[phase], c)));
+    const uint32_t x = lane < cs ? uint32_t(*cluster.map_shared_rank(&sh.part[phase], lane)) : 0u;
     phase ^= 1;
-    return all;
+    return __reduce_max_sync(0xffffffffu, x);
   };
   // An integer number of units, rounded to nearest: the last bits of a sum with 2^52.
   auto fixed = [](double w, double u) { return u64(__double_as_longlong(fma(w, u, 4503599627370496.))) - 0x4330000000000000ull; };
 
-  for (long long node = blockIdx.y; node < p.rows; node += gridDim.y) {
-    const int i = int(node % p.n);
-    const long long first = node - i;                        // the sequence's node 0
+  // Node 0 of all sequences, node 1 of all, ...: a parent is decided before its children begin, if they begin in a later round.
+  const long long B = p.rows / p.n;
+  for (long long turn = blockIdx.y; turn < p.rows; turn += gridDim.y) {
+    const int i = int(turn / B);
+    const long long first = turn % B * p.n, node = first + i;          // the sequence's node 0, this one
     const int up = i == 0 ? -1 : p.parents[node];
     if (i > 0 && (up < 0 || up >= i)) continue;              // not there (the same for the whole cluster)
+    if (p.lazy) {                                            // a node that the text has not come to is not looked at: what one CTA sees
+      __syncthreads();
+      if (rank == 0 && warp == 0) {
+        int above[2], chosen[2], off = 0;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int j = 32 * e + lane;
+          above[e] = j < p.n ? p.parents[first + j] : -1;
+          chosen[e] = j < p.n ? *const_cast<volatile int*>(p.choice + first + j) : kUnknown;
+        }
+        for (int j = i; j > 0 && !off;) {                    // up to the root: each on the way is its parent's choice, or nobody knows
+          const int a = j < 32 ? __shfl_sync(0xffffffffu, above[0], j) : __shfl_sync(0xffffffffu, above[1], j - 32);
+          if (a < 0 || a >= j) {                             // below a node that is not there
+            off = 1;
+          } else {
+            const int c = a < 32 ? __shfl_sync(0xffffffffu, chosen[0], a) : __shfl_sync(0xffffffffu, chosen[1], a - 32);
+            off = c != kUnknown && c != j;
+          }
+          j = a;
+        }
+        if (lane < cs) *cluster.map_shared_rank(&sh.off[parity], lane) = off;
+        if (off && lane == 0) p.choice[node] = -1;
+      }
+      meet();
+      parity ^= 1;
+      if (sh.off[parity ^ 1]) continue;
+    }
     __syncthreads();
+    // Which drafts are this node's children, and what the end will want to know of them: a lane holds drafts `lane` and 32 + lane.
+    int tok[2];
+    float child_x[2] = {0.f, 0.f}, child_q[2] = {0.f, 0.f}, child_a[2] = {0.f, 0.f};
+    uint32_t kid[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int j = 32 * e + lane;
+      const bool mine = j > i && j < p.n && p.parents[first + j] == i;
+      tok[e] = mine ? p.tokens[first + j] : -1;
+      kid[e] = __ballot_sync(0xffffffffu, mine && tok[e] >= 0 && tok[e] < p.V);
+      if (p.q != nullptr && (kid[e] >> lane & 1)) {
+        child_x[e] = logit_at<kBf16>(p, node, tok[e]);
+        child_q[e] = p.q[node * p.V + tok[e]];
+        child_a[e] = p.accept[first + j];
+      }
+    }
+    const u64 kids = u64(kid[1]) << 32 | kid[0];
+    const float drawn_at = p.u[node];
+    auto of = [&](const auto (&x)[2], int j) {
+      const auto a = __shfl_sync(0xffffffffu, x[0], j & 31), c = __shfl_sync(0xffffffffu, x[1], j & 31);
+      return j < 32 ? a : c;
+    };
     float top = -CUDART_INF_F;
     for (int s0 = warp; s0 < segs; s0 += 4 * VD_WARPS) {     // four segments on their way at a time
       float4 x[4];
@@ -222,13 +279,9 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const Verify
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         if (s0 + c * VD_WARPS >= segs) break;
-        float* to = reinterpret_cast<float*>(ws + (s0 + c * VD_WARPS) * VD_SEG + lane);
-        const float y[4] = {tidy(x[c].x), tidy(x[c].y), tidy(x[c].z), tidy(x[c].w)};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          to[64 * e] = y[e];
-          top = fmaxf(top, y[e]);
-        }
+        const float4 y = make_float4(tidy(x[c].x), tidy(x[c].y), tidy(x[c].z), tidy(x[c].w));
+        reinterpret_cast<float4*>(xs)[(s0 + c * VD_WARPS) * 32 + lane] = y;
+        top = fmaxf(fmaxf(fmaxf(top, y.x), fmaxf(y.y, y.z)), y.w);
       }
     }
     // fp32 numbers in the order of unsigned ones
@@ -244,41 +297,55 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const Verify
     int arg = -1;                                            // temperature 0: the first of the largest
     if (p.inv_temp == 0.) {
       uint32_t lowest = 0;
-      for (int s = warp; s < segs; s += VD_WARPS)
-#pragma unroll
-        for (int e = 3; e >= 0; --e)
-          if (*reinterpret_cast<const float*>(ws + s * VD_SEG + 32 * e + lane) == largest) lowest = max(lowest, ~uint32_t(lo + s * VD_SEG + 4 * lane + e));
+      for (int j = tid; j < size; j += VD_THREADS)
+        if (xs[j] == largest) lowest = max(lowest, ~uint32_t(lo + j));
       arg = int(~row_max(lowest));
     }
-    const double zero = wide_of(largest), per32 = p.inv_temp * 46.166241308446828;       // 32 / ln2
-    auto raw = [&](float x, int j) {                         // weight of token j, 1 for the largest; whole warps
+    // The weight of token j, 1 for the largest; whole warps. What is more than 699 temperatures below has none (in fp32: up to twice that).
+    const double per32 = p.inv_temp * 46.166241308446828;                               // 32 / ln2
+    const float none = largest - p.reach;
+    auto raw = [&](float x, int j) {
       if (p.inv_temp == 0.) return j == arg ? 1. : 0.;
-      const double d = wide_of(x) - zero;
-      return exp_of(d * p.inv_temp, d * per32, power);
+      const double d = double(x < none ? largest : x) - double(largest);
+      const double w = exp_of(d * p.inv_temp, fma(d, per32, 6755399441055744.), power);
+      return x < none ? 0. : w;
     };
     const bool nucleus = p.top != 0 && p.inv_temp != 0.;
+    // Bits of the four weights of a lane in segment s; false (and none) if no logit of the segment is `from` or more.
+    auto weights = [&](int s, float from, u64 (&k)[4]) {
+      const float4 x = reinterpret_cast<const float4*>(xs)[s * 32 + lane];
+      const float y[4] = {x.x, x.y, x.z, x.w};
+      if (!__any_sync(0xffffffffu, fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])) >= from)) return false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) k[e] = u64(__double_as_longlong(raw(y[e], lo + s * VD_SEG + 4 * lane + e)));
+      return true;
+    };
+    // A logit that is at most that of a weight: from the logarithm in fp32, 2^-20 of what goes into it to spare.
+    auto logit_of = [&](u64 k) {
+      if (k == 0 || p.inv_temp == 0.) return -CUDART_INF_F;
+      const float d = logf(float(__longlong_as_double((long long)k))) / float(p.inv_temp);
+      return largest + d - 9.5e-7f * (fabsf(largest) + fabsf(d) + 1.f / float(p.inv_temp));
+    };
     u64 cut_w = 0;                                           // weights below it are cut off, and those equal to it behind token cut_i
     int cut_i = 0x7fffffff;
-    u64 khi = 0x3ff0000000000001ull, above = 0;              // the end lies in [klo, khi) (bits of weights), and this much above it
+    u64 khi = kMostWeight + 1, above = 0;              // the end lies in [klo, khi) (bits of weights), and this much above it
     u64 klo = p.tail;
-    int shift = 0;
+    int shift = p.shift;
     if (nucleus) {
-      while ((khi - klo - 1) >> shift >= VD_BINS) ++shift;
       for (int t = tid; t < VD_BINS; t += VD_THREADS) sh.bins[t] = 0;
       __syncthreads();
     }
-    // Weights in the logits' place; sums of the segments, or the first histogram.
+    // All weights: sums of the segments, or the first histogram.
     u64 mine = 0;
     for (int s = warp; s < segs; s += VD_WARPS) {
-      u64 v = 0;
+      u64 k[4], v = 0;
+      if (weights(s, -CUDART_INF_F, k)) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        double* at = ws + s * VD_SEG + 32 * e + lane;
-        const double w = raw(*reinterpret_cast<const float*>(at), lo + s * VD_SEG + 4 * lane + e);
-        *at = w;
-        const u64 f = fixed(w, unit), k = u64(__double_as_longlong(w));
-        v += f;
-        if (nucleus && k >= klo) atomicAdd(&sh.bins[(khi - 1 - k) >> shift], f);
+        for (int e = 0; e < 4; ++e) {
+          const u64 f = fixed(__longlong_as_double((long long)k[e]), unit);
+          v += f;
+          if (nucleus && k[e] >= klo) atomicAdd(&sh.bins[(khi - 1 - k[e]) >> shift], f);
+        }
       }
       mine += v;
       if (!nucleus) {
@@ -286,39 +353,50 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const Verify
         if (lane == 0) sh.seg[s] = v;
       }
     }
+    auto coarse = [&] {                                      // all threads, the bins complete
+      __syncthreads();
+      for (int t = warp; t < VD_COARSE; t += VD_WARPS) {
+        const u64 v = warp_sum(sh.bins[32 * t + lane]);
+        if (lane == 0) sh.coarse[t] = v;
+      }
+    };
+    if (nucleus) coarse();
     u64 before, total = row_sum(mine, &before);
     if (nucleus) {
       const u64 want = part_of(p.top, p.top_shift, total, true);
       while (true) {
-        // The bin in which the masses of all CTAs reach `want`: four bins to a thread.
-        u64 v[VD_BINS / VD_THREADS], sum = 0;
+        // The bin in which the masses of all CTAs reach `want`: among 64 sums of 32, then among those 32.
+        if (warp == 0) {
+          auto of_all = [&](const u64* at) {
+            u64 x[VD_MAX_CLUSTER], v = 0;
 #pragma unroll
-        for (int e = 0; e < VD_BINS / VD_THREADS; ++e) v[e] = 0;
-        for (int c = 0; c < cs; ++c) {
-          const ulonglong2* from = reinterpret_cast<const ulonglong2*>(cluster.map_shared_rank(&sh.bins[tid * (VD_BINS / VD_THREADS)], c));
+            for (int c = 0; c < VD_MAX_CLUSTER; ++c) x[c] = c < cs ? *cluster.map_shared_rank(at, c) : 0;
 #pragma unroll
-          for (int e = 0; e < VD_BINS / VD_THREADS; e += 2) {
-            const ulonglong2 x = from[e / 2];
-            v[e] += x.x;
-            v[e + 1] += x.y;
+            for (int c = 0; c < VD_MAX_CLUSTER; ++c) v += x[c];
+            return v;
+          };
+          int bin = -1;
+          u64 at = above;
+          const u64 a = of_all(&sh.coarse[2 * lane]), c = of_all(&sh.coarse[2 * lane + 1]), scan = warp_scan(a + c, lane);
+          const uint32_t over = __ballot_sync(0xffffffffu, at + scan >= want);
+          if (over != 0) {
+            const int l = __ffs(over) - 1;
+            at += __shfl_sync(0xffffffffu, scan - a - c, l);
+            const u64 low = __shfl_sync(0xffffffffu, a, l);
+            const bool second = at + low < want;
+            at += second ? low : 0;
+            const int block = 2 * l + second;
+            const u64 v = of_all(&sh.bins[32 * block + lane]), upto = warp_scan(v, lane);
+            const uint32_t fine = __ballot_sync(0xffffffffu, at + upto >= want);
+            const int f = fine != 0 ? __ffs(fine) - 1 : 31;
+            at += __shfl_sync(0xffffffffu, upto - v, f);
+            bin = 32 * block + f;
           }
-        }
-#pragma unroll
-        for (int e = 0; e < VD_BINS / VD_THREADS; ++e) sum += v[e];
-        const u64 scan = warp_scan(sum, lane);
-        if (lane == 31) sh.warp[warp] = scan;
-        if (tid == 0) {
-          sh.bin = -1;
-          sh.listed = 0;
-        }
-        __syncthreads();
-        u64 at = above + scan - sum;
-        for (int w = 0; w < warp; ++w) at += sh.warp[w];
-        if (at < want && at + sum >= want) {
-          int e = 0;
-          while (e < VD_BINS / VD_THREADS - 1 && at + v[e] < want) at += v[e++];
-          sh.bin = tid * (VD_BINS / VD_THREADS) + e;
-          sh.above = at;
+          if (lane == 0) {
+            sh.bin = bin;
+            sh.above = at;
+            sh.listed = 0;
+          }
         }
         __syncthreads();
         if (sh.bin < 0) break;                               // (cannot be: everything is kept)
@@ -326,30 +404,37 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const Verify
         khi -= u64(sh.bin) << shift;
         klo = khi - klo > 1ull << shift ? khi - (1ull << shift) : klo;
         // Its tokens, if they are few.
-        for (int s = warp; s < segs; s += VD_WARPS)
+        const float from = logit_of(klo);
+        for (int s = warp; s < segs; s += VD_WARPS) {
+          u64 k[4];
+          if (!weights(s, from, k)) continue;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const u64 k = u64(__double_as_longlong(ws[s * VD_SEG + 32 * e + lane]));
-            if (k >= klo && k < khi && s * VD_SEG + 4 * lane + e < size) {
+          for (int e = 0; e < 4; ++e)
+            if (k[e] >= klo && k[e] < khi && k[e] != 0) {
               const int n = atomicAdd(&sh.listed, 1);
               if (n < VD_LIST) {
-                sh.list_w[n] = k;
+                sh.list_w[n] = k[e];
                 sh.list_i[n] = lo + s * VD_SEG + 4 * lane + e;
               }
             }
-          }
+        }
         meet();
-        int all = 0;
-        for (int c = 0; c < cs; ++c) all = min(all + *cluster.map_shared_rank(&sh.listed, c), 1 << 24);
+        const int found = lane < cs ? min(*cluster.map_shared_rank(&sh.listed, lane), 1 << 24) : 0;
+        const int upto = int(warp_scan8(u64(found), lane));
+        const int all = __shfl_sync(0xffffffffu, upto, VD_MAX_CLUSTER - 1);
         if (all <= VD_LIST) {
-          int n = 0;
-          for (int c = 0; c < cs; ++c) {
-            const int m = *cluster.map_shared_rank(&sh.listed, c);
-            if (tid < m) {
-              sh.all_w[n + tid] = *cluster.map_shared_rank(&sh.list_w[tid], c);
-              sh.all_i[n + tid] = *cluster.map_shared_rank(&sh.list_i[tid], c);
+          int c = 0, at0 = 0;                                // token `tid` of all: whose it is, and how many stand before that CTA's
+#pragma unroll
+          for (int o = 0; o < VD_MAX_CLUSTER - 1; ++o) {
+            const int n = __shfl_sync(0xffffffffu, upto, o);
+            if (tid >= n && o + 1 < cs) {
+              c = o + 1;
+              at0 = n;
             }
-            n += m;
+          }
+          if (tid < all) {
+            sh.all_w[tid] = *cluster.map_shared_rank(&sh.list_w[tid - at0], c);
+            sh.all_i[tid] = *cluster.map_shared_rank(&sh.list_i[tid - at0], c);
           }
           __syncthreads();
           if (tid < all) {
@@ -376,9 +461,8 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const Verify
           u64 need = each == 0 || want <= above + each ? 1 : (want - above + each - 1) / each;
           mine = 0;
           for (int s = warp; s < segs; s += VD_WARPS) {
-            u64 n = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) n += u64(__double_as_longlong(ws[s * VD_SEG + 32 * e + lane])) == klo && s * VD_SEG + 4 * lane + e < size;
+            u64 k[4], n = 0;
+            if (weights(s, from, k)) n = (k[0] == klo) + (k[1] == klo) + (k[2] == klo) + (k[3] == klo);
             n = warp_sum(n);
             if (lane == 0) sh.seg[s] = n;
             mine += lane == 0 ? n : 0;
@@ -391,15 +475,13 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const Verify
           if (warp == 0) {                                   // the owner of the last one: its segment, then its place
             u64 sum = before;
             for (int s = 0; s < segs; ++s) {
-              if (sum < need && sum + sh.seg[s] >= need) {
-                u64 n = 0;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) n += u64(__double_as_longlong(ws[s * VD_SEG + 32 * e + lane])) == klo && s * VD_SEG + 4 * lane + e < size;
+              u64 k[4];
+              if (sum < need && sum + sh.seg[s] >= need && weights(s, from, k)) {
+                const u64 n = (k[0] == klo) + (k[1] == klo) + (k[2] == klo) + (k[3] == klo);
                 u64 at = sum + warp_scan(n, lane) - n;
-                if (at < need && at + n >= need)
-                  for (int e = 0; e < 4; ++e)
-                    if (u64(__double_as_longlong(ws[s * VD_SEG + 32 * e + lane])) == klo && s * VD_SEG + 4 * lane + e < size && ++at == need)
-                      sh.cut_i = lo + s * VD_SEG + 4 * lane + e;
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (k[e] == klo && ++at == need) sh.cut_i = lo + s * VD_SEG + 4 * lane + e;
               }
               sum += sh.seg[s];
             }
@@ -412,13 +494,14 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const Verify
         shift = shift > 11 ? shift - 11 : 0;
         for (int t = tid; t < VD_BINS; t += VD_THREADS) sh.bins[t] = 0;
         __syncthreads();
-        for (int s = warp; s < segs; s += VD_WARPS)
+        for (int s = warp; s < segs; s += VD_WARPS) {
+          u64 k[4];
+          if (!weights(s, from, k)) continue;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const double w = ws[s * VD_SEG + 32 * e + lane];
-            const u64 k = u64(__double_as_longlong(w));
-            if (k >= klo && k < khi) atomicAdd(&sh.bins[(khi - 1 - k) >> shift], fixed(w, unit));
-          }
+          for (int e = 0; e < 4; ++e)
+            if (k[e] >= klo && k[e] < khi) atomicAdd(&sh.bins[(khi - 1 - k[e]) >> shift], fixed(__longlong_as_double((long long)k[e]), unit));
+        }
+        coarse();
         meet();
       }
     }
@@ -428,43 +511,42 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const Verify
       const u64 k = u64(__double_as_longlong(w));
       return k > cut_w || (k == cut_w && j <= cut_i);
     };
-    // Sums of the segments of w, or of max(p - used q, 0) in units of kRest.
-    auto share = [&](int s, int e, bool rest) {
-      const int j = s * VD_SEG + 4 * lane + e;
-      if (j >= size) return u64(0);
-      double w = ws[s * VD_SEG + 32 * e + lane];
-      if (!kept(w, lo + j)) w = 0.;
-      return rest ? (w > 0. ? fixed(fmax(w * norm - used * double(q[lo + j]), 0.), kRest) : 0) : fixed(w, unit);
+    // What a lane adds to the sum of segment s: of w, or of max(p - used q, 0) in units of kRest.
+    auto shares = [&](int s, bool rest, float from, u64 (&v)[4]) {
+      u64 k[4];
+      if (!weights(s, from, k)) return false;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int j = lo + s * VD_SEG + 4 * lane + e;
+        const double w = kept(__longlong_as_double((long long)k[e]), j) ? __longlong_as_double((long long)k[e]) : 0.;
+        v[e] = !rest ? fixed(w, unit) : w > 0. ? fixed(fmax(w * norm - used * double(q[j]), 0.), kRest) : 0;
+      }
+      return true;
     };
+    const float least = logit_of(cut_w);
     auto sum_up = [&](bool rest) {
       u64 sum = 0;
       for (int s = warp; s < segs; s += VD_WARPS) {
-        u64 v = 0;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) v += share(s, e, rest);
-        v = warp_sum(v);
+        u64 v[4], t = 0;
+        if (shares(s, rest, least, v)) t = warp_sum(v[0] + v[1] + v[2] + v[3]);
         if (lane == 0) {
-          sh.seg[s] = v;
-          sum += v;
+          sh.seg[s] = t;
+          sum += t;
         }
       }
       return row_sum(sum, &before);
     };
     if (nucleus) total = sum_up(false);
     norm = unit / double(total);                             // weight -> probability
-    u64 kids = 0;                                            // children, as bits
-    for (int j = lane; j < p.n; j += 32) kids |= u64(j > i && p.parents[first + j] == i) << j;
-    kids = u64(__reduce_or_sync(0xffffffffu, uint32_t(kids >> 32))) << 32 | __reduce_or_sync(0xffffffffu, uint32_t(kids));
     int go = -1;
     u64 all = total;
     bool rest = false;
     if (q != nullptr) {
       for (u64 left = kids; left != 0 && go < 0; left &= left - 1) {
-        const int j = __ffsll((long long)left) - 1, t = p.tokens[first + j];
-        if (t < 0 || t >= p.V) continue;
-        const double w = raw(logit_at<kBf16>(p, node, t), t);
-        const double px = kept(w, t) ? w * norm : 0., qx = double(q[t]);
-        if (double(p.accept[first + j]) * qx * mass < fmax(px - used * qx, 0.)) {
+        const int j = __ffsll((long long)left) - 1, t = of(tok, j);
+        const double w = raw(of(child_x, j), t);
+        const double px = kept(w, t) ? w * norm : 0., qx = double(of(child_q, j));
+        if (double(of(child_a, j)) * qx * mass < fmax(px - used * qx, 0.)) {
           go = j;
         } else {
           used += mass;
@@ -486,7 +568,7 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const Verify
       continue;
     }
     // Where the number falls, in the order of the tokens: the CTA, the segment, the token.
-    const u64 target = min(part_of(p.u[node], all), all - 1), own = sh.part[phase ^ 1];
+    const u64 target = min(part_of(drawn_at, all), all - 1), own = sh.part[phase ^ 1];
     if (target >= before && target < before + own && warp == 0) {
       u64 sum = before;
       int s = 0;
@@ -502,9 +584,9 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const Verify
         }
         sum += __shfl_sync(0xffffffffu, v, 31);
       }
-      u64 v[4], here = 0;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) here += v[e] = share(s, e, rest);
+      u64 v[4] = {0, 0, 0, 0};
+      shares(s, rest, least, v);
+      const u64 here = v[0] + v[1] + v[2] + v[3];
       const u64 upto = warp_scan(here, lane);
       const uint32_t over = __ballot_sync(0xffffffffu, sum + upto > target);
       if (lane == __ffs(over) - 1) {
@@ -516,18 +598,28 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const Verify
             c += v[x];
             ++e;
           }
-        const int token = lo + s * VD_SEG + 4 * lane + e;
-        if (q == nullptr)
-          for (u64 left = kids; left != 0 && go < 0; left &= left - 1) {
-            const int j = __ffsll((long long)left) - 1;
-            if (p.tokens[first + j] == token) go = j;
-          }
+        sum = u64(lo + s * VD_SEG + 4 * lane + e);
+      }
+      const int token = __shfl_sync(0xffffffffu, int(sum), __ffs(over) - 1);
+      if (q == nullptr) {                                    // the first child that holds it
+        const uint32_t a = __ballot_sync(0xffffffffu, tok[0] == token) & kid[0], c = __ballot_sync(0xffffffffu, tok[1] == token) & kid[1];
+        go = a != 0 ? __ffs(a) - 1 : c != 0 ? 31 + __ffs(c) : -1;
+      }
+      if (lane == 0) {
         p.choice[node] = go;
         p.drawn[node] = token;
       }
     }
   }
   if (cs > 1) cluster.sync();                                // peers read this CTA's numbers until here
+}
+
+// Nothing is decided yet.
+__global__ void __launch_bounds__(256) verify_begin_kernel(int* choice, long long rows) {
+  pdl_wait();
+  pdl_trigger();
+  const long long i = blockIdx.x * 256LL + threadIdx.x;
+  if (i < rows) choice[i] = kUnknown;
 }
 
 struct WalkParams {
@@ -606,6 +698,7 @@ B200_API int b200_verify_drafts(const void* logits, const void* q, const void* t
   p.rows = (long long)B * n;
   p.n = n; p.V = V;
   p.inv_temp = temp > 0. ? 1. / temp : 0.;
+  p.reach = float(std::min(699. * temp, 3e38));
   p.top = 0;
   p.top_shift = 0;
   if (top < 1.) {
@@ -616,27 +709,34 @@ B200_API int b200_verify_drafts(const void* logits, const void* q, const void* t
   const double missing = 1. - top, tail = missing > 1e-6 ? 0.9 * missing / V : 0.;
   p.tail = 0;
   memcpy(&p.tail, &tail, 8);
+  p.shift = 0;
+  while ((kMostWeight - p.tail) >> p.shift >= VD_BINS) ++p.shift;
   p.wide = V % 4 == 0 && (reinterpret_cast<uintptr_t>(logits) & (is_bf16 ? 7 : 15)) == 0;
   constexpr int kMostSlice = VD_MAX_SEGS * VD_SEG;
   int cs = 1;
-  while (cs < VD_MAX_CLUSTER && (cs * 8192LL < V || cs * p.rows * 2 <= num_sms())) cs *= 2;
+  while (cs < VD_MAX_CLUSTER && (cs * 16384LL < V || cs * p.rows * 2 <= num_sms())) cs *= 2;
   if ((long long)cs * kMostSlice < V) return static_cast<int>(cudaErrorInvalidValue);
   p.slice = ((V + cs - 1) / cs + VD_SEG - 1) / VD_SEG * VD_SEG;
-  const int smem = kVerifyShared + p.slice * 8;
+  const int smem = kVerifyShared + p.slice * 4;
   static std::atomic<bool> allowed[2][64];
   const auto kern = is_bf16 ? verify_rows_kernel<true> : verify_rows_kernel<false>;
+  std::atomic<bool>* known = allowed[is_bf16 != 0];
   int dev = 0;
   B200_CHECK(cudaGetDevice(&dev));
-  if (dev < 0 || dev >= 64 || !allowed[is_bf16 != 0][dev].load(std::memory_order_acquire)) {
-    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kVerifyShared + kMostSlice * 8);
+  if (dev < 0 || dev >= 64 || !known[dev].load(std::memory_order_acquire)) {
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kVerifyShared + kMostSlice * 4);
     if (e != cudaSuccess) {
       cudaGetLastError();
       return static_cast<int>(e);
     }
-    if (dev >= 0 && dev < 64) allowed[is_bf16 != 0][dev].store(true, std::memory_order_release);
+    if (dev >= 0 && dev < 64) known[dev].store(true, std::memory_order_release);
   }
-  const long long rows = p.rows < 65535 ? p.rows : 65535;
-  B200_CHECK(launch_pdl(kern, dim3(cs, unsigned(rows)), dim3(VD_THREADS), smem, st, cs, p));
+  // CTAs that stay: a cluster takes node after node.
+  const int per = std::min(4, std::max(1, 232448 / (smem + 1024)));
+  const long long most = std::max(1, num_sms() * per / cs);
+  p.lazy = p.rows > most && n > 1;
+  if (p.lazy) B200_CHECK(launch_pdl(verify_begin_kernel, dim3(unsigned((p.rows + 255) / 256)), dim3(256), 0, st, 0, p.choice, p.rows));
+  B200_CHECK(launch_pdl(kern, dim3(cs, unsigned(std::min(p.rows, most))), dim3(VD_THREADS), smem, st, cs, p));
   WalkParams w;
   w.choice = p.choice; w.drawn = p.drawn; w.tokens = p.tokens;
   w.out = static_cast<int*>(out);

@@ -17,7 +17,7 @@ from . import functional as F
 from . import native
 
 MOST_NODES = 64
-MOST_TOKENS = 8 * 195 * 128
+MOST_TOKENS = 8 * 376 * 128
 
 
 def verify_drafts(logits, tokens, parents, u, *, temp: float = 1.0, top: float = 1.0, draft_probs=None, accept=None):

@@ -30,7 +30,7 @@ def test_against_the_definition(dtype, temp, top, drawn):
               O.verify(x, tokens, parents, u, temp, top, q if drawn else None, accept))
 
 
-@pytest.mark.parametrize("V", [32000, 60001, 120000, 8 * 195 * 128])
+@pytest.mark.parametrize("V", [32000, 60001, 120000, 8 * 376 * 128])
 @pytest.mark.parametrize("top", [1.0, 0.9])
 @pytest.mark.parametrize("drawn", [False, True])
 def test_large_vocabularies(V, top, drawn):
