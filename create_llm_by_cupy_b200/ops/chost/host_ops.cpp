@@ -64,7 +64,8 @@ struct Api {
   int (*paged_append)(cptr, cptr, void*, void*, void*, void*, cptr, cptr, cptr, cptr, cptr, int, long long, long long, long long, int, int,
                       int, int, int, int, int, stream_t);
   int (*paged_read)(void*, void*, void*, void*, cptr, cptr, cptr, void*, void*, int, int, int, int, int, int, int, int, stream_t);
-  int (*paged_attn_append)(cptr, void*, void*, void*, void*, cptr, cptr, cptr, cptr, cptr, void*, int, long long, int, int, int, int, int,
+  long long (*paged_attn_workspace)(int, int, int, int, int, int);
+  int (*paged_attn_append)(cptr, void*, void*, void*, void*, cptr, cptr, cptr, cptr, cptr, void*, void*, int, long long, int, int, int, int, int,
                            int, int, int, float, float, stream_t);
   int (*verify_drafts)(cptr, cptr, cptr, cptr, cptr, cptr, void*, void*, void*, void*, int, int, int, int, double, double, stream_t);
 };
@@ -671,7 +672,8 @@ bool pool(PyObject* const* a, int dev, Pool* p) {
   if (p->log_page > 10) return false;
   if ((p->held != 0) != (ks != nullptr) || (ks != nullptr) != (vs != nullptr)) return false;
   for (const Tensor* s : {ks, vs})
-    if (s && (!on(*s, dev) || s->scalar_type() != at::kFloat || s->dim() != 3 || !s->is_contiguous() || s->sizes() != k->sizes().slice(0, 3)))
+    if (s && (!on(*s, dev) || s->scalar_type() != at::kFloat || s->dim() != 3 || !s->is_contiguous() || s->sizes() != k->sizes().slice(0, 3) ||
+              !aligned16(s->const_data_ptr())))
       return false;
   if (!on(*table, dev) || table->scalar_type() != at::kInt || table->dim() != 2 || !table->is_contiguous()) return false;
   p->B = table->size(0), p->width = table->size(1);
@@ -747,7 +749,7 @@ PyObject* paged_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   CHECK_NUMBERS
   Pool p;
   if (!x || !lens || !c || !s || !optional(a[13], &sl) || !tma_rows(*x, dev) || !pool(a + 1, dev, &p)) Py_RETURN_NONE;
-  if (QH <= 0 || KVH != p.KVH || QH % KVH != 0 || p.B > 65535 || int64_t(KVH) * ((QH / KVH + 7) / 8) > 65535 || x->size(0) != p.B ||
+  if (QH <= 0 || KVH != p.KVH || QH % KVH != 0 || p.B > 65535 || int64_t(KVH) * ((QH / KVH + 3) / 4) > 65535 || x->size(0) != p.B ||
       x->size(1) != (2 * int64_t(KVH) + QH) * p.D || (p.B > 1 && x->stride(0) <= 0))
     Py_RETURN_NONE;
   if (!int32_vector(*lens, p.B, dev) || !rotary(*c, *s, p.D, dev)) Py_RETURN_NONE;
@@ -755,10 +757,13 @@ PyObject* paged_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
     Py_RETURN_NONE;
   if (!score_numbers(&scale, cap, sl, p.D)) Py_RETURN_NONE;
   Tensor out = empty({p.B, QH, p.D}, *x, at::kBFloat16);
+  const long long bytes = api.paged_attn_workspace(int(p.B), QH, KVH, int(p.width), p.log_page, int(p.D));
+  OptTensor ws;
+  if (bytes > 0) ws = empty({bytes}, *x, at::kByte);
   if (launched([&] {
         return api.paged_attn_append(x->const_data_ptr(), p.k, p.v, p.ks, p.vs, p.table, lens->const_data_ptr(), c->const_data_ptr(),
-                                     s->const_data_ptr(), sl ? sl->const_data_ptr() : nullptr, out.mutable_data_ptr(), int(c->size(0)),
-                                     x->stride(0), int(p.B), int(p.width), int(p.pages), QH, KVH, p.log_page, int(p.D), p.held,
+                                     s->const_data_ptr(), sl ? sl->const_data_ptr() : nullptr, out.mutable_data_ptr(),
+                                     ws ? ws->mutable_data_ptr() : nullptr, int(c->size(0)), x->stride(0), int(p.B), int(p.width), int(p.pages), QH, KVH, p.log_page, int(p.D), p.held,
                                      float(scale), float(cap), stream(dev));
       }))
     return wrap(out);
@@ -846,6 +851,7 @@ PyObject* bind(PyObject*, PyObject* const* a, Py_ssize_t n) {
   get(api.tree_attn_append, "b200_tree_attn_append");
   get(api.paged_append, "b200_paged_append");
   get(api.paged_read, "b200_paged_read");
+  get(api.paged_attn_workspace, "b200_paged_attn_workspace");
   get(api.paged_attn_append, "b200_paged_attn_append");
   get(api.verify_drafts, "b200_verify_drafts");
   Py_RETURN_NONE;

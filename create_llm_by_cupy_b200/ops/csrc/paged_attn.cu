@@ -1,6 +1,7 @@
 // Attention of one new token of each sequence over a paged cache (paged_cache.cuh), with the token's rotation and append.
 #include <cooperative_groups.h>
 
+#include <algorithm>
 #include <atomic>
 
 #include "paged_cache.cuh"
@@ -10,8 +11,8 @@
 namespace b200 {
 namespace cg = cooperative_groups;
 
-constexpr int PA_WARPS = 4;
-constexpr int PA_HEADS = 8;          // query heads of a CTA: rows 0..7 of a product hold them, rows 8..15 what their rounding left
+constexpr int PA_WARPS = 4, PA_THREADS = 32 * (PA_WARPS + 1);
+constexpr int PA_HEADS = 4;          // query heads of a CTA: columns 0..3 of a product hold them, columns 4..7 what their rounding left
 constexpr int kScorePlain = 0, kScoreCap = 1, kScoreBias = 2;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -27,7 +28,9 @@ struct PagedAttnParams {
   int QH, groups, rows;
   float scale;
   ScoreCap cap;
-  int* status;
+  int pieces;                  // more than 0: a sequence's tokens go to that many CTAs, which leave their parts to another kernel
+  float2* part_ml;             // [B, QH, pieces] maximum and sum
+  float* part_o;               // [B, QH, pieces, D]
 };
 
 template <int D, int kHeld>
@@ -40,19 +43,27 @@ struct PA {
   static constexpr int kWords = kChunk * kBytes / 4;                 // 32-bit words of a chunk
   static constexpr int kMat = kTile * kRow;                          // bytes of a tile of K, or of V
   static constexpr int kStage = 2 * kMat + 2 * kTile * 4;            // and the scales
-  static constexpr int kStages = D == 128 ? 3 : 4;
-  static constexpr int kWarp = kStages * kStage + kTile * 16 + 64;   // ring, numbers of a tile's tokens, barriers
-  static constexpr int kSmem = PA_WARPS * kWarp + 256;
+  static constexpr int kStages = D == 128 ? 2 : 4;
+  static constexpr int kWarp = kStages * kStage + kTile * 16;        // a warp's ring, and numbers of a tile's tokens
+  static constexpr int kPart = (2 + D) * PA_HEADS * 4;               // maxima, sums, values of the heads
+  static constexpr int kOwn = PA_WARPS * kWarp;                      // those of the new token
+  static constexpr int kSmem = kOwn + kPart;
+  static_assert(2 * kPart <= kStages * kStage);
+  // Where byte x of a tile stands: the 16-byte pieces of a 128-byte line in another order from line to line, so that neither the eight lanes
+  // that read K together (two rows, four pieces) nor those that read V (four rows, two pieces) meet a bank twice (256-byte rows: V twice).
+  // The order repeats every eight rows.
+  __host__ __device__ static constexpr int place(int x) {
+    const int line = x >> 7, r = kRow == 256 ? line >> 1 : line;
+    return x ^ (kRow == 64 ? (line & 3) << 5 : ((r & 6) ^ (r & 1) << 2) << 4);
+  }
 };
 
-__device__ __forceinline__ void bulk_to_smem(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
-  asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
-               ::"r"(smem_u32(dst)), "l"(__cvta_generic_to_global(src)), "r"(bytes), "r"(smem_u32(bar)) : "memory");
+// 16 or 4 bytes on their way to shared memory, or zeros in their place.
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(there ? 16 : 0) : "memory");
 }
-// Four bytes, or zeros in their place.
-__device__ __forceinline__ void cp_async4(void* dst, const void* src, bool there) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(smem_u32(dst)), "l"(__cvta_generic_to_global(src)), "r"(there ? 4 : 0)
-               : "memory");
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool there) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(there ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -61,10 +72,10 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 template <int kHeld>
 __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (kHeld == kHeldBf16)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
@@ -80,6 +91,13 @@ __device__ __forceinline__ void two_parts(float x, float y, uint32_t& hi, uint32
     const float2 f = float2_of_half2(hi);
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(y - f.y), "f"(x - f.x));
   }
+}
+
+// An 8 x 8 matrix of 16-bit elements, a row to four lanes, turned over.
+__device__ __forceinline__ uint32_t turned(uint32_t x) {
+  uint32_t y;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 __device__ __forceinline__ float exp2_of(float x) {
@@ -104,12 +122,16 @@ __device__ __forceinline__ void load_bf16(const bf16* x, float* y) {
   }
 }
 
-// The chunks of a head that a lane takes, rotated. The partner of an element is half the chunks away: in the same lane.
+// The chunks of a head that a lane takes, and their rotation. The partner of an element is half the chunks away: in the same lane.
 template <int D, int kHeld>
-__device__ __forceinline__ void rotated_chunks(const bf16* x, int tq, const float* c, const float* s, float (&y)[D / 4]) {
+__device__ __forceinline__ void load_chunks(const bf16* x, int tq, float (&y)[D / 4]) {
   using L = PA<D, kHeld>;
 #pragma unroll
   for (int i = 0; i < L::kChunks; ++i) load_bf16<L::kChunk>(x + (i * 4 + tq) * L::kChunk, y + i * L::kChunk);
+}
+template <int D, int kHeld>
+__device__ __forceinline__ void rotate_chunks(float (&y)[D / 4], int tq, const float* c, const float* s) {
+  using L = PA<D, kHeld>;
 #pragma unroll
   for (int i = 0; i < L::kChunks / 2; ++i)
 #pragma unroll
@@ -123,120 +145,117 @@ __device__ __forceinline__ void rotated_chunks(const bf16* x, int tq, const floa
     }
 }
 
-// Grid (cluster, KVH * groups, B), cluster (size, 1, 1): the CTAs of a cluster share the tokens of one sequence and KV head, their warps
-// take a tile in turn.
+// Grid (cluster or pieces, KVH * groups, B), cluster (size, 1, 1): the CTAs along x share the tokens of one sequence and KV head, their four
+// warps take a tile in turn. A fifth warp deals with the new token. What they have is joined in the cluster, or by the next kernel.
 template <int D, int kHeld, int kScore>
-__global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const PagedAttnParams p) {
+__global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAttnParams p) {
   using L = PA<D, kHeld>;
-  constexpr int kTile = L::kTile, kRow = L::kRow, kNt = kTile / 8;
+  constexpr int kTile = L::kTile, kRow = L::kRow, kNt = kTile / 8, kStages = L::kStages;
   constexpr float kUp = kHeld == kHeldBf16 ? 0.f : 14.f;       // log2 of what the largest weight of a row is held as
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
   uint8_t* mine = smem + warp * L::kWarp;
-  float4* numbers = reinterpret_cast<float4*>(mine + L::kStages * L::kStage);
-  uint64_t* full = reinterpret_cast<uint64_t*>(mine + L::kStages * L::kStage + kTile * 16);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + PA_WARPS * L::kWarp);
-  if (threadIdx.x == 0) *abort_flag = 0;
-  if (lane == 0) {
-    for (int i = 0; i < L::kStages; ++i) mbar_init(&full[i], 1);
-    mbar_fence_init();
-  }
-  __syncthreads();
+  float4* numbers = reinterpret_cast<float4*>(mine + kStages * L::kStage);
   pdl_wait();
   pdl_trigger();
 
   const int cs = gridDim.x, rank = blockIdx.x, b = blockIdx.z, kvh = blockIdx.y / p.groups, grp = blockIdx.y % p.groups;
   const int R = p.QH / p.c.KVH, heads = min(R - grp * PA_HEADS, PA_HEADS), h0 = kvh * R + grp * PA_HEADS;
-  const int pos = p.lens[b], len = int(min((long long)max(pos, 0), p.c.tokens()));
-  const int* table = p.c.table + (long long)b * p.c.width;
+  const bf16* row_in = p.kqv + (long long)b * p.ld;
+  const int pos = p.lens[b];
+  float q[D / 4];
+  load_chunks<D, kHeld>(row_in + ((long long)p.c.KVH + h0 + min(g & 3, heads - 1)) * D, tq, q);
+  const int len = int(min((long long)max(pos, 0), p.c.tokens()));
   const int nt = (len + kTile - 1) / kTile, step = cs * PA_WARPS, first = rank * PA_WARPS + warp;
-  const int count = pos < 0 || first >= nt ? 0 : (nt - first + step - 1) / step;
+  const int count = warp == PA_WARPS || pos < 0 || first >= nt ? 0 : (nt - first + step - 1) / step;
 
-  // Pages of 32 tiles of this warp at a time, a lane each; tiles are asked for ahead, and their pages with them.
+  // Tiles are asked for kStages ahead, with loads of their own of all lanes: bulk copies brought an SM no more than 15 bytes a cycle,
+  // two thirds of its share of HBM. The pages of 32 tiles are looked up at a time, a lane each.
+  const int* table = p.c.table + (long long)b * p.c.width;
   int pages = -1;
-  auto page_of = [&](int i) {                                // all lanes; i goes up by one from call to call
-    if ((i & 31) == 0) {
-      const int t = first + (i + lane) * step;
-      pages = i + lane < count ? table[(t * kTile) >> p.c.log_page] : -1;
-    }
-    return __shfl_sync(0xffffffffu, pages, i & 31);
-  };
   uint32_t skipped = 0;                                      // bit i % 32: tile i has no page
   auto ask = [&](int i) {
     if (i < count) {
-      const int pg = page_of(i), t0 = (first + i * step) * kTile, rows = min(kTile, len - t0);
-      const bool there = pg >= 0 && pg < p.c.pages;
-      uint8_t* st = mine + (i % L::kStages) * L::kStage;
-      const long long row = there ? (((long long)pg * p.c.KVH + kvh) << p.c.log_page) + (t0 & (p.c.page() - 1)) : 0;
-      skipped = (skipped & ~(1u << (i & 31))) | (there ? 0u : 1u << (i & 31));
-      if (there && lane == 0) {
-        mbar_expect_tx(&full[i % L::kStages], 2 * rows * kRow);
-        bulk_to_smem(st, static_cast<const uint8_t*>(p.c.k) + row * kRow, rows * kRow, &full[i % L::kStages]);
-        bulk_to_smem(st + L::kMat, static_cast<const uint8_t*>(p.c.v) + row * kRow, rows * kRow, &full[i % L::kStages]);
-      } else if (lane == 0) {
-        mbar_arrive(&full[i % L::kStages]);
+      if ((i & 31) == 0) {
+        const int t = first + (i + lane) * step;
+        pages = i + lane < count ? table[(t * kTile) >> p.c.log_page] : -1;
       }
-      if constexpr (kHeld != kHeldBf16) {
-        const bool has = there && lane < rows;
-        cp_async4(st + 2 * L::kMat + lane * 4, p.c.ks + (has ? row + lane : 0), has);
-        cp_async4(st + 2 * L::kMat + kTile * 4 + lane * 4, p.c.vs + (has ? row + lane : 0), has);
+      const int pg = __shfl_sync(0xffffffffu, pages, i & 31), t0 = (first + i * step) * kTile, bytes = min(kTile, len - t0) * kRow;
+      const bool there = pg >= 0 && pg < p.c.pages;
+      skipped = (skipped & ~(1u << (i & 31))) | (there ? 0u : 1u << (i & 31));
+      if (there) {
+        const uint32_t st = smem_u32(mine) + (i % kStages) * L::kStage;
+        const long long row = (((long long)pg * p.c.KVH + kvh) << p.c.log_page) + (t0 & (p.c.page() - 1));
+        const uint8_t* k = static_cast<const uint8_t*>(p.c.k) + row * kRow + lane * 16;
+        const uint8_t* v = static_cast<const uint8_t*>(p.c.v) + row * kRow + lane * 16;
+#pragma unroll
+        for (int x = 0; x < L::kMat; x += 512) cp_async16(st + L::place(x + lane * 16), k + (x + lane * 16 < bytes ? x : 0), x + lane * 16 < bytes);
+        if constexpr (kHeld != kHeldBf16) {
+          const bool has = lane * kRow < bytes;
+          cp_async4(st + 2 * L::kMat + lane * 4, p.c.ks + row + (has ? lane : 0), has);
+          cp_async4(st + 2 * L::kMat + kTile * 4 + lane * 4, p.c.vs + row + (has ? lane : 0), has);
+        }
+#pragma unroll
+        for (int x = 0; x < L::kMat; x += 512)
+          cp_async16(st + L::kMat + L::place(x + lane * 16), v + (x + lane * 16 < bytes ? x : 0), x + lane * 16 < bytes);
       }
     }
-    if constexpr (kHeld != kHeldBf16) cp_async_commit();
+    cp_async_commit();
   };
 #pragma unroll
-  for (int i = 0; i < L::kStages; ++i) ask(i);
+  for (int i = 0; i < kStages; ++i) ask(i);
 
-  // The queries as fragments. fp16 has room for little: each row is brought to a largest magnitude of 2^10 by a power of two.
-  uint32_t qf[D / 16][4];
-  float row_mul = 1.f;                                       // what a product is multiplied with, without the token's scale
+  // The queries as fragments: lanes g < 4 the rounded values of head g, the others what that left of head g - 4. fp16 has room for little:
+  // each head is brought to a largest magnitude of 2^10 by a power of two.
+  uint32_t qf[D / 16][2];
+  float row_mul = 1.f;                                       // what a product of head g & 3 is multiplied with, without the token's scale
   const int at = min(max(pos, 0), p.rows - 1);
   const float* cosr = p.cosr + (long long)at * (D / 2);
   const float* sinr = p.sinr + (long long)at * (D / 2);
-  float q[D / 4];
-  {
-    const bf16* x = p.kqv + (long long)b * p.ld + ((long long)p.c.KVH + h0 + min(g, heads - 1)) * D;
-    rotated_chunks<D, kHeld>(x, tq, cosr, sinr, q);
-    if constexpr (kHeld != kHeldBf16) {
-      float m = 0.f;
+  rotate_chunks<D, kHeld>(q, tq, cosr, sinr);
+  if constexpr (kHeld != kHeldBf16) {
+    float m = 0.f;
 #pragma unroll
-      for (int i = 0; i < D / 4; ++i) m = fmaxf(m, fabsf(q[i]));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      const int e = min(max(int(__float_as_uint(m) >> 23) - 127, -100), 100);
-      const float up = __uint_as_float(uint32_t(127 + 10 - e) << 23);
-      row_mul = __uint_as_float(uint32_t(127 - 10 + e) << 23);
+    for (int i = 0; i < D / 4; ++i) m = fmaxf(m, fabsf(q[i]));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
+    m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const int e = min(max(int(__float_as_uint(m) >> 23) - 127, -100), 100);
+    const float up = __uint_as_float(uint32_t(127 + 10 - e) << 23);
+    row_mul = __uint_as_float(uint32_t(127 - 10 + e) << 23);
 #pragma unroll
-      for (int i = 0; i < D / 4; ++i) q[i] *= up;
-    }
-#pragma unroll
-    for (int i = 0; i < D / 16; ++i) {
-      two_parts<kHeld>(q[4 * i], q[4 * i + 1], qf[i][0], qf[i][1]);
-      two_parts<kHeld>(q[4 * i + 2], q[4 * i + 3], qf[i][2], qf[i][3]);
-    }
+    for (int i = 0; i < D / 4; ++i) q[i] *= up;
   }
-  float slope = 0.f;
-  if (kScore == kScoreBias) slope = p.slopes[h0 + min(g, heads - 1)] * kLog2e;
-  const float mul = kScore == kScoreCap ? row_mul : row_mul * p.scale * kLog2e;
-  // log2-unit score of a product of row g with a token that is `dist` back
-  auto score = [&](float s, float dist) {
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      uint32_t hi, lo;
+      two_parts<kHeld>(q[4 * i + 2 * e], q[4 * i + 2 * e + 1], hi, lo);
+      qf[i][e] = g < 4 ? hi : lo;
+    }
+  // Score in units of log2 of a product with a token that is `dist` back.
+  auto score = [&](float s, float mul, float slope, float dist) {
     s *= mul;
     if (kScore == kScoreCap) return cap_any(s, p.cap);
     return kScore == kScoreBias ? fmaf(-slope, dist, s) : s;
   };
+  const float unit = kScore == kScoreCap ? 1.f : p.scale * kLog2e;
 
-  float m_run = -INFINITY, l_run = 0.f;
-  float o[D / 8][4];
+  auto part = [&](int w) { return reinterpret_cast<float*>(smem + (w < PA_WARPS ? w * L::kWarp : L::kOwn)); };
+  float* wm = part(warp);                                    // [4] maxima, [4] sums, [4][D] values of a warp
+  float* wl = wm + PA_HEADS;
+  float* wo = wl + PA_HEADS;
+  // The new token: written to its page, and all that the fifth warp sees.
+  if (warp == PA_WARPS && rank == 0) {
+    float m_new = -INFINITY, l_new = 0.f, v[D / 4];
 #pragma unroll
-  for (int j = 0; j < D / 8; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
-
-  // The new token: written to its page, and the first that its warp sees.
-  if (warp == 0 && rank == 0 && pos >= 0 && pos < p.c.tokens() && pos < p.rows) {
-    const long long row = paged_row(p.c, b, kvh, pos);
+    for (int i = 0; i < D / 4; ++i) v[i] = 0.f;
+    const long long row = pos >= 0 && pos < p.c.tokens() && pos < p.rows ? paged_row(p.c, b, kvh, pos) : -1;
     if (row >= 0) {
-      float k[D / 4], v[D / 4], ks = 1.f, vs = 1.f;
-      rotated_chunks<D, kHeld>(p.kqv + (long long)b * p.ld + (long long)kvh * D, tq, cosr, sinr, k);
-      load_bf16<D / 4>(p.kqv + (long long)b * p.ld + ((long long)p.c.KVH + p.QH + kvh) * D + tq * (D / 4), v);
+      float k[D / 4], ks = 1.f, vs = 1.f;
+      load_chunks<D, kHeld>(row_in + (long long)kvh * D, tq, k);
+      load_bf16<D / 4>(row_in + ((long long)p.c.KVH + p.QH + kvh) * D + tq * (D / 4), v);
+      rotate_chunks<D, kHeld>(k, tq, cosr, sinr);
       const bool writes = g == 0 && grp == 0;
       if constexpr (kHeld == kHeldBf16) {
 #pragma unroll
@@ -304,114 +323,161 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const Page
       for (int i = 0; i < D / 4; ++i) s = fmaf(q[i], k[i], s);
       s += __shfl_xor_sync(0xffffffffu, s, 1);
       s += __shfl_xor_sync(0xffffffffu, s, 2);
-      s = score(s * ks, 0.f);
-      m_run = kHeld == kHeldBf16 ? s : s + __log2f(vs);
+      s = score(s * ks, row_mul * unit, 0.f, 0.f);
+      m_new = kHeld == kHeldBf16 ? s : s + __log2f(vs);
       const float w = exp2_of(kUp);
-      l_run = tq == 0 ? w * (kHeld == kHeldBf16 ? 1.f : __frcp_rn(vs)) : 0.f;
+      l_new = w * (kHeld == kHeldBf16 ? 1.f : __frcp_rn(vs));
 #pragma unroll
-      for (int i = 0; i < D / 4; ++i) o[i % (D / 8)][i / (D / 8)] = v[i] * w;
+      for (int i = 0; i < D / 4; ++i) v[i] *= w;
+    }
+    if (g < PA_HEADS) {
+      if (tq == 0) {
+        wm[g] = m_new;
+        wl[g] = l_new;
+      }
+#pragma unroll
+      for (int i = 0; i < D / 4; i += 4) *reinterpret_cast<float4*>(wo + g * D + tq * (D / 4) + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
     }
   }
 
-  bool ok = true;
+  // This lane's two columns of a tile's products: heads `ha` and `ha + 1`, or what is left of them; running maxima and sums of both.
+  const int ha = 2 * (tq & 1);
+  float mul[2], slope[2] = {0.f, 0.f}, m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    mul[e] = __shfl_sync(0xffffffffu, row_mul, 4 * (ha + e)) * unit;
+    if (kScore == kScoreBias) slope[e] = p.slopes[h0 + min(ha + e, heads - 1)] * kLog2e;
+  }
+  float o[D / 16][4];                                        // dims (D / 8) g + 2 j of both heads, then the next dim of both
+#pragma unroll
+  for (int j = 0; j < D / 16; ++j) o[j][0] = o[j][1] = o[j][2] = o[j][3] = 0.f;
 #pragma unroll 1
   for (int i = 0; i < count; ++i) {
-    const int slot = i % L::kStages, t0 = (first + i * step) * kTile, rows = min(kTile, len - t0);
-    uint8_t* st = mine + slot * L::kStage;
-    if constexpr (kHeld != kHeldBf16) cp_async_wait<L::kStages - 1>();
-    ok = __all_sync(0xffffffffu, mbar_wait(&full[slot], (i / L::kStages) & 1, abort_flag));
-    if (!ok) break;
+    const int t0 = (first + i * step) * kTile, rows = min(kTile, len - t0);
+    const uint8_t* st = mine + (i % kStages) * L::kStage;
+    cp_async_wait<kStages - 1>();
+    __syncwarp();
     if (!(skipped >> (i & 31) & 1)) {
       if constexpr (kHeld != kHeldBf16) {
         // a token's numbers: what its products are multiplied with, log2 of V's scale, and one over it
         const float* sc = reinterpret_cast<const float*>(st + 2 * L::kMat);
         const bool has = lane < rows;
-        const float ks = sc[lane], vs = has ? sc[kTile + lane] : 1.f;
-        numbers[lane] = make_float4(has ? ks : 0.f, has ? __log2f(vs) : 0.f, __fdividef(1.f, vs), 0.f);
+        const float ks = has ? sc[lane] : 0.f, vs = has ? sc[kTile + lane] : 1.f;
+        numbers[lane] = make_float4(ks, has ? __log2f(vs) : 0.f, __fdividef(1.f, vs), 0.f);
       }
-      if (rows < kTile)                                      // what lies behind the last token may be anything: its weight is 0, it shall be
-        for (int x = rows * kRow + lane * 4; x < L::kMat; x += 128) *reinterpret_cast<uint32_t*>(st + L::kMat + x) = 0u;
       __syncwarp();
-      float y[2 * kNt], rv[2 * kNt];
+      // Scores: tokens are the rows of the products, 16 at a time.
+      constexpr int kMt = kTile / 16;
+      float acc[kMt][4];
 #pragma unroll
-      for (int n = 0; n < kNt; ++n) {
-        float acc[4] = {0.f, 0.f, 0.f, 0.f};
-        const uint8_t* kr = st + (8 * n + g) * kRow + tq * L::kChunk * L::kBytes;
+      for (int t = 0; t < kMt; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+      constexpr int kPiece = L::kChunk * L::kBytes;
+      const uint8_t* kr = st + L::place(g * kRow + tq * kPiece);
+      const int other = L::place(g * kRow + (tq + 4) * kPiece) - L::place(g * kRow + tq * kPiece);
 #pragma unroll
-        for (int c = 0; c < L::kChunks; ++c) {
-          uint32_t w[L::kWords];
+      for (int c = 0; c < L::kChunks; ++c) {
+        uint32_t w[2 * kMt][L::kWords];
+#pragma unroll
+        for (int n = 0; n < 2 * kMt; ++n) {
+          const uint8_t* from = kr + 8 * n * kRow + (c & 1) * other + (c >> 1) * 8 * kPiece;
           if constexpr (L::kWords == 4) {
-            const uint4 u = *reinterpret_cast<const uint4*>(kr + c * 4 * L::kChunk * L::kBytes);
-            w[0] = u.x; w[1] = u.y; w[2] = u.z; w[3] = u.w;
+            const uint4 u = *reinterpret_cast<const uint4*>(from);
+            w[n][0] = u.x; w[n][1] = u.y; w[n][2] = u.z; w[n][3] = u.w;
           } else {
-            const uint2 u = *reinterpret_cast<const uint2*>(kr + c * 4 * L::kChunk * L::kBytes);
-            w[0] = u.x; w[1] = u.y;
+            const uint2 u = *reinterpret_cast<const uint2*>(from);
+            w[n][0] = u.x; w[n][1] = u.y;
           }
-          if constexpr (kHeld == kHeldBf16) {
+        }
+        if constexpr (kHeld == kHeldBf16) {
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const uint32_t (&a)[4] = qf[2 * c + e];
-              mma_16816<kHeld>(acc, a[0], a[1], a[2], a[3], w[2 * e], w[2 * e + 1]);
-            }
-          } else {
+          for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int e = 0; e < L::kWords; ++e) {
-              const uint32_t (&a)[4] = qf[c * L::kWords + e];
-              const uint32_t x = kHeld == kHeldInt8 ? w[e] ^ 0x80808080u : w[e];
-              mma_16816<kHeld>(acc, a[0], a[1], a[2], a[3], half2_of<kHeld, false>(x), half2_of<kHeld, true>(x));
+            for (int t = 0; t < kMt; ++t)
+              mma_16816<kHeld>(acc[t], w[2 * t][2 * e], w[2 * t + 1][2 * e], w[2 * t][2 * e + 1], w[2 * t + 1][2 * e + 1], qf[2 * c + e][0],
+                               qf[2 * c + e][1]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < L::kWords; ++e)
+#pragma unroll
+            for (int t = 0; t < kMt; ++t) {
+              const uint32_t x = kHeld == kHeldInt8 ? w[2 * t][e] ^ 0x80808080u : w[2 * t][e];
+              const uint32_t z = kHeld == kHeldInt8 ? w[2 * t + 1][e] ^ 0x80808080u : w[2 * t + 1][e];
+              mma_16816<kHeld>(acc[t], half2_of<kHeld, false>(x), half2_of<kHeld, false>(z), half2_of<kHeld, true>(x), half2_of<kHeld, true>(z),
+                               qf[c * L::kWords + e][0], qf[c * L::kWords + e][1]);
             }
-          }
+        }
+      }
+      // y[n][e]: token 8 n + g, head ha + e; what the rounding of Q left comes from the lane two further.
+      float y[2 * kMt][2], rv[2 * kMt], m[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+      for (int n = 0; n < 2 * kMt; ++n) {
+        const int tok = 8 * n + g;
+        float ks = 1.f, more = 0.f;
+        rv[n] = 1.f;
+        if constexpr (kHeld != kHeldBf16) {
+          const float4 u = numbers[tok];
+          ks = u.x;
+          more = u.y;
+          rv[n] = u.z;
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const int tok = 8 * n + 2 * tq + e;
-          float s = acc[e] + acc[2 + e], more = 0.f;
-          rv[2 * n + e] = 1.f;
-          if constexpr (kHeld != kHeldBf16) {
-            const float4 u = numbers[tok];
-            s *= u.x;
-            more = u.y;
-            rv[2 * n + e] = u.z;
-          }
-          s = score(s, float(pos - t0 - tok)) + more;
-          y[2 * n + e] = tok < rows ? s : -INFINITY;
+          float s = acc[n >> 1][2 * (n & 1) + e];
+          s += __shfl_xor_sync(0xffffffffu, s, 2);
+          s = score(s * ks, mul[e], slope[e], float(pos - t0 - tok)) + more;
+          y[n][e] = tok < rows ? s : -INFINITY;
+          m[e] = fmaxf(m[e], y[n][e]);
         }
       }
-      float m = y[0];
+      float ref[2], f[2];
 #pragma unroll
-      for (int e = 1; e < 2 * kNt; ++e) m = fmaxf(m, y[e]);
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-      const float m_new = fmaxf(m_run, m), ref = m_new == -INFINITY ? 0.f : m_new;
-      const float f = exp2_of(m_run - ref);
-      if (__any_sync(0xffffffffu, f != 1.f)) {
-        l_run *= f;
+      for (int e = 0; e < 2; ++e) {
+        m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 4));
+        m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 8));
+        m[e] = fmaxf(m[e], __shfl_xor_sync(0xffffffffu, m[e], 16));
+        m[e] = fmaxf(m_run[e], m[e]);
+        ref[e] = m[e] == -INFINITY ? 0.f : m[e];
+        f[e] = exp2_of(m_run[e] - ref[e]);
+        m_run[e] = m[e];
+      }
+      if (__any_sync(0xffffffffu, f[0] != 1.f || f[1] != 1.f)) {
+        l_run[0] *= f[0];
+        l_run[1] *= f[1];
 #pragma unroll
-        for (int j = 0; j < D / 8; ++j) {
-          o[j][0] *= f; o[j][1] *= f; o[j][2] *= f; o[j][3] *= f;
+        for (int j = 0; j < D / 16; ++j) {
+          o[j][0] *= f[0]; o[j][1] *= f[1]; o[j][2] *= f[0]; o[j][3] *= f[1];
         }
       }
-      m_run = m_new;
-      uint32_t hi[kNt], lo[kNt];
+      uint32_t pw[2 * kMt];                                  // weights, tokens along the lanes' pairs
 #pragma unroll
-      for (int n = 0; n < kNt; ++n) {
-        const float w0 = exp2_of(y[2 * n] - ref + kUp), w1 = exp2_of(y[2 * n + 1] - ref + kUp);
-        l_run = fmaf(w0, rv[2 * n], l_run);
-        l_run = fmaf(w1, rv[2 * n + 1], l_run);
-        two_parts<kHeld>(w0, w1, hi[n], lo[n]);
+      for (int n = 0; n < 2 * kMt; ++n) {
+        const float w0 = exp2_of(y[n][0] - ref[0] + kUp), w1 = exp2_of(y[n][1] - ref[1] + kUp);
+        l_run[0] = fmaf(w0, rv[n], l_run[0]);
+        l_run[1] = fmaf(w1, rv[n], l_run[1]);
+        uint32_t hi, lo;
+        two_parts<kHeld>(w0, w1, hi, lo);
+        pw[n] = turned(tq < 2 ? hi : lo);
       }
-      const uint8_t* vr = st + L::kMat + 2 * tq * kRow + g * (kRow / 8);
+      // Values: dims are the rows of the products.
+      constexpr int kVw = kRow / 32;                         // words of a lane's piece of a row; of 256-byte rows it is two places
+      const uint8_t* vr[2];
+      int next[2];
 #pragma unroll
-      for (int n = 0; n < kNt; n += 2) {
-        constexpr int kVw = kRow / 32;                       // words of a lane's piece of a row
+      for (int x = 0; x < 2; ++x) {
+        const int from = (2 * tq + x) * kRow + g * (kRow / 8);
+        vr[x] = st + L::kMat + L::place(from);
+        next[x] = L::place(from + 16) - L::place(from);
+      }
+#pragma unroll
+      for (int t = 0; t < kMt; ++t) {
         uint32_t r[4][kVw];
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const uint8_t* from = vr + (8 * n + 8 * (x >> 1) + (x & 1)) * kRow;
+          const uint8_t* from = vr[x & 1] + (16 * t + 8 * (x >> 1)) * kRow;
           if constexpr (kVw >= 4) {
 #pragma unroll
             for (int c = 0; c < kVw / 4; ++c) {
-              const uint4 u = reinterpret_cast<const uint4*>(from)[c];
+              const uint4 u = *reinterpret_cast<const uint4*>(c == 0 ? from : from + next[x & 1]);
               r[x][4 * c] = u.x; r[x][4 * c + 1] = u.y; r[x][4 * c + 2] = u.z; r[x][4 * c + 3] = u.w;
             }
           } else {
@@ -419,68 +485,75 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const Page
             r[x][0] = u.x; r[x][1] = u.y;
           }
         }
+        const uint32_t b0 = pw[2 * t], b1 = pw[2 * t + 1];
 #pragma unroll
         for (int w = 0; w < kVw; ++w) {
           if constexpr (kHeld == kHeldBf16) {
-            mma_16816<kHeld>(o[2 * w], hi[n], lo[n], hi[n + 1], lo[n + 1], __byte_perm(r[0][w], r[1][w], 0x5410),
-                             __byte_perm(r[2][w], r[3][w], 0x5410));
-            mma_16816<kHeld>(o[2 * w + 1], hi[n], lo[n], hi[n + 1], lo[n + 1], __byte_perm(r[0][w], r[1][w], 0x7632),
-                             __byte_perm(r[2][w], r[3][w], 0x7632));
+            mma_16816<kHeld>(o[w], __byte_perm(r[0][w], r[1][w], 0x5410), __byte_perm(r[0][w], r[1][w], 0x7632),
+                             __byte_perm(r[2][w], r[3][w], 0x5410), __byte_perm(r[2][w], r[3][w], 0x7632), b0, b1);
           } else {
             uint32_t a = __byte_perm(r[0][w], r[1][w], 0x5140), c = __byte_perm(r[2][w], r[3][w], 0x5140);
             uint32_t d = __byte_perm(r[0][w], r[1][w], 0x7362), e = __byte_perm(r[2][w], r[3][w], 0x7362);
             if (kHeld == kHeldInt8) {
               a ^= 0x80808080u; c ^= 0x80808080u; d ^= 0x80808080u; e ^= 0x80808080u;
             }
-            mma_16816<kHeld>(o[4 * w], hi[n], lo[n], hi[n + 1], lo[n + 1], half2_of<kHeld, false>(a), half2_of<kHeld, false>(c));
-            mma_16816<kHeld>(o[4 * w + 1], hi[n], lo[n], hi[n + 1], lo[n + 1], half2_of<kHeld, true>(a), half2_of<kHeld, true>(c));
-            mma_16816<kHeld>(o[4 * w + 2], hi[n], lo[n], hi[n + 1], lo[n + 1], half2_of<kHeld, false>(d), half2_of<kHeld, false>(e));
-            mma_16816<kHeld>(o[4 * w + 3], hi[n], lo[n], hi[n + 1], lo[n + 1], half2_of<kHeld, true>(d), half2_of<kHeld, true>(e));
+            mma_16816<kHeld>(o[2 * w], half2_of<kHeld, false>(a), half2_of<kHeld, true>(a), half2_of<kHeld, false>(c), half2_of<kHeld, true>(c),
+                             b0, b1);
+            mma_16816<kHeld>(o[2 * w + 1], half2_of<kHeld, false>(d), half2_of<kHeld, true>(d), half2_of<kHeld, false>(e),
+                             half2_of<kHeld, true>(e), b0, b1);
           }
         }
       }
     }
     __syncwarp();
-    ask(i + L::kStages);
+    ask(i + kStages);
   }
 
-  // Over the lanes, the warps and the CTAs of the cluster. The ring is free: every tile that was asked for has been waited for, or the
-  // kernel gives up (then what still arrives may overwrite these numbers, which nobody uses, but not another kernel's memory).
-  l_run += __shfl_xor_sync(0xffffffffu, l_run, 1);
-  l_run += __shfl_xor_sync(0xffffffffu, l_run, 2);
+  // Over the lanes, the warps and the CTAs of the cluster. The ring is free: every tile that was asked for has arrived.
   cg::cluster_group cluster = cg::this_cluster();
-  float* wm = reinterpret_cast<float*>(mine);                // [8] maxima, [8] sums, [8][D] values of a warp
-  float* wl = wm + PA_HEADS;
-  float* wo = wl + PA_HEADS;
-  if (tq == 0) {
-    wm[g] = m_run;
-    wl[g] = l_run;
+  if (warp < PA_WARPS) {
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 4);
+      l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 8);
+      l_run[e] += __shfl_xor_sync(0xffffffffu, l_run[e], 16);
+      if (g == 0 && tq < 2) {
+        wm[ha + e] = m_run[e];
+        wl[ha + e] = l_run[e];
+      }
+#pragma unroll
+      for (int j = 0; j < D / 16; ++j) {
+        float x = o[j][e], z = o[j][2 + e];
+        x += __shfl_xor_sync(0xffffffffu, x, 2);
+        z += __shfl_xor_sync(0xffffffffu, z, 2);
+        if (tq < 2) *reinterpret_cast<float2*>(wo + (ha + e) * D + g * (D / 8) + 2 * j) = make_float2(x, z);
+      }
+    }
   }
-#pragma unroll
-  for (int j = 0; j < D / 8; j += 4)
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-      *reinterpret_cast<float4*>(wo + g * D + (2 * tq + e) * (D / 8) + j) =
-          make_float4(o[j][e] + o[j][2 + e], o[j + 1][e] + o[j + 1][2 + e], o[j + 2][e] + o[j + 2][2 + e], o[j + 3][e] + o[j + 3][2 + e]);
   __syncthreads();
-  constexpr int kPart = (2 + D) * PA_HEADS * 4;              // bytes of such a set
-  float* cm = reinterpret_cast<float*>(smem + kPart);        // the CTA's, behind the first warp's
+  float* cm = reinterpret_cast<float*>(smem + L::kPart);        // the CTA's, behind the first warp's
   float* cl = cm + PA_HEADS;
   float* co = cl + PA_HEADS;
-  for (int i = threadIdx.x; i < heads * D; i += PA_WARPS * 32) {
+  for (int i = threadIdx.x; i < heads * D; i += PA_THREADS) {
     const int r = i / D, d = i % D;
     float m = -INFINITY, l = 0.f, x = 0.f;
 #pragma unroll
-    for (int w = 0; w < PA_WARPS; ++w) m = fmaxf(m, *reinterpret_cast<const float*>(smem + w * L::kWarp + r * 4));
+    for (int w = 0; w <= PA_WARPS; ++w)
+      if (w < PA_WARPS || rank == 0) m = fmaxf(m, part(w)[r]);
     const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int w = 0; w < PA_WARPS; ++w) {
-      const float* s = reinterpret_cast<const float*>(smem + w * L::kWarp);
+    for (int w = 0; w <= PA_WARPS; ++w) {
+      if (w == PA_WARPS && rank != 0) break;
+      const float* s = part(w);
       const float f = exp2_of(s[r] - ref);
       l = fmaf(s[PA_HEADS + r], f, l);
       x = fmaf(s[2 * PA_HEADS + r * D + d], f, x);
     }
-    if (cs == 1) {
+    if (p.pieces > 0) {
+      const long long at = ((long long)b * p.QH + h0 + r) * p.pieces + rank;
+      p.part_o[at * D + d] = x;
+      if (d == 0) p.part_ml[at] = make_float2(m, l);
+    } else if (cs == 1) {
       p.out[((long long)b * p.QH + h0 + r) * D + d] = __float2bfloat16(l == 0.f ? 0.f : x / l);
     } else {
       co[r * D + d] = x;
@@ -490,9 +563,9 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const Page
       }
     }
   }
-  if (cs > 1) {
+  if (cs > 1 && p.pieces == 0) {
     cluster.sync();
-    for (int i = rank * PA_WARPS * 32 + threadIdx.x; i < heads * D; i += cs * PA_WARPS * 32) {
+    for (int i = rank * PA_THREADS + threadIdx.x; i < heads * D; i += cs * PA_THREADS) {
       const int r = i / D;
       float m = -INFINITY, l = 0.f, x = 0.f;
       for (int c = 0; c < cs; ++c) m = fmaxf(m, *cluster.map_shared_rank(cm + r, c));
@@ -506,7 +579,38 @@ __global__ void __launch_bounds__(PA_WARPS * 32, 2) paged_attn_kernel(const Page
     }
     cluster.sync();                                          // peers read this CTA's numbers until here
   }
-  if (threadIdx.x == 0 && *abort_flag != 0 && p.status != nullptr && atomicCAS(p.status, 0, int(*abort_flag)) == 0) p.status[1] = 361;
+}
+
+// The parts of a query head: grid B * QH, a thread for each dim.
+template <int D>
+__global__ void __launch_bounds__(D) paged_join_kernel(const PagedAttnParams p) {
+  const int d = threadIdx.x;
+  pdl_wait();
+  pdl_trigger();
+  const float2* ml = p.part_ml + (long long)blockIdx.x * p.pieces;
+  const float* o = p.part_o + (long long)blockIdx.x * p.pieces * D + d;
+  float m = -INFINITY, l = 0.f, x = 0.f;
+  for (int c = 0; c < p.pieces; ++c) m = fmaxf(m, ml[c].x);
+  const float ref = m == -INFINITY ? 0.f : m;
+#pragma unroll 8
+  for (int c = 0; c < p.pieces; ++c) {
+    const float f = exp2_of(ml[c].x - ref);
+    l = fmaf(ml[c].y, f, l);
+    x = fmaf(o[(long long)c * D], f, x);
+  }
+  p.out[(long long)blockIdx.x * D + d] = __float2bfloat16(l == 0.f ? 0.f : x / l);
+}
+
+static int paged_groups(int QH, int KVH) { return (QH / KVH + PA_HEADS - 1) / PA_HEADS; }
+
+// CTAs that share a sequence and KV head: {size of their cluster, 0}, or {1, pieces}.
+static int2 paged_split(int B, int QH, int KVH, int width, int log_page) {
+  const long long units = (long long)B * KVH * paged_groups(QH, KVH), slots = 3LL * num_sms(), tokens = (long long)width << log_page;
+  const long long most = std::max(1LL, tokens / 256);
+  if (units * 8 <= slots / 2 && most > 8) return make_int2(1, int(std::min(slots / units, most)));
+  int cs = 1;
+  while (cs < 8 && 2 * cs * units <= slots && cs < most) cs *= 2;
+  return make_int2(cs, 0);
 }
 
 template <int D, int kHeld, int kScore>
@@ -524,10 +628,10 @@ static int launch_paged(const PagedAttnParams& p, cudaStream_t st) {
     }
     if (dev >= 0 && dev < 64) allowed[dev].store(true, std::memory_order_release);
   }
-  const long long units = (long long)p.c.B * p.c.KVH * p.groups;
-  int cs = 1;
-  while (cs < 8 && 2 * cs * units <= 2LL * num_sms() && 2LL * cs * PA_WARPS * L::kTile <= p.c.tokens() + L::kTile - 1) cs *= 2;
-  return static_cast<int>(launch_pdl(kern, dim3(cs, p.c.KVH * p.groups, p.c.B), dim3(PA_WARPS * 32), L::kSmem, st, cs, p));
+  const int cs = p.pieces > 0 ? 1 : paged_split(p.c.B, p.QH, p.c.KVH, p.c.width, p.c.log_page).x;
+  B200_CHECK(launch_pdl(kern, dim3(p.pieces > 0 ? p.pieces : cs, p.c.KVH * p.groups, p.c.B), dim3(PA_THREADS), L::kSmem, st, cs, p));
+  if (p.pieces == 0) return 0;
+  return static_cast<int>(launch_pdl(paged_join_kernel<D>, dim3(unsigned(p.c.B * p.QH)), dim3(D), 0, st, 0, p));
 }
 
 template <int D, int kHeld>
@@ -540,10 +644,17 @@ static int launch_paged_score(const PagedAttnParams& p, float cap, cudaStream_t 
 
 using namespace b200;
 
+// Bytes of the workspace that b200_paged_attn_append wants (16-byte aligned); 0: none, or sizes that it does not take.
+B200_API long long b200_paged_attn_workspace(int B, int QH, int KVH, int width, int log_page, int D) {
+  if (B < 1 || KVH < 1 || QH < 1 || QH % KVH != 0 || width < 1 || log_page < 5 || log_page > 10 || (D != 64 && D != 128)) return 0;
+  return (long long)B * QH * paged_split(B, QH, KVH, width, log_page).y * (D + 2) * 4;
+}
+
 // kqv [B] rows K | Q | V (un-rotated, pitch ld), out [B, QH, D], lens [B], rotary tables [rows, D / 2]. cap > 0: scores c tanh(s / c);
 // slopes [QH]: scores minus slope times distance (not both). held: 0 bf16, 1 int8, 2 e4m3.
 B200_API int b200_paged_attn_append(const void* kqv, void* pk, void* pv, void* ks, void* vs, const void* table, const void* lens,
-                                    const void* cosr, const void* sinr, const void* slopes, void* out, int rows, long long ld, int B,
+                                    const void* cosr, const void* sinr, const void* slopes, void* out, void* workspace, int rows,
+                                    long long ld, int B,
                                     int width, int pages, int QH, int KVH, int log_page, int D, int held, float scale, float cap,
                                     cudaStream_t st) {
   PagedAttnParams p;
@@ -558,7 +669,7 @@ B200_API int b200_paged_attn_append(const void* kqv, void* pk, void* pv, void* k
     return static_cast<int>(cudaErrorInvalidValue);
   for (const void* x : {kqv, cosr, sinr, (const void*)out})
     if (x == nullptr || (reinterpret_cast<uintptr_t>(x) & 15) != 0) return static_cast<int>(cudaErrorInvalidValue);
-  p.groups = (QH / KVH + PA_HEADS - 1) / PA_HEADS;
+  p.groups = paged_groups(QH, KVH);
   if (B > 65535 || (long long)KVH * p.groups > 65535) return static_cast<int>(cudaErrorInvalidValue);
   if (B == 0) return 0;
   p.kqv = static_cast<const bf16*>(kqv);
@@ -569,7 +680,10 @@ B200_API int b200_paged_attn_append(const void* kqv, void* pk, void* pv, void* k
   p.out = static_cast<bf16*>(out);
   p.ld = ld; p.QH = QH; p.rows = rows; p.scale = scale;
   p.cap = make_score_cap(scale, cap);
-  p.status = status_ptr();
+  p.pieces = paged_split(B, QH, KVH, width, log_page).y;
+  if (p.pieces > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) return static_cast<int>(cudaErrorInvalidValue);
+  p.part_o = static_cast<float*>(workspace);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + (long long)B * QH * p.pieces * D);
   if (D == 128)
     return held == kHeldBf16   ? launch_paged_score<128, kHeldBf16>(p, cap, st)
            : held == kHeldInt8 ? launch_paged_score<128, kHeldInt8>(p, cap, st)

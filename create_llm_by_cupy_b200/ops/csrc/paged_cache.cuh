@@ -112,7 +112,8 @@ inline const char* paged_pool_wrong(const PagedPool& c, int held, int D) {
   if (c.B < 0 || c.width < 1 || c.pages < 1 || c.KVH < 1 || c.log_page < 5 || c.log_page > 10) return "sizes";
   if (c.tokens() > 0x7fffffffLL) return "tokens";
   if (c.k == nullptr || c.v == nullptr || c.table == nullptr || (held != kHeldBf16) != (c.ks != nullptr && c.vs != nullptr)) return "pointers";
-  if (((reinterpret_cast<uintptr_t>(c.k) | reinterpret_cast<uintptr_t>(c.v)) & 15) != 0) return "alignment";
+  for (const void* x : {c.k, c.v, (void*)c.ks, (void*)c.vs})
+    if ((reinterpret_cast<uintptr_t>(x) & 15) != 0) return "alignment";
   return nullptr;
 }
 

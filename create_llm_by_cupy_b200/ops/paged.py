@@ -97,8 +97,8 @@ def _check_tables(name: str, cos, sin, D: int, like) -> None:
 def _cuda_only(name: str, cache: PagedCache) -> None:
     if cache.k.shape[3] not in (64, 128):
         raise ValueError(f"{name}: CUDA kernels exist for a head dimension of 64 or 128")
-    if (cache.k.data_ptr() | cache.v.data_ptr()) % 16:
-        raise ValueError(f"{name}: the cache starts on a 16-byte boundary")
+    if any(t is not None and t.data_ptr() % 16 for t in cache):
+        raise ValueError(f"{name}: rows and scales of the cache start on 16-byte boundaries")
 
 
 def _on_16(t):
@@ -301,8 +301,8 @@ def paged_attn_append(kqv, cache: PagedCache, table, lens, QH: int, KVH: int, co
     _cuda_only("paged_attn_append", cache)
     if cos.dtype != torch.float32 or sin.dtype != torch.float32:
         raise TypeError("paged_attn_append: rotary tables are float32")
-    if B > 65535 or KVH * ((QH // KVH + 7) // 8) > 65535:
-        raise ValueError("paged_attn_append: at most 65535 sequences, and KV heads (once for every 8 query heads), a call")
+    if B > 65535 or KVH * ((QH // KVH + 3) // 4) > 65535:
+        raise ValueError("paged_attn_append: at most 65535 sequences, and KV heads (once for every 4 query heads), a call")
     with torch.cuda.device(kqv.device):
         out = torch.empty((B, QH, D), dtype=torch.bfloat16, device=kqv.device)
         if B == 0:
@@ -311,9 +311,13 @@ def paged_attn_append(kqv, cache: PagedCache, table, lens, QH: int, KVH: int, co
             kqv = kqv.clone(memory_format=torch.contiguous_format)
         cos, sin, table, lens = _on_16(cos), _on_16(sin), table.contiguous(), lens.contiguous()
         slopes = slopes if slopes is None else slopes.contiguous()
-        native.check(F._lib().b200_paged_attn_append(
+        lib = F._lib()
+        lib.b200_paged_attn_workspace.restype = _ll
+        size = lib.b200_paged_attn_workspace(B, QH, KVH, table.shape[1], _log_page(cache), D)
+        ws = torch.empty(size, dtype=torch.uint8, device=kqv.device) if size else None
+        native.check(lib.b200_paged_attn_append(
             native.ptr(kqv), *_pool_args(cache), native.ptr(table), native.ptr(lens), native.ptr(cos), native.ptr(sin), native.ptr(slopes),
-            native.ptr(out), cos.shape[0], _ll(kqv.stride(0) if B > 1 else kqv.shape[1]), B, table.shape[1], pages, QH, KVH,
+            native.ptr(out), native.ptr(ws), cos.shape[0], _ll(kqv.stride(0) if B > 1 else kqv.shape[1]), B, table.shape[1], pages, QH, KVH,
             _log_page(cache), D, HELD[cache.k.dtype], _f(scale), _f(softcap), native.stream_ptr()), "paged_attn_append")
     native.bump()
     return out
