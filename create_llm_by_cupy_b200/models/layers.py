@@ -19,6 +19,7 @@ import torch
 
 from ..ops import functional as F
 from ..ops import masked_attn as A
+from ..ops import paged as P
 
 
 def init_weight(shape, std: float, dtype, device, generator=None) -> torch.Tensor:
@@ -313,6 +314,31 @@ class GroupedQueryAttention:
         tabs = self._rope(kcache.shape[2], x.device)
         o = A.tree_attn_append(F.gemm(x, self.params[0]), kcache, vcache, lens, tree, self.QH, self.KVH, tabs[0], tabs[1], scale=self.scale,
                                softcap=self.softcap, slopes=self.slopes)
+        return F.gemm(o.view(x.shape[0], self.H), self.params[1], add=residual)
+
+    def prefill_paged(self, x, B, T, cache, table, seq, pos, residual=None, mask=None):
+        """``prefill`` into pages (``paged.PagedCache``): token i of the ``B * T`` goes to position ``pos`` [i] of sequence ``seq`` [i] (-1:
+        padding, nowhere)."""
+        kqv = F.gemm(x, self.params[0])
+        tabs = self._rope(self.T, x.device)
+        q, k, v = self._split(kqv, B, T)
+        P.paged_append(k.reshape(B * T, self.KVH, self.D), v.reshape(B * T, self.KVH, self.D), cache, table, seq, pos, *tabs)
+        F.rope_inplace(kqv, tabs[0], tabs[1], T, self.KVH + self.QH, self.D, col0=0)
+        if mask is not None or self.modified:
+            mask = A.span_mask(B, T, x.device) if mask is None else mask
+            o, _ = A.span_attn_fwd(q, k, v, mask, scale=self.scale, softcap=self.softcap, slopes=self.slopes)
+        elif self.flash_backend == "none":
+            o, _, _, _, _ = F._attn_reference(q, k, v, None, self.scale, None, None)
+            o = o.to(x.dtype).contiguous()
+        else:
+            o, _ = F.flash_attn_fwd(q, k, v, scale=self.scale, rope=None)
+        return F.gemm(o.reshape(B * T, self.H), self.params[1], add=residual)
+
+    def decode_paged(self, x, cache, table, lens, residual=None):
+        """x: [B, H] normed hidden states of one new token per sequence, at positions ``lens`` [B] (below 0: no token)."""
+        tabs = self._rope(self.T, x.device)
+        o = P.paged_attn_append(F.gemm(x, self.params[0]), cache, table, lens, self.QH, self.KVH, tabs[0], tabs[1], scale=self.scale,
+                                softcap=self.softcap, slopes=self.slopes)
         return F.gemm(o.view(x.shape[0], self.H), self.params[1], add=residual)
 
     @staticmethod

@@ -22,7 +22,9 @@ import numpy as np
 import torch
 
 from ..ops import functional as F
+from ..ops.drafts import verify_drafts
 from ..ops.masked_attn import SpanMask, span_mask, tree_mask
+from ..ops.paged import paged_cache
 from .layers import (ChunkedCrossEntropy_Share, GroupedQueryAttention, RMSNorm, SwiGLU, TimeDropout,
                      TimeEmbedding_shard, init_weight)
 from .sampling import apply_repetition_penalty, top_p_sampling
@@ -538,13 +540,95 @@ class Cupa_ver4:
         return out
 
     @torch.no_grad()
+    def generate_batch(self, prompts, start_id=None, end_id=None, padding_id=None, temp: float = 0.7, top: float = 0.9,
+                       penalty: float = 1.2, max_new_tokens: int | None = None, greedy: bool = False, seed: int | None = None,
+                       prefix: int = 0, cache: str = "bf16", page: int = 64):
+        """``generate`` for several prompts of any lengths at a time, over paged caches: one prefill pass over all of them, then one
+        pass per position. ``cache``: how K and V are held, "bf16", "int8" or "e4m3" (half the memory, and of what a pass reads); ``page``:
+        tokens of a page. Every sequence has pages for its own prompt and new tokens alone. The other arguments as in ``generate``.
+        Returns a list of token lists; a sequence is over at ``end_id``, at ``max_new_tokens``, or when its context is full."""
+        pad = self.padding_id if padding_id is None else padding_id
+        rows = [([int(start_id)] if start_id is not None else []) + [int(t) for t in prompt] for prompt in prompts]
+        if any(not r for r in rows):
+            raise ValueError("generate_batch needs at least one token of context for each sequence")
+        if not rows:
+            return []
+        Tmax, B, dev = self.time_size, len(rows), self.device
+        rows = [r[:Tmax - 1] for r in rows]
+        budget = [Tmax - len(r) if max_new_tokens is None else min(max_new_tokens, Tmax - len(r)) for r in rows]
+        gen = None
+        if seed is not None:
+            gen = torch.Generator(device=dev)
+            gen.manual_seed(seed)
+        need = [(len(r) + max(n, 1) + page - 1) // page for r, n in zip(rows, budget)]
+        table, at = torch.full((B, max(need)), -1, dtype=torch.int32), 0
+        for b, n in enumerate(need):
+            table[b, :n] = torch.arange(at, at + n, dtype=torch.int32)
+            at += n
+        table = table.to(dev)
+        caches = [paged_cache(at, self.kv_head, page, self.head_dim, dev, cache, dtype=self.dtype) for _ in range(self.layernum)]
+        W = self.Af_Em_para[0]
+        Wh = self.head_para[0] if self.head_para is not None else W
+
+        T0 = max(len(r) for r in rows)
+        sizes = torch.tensor([len(r) for r in rows], dtype=torch.int32, device=dev)
+        pos = torch.arange(T0, dtype=torch.int32, device=dev).expand(B, T0)
+        seq = torch.where(pos < sizes[:, None], torch.arange(B, dtype=torch.int32, device=dev)[:, None], -1).reshape(-1)
+        pos = pos.reshape(-1).contiguous()
+        mask = self._rows_mask(B, T0, sizes, prefix)                         # (a prefix may be longer than a prompt)
+        ids = torch.tensor([r + [r[-1]] * (T0 - len(r)) for r in rows], dtype=torch.int32, device=dev)
+        h = F.embedding_fwd(W, ids.view(-1), -1)
+        for b in range(self.layernum):
+            gqa, feed, norm1, norm2 = self.block_modules(b)
+            h = gqa.prefill_paged(norm1.forward(h, False), B, T0, caches[b], table, seq, pos, residual=h, mask=mask)
+            h = feed.forward(norm2.forward(h, False), residual=h, train_flg=False)
+        h = self.norm_.forward(h.view(B, T0, -1)[torch.arange(B, device=dev), sizes.long() - 1].contiguous(), False)
+        seen = None
+        if not greedy and penalty != 1.0:                                    # tokens that a sequence has
+            seen = torch.zeros((B, self.vocab_size), dtype=torch.bool, device=dev)
+            seen.scatter_(1, ids.long().clamp(0, self.vocab_size - 1), (ids >= 0) & (ids < self.vocab_size))
+        none = torch.zeros((B, 1), dtype=torch.int32, device=dev)
+        out, live = [[] for _ in range(B)], [n > 0 for n in budget]
+        lens = sizes
+        while any(live):
+            logits = F.gemm(h, Wh, trans_b=True, out_dtype=torch.float32)
+            if 0 <= pad < self.vocab_size:
+                logits[:, pad] = float("-inf")
+            if seen is not None:
+                logits = torch.where(seen, torch.where(logits < 0, logits * penalty, logits / penalty), logits)
+            u = torch.rand((B, 1), generator=gen, device=dev)
+            nxt = verify_drafts(logits[:, None], none, none - 1, u, temp=0.0 if greedy else max(float(temp), 1e-6), top=float(top))[0][:, 0]
+            for b, t in enumerate(nxt.tolist()):
+                if not live[b]:
+                    continue
+                if t >= 0:
+                    out[b].append(t)
+                live[b] = t >= 0 and t != end_id and len(out[b]) < budget[b]
+            if not any(live):
+                break
+            nxt = nxt.clamp_min(0)
+            if seen is not None:
+                seen.scatter_(1, nxt[:, None].long(), True)
+            at = torch.where(torch.tensor(live, device=dev), lens, -1)
+            h = F.embedding_fwd(W, nxt, -1)
+            for b in range(self.layernum):
+                gqa, feed, norm1, norm2 = self.block_modules(b)
+                h = gqa.decode_paged(norm1.forward(h, False), caches[b], table, at, residual=h)
+                h = feed.forward(norm2.forward(h, False), residual=h, train_flg=False)
+            h = self.norm_.forward(h, False)
+            lens = lens + 1
+        return out
+
+    @torch.no_grad()
     def generate_drafted(self, prompt, draft, start_id=None, end_id=None, padding_id=None, max_new_tokens: int | None = None,
-                         prefix: int = 0):
-        """Greedy decoding that checks a tree of drafted tokens per pass: the same choices as ``generate(..., greedy=True)``, in as many
-        passes as the drafts are wrong. ``draft(tokens)`` gets all tokens so far and returns proposals for those that follow as
-        (token, parent) pairs, at most 63: ``parent`` is the index of an earlier proposal of the same list, or -1 for the last token. A
-        drafted token whose predecessors were all chosen, and which the model chooses, is kept with its cached K and V. ``prefix`` as in
-        ``generate``."""
+                         prefix: int = 0, temp: float | None = None, top: float = 0.9, seed: int | None = None):
+        """Decoding that checks a tree of drafted tokens per pass. Greedy (``temp`` None): the same choices as ``generate(...,
+        greedy=True)``, in as many passes as the drafts are wrong. With a ``temp``: tokens are drawn at that temperature from the nucleus
+        ``top`` (no repetition penalty), whatever the drafts are. ``draft(tokens)`` gets all tokens so far and returns proposals for those
+        that follow as (token, parent) pairs, at most 63: ``parent`` is the index of an earlier proposal of the same list, or -1 for the
+        last token. When tokens are drawn it may return (proposals, probs) instead: row i + 1 of ``probs`` [proposals + 1, vocabulary] is
+        the distribution that the children of proposal i were drawn from, row 0 that of the last token's. A drafted token whose
+        predecessors were all chosen, and which the model chooses, is kept with its cached K and V. ``prefix`` as in ``generate``."""
         pad = self.padding_id if padding_id is None else padding_id
         toks = ([int(start_id)] if start_id is not None else []) + [int(p) for p in prompt]
         if not toks:
@@ -558,11 +642,36 @@ class Cupa_ver4:
         W = self.Af_Em_para[0]
         Wh = self.head_para[0] if self.head_para is not None else W
 
-        def choose(h):
+        gen = None
+        if seed is not None:
+            gen = torch.Generator(device=dev)
+            gen.manual_seed(seed)
+
+        def logits_of(h):
             logits = F.gemm(self.norm_.forward(h, False), Wh, trans_b=True, out_dtype=torch.float32)
             if 0 <= pad < self.vocab_size:
                 logits[:, pad] = float("-inf")
-            return torch.argmax(logits, -1).tolist()
+            return logits
+
+        def walk(h, ids, parents, probs):
+            """(tokens that are chosen one after the other, nodes of the tree that the text goes through behind its root)"""
+            logits, n = logits_of(h), len(ids)
+            if temp is None:
+                best, tokens, path = torch.argmax(logits, -1).tolist(), [], [0]
+                while True:                                                  # down the tree as far as the drafts are right
+                    tokens.append(best[path[-1]])
+                    child = next((i for i in range(1, n) if parents[i] == path[-1] and ids[i] == tokens[-1]), None)
+                    if child is None:
+                        return tokens, path[1:]
+                    path.append(child)
+            u = torch.rand((2, 1, n), generator=gen, device=dev)
+            if probs is not None:
+                probs = torch.as_tensor(probs, dtype=torch.float32, device=dev).view(1, n, self.vocab_size).contiguous()
+            tok, par = (torch.tensor([x], dtype=torch.int32, device=dev) for x in (ids, parents))
+            tokens, path, count = verify_drafts(logits[None], tok, par, u[0], temp=float(temp), top=float(top), draft_probs=probs,
+                                                accept=None if probs is None else u[1])
+            kept = int(count[0])
+            return tokens[0, :kept + 1].tolist(), path[0, :kept].tolist()
 
         mask = self._rows_mask(1, len(toks), None, prefix)
         h = F.embedding_fwd(W, torch.tensor(toks, dtype=torch.int32, device=dev), -1)
@@ -572,10 +681,18 @@ class Cupa_ver4:
             h = feed.forward(norm2.forward(h, False), residual=h, train_flg=False)
         out, cached = [], len(toks)
         if budget > 0:
-            out.append(choose(h[-1:])[0])
+            out += [t for t in walk(h[-1:], [toks[-1]], [-1], None)[0] if t >= 0]
         while 0 < len(out) < budget and (end_id is None or out[-1] != end_id) and cached < Tmax - 1:
             room = min(64, Tmax - cached)
-            proposals = [(int(t), int(p)) for t, p in list(draft(toks + out))[:room - 1]]
+            proposals, probs = draft(toks + out), None
+            if isinstance(proposals, tuple) and len(proposals) == 2 and isinstance(proposals[1], (torch.Tensor, np.ndarray)):
+                proposals, probs = proposals
+                if temp is None:
+                    raise ValueError("generate_drafted: probabilities of drafts are for tokens that are drawn (temp)")
+                if tuple(probs.shape) != (len(proposals) + 1, self.vocab_size):
+                    raise ValueError("generate_drafted: probabilities of drafts are [proposals + 1, vocabulary]")
+                probs = probs[:room]
+            proposals = [(int(t), int(p)) for t, p in list(proposals)[:room - 1]]
             if any(not -1 <= p < i for i, (_, p) in enumerate(proposals)):
                 raise ValueError("generate_drafted: a proposal's parent stands before it, or is -1")
             ids = [out[-1]] + [t for t, _ in proposals]                          # the last token, which is not cached yet, is the root
@@ -586,15 +703,16 @@ class Cupa_ver4:
                 gqa, feed, norm1, norm2 = self.block_modules(b)
                 h = gqa.decode_drafts(norm1.forward(h, False), tree, kc[b], vc[b], lens, residual=h)
                 h = feed.forward(norm2.forward(h, False), residual=h, train_flg=False)
-            best, path = choose(h), [0]
-            while True:                                                          # down the tree as far as the drafts are right
-                out.append(best[path[-1]])
-                if len(out) >= budget or (end_id is not None and out[-1] == end_id):
+            chosen, nodes = walk(h, ids, parents, probs)
+            path, over = [0], False
+            for j, t in enumerate(chosen):
+                if t < 0:
+                    over = True
                     break
-                child = next((i for i in range(1, len(ids)) if parents[i] == path[-1] and ids[i] == out[-1]), None)
-                if child is None:
+                out.append(t)
+                if len(out) >= budget or (end_id is not None and t == end_id):
                     break
-                path.append(child)
+                path += nodes[j:j + 1]
             moved = [i for j, i in enumerate(path) if i != j]
             if moved:                                                            # their rows to where the tokens stand now
                 src = torch.tensor([cached + i for i in moved], device=dev)
@@ -602,6 +720,8 @@ class Cupa_ver4:
                 for c in kc + vc:
                     c[:, :, at:at + len(moved)] = c[:, :, src]
             cached += len(path)
+            if over:                                                         # a row with no token to choose
+                break
         return out
 
     def chat_generate(self, prompt, user_id, bot_id, end_id, padding_id=None, **kw):

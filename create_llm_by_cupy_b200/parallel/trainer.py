@@ -378,11 +378,18 @@ class Trainer:
 
     def generate(self, prompt, **kw):
         """Generation on a sharded model: gather everything, decode, release."""
+        return self._resident(lambda: self.model.generate(prompt, **kw))
+
+    def generate_batch(self, prompts, **kw):
+        """The same for several prompts at a time (``Cupa_ver4.generate_batch``)."""
+        return self._resident(lambda: self.model.generate_batch(prompts, **kw))
+
+    def _resident(self, call):
         self.flush_delayed_update()
         self.join_optimizer()
         self.manager.materialize_all()
         try:
-            return self.model.generate(prompt, **kw)
+            return call()
         finally:
             self.manager.release_all()
 
