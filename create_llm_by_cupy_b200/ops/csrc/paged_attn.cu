@@ -11,6 +11,7 @@
 namespace b200 {
 namespace cg = cooperative_groups;
 
+constexpr int PA_CLUSTER = 8;        // CTAs of a cluster, at most
 constexpr int PA_WARPS = 4, PA_THREADS = 32 * (PA_WARPS + 1);
 constexpr int PA_HEADS = 4;          // query heads of a CTA: columns 0..3 of a product hold them, columns 4..7 what their rounding left
 constexpr int kScorePlain = 0, kScoreCap = 1, kScoreBias = 2;
@@ -567,13 +568,22 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
     cluster.sync();
     for (int i = rank * PA_THREADS + threadIdx.x; i < heads * D; i += cs * PA_THREADS) {
       const int r = i / D;
-      float m = -INFINITY, l = 0.f, x = 0.f;
-      for (int c = 0; c < cs; ++c) m = fmaxf(m, *cluster.map_shared_rank(cm + r, c));
+      float m = -INFINITY, l = 0.f, x = 0.f, ms[PA_CLUSTER], ls[PA_CLUSTER], xs[PA_CLUSTER];
+#pragma unroll
+      for (int c = 0; c < PA_CLUSTER; ++c) {                 // all reads on their way at a time: they take 700 cycles each
+        const int from = min(c, cs - 1);
+        ms[c] = *cluster.map_shared_rank(cm + r, from);
+        ls[c] = *cluster.map_shared_rank(cl + r, from);
+        xs[c] = *cluster.map_shared_rank(co + i, from);
+      }
+#pragma unroll
+      for (int c = 0; c < PA_CLUSTER; ++c) m = fmaxf(m, ms[c]);
       const float ref = m == -INFINITY ? 0.f : m;
-      for (int c = 0; c < cs; ++c) {
-        const float f = exp2_of(*cluster.map_shared_rank(cm + r, c) - ref);
-        l = fmaf(*cluster.map_shared_rank(cl + r, c), f, l);
-        x = fmaf(*cluster.map_shared_rank(co + i, c), f, x);
+#pragma unroll
+      for (int c = 0; c < PA_CLUSTER; ++c) {
+        const float f = c < cs ? exp2_of(ms[c] - ref) : 0.f;
+        l = fmaf(ls[c], f, l);
+        x = fmaf(xs[c], f, x);
       }
       p.out[((long long)b * p.QH + h0) * D + i] = __float2bfloat16(l == 0.f ? 0.f : x / l);
     }
@@ -590,6 +600,7 @@ __global__ void __launch_bounds__(D) paged_join_kernel(const PagedAttnParams p) 
   const float2* ml = p.part_ml + (long long)blockIdx.x * p.pieces;
   const float* o = p.part_o + (long long)blockIdx.x * p.pieces * D + d;
   float m = -INFINITY, l = 0.f, x = 0.f;
+#pragma unroll 8
   for (int c = 0; c < p.pieces; ++c) m = fmaxf(m, ml[c].x);
   const float ref = m == -INFINITY ? 0.f : m;
 #pragma unroll 8
@@ -607,9 +618,9 @@ static int paged_groups(int QH, int KVH) { return (QH / KVH + PA_HEADS - 1) / PA
 static int2 paged_split(int B, int QH, int KVH, int width, int log_page) {
   const long long units = (long long)B * KVH * paged_groups(QH, KVH), slots = 3LL * num_sms(), tokens = (long long)width << log_page;
   const long long most = std::max(1LL, tokens / 256);
-  if (units * 8 <= slots / 2 && most > 8) return make_int2(1, int(std::min(slots / units, most)));
+  if (units * PA_CLUSTER <= slots / 2 && most > PA_CLUSTER) return make_int2(1, int(std::min(slots / units, most)));
   int cs = 1;
-  while (cs < 8 && 2 * cs * units <= slots && cs < most) cs *= 2;
+  while (cs < PA_CLUSTER && 2 * cs * units <= slots && cs < most) cs *= 2;
   return make_int2(cs, 0);
 }
 
