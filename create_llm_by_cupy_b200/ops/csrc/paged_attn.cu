@@ -45,7 +45,7 @@ struct PA {
   static constexpr int kMat = kTile * kRow;                          // bytes of a tile of K, or of V
   static constexpr int kStage = 2 * kMat + 2 * kTile * 4;            // and the scales
   static constexpr int kStages = D == 128 ? 2 : 4;
-  static constexpr int kWarp = kStages * kStage + kTile * 16;        // a warp's ring, and numbers of a tile's tokens
+  static constexpr int kWarp = kStages * kStage;                     // a warp's ring
   static constexpr int kPart = (2 + D) * PA_HEADS * 4;               // maxima, sums, values of the heads
   static constexpr int kOwn = PA_WARPS * kWarp;                      // those of the new token
   static constexpr int kSmem = kOwn + kPart;
@@ -60,10 +60,10 @@ struct PA {
 };
 
 // 16 or 4 bytes on their way to shared memory, or zeros in their place.
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there) {
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there = true) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(there ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool there) {
+__device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool there = true) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(there ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
@@ -156,7 +156,6 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
   uint8_t* mine = smem + warp * L::kWarp;
-  float4* numbers = reinterpret_cast<float4*>(mine + kStages * L::kStage);
   pdl_wait();
   pdl_trigger();
 
@@ -170,9 +169,12 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
   const int nt = (len + kTile - 1) / kTile, step = cs * PA_WARPS, first = rank * PA_WARPS + warp;
   const int count = warp == PA_WARPS || pos < 0 || first >= nt ? 0 : (nt - first + step - 1) / step;
 
-  // Tiles are asked for kStages ahead, with loads of their own of all lanes: bulk copies brought an SM no more than 15 bytes a cycle,
-  // two thirds of its share of HBM. The pages of 32 tiles are looked up at a time, a lane each.
+  // Tiles are asked for kStages ahead, by the lanes themselves (bulk copies took as long, and leave the bytes in the order that they come
+  // in). The pages of 32 tiles are looked up at a time, a lane each.
   const int* table = p.c.table + (long long)b * p.c.width;
+  uint32_t lane_place[4];                                    // of this lane's 16 bytes of every 512
+#pragma unroll
+  for (int x = 0; x < 4; ++x) lane_place[x] = L::place(512 * x + lane * 16) - 512 * x;
   int pages = -1;
   uint32_t skipped = 0;                                      // bit i % 32: tile i has no page
   auto ask = [&](int i) {
@@ -189,16 +191,28 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
         const long long row = (((long long)pg * p.c.KVH + kvh) << p.c.log_page) + (t0 & (p.c.page() - 1));
         const uint8_t* k = static_cast<const uint8_t*>(p.c.k) + row * kRow + lane * 16;
         const uint8_t* v = static_cast<const uint8_t*>(p.c.v) + row * kRow + lane * 16;
+        if (bytes == L::kMat) {
 #pragma unroll
-        for (int x = 0; x < L::kMat; x += 512) cp_async16(st + L::place(x + lane * 16), k + (x + lane * 16 < bytes ? x : 0), x + lane * 16 < bytes);
-        if constexpr (kHeld != kHeldBf16) {
-          const bool has = lane * kRow < bytes;
-          cp_async4(st + 2 * L::kMat + lane * 4, p.c.ks + row + (has ? lane : 0), has);
-          cp_async4(st + 2 * L::kMat + kTile * 4 + lane * 4, p.c.vs + row + (has ? lane : 0), has);
+          for (int x = 0; x < L::kMat; x += 512) cp_async16(st + x + lane_place[x >> 9 & 3], k + x);
+          if constexpr (kHeld != kHeldBf16) {
+            cp_async4(st + 2 * L::kMat + lane * 4, p.c.ks + row + lane);
+            cp_async4(st + 2 * L::kMat + kTile * 4 + lane * 4, p.c.vs + row + lane);
+          }
+#pragma unroll
+          for (int x = 0; x < L::kMat; x += 512) cp_async16(st + L::kMat + x + lane_place[x >> 9 & 3], v + x);
+        } else {                                             // zeros behind the last token
+#pragma unroll
+          for (int x = 0; x < L::kMat; x += 512) {
+            const bool has = x + lane * 16 < bytes;
+            cp_async16(st + x + lane_place[x >> 9 & 3], has ? k + x : k, has);
+            cp_async16(st + L::kMat + x + lane_place[x >> 9 & 3], has ? v + x : v, has);
+          }
+          if constexpr (kHeld != kHeldBf16) {
+            const bool has = lane * kRow < bytes;
+            cp_async4(st + 2 * L::kMat + lane * 4, p.c.ks + row + (has ? lane : 0), has);
+            cp_async4(st + 2 * L::kMat + kTile * 4 + lane * 4, p.c.vs + row + (has ? lane : 0), has);
+          }
         }
-#pragma unroll
-        for (int x = 0; x < L::kMat; x += 512)
-          cp_async16(st + L::kMat + L::place(x + lane * 16), v + (x + lane * 16 < bytes ? x : 0), x + lane * 16 < bytes);
       }
     }
     cp_async_commit();
@@ -359,14 +373,6 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
     cp_async_wait<kStages - 1>();
     __syncwarp();
     if (!(skipped >> (i & 31) & 1)) {
-      if constexpr (kHeld != kHeldBf16) {
-        // a token's numbers: what its products are multiplied with, log2 of V's scale, and one over it
-        const float* sc = reinterpret_cast<const float*>(st + 2 * L::kMat);
-        const bool has = lane < rows;
-        const float ks = has ? sc[lane] : 0.f, vs = has ? sc[kTile + lane] : 1.f;
-        numbers[lane] = make_float4(ks, has ? __log2f(vs) : 0.f, __fdividef(1.f, vs), 0.f);
-      }
-      __syncwarp();
       // Scores: tokens are the rows of the products, 16 at a time.
       constexpr int kMt = kTile / 16;
       float acc[kMt][4];
@@ -416,10 +422,12 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
         float ks = 1.f, more = 0.f;
         rv[n] = 1.f;
         if constexpr (kHeld != kHeldBf16) {
-          const float4 u = numbers[tok];
-          ks = u.x;
-          more = u.y;
-          rv[n] = u.z;
+          // a token's scales: V's as its logarithm, which goes into the weight, and as its reciprocal, for the sum of weights without it
+          const float* scales = reinterpret_cast<const float*>(st + 2 * L::kMat);
+          const float vs = fmaxf(scales[kTile + tok], kLeastScale);
+          ks = scales[tok];
+          more = __log2f(vs);
+          rv[n] = __fdividef(1.f, vs);
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {

@@ -167,9 +167,10 @@ def test_rows_of_any_pitch_and_extreme_rows(kind):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("QH,KVH", [(12, 4), (32, 8), (3, 3), (16, 1), (20, 2)])
-def test_token(kind, D, QH, KVH):
+@pytest.mark.parametrize("room", [1, 20])                    # tables of 320 tokens: clusters; of 928: CTAs that stay
+def test_token(kind, D, QH, KVH, room):
     lens = [0, 1, 15, 16, 31, 32, 33, 127, 128, 300, -1]
-    cache, table, *_, cos, sin = filled(kind, lens, KVH, D, 32, seed=QH)
+    cache, table, *_, cos, sin = filled(kind, lens, KVH, D, 32, seed=QH, room=room)
     kqv = (torch.randn(len(lens), (2 * KVH + QH) * D, generator=torch.Generator().manual_seed(1)) * 1.5).to(torch.bfloat16).to(DEV)
     o = P.paged_attn_append(kqv, cache, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), QH, KVH, cos, sin)
     check_token(cache, table, kqv, o, lens, QH, KVH, D)
@@ -190,7 +191,7 @@ def test_token_with_modified_scores(kind, mod, D):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("B,hi,page", [(1, 9000, 128), (3, 4100, 256), (40, 260, 32), (150, 70, 64)])
+@pytest.mark.parametrize("B,hi,page", [(1, 9000, 128), (3, 4100, 256), (1, 1, 1024), (40, 260, 32), (40, 700, 32), (150, 70, 64), (700, 40, 1024)])
 def test_token_of_long_and_of_many_sequences(kind, B, hi, page):
     QH, KVH, D = 16, 4, 128
     lens = [hi - 61 * b % hi for b in range(B)]
@@ -202,9 +203,10 @@ def test_token_of_long_and_of_many_sequences(kind, B, hi, page):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-def test_pages_that_are_not_there(kind):
+@pytest.mark.parametrize("room", [1, 20])
+def test_pages_that_are_not_there(kind, room):
     QH, KVH, D, page, lens = 8, 2, 128, 32, [200, 200, 95, 64]
-    cache, table, *_, cos, sin = filled(kind, lens, KVH, D, page, room=1)
+    cache, table, *_, cos, sin = filled(kind, lens, KVH, D, page, room=room)
     table[0, 1], table[0, 3], table[1, :] = -1, cache.k.shape[0], -7
     table[2, 2] = 2 ** 31 - 1                                # a page that the new token would be written to
     kqv = (torch.randn(4, (2 * KVH + QH) * D) * 1.5).to(torch.bfloat16).to(DEV)
