@@ -780,7 +780,7 @@ PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!on(*x, dev) || (x->scalar_type() != at::kFloat && x->scalar_type() != at::kBFloat16) || x->dim() != 3 || !x->is_contiguous())
     Py_RETURN_NONE;
   const int64_t B = x->size(0), nodes = x->size(1), V = x->size(2);
-  if (!fits(B) || nodes < 1 || nodes > 64 || !fits(V) || V > 8 * 376 * 128 || !(temp == 0. || temp >= 1e-6) || !std::isfinite(temp) ||
+  if (!fits(B) || nodes < 1 || nodes > 64 || !fits(V) || V > 8 * 376 * 128 || !(temp == 0. || (temp >= 1e-6 && temp <= 1e6)) ||
       !(top > 0.))
     Py_RETURN_NONE;
   for (const Tensor* t : {tok, par, u, acc})

@@ -1,4 +1,24 @@
 // Attention of one new token of each sequence over a paged cache (paged_cache.cuh), with the token's rotation and append.
+//
+//   o = sum_j p_j v_j / sum_j p_j,   p_j = 2^(s_j - m),   s_j = score(scale q . k_j) log2 e
+//
+// What bounds it: each cached row is read once, 2 D + 8 bytes a token and KV head in 8 bits, so HBM, if an SM gets through its tiles fast
+// enough: 3500 cycles for a tile of 32 tokens with twelve warps on an SM, 29 bytes a cycle where HBM has 24 for each SM. Hence:
+//   * products by mma.sync with the TOKENS (dims, for the values) as rows and the heads as columns. Columns 0 to 3 are the four query heads
+//     of the CTA, columns 4 to 7 what rounding left of them: scores and weights go in as two 16-bit parts at no further product. With the
+//     heads as rows (8 and 8 of 16) it were twice the products and accumulators: 107 -> 90 us for 64 x 1500 to 4000 tokens, 32 / 8 heads of
+//     128, int8. (A tcgen05 tile has 128 rows, of which four heads would fill four.)
+//   * 8-bit rows become exact fp16 in registers (no rounding before the products); K's scale multiplies the score; V's joins the weight as a
+//     logarithm: w_j = 2^(s_j + log2 sv_j - M), M the running maximum of that sum, and the sum of the weights without it is that of
+//     w_j / sv_j. The largest weight is held as 2^14, so that fp16 has 2^-38 of it to show for a small one.
+//   * a dot product does not care in which order its dims are walked: a lane's 16-byte pieces of K are fragments as they stand. V needs
+//     pairs of tokens: two byte permutations for four dims. Weights are turned over by movmatrix.
+//   * tiles go through a ring per warp, so warps never wait for one another until the end. Three CTAs an SM.
+//   * few sequences: clusters of up to eight CTAs share one (or, where 8 leave SMs idle, pieces that a second kernel joins: one sequence of
+//     60001 tokens 81 us with clusters of 8, 54 of 16, 41 with 55 pieces).
+// Tried and not kept: bulk copies by a warp of their own (no faster: the time is that of the arithmetic), one list of all tiles cut evenly
+// over CTAs that stay (64 x 1500 to 4000 tokens 88 -> 93 us, 32 x 0 to 1980 21 -> 40: the start of a stretch takes as long as four tiles,
+// and its state does not fit in the registers of three CTAs an SM).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -234,7 +254,7 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
     for (int i = 0; i < D / 4; ++i) m = fmaxf(m, fabsf(q[i]));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const int e = min(max(int(__float_as_uint(m) >> 23) - 127, -100), 100);
+    const int e = max(int(__float_as_uint(m) >> 23) - 127, -116);
     const float up = __uint_as_float(uint32_t(127 + 10 - e) << 23);
     row_mul = __uint_as_float(uint32_t(127 - 10 + e) << 23);
 #pragma unroll
@@ -622,7 +642,9 @@ __global__ void __launch_bounds__(D) paged_join_kernel(const PagedAttnParams p) 
 
 static int paged_groups(int QH, int KVH) { return (QH / KVH + PA_HEADS - 1) / PA_HEADS; }
 
-// CTAs that share a sequence and KV head: {size of their cluster, 0}, or {1, pieces}.
+// CTAs that share a sequence and KV head: {size of their cluster, 0}, or {1, pieces}. Clusters double while all still run at once (three CTAs
+// an SM) and hold 256 tokens a CTA: 32 x 0 to 1980 tokens, 16 / 4 heads, 21 us with two, 26 with one, 23 with four. Pieces where clusters of
+// eight would fill less than half of the GPU; at other numbers of sequences they are no better (two of 64 x 1500 to 4000: 86 us for 88).
 static int2 paged_split(int B, int QH, int KVH, int width, int log_page) {
   const long long units = (long long)B * KVH * paged_groups(QH, KVH), slots = 3LL * num_sms(), tokens = (long long)width << log_page;
   const long long most = std::max(1LL, tokens / 256);

@@ -10,6 +10,14 @@
 // Every node is decided by itself, by a cluster of CTAs that share its row, the row in shared memory; a second kernel walks the trees.
 // Weights are fp64, and sums are sums of integers (2^62 / columns to the largest weight): which token a number falls on depends on the
 // whole row's sum, and integers add up to the same in any order.
+//
+// What bounds it: a row of 32000 logits is 128 KB, 3 us of an SM's share of HBM, and 32000 fp64 exponentials, which take 9; but the chain
+// of a node is about 45000 cycles (25 us) long whatever its slices are: largest logit, weights, the bin, the tokens of the bin, the sums, the
+// draw, each of them once over the row and once through the cluster. So slices are as large as two CTAs an SM hold, and where there are more
+// nodes than clusters, node 0 of all sequences comes first, then node 1: most of the later ones are out of question by then and passed
+// over. Us, 6 nodes of one sequence (probabilities of the drafts, nucleus) / 8 x 24 (the same, no nucleus) / 16 x 63 (looked up,
+// nucleus), 32000 tokens: bits of the nucleus' end one by one 267 / 122 / 1709, histogram 30 / 45 / 417, its search in two steps and
+// nodes passed over 23 / 60 / 83. (CTAs that read one another's whole histograms took 17000 cycles for it.)
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
@@ -683,7 +691,7 @@ using namespace b200;
 B200_API int b200_verify_drafts(const void* logits, const void* q, const void* tokens, const void* parents, const void* u,
                                 const void* accept, void* out, void* path, void* count, void* workspace, int is_bf16, int B, int n, int V,
                                 double temp, double top, cudaStream_t st) {
-  if (B < 0 || n < 1 || n > VD_MAX_NODES || V < 1 || !(temp >= 0.) || !(top > 0.) || (q == nullptr) != (accept == nullptr))
+  if (B < 0 || n < 1 || n > VD_MAX_NODES || V < 1 || !(temp == 0. || (temp >= 1e-6 && temp <= 1e6)) || !(top > 0.) || (q == nullptr) != (accept == nullptr))
     return static_cast<int>(cudaErrorInvalidValue);
   if (B == 0) return 0;
   VerifyParams p;
@@ -698,7 +706,7 @@ B200_API int b200_verify_drafts(const void* logits, const void* q, const void* t
   p.rows = (long long)B * n;
   p.n = n; p.V = V;
   p.inv_temp = temp > 0. ? 1. / temp : 0.;
-  p.reach = float(std::min(699. * temp, 3e38));
+  p.reach = float(699. * temp);
   p.top = 0;
   p.top_shift = 0;
   if (top < 1.) {

@@ -27,7 +27,7 @@ def verify_drafts(logits, tokens, parents, u, *, temp: float = 1.0, top: float =
     may be ragged. ``u`` fp32 [B, n]: numbers from [0, 1), for the draw behind each node.
 
     A node's probabilities p are the softmax of its logits / ``temp`` over its nucleus, the fewest tokens, by falling probability and
-    rising index, whose mass reaches ``top``. ``temp`` = 0 leaves the largest logit, of several the one of the lowest index. Logits of
+    rising index, whose mass reaches ``top``. ``temp`` is from 1e-6 to 1e6, or 0, which leaves the largest logit, of several the one of the lowest index. Logits of
     -infinity and NaN count for nothing, +infinity for the largest number.
 
     Without ``draft_probs`` the token behind a node is the first whose sum of probabilities, in the order of the tokens, exceeds u; if a
@@ -60,10 +60,8 @@ def verify_drafts(logits, tokens, parents, u, *, temp: float = 1.0, top: float =
                                     tuple(accept.shape) != (B, n) or accept.dtype != torch.float32):
         raise ValueError("verify_drafts: draft_probs is float32 [B, n, V], accept float32 [B, n]")
     temp, top = float(temp), float(top)
-    if not (temp >= 0.0 and math.isfinite(temp)) or not top > 0.0:
-        raise ValueError("verify_drafts: temp is a number from 0 on, top is more than 0")
-    if 0.0 < temp < 1e-6:
-        raise ValueError("verify_drafts: temp is 0, or at least 1e-6")
+    if not (temp == 0.0 or 1e-6 <= temp <= 1e6) or not top > 0.0:
+        raise ValueError("verify_drafts: temp is 0 or from 1e-6 to 1e6, top is more than 0")
     if any(t is not None and t.device != logits.device for t in (tokens, parents, u, draft_probs, accept)):
         raise ValueError("verify_drafts: all tensors are on one device")
     if not logits.is_cuda:

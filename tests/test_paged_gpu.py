@@ -167,7 +167,7 @@ def test_rows_of_any_pitch_and_extreme_rows(kind):
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("D", [64, 128])
 @pytest.mark.parametrize("QH,KVH", [(12, 4), (32, 8), (3, 3), (16, 1), (20, 2)])
-@pytest.mark.parametrize("room", [1, 20])                    # tables of 320 tokens: clusters; of 928: CTAs that stay
+@pytest.mark.parametrize("room", [1, 20])                    # tables of 320 tokens, and of 928: larger clusters
 def test_token(kind, D, QH, KVH, room):
     lens = [0, 1, 15, 16, 31, 32, 33, 127, 128, 300, -1]
     cache, table, *_, cos, sin = filled(kind, lens, KVH, D, 32, seed=QH, room=room)
@@ -203,7 +203,22 @@ def test_token_of_long_and_of_many_sequences(kind, B, hi, page):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("room", [1, 20])
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("mod", ["", "cap", "bias"])
+def test_token_in_pieces(kind, D, mod):
+    """Few sequences with room for many tokens: empty ones, one that is none, short and long ones; four groups of heads."""
+    QH, KVH, lens = 16, 1, [0, 5, -1, 2600]
+    cache, table, *_, cos, sin = filled(kind, lens, KVH, D, 64)
+    kqv = (torch.randn(4, (2 * KVH + QH) * D, generator=torch.Generator().manual_seed(2)) * 1.5).to(torch.bfloat16).to(DEV)
+    slopes = torch.tensor([2.0 ** (-(h + 1) / 2) for h in range(QH)], device=DEV) if mod == "bias" else None
+    cap = 20.0 if mod == "cap" else 0.0
+    o = P.paged_attn_append(kqv, cache, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), QH, KVH, cos, sin, softcap=cap,
+                            slopes=slopes)
+    check_token(cache, table, kqv, o, lens, QH, KVH, D, cap, None if slopes is None else slopes.cpu())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("room", [1, 80])                    # clusters, and pieces that another kernel joins
 def test_pages_that_are_not_there(kind, room):
     QH, KVH, D, page, lens = 8, 2, 128, 32, [200, 200, 95, 64]
     cache, table, *_, cos, sin = filled(kind, lens, KVH, D, page, room=room)
@@ -216,6 +231,27 @@ def test_pages_that_are_not_there(kind, room):
     check_token(cache, table, kqv, o, lens, QH, KVH, D, cos_rows=64)
     o = P.paged_attn_append(kqv, cache, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), QH, KVH, cos, sin)
     check_token(cache, table, kqv, o, lens, QH, KVH, D)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", [1e-30, 1e30])
+def test_queries_of_any_magnitude(kind, size):
+    """Scores of 0, or as large as numbers go, where the weight is one token's: the scale brings them back."""
+    QH, KVH, D, lens = 4, 1, 128, [70]
+    cache, table, *_, cos, sin = filled(kind, lens, KVH, D, 32)
+    kqv = torch.randn(1, (2 * KVH + QH) * D, generator=torch.Generator().manual_seed(5))
+    kqv[:, KVH * D:(KVH + QH) * D] *= size
+    kqv = kqv.to(DEV, torch.bfloat16)
+    scale = 1e-18 if size > 1 else 1e18
+    o = P.paged_attn_append(kqv, cache, table.to(DEV), torch.tensor(lens, dtype=torch.int32, device=DEV), QH, KVH, cos, sin, scale=scale)
+    k, v, _ = O.cached(cache, table, 0, 71)
+    q = O.rotated(kqv.cpu()[0].view(2 * KVH + QH, D)[KVH:KVH + QH], 70)
+    want = O.attend(q, k, v, 70, torch.arange(71), scale)
+    x = k[:, 0] @ q.T * scale                                # scores of 10^12 apart from one another, or of nothing
+    clear = (x.topk(2, 0).values.diff(dim=0).abs()[0] > 1e-3 * x.abs().max()) | (x.abs().max() < 1e-6)
+    tol = 2.0 ** -8 * want.abs() + 2.0 ** -14 * v.abs().max()
+    assert bool(torch.isfinite(o).all()) and bool(clear.any())
+    assert bool(((o[0].cpu().double() - want).abs() <= tol)[clear].all())
 
 
 @pytest.mark.parametrize("kind", ["int8", "e4m3"])

@@ -86,7 +86,7 @@ def test_refusals():
     good = dict(logits=logits, tokens=tokens, parents=parents, u=u, temp=1.0, top=1.0)
     verify_drafts(**good)
     for bad in (dict(logits=logits[0]), dict(logits=logits.expand(2, 4, 9)[:, :, :0]), dict(tokens=tokens.long()), dict(parents=parents[:1]),
-                dict(u=u.double()), dict(temp=-1.0), dict(temp=math.nan), dict(temp=math.inf), dict(temp=1e-9), dict(top=0.0), dict(top=math.nan),
+                dict(u=u.double()), dict(temp=-1.0), dict(temp=math.nan), dict(temp=math.inf), dict(temp=1e-9), dict(temp=2e6), dict(top=0.0), dict(top=math.nan),
                 dict(draft_probs=q), dict(accept=a), dict(draft_probs=q.double(), accept=a), dict(draft_probs=q, accept=a[:, :2])):
         with pytest.raises(ValueError):
             verify_drafts(**{**good, **bad})

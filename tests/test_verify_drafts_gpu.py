@@ -30,6 +30,16 @@ def test_against_the_definition(dtype, temp, top, drawn):
               O.verify(x, tokens, parents, u, temp, top, q if drawn else None, accept))
 
 
+@pytest.mark.parametrize("temp", [1e-6, 1e-3, 50.0, 1e6])
+def test_extreme_temperatures(temp):
+    """From the largest logit alone to all tokens alike, with logits that are far apart and large."""
+    x, tokens, parents, u, q, accept = tree(3, 5, 900, 4, spread=30.0)
+    x[1] += 1e4
+    for top in (1.0, 0.7):
+        check(run(x, tokens, parents, u, temp=temp, top=top), O.verify(x, tokens, parents, u, temp, top))
+        check(run(x, tokens, parents, u, q, accept, temp=temp, top=top), O.verify(x, tokens, parents, u, temp, top, q, accept))
+
+
 @pytest.mark.parametrize("V", [32000, 60001, 120000, 8 * 376 * 128])
 @pytest.mark.parametrize("top", [1.0, 0.9])
 @pytest.mark.parametrize("drawn", [False, True])
