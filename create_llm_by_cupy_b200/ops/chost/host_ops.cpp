@@ -65,8 +65,8 @@ struct Api {
                       int, int, int, int, int, stream_t);
   int (*paged_read)(void*, void*, void*, void*, cptr, cptr, cptr, void*, void*, int, int, int, int, int, int, int, int, stream_t);
   long long (*paged_attn_workspace)(int, int, int, int, int, int);
-  int (*paged_attn_append)(cptr, void*, void*, void*, void*, cptr, cptr, cptr, cptr, cptr, void*, void*, int, long long, int, int, int, int, int,
-                           int, int, int, float, float, stream_t);
+  int (*paged_attn_append)(cptr, void*, void*, void*, void*, cptr, cptr, cptr, cptr, cptr, void*, void*, int, long long, int, int, int, int,
+                           int, int, int, int, float, float, stream_t);
   int (*verify_drafts)(cptr, cptr, cptr, cptr, cptr, cptr, void*, void*, void*, void*, int, int, int, int, double, double, stream_t);
 };
 Api api;
@@ -672,8 +672,8 @@ bool pool(PyObject* const* a, int dev, Pool* p) {
   if (p->log_page > 10) return false;
   if ((p->held != 0) != (ks != nullptr) || (ks != nullptr) != (vs != nullptr)) return false;
   for (const Tensor* s : {ks, vs})
-    if (s && (!on(*s, dev) || s->scalar_type() != at::kFloat || s->dim() != 3 || !s->is_contiguous() || s->sizes() != k->sizes().slice(0, 3) ||
-              !aligned16(s->const_data_ptr())))
+    if (s && (!on(*s, dev) || s->scalar_type() != at::kFloat || s->dim() != 3 || !s->is_contiguous() ||
+              s->sizes() != k->sizes().slice(0, 3) || !aligned16(s->const_data_ptr())))
       return false;
   if (!on(*table, dev) || table->scalar_type() != at::kInt || table->dim() != 2 || !table->is_contiguous()) return false;
   p->B = table->size(0), p->width = table->size(1);
@@ -763,8 +763,8 @@ PyObject* paged_attn(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (launched([&] {
         return api.paged_attn_append(x->const_data_ptr(), p.k, p.v, p.ks, p.vs, p.table, lens->const_data_ptr(), c->const_data_ptr(),
                                      s->const_data_ptr(), sl ? sl->const_data_ptr() : nullptr, out.mutable_data_ptr(),
-                                     ws ? ws->mutable_data_ptr() : nullptr, int(c->size(0)), x->stride(0), int(p.B), int(p.width), int(p.pages), QH, KVH, p.log_page, int(p.D), p.held,
-                                     float(scale), float(cap), stream(dev));
+                                     ws ? ws->mutable_data_ptr() : nullptr, int(c->size(0)), x->stride(0), int(p.B), int(p.width),
+                                     int(p.pages), QH, KVH, p.log_page, int(p.D), p.held, float(scale), float(cap), stream(dev));
       }))
     return wrap(out);
   END
@@ -784,8 +784,8 @@ PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
       !(top > 0.))
     Py_RETURN_NONE;
   for (const Tensor* t : {tok, par, u, acc})
-    if (t && (!on(*t, dev) || t->scalar_type() != (t == u || t == acc ? at::kFloat : at::kInt) || t->sizes() != at::IntArrayRef({B, nodes}) ||
-              !t->is_contiguous()))
+    if (t && (!on(*t, dev) || t->scalar_type() != (t == u || t == acc ? at::kFloat : at::kInt) ||
+              t->sizes() != at::IntArrayRef({B, nodes}) || !t->is_contiguous()))
       Py_RETURN_NONE;
   if (q && (!on(*q, dev) || q->scalar_type() != at::kFloat || q->sizes() != x->sizes() || !q->is_contiguous())) Py_RETURN_NONE;
   Tensor out = empty({B, nodes}, *x, at::kInt), path = empty({B, nodes}, *x, at::kInt), count = empty({B}, *x, at::kInt),
@@ -793,8 +793,8 @@ PyObject* verify_drafts(PyObject*, PyObject* const* a, Py_ssize_t n) {
   if (!launched([&] {
         return api.verify_drafts(x->const_data_ptr(), q ? q->const_data_ptr() : nullptr, tok->const_data_ptr(), par->const_data_ptr(),
                                  u->const_data_ptr(), acc ? acc->const_data_ptr() : nullptr, out.mutable_data_ptr(),
-                                 path.mutable_data_ptr(), count.mutable_data_ptr(), ws.mutable_data_ptr(), x->scalar_type() == at::kBFloat16,
-                                 int(B), int(nodes), int(V), temp, top, stream(dev));
+                                 path.mutable_data_ptr(), count.mutable_data_ptr(), ws.mutable_data_ptr(),
+                                 x->scalar_type() == at::kBFloat16, int(B), int(nodes), int(V), temp, top, stream(dev));
       }))
     Py_RETURN_NONE;
   PyObject* r = PyTuple_New(3);
@@ -871,7 +871,8 @@ PyMethodDef methods[] = {METHOD(bind), METHOD(device_ready), METHOD(memory_room)
                          METHOD(embedding_fwd), METHOD(gemm), METHOD(tma_ok), METHOD(gemm_rope), METHOD(gemm_swiglu),
                          METHOD(flash_fwd), METHOD(split_heads), METHOD(decode_attn_block), METHOD(mlp_few_rows),
                          METHOD(span_mask), METHOD(span_fwd), METHOD(span_bwd), METHOD(tree_attn),
-                         METHOD(paged_append), METHOD(paged_read), METHOD(paged_attn), METHOD(verify_drafts), {nullptr, nullptr, 0, nullptr}};
+                         METHOD(paged_append), METHOD(paged_read), METHOD(paged_attn), METHOD(verify_drafts),
+                         {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_b200host", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 
 }  // namespace

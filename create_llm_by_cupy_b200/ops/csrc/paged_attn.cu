@@ -8,8 +8,8 @@
 //     of the CTA, columns 4 to 7 what rounding left of them: scores and weights go in as two 16-bit parts at no further product. With the
 //     heads as rows (8 and 8 of 16) it were twice the products and accumulators: 107 -> 90 us for 64 x 1500 to 4000 tokens, 32 / 8 heads of
 //     128, int8. (A tcgen05 tile has 128 rows, of which four heads would fill four.)
-//   * 8-bit rows become exact fp16 in registers (no rounding before the products); K's scale multiplies the score; V's joins the weight as a
-//     logarithm: w_j = 2^(s_j + log2 sv_j - M), M the running maximum of that sum, and the sum of the weights without it is that of
+//   * 8-bit rows become exact fp16 in registers (no rounding before the products); K's scale multiplies the score; V's joins the weight
+//     as a logarithm: w_j = 2^(s_j + log2 sv_j - M), M the running maximum of that sum, and the sum of the weights without it is that of
 //     w_j / sv_j. The largest weight is held as 2^14, so that fp16 has 2^-38 of it to show for a small one.
 //   * a dot product does not care in which order its dims are walked: a lane's 16-byte pieces of K are fragments as they stand. V needs
 //     pairs of tokens: two byte permutations for four dims. Weights are turned over by movmatrix.
@@ -70,9 +70,9 @@ struct PA {
   static constexpr int kOwn = PA_WARPS * kWarp;                      // those of the new token
   static constexpr int kSmem = kOwn + kPart;
   static_assert(2 * kPart <= kStages * kStage);
-  // Where byte x of a tile stands: the 16-byte pieces of a 128-byte line in another order from line to line, so that neither the eight lanes
-  // that read K together (two rows, four pieces) nor those that read V (four rows, two pieces) meet a bank twice (256-byte rows: V twice).
-  // The order repeats every eight rows.
+  // Where byte x of a tile stands: the 16-byte pieces of a 128-byte line in another order from line to line, so that neither the eight
+  // lanes that read K together (two rows, four pieces) nor those that read V (four rows, two pieces) meet a bank twice (256-byte rows: V
+  // twice). The order repeats every eight rows.
   __host__ __device__ static constexpr int place(int x) {
     const int line = x >> 7, r = kRow == 256 ? line >> 1 : line;
     return x ^ (kRow == 64 ? (line & 3) << 5 : ((r & 6) ^ (r & 1) << 2) << 4);
@@ -81,10 +81,12 @@ struct PA {
 
 // 16 or 4 bytes on their way to shared memory, or zeros in their place.
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool there = true) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(there ? 16 : 0) : "memory");
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(there ? 16 : 0)
+               : "memory");
 }
 __device__ __forceinline__ void cp_async4(uint32_t dst, const void* src, bool there = true) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(there ? 4 : 0) : "memory");
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(dst), "l"(__cvta_generic_to_global(src)), "r"(there ? 4 : 0)
+               : "memory");
 }
 __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
@@ -166,12 +168,12 @@ __device__ __forceinline__ void rotate_chunks(float (&y)[D / 4], int tq, const f
     }
 }
 
-// Grid (cluster or pieces, KVH * groups, B), cluster (size, 1, 1): the CTAs along x share the tokens of one sequence and KV head, their four
-// warps take a tile in turn. A fifth warp deals with the new token. What they have is joined in the cluster, or by the next kernel.
+// Grid (cluster or pieces, KVH * groups, B), cluster (size, 1, 1): the CTAs along x share the tokens of one sequence and KV head, their
+// four warps take a tile in turn. A fifth warp deals with the new token. What they have is joined in the cluster, or by the next kernel.
 template <int D, int kHeld, int kScore>
 __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAttnParams p) {
   using L = PA<D, kHeld>;
-  constexpr int kTile = L::kTile, kRow = L::kRow, kNt = kTile / 8, kStages = L::kStages;
+  constexpr int kTile = L::kTile, kRow = L::kRow, kStages = L::kStages;
   constexpr float kUp = kHeld == kHeldBf16 ? 0.f : 14.f;       // log2 of what the largest weight of a row is held as
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, tq = lane & 3;
@@ -371,7 +373,8 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
         wl[g] = l_new;
       }
 #pragma unroll
-      for (int i = 0; i < D / 4; i += 4) *reinterpret_cast<float4*>(wo + g * D + tq * (D / 4) + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+      for (int i = 0; i < D / 4; i += 4)
+        *reinterpret_cast<float4*>(wo + g * D + tq * (D / 4) + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
     }
   }
 
@@ -429,8 +432,8 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
             for (int t = 0; t < kMt; ++t) {
               const uint32_t x = kHeld == kHeldInt8 ? w[2 * t][e] ^ 0x80808080u : w[2 * t][e];
               const uint32_t z = kHeld == kHeldInt8 ? w[2 * t + 1][e] ^ 0x80808080u : w[2 * t + 1][e];
-              mma_16816<kHeld>(acc[t], half2_of<kHeld, false>(x), half2_of<kHeld, false>(z), half2_of<kHeld, true>(x), half2_of<kHeld, true>(z),
-                               qf[c * L::kWords + e][0], qf[c * L::kWords + e][1]);
+              mma_16816<kHeld>(acc[t], half2_of<kHeld, false>(x), half2_of<kHeld, false>(z), half2_of<kHeld, true>(x),
+                               half2_of<kHeld, true>(z), qf[c * L::kWords + e][0], qf[c * L::kWords + e][1]);
             }
         }
       }
@@ -526,8 +529,8 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
             if (kHeld == kHeldInt8) {
               a ^= 0x80808080u; c ^= 0x80808080u; d ^= 0x80808080u; e ^= 0x80808080u;
             }
-            mma_16816<kHeld>(o[2 * w], half2_of<kHeld, false>(a), half2_of<kHeld, true>(a), half2_of<kHeld, false>(c), half2_of<kHeld, true>(c),
-                             b0, b1);
+            mma_16816<kHeld>(o[2 * w], half2_of<kHeld, false>(a), half2_of<kHeld, true>(a), half2_of<kHeld, false>(c),
+                             half2_of<kHeld, true>(c), b0, b1);
             mma_16816<kHeld>(o[2 * w + 1], half2_of<kHeld, false>(d), half2_of<kHeld, true>(d), half2_of<kHeld, false>(e),
                              half2_of<kHeld, true>(e), b0, b1);
           }
@@ -642,9 +645,10 @@ __global__ void __launch_bounds__(D) paged_join_kernel(const PagedAttnParams p) 
 
 static int paged_groups(int QH, int KVH) { return (QH / KVH + PA_HEADS - 1) / PA_HEADS; }
 
-// CTAs that share a sequence and KV head: {size of their cluster, 0}, or {1, pieces}. Clusters double while all still run at once (three CTAs
-// an SM) and hold 256 tokens a CTA: 32 x 0 to 1980 tokens, 16 / 4 heads, 21 us with two, 26 with one, 23 with four. Pieces where clusters of
-// eight would fill less than half of the GPU; at other numbers of sequences they are no better (two of 64 x 1500 to 4000: 86 us for 88).
+// CTAs that share a sequence and KV head: {size of their cluster, 0}, or {1, pieces}. Clusters double while all still run at once (three
+// CTAs an SM) and hold 256 tokens a CTA: 32 x 0 to 1980 tokens, 16 / 4 heads, 21 us with two, 26 with one, 23 with four. Pieces where
+// clusters of eight would fill less than half of the GPU; at other numbers of sequences they are no better (two of 64 x 1500 to 4000: 86 us
+// for 88).
 static int2 paged_split(int B, int QH, int KVH, int width, int log_page) {
   const long long units = (long long)B * KVH * paged_groups(QH, KVH), slots = 3LL * num_sms(), tokens = (long long)width << log_page;
   const long long most = std::max(1LL, tokens / 256);
@@ -722,7 +726,8 @@ B200_API int b200_paged_attn_append(const void* kqv, void* pk, void* pv, void* k
   p.ld = ld; p.QH = QH; p.rows = rows; p.scale = scale;
   p.cap = make_score_cap(scale, cap);
   p.pieces = paged_split(B, QH, KVH, width, log_page).y;
-  if (p.pieces > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0)) return static_cast<int>(cudaErrorInvalidValue);
+  if (p.pieces > 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0))
+    return static_cast<int>(cudaErrorInvalidValue);
   p.part_o = static_cast<float*>(workspace);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + (long long)B * QH * p.pieces * D);
   if (D == 128)

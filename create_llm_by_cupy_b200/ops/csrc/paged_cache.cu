@@ -1,8 +1,8 @@
 // Rows of K and V into the pages of a cache, and tokens back out of it (paged_cache.cuh says how they are held).
 //
-// Both are one pass over the data with nothing to reuse, bound by HBM: 16 bytes to a load, all lanes of a row beside one another, four rows to
-// a thread so that enough is on its way. int8, 8 KV heads of 128: 4096 tokens written and read back 22.5 us in two launches (24.4 with a row
-// to a thread), 8 x 2000 to 4000 e4m3 tokens read 30.6 us (38.4), 4.9 TB/s.
+// Both are one pass over the data with nothing to reuse, bound by HBM: 16 bytes to a load, all lanes of a row beside one another, four
+// rows to a thread so that enough is on its way. int8, 8 KV heads of 128: 4096 tokens written and read back 22.5 us in two launches (24.4
+// with a row to a thread), 8 x 2000 to 4000 e4m3 tokens read 30.6 us (38.4), 4.9 TB/s.
 #include "paged_cache.cuh"
 
 namespace b200 {

@@ -77,7 +77,7 @@ __device__ __forceinline__ uint32_t half2_of(uint32_t w) {
     return y;
   } else {
     uint32_t y;
-    asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, %2;\n\t}" : "=r"(y) : "r"(w), "h"(uint16_t(kHigh ? w >> 16 : w)));
+    asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(y) : "h"(uint16_t(kHigh ? w >> 16 : w)));
     return y;
   }
 }
@@ -111,7 +111,8 @@ inline const char* paged_pool_wrong(const PagedPool& c, int held, int D) {
   if (held < 0 || held > 2 || (D != 64 && D != 128)) return "type or head dimension";
   if (c.B < 0 || c.width < 1 || c.pages < 1 || c.KVH < 1 || c.log_page < 5 || c.log_page > 10) return "sizes";
   if (c.tokens() > 0x7fffffffLL) return "tokens";
-  if (c.k == nullptr || c.v == nullptr || c.table == nullptr || (held != kHeldBf16) != (c.ks != nullptr && c.vs != nullptr)) return "pointers";
+  if (c.k == nullptr || c.v == nullptr || c.table == nullptr || (held != kHeldBf16) != (c.ks != nullptr && c.vs != nullptr))
+    return "pointers";
   for (const void* x : {c.k, c.v, (void*)c.ks, (void*)c.vs})
     if ((reinterpret_cast<uintptr_t>(x) & 15) != 0) return "alignment";
   return nullptr;

@@ -12,9 +12,9 @@
 // whole row's sum, and integers add up to the same in any order.
 //
 // What bounds it: a row of 32000 logits is 128 KB, 3 us of an SM's share of HBM, and 32000 fp64 exponentials, which take 9; but the chain
-// of a node is about 45000 cycles (25 us) long whatever its slices are: largest logit, weights, the bin, the tokens of the bin, the sums, the
-// draw, each of them once over the row and once through the cluster. So slices are as large as two CTAs an SM hold, and where there are more
-// nodes than clusters, node 0 of all sequences comes first, then node 1: most of the later ones are out of question by then and passed
+// of a node is about 45000 cycles (25 us) long whatever its slices are: largest logit, weights, the bin, the tokens of the bin, the sums,
+// the draw, each of them once over the row and once through the cluster. So slices are as large as two CTAs an SM hold, and where there are
+// more nodes than clusters, node 0 of all sequences comes first, then node 1: most of the later ones are out of question by then and passed
 // over. Us, 6 nodes of one sequence (probabilities of the drafts, nucleus) / 8 x 24 (the same, no nucleus) / 16 x 63 (looked up,
 // nucleus), 32000 tokens: bits of the nucleus' end one by one 267 / 122 / 1709, histogram 30 / 45 / 417, its search in two steps and
 // nodes passed over 23 / 60 / 83. (CTAs that read one another's whole histograms took 17000 cycles for it.)
@@ -507,7 +507,8 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const Verify
           if (!weights(s, from, k)) continue;
 #pragma unroll
           for (int e = 0; e < 4; ++e)
-            if (k[e] >= klo && k[e] < khi) atomicAdd(&sh.bins[(khi - 1 - k[e]) >> shift], fixed(__longlong_as_double((long long)k[e]), unit));
+            if (k[e] >= klo && k[e] < khi)
+              atomicAdd(&sh.bins[(khi - 1 - k[e]) >> shift], fixed(__longlong_as_double((long long)k[e]), unit));
         }
         coarse();
         meet();
@@ -691,7 +692,8 @@ using namespace b200;
 B200_API int b200_verify_drafts(const void* logits, const void* q, const void* tokens, const void* parents, const void* u,
                                 const void* accept, void* out, void* path, void* count, void* workspace, int is_bf16, int B, int n, int V,
                                 double temp, double top, cudaStream_t st) {
-  if (B < 0 || n < 1 || n > VD_MAX_NODES || V < 1 || !(temp == 0. || (temp >= 1e-6 && temp <= 1e6)) || !(top > 0.) || (q == nullptr) != (accept == nullptr))
+  if (B < 0 || n < 1 || n > VD_MAX_NODES || V < 1 || !(temp == 0. || (temp >= 1e-6 && temp <= 1e6)) || !(top > 0.) ||
+      (q == nullptr) != (accept == nullptr))
     return static_cast<int>(cudaErrorInvalidValue);
   if (B == 0) return 0;
   VerifyParams p;

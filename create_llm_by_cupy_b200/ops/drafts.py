@@ -27,8 +27,8 @@ def verify_drafts(logits, tokens, parents, u, *, temp: float = 1.0, top: float =
     may be ragged. ``u`` fp32 [B, n]: numbers from [0, 1), for the draw behind each node.
 
     A node's probabilities p are the softmax of its logits / ``temp`` over its nucleus, the fewest tokens, by falling probability and
-    rising index, whose mass reaches ``top``. ``temp`` is from 1e-6 to 1e6, or 0, which leaves the largest logit, of several the one of the lowest index. Logits of
-    -infinity and NaN count for nothing, +infinity for the largest number.
+    rising index, whose mass reaches ``top``. ``temp`` is from 1e-6 to 1e6, or 0, which leaves the largest logit, of several the one of the
+    lowest index. Logits of -infinity and NaN count for nothing, +infinity for the largest number.
 
     Without ``draft_probs`` the token behind a node is the first whose sum of probabilities, in the order of the tokens, exceeds u; if a
     child holds it (of several the first) the text goes on there. With ``draft_probs`` fp32 [B, n, V] - row i: the distribution q that

@@ -7,7 +7,7 @@ tensors take a plain torch restatement (fp32, or fp64 for fp64 inputs).
     cache = paged_cache(pages, KVH, page, D, device, "int8")              # one per layer; a table serves all of them
     paged_append(k, v, cache, table, seq, pos, cos, sin)                  # prompts: any tokens of any sequences
     o = paged_attn_append(kqv, cache, table, lens, QH, KVH, cos, sin)     # one new token of each sequence
-    paged_read(cache, table, lens, kcache, vcache)                        # out into contiguous caches (``tree_attn_append``, ``decode_attn``)
+    paged_read(cache, table, lens, kcache, vcache)                        # out into contiguous caches, for ``tree_attn_append``
 
 ``table`` int32 [B, width] names the pages of each sequence: token t stands in row t % page of page table[b, t // page]. An entry that is
 no page of the pool is one that is not there: what would be written to it is left out, what would be read from it is not seen. Sequences
@@ -205,7 +205,7 @@ def paged_append(k, v, cache: PagedCache, table, seq, pos, cos=None, sin=None) -
     if M == 0 or table.shape[0] == 0:
         return
     with torch.cuda.device(k.device):
-        k, v = (t if t.stride(2) == 1 and t.stride(1) == D and (M == 1 or t.stride(0) % 8 == 0 and t.stride(0) > 0) and t.data_ptr() % 16 == 0
+        k, v = (t if t.stride()[1:] == (D, 1) and (M == 1 or t.stride(0) % 8 == 0 and t.stride(0) > 0) and t.data_ptr() % 16 == 0
                 else t.clone(memory_format=torch.contiguous_format) for t in (k, v))
         if cos is not None:
             cos, sin = _on_16(cos), _on_16(sin)

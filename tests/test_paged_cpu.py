@@ -144,7 +144,8 @@ def test_refusals():
             P.paged_append(args[0], args[1], cache, table, args[2], args[3], cos, sin)
     with pytest.raises(ValueError):
         P.paged_append(kv, kv, cache, table, seq, pos, cos[:, :4], sin[:, :4])
-    for kw in (dict(lens=lens.long()), dict(lens=lens[:1]), dict(kcache=kc[:1], vcache=kc[:1]), dict(start=lens.long()), dict(vcache=kc[:, :, :4])):
+    for kw in (dict(lens=lens.long()), dict(lens=lens[:1]), dict(kcache=kc[:1], vcache=kc[:1]), dict(start=lens.long()),
+               dict(vcache=kc[:, :, :4])):
         with pytest.raises(ValueError):
             P.paged_read(**{**dict(cache=cache, table=table, lens=lens, kcache=kc, vcache=kc.clone()), **kw})
     for kw in (dict(QH=5), dict(KVH=1), dict(lens=lens.long()), dict(cos=cos[:0], sin=sin[:0]), dict(softcap=-1.0),

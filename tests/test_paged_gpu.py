@@ -191,7 +191,8 @@ def test_token_with_modified_scores(kind, mod, D):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("B,hi,page", [(1, 9000, 128), (3, 4100, 256), (1, 1, 1024), (40, 260, 32), (40, 700, 32), (150, 70, 64), (700, 40, 1024)])
+@pytest.mark.parametrize("B,hi,page", [(1, 9000, 128), (3, 4100, 256), (1, 1, 1024), (40, 260, 32), (40, 700, 32), (150, 70, 64),
+                                       (700, 40, 1024)])
 def test_token_of_long_and_of_many_sequences(kind, B, hi, page):
     QH, KVH, D = 16, 4, 128
     lens = [hi - 61 * b % hi for b in range(B)]
@@ -291,7 +292,8 @@ def test_strides_streams_graphs_and_the_general_path(monkeypatch):
         m.setattr(native, "host", None)
         assert torch.equal(P.paged_attn_append(kqv, cache, table, n, QH, KVH, cos, sin), want)
         rows = kqv[:, :KVH * D].unflatten(1, (KVH, D))
-        P.paged_append(rows, kqv[:, (KVH + QH) * D:].unflatten(1, (KVH, D)), cache, table, torch.arange(2, dtype=torch.int32, device=DEV), n, cos, sin)
+        seq = torch.arange(2, dtype=torch.int32, device=DEV)
+        P.paged_append(rows, kqv[:, (KVH + QH) * D:].unflatten(1, (KVH, D)), cache, table, seq, n, cos, sin)
         assert same(cache, after)                            # the same row from either kernel
         kc, vc = (torch.zeros(2, KVH, 101, D, dtype=torch.bfloat16, device=DEV) for _ in range(2))
         P.paged_read(cache, table, n + 1, kc, vc)
@@ -358,7 +360,8 @@ def test_calls_without_rows():
     none = torch.zeros(0, dtype=torch.int32, device=DEV)
     table = torch.zeros((0, 1), dtype=torch.int32, device=DEV)
     cos, sin = O.tables(32, 64, device=DEV)
-    assert P.paged_attn_append(torch.zeros(0, 8 * 64, dtype=torch.bfloat16, device=DEV), cache, table, none, 4, 2, cos, sin).shape == (0, 4, 64)
+    kqv = torch.zeros(0, 8 * 64, dtype=torch.bfloat16, device=DEV)
+    assert P.paged_attn_append(kqv, cache, table, none, 4, 2, cos, sin).shape == (0, 4, 64)
     x = torch.zeros(0, 2, 64, dtype=torch.bfloat16, device=DEV)
     P.paged_append(x, x, cache, table, none, none, cos, sin)
     kc = torch.zeros(0, 2, 5, 64, dtype=torch.bfloat16, device=DEV)

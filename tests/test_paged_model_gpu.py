@@ -56,6 +56,6 @@ def test_drawn_batches_and_drafts():
         row = logits[63 + i - 1]
         assert float(row.max() - row[tok]) <= 2e-2 * float(row.abs()[:511].max())
     assert len(out) == 24 and len(calls) < 24
-    assert m.generate_drafted(PROMPTS[2], draft, max_new_tokens=9, temp=1.0, seed=3) == m.generate_drafted(PROMPTS[2], draft, max_new_tokens=9,
-                                                                                                       temp=1.0, seed=3)
+    twice = [m.generate_drafted(PROMPTS[2], draft, max_new_tokens=9, temp=1.0, seed=3) for _ in range(2)]
+    assert twice[0] == twice[1]
     assert native.read_status() == (0, 0)

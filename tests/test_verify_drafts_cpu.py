@@ -20,7 +20,8 @@ def tree(B, n, V, seed, width=3, spread=2.0, dtype=torch.float32):
             parents[b, i] = int(torch.randint(max(0, i - width), i, (1,), generator=g)) if torch.rand(1, generator=g) > 0.1 else -1
     probs = torch.softmax(logits.float() + 0.3 * torch.randn(B, n, V, generator=g), -1)
     tokens = torch.multinomial(probs.view(-1, V), n, replacement=True, generator=g).view(B, n, n)
-    tokens = torch.gather(tokens, 1, parents.clamp_min(0).long()[..., None].expand(B, n, n))[:, torch.arange(n), torch.arange(n)].to(torch.int32)
+    of_parent = torch.gather(tokens, 1, parents.clamp_min(0).long()[..., None].expand(B, n, n))
+    tokens = of_parent[:, torch.arange(n), torch.arange(n)].to(torch.int32)
     return logits, tokens, parents, torch.rand(B, n, generator=g), probs, torch.rand(B, n, generator=g)
 
 
@@ -85,8 +86,9 @@ def test_refusals():
     logits, tokens, parents, u, q, a = tree(2, 4, 9, 0)
     good = dict(logits=logits, tokens=tokens, parents=parents, u=u, temp=1.0, top=1.0)
     verify_drafts(**good)
-    for bad in (dict(logits=logits[0]), dict(logits=logits.expand(2, 4, 9)[:, :, :0]), dict(tokens=tokens.long()), dict(parents=parents[:1]),
-                dict(u=u.double()), dict(temp=-1.0), dict(temp=math.nan), dict(temp=math.inf), dict(temp=1e-9), dict(temp=2e6), dict(top=0.0), dict(top=math.nan),
+    for bad in (dict(logits=logits[0]), dict(logits=logits[:, :, :0]), dict(tokens=tokens.long()), dict(parents=parents[:1]),
+                dict(u=u.double()), dict(temp=-1.0), dict(temp=math.nan), dict(temp=math.inf), dict(temp=1e-9), dict(temp=2e6),
+                dict(top=0.0), dict(top=math.nan),
                 dict(draft_probs=q), dict(accept=a), dict(draft_probs=q.double(), accept=a), dict(draft_probs=q, accept=a[:, :2])):
         with pytest.raises(ValueError):
             verify_drafts(**{**good, **bad})

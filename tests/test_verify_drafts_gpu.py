@@ -95,7 +95,8 @@ def test_paths_streams_and_graphs(monkeypatch):
         for got, w in zip(run(x, tokens, parents, u, q, a, temp=0.7, top=0.95), want):
             assert torch.equal(got, w)
     big = torch.stack([x.cuda(), x.cuda()], 3)[..., 0]                    # a view that is not contiguous
-    for got, w in zip(verify_drafts(big, tokens.cuda(), parents.cuda(), u.cuda(), temp=0.7, top=0.95, draft_probs=q.cuda(), accept=a.cuda()), want):
+    more = dict(temp=0.7, top=0.95, draft_probs=q.cuda(), accept=a.cuda())
+    for got, w in zip(verify_drafts(big, tokens.cuda(), parents.cuda(), u.cuda(), **more), want):
         assert torch.equal(got, w)
     side = torch.cuda.Stream()
     side.wait_stream(torch.cuda.current_stream())
