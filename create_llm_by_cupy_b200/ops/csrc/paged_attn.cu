@@ -184,27 +184,30 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
   const int cs = gridDim.x, rank = blockIdx.x, b = blockIdx.z, kvh = blockIdx.y / p.groups, grp = blockIdx.y % p.groups;
   const int R = p.QH / p.c.KVH, heads = min(R - grp * PA_HEADS, PA_HEADS), h0 = kvh * R + grp * PA_HEADS;
   const bf16* row_in = p.kqv + (long long)b * p.ld;
+  const int step = cs * PA_WARPS, first = rank * PA_WARPS + warp;
+  const int* table = p.c.table + (long long)b * p.c.width;
+  // Pages of 32 tiles at a time, a lane each; of the first ones while the length is still on its way.
+  const auto page_at = [&](int i) {
+    const long long at = ((long long)first + (long long)(i + lane) * step) * kTile >> p.c.log_page;
+    return at < p.c.width ? table[at] : -1;
+  };
+  int pages = page_at(0);
   const int pos = p.lens[b];
   float q[D / 4];
   load_chunks<D, kHeld>(row_in + ((long long)p.c.KVH + h0 + min(g & 3, heads - 1)) * D, tq, q);
   const int len = int(min((long long)max(pos, 0), p.c.tokens()));
-  const int nt = (len + kTile - 1) / kTile, step = cs * PA_WARPS, first = rank * PA_WARPS + warp;
+  const int nt = (len + kTile - 1) / kTile;
   const int count = warp == PA_WARPS || pos < 0 || first >= nt ? 0 : (nt - first + step - 1) / step;
 
   // Tiles are asked for kStages ahead, by the lanes themselves (bulk copies took as long, and leave the bytes in the order that they come
-  // in). The pages of 32 tiles are looked up at a time, a lane each.
-  const int* table = p.c.table + (long long)b * p.c.width;
+  // in).
   uint32_t lane_place[4];                                    // of this lane's 16 bytes of every 512
 #pragma unroll
   for (int x = 0; x < 4; ++x) lane_place[x] = L::place(512 * x + lane * 16) - 512 * x;
-  int pages = -1;
   uint32_t skipped = 0;                                      // bit i % 32: tile i has no page
   auto ask = [&](int i) {
     if (i < count) {
-      if ((i & 31) == 0) {
-        const int t = first + (i + lane) * step;
-        pages = i + lane < count ? table[(t * kTile) >> p.c.log_page] : -1;
-      }
+      if ((i & 31) == 0 && i > 0) pages = page_at(i);
       const int pg = __shfl_sync(0xffffffffu, pages, i & 31), t0 = (first + i * step) * kTile, bytes = min(kTile, len - t0) * kRow;
       const bool there = pg >= 0 && pg < p.c.pages;
       skipped = (skipped & ~(1u << (i & 31))) | (there ? 0u : 1u << (i & 31));
@@ -645,17 +648,15 @@ __global__ void __launch_bounds__(D) paged_join_kernel(const PagedAttnParams p) 
 
 static int paged_groups(int QH, int KVH) { return (QH / KVH + PA_HEADS - 1) / PA_HEADS; }
 
-// CTAs that share a sequence and KV head: {size of their cluster, 0}, or {1, pieces}. Clusters double while all still run at once (three
-// CTAs an SM) and hold 256 tokens a CTA: 32 x 0 to 1980 tokens, 16 / 4 heads, 21 us with two, 26 with one, 23 with four. Pieces where
-// clusters of eight would fill less than half of the GPU; at other numbers of sequences they are no better (two of 64 x 1500 to 4000: 86 us
-// for 88).
+// CTAs that share a sequence and KV head: {size of their cluster, 0}, or {1, pieces}. As many as still run at once, three CTAs an SM with a
+// twentieth to spare for an uneven spread, and hold 256 tokens each: 32 x 0 to 1980 tokens, 16 / 4 heads, 25.8, 21.0, 18.8, 23.3, 28.5 us
+// with clusters of 1, 2, 3, 4, 8; 16 x 900 to 2047 in bf16 28.5, 21.6, 18.5, 17.9, 22.4 with 1, 2, 4, 6, 8. Pieces where clusters of eight
+// would fill less than half of the GPU; at other numbers of sequences they are no better (two of 64 x 1500 to 4000: 86 us for 88).
 static int2 paged_split(int B, int QH, int KVH, int width, int log_page) {
   const long long units = (long long)B * KVH * paged_groups(QH, KVH), slots = 3LL * num_sms(), tokens = (long long)width << log_page;
   const long long most = std::max(1LL, tokens / 256);
   if (units * PA_CLUSTER <= slots / 2 && most > PA_CLUSTER) return make_int2(1, int(std::min(slots / units, most)));
-  int cs = 1;
-  while (cs < PA_CLUSTER && 2 * cs * units <= slots && cs < most) cs *= 2;
-  return make_int2(cs, 0);
+  return make_int2(int(std::max(1LL, std::min({(long long)PA_CLUSTER, most, slots * 19 / (20 * units)}))), 0);
 }
 
 template <int D, int kHeld, int kScore>

@@ -1,8 +1,9 @@
 // Rows of K and V into the pages of a cache, and tokens back out of it (paged_cache.cuh says how they are held).
 //
-// Both are one pass over the data with nothing to reuse, bound by HBM: 16 bytes to a load, all lanes of a row beside one another, four
-// rows to a thread so that enough is on its way. int8, 8 KV heads of 128: 4096 tokens written and read back 22.5 us in two launches (24.4
-// with a row to a thread), 8 x 2000 to 4000 e4m3 tokens read 30.6 us (38.4), 4.9 TB/s.
+// Both are one pass over the data with nothing to reuse, bound by HBM: 16 bytes to a load, all lanes of a row beside one another, two rows to
+// a thread so that enough is on its way. int8, 8 KV heads of 128, 4096 tokens written and read back, in two launches: 20 us; with 8 bytes of
+// one row to a thread 24.4, with four heads and four rows 22.5, with one head 24.3, with eight rows 23.9. 8 x 2000 to 4000 e4m3 tokens read:
+// 29.4 us, 5.1 TB/s (38.4, and 30.7 with four rows, 34.1 with eight).
 #include "paged_cache.cuh"
 
 namespace b200 {
@@ -19,9 +20,9 @@ struct AppendParams {
   int rows;
 };
 
-// D / 8 lanes for a token's K (or V) of four heads, whose loads are all on their way before the first is used: its place and its angles are
+// D / 8 lanes for a token's K (or V) of two heads, whose loads are all on their way before the first is used: its place and its angles are
 // looked up once for them. A row is left out when its sequence, position or page is none of the cache.
-constexpr int kAppendHeads = 4;
+constexpr int kAppendHeads = 2;
 
 template <int D, int kHeld>
 __global__ void __launch_bounds__(256) paged_append_kernel(const AppendParams p) {
@@ -107,8 +108,8 @@ struct ReadParams {
   int Tmax;
 };
 
-// 16 bytes of four rows to a thread, all on their way before the first is used; grid (groups of rows, KVH, 2 B).
-constexpr int kReadRows = 4;
+// 16 bytes of two rows to a thread, both on their way before the first is used; grid (groups of rows, KVH, 2 B).
+constexpr int kReadRows = 2;
 
 template <int D, int kHeld>
 __global__ void __launch_bounds__(256) paged_read_kernel(const ReadParams p) {
