@@ -625,23 +625,57 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
   }
 }
 
-// The parts of a query head: grid B * QH, a thread for each dim.
+// The parts of a query head: grid B * QH, block (D, PA_JOIN): a thread for each dim takes every PA_JOIN-th part, four on their way at a time.
+constexpr int PA_JOIN = 4;
+
 template <int D>
-__global__ void __launch_bounds__(D) paged_join_kernel(const PagedAttnParams p) {
-  const int d = threadIdx.x;
+__global__ void __launch_bounds__(D * PA_JOIN) paged_join_kernel(const PagedAttnParams p) {
+  __shared__ float sm[PA_JOIN], sl[PA_JOIN], so[PA_JOIN][D];
+  const int d = threadIdx.x, w = threadIdx.y;
   pdl_wait();
   pdl_trigger();
   const float2* ml = p.part_ml + (long long)blockIdx.x * p.pieces;
   const float* o = p.part_o + (long long)blockIdx.x * p.pieces * D + d;
   float m = -INFINITY, l = 0.f, x = 0.f;
-#pragma unroll 8
-  for (int c = 0; c < p.pieces; ++c) m = fmaxf(m, ml[c].x);
+  for (int c0 = w; c0 < p.pieces; c0 += 4 * PA_JOIN) {
+    float2 a[4];
+    float y[4], m_new = m;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int c = c0 + e * PA_JOIN, from = min(c, p.pieces - 1);
+      a[e] = ml[from];
+      y[e] = o[(long long)from * D];
+      if (c != from) a[e] = make_float2(-INFINITY, 0.f);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m_new = fmaxf(m_new, a[e].x);
+    const float ref = m_new == -INFINITY ? 0.f : m_new, f0 = exp2_of(m - ref);
+    l *= f0;
+    x *= f0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const float f = exp2_of(a[e].x - ref);
+      l = fmaf(a[e].y, f, l);
+      x = fmaf(y[e], f, x);
+    }
+    m = m_new;
+  }
+  so[w][d] = x;
+  if (d == 0) {
+    sm[w] = m;
+    sl[w] = l;
+  }
+  __syncthreads();
+  if (w != 0) return;
+#pragma unroll
+  for (int e = 1; e < PA_JOIN; ++e) m = fmaxf(m, sm[e]);
   const float ref = m == -INFINITY ? 0.f : m;
-#pragma unroll 8
-  for (int c = 0; c < p.pieces; ++c) {
-    const float f = exp2_of(ml[c].x - ref);
-    l = fmaf(ml[c].y, f, l);
-    x = fmaf(o[(long long)c * D], f, x);
+  l = x = 0.f;
+#pragma unroll
+  for (int e = 0; e < PA_JOIN; ++e) {
+    const float f = exp2_of(sm[e] - ref);
+    l = fmaf(sl[e], f, l);
+    x = fmaf(so[e][d], f, x);
   }
   p.out[(long long)blockIdx.x * D + d] = __float2bfloat16(l == 0.f ? 0.f : x / l);
 }
@@ -677,7 +711,7 @@ static int launch_paged(const PagedAttnParams& p, cudaStream_t st) {
   const int cs = p.pieces > 0 ? 1 : paged_split(p.c.B, p.QH, p.c.KVH, p.c.width, p.c.log_page).x;
   B200_CHECK(launch_pdl(kern, dim3(p.pieces > 0 ? p.pieces : cs, p.c.KVH * p.groups, p.c.B), dim3(PA_THREADS), L::kSmem, st, cs, p));
   if (p.pieces == 0) return 0;
-  return static_cast<int>(launch_pdl(paged_join_kernel<D>, dim3(unsigned(p.c.B * p.QH)), dim3(D), 0, st, 0, p));
+  return static_cast<int>(launch_pdl(paged_join_kernel<D>, dim3(unsigned(p.c.B * p.QH)), dim3(D, PA_JOIN), 0, st, 0, p));
 }
 
 template <int D, int kHeld>
