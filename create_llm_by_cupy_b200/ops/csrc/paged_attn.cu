@@ -23,6 +23,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <type_traits>
 
 #include "paged_cache.cuh"
 #include "ptx.cuh"
@@ -100,6 +101,12 @@ __device__ __forceinline__ void mma_16816(float (&d)[4], uint32_t a0, uint32_t a
   else
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+// 16 x 8 sums of products of 32 signed bytes.
+__device__ __forceinline__ void mma_16832(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+r"(d[0]), "+r"(d[1]), "+r"(d[2]), "+r"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
 // Two numbers as a pair of the products' type, and as another pair what that rounding left.
@@ -245,11 +252,14 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
 #pragma unroll
   for (int i = 0; i < kStages; ++i) ask(i);
 
-  // The queries as fragments: lanes g < 4 the rounded values of head g, the others what that left of head g - 4. fp16 has room for little:
-  // each head is brought to a largest magnitude of 2^10 by a power of two.
-  uint32_t qf[D / 16][2];
-  float row_mul = 1.f;                                       // what a product of head g & 3 is multiplied with, without the token's scale
-  const int at = min(max(pos, 0), p.rows - 1);
+  // The queries as fragments: lanes g < 4 the rounded values of head g, the others what that left of head g - 4. For e4m3 as fp16, which has
+  // room for little: each head is brought to a largest magnitude of 2^10 by a power of two. For int8 as whole numbers up to 32512 of the
+  // head's largest in two bytes, hi 256 + lo: K goes into the products as it is held, their sums are exact (32512 127 128 < 2^31), and what
+  // a number is off by, 2^-16 of the head's largest, is less than its own rounding to bf16 from a 128th of that largest on.
+  constexpr bool kWhole = kHeld == kHeldInt8;
+  uint32_t qf[kWhole ? D / 32 : D / 16][2];
+  float row_mul = 1.f, own_mul = 1.f;                        // what a product of head g & 3 is multiplied with, without the token's scale;
+  const int at = min(max(pos, 0), p.rows - 1);               // and one of `q`
   const float* cosr = p.cosr + (long long)at * (D / 2);
   const float* sinr = p.sinr + (long long)at * (D / 2);
   rotate_chunks<D, kHeld>(q, tq, cosr, sinr);
@@ -259,20 +269,37 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
     for (int i = 0; i < D / 4; ++i) m = fmaxf(m, fabsf(q[i]));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
-    const int e = max(int(__float_as_uint(m) >> 23) - 127, -116);
-    const float up = __uint_as_float(uint32_t(127 + 10 - e) << 23);
-    row_mul = __uint_as_float(uint32_t(127 - 10 + e) << 23);
+    if constexpr (kWhole) {
+      const float inv = m > 7.8886091e-31f ? __fdividef(32512.f, m) : 0.f;       // 2^-100: less than that is 0
+      row_mul = m * (1.f / 32512.f);
 #pragma unroll
-    for (int i = 0; i < D / 4; ++i) q[i] *= up;
-  }
+      for (int i = 0; i < D / 4; i += 4) {
+        uint32_t w = 0;
 #pragma unroll
-  for (int i = 0; i < D / 16; ++i)
+        for (int e = 0; e < 4; ++e) {
+          const int n = min(max(__float2int_rn(q[i + e] * inv), -32512), 32512), hi = (n + 128) >> 8;
+          w |= (uint32_t(g < 4 ? hi : n - 256 * hi) & 0xffu) << (8 * e);
+        }
+        qf[i / 8][i / 4 % 2] = w;
+      }
+    } else {
+      const int e = max(int(__float_as_uint(m) >> 23) - 127, -116);
+      const float up = __uint_as_float(uint32_t(127 + 10 - e) << 23);
+      own_mul = row_mul = __uint_as_float(uint32_t(127 - 10 + e) << 23);
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      uint32_t hi, lo;
-      two_parts<kHeld>(q[4 * i + 2 * e], q[4 * i + 2 * e + 1], hi, lo);
-      qf[i][e] = g < 4 ? hi : lo;
+      for (int i = 0; i < D / 4; ++i) q[i] *= up;
     }
+  }
+  if constexpr (!kWhole) {
+#pragma unroll
+    for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        uint32_t hi, lo;
+        two_parts<kHeld>(q[4 * i + 2 * e], q[4 * i + 2 * e + 1], hi, lo);
+        qf[i][e] = g < 4 ? hi : lo;
+      }
+  }
   // Score in units of log2 of a product with a token that is `dist` back.
   auto score = [&](float s, float mul, float slope, float dist) {
     s *= mul;
@@ -363,7 +390,7 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
       for (int i = 0; i < D / 4; ++i) s = fmaf(q[i], k[i], s);
       s += __shfl_xor_sync(0xffffffffu, s, 1);
       s += __shfl_xor_sync(0xffffffffu, s, 2);
-      s = score(s * ks, row_mul * unit, 0.f, 0.f);
+      s = score(s * ks, own_mul * unit, 0.f, 0.f);
       m_new = kHeld == kHeldBf16 ? s : s + __log2f(vs);
       const float w = exp2_of(kUp);
       l_new = w * (kHeld == kHeldBf16 ? 1.f : __frcp_rn(vs));
@@ -401,9 +428,9 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
     if (!(skipped >> (i & 31) & 1)) {
       // Scores: tokens are the rows of the products, 16 at a time.
       constexpr int kMt = kTile / 16;
-      float acc[kMt][4];
+      std::conditional_t<kWhole, int, float> acc[kMt][4];
 #pragma unroll
-      for (int t = 0; t < kMt; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0.f;
+      for (int t = 0; t < kMt; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0;
       constexpr int kPiece = L::kChunk * L::kBytes;
       const uint8_t* kr = st + L::place(g * kRow + tq * kPiece);
       const int other = L::place(g * kRow + (tq + 4) * kPiece) - L::place(g * kRow + tq * kPiece);
@@ -428,16 +455,25 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
             for (int t = 0; t < kMt; ++t)
               mma_16816<kHeld>(acc[t], w[2 * t][2 * e], w[2 * t + 1][2 * e], w[2 * t][2 * e + 1], w[2 * t + 1][2 * e + 1], qf[2 * c + e][0],
                                qf[2 * c + e][1]);
+        } else if constexpr (kWhole) {
+#pragma unroll
+          for (int e = 0; e < L::kWords / 2; ++e) {
+            const uint32_t (&a)[2] = qf[c * (L::kWords / 2) + e];
+#pragma unroll
+            for (int t = 0; t < kMt; ++t)
+              mma_16832(acc[t], w[2 * t][2 * e], w[2 * t + 1][2 * e], w[2 * t][2 * e + 1], w[2 * t + 1][2 * e + 1], a[0], a[1]);
+          }
         } else {
 #pragma unroll
-          for (int e = 0; e < L::kWords; ++e)
+          for (int e = 0; e < L::kWords; ++e) {
+            const uint32_t (&a)[2] = qf[c * L::kWords + e];
 #pragma unroll
             for (int t = 0; t < kMt; ++t) {
-              const uint32_t x = kHeld == kHeldInt8 ? w[2 * t][e] ^ 0x80808080u : w[2 * t][e];
-              const uint32_t z = kHeld == kHeldInt8 ? w[2 * t + 1][e] ^ 0x80808080u : w[2 * t + 1][e];
+              const uint32_t x = w[2 * t][e], z = w[2 * t + 1][e];
               mma_16816<kHeld>(acc[t], half2_of<kHeld, false>(x), half2_of<kHeld, false>(z), half2_of<kHeld, true>(x),
-                               half2_of<kHeld, true>(z), qf[c * L::kWords + e][0], qf[c * L::kWords + e][1]);
+                               half2_of<kHeld, true>(z), a[0], a[1]);
             }
+          }
         }
       }
       // y[n][e]: token 8 n + g, head ha + e; what the rounding of Q left comes from the lane two further.
@@ -457,8 +493,10 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          float s = acc[n >> 1][2 * (n & 1) + e];
-          s += __shfl_xor_sync(0xffffffffu, s, 2);
+          const auto part_s = acc[n >> 1][2 * (n & 1) + e], rest = __shfl_xor_sync(0xffffffffu, part_s, 2);
+          float s;
+          if constexpr (kWhole) s = float(tq < 2 ? part_s * 256 + rest : rest * 256 + part_s);
+          else s = part_s + rest;
           s = score(s * ks, mul[e], slope[e], float(pos - t0 - tok)) + more;
           y[n][e] = tok < rows ? s : -INFINITY;
           m[e] = fmaxf(m[e], y[n][e]);

@@ -2,7 +2,8 @@
 
 Tolerances. A held value: half a step (``paged_oracle.step``). An output: half a bf16 step, 2^-8 |o|, and what the weights are off by
 times the largest |v|. A score's error is at most (2^-16 + D 2^-23) sum |q||k| (Q in two bf16 parts and fp32 sums; two fp16 parts are
-finer), a bias's or cap's 2^-21 of the largest score; weights change by at most expm1 of twice that, and by 2^-15 for their own two
+finer); over int8 rows Q is rounded to whole numbers of 1 / 32512 of its largest, off by half of one, so that 1 / 65024 of the largest times
+sum |k| comes on top. A bias's or cap's 2^-21 of the largest score; weights change by at most expm1 of twice that, and by 2^-15 for their own two
 parts, the exponential's and the sums' error."""
 import math
 
@@ -81,6 +82,8 @@ def check_token(cache, table, kqv, o, lens, QH, KVH, D, cap=0.0, slopes=None, co
             size = float((k[:, h // (QH // KVH)].abs() @ q[h].abs()).max()) * scale
             big = size + (0 if slopes is None else float(slopes[h]) * n)
             off = (2.0 ** -16 + D * 2.0 ** -23) * size + 2.0 ** -21 * big
+            if cache.k.dtype == torch.int8:
+                off += float(q[h].abs().max()) / 65024 * float(k[:, h // (QH // KVH)].abs().sum(-1).max()) * scale
             tol = 2.0 ** -8 * want[h].abs() + (math.expm1(2 * off) + 2.0 ** -15) * float(v[:, h // (QH // KVH)].abs().max())
             assert bool(((o[b, h] - want[h]).abs() <= tol).all()), (b, h, float((o[b, h] - want[h]).abs().max()), float(tol.max()))
 
