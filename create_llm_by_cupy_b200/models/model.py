@@ -586,7 +586,8 @@ class Cupa_ver4:
         seen = None
         if not greedy and penalty != 1.0:                                    # tokens that a sequence has
             seen = torch.zeros((B, self.vocab_size), dtype=torch.bool, device=dev)
-            seen.scatter_(1, ids.long().clamp(0, self.vocab_size - 1), (ids >= 0) & (ids < self.vocab_size))
+            known = (ids >= 0) & (ids < self.vocab_size)
+            seen[torch.arange(B, device=dev)[:, None].expand(B, T0)[known], ids[known].long()] = True
         none = torch.zeros((B, 1), dtype=torch.int32, device=dev)
         out, live = [[] for _ in range(B)], [n > 0 for n in budget]
         lens = sizes

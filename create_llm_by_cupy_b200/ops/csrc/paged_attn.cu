@@ -3,19 +3,21 @@
 //   o = sum_j p_j v_j / sum_j p_j,   p_j = 2^(s_j - m),   s_j = score(scale q . k_j) log2 e
 //
 // What bounds it: each cached row is read once, 2 D + 8 bytes a token and KV head in 8 bits, so HBM, if an SM gets through its tiles fast
-// enough: 3500 cycles for a tile of 32 tokens with twelve warps on an SM, 29 bytes a cycle where HBM has 24 for each SM. Hence:
+// enough (it has 24 bytes of HBM a cycle). 64 x 1500 to 4000 tokens, 32 / 8 heads of 128, int8, with the append: 80 us, 4.7 TB/s; bytes to
+// fp16 on the ALU and the last CTAs, which run alone, are the rest. Hence:
 //   * products by mma.sync with the TOKENS (dims, for the values) as rows and the heads as columns. Columns 0 to 3 are the four query heads
-//     of the CTA, columns 4 to 7 what rounding left of them: scores and weights go in as two 16-bit parts at no further product. With the
-//     heads as rows (8 and 8 of 16) it were twice the products and accumulators: 107 -> 90 us for 64 x 1500 to 4000 tokens, 32 / 8 heads of
-//     128, int8. (A tcgen05 tile has 128 rows, of which four heads would fill four.)
-//   * 8-bit rows become exact fp16 in registers (no rounding before the products); K's scale multiplies the score; V's joins the weight
-//     as a logarithm: w_j = 2^(s_j + log2 sv_j - M), M the running maximum of that sum, and the sum of the weights without it is that of
-//     w_j / sv_j. The largest weight is held as 2^14, so that fp16 has 2^-38 of it to show for a small one.
+//     of the CTA, columns 4 to 7 what rounding left of them: scores and weights go in as two parts at no further product. With the heads as
+//     rows (8 and 8 of 16) it were twice the products and accumulators (107 -> 90 us). (A tcgen05 tile has 128 rows, of which four heads
+//     would fill four.)
+//   * int8 keys go in as they are held, with Q as 16-bit whole numbers in two bytes (88 -> 80 us, no conversion and products of twice the
+//     depth). Values and e4m3 become exact fp16 in registers. K's scale multiplies the score; V's joins the weight as a logarithm:
+//     w_j = 2^(s_j + log2 sv_j - M), M the running maximum of that sum, and the sum of the weights without it is that of w_j / sv_j. The
+//     largest weight is held as 2^14, so that fp16 has 2^-38 of it to show for a small one.
 //   * a dot product does not care in which order its dims are walked: a lane's 16-byte pieces of K are fragments as they stand. V needs
 //     pairs of tokens: two byte permutations for four dims. Weights are turned over by movmatrix.
 //   * tiles go through a ring per warp, so warps never wait for one another until the end. Three CTAs an SM.
-//   * few sequences: clusters of up to eight CTAs share one (or, where 8 leave SMs idle, pieces that a second kernel joins: one sequence of
-//     60001 tokens 81 us with clusters of 8, 54 of 16, 41 with 55 pieces).
+//   * few sequences: clusters of up to eight CTAs share one or, where 8 leave SMs idle, pieces that a second kernel joins (one sequence of
+//     60001 tokens 68 us with clusters of 8, 54 of 16, 41 with 55 pieces; 32 since four threads a dim join them, and Q went in as bytes).
 // Tried and not kept: bulk copies by a warp of their own (no faster: the time is that of the arithmetic), one list of all tiles cut evenly
 // over CTAs that stay (64 x 1500 to 4000 tokens 88 -> 93 us, 32 x 0 to 1980 21 -> 40: the start of a stretch takes as long as four tiles,
 // and its state does not fit in the registers of three CTAs an SM).
@@ -252,10 +254,10 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
 #pragma unroll
   for (int i = 0; i < kStages; ++i) ask(i);
 
-  // The queries as fragments: lanes g < 4 the rounded values of head g, the others what that left of head g - 4. For e4m3 as fp16, which has
-  // room for little: each head is brought to a largest magnitude of 2^10 by a power of two. For int8 as whole numbers up to 32512 of the
-  // head's largest in two bytes, hi 256 + lo: K goes into the products as it is held, their sums are exact (32512 127 128 < 2^31), and what
-  // a number is off by, 2^-16 of the head's largest, is less than its own rounding to bf16 from a 128th of that largest on.
+  // The queries as fragments: lanes g < 4 the rounded values of head g, the others what that left of head g - 4. For e4m3 as fp16, which
+  // has room for little: each head is brought to a largest magnitude of 2^10 by a power of two. For int8 as whole numbers up to 32512 of
+  // the head's largest in two bytes, hi 256 + lo: K goes into the products as it is held, their sums are exact (32512 128 128 < 2^31), and
+  // what a number is off by, 2^-16 of the head's largest, is less than its own rounding to bf16 from a 128th of that largest on.
   constexpr bool kWhole = kHeld == kHeldInt8;
   uint32_t qf[kWhole ? D / 32 : D / 16][2];
   float row_mul = 1.f, own_mul = 1.f;                        // what a product of head g & 3 is multiplied with, without the token's scale;
@@ -663,7 +665,8 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
   }
 }
 
-// The parts of a query head: grid B * QH, block (D, PA_JOIN): a thread for each dim takes every PA_JOIN-th part, four on their way at a time.
+// The parts of a query head: grid B * QH, block (D, PA_JOIN): a thread for each dim takes every PA_JOIN-th part, four on their way at a
+// time.
 constexpr int PA_JOIN = 4;
 
 template <int D>

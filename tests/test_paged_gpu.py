@@ -2,9 +2,9 @@
 
 Tolerances. A held value: half a step (``paged_oracle.step``). An output: half a bf16 step, 2^-8 |o|, and what the weights are off by
 times the largest |v|. A score's error is at most (2^-16 + D 2^-23) sum |q||k| (Q in two bf16 parts and fp32 sums; two fp16 parts are
-finer); over int8 rows Q is rounded to whole numbers of 1 / 32512 of its largest, off by half of one, so that 1 / 65024 of the largest times
-sum |k| comes on top. A bias's or cap's 2^-21 of the largest score; weights change by at most expm1 of twice that, and by 2^-15 for their own two
-parts, the exponential's and the sums' error."""
+finer); over int8 rows Q is rounded to whole numbers of 1 / 32512 of its largest, off by half of one, so that 1 / 65024 of the largest
+times sum |k| comes on top. A bias's or cap's is 2^-21 of the largest score. Weights change by at most expm1 of twice that, and by 2^-15
+for their own two parts, the exponential's and the sums' error."""
 import math
 
 import pytest
