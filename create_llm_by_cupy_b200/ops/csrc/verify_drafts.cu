@@ -212,6 +212,7 @@ __global__ void __launch_bounds__(VD_THREADS, 2) verify_rows_kernel(const Verify
   // An integer number of units, rounded to nearest: the last bits of a sum with 2^52.
   auto fixed = [](double w, double u) { return u64(__double_as_longlong(fma(w, u, 4503599627370496.))) - 0x4330000000000000ull; };
 
+  if (p.lazy && cs > 1) cluster.sync();                      // the first CTA writes into the others: they have to be there
   // Node 0 of all sequences, node 1 of all, ...: a parent is decided before its children begin, if they begin in a later round.
   const long long B = p.rows / p.n;
   for (long long turn = blockIdx.y; turn < p.rows; turn += gridDim.y) {
