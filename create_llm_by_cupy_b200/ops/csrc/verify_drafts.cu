@@ -17,7 +17,7 @@
 // more nodes than clusters, node 0 of all sequences comes first, then node 1: most of the later ones are out of question by then and passed
 // over. Us, 6 nodes of one sequence (probabilities of the drafts, nucleus) / 8 x 24 (the same, no nucleus) / 16 x 63 (looked up,
 // nucleus), 32000 tokens: bits of the nucleus' end one by one 267 / 122 / 1709, histogram 30 / 45 / 417, its search in two steps and
-// nodes passed over 22 / 62 / 79. (CTAs that read one another's whole histograms took 17000 cycles for it.)
+// nodes passed over 22 / 55 to 63 / 80 to 86. (CTAs that read one another's whole histograms took 17000 cycles for it.)
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
