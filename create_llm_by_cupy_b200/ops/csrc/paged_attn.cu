@@ -254,10 +254,11 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
 #pragma unroll
   for (int i = 0; i < kStages; ++i) ask(i);
 
-  // The queries as fragments: lanes g < 4 the rounded values of head g, the others what that left of head g - 4. For e4m3 as fp16, which
-  // has room for little: each head is brought to a largest magnitude of 2^10 by a power of two. For int8 as whole numbers up to 32512 of
-  // the head's largest in two bytes, hi 256 + lo: K goes into the products as it is held, their sums are exact (32512 128 128 < 2^31), and
-  // what a number is off by, 2^-16 of the head's largest, is less than its own rounding to bf16 from a 128th of that largest on.
+  // The queries as fragments: lanes g < 4 the rounded values of head g, the others what that left of head g - 4. Over 8-bit rows each head
+  // is first brought to a largest magnitude of 2^10 by a power of two, whatever its numbers are. For e4m3 they go in as fp16, which has room
+  // for little. For int8 as whole numbers up to 32512 of the head's largest in two bytes, hi 256 + lo: K goes into the products as it is held,
+  // their sums are exact (32512 128 128 < 2^31), and what a number is off by, 2^-16 of the head's largest, is less than its own rounding to
+  // bf16 from a 128th of that largest on.
   constexpr bool kWhole = kHeld == kHeldInt8;
   uint32_t qf[kWhole ? D / 32 : D / 16][2];
   float row_mul = 1.f, own_mul = 1.f;                        // what a product of head g & 3 is multiplied with, without the token's scale;
@@ -271,25 +272,25 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
     for (int i = 0; i < D / 4; ++i) m = fmaxf(m, fabsf(q[i]));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 1));
     m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, 2));
+    const int e = max(int(__float_as_uint(m) >> 23) - 127, -116);
+    const float up = __uint_as_float(uint32_t(127 + 10 - e) << 23);
+    own_mul = row_mul = __uint_as_float(uint32_t(127 - 10 + e) << 23);
+#pragma unroll
+    for (int i = 0; i < D / 4; ++i) q[i] *= up;
     if constexpr (kWhole) {
-      const float inv = m > 7.8886091e-31f ? __fdividef(32512.f, m) : 0.f;       // 2^-100: less than that is 0
-      row_mul = m * (1.f / 32512.f);
+      m *= up;
+      const float inv = m > 0.f ? __fdividef(32512.f, m) : 0.f;
+      row_mul *= m * (1.f / 32512.f);
 #pragma unroll
       for (int i = 0; i < D / 4; i += 4) {
         uint32_t w = 0;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int n = min(max(__float2int_rn(q[i + e] * inv), -32512), 32512), hi = (n + 128) >> 8;
-          w |= (uint32_t(g < 4 ? hi : n - 256 * hi) & 0xffu) << (8 * e);
+        for (int x = 0; x < 4; ++x) {
+          const int n = min(max(__float2int_rn(q[i + x] * inv), -32512), 32512), hi = (n + 128) >> 8;
+          w |= (uint32_t(g < 4 ? hi : n - 256 * hi) & 0xffu) << (8 * x);
         }
         qf[i / 8][i / 4 % 2] = w;
       }
-    } else {
-      const int e = max(int(__float_as_uint(m) >> 23) - 127, -116);
-      const float up = __uint_as_float(uint32_t(127 + 10 - e) << 23);
-      own_mul = row_mul = __uint_as_float(uint32_t(127 - 10 + e) << 23);
-#pragma unroll
-      for (int i = 0; i < D / 4; ++i) q[i] *= up;
     }
   }
   if constexpr (!kWhole) {
