@@ -3,16 +3,17 @@
 //   o = sum_j p_j v_j / sum_j p_j,   p_j = 2^(s_j - m),   s_j = score(scale q . k_j) log2 e
 //
 // What bounds it: each cached row is read once, 2 D + 8 bytes a token and KV head in 8 bits, so HBM, if an SM gets through its tiles fast
-// enough (it has 24 bytes of HBM a cycle). 64 x 1500 to 4000 tokens, 32 / 8 heads of 128, int8, with the append: 80 us, 4.7 TB/s; bytes to
+// enough (it has 24 bytes of HBM a cycle). 64 x 1500 to 4000 tokens, 32 / 8 heads of 128, int8, with the append: 81 us, 4.6 TB/s; bytes to
 // fp16 on the ALU and the last CTAs, which run alone, are the rest. Hence:
 //   * products by mma.sync with the TOKENS (dims, for the values) as rows and the heads as columns. Columns 0 to 3 are the four query heads
 //     of the CTA, columns 4 to 7 what rounding left of them: scores and weights go in as two parts at no further product. With the heads as
 //     rows (8 and 8 of 16) it were twice the products and accumulators (107 -> 90 us). (A tcgen05 tile has 128 rows, of which four heads
 //     would fill four.)
-//   * int8 keys go in as they are held, with Q as 16-bit whole numbers in two bytes (88 -> 80 us, no conversion and products of twice the
-//     depth). Values and e4m3 become exact fp16 in registers. K's scale multiplies the score; V's joins the weight as a logarithm:
-//     w_j = 2^(s_j + log2 sv_j - M), M the running maximum of that sum, and the sum of the weights without it is that of w_j / sv_j. The
-//     largest weight is held as 2^14, so that fp16 has 2^-38 of it to show for a small one.
+//   * int8 keys go in as they are held, with Q as whole numbers of four bytes, in two products of twice the depth that need no conversion
+//     (88 -> 81 us; two bytes in one product 79, but off by up to 1.6e-2 where two dims of Q are 1000 times the others). Values and e4m3
+//     become exact fp16 in registers. K's scale multiplies the score; V's joins the weight as a logarithm: w_j = 2^(s_j + log2 sv_j - M), M
+//     the running maximum of that sum, and the sum of the weights without it is that of w_j / sv_j. The largest weight is held as 2^14, so
+//     that fp16 has 2^-38 of it to show for a small one.
 //   * a dot product does not care in which order its dims are walked: a lane's 16-byte pieces of K are fragments as they stand. V needs
 //     pairs of tokens: two byte permutations for four dims. Weights are turned over by movmatrix.
 //   * tiles go through a ring per warp, so warps never wait for one another until the end. Three CTAs an SM.
@@ -256,11 +257,12 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
 
   // The queries as fragments: lanes g < 4 the rounded values of head g, the others what that left of head g - 4. Over 8-bit rows each head
   // is first brought to a largest magnitude of 2^10 by a power of two, whatever its numbers are. For e4m3 they go in as fp16, which has room
-  // for little. For int8 as whole numbers up to 32512 of the head's largest in two bytes, hi 256 + lo: K goes into the products as it is held,
-  // their sums are exact (32512 128 128 < 2^31), and what a number is off by, 2^-16 of the head's largest, is less than its own rounding to
-  // bf16 from a 128th of that largest on.
+  // for little. For int8 as whole numbers of 2^-19, below 2^30, in four signed bytes: K goes into the products as it is held, their sums are
+  // exact (at most 2^21, also as fp32), and a number is off by 2^-30 of its head's largest at most, not at all from a 64th of it on. The
+  // upper two bytes are the eight columns of one product, the lower two of another. (Two bytes, off by 2^-16 of the largest, were half of the
+  // products, but heads with a few dims 100 times the others lost what the others say.)
   constexpr bool kWhole = kHeld == kHeldInt8;
-  uint32_t qf[kWhole ? D / 32 : D / 16][2];
+  uint32_t qf[D / 16][2];                                    // over int8 rows the upper bytes, then the lower ones
   float row_mul = 1.f, own_mul = 1.f;                        // what a product of head g & 3 is multiplied with, without the token's scale;
   const int at = min(max(pos, 0), p.rows - 1);               // and one of `q`
   const float* cosr = p.cosr + (long long)at * (D / 2);
@@ -278,18 +280,17 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
 #pragma unroll
     for (int i = 0; i < D / 4; ++i) q[i] *= up;
     if constexpr (kWhole) {
-      m *= up;
-      const float inv = m > 0.f ? __fdividef(32512.f, m) : 0.f;
-      row_mul *= m * (1.f / 32512.f);
+      row_mul *= 32.f;                                       // sums come in units of 2^5 of `q`'s
 #pragma unroll
       for (int i = 0; i < D / 4; i += 4) {
-        uint32_t w = 0;
+        uint32_t n[4];                                       // bytes b3 b2 b1 b0 of a number (b3 2^24 + ..), b2 b1 b0 x in lanes g >= 4
 #pragma unroll
         for (int x = 0; x < 4; ++x) {
-          const int n = min(max(__float2int_rn(q[i + x] * inv), -32512), 32512), hi = (n + 128) >> 8;
-          w |= (uint32_t(g < 4 ? hi : n - 256 * hi) & 0xffu) << (8 * x);
+          n[x] = (uint32_t(__float2int_rn(q[i + x] * 524288.f)) + 0x808080u) ^ 0x808080u;
+          if (g >= 4) n[x] <<= 8;
         }
-        qf[i / 8][i / 4 % 2] = w;
+        qf[i / 8][i / 4 % 2] = __byte_perm(__byte_perm(n[0], n[1], 0x0073), __byte_perm(n[2], n[3], 0x0073), 0x5410);
+        qf[D / 32 + i / 8][i / 4 % 2] = __byte_perm(__byte_perm(n[0], n[1], 0x0051), __byte_perm(n[2], n[3], 0x0051), 0x5410);
       }
     }
   }
@@ -432,8 +433,12 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
       // Scores: tokens are the rows of the products, 16 at a time.
       constexpr int kMt = kTile / 16;
       std::conditional_t<kWhole, int, float> acc[kMt][4];
+      int low[kWhole ? kMt : 1][4];                          // of the lower two bytes
 #pragma unroll
-      for (int t = 0; t < kMt; ++t) acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0;
+      for (int t = 0; t < kMt; ++t) {
+        acc[t][0] = acc[t][1] = acc[t][2] = acc[t][3] = 0;
+        if constexpr (kWhole) low[t][0] = low[t][1] = low[t][2] = low[t][3] = 0;
+      }
       constexpr int kPiece = L::kChunk * L::kBytes;
       const uint8_t* kr = st + L::place(g * kRow + tq * kPiece);
       const int other = L::place(g * kRow + (tq + 4) * kPiece) - L::place(g * kRow + tq * kPiece);
@@ -461,10 +466,12 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
         } else if constexpr (kWhole) {
 #pragma unroll
           for (int e = 0; e < L::kWords / 2; ++e) {
-            const uint32_t (&a)[2] = qf[c * (L::kWords / 2) + e];
+            const uint32_t (&a)[2] = qf[c * (L::kWords / 2) + e], (&z)[2] = qf[D / 32 + c * (L::kWords / 2) + e];
 #pragma unroll
-            for (int t = 0; t < kMt; ++t)
+            for (int t = 0; t < kMt; ++t) {
               mma_16832(acc[t], w[2 * t][2 * e], w[2 * t + 1][2 * e], w[2 * t][2 * e + 1], w[2 * t + 1][2 * e + 1], a[0], a[1]);
+              mma_16832(low[t], w[2 * t][2 * e], w[2 * t + 1][2 * e], w[2 * t][2 * e + 1], w[2 * t + 1][2 * e + 1], z[0], z[1]);
+            }
           }
         } else {
 #pragma unroll
@@ -496,9 +503,10 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
         }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const auto part_s = acc[n >> 1][2 * (n & 1) + e], rest = __shfl_xor_sync(0xffffffffu, part_s, 2);
-          float s;
-          if constexpr (kWhole) s = float(tq < 2 ? part_s * 256 + rest : rest * 256 + part_s);
+          float part_s = float(acc[n >> 1][2 * (n & 1) + e]), s;
+          if constexpr (kWhole) part_s = fmaf(float(low[n >> 1][2 * (n & 1) + e]), 1.f / 65536.f, part_s);       // bytes 3 and 1, or 2 and 0
+          const float rest = __shfl_xor_sync(0xffffffffu, part_s, 2);
+          if constexpr (kWhole) s = tq < 2 ? fmaf(rest, 1.f / 256.f, part_s) : fmaf(part_s, 1.f / 256.f, rest);
           else s = part_s + rest;
           s = score(s * ks, mul[e], slope[e], float(pos - t0 - tok)) + more;
           y[n][e] = tok < rows ? s : -INFINITY;

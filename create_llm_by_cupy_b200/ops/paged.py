@@ -278,7 +278,7 @@ def paged_attn_append(kqv, cache: PagedCache, table, lens, QH: int, KVH: int, co
     fewer than 0 tokens is none (a padded batch): nothing is written for it, and its result is 0, as it is where nothing is seen.
     ``softcap`` > 0 caps the scores (c tanh(s / c)); ``slopes`` fp32 [QH]: scores lose slope[head] * distance. Pages that are written
     belong to one sequence. Q and the weights go to the products as two parts of 8 bits and more: over int8 rows Q is off by at most
-    1 / 65024 of its head's largest element, else by 2^-17 of each. Returns [B, QH, D]."""
+    2^-30 of its head's largest element, else by 2^-17 of each. Returns [B, QH, D]."""
     if native.host is not None:
         out = native.host.paged_attn(kqv, *cache, table, lens, QH, KVH, cos, sin, 0.0 if scale is None else scale or -1.0, softcap, slopes)
         if out is not None:

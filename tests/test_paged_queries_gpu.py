@@ -1,11 +1,10 @@
 """Queries over 8-bit and bf16 pages whose numbers are far from 1, or far from one another: what the products see of them.
 
 Tolerances. An output: half a bf16 step, 2^-8 |o|, and what the weights are off by times the largest |v|. With S = sum |q||k| a score is
-off by at most 2^-16 S over bf16 rows (two bf16 parts), (2^-21 + 2^-34 / 2^-10) S over e4m3 rows for elements that are 2^-10 or more of
-their head's largest (two fp16 parts of 22 bits, the smallest of which is 2^-35 of the largest), 0.52 / 32512 of the largest element
-times sum |k| over int8 rows (half a whole number, and its quotient's own rounding); fp32 sums add D 2^-23 S, and int8 rows, whose sums are
-whole, eight roundings, 2^-20 S. Weights change by at most
-expm1 of twice that, and by 2^-15 for their own two parts, the exponential's and the sums' error."""
+off by at most 2^-17 S over bf16 rows (two bf16 parts), 2^-23 S and 2^-35 of the head's largest element times sum |k| over e4m3 rows (two
+fp16 parts, whose smallest step is at most 2^-34 of the largest), and 2^-30 of the largest element times sum |k| over int8 rows (half a
+whole number); fp32 sums add D 2^-23 S, int8 rows, whose sums are whole, eight roundings, 2^-20 S. Weights change by at most expm1 of
+twice that, and by 2^-15 for their own two parts, the exponential's and the sums' error."""
 import math
 
 import pytest
@@ -40,10 +39,10 @@ def attended(kind, k, v, kqv, scale, room):
     for h in range(QH):
         kh, vh = k[:, h // (QH // KVH)].abs(), v[:, h // (QH // KVH)].abs()
         size = float((kh @ q[h].abs()).max()) * scale
-        if kind == "int8":
-            off = 2.0 ** -20 * size + 0.52 / 32512 * float(q[h].abs().max()) * float(kh.sum(-1).max()) * scale
-        else:
-            off = ((2.0 ** -16 if kind == "bf16" else 2.0 ** -21 + 2.0 ** -24) + D * 2.0 ** -23) * size
+        all_k = float(q[h].abs().max()) * float(kh.sum(-1).max()) * scale
+        off = {"bf16": (2.0 ** -17 + D * 2.0 ** -23) * size,
+               "int8": 2.0 ** -20 * size + 2.0 ** -30 * all_k,
+               "e4m3": (2.0 ** -23 + D * 2.0 ** -23) * size + 2.0 ** -35 * all_k}[kind]
         tol[h] = 2.0 ** -8 * want[h].abs() + (math.expm1(2 * off) + 2.0 ** -15) * float(vh.max())
     return o, want, tol
 
@@ -59,6 +58,15 @@ def rows(seed, ratio=1.0):
     k[..., far] /= ratio
     kqv[:, :KVH, far] /= ratio
     return k * 1.5, v, kqv
+
+
+@pytest.mark.parametrize("ratio", [30.0, 100.0, 1000.0])
+@pytest.mark.parametrize("room", [1, 300])                   # clusters, and pieces that another kernel joins
+def test_a_few_large_dims(ratio, room):
+    """Heads as trained models have them, over int8 keys: the small dims count as much as the large ones."""
+    k, v, kqv = rows(3, ratio)
+    o, want, tol = attended("int8", k, v, kqv.flatten(1), 1 / math.sqrt(D), room)
+    assert bool(((o - want).abs() <= tol).all()), (float(((o - want).abs() - tol).max()), float((o - want).abs().max()))
 
 
 @pytest.mark.parametrize("kind", KINDS)
