@@ -277,8 +277,9 @@ def paged_attn_append(kqv, cache: PagedCache, table, lens, QH: int, KVH: int, co
     that would stand behind the table's pages or the rotary tables, or whose page is not there, is not kept and not seen. A sequence of
     fewer than 0 tokens is none (a padded batch): nothing is written for it, and its result is 0, as it is where nothing is seen.
     ``softcap`` > 0 caps the scores (c tanh(s / c)); ``slopes`` fp32 [QH]: scores lose slope[head] * distance. Pages that are written
-    belong to one sequence. Q and the weights go to the products as two parts of 8 bits and more: over int8 rows Q is off by at most
-    2^-30 of its head's largest element, else by 2^-17 of each. Returns [B, QH, D]."""
+    belong to one sequence. Elements of Q go to the products off by at most 2^-17 of themselves over bf16 rows, 2^-30 of their head's
+    largest over int8 rows, 2^-23 of themselves or 2^-35 of the largest, whichever is more, over e4m3 rows; weights off by 2^-17 of
+    themselves over bf16 rows, else 2^-23 of themselves or 2^-39 of the largest. Returns [B, QH, D]."""
     if native.host is not None:
         out = native.host.paged_attn(kqv, *cache, table, lens, QH, KVH, cos, sin, 0.0 if scale is None else scale or -1.0, softcap, slopes)
         if out is not None:
