@@ -25,7 +25,9 @@
 #include <atomic>
 #include <cmath>
 #include <cstring>
+#include <functional>
 
+#include "bounded_cache.h"
 #include "common.cuh"
 
 namespace b200 {
@@ -684,6 +686,34 @@ __global__ void __launch_bounds__(128) verify_walk_kernel(const WalkParams p) {
   if (lane == 0) p.count[b] = count;
 }
 
+// How many clusters of `cs` CTAs with `smem` bytes each run at the same time: two CTAs an SM go by the registers, fewer by the shared memory,
+// and a cluster lies within one GPC. Asked for once for each device and configuration.
+template <typename Kernel>
+static long long clusters_at_once(Kernel kern, int dev, bool bf16_logits, int cs, int smem) {
+  struct Hash {
+    size_t operator()(u64 key) const { return std::hash<u64>()(key); }
+  };
+  static BoundedCache<u64, int, Hash> kept(256);
+  int n = 0;
+  const u64 key = u64(uint32_t(dev)) << 32 | u64(bf16_logits) << 31 | u64(cs) << 24 | u64(smem);       // smem < 2^24, cs <= 8
+  const bool known = kept.get(key, &n, [&](int* out) {
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeClusterDimension;
+    at[0].val.clusterDim.x = cs;
+    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(cs);
+    cfg.blockDim = dim3(VD_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(out, kern, &cfg) == cudaSuccess && *out > 0) return true;
+    cudaGetLastError();
+    return false;
+  });
+  return known ? n : std::max(1, num_sms() / cs);
+}
+
 }  // namespace b200
 
 using namespace b200;
@@ -743,8 +773,7 @@ B200_API int b200_verify_drafts(const void* logits, const void* q, const void* t
     if (dev >= 0 && dev < 64) known[dev].store(true, std::memory_order_release);
   }
   // CTAs that stay: a cluster takes node after node.
-  const int per = std::min(4, std::max(1, 232448 / (smem + 1024)));
-  const long long most = std::max(1, num_sms() * per / cs);
+  const long long most = clusters_at_once(kern, dev, is_bf16 != 0, cs, smem);
   p.lazy = p.rows > most && n > 1;
   if (p.lazy) B200_CHECK(launch_pdl(verify_begin_kernel, dim3(unsigned((p.rows + 255) / 256)), dim3(256), 0, st, 0, p.choice, p.rows));
   B200_CHECK(launch_pdl(kern, dim3(cs, unsigned(std::min(p.rows, most))), dim3(VD_THREADS), smem, st, cs, p));
