@@ -2,7 +2,7 @@
 //
 // A pool [pages, KV heads, page, D] per K and V; a sequence's tokens lie in the pages that its row of the table names, token t in row
 // t % page of page table[t / page]. Rows are bf16, or 8 bits with one fp32 scale per token and head ([pages, KV heads, page]):
-//   scale = max(largest |x| (1 / L), 2^-80), L = 127 (int8) or 448 (e4m3); held = x / scale, rounded to nearest even.
+//   scale = max(largest |x| / L, 2^-80), L = 127 (int8) or 448 (e4m3); held = x / scale, rounded to nearest even.
 // One scale per row is what a decoded token can be written with, without a look at its neighbours. The floor of the scale keeps
 // reciprocals and logarithms of it finite; a row of zeros gets it.
 #pragma once
