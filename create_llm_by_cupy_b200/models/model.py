@@ -27,7 +27,7 @@ from ..ops.masked_attn import SpanMask, span_mask, tree_mask
 from ..ops.paged import paged_cache
 from .layers import (ChunkedCrossEntropy_Share, GroupedQueryAttention, RMSNorm, SwiGLU, TimeDropout,
                      TimeEmbedding_shard, init_weight)
-from .sampling import apply_repetition_penalty, top_p_sampling
+from .sampling import apply_repetition_penalty, draw_numbers, top_p_sampling
 
 _DTYPES = {"bf16": torch.bfloat16, "bfloat16": torch.bfloat16, "fp32": torch.float32, "float32": torch.float32}
 
@@ -545,12 +545,14 @@ class Cupa_ver4:
                        prefix: int = 0, cache: str = "bf16", page: int = 64):
         """``generate`` for several prompts of any lengths at a time, over paged caches: one prefill pass over all of them, then one
         pass per position. ``cache``: how K and V are held, "bf16", "int8" or "e4m3" (half the memory, and of what a pass reads); ``page``:
-        tokens of a page. Every sequence has pages for its own prompt and new tokens alone. The other arguments as in ``generate``.
+        tokens of a page. Every sequence has pages for its own prompt and new tokens alone. The other arguments as in ``generate``
+        (temperatures above 1e6 count as 1e6).
         Returns a list of token lists; a sequence is over at ``end_id``, at ``max_new_tokens``, or when its context is full."""
         pad = self.padding_id if padding_id is None else padding_id
         rows = [([int(start_id)] if start_id is not None else []) + [int(t) for t in prompt] for prompt in prompts]
         if any(not r for r in rows):
             raise ValueError("generate_batch needs at least one token of context for each sequence")
+        temp, top = (0.0, 1.0) if greedy else draw_numbers(temp, top)
         if not rows:
             return []
         Tmax, B, dev = self.time_size, len(rows), self.device
@@ -598,7 +600,7 @@ class Cupa_ver4:
             if seen is not None:
                 logits = torch.where(seen, torch.where(logits < 0, logits * penalty, logits / penalty), logits)
             u = torch.rand((B, 1), generator=gen, device=dev)
-            nxt = verify_drafts(logits[:, None], none, none - 1, u, temp=0.0 if greedy else max(float(temp), 1e-6), top=float(top))[0][:, 0]
+            nxt = verify_drafts(logits[:, None], none, none - 1, u, temp=temp, top=top)[0][:, 0]
             for b, t in enumerate(nxt.tolist()):
                 if not live[b]:
                     continue

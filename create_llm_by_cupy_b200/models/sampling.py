@@ -25,6 +25,16 @@ def softmax_with_temperature(logits: torch.Tensor, temp: float = 1.0) -> torch.T
     return torch.softmax(logits.float() / max(float(temp), 1e-6), dim=-1)
 
 
+def draw_numbers(temp: float, top: float) -> tuple[float, float]:
+    """A temperature and a nucleus as ``verify_drafts`` takes them, for any that ``top_p_sampling`` takes: temperatures below 1e-6 are 1e-6,
+    those above 1e6, where tokens are as good as alike, 1e6; a nucleus of 0 or less is the likeliest token (a mass of 1e-9, which the
+    first token of any vocabulary reaches)."""
+    temp, top = float(temp), float(top)
+    if temp != temp or top != top:
+        raise ValueError("temp and top are numbers")
+    return min(max(temp, 1e-6), 1e6), max(top, 1e-9)
+
+
 def top_p_sampling(logits: torch.Tensor, temp: float = 0.7, top_p: float = 0.9, generator=None) -> int:
     """Temperature softmax, keep the smallest set of tokens whose mass reaches ``top_p``, draw one
     of them with probability proportional to its mass."""

@@ -1,0 +1,37 @@
+"""What generation of batches and from drafts takes beside ``generate``: temperatures, nuclei and proposals of any kind (CPU forms)."""
+import pytest
+
+from .test_paged_model_cpu import PROMPTS, model
+
+
+@pytest.mark.parametrize("top", [0.0, -1.0, 0])
+def test_a_nucleus_of_nothing_is_the_likeliest_token(top):
+    m = model()
+    want = [m.generate(p, top=top, penalty=1.3, max_new_tokens=7) for p in PROMPTS]
+    assert m.generate_batch(PROMPTS, top=top, penalty=1.3, max_new_tokens=7) == want
+    greedy = [m.generate(p, greedy=True, max_new_tokens=7) for p in PROMPTS]
+    assert m.generate_batch(PROMPTS, greedy=True, top=top, max_new_tokens=7) == greedy
+
+
+@pytest.mark.parametrize("temp", [0.0, -1.0, 1e-9])
+def test_temperatures_of_nothing(temp):
+    m = model()
+    want = [m.generate(p, temp=temp, penalty=1.3, max_new_tokens=7) for p in PROMPTS]
+    assert m.generate_batch(PROMPTS, temp=temp, penalty=1.3, max_new_tokens=7) == want
+
+
+def test_very_high_temperatures():
+    """All tokens but the padding are alike: 322 draws of 39 tokens miss one with a probability of at most 39 (38 / 39)^322 = 0.009 (the
+    seed is fixed)."""
+    m = model()
+    for temp in (1e6, 1e7, 1e30, float("inf")):
+        outs = m.generate_batch([[1, 2]] * 7, temp=temp, top=1.0, penalty=1.0, seed=5)
+        assert all(len(x) == 46 and 39 not in x for x in outs) and len({t for x in outs for t in x}) == 39
+
+
+def test_numbers_are_checked_first(monkeypatch):
+    m = model()
+    monkeypatch.setattr(type(m), "_rows_mask", lambda *a, **k: pytest.fail("a pass was begun"))
+    for kw in (dict(temp=float("nan")), dict(top=float("nan"))):
+        with pytest.raises(ValueError):
+            m.generate_batch(PROMPTS, **kw)
