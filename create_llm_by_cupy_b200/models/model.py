@@ -627,15 +627,17 @@ class Cupa_ver4:
                          prefix: int = 0, temp: float | None = None, top: float = 0.9, seed: int | None = None):
         """Decoding that checks a tree of drafted tokens per pass. Greedy (``temp`` None): the same choices as ``generate(...,
         greedy=True)``, in as many passes as the drafts are wrong. With a ``temp``: tokens are drawn at that temperature from the nucleus
-        ``top`` (no repetition penalty), whatever the drafts are. ``draft(tokens)`` gets all tokens so far and returns proposals for those
-        that follow as (token, parent) pairs, at most 63: ``parent`` is the index of an earlier proposal of the same list, or -1 for the
-        last token. When tokens are drawn it may return (proposals, probs) instead: row i + 1 of ``probs`` [proposals + 1, vocabulary] is
+        ``top`` (no repetition penalty), whatever the drafts are; 0 takes the largest logit. ``draft(tokens)`` gets all tokens so far and
+        returns proposals for those that follow as (token, parent) pairs, at most 63: ``parent`` is the index of an earlier proposal of the
+        same list, or -1 for the last token. When tokens are drawn it may return (proposals, probs) instead: row i + 1 of ``probs`` [proposals + 1, vocabulary] is
         the distribution that the children of proposal i were drawn from, row 0 that of the last token's. A drafted token whose
         predecessors were all chosen, and which the model chooses, is kept with its cached K and V. ``prefix`` as in ``generate``."""
         pad = self.padding_id if padding_id is None else padding_id
         toks = ([int(start_id)] if start_id is not None else []) + [int(p) for p in prompt]
         if not toks:
             raise ValueError("generate_drafted needs at least one token of context")
+        if temp is not None:
+            temp, top = (0.0, 1.0) if temp == 0 else draw_numbers(temp, top)
         Tmax = self.time_size
         toks = toks[:Tmax - 1]
         budget = Tmax - len(toks) if max_new_tokens is None else min(max_new_tokens, Tmax - len(toks))
@@ -671,7 +673,7 @@ class Cupa_ver4:
             if probs is not None:
                 probs = torch.as_tensor(probs, dtype=torch.float32, device=dev).view(1, n, self.vocab_size).contiguous()
             tok, par = (torch.tensor([x], dtype=torch.int32, device=dev) for x in (ids, parents))
-            tokens, path, count = verify_drafts(logits[None], tok, par, u[0], temp=float(temp), top=float(top), draft_probs=probs,
+            tokens, path, count = verify_drafts(logits[None], tok, par, u[0], temp=temp, top=top, draft_probs=probs,
                                                 accept=None if probs is None else u[1])
             kept = int(count[0])
             return tokens[0, :kept + 1].tolist(), path[0, :kept].tolist()

@@ -35,3 +35,19 @@ def test_numbers_are_checked_first(monkeypatch):
     for kw in (dict(temp=float("nan")), dict(top=float("nan"))):
         with pytest.raises(ValueError):
             m.generate_batch(PROMPTS, **kw)
+
+
+@pytest.mark.parametrize("temp,top", [(1e-9, 0.9), (-1.0, 0.9), (1e-7, 1.0), (0.0, 0.5), (1.0, 0.0), (0.7, -2.0)])
+def test_drafts_with_nothing_to_draw_are_greedy(temp, top):
+    m = model()
+    want = m.generate([1, 2], greedy=True)
+    assert m.generate_drafted([1, 2], lambda t: [(want[len(t) - 2], -1), (5, 0)], temp=temp, top=top) == want
+
+
+def test_drafts_at_very_high_temperatures_and_numbers_that_are_none(monkeypatch):
+    m = model()
+    assert len(m.generate_drafted([1, 2], lambda t: [(5, -1)], temp=1e9, seed=0)) == 46
+    monkeypatch.setattr(type(m), "_rows_mask", lambda *a, **k: pytest.fail("a pass was begun"))
+    for kw in (dict(temp=float("nan")), dict(temp=1.0, top=float("nan"))):
+        with pytest.raises(ValueError):
+            m.generate_drafted([1, 2], lambda t: [], **kw)
