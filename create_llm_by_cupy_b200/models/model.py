@@ -629,9 +629,10 @@ class Cupa_ver4:
         greedy=True)``, in as many passes as the drafts are wrong. With a ``temp``: tokens are drawn at that temperature from the nucleus
         ``top`` (no repetition penalty), whatever the drafts are; 0 takes the largest logit. ``draft(tokens)`` gets all tokens so far and
         returns proposals for those that follow as (token, parent) pairs, at most 63: ``parent`` is the index of an earlier proposal of the
-        same list, or -1 for the last token. When tokens are drawn it may return (proposals, probs) instead: row i + 1 of ``probs`` [proposals + 1, vocabulary] is
-        the distribution that the children of proposal i were drawn from, row 0 that of the last token's. A drafted token whose
-        predecessors were all chosen, and which the model chooses, is kept with its cached K and V. ``prefix`` as in ``generate``."""
+        same list, or -1 for the last token. When tokens are drawn it may return (proposals, probs) instead: row i + 1 of ``probs``
+        [proposals + 1, vocabulary], a tensor or an array, is the distribution that the children of proposal i were drawn from, row 0 that
+        of the last token's. A drafted token whose predecessors were all chosen, and which the model chooses, is kept with its cached K and
+        V. ``prefix`` as in ``generate``."""
         pad = self.padding_id if padding_id is None else padding_id
         toks = ([int(start_id)] if start_id is not None else []) + [int(p) for p in prompt]
         if not toks:
@@ -690,7 +691,8 @@ class Cupa_ver4:
         while 0 < len(out) < budget and (end_id is None or out[-1] != end_id) and cached < Tmax - 1:
             room = min(64, Tmax - cached)
             proposals, probs = draft(toks + out), None
-            if isinstance(proposals, tuple) and len(proposals) == 2 and isinstance(proposals[1], (torch.Tensor, np.ndarray)):
+            if (isinstance(proposals, tuple) and len(proposals) == 2 and isinstance(proposals[1], (torch.Tensor, np.ndarray))
+                    and tuple(proposals[1].shape) != (2,)):                      # (a pair that is an array is a proposal)
                 proposals, probs = proposals
                 if temp is None:
                     raise ValueError("generate_drafted: probabilities of drafts are for tokens that are drawn (temp)")

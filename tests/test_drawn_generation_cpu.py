@@ -1,5 +1,7 @@
 """What generation of batches and from drafts takes beside ``generate``: temperatures, nuclei and proposals of any kind (CPU forms)."""
+import numpy as np
 import pytest
+import torch
 
 from .test_paged_model_cpu import PROMPTS, model
 
@@ -51,3 +53,26 @@ def test_drafts_at_very_high_temperatures_and_numbers_that_are_none(monkeypatch)
     for kw in (dict(temp=float("nan")), dict(temp=1.0, top=float("nan"))):
         with pytest.raises(ValueError):
             m.generate_drafted([1, 2], lambda t: [], **kw)
+
+
+@pytest.mark.parametrize("pack", [np.array, torch.tensor, tuple, list])
+@pytest.mark.parametrize("outer", [tuple, list])
+@pytest.mark.parametrize("temp", [None, 1e-6])
+def test_two_proposals_in_any_container(pack, outer, temp):
+    """Two pairs that are arrays, in a tuple, are two proposals, not proposals and their probabilities."""
+    m = model()
+    want, calls = m.generate([1, 2], greedy=True), []
+
+    def draft(tokens):
+        calls.append(len(tokens))
+        ahead = (want + [0, 0])[len(tokens) - 2:][:2]
+        return outer([pack([ahead[0], -1]), pack([ahead[1], 0])])
+
+    assert m.generate_drafted([1, 2], draft, temp=temp, top=1.0) == want and len(calls) <= 16
+
+
+def test_probabilities_that_are_no_rows_are_refused():
+    m = model()
+    for q in (torch.full((40,), 1 / 40), torch.full((1, 2, 40), 1 / 40), torch.tensor(1.0)):
+        with pytest.raises(ValueError):
+            m.generate_drafted([1, 2], lambda t: ([(3, -1)], q), temp=1.0)
