@@ -22,9 +22,9 @@ import numpy as np
 import torch
 
 from ..ops import functional as F
-from ..ops.drafts import verify_drafts
+from ..ops.drafts import MOST_TOKENS, verify_drafts
 from ..ops.masked_attn import SpanMask, span_mask, tree_mask
-from ..ops.paged import paged_cache
+from ..ops.paged import HEAD_DIMS, paged_cache
 from .layers import (ChunkedCrossEntropy_Share, GroupedQueryAttention, RMSNorm, SwiGLU, TimeDropout,
                      TimeEmbedding_shard, init_weight)
 from .sampling import apply_repetition_penalty, draw_numbers, top_p_sampling
@@ -539,6 +539,10 @@ class Cupa_ver4:
             h_last = self.norm_.forward(h, False)
         return out
 
+    def _check_drawable(self, name: str):
+        if self.vocab_size > MOST_TOKENS:
+            raise ValueError(f"{name}: vocabularies of up to {MOST_TOKENS} tokens")
+
     @torch.no_grad()
     def generate_batch(self, prompts, start_id=None, end_id=None, padding_id=None, temp: float = 0.7, top: float = 0.9,
                        penalty: float = 1.2, max_new_tokens: int | None = None, greedy: bool = False, seed: int | None = None,
@@ -546,13 +550,16 @@ class Cupa_ver4:
         """``generate`` for several prompts of any lengths at a time, over paged caches: one prefill pass over all of them, then one
         pass per position. ``cache``: how K and V are held, "bf16", "int8" or "e4m3" (half the memory, and of what a pass reads); ``page``:
         tokens of a page. Every sequence has pages for its own prompt and new tokens alone. The other arguments as in ``generate``
-        (temperatures above 1e6 count as 1e6).
+        (temperatures above 1e6 count as 1e6). On CUDA the head dimension is 64 or 128; up to 385024 tokens in a vocabulary.
         Returns a list of token lists; a sequence is over at ``end_id``, at ``max_new_tokens``, or when its context is full."""
         pad = self.padding_id if padding_id is None else padding_id
         rows = [([int(start_id)] if start_id is not None else []) + [int(t) for t in prompt] for prompt in prompts]
         if any(not r for r in rows):
             raise ValueError("generate_batch needs at least one token of context for each sequence")
         temp, top = (0.0, 1.0) if greedy else draw_numbers(temp, top)
+        if self.device.type == "cuda" and self.head_dim not in HEAD_DIMS:
+            raise ValueError(f"generate_batch: a head dimension of {' or '.join(map(str, HEAD_DIMS))} on CUDA")
+        self._check_drawable("generate_batch")
         if not rows:
             return []
         Tmax, B, dev = self.time_size, len(rows), self.device
@@ -639,6 +646,7 @@ class Cupa_ver4:
             raise ValueError("generate_drafted needs at least one token of context")
         if temp is not None:
             temp, top = (0.0, 1.0) if temp == 0 else draw_numbers(temp, top)
+            self._check_drawable("generate_drafted")
         Tmax = self.time_size
         toks = toks[:Tmax - 1]
         budget = Tmax - len(toks) if max_new_tokens is None else min(max_new_tokens, Tmax - len(toks))

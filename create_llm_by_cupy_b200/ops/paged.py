@@ -33,6 +33,7 @@ KINDS = {"bf16": torch.bfloat16, "int8": torch.int8, "e4m3": torch.float8_e4m3fn
 HELD = {torch.bfloat16: 0, torch.int8: 1, torch.float8_e4m3fn: 2}
 LARGEST = {torch.int8: 127.0, torch.float8_e4m3fn: 448.0}
 LEAST_SCALE = 2.0 ** -80
+HEAD_DIMS = (64, 128)                                        # that there are CUDA kernels for
 PAGES = (32, 64, 128, 256, 512, 1024)
 
 
@@ -95,7 +96,7 @@ def _check_tables(name: str, cos, sin, D: int, like) -> None:
 
 
 def _cuda_only(name: str, cache: PagedCache) -> None:
-    if cache.k.shape[3] not in (64, 128):
+    if cache.k.shape[3] not in HEAD_DIMS:
         raise ValueError(f"{name}: CUDA kernels exist for a head dimension of 64 or 128")
     if any(t is not None and t.data_ptr() % 16 for t in cache):
         raise ValueError(f"{name}: rows and scales of the cache start on 16-byte boundaries")

@@ -3,6 +3,8 @@ import numpy as np
 import pytest
 import torch
 
+from create_llm_by_cupy_b200.models import model as M
+
 from .test_paged_model_cpu import PROMPTS, model
 
 
@@ -76,3 +78,20 @@ def test_probabilities_that_are_no_rows_are_refused():
     for q in (torch.full((40,), 1 / 40), torch.full((1, 2, 40), 1 / 40), torch.tensor(1.0)):
         with pytest.raises(ValueError):
             m.generate_drafted([1, 2], lambda t: ([(3, -1)], q), temp=1.0)
+
+
+def test_models_that_the_kernels_do_not_take_are_refused_first(monkeypatch):
+    """Before any pool is made: head dimensions other than 64 and 128 on CUDA, vocabularies that the verification has no room for."""
+    monkeypatch.setattr(M, "paged_cache", lambda *a, **k: pytest.fail("a pool was made"))
+    m = model()
+    m.device = torch.device("cuda")                          # head dimension 8
+    with pytest.raises(ValueError, match="head dimension"):
+        m.generate_batch(PROMPTS)
+    m = model()
+    m.vocab_size = 8 * 376 * 128 + 1
+    for greedy in (False, True):
+        with pytest.raises(ValueError, match="vocabularies"):
+            m.generate_batch(PROMPTS, greedy=greedy)
+    monkeypatch.setattr(type(m), "_rows_mask", lambda *a, **k: pytest.fail("a pass was begun"))
+    with pytest.raises(ValueError, match="vocabularies"):
+        m.generate_drafted([1, 2], lambda t: [], temp=1.0)
