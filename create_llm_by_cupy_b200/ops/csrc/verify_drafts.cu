@@ -25,9 +25,7 @@
 #include <atomic>
 #include <cmath>
 #include <cstring>
-#include <functional>
 
-#include "bounded_cache.h"
 #include "common.cuh"
 
 namespace b200 {
@@ -686,32 +684,31 @@ __global__ void __launch_bounds__(128) verify_walk_kernel(const WalkParams p) {
   if (lane == 0) p.count[b] = count;
 }
 
-// How many clusters of `cs` CTAs with `smem` bytes each run at the same time: two CTAs an SM go by the registers, fewer by the shared memory,
-// and a cluster lies within one GPC. Asked for once for each device and configuration.
+// How many clusters of `cs` CTAs with `smem` bytes each run at the same time: registers allow two CTAs an SM, shared memory perhaps one, and
+// a cluster lies within one GPC. The last answer is kept for each device, type of logits and size of clusters.
 template <typename Kernel>
 static long long clusters_at_once(Kernel kern, int dev, bool bf16_logits, int cs, int smem) {
-  struct Hash {
-    size_t operator()(u64 key) const { return std::hash<u64>()(key); }
-  };
-  static BoundedCache<u64, int, Hash> kept(256);
+  static std::atomic<u64> kept[64][2][4];                    // shared memory and count
+  std::atomic<u64>* at = dev >= 0 && dev < 64 ? &kept[dev][bf16_logits][cs == 8 ? 3 : cs >> 1] : nullptr;
+  const u64 known = at != nullptr ? at->load(std::memory_order_relaxed) : 0;
+  if (known != 0 && int(known >> 32) == smem) return (long long)(known & 0xffffffffu);
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = cs;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(cs);
+  cfg.blockDim = dim3(VD_THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
   int n = 0;
-  const u64 key = u64(uint32_t(dev)) << 32 | u64(bf16_logits) << 31 | u64(cs) << 24 | u64(smem);       // smem < 2^24, cs <= 8
-  const bool known = kept.get(key, &n, [&](int* out) {
-    cudaLaunchAttribute at[1];
-    at[0].id = cudaLaunchAttributeClusterDimension;
-    at[0].val.clusterDim.x = cs;
-    at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(cs);
-    cfg.blockDim = dim3(VD_THREADS);
-    cfg.dynamicSmemBytes = smem;
-    cfg.attrs = at;
-    cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(out, kern, &cfg) == cudaSuccess && *out > 0) return true;
+  if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess || n < 1) {
     cudaGetLastError();
-    return false;
-  });
-  return known ? n : std::max(1, num_sms() / cs);
+    return std::max(1, num_sms() / cs);
+  }
+  if (at != nullptr) at->store(u64(smem) << 32 | u64(n), std::memory_order_relaxed);
+  return n;
 }
 
 }  // namespace b200

@@ -89,7 +89,8 @@ int main() {
               return 1;
             }
           }
-  const int before = queries;
+  assert(call(1, 700, 64, 600) == 0);
+  const int before = queries;                                // an answer is kept
   for (int i = 0; i < 5; ++i) assert(call(1, 700, 64, 600) == 0);
   assert(queries == before);
   return 0;
