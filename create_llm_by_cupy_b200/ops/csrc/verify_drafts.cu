@@ -11,13 +11,17 @@
 // Weights are fp64, and sums are sums of integers (2^62 / columns to the largest weight): which token a number falls on depends on the
 // whole row's sum, and integers add up to the same in any order.
 //
-// What bounds it: a row of 32000 logits is 128 KB, 3 us of an SM's share of HBM, and 32000 fp64 exponentials, which take 9; but the chain
-// of a node is about 45000 cycles (25 us) long whatever its slices are: largest logit, weights, the bin, the tokens of the bin, the sums,
-// the draw, each of them once over the row and once through the cluster. So slices are as large as two CTAs an SM hold, and where there are
-// more nodes than clusters, node 0 of all sequences comes first, then node 1: most of the later ones are out of question by then and passed
-// over. Us, 6 nodes of one sequence (probabilities of the drafts, nucleus) / 8 x 24 (the same, no nucleus) / 16 x 63 (looked up,
-// nucleus), 32000 tokens: bits of the nucleus' end one by one 267 / 122 / 1709, histogram 30 / 45 / 417, its search in two steps and
-// nodes passed over 22 / 55 to 63 / 80 to 86. (CTAs that read one another's whole histograms took 17000 cycles for it.)
+// What bounds it: a row of 32000 logits is 128 KB, 3 us of an SM's share of HBM, and 32000 fp64 exponentials, which take 9; the chain of a
+// node is longer: largest logit, weights, the bin, the tokens of the bin, the sums, the draw, each of them once over the CTA's slice and
+// once through the cluster. A call with one node (no walk to speak of) takes 18 us with 4000 tokens to a CTA (a row in eight), 32 with
+// 16000 (64 nodes in two CTAs each, one CTA an SM), 38 with two such CTAs an SM (148 nodes); without a nucleus 11 and, on full SMs, 23. So
+// a row is cut into more CTAs while half of the SMs would be idle, and slices are else as large as two CTAs an SM hold, which is more
+// nodes in a given time. Where there are more nodes than clusters, node 0 of all sequences comes first, then node 1: most of the later
+// ones are out of question by then and passed over. Us, 6 nodes of one sequence (probabilities of the drafts, nucleus) / 8 x 24 (the same,
+// no nucleus) / 16 x 63 (looked up, nucleus), 32000 tokens: bits of the nucleus' end one by one 267 / 122 / 1709, histogram 30 / 45 / 417,
+// its search in two steps, weights remade and nodes passed over 22 to 24 / 56 to 63 / 78 to 95 (from box to box; the second was faster
+// with its weights kept in shared memory, which leaves an SM one row). (CTAs that read one another's whole histograms took 17000 cycles
+// for it.)
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
@@ -684,8 +688,8 @@ __global__ void __launch_bounds__(128) verify_walk_kernel(const WalkParams p) {
   if (lane == 0) p.count[b] = count;
 }
 
-// How many clusters of `cs` CTAs with `smem` bytes each run at the same time: registers allow two CTAs an SM, shared memory perhaps one, and
-// a cluster lies within one GPC. The last answer is kept for each device, type of logits and size of clusters.
+// How many clusters of `cs` CTAs with `smem` bytes each run at the same time: registers allow two CTAs an SM, shared memory perhaps one,
+// and a cluster lies within one GPC. The last answer is kept for each device, type of logits and size of clusters.
 template <typename Kernel>
 static long long clusters_at_once(Kernel kern, int dev, bool bf16_logits, int cs, int smem) {
   static std::atomic<u64> kept[64][2][4];                    // shared memory and count
