@@ -256,11 +256,11 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
   for (int i = 0; i < kStages; ++i) ask(i);
 
   // The queries as fragments: lanes g < 4 the rounded values of head g, the others what that left of head g - 4. Over 8-bit rows each head
-  // is first brought to a largest magnitude of 2^10 by a power of two, whatever its numbers are. For e4m3 they go in as fp16, which has room
-  // for little. For int8 as whole numbers of 2^-19, below 2^30, in four signed bytes: K goes into the products as it is held, their sums are
-  // exact (at most 2^21, also as fp32), and a number is off by 2^-30 of its head's largest at most, not at all from a 64th of it on. The
-  // upper two bytes are the eight columns of one product, the lower two of another. (Two bytes, off by 2^-16 of the largest, were half of the
-  // products, but heads with a few dims 100 times the others lost what the others say.)
+  // is first brought to a largest magnitude of 2^10 by a power of two, whatever its numbers are. For e4m3 they go in as fp16, which has
+  // room for little. For int8 as whole numbers of 2^-19, below 2^30, in four signed bytes: K goes into the products as it is held, their
+  // sums are exact (at most 2^21, also as fp32), and a number is off by 2^-30 of its head's largest at most, not at all from a 64th of it
+  // on. The upper two bytes are the eight columns of one product, the lower two of another. (Two bytes, off by 2^-16 of the largest, were
+  // half of the products, but heads with a few dims 100 times the others lost what the others say.)
   constexpr bool kWhole = kHeld == kHeldInt8;
   uint32_t qf[D / 16][2];                                    // over int8 rows the upper bytes, then the lower ones
   float row_mul = 1.f, own_mul = 1.f;                        // what a product of head g & 3 is multiplied with, without the token's scale;
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
           float part_s = float(acc[n >> 1][2 * (n & 1) + e]), s;
-          if constexpr (kWhole) part_s = fmaf(float(low[n >> 1][2 * (n & 1) + e]), 1.f / 65536.f, part_s);       // bytes 3 and 1, or 2 and 0
+          if constexpr (kWhole) part_s = fmaf(float(low[n >> 1][2 * (n & 1) + e]), 1.f / 65536.f, part_s);  // bytes 3 and 1, or 2 and 0
           const float rest = __shfl_xor_sync(0xffffffffu, part_s, 2);
           if constexpr (kWhole) s = tq < 2 ? fmaf(rest, 1.f / 256.f, part_s) : fmaf(part_s, 1.f / 256.f, rest);
           else s = part_s + rest;

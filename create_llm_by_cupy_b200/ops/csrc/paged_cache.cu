@@ -1,9 +1,10 @@
 // Rows of K and V into the pages of a cache, and tokens back out of it (paged_cache.cuh says how they are held).
 //
-// Both are one pass over the data with nothing to reuse, bound by HBM: 16 bytes to a load, all lanes of a row beside one another, two rows to
-// a thread so that enough is on its way. int8, 8 KV heads of 128, 4096 tokens written and read back, in two launches: 20 us; with 8 bytes of
-// one row to a thread 24.4, with four heads and four rows 22.5, with one head 24.3, with eight rows 23.9. 8 x 2000 to 4000 e4m3 tokens read:
-// 29.4 us, 5.1 TB/s (38.4, and 30.7 with four rows, 34.1 with eight).
+// Both are one pass over the data with nothing to reuse: 16 bytes to a load, all lanes of a row beside one another, two rows to a thread
+// so that enough is on its way. Reading is bound by HBM, writing by the trips that follow one another (sequence and position, page,
+// angles): it waits for its loads at 16 % of DRAM. int8, 8 KV heads of 128, 4096 tokens written and read back, in two launches: 20 us;
+// with 8 bytes of one row to a thread 24.4, with four heads and four rows 22.5, with one head 24.3, with eight rows 23.9. 8 x 2000 to 4000
+// e4m3 tokens read: 29.2 us, 5.1 TB/s (38.4, and 30.7 with four rows, 34.1 with eight).
 #include "paged_cache.cuh"
 
 namespace b200 {

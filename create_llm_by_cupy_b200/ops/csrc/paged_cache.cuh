@@ -41,8 +41,8 @@ __device__ __forceinline__ float quotient(float x, float s, float inv) {
   return __fmaf_rn(__fmaf_rn(-q, s, x), inv, q);
 }
 
-// largest / L as a division gives it, so that pools written by any of the framework's forms are the same bit for bit. (Times the rounded 1 / L
-// it is off by its last place in 5 % of int8 rows and 55 % of e4m3 rows.)
+// largest / L as a division gives it, so that pools written by any of the framework's forms are the same bit for bit. (Times the rounded 1
+// / L it is off by its last place in 5 % of int8 rows and 55 % of e4m3 rows.)
 template <int kHeld>
 __device__ __forceinline__ float held_scale(float largest) {
   constexpr float most = kHeld == kHeldInt8 ? 127.f : 448.f;
