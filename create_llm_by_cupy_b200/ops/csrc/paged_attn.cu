@@ -304,7 +304,8 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
         qf[i][e] = g < 4 ? hi : lo;
       }
   }
-  // Score in units of log2 of a product with a token that is `dist` back.
+  // Score in units of log2 of a product with a token that is `dist` back. `mul` has the token's scale in it: of large keys and small
+  // queries the product times either alone could be infinite.
   auto score = [&](float s, float mul, float slope, float dist) {
     s *= mul;
     if (kScore == kScoreCap) return cap_any(s, p.cap);
@@ -394,7 +395,7 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
       for (int i = 0; i < D / 4; ++i) s = fmaf(q[i], k[i], s);
       s += __shfl_xor_sync(0xffffffffu, s, 1);
       s += __shfl_xor_sync(0xffffffffu, s, 2);
-      s = score(s * ks, own_mul * unit, 0.f, 0.f);
+      s = score(s, ks * (own_mul * unit), 0.f, 0.f);
       m_new = kHeld == kHeldBf16 ? s : s + __log2f(vs);
       const float w = exp2_of(kUp);
       l_new = w * (kHeld == kHeldBf16 ? 1.f : __frcp_rn(vs));
@@ -508,7 +509,7 @@ __global__ void __launch_bounds__(PA_THREADS, 3) paged_attn_kernel(const PagedAt
           const float rest = __shfl_xor_sync(0xffffffffu, part_s, 2);
           if constexpr (kWhole) s = tq < 2 ? fmaf(rest, 1.f / 256.f, part_s) : fmaf(part_s, 1.f / 256.f, rest);
           else s = part_s + rest;
-          s = score(s * ks, mul[e], slope[e], float(pos - t0 - tok)) + more;
+          s = score(s, ks * mul[e], slope[e], float(pos - t0 - tok)) + more;
           y[n][e] = tok < rows ? s : -INFINITY;
           m[e] = fmaxf(m[e], y[n][e]);
         }

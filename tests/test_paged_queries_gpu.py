@@ -81,3 +81,14 @@ def test_queries_near_the_ends_of_the_range(kind, power):
     o, want, tol = attended(kind, k, v, kqv.flatten(1), 2.0 ** -left / math.sqrt(D), 1)
     assert float((want - want.mean()).abs().max()) > 0.05    # not the mean of V, which equal weights would give
     assert bool(((o - want).abs() <= tol).all()), (float(((o - want).abs() - tol).max()), float((o - want).abs().max()))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("room", [1, 300])
+def test_keys_near_the_end_of_the_range(kind, room):
+    """Keys of 2^120 and queries that bring the scores back: a score is finite, and so is all on the way to it."""
+    k, v, kqv = rows(4)
+    kqv[:, KVH:KVH + QH] *= 2.0 ** -110
+    k, kqv[:, :KVH] = k * 2.0 ** 120, kqv[:, :KVH] * 2.0 ** 120
+    o, want, tol = attended(kind, k, v, kqv.flatten(1), 2.0 ** -10 / math.sqrt(D), room)
+    assert bool(((o - want).abs() <= tol).all()), (float(((o - want).abs() - tol).max()), float((o - want).abs().max()))
