@@ -92,3 +92,18 @@ def test_keys_near_the_end_of_the_range(kind, room):
     k, kqv[:, :KVH] = k * 2.0 ** 120, kqv[:, :KVH] * 2.0 ** 120
     o, want, tol = attended(kind, k, v, kqv.flatten(1), 2.0 ** -10 / math.sqrt(D), room)
     assert bool(((o - want).abs() <= tol).all()), (float(((o - want).abs() - tol).max()), float((o - want).abs().max()))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("room", [1, 300])
+@pytest.mark.parametrize("order", ["turns", "last", "first"])
+@pytest.mark.parametrize("power", [45, 70, 110])
+def test_values_of_any_scale(kind, room, order, power):
+    """Rows of V up to 2^110 beside rows of nothing, which count in the sum of weights all the same: in turns, the large ones in the last
+    tiles alone, in the first alone."""
+    k, v, kqv = rows(5)
+    t = torch.arange(LEN)
+    large = {"turns": t % 2 == 0, "last": t >= 270, "first": t < 40}[order]
+    v = torch.where(large[:, None, None], v * 2.0 ** power, torch.where((t % 3 == 0)[:, None, None], v * 2.0 ** -70, torch.zeros(())))
+    o, want, tol = attended(kind, k, v, kqv.flatten(1), 1 / math.sqrt(D), room)
+    assert bool(((o - want).abs() <= tol).all()), (float(((o - want).abs() - tol).max()), float((o - want).abs().max()))
