@@ -2,7 +2,7 @@
 //
 // A pool [pages, KV heads, page, D] per K and V; a sequence's tokens lie in the pages that its row of the table names, token t in row
 // t % page of page table[t / page]. Rows are bf16, or 8 bits with one fp32 scale per token and head ([pages, KV heads, page]):
-//   scale = max(largest |x| / L, 2^-80), L = 127 (int8) or 448 (e4m3); held = x / scale, rounded to nearest even.
+//   scale = max(largest |x| (1 / L), 2^-80), L = 127 (int8) or 448 (e4m3), 1 / L rounded; held = x / scale, rounded to nearest even.
 // One scale per row is what a decoded token can be written with, without a look at its neighbours. The floor of the scale keeps
 // reciprocals and logarithms of it finite; a row of zeros gets it.
 #pragma once
@@ -34,19 +34,19 @@ __device__ __forceinline__ long long paged_row(const PagedPool& c, int b, int h,
   return (((long long)pg * c.KVH + h) << c.log_page) + (t & (c.page() - 1));
 }
 
+// One product with the rounded 1 / L, as every form of the framework takes it (and torch on a GPU, where it divides by a number): pools of
+// all of them are the same bit for bit. A division differs from it in the last place of 5 % of int8 and 55 % of e4m3 scales, and in which
+// of its two neighbours an e4m3 value halfway between them becomes, 1 in 1000; a row is represented equally well.
+template <int kHeld>
+__device__ __forceinline__ float held_scale(float largest) {
+  return fmaxf(__fmul_rn(largest, kHeld == kHeldInt8 ? 1.f / 127.f : 1.f / 448.f), kLeastScale);
+}
+
 // x / s correctly rounded, given inv = 1 / s correctly rounded: Markstein's theorem (IBM J. Res. Dev. 34, 1990). A product with the
 // reciprocal alone went the other way at one e4m3 value in 600 of rows that come from bf16, whose quotients often lie halfway.
 __device__ __forceinline__ float quotient(float x, float s, float inv) {
   const float q = __fmul_rn(x, inv);
   return __fmaf_rn(__fmaf_rn(-q, s, x), inv, q);
-}
-
-// largest / L as a division gives it, so that pools written by any of the framework's forms are the same bit for bit. (Times the rounded 1
-// / L it is off by its last place in 5 % of int8 rows and 55 % of e4m3 rows.)
-template <int kHeld>
-__device__ __forceinline__ float held_scale(float largest) {
-  constexpr float most = kHeld == kHeldInt8 ? 127.f : 448.f;
-  return fmaxf(quotient(largest, most, 1.f / most), kLeastScale);
 }
 
 // Four values as they are held, the first in the lowest byte, given the scale and its reciprocal.

@@ -13,8 +13,8 @@ tensors take a plain torch restatement (fp32, or fp64 for fp64 inputs).
 no page of the pool is one that is not there: what would be written to it is left out, what would be read from it is not seen. Sequences
 may share pages that are only read.
 
-In 8 bits a row x of one token and head is held as round(x / scale), scale = max(largest |x| / L, 2^-80), with L = 127 (int8) or 448
-(e4m3). Rows have to be finite.
+In 8 bits a row x of one token and head is held as round(x / scale), scale = max(largest |x| (1 / L), 2^-80), with L = 127 (int8) or 448
+(e4m3) and 1 / L rounded to fp32. Rows have to be finite.
 """
 from __future__ import annotations
 
@@ -120,7 +120,7 @@ def _hold(x, dtype):
     """fp rows as they are held: (rows, scales)."""
     if dtype not in LARGEST:
         return x.to(dtype), None
-    s = (x.abs().amax(-1) / LARGEST[dtype]).clamp_min(LEAST_SCALE)
+    s = (x.abs().amax(-1) * torch.tensor(1.0 / LARGEST[dtype], dtype=torch.float32).to(x)).clamp_min(LEAST_SCALE)
     y = x / s[..., None]
     return (torch.round(y).to(dtype) if dtype == torch.int8 else y.float().to(dtype)), s.float()
 
