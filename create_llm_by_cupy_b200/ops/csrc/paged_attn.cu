@@ -3,7 +3,7 @@
 //   o = sum_j p_j v_j / sum_j p_j,   p_j = 2^(s_j - m),   s_j = score(scale q . k_j) log2 e
 //
 // What bounds it: each cached row is read once, 2 D + 8 bytes a token and KV head in 8 bits, so HBM, if an SM gets through its tiles fast
-// enough (it has 24 bytes of HBM a cycle). 64 x 1500 to 4000 tokens, 32 / 8 heads of 128, int8, with the append: 81 us, 4.6 TB/s; bytes to
+// enough (it has 24 bytes of HBM a cycle). 64 x 1500 to 4000 tokens, 32 / 8 heads of 128, int8, with the append: 82 us, 4.6 TB/s; bytes to
 // fp16 on the ALU and the last CTAs, which run alone, are the rest. Hence:
 //   * products by mma.sync with the TOKENS (dims, for the values) as rows and the heads as columns. Columns 0 to 3 are the four query heads
 //     of the CTA, columns 4 to 7 what rounding left of them: scores and weights go in as two parts at no further product. With the heads as
@@ -19,7 +19,7 @@
 //     pairs of tokens: two byte permutations for four dims. Weights are turned over by movmatrix.
 //   * tiles go through a ring per warp, so warps never wait for one another until the end. Three CTAs an SM.
 //   * few sequences: clusters of up to eight CTAs share one or, where 8 leave SMs idle, pieces that a second kernel joins (one sequence of
-//     60001 tokens 68 us with clusters of 8, 54 of 16, 41 with 55 pieces; 32 since four threads a dim join them, and Q went in as bytes).
+//     60001 tokens 68 us with clusters of 8, 54 of 16, 41 with 55 pieces; 33 since four threads a dim join them, and Q went in as bytes).
 // Tried and not kept: bulk copies by a warp of their own (no faster: the time is that of the arithmetic), one list of all tiles cut evenly
 // over CTAs that stay (64 x 1500 to 4000 tokens 88 -> 93 us, 32 x 0 to 1980 21 -> 40: the start of a stretch takes as long as four tiles,
 // and its state does not fit in the registers of three CTAs an SM).

@@ -19,9 +19,9 @@
 // nodes in a given time. Where there are more nodes than clusters, node 0 of all sequences comes first, then node 1: most of the later
 // ones are out of question by then and passed over. Us, 6 nodes of one sequence (probabilities of the drafts, nucleus) / 8 x 24 (the same,
 // no nucleus) / 16 x 63 (looked up, nucleus), 32000 tokens: bits of the nucleus' end one by one 267 / 122 / 1709, histogram 30 / 45 / 417,
-// its search in two steps, weights remade and nodes passed over 22 to 24 / 56 to 63 / 78 to 95 (from box to box; the second was faster
-// with its weights kept in shared memory, which leaves an SM one row). (CTAs that read one another's whole histograms took 17000 cycles
-// for it.)
+// its search in two steps, weights remade and nodes passed over 20 to 25 / 54 to 63 / 72 to 104 (ten inputs, by how far their texts go;
+// the second was faster with its weights kept in shared memory, which leaves an SM one row). (CTAs that read one another's whole
+// histograms took 17000 cycles for it.)
 #include <cooperative_groups.h>
 #include <math_constants.h>
 
